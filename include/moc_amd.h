@@ -37,6 +37,10 @@ extern "C" {
 #define MOC_BF16 0
 #define MOC_F32 1
 
+/* element types of a paged cache's codes */
+#define MOC_E4M3 0 /* OCP float8 e4m3 */
+#define MOC_I8 1
+
 /* index types */
 #define MOC_I16 0
 #define MOC_I32 1
@@ -714,6 +718,70 @@ int64_t moc_sparse28_down_workspace_size(int64_t nb, int64_t inter, int64_t hidd
 int moc_sparse28_down_bf16(const void* ap, int64_t ld_ap, const uint32_t* meta, int64_t meta_rows,
                            int64_t nb, int64_t inter, const void* w, int64_t ldw, int w_kc, int64_t hidden,
                            void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------- batched decode, paged 8-bit cache
+ * A paged cache: codes [pages, kv_heads, page, head_dim] of keys and of values,
+ * one byte each (MOC_E4M3 or MOC_I8), and one f32 scale for each page and head
+ * (k_scale, v_scale [pages, kv_heads]); a value is code * scale.  page: a power
+ * of two from 16 to 256; head_dim: 64, 128 or 256.  table [seqs, width] (row
+ * pitch ld_table, int32): position p of sequence b lies in place p % page of page
+ * table[b][p / page].
+ *
+ * A batch: seqs sequences, the new tokens of sequence b are rows cu[b] to cu[b +
+ * 1] - 1 of q (cu int32 [seqs + 1], ascending; NULL: one token a sequence, tokens
+ * == seqs), at positions lens[b] - n to lens[b] - 1: lens (int32) counts the new
+ * ones.  Rows behind cu[seqs] are neither read nor written.
+ *
+ * Rows: element strides between tokens (ld) and heads (lh), multiples of 8, bases
+ * 16-byte aligned.  Whatever table, lens and cu hold, nothing outside the given
+ * extents is read or written. */
+
+/* RoPE on q and k (interleaved pairs, cos and sin [angles, head_dim / 2] in
+ * table_dtype) and the new k and v into the cache.  q_out = rotated q as bf16 (may
+ * be q).  A block (one page's places of one head) gets the least power of two s
+ * with |x| <= 448 s (e4m3) or 127 s (int8), at least 2^-100, for what it held and
+ * gets; a call that writes a page's first place begins it anew; where the scale
+ * grows, older codes are encoded again.  Codes are rounded to nearest even; values
+ * that are not finite do not count for s and become NaN (e4m3), the ends or 0 (int8).
+ * A token without a place (position negative, behind the table or the angles, page
+ * number out of range) is not stored; its q_out is 0 before position 0, NaN behind
+ * the table or the angles.  A page that a call writes to belongs to one sequence. */
+int moc_paged_append_bf16(const void* q, int64_t q_ld, int64_t q_lh, const void* k, int64_t k_ld, int64_t k_lh,
+                          const void* v, int64_t v_ld, int64_t v_lh, int64_t tokens, int64_t q_heads,
+                          int64_t kv_heads, int64_t head_dim, const void* cos, const void* sin, int table_dtype,
+                          int64_t angles, int code, void* k_codes, void* v_codes, float* k_scale, float* v_scale,
+                          int64_t pages, int64_t page, const int32_t* table, int64_t ld_table, int64_t width,
+                          const int32_t* lens, const int32_t* cu, int64_t seqs, void* q_out, int64_t o_ld,
+                          int64_t o_lh, void* stream);
+
+/* Workspace bytes of moc_paged_attention_bf16 (ragged: cu given). */
+int64_t moc_paged_attention_workspace_size(int64_t tokens, int64_t seqs, int ragged, int64_t q_heads,
+                                           int64_t kv_heads, int64_t head_dim, int64_t page, int64_t width);
+
+/* out = softmax(scale q K^T) V of each row of q over the positions up to its own;
+ * q head h reads kv head h / (q_heads / kv_heads).  Scores, softmax and sums in
+ * f32; probabilities go to the second product as bf16.  A row that sees no
+ * position is 0; one that sees a position without a page is NaN. */
+int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_lh, int64_t tokens, int64_t q_heads,
+                             int64_t kv_heads, int64_t head_dim, int code, const void* k_codes, const void* v_codes,
+                             const float* k_scale, const float* v_scale, int64_t pages, int64_t page,
+                             const int32_t* table, int64_t ld_table, int64_t width, const int32_t* lens,
+                             const int32_t* cu, int64_t seqs, float scale, void* out, int64_t o_ld, int64_t o_lh,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* out[r] (int64) = the token drawn from row r of logits (bf16 or f32, row pitch
+ * ld, at most 2^18 words) with the uniform number u[r] (f32 in [0, 1)): ids ordered
+ * by logit descending, then id ascending; the first top_k of them (<= 0: all); of
+ * those the ones with less than top_p of their weight exp(logit / temperature)
+ * before them (the best at least; >= 1: all); of those the ones with at least min_p
+ * of the best's weight; and of those the first, by id, whose weights up to and with
+ * it exceed u times all.  temperature <= 0: the best.  NaN counts as -infinity; -1
+ * for a row of nothing else.  temperature, top_k, top_p, min_p: arrays over the
+ * rows, or NULL and the number behind for all. */
+int moc_sample_tokens(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t ld, const float* u,
+                      const float* temperature, float temperature1, const int32_t* top_k, int top_k1,
+                      const float* top_p, float top_p1, const float* min_p, float min_p1, int64_t* out,
+                      void* stream);
 
 #ifdef __cplusplus
 }

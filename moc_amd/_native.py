@@ -27,6 +27,8 @@ MOC_ERR_INVALID = -1
 MOC_ERR_HIP = -2
 MOC_BF16 = 0
 MOC_F32 = 1
+MOC_E4M3 = 0
+MOC_I8 = 1
 MOC_I16 = 0
 MOC_I32 = 1
 MOC_I64 = 2
@@ -166,6 +168,15 @@ SIGNATURES: dict[str, tuple] = {
     "moc_sparse28_down_workspace_size": (_i64, [_i64, _i64, _i64]),
     "moc_sparse28_down_bf16": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _int, _i64, _vp,
                                       _i64, _vp, _i64, _vp]),
+    "moc_paged_append_bf16": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+                                     _vp, _vp, _int, _i64, _int, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
+                                     _vp, _vp, _i64, _vp, _i64, _i64, _vp]),
+    "moc_paged_attention_workspace_size": (_i64, [_i64, _i64, _int, _i64, _i64, _i64, _i64, _i64]),
+    "moc_paged_attention_bf16": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _i64,
+                                        _i64, _vp, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp, _i64, _i64,
+                                        _vp, _i64, _vp]),
+    "moc_sample_tokens": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _int, _vp,
+                                 ctypes.c_float, _vp, ctypes.c_float, _vp, _vp]),
 }
 
 _LIB = None

@@ -1,0 +1,427 @@
+// Causal attention of new tokens over a paged 8-bit cache (gfx950):
+//   o = sum_j p_j v_j,  p = softmax_j(scale q k_j) over the positions j that the
+//   token sees, k_j and v_j a code times the scale of its page and head.
+//
+// A row tile holds 16 rows, one column of the MFMA each: the heads of a group
+// (those that share a key head) of one token after the other.  Orientation:
+// S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_16x16x32_bf16, so a lane has one
+// row (l & 15), its softmax factors are per-lane values, and the four positions
+// that a 16-position tile of S^T leaves in a lane (4 (l >> 4) + r) are, two
+// tiles together, the eight k of the second product's operand: P never moves
+// between lanes.  V's operand needs the same positions for one dimension: a
+// lane reads D / 16 neighbouring dimensions of each of its eight positions and
+// transposes them in registers (v_perm).  Codes become bf16 exactly; the page's
+// scales go onto the scores and the probabilities in f32.
+//
+// The cache is read once for a tile, straight into registers; one workgroup
+// takes a chunk of the positions, a wave 64 at a time, and the waves join
+// through LDS.  Chunks of one row join in a second launch.  Bound: HBM bytes of
+// the codes.
+#include <algorithm>
+
+#include "abi.h"
+#include "paged.h"
+
+namespace moc {
+namespace {
+
+constexpr int kPaWaves = 4;
+constexpr int kPaThreads = 64 * kPaWaves;
+constexpr int kPaTile = 64;  // positions per wave and step
+
+struct PagedAttnArgs {
+  PagedSeqs s;
+  const uint16_t* q;
+  int64_t q_ld, q_lh;
+  uint16_t* o;
+  int64_t o_ld, o_lh;
+  const uint8_t *kc, *vc;
+  const float *ks, *vs;
+  int pages, log_page, heads, kv_heads, group;
+  float c2;      // scale log2(e)
+  int chunk, splits;
+  float* part_o;   // [tokens heads][splits][D]
+  float2* part_ml;  // [tokens heads][splits]: largest score, sum
+};
+
+// Two codes (bytes 2 H, 2 H + 1 of w) as bf16.
+template <bool INT8, bool H>
+__device__ __forceinline__ uint32_t two_bf16(uint32_t w) {
+  if constexpr (INT8) {
+    const float a = static_cast<float>(static_cast<int8_t>(w >> (H ? 16 : 0)));
+    const float b = static_cast<float>(static_cast<int8_t>(w >> (H ? 24 : 8)));
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  } else {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, H));
+  }
+}
+
+template <bool INT8>
+__device__ __forceinline__ bf16x8_t eight_bf16(uint32_t lo, uint32_t hi) {
+  return __builtin_bit_cast(bf16x8_t, make_uint4(two_bf16<INT8, false>(lo), two_bf16<INT8, true>(lo),
+                                                 two_bf16<INT8, false>(hi), two_bf16<INT8, true>(hi)));
+}
+
+template <int D, bool INT8>
+__global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a) {
+  constexpr int kLoads = D / 64;     // 16-byte loads of a K row per lane
+  constexpr int kVDims = D / 16;     // dimensions of V per lane
+  constexpr int kVWords = kVDims / 4;
+  __shared__ float part[kPaWaves][16][D + 4];
+  __shared__ float2 ml[kPaWaves][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int col = lane & 15, h = lane >> 4;
+  const int head = blockIdx.y, lp = a.log_page, page = 1 << lp;
+  // the row tile: rows [unit 16, unit 16 + 16) of a sequence's n group
+  SeqSpan sp;
+  const int group = a.group;
+  if (a.s.cu == nullptr) {
+    const int tiles = (group + 15) / 16;
+    sp.seq = sp.row0 = blockIdx.x / tiles;
+    sp.unit = blockIdx.x - sp.seq * tiles;
+    sp.n = 1;
+    sp.len = a.s.lens[sp.seq];
+  } else {
+    sp = find_unit(a.s, blockIdx.x, [group](int n, int64_t) { return (n * group + 15) / 16; });
+    if (sp.seq < 0) return;
+  }
+  const int r = sp.unit * 16 + col, token = r / group, sub = r - token * group;
+  const bool live = token < sp.n;
+  const int64_t room = static_cast<int64_t>(a.s.width) << lp;
+  // positions that this lane's row sees, and that any row of the tile does
+  const int64_t sees = live ? sp.len - sp.n + 1 + token : 0;
+  const int last = min(sp.unit * 16 + 15, sp.n * group - 1) / group;
+  const int64_t most = min(max(sp.len - sp.n + 1 + last, int64_t(0)), room);
+  bool lost = sees > room;  // positions without a page: NaN
+  const int64_t lim = sees;
+  const int64_t from = static_cast<int64_t>(blockIdx.z) * a.chunk, to = min(most, from + a.chunk);
+
+  bf16x8_t qf[kLoads][2];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint4 t = make_uint4(0, 0, 0, 0);
+      if (live)
+        t = *reinterpret_cast<const uint4*>(a.q + (sp.row0 + token) * a.q_ld + (head * group + sub) * a.q_lh + i * 64 +
+                                            h * 16 + j * 8);
+      qf[i][j] = __builtin_bit_cast(bf16x8_t, t);
+    }
+
+  float m = -INFINITY, l = 0.f;
+  f32x4_t acc[kVDims];
+#pragma unroll
+  for (int j = 0; j < kVDims; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const int32_t* table = a.s.table + sp.seq * a.s.ld_table;
+  const uint32_t k_off = col * D + h * 16, v_off = 4 * h * D + col * kVDims;
+
+  for (int64_t t0 = from + wave * kPaTile; t0 < to; t0 += kPaTile * kPaWaves) {
+    const int groups = static_cast<int>(min((to - t0 + 15) >> 4, int64_t(4)));
+    const uint8_t *kp[4], *vp[4];
+    float ksc[4], vsc[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {  // groups past the last repeat it, masked
+      const int64_t p = t0 + 16 * min(g, groups - 1);
+      int id = __builtin_amdgcn_readfirstlane(table[p >> lp]);
+      if (id < 0 || id >= a.pages) {
+        id = 0;
+        lost |= p < lim;
+      }
+      const int64_t block = static_cast<int64_t>(id) * a.kv_heads + head;
+      const int64_t byte = ((block << lp) + (p & (page - 1))) * D;
+      kp[g] = a.kc + byte;
+      vp[g] = a.vc + byte;
+      ksc[g] = a.ks[block] * a.c2;
+      vsc[g] = a.vs[block];
+    }
+    uint4 kr[4][kLoads];
+    uint32_t vr[4][4][kVWords];
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) kr[g][i] = *reinterpret_cast<const uint4*>(kp[g] + k_off + 64 * i);
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* p = vp[g] + v_off + i * D;
+        if constexpr (kVWords == 1) {
+          vr[g][i][0] = *reinterpret_cast<const uint32_t*>(p);
+        } else if constexpr (kVWords == 2) {
+          const uint2 t = *reinterpret_cast<const uint2*>(p);
+          vr[g][i][0] = t.x; vr[g][i][1] = t.y;
+        } else {
+          const uint4 t = *reinterpret_cast<const uint4*>(p);
+          vr[g][i][0] = t.x; vr[g][i][1] = t.y; vr[g][i][2] = t.z; vr[g][i][3] = t.w;
+        }
+      }
+    float s[4][4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<INT8>(kr[g][i].x, kr[g][i].y), qf[i][0], x, 0, 0, 0);
+        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<INT8>(kr[g][i].z, kr[g][i].w), qf[i][1], x, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[g][i] = x[i] * ksc[g];
+    }
+    const int64_t whole = min(sp.len - sp.n + 1 + sp.unit * 16 / group, to);  // every row sees up to here
+    const bool edge = t0 + kPaTile > whole;
+    if (edge) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t p = t0 + 16 * g + 4 * h + i;
+          if (p >= lim || p >= to) s[g][i] = -INFINITY;
+          if (p >= to) {  // places that hold no token may hold anything, NaN codes too
+#pragma unroll
+            for (int w = 0; w < kVWords; ++w) vr[g][i][w] = 0;
+          }
+        }
+    }
+    float mt = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[g][i]);
+    mt = fmaxf(mt, __shfl_xor(mt, 16));
+    mt = fmaxf(mt, __shfl_xor(mt, 32));
+    const float mn = fmaxf(m, mt);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    if (__any(mn > m)) {
+      const float f = __builtin_amdgcn_exp2f(m - base);
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < kVDims; ++j) acc[j] *= f;
+      m = mn;
+    }
+    uint32_t pb[4][2];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(s[g][i] - base);
+        l += p[i];
+        p[i] = p[i] == 0.f ? 0.f : p[i] * vsc[g];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        pb[g][i] = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector((cvt_f32x2_t){p[2 * i], p[2 * i + 1]}, cvt_bf16x2_t));
+    }
+#pragma unroll
+    for (int gg = 0; gg < 2; ++gg) {
+      const bf16x8_t pf = __builtin_bit_cast(
+          bf16x8_t, make_uint4(pb[2 * gg][0], pb[2 * gg][1], pb[2 * gg + 1][0], pb[2 * gg + 1][1]));
+#pragma unroll
+      for (int w = 0; w < kVWords; ++w) {
+        // [position][two dimensions] -> [dimension][two positions]
+        uint32_t x[2][4][2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[g][i][0] = two_bf16<INT8, false>(vr[2 * gg + g][i][w]);
+            x[g][i][1] = two_bf16<INT8, true>(vr[2 * gg + g][i][w]);
+          }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+          uint32_t v[4];
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              v[2 * g + i] = __builtin_amdgcn_perm(x[g][2 * i + 1][j >> 1], x[g][2 * i][j >> 1], sel);
+          const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, make_uint4(v[0], v[1], v[2], v[3]));
+          acc[4 * w + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, acc[4 * w + j], 0, 0, 0);
+        }
+      }
+    }
+  }
+  // join the waves: a lane holds dimensions h D / 4 .. of its row
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (lost) l = __uint_as_float(0x7FC00000u);
+  if (h == 0) ml[wave][col] = make_float2(m, l);
+#pragma unroll
+  for (int j = 0; j < kVDims; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][col][(4 * h + i) * kVDims + j] = acc[j][i];
+  __syncthreads();
+  constexpr int kPer = D * 16 / kPaThreads;  // values per thread: D / 16
+  const int row = tid / 16, d0 = (tid & 15) * kPer;
+  const int rr = sp.unit * 16 + row, tk = rr / group, sb = rr - tk * group;
+  if (tk >= sp.n) return;
+  float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+  for (int w = 0; w < kPaWaves; ++w) mm = fmaxf(mm, ml[w][row].x);
+  const float base = mm == -INFINITY ? 0.f : mm;
+  float out[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) out[i] = 0.f;
+#pragma unroll
+  for (int w = 0; w < kPaWaves; ++w) {
+    const float f = __builtin_amdgcn_exp2f(ml[w][row].x - base);
+    ll += ml[w][row].y * f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) out[i] += part[w][row][d0 + i] * f;
+  }
+  const int64_t token_row = sp.row0 + tk;
+  if (a.splits == 1) {
+    const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+    uint16_t* o = a.o + token_row * a.o_ld + (head * group + sb) * a.o_lh + d0;
+#pragma unroll
+    for (int i = 0; i < kPer; i += 2)
+      *reinterpret_cast<uint32_t*>(o + i) =
+          __builtin_bit_cast(uint32_t, __builtin_convertvector((cvt_f32x2_t){out[i] * inv, out[i + 1] * inv}, cvt_bf16x2_t));
+    return;
+  }
+  const int64_t slot = (token_row * a.heads + head * group + sb) * a.splits + blockIdx.z;
+  if ((tid & 15) == 0) a.part_ml[slot] = make_float2(mm, ll);
+  if (mm == -INFINITY) return;  // nothing in this chunk
+  float* po = a.part_o + slot * D + d0;
+#pragma unroll
+  for (int i = 0; i < kPer; i += 4)
+    *reinterpret_cast<float4*>(po + i) = make_float4(out[i], out[i + 1], out[i + 2], out[i + 3]);
+}
+
+// o from the chunks of a row: one wave a row, D / 64 values a lane.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int64_t rows) {
+  constexpr int kPer = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int64_t token = row / a.heads;
+  if (a.s.cu != nullptr && (token < a.s.cu[0] || token >= a.s.cu[a.s.seqs])) return;  // nobody's row
+  const float2* ml = a.part_ml + row * a.splits;
+  float m = -INFINITY;
+  for (int i = lane; i < a.splits; i += 64) m = fmaxf(m, ml[i].x);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, out[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) out[i] = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 t = ml[s];
+    const float f = __builtin_amdgcn_exp2f(t.x - base);
+    l += t.y * f;
+    if (t.x == -INFINITY) {
+      l += t.y;  // 0, or NaN where a chunk lies outside the cache
+      continue;
+    }
+    const float* p = a.part_o + (row * a.splits + s) * D + lane * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) out[i] += p[i] * f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  uint16_t* o = a.o + token * a.o_ld + (row - token * a.heads) * a.o_lh + lane * kPer;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) o[i] = bf16_rne(out[i] * inv);
+}
+
+}  // namespace
+}  // namespace moc
+
+using namespace moc;
+
+namespace {
+// Chunks of the positions: enough workgroups for the CUs, whole tiles a wave.
+struct Plan {
+  int64_t tiles, chunk, splits;
+};
+Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t kv_heads, int64_t room) {
+  Plan p;
+  p.tiles = ragged ? tokens * group / 16 + std::min(seqs, tokens) : seqs * ((group + 15) / 16);
+  const int64_t step = kPaTile * kPaWaves;
+  const int64_t want = std::max<int64_t>(1, 4LL * cu_count() / std::max<int64_t>(1, p.tiles * kv_heads));
+  const int64_t steps = std::max<int64_t>(1, (room + step - 1) / step);
+  const int64_t per = std::max<int64_t>(1, (steps + want - 1) / want);
+  p.chunk = per * step;
+  p.splits = (steps + per - 1) / per;
+  return p;
+}
+}  // namespace
+
+extern "C" int64_t moc_paged_attention_workspace_size(int64_t tokens, int64_t seqs, int ragged, int64_t q_heads,
+                                                      int64_t kv_heads, int64_t head_dim, int64_t page, int64_t width) {
+  if (tokens <= 0 || seqs <= 0 || kv_heads <= 0 || q_heads <= 0) return 0;
+  const Plan p = plan_of(tokens, seqs, ragged != 0, q_heads / kv_heads, kv_heads, page * width);
+  return p.splits > 1 ? tokens * q_heads * p.splits * (head_dim * 4 + 8) : 0;
+}
+
+extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_lh, int64_t tokens, int64_t q_heads,
+                                        int64_t kv_heads, int64_t head_dim, int code, const void* k_codes,
+                                        const void* v_codes, const float* k_scale, const float* v_scale, int64_t pages,
+                                        int64_t page, const int32_t* table, int64_t ld_table, int64_t width,
+                                        const int32_t* lens, const int32_t* cu, int64_t seqs, float scale, void* out,
+                                        int64_t o_ld, int64_t o_lh, void* workspace, int64_t workspace_bytes,
+                                        void* stream) {
+  MOC_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256,
+              "moc_paged_attention_bf16: head_dim must be 64, 128 or 256");
+  MOC_REQUIRE(page >= 16 && page <= 256 && (page & (page - 1)) == 0,
+              "moc_paged_attention_bf16: page must be a power of two from 16 to 256");
+  MOC_REQUIRE(code == MOC_E4M3 || code == MOC_I8, "moc_paged_attention_bf16: codes must be e4m3 or int8");
+  MOC_REQUIRE(tokens >= 0 && seqs >= 0 && kv_heads >= 1 && q_heads >= 1 && q_heads % kv_heads == 0 && width >= 0 &&
+                  pages >= 0 && tokens < (1 << 24) && seqs < (1 << 24) && kv_heads <= 65535 && q_heads <= 65536 &&
+                  pages < (1LL << 31) && width < (1LL << 31),
+              "moc_paged_attention_bf16: bad shape");
+  MOC_REQUIRE(cu != nullptr || tokens == seqs, "moc_paged_attention_bf16: one token a sequence without cu");
+  if (tokens == 0 || seqs == 0) return MOC_OK;
+  MOC_REQUIRE(pages >= 1, "moc_paged_attention_bf16: the cache has no pages");
+  MOC_REQUIRE(q && k_codes && v_codes && k_scale && v_scale && (table || width == 0) && lens && out,
+              "moc_paged_attention_bf16: null pointer");
+  MOC_REQUIRE(aligned16(q) && aligned16(out) && aligned16(k_codes) && aligned16(v_codes) &&
+                  (q_ld | q_lh | o_ld | o_lh) % 8 == 0,
+              "moc_paged_attention_bf16: rows must be 16-byte aligned");
+  const int64_t group = q_heads / kv_heads;
+  const Plan p = plan_of(tokens, seqs, cu != nullptr, group, kv_heads, page * width);
+  const int64_t need = moc_paged_attention_workspace_size(tokens, seqs, cu != nullptr, q_heads, kv_heads, head_dim, page,
+                                                          width);
+  MOC_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
+              "moc_paged_attention_bf16: workspace of %lld bytes required", (long long)need);
+  PagedAttnArgs a;
+  a.s = PagedSeqs{cu, lens, table, ld_table, static_cast<int>(seqs), static_cast<int>(tokens), static_cast<int>(width)};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_ld = q_ld; a.q_lh = q_lh;
+  a.o = static_cast<uint16_t*>(out);
+  a.o_ld = o_ld; a.o_lh = o_lh;
+  a.kc = static_cast<const uint8_t*>(k_codes);
+  a.vc = static_cast<const uint8_t*>(v_codes);
+  a.ks = k_scale; a.vs = v_scale;
+  a.pages = static_cast<int>(pages);
+  a.log_page = __builtin_ctzll(static_cast<unsigned long long>(page));
+  a.heads = static_cast<int>(q_heads);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.group = static_cast<int>(group);
+  a.c2 = scale * 1.4426950408889634f;
+  a.chunk = static_cast<int>(std::min<int64_t>(p.chunk, 1 << 30));
+  a.splits = static_cast<int>(p.splits);
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + tokens * q_heads * p.splits * head_dim);
+  const dim3 grid(static_cast<unsigned>(p.tiles), static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.splits));
+  hipStream_t st = as_stream(stream);
+#define MOC_PA(D)                                                                \
+  do {                                                                           \
+    if (code == MOC_I8) paged_attn_kernel<D, true><<<grid, kPaThreads, 0, st>>>(a); \
+    else paged_attn_kernel<D, false><<<grid, kPaThreads, 0, st>>>(a);            \
+  } while (0)
+  if (head_dim == 64) MOC_PA(64);
+  else if (head_dim == 128) MOC_PA(128);
+  else MOC_PA(256);
+#undef MOC_PA
+  int rc = check_launch("paged_attn_kernel");
+  if (rc != MOC_OK || p.splits == 1) return rc;
+  const int64_t rows = tokens * q_heads;
+  const dim3 jg(static_cast<unsigned>((rows + 3) / 4));
+  if (head_dim == 64) paged_join_kernel<64><<<jg, 256, 0, st>>>(a, rows);
+  else if (head_dim == 128) paged_join_kernel<128><<<jg, 256, 0, st>>>(a, rows);
+  else paged_join_kernel<256><<<jg, 256, 0, st>>>(a, rows);
+  return check_launch("paged_join_kernel");
+}

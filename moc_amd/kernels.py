@@ -11,6 +11,8 @@ is 16-byte aligned; functions return the logical [:, :intermediate] view.
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import _native as N
@@ -1191,3 +1193,190 @@ def selected_grouped_down(sparse_z, idx, down_weight_t, *, out=None, workspace=N
            wdt.data_ptr(), ldw, inter, hidden, r.data_ptr(), y.data_ptr(), ws.data_ptr(), ws_bytes,
            N.stream_of(sz))
     return y
+
+
+# ------------------------------------- batched decode over a paged 8-bit cache
+class PagedKV(NamedTuple):
+    """Keys and values of many sequences in pages: codes [pages, kv_heads, page,
+    head_dim] (float8_e4m3fn or int8) and one f32 scale for each page and head
+    ([pages, kv_heads]); a value is code * scale.  page is a power of two from 16
+    to 256, head_dim 64, 128 or 256."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+_CODES = {torch.float8_e4m3fn: N.MOC_E4M3, torch.int8: N.MOC_I8}
+
+
+def paged_kv(pages: int, kv_heads: int, page: int, head_dim: int, *, dtype=torch.float8_e4m3fn,
+             device="cuda") -> PagedKV:
+    """An empty PagedKV.  Pages need no clearing between sequences: paged_append
+    begins a page anew when it writes its first place."""
+    if dtype not in _CODES:
+        raise ValueError(f"paged_kv: codes are float8_e4m3fn or int8, got {dtype}")
+    if pages < 0 or kv_heads < 1:
+        raise ValueError("paged_kv: pages >= 0 and kv_heads >= 1")
+    if head_dim not in (64, 128, 256):
+        raise ValueError("paged_kv: head_dim must be 64, 128 or 256")
+    if not 16 <= page <= 256 or page & (page - 1):
+        raise ValueError("paged_kv: page must be a power of two from 16 to 256")
+    shape = (pages, kv_heads, page, head_dim)
+    return PagedKV(*(torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for _ in range(2)),
+                   *(torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _paged_operands(what: str, kv: PagedKV, table, lens, cu, tokens: int):
+    """(code, codes' shape, sequences) after the checks that paged_append and
+    paged_attention share."""
+    k, v, ks, vs = kv
+    shape = k.shape
+    code = _CODES.get(k.dtype)
+    if code is None or v.dtype != k.dtype or ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        raise ValueError(f"{what}: the cache holds float8_e4m3fn or int8 codes and f32 scales")
+    if k.dim() != 4 or v.shape != shape or ks.shape != shape[:2] or vs.shape != shape[:2] or not (
+            k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError(f"{what}: the cache is contiguous [pages, kv_heads, page, head_dim] with [pages, kv_heads] scales")
+    if lens.dim() != 1 or table.dim() != 2 or table.shape[0] != lens.shape[0] or (
+            cu is not None and cu.shape != (lens.shape[0] + 1,)):
+        raise ValueError(f"{what}: lens [seqs], table [seqs, width], cu [seqs + 1]")
+    if cu is None and tokens != lens.shape[0]:
+        raise ValueError(f"{what}: {tokens} tokens of {lens.shape[0]} sequences need cu")
+    if lens.dtype != torch.int32 or table.dtype != torch.int32 or (cu is not None and cu.dtype != torch.int32):
+        raise ValueError(f"{what}: lens, table and cu are int32")
+    if not lens.is_contiguous() or (table.stride(1) != 1 and table.shape[1] > 1) or (
+            cu is not None and not cu.is_contiguous()):
+        raise ValueError(f"{what}: lens, cu and the rows of table are contiguous")
+    return code, shape, lens.shape[0]
+
+
+def _head_rows(t: torch.Tensor) -> torch.Tensor:
+    """[tokens, heads, dim] whose rows the kernels can read: unit stride inside,
+    16-byte aligned (a copy where they are not)."""
+    s = t.stride()
+    if s[2] == 1 and (s[0] | s[1]) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _rows_out(what: str, out, like: torch.Tensor) -> torch.Tensor:
+    """The output rows: new, or the caller's if the kernels can write them."""
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    t, h, d = like.shape
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise ValueError(f"{what}: out must be bf16 {tuple(like.shape)}")
+    s0, s1, s2 = out.stride()
+    if s2 != 1 or (s0 | s1) % 8 or out.data_ptr() % 16 or (h > 1 and s1 < d) or (t > 1 and s0 < (h - 1) * s1 + d):
+        raise ValueError(f"{what}: out needs 16-byte aligned rows that do not overlap")
+    return out
+
+
+def paged_append(q, k, v, cos, sin, kv: PagedKV, table, lens, cu=None, *, out=None) -> torch.Tensor:
+    """New tokens into the cache: q [tokens, q_heads, dim], k and v [tokens,
+    kv_heads, dim] in bf16 (any row strides: a projection's sections), RoPE on q
+    and k with the tables cos, sin [angles, dim / 2] (bf16 or f32), k and v into
+    kv at the last positions of each sequence; returns the rotated q.
+
+    table [seqs, width] (int32): the page that holds each sequence's positions
+    page * i ..; lens [seqs]: its tokens, the new ones counted; cu [seqs + 1]: its
+    rows of q (ascending), None for one token each.  A page that the call writes
+    to belongs to one sequence.  Scales are powers of two and grow with a page's
+    largest value, its older codes are then encoded again
+    (moc_paged_append_bf16).  Tokens without a place are not stored; rows behind
+    cu[-1] are left alone.  out: where the rotated q goes (may be q)."""
+    N.require_device(q, k, v, cos, sin, *kv, table, lens, cu, out)
+    if q.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return paged_append(q, k, v, cos, sin, kv, table, lens, cu, out=out)
+    if q.dim() != 3 or k.dim() != 3 or q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError("paged_append: q, k and v are bf16 [tokens, heads, dim]")
+    tokens, heads, dim = q.shape
+    code, (pages, kv_heads, page, kv_dim), seqs = _paged_operands("paged_append", kv, table, lens, cu, tokens)
+    if kv_dim != dim or k.shape != (tokens, kv_heads, dim) or v.shape != k.shape:
+        raise ValueError(f"paged_append: k and v must be {(tokens, kv_heads, kv_dim)}, q {(tokens, heads, kv_dim)}")
+    if cos.dim() != 2 or cos.shape[1] != dim // 2 or sin.shape != cos.shape or sin.dtype != cos.dtype or not (
+            cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("paged_append: cos and sin are contiguous [angles, dim / 2] of one dtype")
+    table_dtype = N.dtype_code(cos.dtype)
+    q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
+    out = _rows_out("paged_append", out, q)
+    (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), out.stride()
+    N.call("moc_paged_append_bf16", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, tokens, heads,
+           kv_heads, dim, cos.data_ptr(), sin.data_ptr(), table_dtype, cos.shape[0], code, kv.k.data_ptr(),
+           kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), pages, page, table.data_ptr(),
+           table.stride(0), table.shape[1], lens.data_ptr(), N.ptr(cu), seqs, out.data_ptr(), o0, o1, N.stream_of(q))
+    return out
+
+
+def paged_attention(q, kv: PagedKV, table, lens, cu=None, *, scale: float | None = None, out=None) -> torch.Tensor:
+    """Causal attention of q [tokens, q_heads, dim] (bf16, rotated) over the cache:
+    row r of a sequence sees the positions up to its own (table, lens, cu as for
+    paged_append, after which it is called); q_heads is a multiple of kv_heads and
+    head h reads kv head h // (q_heads // kv_heads).  scale: 1 / sqrt(dim) if None.
+    A row that sees nothing (lens 0: a slot of the batch not in use) is 0, one
+    that sees a position without a page NaN; rows behind cu[-1] are left alone.
+    The table's width bounds the work that is split over the length: pass the
+    columns in use."""
+    N.require_device(q, *kv, table, lens, cu, out)
+    if q.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return paged_attention(q, kv, table, lens, cu, scale=scale, out=out)
+    if q.dim() != 3 or q.dtype != torch.bfloat16:
+        raise ValueError("paged_attention: q is bf16 [tokens, heads, dim]")
+    tokens, heads, dim = q.shape
+    code, (pages, kv_heads, page, kv_dim), seqs = _paged_operands("paged_attention", kv, table, lens, cu, tokens)
+    if kv_dim != dim or heads < 1 or heads % kv_heads:
+        raise ValueError(f"paged_attention: q of {heads} heads of {dim} over a cache of {kv_heads} of {kv_dim}")
+    q = _head_rows(q)
+    out = _rows_out("paged_attention", out, q)
+    width = table.shape[1]
+    nbytes = N.query("moc_paged_attention_workspace_size", tokens, seqs, int(cu is not None), heads, kv_heads, dim,
+                     page, width)
+    ws = _empty((nbytes,), torch.uint8, q.device) if nbytes else None
+    (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
+    N.call("moc_paged_attention_bf16", q.data_ptr(), q0, q1, tokens, heads, kv_heads, dim, code, kv.k.data_ptr(),
+           kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), pages, page, table.data_ptr(),
+           table.stride(0), width, lens.data_ptr(), N.ptr(cu), seqs,
+           float(dim ** -0.5 if scale is None else scale), out.data_ptr(), o0, o1, N.ptr(ws), nbytes, N.stream_of(q))
+    return out
+
+
+def _per_row(name: str, value, rows: int, dtype) -> tuple[int | None, float]:
+    """A sampling setting as (pointer to one a row | None, one for all rows)."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    if value.dtype != dtype or value.shape != (rows,) or not value.is_contiguous():
+        raise ValueError(f"sample_tokens: {name} is a number or a contiguous {dtype} tensor [{rows}]")
+    return value.data_ptr(), 0
+
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
+    """One token id (int64 [rows]) drawn from each row of logits [rows, vocab]
+    (bf16 or f32) with the uniform numbers u (f32 [rows], in [0, 1)).  Settings are
+    numbers or tensors [rows] (f32; top_k int32): temperature <= 0 takes the best
+    id; top_k <= 0, top_p >= 1 and min_p <= 0 are off.  In this order: the first
+    top_k ids (by logit, then the lower id), of those the fewest that hold top_p of
+    their weight, of those the ones with min_p of the best's weight; the draw walks
+    what is left by ascending id.  Weights are held in 64 bits, so the id is that
+    of exact arithmetic.  NaN logits are never drawn; a row with nothing to draw
+    gives -1 (moc_sample_tokens)."""
+    settings = (temperature, top_k, top_p, min_p)
+    N.require_device(logits, u, *(t for t in settings if isinstance(t, torch.Tensor)))
+    if logits.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            return sample_tokens(logits, u, *settings)
+    x, ld = _rows_view(logits)
+    rows, vocab = x.shape
+    if u.dtype != torch.float32 or u.shape != (rows,) or not u.is_contiguous():
+        raise ValueError(f"sample_tokens: u is a contiguous f32 tensor [{rows}]")
+    f32 = torch.float32
+    temperature, top_p, min_p = (_per_row(n, t, rows, f32) for n, t in (
+        ("temperature", temperature), ("top_p", top_p), ("min_p", min_p)))
+    top_k = _per_row("top_k", top_k, rows, torch.int32)
+    out = _empty((rows,), torch.int64, x.device)
+    N.call("moc_sample_tokens", N.dtype_code(x.dtype), x.data_ptr(), rows, vocab, ld, u.data_ptr(), *temperature,
+           top_k[0], max(min(int(top_k[1]), vocab), 0), *top_p, *min_p, out.data_ptr(), N.stream_of(x))
+    return out
