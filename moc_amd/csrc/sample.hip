@@ -7,15 +7,29 @@
 //   token is the first id, in ascending order, whose kept weight up to and with
 //   it exceeds u times the kept weight.  T <= 0: the best id.
 //
-// All three rules keep a prefix of one order, so what is kept is one key (the
-// order key of x), how many ids of that key, and min-p's bound.
-//
 // Weights.  A draw falls between two words' shares; with f32 weights the border
 // is off by 1e-7 of the row's weight and one draw in a few hundred over 32000
-// words would give the neighbour.  So w is 2^y with y in 64 bits, from the series of
-// exp to the tenth power (|z| <= ln 2 / 2: 3e-13), held as an integer of 2^-44
-// units: sums of integers have no order, so that histograms by atomics give the
-// same bits each time; 2^18 words sum to less than 2^62.
+// words would give the neighbour.  So w = 2^y with y in 64 bits: a table of
+// 2^(i/64) and the series of 2^r to the fourth power (|r| <= 2^-7: 4e-14), held
+// in units of 2^-44.  Sums of these are sums of integers (2^18 words: less than
+// 2^62) and have no order, so histograms by atomics give the same bits each time.
+//
+// Rules.  Top-k and top-p keep a prefix of one order, so what is kept is its last
+// word, (key, id).  It is found with a histogram over the distance from the best
+// in 1/88 octaves of weight (numbers of words for top-k, their weights for top-p;
+// 4096 bins reach 46.5 octaves, below which a weight is 0) and then among the
+// words of the bin where the rule's amount is reached, each against all others;
+// where they are too many (equal logits), digit by digit of the order key.
+// A few hundred words or less left by top-k go on as a list in LDS.
+//
+// One workgroup a row: the largest value, a histogram for each rule in use, the
+// weights by blocks of 16 bytes a lane, the block and then the lane of the draw.
+// The row is read again for each pass (128 KB of 32000 words from L2 at 64 B a
+// clock: under a microsecond).  Bound by the 64-bit arithmetic of the weights,
+// about 25 instructions a word and pass, and for few words by the chain of
+// passes and barriers.
+#include <type_traits>
+
 #include "abi.h"
 #include "common.h"
 
@@ -24,13 +38,18 @@ namespace {
 
 constexpr int kSmThreads = 1024;
 constexpr int kSmWaves = kSmThreads / 64;
-constexpr int kSmBits = 44;
+constexpr int kSmBins = 4 * kSmThreads;
+constexpr double kSmBinsPerOctave = 88.0;
 constexpr int64_t kSmMaxVocab = 1 << 18;
+constexpr int kSmBlocks = kSmMaxVocab / 256;  // blocks of f32 words
+constexpr int kSmList = 512;                  // words compared each with all
+constexpr int kSmFew = 256;                   // words left by top-k that go on as a list
 
 struct SampleArgs {
   const void* x;
   int64_t ld;
   int vocab;
+  bool wide;  // rows in 16-byte loads
   const float *u, *temp, *top_p, *min_p;  // per row, or null: the number below
   const int32_t* top_k;
   float temp1, top_p1, min_p1;
@@ -38,242 +57,438 @@ struct SampleArgs {
   int64_t* out;
 };
 
-template <bool BF16>
-__device__ __forceinline__ float logit(const SampleArgs& a, int64_t row, int i) {
-  const float x = BF16 ? bf16_to_f32(static_cast<const uint16_t*>(a.x)[row * a.ld + i])
-                       : static_cast<const float*>(a.x)[row * a.ld + i];
-  return x != x ? -INFINITY : x;  // NaN is never drawn
-}
-
-struct Weights {
-  float max;
-  double c;  // log2(e) / T
-  __device__ __forceinline__ uint64_t operator()(float x) const {
-    if (x == max) return 1ull << kSmBits;
-    const double y = (static_cast<double>(x) - static_cast<double>(max)) * c;
-    if (!(y > -46.0)) return 0;
-    const double n = rint(y), z = (y - n) * 0.69314718055994530942;
-    double p = 1.0 / 3628800.0;
-    p = fma(p, z, 1.0 / 362880.0);
-    p = fma(p, z, 1.0 / 40320.0);
-    p = fma(p, z, 1.0 / 5040.0);
-    p = fma(p, z, 1.0 / 720.0);
-    p = fma(p, z, 1.0 / 120.0);
-    p = fma(p, z, 1.0 / 24.0);
-    p = fma(p, z, 1.0 / 6.0);
-    p = fma(p, z, 0.5);
-    p = fma(p, z, 1.0);
-    p = fma(p, z, 1.0);
-    return static_cast<uint64_t>(rint(ldexp(p, static_cast<int>(n) + kSmBits)));
-  }
-};
-
-struct Lds {
-  uint64_t mass[256];
-  uint32_t count[256];
+struct SampleLds {
+  uint64_t hist[kSmBins];    // weights; as uint32_t: numbers of words
+  uint64_t block[kSmBlocks];  // kept weight of each block of words
+  double pow2[64];
+  uint32_t key[kSmList];
+  int id[kSmList];
+  uint64_t w[kSmList];
   uint64_t wave[kSmWaves];
-  float fmax[kSmWaves];
-  int imin[kSmWaves];
-  uint64_t r64[2];
-  int r32[4];
+  float top[kSmWaves];
+  int first;
+  int n;
+  uint32_t cut_key;
+  int cut_id;
+  int bin;
+  uint64_t above;
 };
+
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
+  return __shfl_xor(static_cast<unsigned long long>(v), o);
+}
 
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(static_cast<unsigned long long>(v), o);
+  for (int o = 32; o > 0; o >>= 1) v += shfl_xor64(v, o);
   return v;
 }
 
-// Sum of v over the lanes before this one.
-__device__ __forceinline__ uint64_t wave_before64(uint64_t v) {
+// Sum of v over the lanes up to and with this one.
+__device__ __forceinline__ uint64_t wave_upto64(uint64_t v) {
   const int lane = threadIdx.x & 63;
-  uint64_t s = v;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t t = __shfl_up(static_cast<unsigned long long>(s), o);
-    if (lane >= o) s += t;
+    const uint64_t t = __shfl_up(static_cast<unsigned long long>(v), o);
+    if (lane >= o) v += t;
   }
-  return s - v;
+  return v;
+}
+
+// Sum of v over the threads before this one; total over all.
+__device__ __forceinline__ uint64_t block_before64(uint64_t v, uint64_t* wave_lds, uint64_t& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t upto = wave_upto64(v);
+  __syncthreads();
+  if (lane == 63) wave_lds[wave] = upto;
+  __syncthreads();
+  uint64_t before = upto - v;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kSmWaves; ++w) {
+    const uint64_t t = wave_lds[w];
+    if (w < wave) before += t;
+    total += t;
+  }
+  return before;
+}
+
+__device__ __forceinline__ uint32_t key_of(float x) { return f32_order_key(__float_as_uint(x)); }
+
+// Weights relative to the best, in units of 2^-44, and bins.
+struct Scale {
+  float top;
+  double c;  // log2(e) / T
+  float cf;  // bins per unit of x
+  const double* pow2;
+
+  __device__ __forceinline__ uint64_t weight(float x) const {
+    const double y = (static_cast<double>(x) - static_cast<double>(top)) * c;
+    // to the nearest 1/64: the low bits of y + 1.5 2^46 hold 64 y
+    const double t = y + 105553116266496.0;
+    const int n = static_cast<int>(__double_as_longlong(t));
+    const double r = y - (t - 105553116266496.0);
+    double q = fma(r, 9.618129107628477e-3, 5.550410866482158e-2);  // ln2^4 / 24, ln2^3 / 6
+    q = fma(q, r, 2.402265069591007e-1);                            // ln2^2 / 2
+    q = fma(q, r, 6.931471805599453e-1);                            // ln2
+    const double b = pow2[n & 63];
+    const double w = __longlong_as_double(__double_as_longlong(fma(q * r, b, b)) + (static_cast<int64_t>(n >> 6) << 52));
+    // 256 + w has units of 2^-44
+    const uint64_t i = static_cast<uint64_t>(__double_as_longlong(256.0 + w)) - 0x4070000000000000ull;
+    return x == top ? 1ull << 44 : y > -46.0 ? i : 0;
+  }
+  // The bin of x; kSmBins or more: no weight.  Never lower for a smaller x.
+  __device__ __forceinline__ int bin(float x) const {
+    const float y = (top - x) * cf;
+    return x == top ? 0 : y < static_cast<float>(kSmBins) ? static_cast<int>(y) : kSmBins;
+  }
+};
+
+// f(block, first id, words of this lane) over the row's blocks, each wave its own,
+// four loads in flight; words past the row and NaN are -infinity.
+template <bool BF16, typename F>
+__device__ __forceinline__ void each_block(const SampleArgs& a, int64_t row, int first, int stride, int blocks, F f) {
+  constexpr int kPer = BF16 ? 8 : 4, kAhead = 4;
+  const int lane = threadIdx.x & 63;
+  const uint16_t* p16 = static_cast<const uint16_t*>(a.x) + row * a.ld;
+  const float* p32 = static_cast<const float*>(a.x) + row * a.ld;
+  for (int b0 = first; b0 < blocks; b0 += kAhead * stride) {
+    uint4 raw[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int b = b0 + j * stride, i = (b * 64 + lane) * kPer;
+      raw[j] = BF16 ? make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u)
+                    : make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
+      if (b >= blocks || i >= a.vocab) continue;
+      if (a.wide && i + kPer <= a.vocab) {
+        raw[j] = BF16 ? *reinterpret_cast<const uint4*>(p16 + i) : *reinterpret_cast<const uint4*>(p32 + i);
+      } else {
+        uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          if (i + e >= a.vocab) continue;
+          if (BF16)
+            w[e / 2] = (e & 1) ? (w[e / 2] & 0xFFFFu) | (static_cast<uint32_t>(p16[i + e]) << 16)
+                               : (w[e / 2] & 0xFFFF0000u) | p16[i + e];
+          else
+            w[e & 3] = __float_as_uint(p32[i + e]);
+        }
+        raw[j] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int b = b0 + j * stride;
+      if (b >= blocks) break;
+      const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+      float x[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        x[e] = __uint_as_float(BF16 ? ((e & 1) ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16) : w[e & 3]);
+        x[e] = x[e] != x[e] ? -INFINITY : x[e];
+      }
+      f(b, (b * 64 + lane) * kPer, x);
+    }
+  }
 }
 
 template <bool BF16>
 __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
-  __shared__ Lds lds;
+  constexpr int kPer = BF16 ? 8 : 4;
+  __shared__ SampleLds s;
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int blocks = (a.vocab + 64 * kPer - 1) / (64 * kPer);
   const float T = a.temp ? a.temp[row] : a.temp1;
   const int k = a.top_k ? a.top_k[row] : a.top_k1;
   const float p = a.top_p ? a.top_p[row] : a.top_p1, min_p = a.min_p ? a.min_p[row] : a.min_p1;
+  const float u = a.u[row];
+  auto pass = [&](auto f) { each_block<BF16>(a, row, wave, kSmWaves, blocks, f); };
 
-  // the best, lowest id first
-  float best = -INFINITY;
-  int at = V;
-  for (int i = tid; i < V; i += kSmThreads) {
-    const float x = logit<BF16>(a, row, i);
-    if (x > best) {
-      best = x;
-      at = i;
-    }
-  }
+  // the best
+  float top = -INFINITY;
+  pass([&](int, int, const float(&x)[kPer]) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float x = __shfl_xor(best, o);
-    const int j = __shfl_xor(at, o);
-    if (x > best || (x == best && j < at)) {
-      best = x;
-      at = j;
-    }
-  }
-  if (lane == 0) {
-    lds.fmax[wave] = best;
-    lds.imin[wave] = at;
+    for (int e = 0; e < kPer; ++e) top = fmaxf(top, x[e]);
+  });
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (lane == 0) s.top[wave] = top;
+  if (tid < 64) s.pow2[tid] = exp2(tid / 64.0);
+  if (tid == 0) {
+    s.first = a.vocab;
+    s.cut_key = 0;
+    s.cut_id = a.vocab;
   }
   __syncthreads();
-  for (int w = 0; w < kSmWaves; ++w) {
-    const float x = lds.fmax[w];
-    const int j = lds.imin[w];
-    if (x > best || (x == best && j < at)) {
-      best = x;
-      at = j;
-    }
-  }
-  if (best == -INFINITY) {  // nothing to draw
+#pragma unroll
+  for (int w = 0; w < kSmWaves; ++w) top = fmaxf(top, s.top[w]);
+  if (top == -INFINITY) {  // nothing to draw
     if (tid == 0) a.out[row] = -1;
     return;
   }
-  if (!(T > 0.f)) {
-    if (tid == 0) a.out[row] = at;
+  if (!(T > 0.f) || k == 1 || p <= 0.f) {  // the best alone: its lowest id
+    int at = a.vocab;
+    pass([&](int, int i, const float(&x)[kPer]) {
+#pragma unroll
+      for (int e = kPer - 1; e >= 0; --e)
+        if (x[e] == top) at = min(at, i + e);
+    });
+    if (at < a.vocab) atomicMin(&s.first, at);
+    __syncthreads();
+    if (tid == 0) a.out[row] = s.first;
     return;
   }
-  const Weights weight{best, 1.4426950408889634074 / static_cast<double>(T)};
+  const double c = 1.4426950408889634074 / static_cast<double>(T);
+  const Scale sc{top, c, static_cast<float>(c * kSmBinsPerOctave), s.pow2};
+  const uint64_t least =
+      min_p > 0.f ? static_cast<uint64_t>(ceil(ldexp(fmin(static_cast<double>(min_p), 1.0), 44))) : 1;
+  uint32_t cut_key = 0;
+  int cut_id = a.vocab;
+  auto kept = [&](uint32_t key, int id) { return key > cut_key || (key == cut_key && id <= cut_id); };
+  uint32_t* const count = reinterpret_cast<uint32_t*>(s.hist);
 
-  // kept so far: keys above `key`, and the first `ties` ids of that key
-  uint32_t key = 0;
-  int ties = V;
-  // One digit of the order key at a time: the digit where the ids above
-  // (`before`) reach the rule's amount.
-  auto descend = [&](bool by_mass, uint64_t target, double share) {
-    uint32_t prefix = 0, mask = 0;
-    uint64_t above_mass = 0;
-    int above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (tid < 256) {
-        lds.mass[tid] = 0;
-        lds.count[tid] = 0;
-      }
-      __syncthreads();
-      for (int i = tid; i < V; i += kSmThreads) {
-        const float x = logit<BF16>(a, row, i);
-        const uint32_t q = f32_order_key(__float_as_uint(x));
-        if ((q & mask) != prefix || q < key) continue;
-        const int b = (q >> shift) & 255;
-        atomicAdd(&lds.count[b], 1u);
-        if (by_mass) atomicAdd(reinterpret_cast<unsigned long long*>(&lds.mass[b]), weight(x));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int b = 255;
-        for (; b > 0; --b) {
-          // the ids of this bin exhaust the rule?
-          uint32_t n = lds.count[b];
-          if (by_mass ? static_cast<double>(above_mass + lds.mass[b]) >= share
-                      : static_cast<uint64_t>(above) + n >= target)
-            break;
-          above += n;
-          above_mass += lds.mass[b];
+  // The last word that a rule keeps: the one whose number of words (BY false:
+  // `words`) or weight (`share`) before it is the last below the rule's amount.
+  // False if the rule keeps all words with weight.
+  auto cut = [&](auto by, uint32_t words, double share) -> bool {
+    constexpr bool BY = decltype(by)::value;
+    __syncthreads();
+    for (int i = tid; i < kSmBins; i += kSmThreads) {
+      if (BY) s.hist[i] = 0;
+      else count[i] = 0;
+    }
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    pass([&](int, int i, const float(&x)[kPer]) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int b = sc.bin(x[e]);
+        if (b >= kSmBins) continue;
+        if (BY) {
+          if (kept(key_of(x[e]), i + e))
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[b]), sc.weight(x[e]));
+        } else {
+          atomicAdd(&count[b], 1u);
         }
-        lds.r32[0] = b;
-        lds.r32[1] = above;
-        lds.r64[0] = above_mass;
+      }
+    });
+    __syncthreads();
+    uint64_t v[4], sum = 0, total;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = BY ? s.hist[4 * tid + j] : count[4 * tid + j];
+      sum += v[j];
+    }
+    uint64_t before = block_before64(sum, s.wave, total);
+    if (BY) share *= static_cast<double>(total);
+    auto reached = [&](uint64_t t) { return BY ? static_cast<double>(t) >= share : t >= words; };
+    if (!reached(total) || (!BY && total == words)) return false;
+    if (!reached(before) && reached(before + sum)) {
+      int j = 0;
+      while (!reached(before + v[j])) before += v[j++];
+      s.bin = 4 * tid + j;
+      s.above = before;
+    }
+    __syncthreads();
+    const int bin = s.bin;
+    const uint64_t above = s.above;
+    pass([&](int, int i, const float(&x)[kPer]) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        if (sc.bin(x[e]) != bin) continue;
+        const uint32_t key = key_of(x[e]);
+        if (!kept(key, i + e)) continue;
+        const int at = atomicAdd(&s.n, 1);
+        if (at < kSmList) {
+          s.key[at] = key;
+          s.id[at] = i + e;
+          s.w[at] = BY ? sc.weight(x[e]) : 1;
+        }
+      }
+    });
+    __syncthreads();
+    const int n = s.n;
+    if (n <= kSmList) {
+      // 2^g threads for each word, its own share of the others each
+      const int g = n <= 1 ? 6 : min(6, 10 - (32 - __clz(n - 1))), e = tid >> g;
+      uint64_t b = 0;
+      if (e < n) {
+        const uint32_t key = s.key[e];
+        const int id = s.id[e];
+        for (int o = tid & ((1 << g) - 1); o < n; o += 1 << g)
+          if (s.key[o] > key || (s.key[o] == key && s.id[o] < id)) b += s.w[o];
+      }
+      for (int o = 1; o < (1 << g); o <<= 1) b += shfl_xor64(b, o);
+      if (e < n && (tid & ((1 << g) - 1)) == 0 && !reached(above + b) && reached(above + b + s.w[e])) {
+        s.cut_key = s.key[e];
+        s.cut_id = s.id[e];
+      }
+    } else {
+      // the order key of the word where the amount is reached, a digit at a time
+      uint32_t prefix = 0;
+      uint64_t high = above;
+      for (int shift = 24; shift >= 0; shift -= 8) {
+        const uint32_t mask = shift == 24 ? 0 : ~0u << (shift + 8);
+        __syncthreads();
+        if (tid < 256) s.hist[tid] = 0;
+        __syncthreads();
+        pass([&](int, int i, const float(&x)[kPer]) {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const uint32_t key = key_of(x[e]);
+            if (sc.bin(x[e]) != bin || (key & mask) != prefix || !kept(key, i + e)) continue;
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[(key >> shift) & 255]),
+                      BY ? sc.weight(x[e]) : 1ull);
+          }
+        });
+        __syncthreads();
+        // thread t: digit 255 - t
+        const uint64_t mine = tid < 256 ? s.hist[255 - tid] : 0;
+        const uint64_t ahead = high + block_before64(mine, s.wave, total);
+        if (!reached(ahead) && reached(ahead + mine)) {
+          s.bin = 255 - tid;
+          s.above = ahead;
+        }
+        __syncthreads();
+        prefix |= static_cast<uint32_t>(s.bin) << shift;
+        high = s.above;
+      }
+      // of the equal words, the one where it is reached: one block of words at a time
+      for (int b = tid; b < kSmBlocks; b += kSmThreads) s.block[b] = 0;
+      __syncthreads();
+      auto mine_of = [&](int i, const float(&x)[kPer]) {
+        uint64_t m = 0;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+          if (key_of(x[e]) == prefix && kept(prefix, i + e)) m += BY ? sc.weight(x[e]) : 1;
+        return m;
+      };
+      pass([&](int b, int i, const float(&x)[kPer]) {
+        const uint64_t m = wave_sum64(mine_of(i, x));
+        if (lane == 0) s.block[b] = m;
+      });
+      __syncthreads();
+      uint64_t m = tid < blocks ? s.block[tid] : 0;
+      uint64_t ahead = high + block_before64(m, s.wave, total);
+      if (!reached(ahead) && reached(ahead + m)) {
+        s.bin = tid;
+        s.above = ahead;
       }
       __syncthreads();
-      prefix |= static_cast<uint32_t>(lds.r32[0]) << shift;
-      mask |= 255u << shift;
-      above = lds.r32[1];
-      above_mass = lds.r64[0];
+      if (wave == 0) {
+        const uint64_t from = s.above;
+        each_block<BF16>(a, row, s.bin, kSmBlocks, min(blocks, s.bin + 1), [&](int, int i, const float(&x)[kPer]) {
+          uint64_t at = from + wave_upto64(mine_of(i, x)) - mine_of(i, x);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            if (key_of(x[e]) != prefix || !kept(prefix, i + e)) continue;
+            const uint64_t w = BY ? sc.weight(x[e]) : 1;
+            if (!reached(at) && reached(at + w)) {
+              s.cut_key = prefix;
+              s.cut_id = i + e;
+            }
+            at += w;
+          }
+        });
+      }
     }
-    int n = static_cast<int>(lds.count[prefix & 255]);
-    if (prefix == key) n = min(n, ties);
-    if (by_mass) {  // of equal weights, those with less than the share before them
-      const uint64_t w = n > 0 ? lds.mass[prefix & 255] / lds.count[prefix & 255] : 0;
-      int c = 0;
-      while (c < n && static_cast<double>(above_mass + w * static_cast<uint64_t>(c)) < share) ++c;
-      n = c;
-    } else {
-      n = min(n, static_cast<int>(target) - above);
-    }
-    key = prefix;
-    ties = n;
     __syncthreads();
+    cut_key = s.cut_key;
+    cut_id = s.cut_id;
+    return true;
   };
-  if (k > 0 && k < V) descend(false, static_cast<uint64_t>(k), 0.0);
 
-  // A thread owns a run of ids, so that the ids of one key are met in order.
-  const int run = (V + kSmThreads - 1) / kSmThreads, i0 = min(tid * run, V), i1 = min(i0 + run, V);
-  auto totals = [&](uint64_t floor, uint64_t& before, uint64_t& total, int& rank) {
-    int mine = 0;
-    for (int i = i0; i < i1; ++i) mine += f32_order_key(__float_as_uint(logit<BF16>(a, row, i))) == key;
+  if (k > 0 && k < a.vocab && cut(std::false_type(), static_cast<uint32_t>(k), 0.0) && k <= kSmFew) {
+    // few words: a list
+    if (tid == 0) s.n = 0;
     __syncthreads();
-    const uint64_t rb = wave_before64(static_cast<uint64_t>(mine));
-    if (lane == 63) lds.wave[wave] = rb + mine;
+    pass([&](int, int i, const float(&x)[kPer]) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const uint32_t key = key_of(x[e]);
+        if (!kept(key, i + e)) continue;
+        const int at = atomicAdd(&s.n, 1);
+        if (at < kSmList) {
+          s.key[at] = key;
+          s.id[at] = i + e;
+          s.w[at] = sc.weight(x[e]);
+        }
+      }
+    });
     __syncthreads();
-    uint64_t r = rb;
-    for (int w = 0; w < wave; ++w) r += lds.wave[w];
-    rank = static_cast<int>(r);
-    int seen = rank;
-    uint64_t s = 0;
-    for (int i = i0; i < i1; ++i) {
-      const float x = logit<BF16>(a, row, i);
-      const uint32_t q = f32_order_key(__float_as_uint(x));
-      if (q < key || (q == key && seen++ >= ties)) continue;
-      const uint64_t w = weight(x);
-      if (w >= floor) s += w;
+    const int n = min(s.n, kSmList);  // k
+    const int g = min(6, 10 - (32 - __clz(n - 1))), e = tid >> g, sub = tid & ((1 << g) - 1);
+    const bool mine = e < n && sub == 0;
+    const uint32_t key = e < n ? s.key[e] : 0;
+    const int id = e < n ? s.id[e] : 0;
+    uint64_t w = e < n ? s.w[e] : 0, total;
+    if (p < 1.f) {
+      uint64_t b = 0;
+      for (int o = sub; o < n && e < n; o += 1 << g)
+        if (s.key[o] > key || (s.key[o] == key && s.id[o] < id)) b += s.w[o];
+      for (int o = 1; o < (1 << g); o <<= 1) b += shfl_xor64(b, o);
+      block_before64(mine ? w : 0, s.wave, total);
+      if (!(static_cast<double>(b) < static_cast<double>(p) * static_cast<double>(total))) w = 0;
     }
+    if (w < least) w = 0;
+    block_before64(mine ? w : 0, s.wave, total);
+    if (mine) s.w[e] = w;
     __syncthreads();
-    const uint64_t sb = wave_before64(s);
-    if (lane == 63) lds.wave[wave] = sb + s;
-    __syncthreads();
-    before = sb;
-    total = 0;
-    for (int w = 0; w < kSmWaves; ++w) {
-      if (w < wave) before += lds.wave[w];
-      total += lds.wave[w];
+    const double target = (u > 0.f ? static_cast<double>(u) : 0.0) * static_cast<double>(total);
+    uint64_t b = 0;
+    for (int o = sub; o < n && e < n; o += 1 << g)
+      if (s.id[o] < id) b += s.w[o];
+    for (int o = 1; o < (1 << g); o <<= 1) b += shfl_xor64(b, o);
+    if (mine && w > 0 && (target < static_cast<double>(total)
+                              ? static_cast<double>(b) <= target && static_cast<double>(b + w) > target
+                              : b + w == total))
+      a.out[row] = id;
+    return;
+  }
+  if (p < 1.f) cut(std::true_type(), 0, static_cast<double>(p));
+
+  // kept weight of each block of words
+  auto weights = [&](int i, const float(&x)[kPer], uint64_t(&w)[kPer]) {
+    uint64_t sum = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const uint64_t t = sc.weight(x[e]);
+      w[e] = t >= least && kept(key_of(x[e]), i + e) ? t : 0;
+      sum += w[e];
     }
+    return sum;
   };
-  uint64_t before, total;
-  int rank;
-  if (p < 1.f) {
-    totals(0, before, total, rank);
-    const double share = fmax(static_cast<double>(p), 0.0) * static_cast<double>(total);
-    if (share > 0.0) {
-      descend(true, 0, share);
-    } else {  // the best alone
-      key = f32_order_key(__float_as_uint(best));
-      ties = 1;
+  pass([&](int b, int i, const float(&x)[kPer]) {
+    uint64_t w[kPer];
+    const uint64_t sum = wave_sum64(weights(i, x, w));
+    if (lane == 0) s.block[b] = sum;
+  });
+  __syncthreads();
+  const uint64_t mine = tid < blocks ? s.block[tid] : 0;
+  uint64_t total;
+  const uint64_t before = block_before64(mine, s.wave, total);
+  const double target = (u > 0.f ? static_cast<double>(u) : 0.0) * static_cast<double>(total);
+  const bool inside = target < static_cast<double>(total);  // else the last word with weight
+  if (mine > 0 && (inside ? static_cast<double>(before) <= target && static_cast<double>(before + mine) > target
+                          : before + mine == total)) {
+    s.bin = tid;
+    s.above = before;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  each_block<BF16>(a, row, s.bin, kSmBlocks, s.bin + 1, [&](int, int i, const float(&x)[kPer]) {
+    uint64_t w[kPer];
+    const uint64_t sum = weights(i, x, w);
+    uint64_t at = s.above + wave_upto64(sum) - sum;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (w[e] > 0 && (inside ? static_cast<double>(at) <= target && static_cast<double>(at + w[e]) > target
+                              : at + w[e] == total))
+        a.out[row] = i + e;
+      at += w[e];
     }
-    if (ties < 1) ties = 1;
-  }
-  uint64_t floor = 1;
-  if (min_p > 0.f) floor = static_cast<uint64_t>(ceil(ldexp(fmin(static_cast<double>(min_p), 1.0), kSmBits)));
-  totals(floor, before, total, rank);
-  const float u = a.u[row];
-  const double target = (u > 0.f ? static_cast<double>(fminf(u, 1.f)) : 0.0) * static_cast<double>(total);
-  // u >= 1: the last id with weight
-  uint64_t sum = before;
-  int seen = rank, got = -1, last = -1;
-  for (int i = i0; i < i1; ++i) {
-    const float x = logit<BF16>(a, row, i);
-    const uint32_t q = f32_order_key(__float_as_uint(x));
-    if (q < key || (q == key && seen++ >= ties)) continue;
-    const uint64_t w = weight(x);
-    if (w < floor) continue;
-    last = i;
-    if (got < 0 && static_cast<double>(sum) <= target && static_cast<double>(sum + w) > target) got = i;
-    sum += w;
-  }
-  if (got >= 0) a.out[row] = got;
-  if (static_cast<double>(total) <= target && last >= 0 && sum == total) a.out[row] = last;
+  });
 }
 
 }  // namespace
@@ -290,7 +505,8 @@ extern "C" int moc_sample_tokens(int dtype, const void* logits, int64_t rows, in
               "moc_sample_tokens: 1 to %lld words a row", (long long)kSmMaxVocab);
   if (rows == 0) return MOC_OK;
   MOC_REQUIRE(logits && u && out, "moc_sample_tokens: null pointer");
-  const SampleArgs a{logits, ld, static_cast<int>(vocab), u, temperature, top_p, min_p, top_k,
+  const bool wide = aligned16(logits) && (rows == 1 || ld % (dtype == MOC_BF16 ? 8 : 4) == 0);
+  const SampleArgs a{logits, ld, static_cast<int>(vocab), wide, u, temperature, top_p, min_p, top_k,
                      temperature1, top_p1, min_p1, top_k1, out};
   const dim3 grid(static_cast<unsigned>(rows));
   if (dtype == MOC_BF16) sample_kernel<true><<<grid, kSmThreads, 0, as_stream(stream)>>>(a);
