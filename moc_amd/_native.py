@@ -256,6 +256,27 @@ def require_device(*tensors: torch.Tensor) -> None:
             raise ValueError(f"MoC HIP kernels need all tensors on one device, got {devs}")
 
 
+def one_device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """require_device in one look at each tensor; the device's index."""
+    dev = first.get_device()
+    if dev < 0:
+        require_device(first, *others)
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            require_device(first, *others)
+    return dev
+
+
+def is_current(device_index: int) -> bool:
+    """Whether launches go to this device as they are."""
+    return torch._C._cuda_getDevice() == device_index
+
+
+def stream_on(device_index: int) -> int:
+    """stream_of a tensor on this device."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.bfloat16:
         return MOC_BF16

@@ -1228,50 +1228,54 @@ def paged_kv(pages: int, kv_heads: int, page: int, head_dim: int, *, dtype=torch
 
 
 def _paged_operands(what: str, kv: PagedKV, table, lens, cu, tokens: int):
-    """(code, codes' shape, sequences) after the checks that paged_append and
-    paged_attention share."""
+    """(code, codes' shape, sequences, width) after the checks that paged_append
+    and paged_attention share."""
     k, v, ks, vs = kv
-    shape = k.shape
-    code = _CODES.get(k.dtype)
+    shape, code = k.shape, _CODES.get(k.dtype)
     if code is None or v.dtype != k.dtype or ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise ValueError(f"{what}: the cache holds float8_e4m3fn or int8 codes and f32 scales")
-    if k.dim() != 4 or v.shape != shape or ks.shape != shape[:2] or vs.shape != shape[:2] or not (
+    scales = shape[:2]
+    if len(shape) != 4 or v.shape != shape or ks.shape != scales or vs.shape != scales or not (
             k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError(f"{what}: the cache is contiguous [pages, kv_heads, page, head_dim] with [pages, kv_heads] scales")
-    if lens.dim() != 1 or table.dim() != 2 or table.shape[0] != lens.shape[0] or (
-            cu is not None and cu.shape != (lens.shape[0] + 1,)):
+    wide, (seqs, *more) = table.shape, lens.shape or (0, 0)
+    if more or len(wide) != 2 or wide[0] != seqs or (cu is not None and cu.shape != (seqs + 1,)):
         raise ValueError(f"{what}: lens [seqs], table [seqs, width], cu [seqs + 1]")
-    if cu is None and tokens != lens.shape[0]:
-        raise ValueError(f"{what}: {tokens} tokens of {lens.shape[0]} sequences need cu")
+    if cu is None and tokens != seqs:
+        raise ValueError(f"{what}: {tokens} tokens of {seqs} sequences need cu")
     if lens.dtype != torch.int32 or table.dtype != torch.int32 or (cu is not None and cu.dtype != torch.int32):
         raise ValueError(f"{what}: lens, table and cu are int32")
-    if not lens.is_contiguous() or (table.stride(1) != 1 and table.shape[1] > 1) or (
+    if not lens.is_contiguous() or (wide[1] > 1 and table.stride(1) != 1) or (
             cu is not None and not cu.is_contiguous()):
         raise ValueError(f"{what}: lens, cu and the rows of table are contiguous")
-    return code, shape, lens.shape[0]
+    return code, shape, seqs, wide[1]
 
 
-def _head_rows(t: torch.Tensor) -> torch.Tensor:
-    """[tokens, heads, dim] whose rows the kernels can read: unit stride inside,
-    16-byte aligned (a copy where they are not)."""
-    s = t.stride()
-    if s[2] == 1 and (s[0] | s[1]) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
+def _head_rows(t: torch.Tensor):
+    """([tokens, heads, dim] whose rows the kernels can read: unit stride inside,
+    16-byte aligned, a copy where they are not; strides; address)."""
+    s, p = t.stride(), t.data_ptr()
+    if s[2] == 1 and not ((s[0] | s[1]) & 7 or p & 15):
+        return t, s, p
     t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
+    if t.data_ptr() & 15:
+        t = t.clone()
+    return t, t.stride(), t.data_ptr()
 
 
-def _rows_out(what: str, out, like: torch.Tensor) -> torch.Tensor:
-    """The output rows: new, or the caller's if the kernels can write them."""
+def _rows_out(what: str, out, like: torch.Tensor):
+    """(output rows: new, or the caller's if the kernels can write them; strides;
+    address)."""
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        out = torch.empty_like(like, memory_format=torch.contiguous_format)
+        return out, out.stride(), out.data_ptr()
     t, h, d = like.shape
     if out.shape != like.shape or out.dtype != like.dtype:
         raise ValueError(f"{what}: out must be bf16 {tuple(like.shape)}")
-    s0, s1, s2 = out.stride()
-    if s2 != 1 or (s0 | s1) % 8 or out.data_ptr() % 16 or (h > 1 and s1 < d) or (t > 1 and s0 < (h - 1) * s1 + d):
+    s, p = out.stride(), out.data_ptr()
+    if s[2] != 1 or (s[0] | s[1]) & 7 or p & 15 or (h > 1 and s[1] < d) or (t > 1 and s[0] < (h - 1) * s[1] + d):
         raise ValueError(f"{what}: out needs 16-byte aligned rows that do not overlap")
-    return out
+    return out, s, p
 
 
 def paged_append(q, k, v, cos, sin, kv: PagedKV, table, lens, cu=None, *, out=None) -> torch.Tensor:
@@ -1287,27 +1291,30 @@ def paged_append(q, k, v, cos, sin, kv: PagedKV, table, lens, cu=None, *, out=No
     largest value, its older codes are then encoded again
     (moc_paged_append_bf16).  Tokens without a place are not stored; rows behind
     cu[-1] are left alone.  out: where the rotated q goes (may be q)."""
-    N.require_device(q, k, v, cos, sin, *kv, table, lens, cu, out)
-    if q.get_device() != torch.cuda.current_device():
-        with torch.cuda.device(q.device):
+    dev = N.one_device(q, k, v, cos, sin, *kv, table, lens, cu, out)
+    if not N.is_current(dev):
+        with torch.cuda.device(dev):
             return paged_append(q, k, v, cos, sin, kv, table, lens, cu, out=out)
-    if q.dim() != 3 or k.dim() != 3 or q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+    shape, kshape, bf16 = q.shape, k.shape, torch.bfloat16
+    if len(shape) != 3 or len(kshape) != 3 or q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16:
         raise ValueError("paged_append: q, k and v are bf16 [tokens, heads, dim]")
-    tokens, heads, dim = q.shape
-    code, (pages, kv_heads, page, kv_dim), seqs = _paged_operands("paged_append", kv, table, lens, cu, tokens)
-    if kv_dim != dim or k.shape != (tokens, kv_heads, dim) or v.shape != k.shape:
+    tokens, heads, dim = shape
+    code, (pages, kv_heads, page, kv_dim), seqs, width = _paged_operands("paged_append", kv, table, lens, cu, tokens)
+    if kv_dim != dim or kshape != (tokens, kv_heads, dim) or v.shape != kshape:
         raise ValueError(f"paged_append: k and v must be {(tokens, kv_heads, kv_dim)}, q {(tokens, heads, kv_dim)}")
-    if cos.dim() != 2 or cos.shape[1] != dim // 2 or sin.shape != cos.shape or sin.dtype != cos.dtype or not (
+    angles = cos.shape
+    if len(angles) != 2 or angles[1] != dim // 2 or sin.shape != angles or sin.dtype != cos.dtype or not (
             cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError("paged_append: cos and sin are contiguous [angles, dim / 2] of one dtype")
     table_dtype = N.dtype_code(cos.dtype)
-    q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
-    out = _rows_out("paged_append", out, q)
-    (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), out.stride()
-    N.call("moc_paged_append_bf16", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, tokens, heads,
-           kv_heads, dim, cos.data_ptr(), sin.data_ptr(), table_dtype, cos.shape[0], code, kv.k.data_ptr(),
-           kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), pages, page, table.data_ptr(),
-           table.stride(0), table.shape[1], lens.data_ptr(), N.ptr(cu), seqs, out.data_ptr(), o0, o1, N.stream_of(q))
+    q, (q0, q1, _), qp = _head_rows(q)
+    k, (k0, k1, _), kp = _head_rows(k)
+    v, (v0, v1, _), vp = _head_rows(v)
+    out, (o0, o1, _), op = _rows_out("paged_append", out, q)
+    N.call("moc_paged_append_bf16", qp, q0, q1, kp, k0, k1, vp, v0, v1, tokens, heads, kv_heads, dim, cos.data_ptr(),
+           sin.data_ptr(), table_dtype, angles[0], code, kv[0].data_ptr(), kv[1].data_ptr(), kv[2].data_ptr(),
+           kv[3].data_ptr(), pages, page, table.data_ptr(), table.stride(0), width, lens.data_ptr(), N.ptr(cu), seqs,
+           op, o0, o1, N.stream_on(dev))
     return out
 
 
@@ -1320,27 +1327,25 @@ def paged_attention(q, kv: PagedKV, table, lens, cu=None, *, scale: float | None
     that sees a position without a page NaN; rows behind cu[-1] are left alone.
     The table's width bounds the work that is split over the length: pass the
     columns in use."""
-    N.require_device(q, *kv, table, lens, cu, out)
-    if q.get_device() != torch.cuda.current_device():
-        with torch.cuda.device(q.device):
+    dev = N.one_device(q, *kv, table, lens, cu, out)
+    if not N.is_current(dev):
+        with torch.cuda.device(dev):
             return paged_attention(q, kv, table, lens, cu, scale=scale, out=out)
-    if q.dim() != 3 or q.dtype != torch.bfloat16:
+    shape = q.shape
+    if len(shape) != 3 or q.dtype != torch.bfloat16:
         raise ValueError("paged_attention: q is bf16 [tokens, heads, dim]")
-    tokens, heads, dim = q.shape
-    code, (pages, kv_heads, page, kv_dim), seqs = _paged_operands("paged_attention", kv, table, lens, cu, tokens)
+    tokens, heads, dim = shape
+    code, (pages, kv_heads, page, kv_dim), seqs, width = _paged_operands("paged_attention", kv, table, lens, cu, tokens)
     if kv_dim != dim or heads < 1 or heads % kv_heads:
         raise ValueError(f"paged_attention: q of {heads} heads of {dim} over a cache of {kv_heads} of {kv_dim}")
-    q = _head_rows(q)
-    out = _rows_out("paged_attention", out, q)
-    width = table.shape[1]
-    nbytes = N.query("moc_paged_attention_workspace_size", tokens, seqs, int(cu is not None), heads, kv_heads, dim,
-                     page, width)
+    q, (q0, q1, _), qp = _head_rows(q)
+    out, (o0, o1, _), op = _rows_out("paged_attention", out, q)
+    nbytes = N.query("moc_paged_attention_workspace_size", tokens, seqs, cu is not None, heads, kv_heads, dim, page, width)
     ws = _empty((nbytes,), torch.uint8, q.device) if nbytes else None
-    (q0, q1, _), (o0, o1, _) = q.stride(), out.stride()
-    N.call("moc_paged_attention_bf16", q.data_ptr(), q0, q1, tokens, heads, kv_heads, dim, code, kv.k.data_ptr(),
-           kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), pages, page, table.data_ptr(),
-           table.stride(0), width, lens.data_ptr(), N.ptr(cu), seqs,
-           float(dim ** -0.5 if scale is None else scale), out.data_ptr(), o0, o1, N.ptr(ws), nbytes, N.stream_of(q))
+    N.call("moc_paged_attention_bf16", qp, q0, q1, tokens, heads, kv_heads, dim, code, kv[0].data_ptr(),
+           kv[1].data_ptr(), kv[2].data_ptr(), kv[3].data_ptr(), pages, page, table.data_ptr(), table.stride(0), width,
+           lens.data_ptr(), N.ptr(cu), seqs, dim ** -0.5 if scale is None else float(scale), op, o0, o1, N.ptr(ws), nbytes,
+           N.stream_on(dev))
     return out
 
 
@@ -1364,19 +1369,20 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> 
     of exact arithmetic.  NaN logits are never drawn; a row with nothing to draw
     gives -1 (moc_sample_tokens)."""
     settings = (temperature, top_k, top_p, min_p)
-    N.require_device(logits, u, *(t for t in settings if isinstance(t, torch.Tensor)))
-    if logits.get_device() != torch.cuda.current_device():
-        with torch.cuda.device(logits.device):
+    dev = N.one_device(logits, u, *[t for t in settings if isinstance(t, torch.Tensor)])
+    if not N.is_current(dev):
+        with torch.cuda.device(dev):
             return sample_tokens(logits, u, *settings)
     x, ld = _rows_view(logits)
     rows, vocab = x.shape
-    if u.dtype != torch.float32 or u.shape != (rows,) or not u.is_contiguous():
-        raise ValueError(f"sample_tokens: u is a contiguous f32 tensor [{rows}]")
     f32 = torch.float32
-    temperature, top_p, min_p = (_per_row(n, t, rows, f32) for n, t in (
-        ("temperature", temperature), ("top_p", top_p), ("min_p", min_p)))
-    top_k = _per_row("top_k", top_k, rows, torch.int32)
-    out = _empty((rows,), torch.int64, x.device)
-    N.call("moc_sample_tokens", N.dtype_code(x.dtype), x.data_ptr(), rows, vocab, ld, u.data_ptr(), *temperature,
-           top_k[0], max(min(int(top_k[1]), vocab), 0), *top_p, *min_p, out.data_ptr(), N.stream_of(x))
+    if u.dtype != f32 or u.shape != (rows,) or not u.is_contiguous():
+        raise ValueError(f"sample_tokens: u is a contiguous f32 tensor [{rows}]")
+    tp, t1 = _per_row("temperature", temperature, rows, f32)
+    kp, k1 = _per_row("top_k", top_k, rows, torch.int32)
+    pp, p1 = _per_row("top_p", top_p, rows, f32)
+    mp, m1 = _per_row("min_p", min_p, rows, f32)
+    out = torch.empty_like(u, dtype=torch.int64)
+    N.call("moc_sample_tokens", N.dtype_code(x.dtype), x.data_ptr(), rows, vocab, ld, u.data_ptr(), tp, t1, kp,
+           max(min(int(k1), vocab), 0), pp, p1, mp, m1, out.data_ptr(), N.stream_on(dev))
     return out

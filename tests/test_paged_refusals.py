@@ -16,9 +16,9 @@ def calls(monkeypatch):
     """CPU tensors taken for device tensors; the calls that reach the library."""
     seen = []
     monkeypatch.setattr(N, "require_device", lambda *t: None)
-    monkeypatch.setattr(N, "stream_of", lambda t: 0)
+    monkeypatch.setattr(N, "stream_on", lambda d: 0)
+    monkeypatch.setattr(N, "is_current", lambda d: True)
     monkeypatch.setattr(N, "call", lambda name, *a: seen.append((name, a)))
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
     return seen
 
 
