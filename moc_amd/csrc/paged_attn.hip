@@ -28,6 +28,8 @@ namespace {
 constexpr int kPaWaves = 4;
 constexpr int kPaThreads = 64 * kPaWaves;
 constexpr int kPaTile = 64;  // positions per wave and step
+constexpr int kPaMaxSplits = 1024;
+constexpr int kPaFew = 16;   // rows of a sequence and key head up to which paged_attn_kernel takes it
 
 struct PagedAttnArgs {
   PagedSeqs s;
@@ -40,8 +42,8 @@ struct PagedAttnArgs {
   int pages, log_page, heads, kv_heads, group;
   float c2;      // scale log2(e)
   int chunk, splits;
-  float* part_o;   // [tokens heads][splits][D]
-  float2* part_ml;  // [tokens heads][splits]: largest score, sum
+  float* part_o;    // [tiles][kv_heads][16 rows][splits][D]
+  float2* part_ml;  // [tiles][kv_heads][16 rows][splits]: largest score, sum
 };
 
 // Two codes (bytes 2 H, 2 H + 1 of w) as bf16.
@@ -60,6 +62,11 @@ template <bool INT8>
 __device__ __forceinline__ bf16x8_t eight_bf16(uint32_t lo, uint32_t hi) {
   return __builtin_bit_cast(bf16x8_t, make_uint4(two_bf16<INT8, false>(lo), two_bf16<INT8, true>(lo),
                                                  two_bf16<INT8, false>(hi), two_bf16<INT8, true>(hi)));
+}
+
+// Any of four e4m3 codes NaN.
+__device__ __forceinline__ bool has_nan_code(uint32_t w) {
+  return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
 }
 
 template <int D, bool INT8>
@@ -82,7 +89,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
     sp.n = 1;
     sp.len = a.s.lens[sp.seq];
   } else {
-    sp = find_unit(a.s, blockIdx.x, [group](int n, int64_t) { return (n * group + 15) / 16; });
+    sp = find_unit(a.s, blockIdx.x, [group](int n, int64_t) { return n * group <= kPaFew ? 1 : 0; });
     if (sp.seq < 0) return;
   }
   const int r = sp.unit * 16 + col, token = r / group, sub = r - token * group;
@@ -175,8 +182,17 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int64_t p = t0 + 16 * g + 4 * h + i;
+          // places that a row does not see may hold anything: 0 times a NaN code is
+          // NaN.  Such a position's V counts as 0, and its score as NaN
+          bool nan = false;
+          if constexpr (!INT8) {
+#pragma unroll
+            for (int w = 0; w < kVWords; ++w) nan |= has_nan_code(vr[g][i][w]);
+            nan = (__ballot(nan) >> (16 * h)) & 0xFFFFu;  // in any lane's dimensions
+          }
+          if (nan) s[g][i] = __uint_as_float(0x7FC00000u);
           if (p >= lim || p >= to) s[g][i] = -INFINITY;
-          if (p >= to) {  // places that hold no token may hold anything, NaN codes too
+          if (nan || p >= to) {
 #pragma unroll
             for (int w = 0; w < kVWords; ++w) vr[g][i][w] = 0;
           }
@@ -281,7 +297,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
           __builtin_bit_cast(uint32_t, __builtin_convertvector((cvt_f32x2_t){out[i] * inv, out[i + 1] * inv}, cvt_bf16x2_t));
     return;
   }
-  const int64_t slot = (token_row * a.heads + head * group + sb) * a.splits + blockIdx.z;
+  const int64_t slot = ((static_cast<int64_t>(blockIdx.x) * a.kv_heads + head) * 16 + row) * a.splits + blockIdx.z;
   if ((tid & 15) == 0) a.part_ml[slot] = make_float2(mm, ll);
   if (mm == -INFINITY) return;  // nothing in this chunk
   float* po = a.part_o + slot * D + d0;
@@ -290,40 +306,359 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
     *reinterpret_cast<float4*>(po + i) = make_float4(out[i], out[i + 1], out[i + 2], out[i + 3]);
 }
 
-// o from the chunks of a row: one wave a row, D / 64 values a lane.
+// o from the chunks of a row: one workgroup a row, 16 bytes of a chunk a thread.
 template <int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int64_t rows) {
-  constexpr int kPer = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const int64_t token = row / a.heads;
-  if (a.s.cu != nullptr && (token < a.s.cu[0] || token >= a.s.cu[a.s.seqs])) return;  // nobody's row
-  const float2* ml = a.part_ml + row * a.splits;
+__global__ __launch_bounds__(kPaThreads) void paged_join_kernel(PagedAttnArgs a) {
+  constexpr int kLanes = D / 4, kSlots = kPaThreads / kLanes;  // chunks at a time
+  __shared__ float weight[kPaMaxSplits];
+  __shared__ float red[2][kPaWaves];
+  __shared__ float4 sums[kSlots][kLanes];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = a.group, row = blockIdx.z;
+  SeqSpan sp;
+  if (a.s.cu == nullptr) {
+    const int tiles = (group + 15) / 16;
+    sp.seq = sp.row0 = blockIdx.x / tiles;
+    sp.unit = blockIdx.x - sp.seq * tiles;
+    sp.n = 1;
+  } else {
+    sp = find_unit(a.s, blockIdx.x, [group](int n, int64_t) { return n * group <= kPaFew ? 1 : 0; });
+    if (sp.seq < 0) return;
+  }
+  const int r = sp.unit * 16 + row, token = r / group, sub = r - token * group;
+  if (token >= sp.n) return;
+  const int64_t slot = ((static_cast<int64_t>(blockIdx.x) * a.kv_heads + blockIdx.y) * 16 + row) * a.splits;
   float m = -INFINITY;
-  for (int i = lane; i < a.splits; i += 64) m = fmaxf(m, ml[i].x);
+  for (int i = tid; i < a.splits; i += kPaThreads) m = fmaxf(m, a.part_ml[slot + i].x);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if (lane == 0) red[0][wave] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPaWaves; ++w) m = fmaxf(m, red[0][w]);
   const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, out[kPer];
+  float l = 0.f;
+  for (int i = tid; i < a.splits; i += kPaThreads) {
+    const float2 t = a.part_ml[slot + i];
+    weight[i] = __builtin_amdgcn_exp2f(t.x - base);
+    l += t.x == -INFINITY ? t.y : t.y * weight[i];  // an empty chunk: 0, or NaN where it lies outside the cache
+  }
+  l = wave_sum(l);
+  if (lane == 0) red[1][wave] = l;
+  __syncthreads();
+  const int c = tid % kLanes, at = tid / kLanes;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = at; i < a.splits; i += kSlots) {
+    const float f = weight[i];
+    if (f == 0.f) continue;  // also: nothing was written there
+    const float4 t = reinterpret_cast<const float4*>(a.part_o + (slot + i) * D)[c];
+    v.x += f * t.x;
+    v.y += f * t.y;
+    v.z += f * t.z;
+    v.w += f * t.w;
+  }
+  sums[at][c] = v;
+  __syncthreads();
+  if (at > 0) return;
+  l = 0.f;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) out[i] = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 t = ml[s];
-    const float f = __builtin_amdgcn_exp2f(t.x - base);
-    l += t.y * f;
-    if (t.x == -INFINITY) {
-      l += t.y;  // 0, or NaN where a chunk lies outside the cache
-      continue;
-    }
-    const float* p = a.part_o + (row * a.splits + s) * D + lane * kPer;
+  for (int w = 0; w < kPaWaves; ++w) l += red[1][w];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) out[i] += p[i] * f;
+  for (int i = 1; i < kSlots; ++i) {
+    const float4 t = sums[i][c];
+    v.x += t.x;
+    v.y += t.y;
+    v.z += t.z;
+    v.w += t.w;
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  uint16_t* o = a.o + token * a.o_ld + (row - token * a.heads) * a.o_lh + lane * kPer;
+  uint16_t* o = a.o + static_cast<int64_t>(sp.row0 + token) * a.o_ld + (blockIdx.y * group + sub) * a.o_lh + 4 * c;
+  const cvt_bf16x2_t lo = __builtin_convertvector((cvt_f32x2_t){v.x * inv, v.y * inv}, cvt_bf16x2_t);
+  const cvt_bf16x2_t hi = __builtin_convertvector((cvt_f32x2_t){v.z * inv, v.w * inv}, cvt_bf16x2_t);
+  *reinterpret_cast<uint2*>(o) = make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+
+// ------------------------------------------------------------- many rows
+// Sequences with more than 16 rows a key head (prompts, chunks of them, groups of
+// several drafted tokens): v_mfma_f32_32x32x16_bf16 in the same orientation, 32
+// rows a wave, the cache's tiles of 64 positions staged in LDS as codes and read
+// by every wave, which makes bf16 of them for itself: half the LDS bytes of a
+// bf16 tile, and 192 conversions and permutations against the tile's 64 MFMAs.
+// Rows of the tile are D + 32 bytes apart, so that the b128 reads of K rows and
+// the reads of V rows four positions apart fall on different banks.
+//
+// KVS of the four waves share 32 rows and take every KVS'th tile (their sums join
+// through LDS): 128 / KVS rows a workgroup.  Bound by VALU work beside the MFMAs:
+// per 64 positions and 32 rows 64 MFMAs of 16 clocks, about 400 VALU instructions
+// and 32 exponentials.
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+template <int D, bool INT8, int KVS>
+__global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kernel(PagedAttnArgs a) {
+  constexpr int kGroups = kPaWaves / KVS;       // of 32 rows
+  constexpr int kRows = 32 * kGroups;
+  constexpr int kPos = kPaTile * KVS;           // positions a step
+  constexpr int kPitch = D + 32;
+  constexpr int kCh = D / 16;                   // 16-byte chunks of a row
+  constexpr int kStage = kPos * kCh / kPaThreads;  // chunks of K per thread, and of V
+  constexpr int kQ = D / 32, kV = D / 32;       // chunks of K per lane; dimensions of V per lane
+  __shared__ __attribute__((aligned(16))) uint8_t tile[2][kPos * kPitch];
+  __shared__ float scale[2][kPos / 16];
+  __shared__ uint32_t nan_at[kPos / 32];  // positions whose V holds a NaN code
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int col = lane & 31, h = lane >> 5, part = wave / kGroups;
+  const int head = blockIdx.x % a.kv_heads, lp = a.log_page, page = 1 << lp, group = a.group;
+  const SeqSpan sp = find_unit(a.s, blockIdx.x / a.kv_heads, [group](int n, int64_t) {
+    return n * group > kPaFew ? (n * group + kRows - 1) / kRows : 0;
+  });
+  if (sp.seq < 0) return;
+  // the last rows, which see most, first
+  const int unit = (sp.n * group + kRows - 1) / kRows - 1 - sp.unit;
+  const int r0 = unit * kRows + (wave % kGroups) * 32, r = r0 + col, token = r / group, sub = r - token * group;
+  const bool live = token < sp.n;
+  const int64_t room = static_cast<int64_t>(a.s.width) << lp, before = sp.len - sp.n;
+  const int64_t lim = live ? before + 1 + token : 0;
+  const bool lost = lim > room;
+  auto seen = [&](int row) { return min(max(before + 1 + min(row, sp.n * group - 1) / group, int64_t(0)), room); };
+  const int64_t most = seen(unit * kRows + kRows - 1);     // by any row of the workgroup
+  const int64_t mine = r0 < sp.n * group ? seen(r0 + 31) : 0;  // of the wave
+  const int64_t whole = r0 < sp.n * group ? seen(r0) : 0;      // by each row of the wave
+
+  bf16x8_t qf[kQ][2];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) o[i] = bf16_rne(out[i] * inv);
+  for (int i = 0; i < kQ; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint4 t = make_uint4(0, 0, 0, 0);
+      if (live)
+        t = *reinterpret_cast<const uint4*>(a.q + (sp.row0 + token) * a.q_ld + (head * group + sub) * a.q_lh +
+                                            (2 * i + h) * 16 + j * 8);
+      qf[i][j] = __builtin_bit_cast(bf16x8_t, t);
+    }
+  float m = -INFINITY, l = 0.f;
+  f32x16_t acc[kV];
+#pragma unroll
+  for (int j = 0; j < kV; ++j) acc[j] = f32x16_t{};
+  const int32_t* table = a.s.table + sp.seq * a.s.ld_table;
+
+  // staging: chunk c of rows row0 + i kPaThreads / kCh; thread t < kPos / 16 the
+  // scales of positions 16 t ..
+  const int row0 = tid / kCh, ch = tid % kCh;
+  constexpr int kStep = kPaThreads / kCh;
+  int id[kStage], id_s = 0;
+  uint4 kr[kStage], vr[kStage];
+  float ks = 0.f, vs = 0.f;
+  auto load_ids = [&](int64_t t0) {
+#pragma unroll
+    for (int i = 0; i < kStage; ++i) {
+      const int64_t p = t0 + row0 + i * kStep;
+      id[i] = p < most ? table[p >> lp] : 0;
+    }
+    const int64_t p = t0 + 16 * tid;
+    if (tid < kPos / 16) id_s = p < most ? table[p >> lp] : 0;
+  };
+  auto load_tile = [&](int64_t t0) {
+#pragma unroll
+    for (int i = 0; i < kStage; ++i) {
+      const int64_t p = t0 + row0 + i * kStep;
+      const int64_t block = static_cast<int64_t>(id[i] >= 0 && id[i] < a.pages ? id[i] : 0) * a.kv_heads + head;
+      const int64_t byte = ((block << lp) + (p & (page - 1))) * D + 16 * ch;
+      kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+      if (p < most) {
+        kr[i] = *reinterpret_cast<const uint4*>(a.kc + byte);
+        vr[i] = *reinterpret_cast<const uint4*>(a.vc + byte);
+      }
+    }
+    if (tid < kPos / 16) {
+      const bool ok = id_s >= 0 && id_s < a.pages;
+      const int64_t block = static_cast<int64_t>(ok ? id_s : 0) * a.kv_heads + head;
+      // a page out of range makes its scores NaN
+      ks = ok ? a.ks[block] * a.c2 : __uint_as_float(0x7FC00000u);
+      vs = ok ? a.vs[block] : 0.f;
+      if (t0 + 16 * tid >= most) ks = vs = 0.f;
+    }
+  };
+
+  if (most > 0) {
+    load_ids(0);
+    load_tile(0);
+    load_ids(kPos);
+  }
+  for (int64_t t0 = 0; t0 < most; t0 += kPos) {
+    const bool edge_step = !INT8 && t0 + kPos > seen(unit * kRows);  // some row does not see all of it
+    __syncthreads();
+    if (tid < kPos / 32) nan_at[tid] = 0;
+    if (tid < kPos / 16) {
+      scale[0][tid] = ks;
+      scale[1][tid] = vs;
+    }
+    if (edge_step) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kStage; ++i) {
+      const int row = row0 + i * kStep;
+      if (edge_step) {
+        // 0 times a NaN code would reach rows that do not see it
+        uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+        if (has_nan_code(w[0]) || has_nan_code(w[1]) || has_nan_code(w[2]) || has_nan_code(w[3])) {
+          atomicOr(&nan_at[row >> 5], 1u << (row & 31));
+          vr[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      *reinterpret_cast<uint4*>(&tile[0][row * kPitch + 16 * ch]) = kr[i];
+      *reinterpret_cast<uint4*>(&tile[1][row * kPitch + 16 * ch]) = vr[i];
+    }
+    __syncthreads();
+    if (t0 + kPos < most) {
+      load_tile(t0 + kPos);
+      load_ids(t0 + 2 * kPos);
+    }
+    const int64_t t1 = t0 + part * kPaTile;
+    if (t1 >= mine) continue;
+    const uint8_t* kt = tile[0] + part * kPaTile * kPitch;
+    const uint8_t* vt = tile[1] + part * kPaTile * kPitch;
+    f32x16_t s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = f32x16_t{};
+#pragma unroll
+      for (int i = 0; i < kQ; ++i) {
+        const uint4 t = *reinterpret_cast<const uint4*>(kt + (32 * b + col) * kPitch + (2 * i + h) * 16);
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_bf16<INT8>(t.x, t.y), qf[i][0], s[b], 0, 0, 0);
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_bf16<INT8>(t.z, t.w), qf[i][1], s[b], 0, 0, 0);
+      }
+    }
+    float ksc[4], vsc[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      ksc[g] = scale[0][4 * part + g];
+      vsc[g] = scale[1][4 * part + g];
+    }
+    float mt = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] *= ksc[2 * b + (i >> 3)];
+    if (t1 + kPaTile > whole) {
+      uint32_t nans[2] = {edge_step ? nan_at[2 * part] : 0u, edge_step ? nan_at[2 * part + 1] : 0u};
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (!(fabsf(vsc[g]) <= 3.4028234e38f)) {
+          nans[g >> 1] |= 0xFFFFu << (16 * (g & 1));
+          vsc[g] = 0.f;
+        }
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int at = 8 * (i >> 2) + 4 * h + (i & 3);
+          if ((nans[b] >> at) & 1) s[b][i] = __uint_as_float(0x7FC00000u);
+          if (t1 + 32 * b + at >= lim) s[b][i] = -INFINITY;
+        }
+    } else if (edge_step) {
+      const uint32_t nans[2] = {nan_at[2 * part], nan_at[2 * part + 1]};
+      if (nans[0] | nans[1]) l = __uint_as_float(0x7FC00000u);  // every row of the wave sees it
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[b][i]);
+    mt = fmaxf(mt, __shfl_xor(mt, 32));
+    const float mn = fmaxf(m, mt);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    if (__any(mn > m)) {
+      const float f = __builtin_amdgcn_exp2f(m - base);
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < kV; ++j) acc[j] *= f;
+      m = mn;
+    }
+    uint32_t pb[2][8];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float p[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(s[b][2 * i + e] - base);
+          l += p[e];
+          p[e] *= vsc[2 * b + (i >> 2)];
+        }
+        pb[b][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((cvt_f32x2_t){p[0], p[1]}, cvt_bf16x2_t));
+      }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const bf16x8_t pf = __builtin_bit_cast(
+          bf16x8_t, make_uint4(pb[g >> 1][4 * (g & 1)], pb[g >> 1][4 * (g & 1) + 1], pb[g >> 1][4 * (g & 1) + 2],
+                               pb[g >> 1][4 * (g & 1) + 3]));
+      // positions 16 g + 4 h + {0 .. 3, 8 .. 11}, kV neighbouring dimensions
+      constexpr int kW = kV >= 4 ? kV / 4 : 1;
+      uint32_t v[8][kW];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint8_t* src = vt + (16 * g + 4 * h + (i & 3) + 8 * (i >> 2)) * kPitch + col * kV;
+        if constexpr (kV == 2) {
+          v[i][0] = *reinterpret_cast<const uint16_t*>(src);
+        } else if constexpr (kV == 4) {
+          v[i][0] = *reinterpret_cast<const uint32_t*>(src);
+        } else {
+          const uint2 t = *reinterpret_cast<const uint2*>(src);
+          v[i][0] = t.x;
+          v[i][1] = t.y;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < kW; ++w)
+#pragma unroll
+        for (int jj = 0; jj < (kV == 2 ? 1 : 2); ++jj) {
+          uint32_t x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = jj ? two_bf16<INT8, true>(v[i][w]) : two_bf16<INT8, false>(v[i][w]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+            const bf16x8_t vf = __builtin_bit_cast(
+                bf16x8_t, make_uint4(__builtin_amdgcn_perm(x[1], x[0], sel), __builtin_amdgcn_perm(x[3], x[2], sel),
+                                     __builtin_amdgcn_perm(x[5], x[4], sel), __builtin_amdgcn_perm(x[7], x[6], sel)));
+            const int j = 4 * w + 2 * jj + e;
+            acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, acc[j], 0, 0, 0);
+          }
+        }
+    }
+  }
+  l += __shfl_xor(l, 32);
+  if (lost) l = __uint_as_float(0x7FC00000u);
+  if constexpr (KVS == 2) {
+    // the second half of the waves hands its sums to the first
+    float* po = reinterpret_cast<float*>(tile) + (wave % kGroups) * 32 * D;
+    __shared__ float2 ml[kGroups][32];
+    __syncthreads();
+    if (part == 1) {
+      if (h == 0) ml[wave % kGroups][col] = make_float2(m, l);
+#pragma unroll
+      for (int j = 0; j < kV; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) po[(j * 16 + i) * 64 + lane] = acc[j][i];
+    }
+    __syncthreads();
+    if (part == 1) return;
+    const float2 o = ml[wave % kGroups][col];
+    const float mn = fmaxf(m, o.x), base = mn == -INFINITY ? 0.f : mn;
+    const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(o.x - base);
+    l = l * f0 + o.y * f1;
+#pragma unroll
+    for (int j = 0; j < kV; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[j][i] = acc[j][i] * f0 + po[(j * 16 + i) * 64 + lane] * f1;
+  }
+  if (!live) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  uint16_t* o = a.o + (sp.row0 + token) * a.o_ld + (head * group + sub) * a.o_lh;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int j = 0; j < kV; j += 2)
+      *reinterpret_cast<uint32_t*>(o + (8 * (i >> 2) + 4 * h + (i & 3)) * kV + j) = __builtin_bit_cast(
+          uint32_t, __builtin_convertvector((cvt_f32x2_t){acc[j][i] * inv, acc[j + 1][i] * inv}, cvt_bf16x2_t));
 }
 
 }  // namespace
@@ -332,15 +667,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int64_
 using namespace moc;
 
 namespace {
-// Chunks of the positions: enough workgroups for the CUs, whole tiles a wave.
+// paged_attn_kernel's chunks of the positions: enough workgroups for the CUs,
+// whole steps.
 struct Plan {
   int64_t tiles, chunk, splits;
 };
 Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t kv_heads, int64_t room) {
   Plan p;
-  p.tiles = ragged ? tokens * group / 16 + std::min(seqs, tokens) : seqs * ((group + 15) / 16);
+  p.tiles = ragged ? (group <= kPaFew ? std::min(seqs, tokens) : 0) : seqs * ((group + 15) / 16);
   const int64_t step = kPaTile * kPaWaves;
-  const int64_t want = std::max<int64_t>(1, 4LL * cu_count() / std::max<int64_t>(1, p.tiles * kv_heads));
+  const int64_t want =
+      std::min<int64_t>(kPaMaxSplits, std::max<int64_t>(1, 4LL * cu_count() / std::max<int64_t>(1, p.tiles * kv_heads)));
   const int64_t steps = std::max<int64_t>(1, (room + step - 1) / step);
   const int64_t per = std::max<int64_t>(1, (steps + want - 1) / want);
   p.chunk = per * step;
@@ -353,7 +690,7 @@ extern "C" int64_t moc_paged_attention_workspace_size(int64_t tokens, int64_t se
                                                       int64_t kv_heads, int64_t head_dim, int64_t page, int64_t width) {
   if (tokens <= 0 || seqs <= 0 || kv_heads <= 0 || q_heads <= 0) return 0;
   const Plan p = plan_of(tokens, seqs, ragged != 0, q_heads / kv_heads, kv_heads, page * width);
-  return p.splits > 1 ? tokens * q_heads * p.splits * (head_dim * 4 + 8) : 0;
+  return p.splits > 1 ? p.tiles * kv_heads * 16 * p.splits * (head_dim * 4 + 8) : 0;
 }
 
 extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_lh, int64_t tokens, int64_t q_heads,
@@ -404,24 +741,49 @@ extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_l
   a.chunk = static_cast<int>(std::min<int64_t>(p.chunk, 1 << 30));
   a.splits = static_cast<int>(p.splits);
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + tokens * q_heads * p.splits * head_dim);
-  const dim3 grid(static_cast<unsigned>(p.tiles), static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.splits));
+  a.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + p.tiles * kv_heads * 16 * p.splits * head_dim);
   hipStream_t st = as_stream(stream);
-#define MOC_PA(D)                                                                \
-  do {                                                                           \
+  int rc = MOC_OK;
+  if (cu != nullptr && tokens * group > kPaFew) {
+    // 64 rows a workgroup where 128 would leave CUs without one
+    const bool half = tokens * group / 128 * kv_heads < 2 * cu_count();
+    const int64_t units = tokens * group / (half ? 64 : 128) + std::min(seqs, tokens);
+    MOC_REQUIRE(units * kv_heads < (1LL << 31), "moc_paged_attention_bf16: too many rows for one call");
+    const dim3 grid(static_cast<unsigned>(units * kv_heads));
+#define MOC_PW(D)                                                                                  \
+  do {                                                                                             \
+    if (code == MOC_I8) {                                                                          \
+      if (half) paged_wide_kernel<D, true, 2><<<grid, kPaThreads, 0, st>>>(a);                     \
+      else paged_wide_kernel<D, true, 1><<<grid, kPaThreads, 0, st>>>(a);                          \
+    } else {                                                                                       \
+      if (half) paged_wide_kernel<D, false, 2><<<grid, kPaThreads, 0, st>>>(a);                    \
+      else paged_wide_kernel<D, false, 1><<<grid, kPaThreads, 0, st>>>(a);                         \
+    }                                                                                              \
+  } while (0)
+    if (head_dim == 64) MOC_PW(64);
+    else if (head_dim == 128) MOC_PW(128);
+    else MOC_PW(256);
+#undef MOC_PW
+    rc = check_launch("paged_wide_kernel");
+    if (rc != MOC_OK) return rc;
+  }
+  if (p.tiles == 0) return rc;
+  const dim3 grid(static_cast<unsigned>(p.tiles), static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.splits));
+#define MOC_PA(D)                                                                  \
+  do {                                                                             \
     if (code == MOC_I8) paged_attn_kernel<D, true><<<grid, kPaThreads, 0, st>>>(a); \
-    else paged_attn_kernel<D, false><<<grid, kPaThreads, 0, st>>>(a);            \
+    else paged_attn_kernel<D, false><<<grid, kPaThreads, 0, st>>>(a);              \
   } while (0)
   if (head_dim == 64) MOC_PA(64);
   else if (head_dim == 128) MOC_PA(128);
   else MOC_PA(256);
 #undef MOC_PA
-  int rc = check_launch("paged_attn_kernel");
+  rc = check_launch("paged_attn_kernel");
   if (rc != MOC_OK || p.splits == 1) return rc;
-  const int64_t rows = tokens * q_heads;
-  const dim3 jg(static_cast<unsigned>((rows + 3) / 4));
-  if (head_dim == 64) paged_join_kernel<64><<<jg, 256, 0, st>>>(a, rows);
-  else if (head_dim == 128) paged_join_kernel<128><<<jg, 256, 0, st>>>(a, rows);
-  else paged_join_kernel<256><<<jg, 256, 0, st>>>(a, rows);
+  const dim3 jg(static_cast<unsigned>(p.tiles), static_cast<unsigned>(kv_heads),
+                static_cast<unsigned>(cu != nullptr ? 16 : std::min<int64_t>(group, 16)));
+  if (head_dim == 64) paged_join_kernel<64><<<jg, kPaThreads, 0, st>>>(a);
+  else if (head_dim == 128) paged_join_kernel<128><<<jg, kPaThreads, 0, st>>>(a);
+  else paged_join_kernel<256><<<jg, kPaThreads, 0, st>>>(a);
   return check_launch("paged_join_kernel");
 }

@@ -58,9 +58,9 @@ def half_step(y, kind):
     return 2.0 ** (e - 4)
 
 
-def attention(q, kv, table, lens, cu, scale):
+def attention(q, kv, table, lens, cu, scale, rows=None):
     """(o, the same sums over |v|) in 64 bits; NaN for rows that see a position
-    without a page."""
+    without a page.  rows: only these."""
     q, table = q.cpu().double(), table.cpu()
     codes_k, codes_v = values(kv.k), values(kv.v)
     ks, vs = kv.k_scale.cpu().double(), kv.v_scale.cpu().double()
@@ -71,7 +71,7 @@ def attention(q, kv, table, lens, cu, scale):
     for b, start, n, length in spans(tokens, lens.cpu(), None if cu is None else cu.cpu()):
         for i in range(n):
             sees = length - n + i + 1
-            if sees <= 0:
+            if sees <= 0 or (rows is not None and start + i not in rows):
                 continue
             ids = [int(table[b, p // page]) if p < room else -1 for p in range(0, sees, page)]
             if any(not 0 <= j < pages for j in ids):

@@ -104,6 +104,50 @@ def test_attention_split_over_the_length(seqs, length):
     _attend([1] * seqs, before, 4, 2, 128, 64, E4)
 
 
+@pytest.mark.parametrize("kind", [E4, I8])
+@pytest.mark.parametrize("new,before,q_heads,kv_heads,dim,page", [
+    ([700, 3, 900, 500, 1], [0, 40, 130, 7, 2000], 32, 16, 64, 32), ([1100, 0, 900], [0, 0, 513], 20, 10, 128, 64),
+    ([400, 1, 1300], [65, 3, 0], 40, 8, 256, 16), ([33, 65, 300], [0, 5, 64], 3, 3, 128, 256)])
+def test_attention_prompts(kind, new, before, q_heads, kv_heads, dim, page):
+    """Row tiles of both sizes; the ends of each sequence and rows between."""
+    table, lens, cu, pool = _batch(new, before, page, seed=2)
+    kv = _cache(pool, kv_heads, page, dim, kind, 2)
+    q = (1.5 * torch.randn(sum(new), q_heads, dim, generator=_gen(3))).to(BF).cuda()
+    o = K.paged_attention(q, kv, table, lens, cu)
+    ends = [e for s, n in zip(cu.tolist(), new) for e in (s, s + n // 3, s + n // 2 + 1, s + n - 2, s + n - 1) if n > 2]
+    rows = sorted({r for r in ends + list(range(0, sum(new), 131)) if 0 <= r < sum(new)})
+    ref, size = R.attention(q, kv, table, lens, cu, dim ** -0.5, set(rows))
+    _close(o[rows], ref[rows], size[rows])
+
+
+@pytest.mark.parametrize("n", [4, 12, 60, 200])
+def test_attention_codes_that_later_rows_see(n):
+    """NaN codes and scales, a page out of range: the rows before them are as
+    without them, the rows from them on are NaN."""
+    table, lens, cu, pool = _batch([n, 2], [50, 9], 16)
+    kv = _cache(pool, 2, 16, 64, E4)
+    q = torch.randn(n + 2, 4, 64, generator=_gen(5)).to(BF).cuda()
+    clean = K.paged_attention(q, kv, table, lens, cu)
+    for at in (0, 1, n // 2, n - 1):
+        pos = 50 + at
+        for part in ("k", "v"):
+            bad = _clone(kv)
+            _bits(getattr(bad, part))[table[0, pos // 16].long(), :, pos % 16, 5] = 0x7F
+            o = K.paged_attention(q, bad, table, lens, cu)
+            assert torch.equal(o[:at], clean[:at]) and torch.equal(o[n:], clean[n:])
+            assert torch.isnan(o[at:n]).flatten(1).any(1).all()
+        first = max(0, pos // 16 * 16 - 50)  # the first row that sees the page
+        for part in ("k_scale", "v_scale"):
+            bad = _clone(kv)
+            getattr(bad, part)[table[0, pos // 16].long()] = math.nan
+            o = K.paged_attention(q, bad, table, lens, cu)
+            assert torch.equal(o[:first], clean[:first]) and torch.isnan(o[first:n]).all() and torch.equal(o[n:], clean[n:])
+        wrong = table.clone()
+        wrong[0, pos // 16] = pool + 3
+        o = K.paged_attention(q, kv, wrong, lens, cu)
+        assert torch.equal(o[:first], clean[:first]) and torch.isnan(o[first:n]).all() and torch.equal(o[n:], clean[n:])
+
+
 def test_attention_many_ragged_sequences():
     """More sequences than a wave has lanes, some empty."""
     new = [(i * 7) % 4 for i in range(150)]
