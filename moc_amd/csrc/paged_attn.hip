@@ -398,8 +398,7 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
   constexpr int kRows = 32 * kGroups;
   constexpr int kPos = kPaTile * KVS;           // positions a step
   constexpr int kPitch = D + 32;
-  constexpr int kCh = D / 16;                   // 16-byte chunks of a row
-  constexpr int kStage = kPos * kCh / kPaThreads;  // chunks of K per thread, and of V
+  constexpr int kLd = D / 64;                   // 16-byte loads per lane of 16 positions
   constexpr int kQ = D / 32, kV = D / 32;       // chunks of K per lane; dimensions of V per lane
   __shared__ __attribute__((aligned(16))) uint8_t tile[2][kPos * kPitch];
   __shared__ float scale[2][kPos / 16];
@@ -434,47 +433,49 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
                                             (2 * i + h) * 16 + j * 8);
       qf[i][j] = __builtin_bit_cast(bf16x8_t, t);
     }
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, v_unit = 0.f;
   f32x16_t acc[kV];
 #pragma unroll
   for (int j = 0; j < kV; ++j) acc[j] = f32x16_t{};
   const int32_t* table = a.s.table + sp.seq * a.s.ld_table;
 
-  // staging: chunk c of rows row0 + i kPaThreads / kCh; thread t < kPos / 16 the
-  // scales of positions 16 t ..
-  const int row0 = tid / kCh, ch = tid % kCh;
-  constexpr int kStep = kPaThreads / kCh;
-  int id[kStage], id_s = 0;
-  uint4 kr[kStage], vr[kStage];
-  float ks = 0.f, vs = 0.f;
+  // staging: wave w takes the 16-position groups w, w + 4, ..: 16 D bytes in a row
+  // of the cache, kLd loads of the whole wave
+  int id[KVS];
+  uint4 kr[KVS][kLd], vr[KVS][kLd];
+  float ks[KVS], vs[KVS];
   auto load_ids = [&](int64_t t0) {
 #pragma unroll
-    for (int i = 0; i < kStage; ++i) {
-      const int64_t p = t0 + row0 + i * kStep;
-      id[i] = p < most ? table[p >> lp] : 0;
+    for (int i = 0; i < KVS; ++i) {
+      const int64_t p = t0 + 16 * (wave + kPaWaves * i);
+      id[i] = p < most ? __builtin_amdgcn_readfirstlane(table[p >> lp]) : 0;
     }
-    const int64_t p = t0 + 16 * tid;
-    if (tid < kPos / 16) id_s = p < most ? table[p >> lp] : 0;
   };
   auto load_tile = [&](int64_t t0) {
 #pragma unroll
-    for (int i = 0; i < kStage; ++i) {
-      const int64_t p = t0 + row0 + i * kStep;
-      const int64_t block = static_cast<int64_t>(id[i] >= 0 && id[i] < a.pages ? id[i] : 0) * a.kv_heads + head;
-      const int64_t byte = ((block << lp) + (p & (page - 1))) * D + 16 * ch;
-      kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < KVS; ++i) {
+      const int64_t p = t0 + 16 * (wave + kPaWaves * i);
+      const bool ok = id[i] >= 0 && id[i] < a.pages;
+      const int64_t block = static_cast<int64_t>(ok ? id[i] : 0) * a.kv_heads + head;
+      const int64_t byte = ((block << lp) + (p & (page - 1))) * D;
+#pragma unroll
+      for (int j = 0; j < kLd; ++j) kr[i][j] = vr[i][j] = make_uint4(0, 0, 0, 0);
+      ks[i] = vs[i] = 0.f;
       if (p < most) {
-        kr[i] = *reinterpret_cast<const uint4*>(a.kc + byte);
-        vr[i] = *reinterpret_cast<const uint4*>(a.vc + byte);
+#pragma unroll
+        for (int j = 0; j < kLd; ++j) {
+          kr[i][j] = *reinterpret_cast<const uint4*>(a.kc + byte + 1024 * j + 16 * lane);
+          vr[i][j] = *reinterpret_cast<const uint4*>(a.vc + byte + 1024 * j + 16 * lane);
+        }
+        // a page out of range makes its scores NaN
+        ks[i] = ok ? a.ks[block] * a.c2 : __uint_as_float(0x7FC00000u);
+        vs[i] = ok ? a.vs[block] : 0.f;
+        if (p + 16 > most) {  // behind the last position
+#pragma unroll
+          for (int j = 0; j < kLd; ++j)
+            if (p + (1024 * j + 16 * lane) / D >= most) kr[i][j] = vr[i][j] = make_uint4(0, 0, 0, 0);
+        }
       }
-    }
-    if (tid < kPos / 16) {
-      const bool ok = id_s >= 0 && id_s < a.pages;
-      const int64_t block = static_cast<int64_t>(ok ? id_s : 0) * a.kv_heads + head;
-      // a page out of range makes its scores NaN
-      ks = ok ? a.ks[block] * a.c2 : __uint_as_float(0x7FC00000u);
-      vs = ok ? a.vs[block] : 0.f;
-      if (t0 + 16 * tid >= most) ks = vs = 0.f;
     }
   };
 
@@ -486,25 +487,30 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
   for (int64_t t0 = 0; t0 < most; t0 += kPos) {
     const bool edge_step = !INT8 && t0 + kPos > seen(unit * kRows);  // some row does not see all of it
     __syncthreads();
-    if (tid < kPos / 32) nan_at[tid] = 0;
-    if (tid < kPos / 16) {
-      scale[0][tid] = ks;
-      scale[1][tid] = vs;
+    if (edge_step) {
+      if (tid < kPos / 32) nan_at[tid] = 0;
+      __syncthreads();
     }
-    if (edge_step) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kStage; ++i) {
-      const int row = row0 + i * kStep;
-      if (edge_step) {
-        // 0 times a NaN code would reach rows that do not see it
-        uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-        if (has_nan_code(w[0]) || has_nan_code(w[1]) || has_nan_code(w[2]) || has_nan_code(w[3])) {
-          atomicOr(&nan_at[row >> 5], 1u << (row & 31));
-          vr[i] = make_uint4(0, 0, 0, 0);
-        }
+    for (int i = 0; i < KVS; ++i) {
+      if (lane == 0) {
+        scale[0][wave + kPaWaves * i] = ks[i];
+        scale[1][wave + kPaWaves * i] = vs[i];
       }
-      *reinterpret_cast<uint4*>(&tile[0][row * kPitch + 16 * ch]) = kr[i];
-      *reinterpret_cast<uint4*>(&tile[1][row * kPitch + 16 * ch]) = vr[i];
+#pragma unroll
+      for (int j = 0; j < kLd; ++j) {
+        const int row = 16 * (wave + kPaWaves * i) + (1024 * j + 16 * lane) / D, c = 16 * lane % D;
+        if (edge_step) {
+          // 0 times a NaN code would reach rows that do not see it
+          const uint4 v = vr[i][j];
+          if (has_nan_code(v.x) || has_nan_code(v.y) || has_nan_code(v.z) || has_nan_code(v.w)) {
+            atomicOr(&nan_at[row >> 5], 1u << (row & 31));
+            vr[i][j] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        *reinterpret_cast<uint4*>(&tile[0][row * kPitch + c]) = kr[i][j];
+        *reinterpret_cast<uint4*>(&tile[1][row * kPitch + c]) = vr[i][j];
+      }
     }
     __syncthreads();
     if (t0 + kPos < most) {
@@ -526,41 +532,50 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_bf16<INT8>(t.z, t.w), qf[i][1], s[b], 0, 0, 0);
       }
     }
+    // x[i]: position 32 (i >> 4) + 8 ((i >> 2) & 3) + 4 h + (i & 3), group i >> 3
+    float x[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = s[i >> 4][i & 15];
     float ksc[4], vsc[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       ksc[g] = scale[0][4 * part + g];
       vsc[g] = scale[1][4 * part + g];
     }
-    float mt = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int g = 0; g < 4; ++g)
+      if (!(ksc[g] > 0.f)) {  // the largest score is the largest product only for scales above 0
+        const float sign = ksc[g] < 0.f ? -1.f : 1.f;
+        ksc[g] = ksc[g] == 0.f ? 1e-30f : fabsf(ksc[g]);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[b][i] *= ksc[2 * b + (i >> 3)];
+        for (int i = 0; i < 8; ++i) x[8 * g + i] *= sign;
+      }
     if (t1 + kPaTile > whole) {
       uint32_t nans[2] = {edge_step ? nan_at[2 * part] : 0u, edge_step ? nan_at[2 * part + 1] : 0u};
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        if (!(fabsf(vsc[g]) <= 3.4028234e38f)) {
+        if (!(fabsf(vsc[g]) <= 3.4028234e38f) || !(ksc[g] <= 3.4028234e38f)) {
           nans[g >> 1] |= 0xFFFFu << (16 * (g & 1));
-          vsc[g] = 0.f;
+          ksc[g] = vsc[g] = 1.f;
         }
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int at = 8 * (i >> 2) + 4 * h + (i & 3);
-          if ((nans[b] >> at) & 1) s[b][i] = __uint_as_float(0x7FC00000u);
-          if (t1 + 32 * b + at >= lim) s[b][i] = -INFINITY;
-        }
+      for (int i = 0; i < 32; ++i) {
+        const int at = 8 * ((i >> 2) & 3) + 4 * h + (i & 3);
+        if ((nans[i >> 4] >> at) & 1) x[i] = __uint_as_float(0x7FC00000u);
+        if (t1 + 32 * (i >> 4) + at >= lim) x[i] = -INFINITY;
+      }
     } else if (edge_step) {
       const uint32_t nans[2] = {nan_at[2 * part], nan_at[2 * part + 1]};
       if (nans[0] | nans[1]) l = __uint_as_float(0x7FC00000u);  // every row of the wave sees it
     }
+    float mt = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int g = 0; g < 4; ++g) {
+      float y = x[8 * g];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[b][i]);
+      for (int i = 1; i < 8; ++i) y = fmaxf(y, x[8 * g + i]);
+      mt = fmaxf(mt, y * ksc[g]);
+    }
     mt = fmaxf(mt, __shfl_xor(mt, 32));
     const float mn = fmaxf(m, mt);
     const float base = mn == -INFINITY ? 0.f : mn;
@@ -571,25 +586,32 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
       for (int j = 0; j < kV; ++j) acc[j] *= f;
       m = mn;
     }
-    uint32_t pb[2][8];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int g = 0; g < 4; ++g)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float p[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(s[b][2 * i + e] - base);
-          l += p[e];
-          p[e] *= vsc[2 * b + (i >> 2)];
-        }
-        pb[b][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((cvt_f32x2_t){p[0], p[1]}, cvt_bf16x2_t));
+        x[8 * g + i] = __builtin_amdgcn_exp2f(fmaf(x[8 * g + i], ksc[g], -base));
+        l += x[8 * g + i];
       }
+    // V's scale goes onto the probabilities, relative to the first one: pages of
+    // one size of values share theirs
+    if (v_unit == 0.f) v_unit = vsc[0] > 0.f && vsc[0] <= 3.4028234e38f ? vsc[0] : 1.f;
+    if (vsc[0] != v_unit || vsc[1] != v_unit || vsc[2] != v_unit || vsc[3] != v_unit) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float f = vsc[g] / v_unit;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[8 * g + i] *= f;
+      }
+    }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const bf16x8_t pf = __builtin_bit_cast(
-          bf16x8_t, make_uint4(pb[g >> 1][4 * (g & 1)], pb[g >> 1][4 * (g & 1) + 1], pb[g >> 1][4 * (g & 1) + 2],
-                               pb[g >> 1][4 * (g & 1) + 3]));
+      uint32_t pb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        pb[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(
+                                                 (cvt_f32x2_t){x[8 * g + 2 * i], x[8 * g + 2 * i + 1]}, cvt_bf16x2_t));
+      const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, make_uint4(pb[0], pb[1], pb[2], pb[3]));
       // positions 16 g + 4 h + {0 .. 3, 8 .. 11}, kV neighbouring dimensions
       constexpr int kW = kV >= 4 ? kV / 4 : 1;
       uint32_t v[8][kW];
@@ -610,15 +632,15 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
       for (int w = 0; w < kW; ++w)
 #pragma unroll
         for (int jj = 0; jj < (kV == 2 ? 1 : 2); ++jj) {
-          uint32_t x[8];
+          uint32_t z[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = jj ? two_bf16<INT8, true>(v[i][w]) : two_bf16<INT8, false>(v[i][w]);
+          for (int i = 0; i < 8; ++i) z[i] = jj ? two_bf16<INT8, true>(v[i][w]) : two_bf16<INT8, false>(v[i][w]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t sel = e ? 0x07060302u : 0x05040100u;
             const bf16x8_t vf = __builtin_bit_cast(
-                bf16x8_t, make_uint4(__builtin_amdgcn_perm(x[1], x[0], sel), __builtin_amdgcn_perm(x[3], x[2], sel),
-                                     __builtin_amdgcn_perm(x[5], x[4], sel), __builtin_amdgcn_perm(x[7], x[6], sel)));
+                bf16x8_t, make_uint4(__builtin_amdgcn_perm(z[1], z[0], sel), __builtin_amdgcn_perm(z[3], z[2], sel),
+                                     __builtin_amdgcn_perm(z[5], z[4], sel), __builtin_amdgcn_perm(z[7], z[6], sel)));
             const int j = 4 * w + 2 * jj + e;
             acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, acc[j], 0, 0, 0);
           }
@@ -637,7 +659,7 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
 #pragma unroll
       for (int j = 0; j < kV; ++j)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) po[(j * 16 + i) * 64 + lane] = acc[j][i];
+        for (int i = 0; i < 16; ++i) po[(j * 16 + i) * 64 + lane] = acc[j][i] * v_unit;
     }
     __syncthreads();
     if (part == 1) return;
@@ -648,10 +670,10 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
 #pragma unroll
     for (int j = 0; j < kV; ++j)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[j][i] = acc[j][i] * f0 + po[(j * 16 + i) * 64 + lane] * f1;
+      for (int i = 0; i < 16; ++i) acc[j][i] = acc[j][i] * (f0 * v_unit) + po[(j * 16 + i) * 64 + lane] * f1;
   }
   if (!live) return;
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const float inv = l == 0.f ? 0.f : (KVS == 1 ? v_unit : 1.f) / l;
   uint16_t* o = a.o + (sp.row0 + token) * a.o_ld + (head * group + sub) * a.o_lh;
 #pragma unroll
   for (int i = 0; i < 16; ++i)
