@@ -380,30 +380,46 @@ __global__ __launch_bounds__(kPaThreads) void paged_join_kernel(PagedAttnArgs a)
 // ------------------------------------------------------------- many rows
 // Sequences with more than 16 rows a key head (prompts, chunks of them, groups of
 // several drafted tokens): v_mfma_f32_32x32x16_bf16 in the same orientation, 32
-// rows a wave, the cache's tiles of 64 positions staged in LDS as codes and read
-// by every wave, which makes bf16 of them for itself: half the LDS bytes of a
-// bf16 tile, and 192 conversions and permutations against the tile's 64 MFMAs.
-// Rows of the tile are D + 32 bytes apart, so that the b128 reads of K rows and
-// the reads of V rows four positions apart fall on different banks.
+// rows a wave.  The cache's tiles of 64 positions go to LDS as codes, straight from
+// memory (16 positions of a page are 16 D bytes in a row), one step ahead; every
+// wave makes bf16 of them for itself, which halves the LDS bytes of a bf16 tile.
+// 16-byte chunk c of row r lies in slot c ^ chunk_swz(r): the b128 reads of K, a
+// row a lane, then meet all banks, and V's rows are read whole.
 //
 // KVS of the four waves share 32 rows and take every KVS'th tile (their sums join
 // through LDS): 128 / KVS rows a workgroup.  Bound by VALU work beside the MFMAs:
-// per 64 positions and 32 rows 64 MFMAs of 16 clocks, about 400 VALU instructions
+// per 64 positions and 32 rows 32 MFMAs of 32 clocks, about 330 VALU instructions
 // and 32 exponentials.
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+template <int D>
+__device__ __forceinline__ int chunk_swz(int r) {
+  return D == 64 ? (r >> 2) & 3 : D == 128 ? r & 7 : r & 15;
+}
+
+// 16 bytes per lane from base + off to LDS bytes m0 + 16 lane.  Counted by hand
+// (vmcnt): the compiler knows nothing of it.
+__device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint32_t m0) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2"
+      :
+      : "s"(m0), "v"(off), "s"(base)
+      : "memory");
+}
 
 template <int D, bool INT8, int KVS>
 __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kernel(PagedAttnArgs a) {
   constexpr int kGroups = kPaWaves / KVS;       // of 32 rows
   constexpr int kRows = 32 * kGroups;
   constexpr int kPos = kPaTile * KVS;           // positions a step
-  constexpr int kPitch = D + 32;
   constexpr int kLd = D / 64;                   // 16-byte loads per lane of 16 positions
   constexpr int kQ = D / 32, kV = D / 32;       // chunks of K per lane; dimensions of V per lane
-  __shared__ __attribute__((aligned(16))) uint8_t tile[2][kPos * kPitch];
-  __shared__ float scale[2][kPos / 16];
-  __shared__ uint32_t nan_at[kPos / 32];  // positions whose V holds a NaN code
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __attribute__((aligned(1024))) uint8_t tile[2][2][kPos * D];  // [step & 1][K, V]
+  __shared__ float scale[2][2][kPos / 16];
+  __shared__ uint32_t nan_at[2][kPos / 32];  // positions whose V holds a NaN code
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5, part = wave / kGroups;
   const int head = blockIdx.x % a.kv_heads, lp = a.log_page, page = 1 << lp, group = a.group;
   const SeqSpan sp = find_unit(a.s, blockIdx.x / a.kv_heads, [group](int n, int64_t) {
@@ -439,10 +455,17 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
   for (int j = 0; j < kV; ++j) acc[j] = f32x16_t{};
   const int32_t* table = a.s.table + sp.seq * a.s.ld_table;
 
-  // staging: wave w takes the 16-position groups w, w + 4, ..: 16 D bytes in a row
-  // of the cache, kLd loads of the whole wave
+  // staging: wave w takes the 16-position groups w, w + 4, ..: kLd loads of the
+  // whole wave each, lane l's chunk of row (1024 j + 16 l) / D of the group
+  uint32_t src[kLd];
+#pragma unroll
+  for (int j = 0; j < kLd; ++j) {
+    const int row = (1024 * j + 16 * lane) / D, c = 16 * lane % D / 16;
+    src[j] = row * D + 16 * (c ^ chunk_swz<D>(row));
+  }
+  const uint32_t lds0 = static_cast<uint32_t>(
+      (uintptr_t)((__attribute__((address_space(3))) const char*)(const void*)&tile[0][0][0]));
   int id[KVS];
-  uint4 kr[KVS][kLd], vr[KVS][kLd];
   float ks[KVS], vs[KVS];
   auto load_ids = [&](int64_t t0) {
 #pragma unroll
@@ -451,83 +474,86 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
       id[i] = p < most ? __builtin_amdgcn_readfirstlane(table[p >> lp]) : 0;
     }
   };
-  auto load_tile = [&](int64_t t0) {
+  auto load_tile = [&](int64_t t0, int buf) {
 #pragma unroll
     for (int i = 0; i < KVS; ++i) {
-      const int64_t p = t0 + 16 * (wave + kPaWaves * i);
+      const int at = wave + kPaWaves * i;
+      const int64_t p = t0 + 16 * at;
+      ks[i] = vs[i] = 0.f;
+      if (p >= most) continue;  // what LDS holds there is not seen
       const bool ok = id[i] >= 0 && id[i] < a.pages;
       const int64_t block = static_cast<int64_t>(ok ? id[i] : 0) * a.kv_heads + head;
       const int64_t byte = ((block << lp) + (p & (page - 1))) * D;
+      const uint32_t dst = lds0 + (2 * buf * kPos + 16 * at) * D;
 #pragma unroll
-      for (int j = 0; j < kLd; ++j) kr[i][j] = vr[i][j] = make_uint4(0, 0, 0, 0);
-      ks[i] = vs[i] = 0.f;
-      if (p < most) {
+      for (int j = 0; j < kLd; ++j) to_lds16(a.kc + byte, src[j], dst + 1024 * j);
 #pragma unroll
-        for (int j = 0; j < kLd; ++j) {
-          kr[i][j] = *reinterpret_cast<const uint4*>(a.kc + byte + 1024 * j + 16 * lane);
-          vr[i][j] = *reinterpret_cast<const uint4*>(a.vc + byte + 1024 * j + 16 * lane);
-        }
-        // a page out of range makes its scores NaN
-        ks[i] = ok ? a.ks[block] * a.c2 : __uint_as_float(0x7FC00000u);
-        vs[i] = ok ? a.vs[block] : 0.f;
-        if (p + 16 > most) {  // behind the last position
-#pragma unroll
-          for (int j = 0; j < kLd; ++j)
-            if (p + (1024 * j + 16 * lane) / D >= most) kr[i][j] = vr[i][j] = make_uint4(0, 0, 0, 0);
-        }
-      }
+      for (int j = 0; j < kLd; ++j) to_lds16(a.vc + byte, src[j], dst + kPos * D + 1024 * j);
+      // a page out of range makes its scores NaN
+      ks[i] = ok ? a.ks[block] * a.c2 : __uint_as_float(0x7FC00000u);
+      vs[i] = ok ? a.vs[block] : 0.f;
     }
   };
 
+  // LDS bytes of a tile that this lane reads
+  uint32_t k_at[kQ], v_at[8];
+#pragma unroll
+  for (int i = 0; i < kQ; ++i) k_at[i] = col * D + 16 * ((2 * i + h) ^ chunk_swz<D>(col));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = 4 * h + (i & 3) + 8 * (i >> 2);
+    v_at[i] = row * D + 16 * ((col * kV / 16) ^ chunk_swz<D>(row)) + col * kV % 16;
+  }
+
   if (most > 0) {
     load_ids(0);
-    load_tile(0);
+    load_tile(0, 0);
     load_ids(kPos);
   }
-  for (int64_t t0 = 0; t0 < most; t0 += kPos) {
+  int buf = 0;
+  for (int64_t t0 = 0; t0 < most; t0 += kPos, buf ^= 1) {
     const bool edge_step = !INT8 && t0 + kPos > seen(unit * kRows);  // some row does not see all of it
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < KVS; ++i) {
+        scale[buf][0][wave + kPaWaves * i] = ks[i];
+        scale[buf][1][wave + kPaWaves * i] = vs[i];
+      }
+    }
+    if (edge_step && tid < kPos / 32) nan_at[buf][tid] = 0;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (edge_step) {
-      if (tid < kPos / 32) nan_at[tid] = 0;
-      __syncthreads();
-    }
+      // 0 times a NaN code would reach rows that do not see it
 #pragma unroll
-    for (int i = 0; i < KVS; ++i) {
-      if (lane == 0) {
-        scale[0][wave + kPaWaves * i] = ks[i];
-        scale[1][wave + kPaWaves * i] = vs[i];
-      }
+      for (int i = 0; i < KVS; ++i)
 #pragma unroll
-      for (int j = 0; j < kLd; ++j) {
-        const int row = 16 * (wave + kPaWaves * i) + (1024 * j + 16 * lane) / D, c = 16 * lane % D;
-        if (edge_step) {
-          // 0 times a NaN code would reach rows that do not see it
-          const uint4 v = vr[i][j];
+        for (int j = 0; j < kLd; ++j) {
+          const int row = 16 * (wave + kPaWaves * i) + (1024 * j + 16 * lane) / D;
+          uint4* q = reinterpret_cast<uint4*>(&tile[buf][1][16 * (wave + kPaWaves * i) * D + 1024 * j + 16 * lane]);
+          const uint4 v = *q;
           if (has_nan_code(v.x) || has_nan_code(v.y) || has_nan_code(v.z) || has_nan_code(v.w)) {
-            atomicOr(&nan_at[row >> 5], 1u << (row & 31));
-            vr[i][j] = make_uint4(0, 0, 0, 0);
+            if (t0 + row < most) atomicOr(&nan_at[buf][row >> 5], 1u << (row & 31));
+            *q = make_uint4(0, 0, 0, 0);
           }
         }
-        *reinterpret_cast<uint4*>(&tile[0][row * kPitch + c]) = kr[i][j];
-        *reinterpret_cast<uint4*>(&tile[1][row * kPitch + c]) = vr[i][j];
-      }
+      __syncthreads();
     }
-    __syncthreads();
     if (t0 + kPos < most) {
-      load_tile(t0 + kPos);
+      load_tile(t0 + kPos, buf ^ 1);
       load_ids(t0 + 2 * kPos);
     }
     const int64_t t1 = t0 + part * kPaTile;
     if (t1 >= mine) continue;
-    const uint8_t* kt = tile[0] + part * kPaTile * kPitch;
-    const uint8_t* vt = tile[1] + part * kPaTile * kPitch;
+    const uint8_t* kt = &tile[buf][0][part * kPaTile * D];
+    const uint8_t* vt = &tile[buf][1][part * kPaTile * D];
     f32x16_t s[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       s[b] = f32x16_t{};
 #pragma unroll
       for (int i = 0; i < kQ; ++i) {
-        const uint4 t = *reinterpret_cast<const uint4*>(kt + (32 * b + col) * kPitch + (2 * i + h) * 16);
+        const uint4 t = *reinterpret_cast<const uint4*>(kt + 32 * b * D + k_at[i]);
         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_bf16<INT8>(t.x, t.y), qf[i][0], s[b], 0, 0, 0);
         s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_bf16<INT8>(t.z, t.w), qf[i][1], s[b], 0, 0, 0);
       }
@@ -539,8 +565,8 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
     float ksc[4], vsc[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      ksc[g] = scale[0][4 * part + g];
-      vsc[g] = scale[1][4 * part + g];
+      ksc[g] = scale[buf][0][4 * part + g];
+      vsc[g] = scale[buf][1][4 * part + g];
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g)
@@ -551,7 +577,7 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
         for (int i = 0; i < 8; ++i) x[8 * g + i] *= sign;
       }
     if (t1 + kPaTile > whole) {
-      uint32_t nans[2] = {edge_step ? nan_at[2 * part] : 0u, edge_step ? nan_at[2 * part + 1] : 0u};
+      uint32_t nans[2] = {edge_step ? nan_at[buf][2 * part] : 0u, edge_step ? nan_at[buf][2 * part + 1] : 0u};
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         if (!(fabsf(vsc[g]) <= 3.4028234e38f) || !(ksc[g] <= 3.4028234e38f)) {
@@ -565,7 +591,7 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
         if (t1 + 32 * (i >> 4) + at >= lim) x[i] = -INFINITY;
       }
     } else if (edge_step) {
-      const uint32_t nans[2] = {nan_at[2 * part], nan_at[2 * part + 1]};
+      const uint32_t nans[2] = {nan_at[buf][2 * part], nan_at[buf][2 * part + 1]};
       if (nans[0] | nans[1]) l = __uint_as_float(0x7FC00000u);  // every row of the wave sees it
     }
     float mt = -INFINITY;
@@ -577,15 +603,17 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
       mt = fmaxf(mt, y * ksc[g]);
     }
     mt = fmaxf(mt, __shfl_xor(mt, 32));
-    const float mn = fmaxf(m, mt);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    if (__any(mn > m)) {
-      const float f = __builtin_amdgcn_exp2f(m - base);
+    // m may lag the largest score by 2^8: of 32 rows some find a larger one in most
+    // tiles, and the sums have the range
+    if (__any(mt > m + 8.f)) {
+      const float mn = fmaxf(m, mt);
+      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       l *= f;
 #pragma unroll
       for (int j = 0; j < kV; ++j) acc[j] *= f;
       m = mn;
     }
+    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int g = 0; g < 4; ++g)
 #pragma unroll
@@ -617,7 +645,7 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
       uint32_t v[8][kW];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint8_t* src = vt + (16 * g + 4 * h + (i & 3) + 8 * (i >> 2)) * kPitch + col * kV;
+        const uint8_t* src = vt + 16 * g * D + v_at[i];
         if constexpr (kV == 2) {
           v[i][0] = *reinterpret_cast<const uint16_t*>(src);
         } else if constexpr (kV == 4) {
