@@ -64,12 +64,12 @@ struct SampleArgs {
 
 struct SampleLds {
   uint64_t hist[kSmBins];     // weights; as uint32_t: numbers of words
-  uint64_t block[kSmBlocks];  // kept weight of each block of words
+  uint64_t sums[kSmBlocks / 4];  // kept weight of each group of four blocks
   float x[kSmList];
   int id[kSmList];
   uint64_t w[kSmList];
   uint64_t wave[2][kSmWaves];
-  float top[kSmWaves];
+  float best[kSmWaves], odd[kSmWaves];
   int first;
   int n;
   float cut_x;
@@ -111,6 +111,27 @@ __device__ __forceinline__ uint64_t wave_upto64(uint64_t v) {
   v += dpp_u64<0x142, 0xA>(v);
   v += dpp_u64<0x143, 0xC>(v);
   return v;
+}
+
+// Sum over the 64 lanes, returned to every lane.
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  auto dpp = [](auto ctrl, double x) {
+    return __longlong_as_double(static_cast<long long>(dpp_u64<decltype(ctrl)::value>(static_cast<uint64_t>(__double_as_longlong(x)))));
+  };
+  v += dpp(std::integral_constant<int, 0xB1>(), v);
+  v += dpp(std::integral_constant<int, 0x4E>(), v);
+  v += dpp(std::integral_constant<int, 0x141>(), v);
+  v += dpp(std::integral_constant<int, 0x140>(), v);
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+  auto lane = [&](int l) { return __longlong_as_double(static_cast<long long>(lane_u64(b, l))); };
+  return (lane(0) + lane(16)) + (lane(32) + lane(48));
+}
+
+// A sum of weights of at most 512 in units of 2^-44.
+__device__ __forceinline__ uint64_t units(double s) {
+  const double hi = floor(s);
+  return (static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 44) +
+         (static_cast<uint64_t>(__double_as_longlong(256.0 + (s - hi))) - 0x4070000000000000ull);
 }
 
 __device__ __forceinline__ float wave_max_f32(float v) {
@@ -163,8 +184,8 @@ struct Scale {
   double c;  // log2(e) / T
   float cf;  // bins per unit of x
 
-  // For words of the bins: 2^44 for the best, 0 below 2^-45 of it.
-  __device__ __forceinline__ uint64_t weight(float x) const {
+  // For words of the bins: 256 and the weight, which 256 gives units of 2^-44.
+  __device__ __forceinline__ double weight256(float x) const {
     const double y = (static_cast<double>(x) - static_cast<double>(top)) * c;
     const double t = y + 6755399441055744.0;  // 1.5 2^52: y to the nearest integer, in the low bits
     const double f = y - (t - 6755399441055744.0);
@@ -176,16 +197,24 @@ struct Scale {
     p = fma_s(p, f, 0.24022650698110454);
     p = fma_s(p, f, 0.6931471805482117);
     p = fma(p, f, 1.0);
-    // 256 + w has units of 2^-44
-    const double w = 256.0 + __builtin_amdgcn_ldexp(p, static_cast<int>(__double_as_longlong(t)));
-    return static_cast<uint64_t>(__double_as_longlong(w)) - 0x4070000000000000ull;
+    return 256.0 + __builtin_amdgcn_ldexp(p, static_cast<int>(__double_as_longlong(t)));
   }
+  // In units of 2^-44: 2^44 for the best, 0 below 2^-45 of it.
+  __device__ __forceinline__ uint64_t weight(float x) const {
+    return static_cast<uint64_t>(__double_as_longlong(weight256(x))) - 0x4070000000000000ull;
+  }
+  // As a number; sums of up to 512 of these are exact.
+  __device__ __forceinline__ double weight_f64(float x) const { return weight256(x) - 256.0; }
   // The bin of x; kSmBins or more: no weight.  Never lower for a smaller x.
   __device__ __forceinline__ int bin(float x) const {
     const float y = (top - x) * cf;
     return y < static_cast<float>(kSmBins) ? static_cast<int>(y) : kSmBins;
   }
 };
+
+// Blocks of a wave: four in a row, then the next four 64 on; bit l of a set and
+// lane l stand for block block_of(l, wave).  A group of four is a row of s.sums.
+__device__ __forceinline__ int block_of(int l, int wave) { return (l >> 2) * (4 * kSmWaves) + 4 * wave + (l & 3); }
 
 // A row in blocks of 16 bytes a lane.
 template <bool BF16>
@@ -215,38 +244,43 @@ struct Row {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // NaN is -infinity, infinity the largest finite number.
+  // NaN is -infinity, infinity the largest finite number (PLAIN: the row has neither).
+  template <bool PLAIN = false>
   __device__ __forceinline__ void words(const uint4& raw, float (&x)[kPer]) const {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       const float v = __uint_as_float(BF16 ? ((e & 1) ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16) : w[e & 3]);
-      x[e] = __builtin_amdgcn_fmed3f(v >= -INFINITY ? v : -INFINITY, -INFINITY, 3.4028234663852886e38f);
+      x[e] = PLAIN ? v : __builtin_amdgcn_fmed3f(v >= -INFINITY ? v : -INFINITY, -INFINITY, 3.4028234663852886e38f);
     }
   }
   // f(block, first id, words of this lane, the block's bit) over this wave's blocks
-  // in `set` (bit l: block wave + 16 l), four loads in flight.
-  template <typename F>
-  __device__ __forceinline__ void each(uint64_t set, int wave, F f) const {
-    constexpr int kAhead = 4;
+  // in `set` (block_of), then done(group) after the last of a group of four, whose
+  // loads are in flight together.
+  template <bool PLAIN = false, typename F, typename G>
+  __device__ __forceinline__ void each(uint64_t set, int wave, F f, G done) const {
     while (set != 0) {
-      uint4 raw[kAhead];
-      int at[kAhead];
+      const int group = __builtin_ctzll(set) >> 2;
+      const uint32_t four = static_cast<uint32_t>(set >> (4 * group)) & 15u;
+      set &= ~(15ull << (4 * group));
+      uint4 raw[4];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        at[j] = set != 0 ? __builtin_ctzll(set) : -1;
-        set &= set - 1;
-        if (at[j] >= 0) raw[j] = load(wave + kSmWaves * at[j]);
-      }
+      for (int j = 0; j < 4; ++j)
+        if ((four >> j) & 1) raw[j] = load(block_of(4 * group + j, wave));
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        if (at[j] < 0) break;
+      for (int j = 0; j < 4; ++j) {
+        if (!((four >> j) & 1)) continue;
         float x[kPer];
-        words(raw[j], x);
-        const int b = wave + kSmWaves * at[j];
-        f(b, first(b), x, at[j]);
+        words<PLAIN>(raw[j], x);
+        const int b = block_of(4 * group + j, wave);
+        f(b, first(b), x, 4 * group + j);
       }
+      done(group * kSmWaves + wave);
     }
+  }
+  template <bool PLAIN = false, typename F>
+  __device__ __forceinline__ void each(uint64_t set, int wave, F f) const {
+    each<PLAIN>(set, wave, f, [](int) {});
   }
 };
 
@@ -266,29 +300,40 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
   int turn = 0;
   auto before64 = [&](uint64_t v, uint64_t& total) { return block_before64(v, s.wave, turn, total); };
 
-  // the best of each of the wave's blocks, lane l: block wave + 16 l, and of the row
-  const int own = blocks > wave ? (blocks - wave + kSmWaves - 1) / kSmWaves : 0;
+  // the best of each of the wave's blocks, lane l: block_of(l, wave), and of the row
+  const int own = 4 * (blocks / (4 * kSmWaves)) + min(max(blocks % (4 * kSmWaves) - 4 * wave, 0), 4);
   float high = -INFINITY;
-  words.each(own >= 64 ? ~0ull : (1ull << own) - 1, wave, [&](int, int, const float(&x)[kPer], int bit) {
-    float m = x[0];
+  bool odd = false;
+  words.template each<true>(own >= 64 ? ~0ull : (1ull << own) - 1, wave, [&](int, int, const float(&x)[kPer], int bit) {
+    float m = -INFINITY;
 #pragma unroll
-    for (int e = 1; e < kPer; ++e) m = fmaxf(m, x[e]);
-    m = wave_max_f32(m);
+    for (int e = 0; e < kPer; ++e) {
+      odd |= !(x[e] < INFINITY);
+      m = fmaxf(m, x[e]);
+    }
+    m = fminf(wave_max_f32(m), 3.4028234663852886e38f);
     high = lane == bit ? m : high;
   });
   float top = wave_max_f32(high);
-  if (lane == 0) s.top[wave] = top;
+  const bool any_odd = any_lane(odd);
+  if (lane == 0) s.odd[wave] = any_odd ? 1.f : 0.f;
+  if (lane == 0) s.best[wave] = top;
   if (tid == 0) s.first = a.vocab;
   for (int i = tid; i < kSmBins; i += kSmThreads) s.hist[i] = 0;
   if (tid == 0) s.n = 0;
   __syncthreads();
-  top = wave_max_f32(lane < kSmWaves ? s.top[lane] : -INFINITY);
+  top = wave_max_f32(lane < kSmWaves ? s.best[lane] : -INFINITY);
+  const bool plain = wave_max_f32(lane < kSmWaves ? s.odd[lane] : 0.f) == 0.f;  // no NaN, no infinity
   if (top == -INFINITY) {  // nothing to draw
     if (tid == 0) a.out[row] = -1;
     return;
   }
   // f over the words of blocks with a value of at least `floor`
   auto pass = [&](float floor, auto f) { words.each(__ballot(high >= floor), wave, f); };
+  auto plain_pass = [&](float floor, auto f, auto done) {  // two forms of the code: for the passes that compute much
+    if (plain) words.template each<true>(__ballot(high >= floor), wave, f, done);
+    else words.each(__ballot(high >= floor), wave, f, done);
+  };
   if (!(T > 0.f) || k == 1 || p <= 0.f) {  // the best alone: its lowest id
     int at = a.vocab;
     pass(top, [&](int, int i, const float(&x)[kPer], int) {
@@ -305,8 +350,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
   const Scale sc{top, c, static_cast<float>(fmin(c * kSmBinsPerOctave, 3e38))};
   // words from here on have weight
   const float reach = fmaxf(static_cast<float>(static_cast<double>(top) - 47.0 / c), -3.4028234663852886e38f);
-  const uint64_t least =
-      min_p > 0.f ? static_cast<uint64_t>(ceil(ldexp(fmin(static_cast<double>(min_p), 1.0), 44))) : 1;
+  const double least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
   float cut_x = -INFINITY, floor = reach;
   int cut_id = a.vocab;
   auto kept = [&](float x, int id) { return x > cut_x || (x == cut_x && id <= cut_id); };
@@ -354,16 +398,14 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
     });
   };
   auto add_weights_of = [&](auto all) {
-    pass(floor, [&](int, int i, const float(&x)[kPer], int) {
+    plain_pass(floor, [&](int, int i, const float(&x)[kPer], int) {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
         const int b = sc.bin(x[e]);
-        const bool in = b < kSmBins && (decltype(all)::value || kept(x[e], i + e));
-        if (!any_lane(in)) continue;
-        const uint64_t w = sc.weight(x[e]);
-        if (in) atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[b]), w);
+        if (b < kSmBins && (decltype(all)::value || kept(x[e], i + e)))
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[b]), sc.weight(x[e]));
       }
-    });
+    }, [](int) {});
   };
   auto add_weights = [&] {
     if (cut_x == -INFINITY) add_weights_of(std::true_type());
@@ -376,13 +418,12 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
 
   // The last word that a rule keeps: the one whose amount before it is the last
   // below the rule's.  After find_bin.
-  auto cut = [&](auto by, uint32_t wanted, double share) {
+  // listed: the words of the bin are in the list already, if there is room.
+  auto cut = [&](auto by, uint32_t wanted, double share, int bin, uint64_t above, bool listed) {
     constexpr bool BY = decltype(by)::value;
-    const int bin = s.bin;
-    const uint64_t above = s.above;
     auto full = [&](uint64_t t) { return BY ? static_cast<double>(t) >= share : t >= wanted; };
     const float low = bin_floor(bin), up = static_cast<float>(static_cast<double>(top) - (bin - 1) / (c * kSmBinsPerOctave));
-    pass(low, [&](int, int i, const float(&x)[kPer], int) {
+    if (!listed) pass(low, [&](int, int i, const float(&x)[kPer], int) {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
         if (!any_lane(x[e] >= low && x[e] <= up)) continue;
@@ -441,8 +482,9 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
         past = s.above;
         __syncthreads();
       }
-      // of the equal words, the one where it is reached: its block, then its lane
-      for (int b = tid; b < kSmBlocks; b += kSmThreads) s.block[b] = 0;
+      // of the equal words, the one where it is reached: its group of blocks, its
+      // block, its lane
+      if (tid < kSmBlocks / 4) s.sums[tid] = 0;
       __syncthreads();
       const float value = of_key(prefix);
       auto mine_of = [&](int i, const float(&x)[kPer]) {
@@ -452,12 +494,15 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
           if (x[e] == value && kept(value, i + e)) m += BY ? sc.weight(x[e]) : 1;
         return m;
       };
-      pass(low, [&](int b, int i, const float(&x)[kPer], int) {
-        const uint64_t m = wave_sum64(mine_of(i, x));
-        if (lane == 0) s.block[b] = m;
-      });
+      uint64_t of_group = 0;
+      words.each(__ballot(high >= low), wave, [&](int, int i, const float(&x)[kPer], int) { of_group += mine_of(i, x); },
+                 [&](int group) {
+                   const uint64_t m = wave_sum64(of_group);
+                   if (lane == 0) s.sums[group] = m;
+                   of_group = 0;
+                 });
       __syncthreads();
-      const uint64_t m = s.block[tid];
+      const uint64_t m = tid < kSmBlocks / 4 ? s.sums[tid] : 0;
       const uint64_t ahead = past + before64(m, total);
       if (!full(ahead) && full(ahead + m)) {
         s.bin = tid;
@@ -465,20 +510,24 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
       }
       __syncthreads();
       if (wave == 0) {
-        float x[kPer];
-        words.words(words.load(s.bin), x);
-        const int i = words.first(s.bin);
-        const uint64_t of_lane = mine_of(i, x);
-        uint64_t at = s.above + wave_upto64(of_lane) - of_lane;
+        uint64_t from = s.above;
+        for (int b = 4 * s.bin; b < 4 * s.bin + 4; ++b) {
+          float x[kPer];
+          words.words(words.load(b), x);
+          const int i = words.first(b);
+          const uint64_t of_lane = mine_of(i, x), upto = wave_upto64(of_lane);
+          uint64_t at = from + upto - of_lane;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          if (x[e] != value || !kept(value, i + e)) continue;
-          const uint64_t w = BY ? sc.weight(x[e]) : 1;
-          if (!full(at) && full(at + w)) {
-            s.cut_x = value;
-            s.cut_id = i + e;
+          for (int e = 0; e < kPer; ++e) {
+            if (x[e] != value || !kept(value, i + e)) continue;
+            const uint64_t w = BY ? sc.weight(x[e]) : 1;
+            if (!full(at) && full(at + w)) {
+              s.cut_x = value;
+              s.cut_id = i + e;
+            }
+            at += w;
           }
-          at += w;
+          from += lane_u64(upto, 63);
         }
       }
     }
@@ -536,7 +585,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
       before64(mine ? w : 0, total);
       if (!(static_cast<double>(b) < share * static_cast<double>(total))) w = 0;
     }
-    if (w < least) w = 0;
+    if (static_cast<double>(w) < ldexp(least, 44)) w = 0;
     __syncthreads();  // the list's weights are read
     if (mine) s.w[e] = w;
     before64(mine ? w : 0, total);
@@ -565,40 +614,76 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
         draw_from_list();
         return;
       }
-      cut(by_words, wanted, share);
+      cut(by_words, wanted, share, s.bin, s.above, false);
       __syncthreads();
     }
   }
-  if (p < 1.f && find_bin(std::true_type(), 0, share, add_weights)) cut(std::true_type(), 0, share);
+  const bool by_share = p < 1.f && find_bin(std::true_type(), 0, share, add_weights);
+  const int border = by_share ? s.bin : kSmBins;
+  const uint64_t above = by_share ? s.above : 0;
+  if (tid < kSmBlocks / 4) s.sums[tid] = 0;
+  __syncthreads();
 
-  // kept weight of each block of words
-  auto weights = [&](auto bounded, int i, const float(&x)[kPer], uint64_t(&w)[kPer]) {
-    uint64_t sum = 0;
+  // kept weight of each group of blocks, those of top-p's bin in the list for now
+  float need = floor;
+  if (least > 0.0) need = fmaxf(need, static_cast<float>(static_cast<double>(top) + (log2(least) - 0.01) / c));
+  auto by_groups = [&](auto part, auto simple) {  // simple: no top-k, no min-p
+    constexpr bool SIMPLE = decltype(simple)::value;
+    double sum = 0.0;
+    plain_pass(decltype(part)::value ? fmaxf(floor, bin_floor(border)) : need, [&](int, int i, const float(&x)[kPer], int) {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      w[e] = 0;
-      const bool in = x[e] >= floor && kept(x[e], i + e);
-      if (!any_lane(in)) continue;
-      const uint64_t t = sc.weight(x[e]);
-      if (in && (!decltype(bounded)::value || t >= least)) w[e] = t;
-      sum += w[e];
-    }
-    return sum;
-  };
-  __syncthreads();
-  for (int b = tid; b < kSmBlocks; b += kSmThreads) s.block[b] = 0;
-  __syncthreads();
-  auto by_blocks = [&](auto bounded) {
-    pass(floor, [&](int b, int i, const float(&x)[kPer], int) {
-      uint64_t w[kPer];
-      const uint64_t sum = wave_sum64(weights(bounded, i, x, w));
-      if (lane == 0) s.block[b] = sum;
+      for (int e = 0; e < kPer; ++e) {
+        if constexpr (decltype(part)::value) {
+          const int bin = sc.bin(x[e]);
+          if (bin <= border && (SIMPLE || kept(x[e], i + e))) {
+            const double w = sc.weight_f64(x[e]);
+            sum += bin < border && (SIMPLE || w >= least) ? w : 0.0;
+            if (bin == border) {
+              const int at = atomicAdd(&s.n, 1);
+              if (at < kSmList) {
+                s.x[at] = x[e];
+                s.id[at] = i + e;
+                s.w[at] = units(w);
+              }
+            }
+          }
+        } else if (x[e] >= need && (SIMPLE || kept(x[e], i + e))) {
+          const double w = sc.weight_f64(x[e]);
+          sum += SIMPLE || w >= least ? w : 0.0;
+        }
+      }
+    }, [&](int group) {
+      const uint64_t all = wave_sum64(units(sum));
+      if (lane == 0) s.sums[group] = all;
+      sum = 0.0;
     });
   };
-  if (least > 1) by_blocks(std::true_type());
-  else by_blocks(std::false_type());
+  const bool simple = cut_x == -INFINITY && least == 0.0;
+  if (by_share) {
+    if (simple) by_groups(std::true_type(), std::true_type());
+    else by_groups(std::true_type(), std::false_type());
+    __syncthreads();
+    const int n = s.n;
+    cut(std::true_type(), 0, share, border, above, true);
+    if (n <= kSmList) {
+      if (tid < n && kept(s.x[tid], s.id[tid]) && static_cast<double>(s.w[tid]) >= ldexp(least, 44)) {
+        const int b = s.id[tid] / (64 * kPer);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.sums[b / 4]), s.w[tid]);
+      }
+    } else {  // the cut took the table; and it is known now
+      __syncthreads();
+      if (tid < kSmBlocks / 4) s.sums[tid] = 0;
+      __syncthreads();
+      need = fmaxf(need, floor);
+      by_groups(std::false_type(), std::false_type());
+    }
+  } else if (simple) {
+    by_groups(std::false_type(), std::true_type());
+  } else {
+    by_groups(std::false_type(), std::false_type());
+  }
   __syncthreads();
-  const uint64_t mine = s.block[tid];
+  const uint64_t mine = tid < kSmBlocks / 4 ? s.sums[tid] : 0;
   uint64_t total;
   const uint64_t before = before64(mine, total);
   const double target = (u > 0.f ? static_cast<double>(u) : 0.0) * static_cast<double>(total);
@@ -609,13 +694,29 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
     s.above = before;
   }
   __syncthreads();
-  if (wave != 0) return;
-  float x[kPer];
-  uint64_t w[kPer];
-  words.words(words.load(s.bin), x);
-  const int i = words.first(s.bin);
-  const uint64_t sum = weights(std::true_type(), i, x, w);
-  uint64_t at = s.above + wave_upto64(sum) - sum;
+  // a wave for each block of the group
+  uint64_t w[kPer], sum = 0, upto = 0;
+  int i = 0;
+  if (wave < 4) {
+    float x[kPer];
+    words.words(words.load(4 * s.bin + wave), x);
+    i = words.first(4 * s.bin + wave);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      w[e] = 0;
+      if (x[e] >= floor && kept(x[e], i + e)) {
+        const double v = sc.weight_f64(x[e]);
+        w[e] = v >= least ? units(v) : 0;
+      }
+      sum += w[e];
+    }
+    upto = wave_upto64(sum);
+    if (lane == 63) s.hist[wave] = upto;
+  }
+  __syncthreads();
+  if (wave >= 4) return;
+  uint64_t at = s.above + upto - sum;
+  for (int j = 0; j < wave; ++j) at += s.hist[j];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     if (w[e] > 0 && (inside ? static_cast<double>(at) <= target && static_cast<double>(at + w[e]) > target
