@@ -64,6 +64,48 @@ __device__ __forceinline__ bf16x8_t eight_bf16(uint32_t lo, uint32_t hi) {
                                                  two_bf16<INT8, false>(hi), two_bf16<INT8, true>(hi)));
 }
 
+__device__ __forceinline__ SeqSpan uniform(SeqSpan s) {
+  s.seq = __builtin_amdgcn_readfirstlane(s.seq);
+  s.row0 = __builtin_amdgcn_readfirstlane(s.row0);
+  s.n = __builtin_amdgcn_readfirstlane(s.n);
+  s.unit = __builtin_amdgcn_readfirstlane(s.unit);
+  s.len = __builtin_amdgcn_readfirstlane(static_cast<int>(s.len));
+  return s;
+}
+
+// Where 16-position groups of a head lie and their scales, one group a lane, so
+// that the loops look nothing up in memory: the next 64 pages' numbers are on their
+// way from when the last 64 were taken.
+struct Groups {
+  uint32_t lo, hi;  // byte offset of the group's first code
+  float ks, vs;     // K's scale times the scores' factor, V's
+  int page;         // of the 64 groups after these
+
+  // Position p of this lane's group, or -1.
+  __device__ __forceinline__ void ask(const PagedAttnArgs& a, const int32_t* table, int64_t p) {
+    page = p >= 0 ? table[p >> a.log_page] : 0;
+  }
+  __device__ __forceinline__ void take(const PagedAttnArgs& a, int64_t p, int head, int dim) {
+    const bool ok = p >= 0 && page >= 0 && page < a.pages;
+    const int64_t block = static_cast<int64_t>(ok ? page : 0) * a.kv_heads + head;
+    const int64_t byte = ((block << a.log_page) + (p >= 0 ? p & ((1 << a.log_page) - 1) : 0)) * dim;
+    lo = static_cast<uint32_t>(byte);
+    hi = static_cast<uint32_t>(byte >> 32);
+    ks = vs = 1.f;
+    if (ok) {
+      ks = a.ks[block] * a.c2;
+      vs = a.vs[block];
+    } else if (p >= 0) {
+      ks = __uint_as_float(0x7FC00000u);  // a page out of range: NaN for who sees it
+    }
+  }
+  __device__ __forceinline__ int64_t byte_of(int l) const {
+    return static_cast<int64_t>(wave_read_lane(lo, l) | (static_cast<uint64_t>(wave_read_lane(hi, l)) << 32));
+  }
+  __device__ __forceinline__ float ks_of(int l) const { return __uint_as_float(wave_read_lane(__float_as_uint(ks), l)); }
+  __device__ __forceinline__ float vs_of(int l) const { return __uint_as_float(wave_read_lane(__float_as_uint(vs), l)); }
+};
+
 // Any of four e4m3 codes NaN.
 __device__ __forceinline__ bool has_nan_code(uint32_t w) {
   return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
@@ -76,7 +118,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
   constexpr int kVWords = kVDims / 4;
   __shared__ float part[kPaWaves][16][D + 4];
   __shared__ float2 ml[kPaWaves][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, h = lane >> 4;
   const int head = blockIdx.y, lp = a.log_page, page = 1 << lp;
   // the row tile: rows [unit 16, unit 16 + 16) of a sequence's n group
@@ -92,6 +134,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
     sp = find_unit(a.s, blockIdx.x, [group](int n, int64_t) { return n * group <= kPaFew ? 1 : 0; });
     if (sp.seq < 0) return;
   }
+  sp = uniform(sp);
   const int r = sp.unit * 16 + col, token = r / group, sub = r - token * group;
   const bool live = token < sp.n;
   const int64_t room = static_cast<int64_t>(a.s.width) << lp;
@@ -99,7 +142,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
   const int64_t sees = live ? sp.len - sp.n + 1 + token : 0;
   const int last = min(sp.unit * 16 + 15, sp.n * group - 1) / group;
   const int64_t most = min(max(sp.len - sp.n + 1 + last, int64_t(0)), room);
-  bool lost = sees > room;  // positions without a page: NaN
+  const bool lost = sees > room;  // positions without a page: NaN
   const int64_t lim = sees;
   const int64_t from = static_cast<int64_t>(blockIdx.z) * a.chunk, to = min(most, from + a.chunk);
 
@@ -122,36 +165,32 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
   const int32_t* table = a.s.table + sp.seq * a.s.ld_table;
   const uint32_t k_off = col * D + h * 16, v_off = 4 * h * D + col * kVDims;
 
-  for (int64_t t0 = from + wave * kPaTile; t0 < to; t0 += kPaTile * kPaWaves) {
-    const int groups = static_cast<int>(min((to - t0 + 15) >> 4, int64_t(4)));
-    const uint8_t *kp[4], *vp[4];
-    float ksc[4], vsc[4];
+  // lane l: group l & 3 of the wave's tile l >> 2
+  constexpr int64_t kStep = kPaTile * kPaWaves;
+  Groups pg;
+  auto group_at = [&](int64_t t0) {
+    const int64_t p = t0 + kStep * (lane >> 2) + 16 * (lane & 3);
+    return p < to ? p : int64_t(-1);
+  };
+  // K's registers are loaded again as soon as the scores are computed from them,
+  // V's after the products, so that a wave always has one of them on its way
+  uint4 kr[4][kLoads];
+  uint32_t vr[4][4][kVWords];
+  int64_t byte[4];
+  auto load_k = [&](int j) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {  // groups past the last repeat it, masked
-      const int64_t p = t0 + 16 * min(g, groups - 1);
-      int id = __builtin_amdgcn_readfirstlane(table[p >> lp]);
-      if (id < 0 || id >= a.pages) {
-        id = 0;
-        lost |= p < lim;
-      }
-      const int64_t block = static_cast<int64_t>(id) * a.kv_heads + head;
-      const int64_t byte = ((block << lp) + (p & (page - 1))) * D;
-      kp[g] = a.kc + byte;
-      vp[g] = a.vc + byte;
-      ksc[g] = a.ks[block] * a.c2;
-      vsc[g] = a.vs[block];
+    for (int g = 0; g < 4; ++g) {
+      byte[g] = pg.byte_of(4 * j + g);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) kr[g][i] = *reinterpret_cast<const uint4*>(a.kc + byte[g] + k_off + 64 * i);
     }
-    uint4 kr[4][kLoads];
-    uint32_t vr[4][4][kVWords];
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) kr[g][i] = *reinterpret_cast<const uint4*>(kp[g] + k_off + 64 * i);
+  };
+  auto load_v = [&] {
 #pragma unroll
     for (int g = 0; g < 4; ++g)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* p = vp[g] + v_off + i * D;
+        const uint8_t* p = a.vc + byte[g] + v_off + i * D;
         if constexpr (kVWords == 1) {
           vr[g][i][0] = *reinterpret_cast<const uint32_t*>(p);
         } else if constexpr (kVWords == 2) {
@@ -162,6 +201,31 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
           vr[g][i][0] = t.x; vr[g][i][1] = t.y; vr[g][i][2] = t.z; vr[g][i][3] = t.w;
         }
       }
+  };
+  float ksc[4], vsc[4];
+  auto scales = [&](int j) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      ksc[g] = pg.ks_of(4 * j + g);
+      vsc[g] = pg.vs_of(4 * j + g);
+    }
+  };
+  const int64_t start = from + wave * kPaTile;
+  if (start < to) {
+    pg.ask(a, table, group_at(start));
+    pg.take(a, group_at(start), head, D);
+    pg.ask(a, table, group_at(start + 16 * kStep));
+    // K before V, as in the loop: its scores wait for K's loads alone
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_v();
+    __builtin_amdgcn_sched_barrier(0);
+    scales(0);
+  }
+  int j = 0;  // the tile's lanes are 4 j ..
+  for (int64_t t0 = start; t0 < to; t0 += kStep) {
+    const bool more = t0 + kStep < to;
     float s[4][4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -173,6 +237,14 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[g][i] = x[i] * ksc[g];
+    }
+    if (more) {
+      if (++j == 16) {
+        j = 0;
+        pg.take(a, group_at(t0 + kStep), head, D);
+        pg.ask(a, table, group_at(t0 + 17 * kStep));
+      }
+      load_k(j);
     }
     const int64_t whole = min(sp.len - sp.n + 1 + sp.unit * 16 / group, to);  // every row sees up to here
     const bool edge = t0 + kPaTile > whole;
@@ -205,15 +277,16 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
       for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[g][i]);
     mt = fmaxf(mt, __shfl_xor(mt, 16));
     mt = fmaxf(mt, __shfl_xor(mt, 32));
-    const float mn = fmaxf(m, mt);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    if (__any(mn > m)) {
-      const float f = __builtin_amdgcn_exp2f(m - base);
+    // m may lag the largest score by 2^8: the sums have the range
+    if (__builtin_amdgcn_ballot_w64(mt > m + 8.f) != 0) {
+      const float mn = fmaxf(m, mt);
+      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       l *= f;
 #pragma unroll
       for (int j = 0; j < kVDims; ++j) acc[j] *= f;
       m = mn;
     }
+    const float base = m == -INFINITY ? 0.f : m;
     uint32_t pb[4][2];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -257,6 +330,10 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
           acc[4 * w + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, acc[4 * w + j], 0, 0, 0);
         }
       }
+    }
+    if (more) {
+      load_v();
+      scales(j);
     }
   }
   // join the waves: a lane holds dimensions h D / 4 .. of its row
@@ -417,14 +494,13 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
   constexpr int kLd = D / 64;                   // 16-byte loads per lane of 16 positions
   constexpr int kQ = D / 32, kV = D / 32;       // chunks of K per lane; dimensions of V per lane
   __shared__ __attribute__((aligned(1024))) uint8_t tile[2][2][kPos * D];  // [step & 1][K, V]
-  __shared__ float scale[2][2][kPos / 16];
   __shared__ uint32_t nan_at[2][kPos / 32];  // positions whose V holds a NaN code
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5, part = wave / kGroups;
   const int head = blockIdx.x % a.kv_heads, lp = a.log_page, page = 1 << lp, group = a.group;
-  const SeqSpan sp = find_unit(a.s, blockIdx.x / a.kv_heads, [group](int n, int64_t) {
+  const SeqSpan sp = uniform(find_unit(a.s, blockIdx.x / a.kv_heads, [group](int n, int64_t) {
     return n * group > kPaFew ? (n * group + kRows - 1) / kRows : 0;
-  });
+  }));
   if (sp.seq < 0) return;
   // the last rows, which see most, first
   const int unit = (sp.n * group + kRows - 1) / kRows - 1 - sp.unit;
@@ -465,33 +541,19 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
   }
   const uint32_t lds0 = static_cast<uint32_t>(
       (uintptr_t)((__attribute__((address_space(3))) const char*)(const void*)&tile[0][0][0]));
-  int id[KVS];
-  float ks[KVS], vs[KVS];
-  auto load_ids = [&](int64_t t0) {
-#pragma unroll
-    for (int i = 0; i < KVS; ++i) {
-      const int64_t p = t0 + 16 * (wave + kPaWaves * i);
-      id[i] = p < most ? __builtin_amdgcn_readfirstlane(table[p >> lp]) : 0;
-    }
-  };
+  Groups pg;  // lane l: positions 16 l .. of 1024
+  auto group_at = [&](int64_t t0) { return t0 + 16 * lane < most ? t0 + 16 * lane : int64_t(-1); };
   auto load_tile = [&](int64_t t0, int buf) {
 #pragma unroll
     for (int i = 0; i < KVS; ++i) {
       const int at = wave + kPaWaves * i;
-      const int64_t p = t0 + 16 * at;
-      ks[i] = vs[i] = 0.f;
-      if (p >= most) continue;  // what LDS holds there is not seen
-      const bool ok = id[i] >= 0 && id[i] < a.pages;
-      const int64_t block = static_cast<int64_t>(ok ? id[i] : 0) * a.kv_heads + head;
-      const int64_t byte = ((block << lp) + (p & (page - 1))) * D;
+      if (t0 + 16 * at >= most) continue;  // what LDS holds there is not seen
+      const int64_t byte = pg.byte_of(static_cast<int>(t0 % 1024) / 16 + at);
       const uint32_t dst = lds0 + (2 * buf * kPos + 16 * at) * D;
 #pragma unroll
       for (int j = 0; j < kLd; ++j) to_lds16(a.kc + byte, src[j], dst + 1024 * j);
 #pragma unroll
       for (int j = 0; j < kLd; ++j) to_lds16(a.vc + byte, src[j], dst + kPos * D + 1024 * j);
-      // a page out of range makes its scores NaN
-      ks[i] = ok ? a.ks[block] * a.c2 : __uint_as_float(0x7FC00000u);
-      vs[i] = ok ? a.vs[block] : 0.f;
     }
   };
 
@@ -505,21 +567,25 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
     v_at[i] = row * D + 16 * ((col * kV / 16) ^ chunk_swz<D>(row)) + col * kV % 16;
   }
 
+  float ksc[4], vsc[4];
+  auto scales = [&](int64_t t0) {
+    const int l = (static_cast<int>(t0 % 1024) + part * kPaTile) / 16;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      ksc[g] = pg.ks_of(l + g);
+      vsc[g] = pg.vs_of(l + g);
+    }
+  };
   if (most > 0) {
-    load_ids(0);
+    pg.ask(a, table, group_at(0));
+    pg.take(a, group_at(0), head, D);
+    pg.ask(a, table, group_at(1024));
     load_tile(0, 0);
-    load_ids(kPos);
   }
   int buf = 0;
   for (int64_t t0 = 0; t0 < most; t0 += kPos, buf ^= 1) {
     const bool edge_step = !INT8 && t0 + kPos > seen(unit * kRows);  // some row does not see all of it
-    if (lane == 0) {
-#pragma unroll
-      for (int i = 0; i < KVS; ++i) {
-        scale[buf][0][wave + kPaWaves * i] = ks[i];
-        scale[buf][1][wave + kPaWaves * i] = vs[i];
-      }
-    }
+    scales(t0);
     if (edge_step && tid < kPos / 32) nan_at[buf][tid] = 0;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -540,8 +606,11 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
       __syncthreads();
     }
     if (t0 + kPos < most) {
+      if ((t0 + kPos) % 1024 == 0) {
+        pg.take(a, group_at(t0 + kPos), head, D);
+        pg.ask(a, table, group_at(t0 + kPos + 1024));
+      }
       load_tile(t0 + kPos, buf ^ 1);
-      load_ids(t0 + 2 * kPos);
     }
     const int64_t t1 = t0 + part * kPaTile;
     if (t1 >= mine) continue;
@@ -562,12 +631,6 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
     float x[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) x[i] = s[i >> 4][i & 15];
-    float ksc[4], vsc[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      ksc[g] = scale[buf][0][4 * part + g];
-      vsc[g] = scale[buf][1][4 * part + g];
-    }
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       if (!(ksc[g] > 0.f)) {  // the largest score is the largest product only for scales above 0
@@ -605,7 +668,7 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
     mt = fmaxf(mt, __shfl_xor(mt, 32));
     // m may lag the largest score by 2^8: of 32 rows some find a larger one in most
     // tiles, and the sums have the range
-    if (__any(mt > m + 8.f)) {
+    if (__builtin_amdgcn_ballot_w64(mt > m + 8.f) != 0) {
       const float mn = fmaxf(m, mt);
       const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       l *= f;
