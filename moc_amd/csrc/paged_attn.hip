@@ -29,7 +29,8 @@ constexpr int kPaWaves = 4;
 constexpr int kPaThreads = 64 * kPaWaves;
 constexpr int kPaTile = 64;  // positions per wave and step
 constexpr int kPaMaxSplits = 1024;
-constexpr int kPaFew = 16;   // rows of a sequence and key head up to which paged_attn_kernel takes it
+constexpr int kPaFew = 16;   // rows of a sequence and key head up to which paged_attn_kernel takes it,
+constexpr int kPaAll = 256;  // rows of a ragged batch up to which it takes all: 2.5 us for a launch without work
 
 struct PagedAttnArgs {
   PagedSeqs s;
@@ -41,6 +42,7 @@ struct PagedAttnArgs {
   const float *ks, *vs;
   int pages, log_page, heads, kv_heads, group;
   float c2;      // scale log2(e)
+  int few;       // rows of a sequence for paged_attn_kernel, more for paged_wide_kernel
   int chunk, splits;
   float* part_o;    // [tiles][kv_heads][16 rows][splits][D]
   float2* part_ml;  // [tiles][kv_heads][16 rows][splits]: largest score, sum
@@ -112,7 +114,7 @@ __device__ __forceinline__ bool has_nan_code(uint32_t w) {
 }
 
 template <int D, bool INT8>
-__global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kPaThreads, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_attn_kernel(PagedAttnArgs a) {
   constexpr int kLoads = D / 64;     // 16-byte loads of a K row per lane
   constexpr int kVDims = D / 16;     // dimensions of V per lane
   constexpr int kVWords = kVDims / 4;
@@ -131,7 +133,9 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
     sp.n = 1;
     sp.len = a.s.lens[sp.seq];
   } else {
-    sp = find_unit(a.s, blockIdx.x, [group](int n, int64_t) { return n * group <= kPaFew ? 1 : 0; });
+    sp = find_unit(a.s, blockIdx.x, [group, few = a.few](int n, int64_t) {
+      return n * group <= few ? (n * group + 15) / 16 : 0;
+    });
     if (sp.seq < 0) return;
   }
   sp = uniform(sp);
@@ -398,7 +402,9 @@ __global__ __launch_bounds__(kPaThreads) void paged_join_kernel(PagedAttnArgs a)
     sp.unit = blockIdx.x - sp.seq * tiles;
     sp.n = 1;
   } else {
-    sp = find_unit(a.s, blockIdx.x, [group](int n, int64_t) { return n * group <= kPaFew ? 1 : 0; });
+    sp = find_unit(a.s, blockIdx.x, [group, few = a.few](int n, int64_t) {
+      return n * group <= few ? (n * group + 15) / 16 : 0;
+    });
     if (sp.seq < 0) return;
   }
   const int r = sp.unit * 16 + row, token = r / group, sub = r - token * group;
@@ -498,8 +504,8 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5, part = wave / kGroups;
   const int head = blockIdx.x % a.kv_heads, lp = a.log_page, page = 1 << lp, group = a.group;
-  const SeqSpan sp = uniform(find_unit(a.s, blockIdx.x / a.kv_heads, [group](int n, int64_t) {
-    return n * group > kPaFew ? (n * group + kRows - 1) / kRows : 0;
+  const SeqSpan sp = uniform(find_unit(a.s, blockIdx.x / a.kv_heads, [group, few = a.few](int n, int64_t) {
+    return n * group > few ? (n * group + kRows - 1) / kRows : 0;
   }));
   if (sp.seq < 0) return;
   // the last rows, which see most, first
@@ -783,11 +789,15 @@ namespace {
 // paged_attn_kernel's chunks of the positions: enough workgroups for the CUs,
 // whole steps.
 struct Plan {
-  int64_t tiles, chunk, splits;
+  int64_t tiles, chunk, splits, few;
 };
 Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t kv_heads, int64_t room) {
   Plan p;
-  p.tiles = ragged ? (group <= kPaFew ? std::min(seqs, tokens) : 0) : seqs * ((group + 15) / 16);
+  const int64_t rows = tokens * group;
+  p.few = !ragged ? group : rows <= kPaAll ? kPaAll : kPaFew;
+  p.tiles = !ragged ? seqs * ((group + 15) / 16)
+            : p.few == kPaAll ? rows / 16 + std::min(seqs, tokens)
+            : group <= kPaFew ? std::min(seqs, tokens) : 0;
   const int64_t step = kPaTile * kPaWaves;
   const int64_t want =
       std::min<int64_t>(kPaMaxSplits, std::max<int64_t>(1, 4LL * cu_count() / std::max<int64_t>(1, p.tiles * kv_heads)));
@@ -853,11 +863,12 @@ extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_l
   a.c2 = scale * 1.4426950408889634f;
   a.chunk = static_cast<int>(std::min<int64_t>(p.chunk, 1 << 30));
   a.splits = static_cast<int>(p.splits);
+  a.few = static_cast<int>(p.few);
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + p.tiles * kv_heads * 16 * p.splits * head_dim);
   hipStream_t st = as_stream(stream);
   int rc = MOC_OK;
-  if (cu != nullptr && tokens * group > kPaFew) {
+  if (cu != nullptr && p.few == kPaFew) {
     // 64 rows a workgroup where 128 would leave CUs without one
     const bool half = tokens * group / 128 * kv_heads < 2 * cu_count();
     const int64_t units = tokens * group / (half ? 64 : 128) + std::min(seqs, tokens);
