@@ -1,0 +1,172 @@
+"""Decode of a batch of sequences with a DecoderModel over a paged 8-bit cache:
+ragged prompts in one forward, then one token a sequence and step, drawn with
+temperature, top-k, top-p and min-p.  The reference decodes one sequence
+greedily over a static bf16 cache (benchmark_decode.py:366-420,
+moc_amd/inference/decode_model.py); layers, weights and FFN forms are those.
+
+A step of a layer: norm, q/k/v projection, K.paged_append (RoPE, keys and values
+into the pages), K.paged_attention, out_proj, residual, then the FFN half.  A
+whole step, the draw included, is captured in one HIP graph: the sequences'
+lengths, page tables and tokens are device buffers that it reads.
+"""
+from __future__ import annotations
+
+import math
+from typing import Sequence
+
+import torch
+
+from .. import kernels as K
+from .decode_model import DecoderModel
+
+
+class BatchDecoder:
+    """`slots` sequences over one pool of pages for each layer.
+
+    codes: float8_e4m3fn or int8, what keys and values are held in; page: tokens a
+    page (a power of two from 16 to 256); pages: of the pool, by default enough
+    for every slot at the model's max_seq."""
+
+    def __init__(self, model: DecoderModel, slots: int, *, page: int = 64, pages: int | None = None,
+                 codes: torch.dtype = torch.float8_e4m3fn):
+        cfg, w = model.cfg, model.embed.weight
+        if w.dtype != torch.bfloat16:
+            raise ValueError(f"BatchDecoder runs bf16 models, got {w.dtype}")
+        if slots < 1:
+            raise ValueError("BatchDecoder: at least one slot")
+        width = -(-cfg.max_seq // page)
+        self.model, self.slots, self.page = model, slots, page
+        self.pages = slots * width if pages is None else pages
+        self.heads, self.head_dim = cfg.heads, cfg.hidden // cfg.heads
+        self.kv = [K.paged_kv(self.pages, self.heads, page, self.head_dim, dtype=codes, device=w.device)
+                   for _ in model.layers]
+        zeros = lambda *s, dtype=torch.int32: torch.zeros(*s, dtype=dtype, device=w.device)  # noqa: E731
+        self.table, self.lens = zeros(slots, width), zeros(slots)
+        self.live = zeros(slots)                       # 1: the slot takes a token a step
+        self.tokens = zeros(slots, dtype=torch.int64)  # the last token of each
+        self.release()
+
+    def release(self) -> None:
+        """Every page back to the pool, every slot out of use."""
+        self._free = list(range(self.pages - 1, -1, -1))
+        self._held: list[list[int]] = [[] for _ in range(self.slots)]
+        self._live = [False] * self.slots
+        self._upload()
+        self.lens.zero_()
+
+    def _upload(self) -> None:
+        rows = [h + [0] * (self.table.shape[1] - len(h)) for h in self._held]
+        self.table.copy_(torch.tensor(rows, dtype=torch.int32))
+        self.live.copy_(torch.tensor(self._live, dtype=torch.int32))
+
+    def reserve(self, tokens: Sequence[int]) -> None:
+        """Pages for tokens[slot] tokens of each slot (0: out of use)."""
+        if len(tokens) != self.slots:
+            raise ValueError(f"reserve: {self.slots} slots, got {len(tokens)}")
+        if max(tokens) > self.model.cfg.max_seq:
+            raise ValueError(f"reserve: {max(tokens)} tokens, the model has {self.model.cfg.max_seq} positions")
+        more = [max(-(-n // self.page) - len(h), 0) for n, h in zip(tokens, self._held)]
+        if sum(more) > len(self._free):
+            raise ValueError(f"reserve: {sum(more)} pages wanted, {len(self._free)} are free")
+        for held, m in zip(self._held, more):
+            held.extend(self._free.pop() for _ in range(m))
+        self._live = [n > 0 for n in tokens]
+        self._upload()
+
+    @torch.no_grad()
+    def forward(self, tokens: torch.Tensor, cu: torch.Tensor | None = None) -> torch.Tensor:
+        """Hidden states [tokens, hidden] of new tokens whose sequences' lengths
+        (self.lens, these counted) are set; cu as in K.paged_append."""
+        x = self.model.embed(tokens)
+        scale = 1.0 / math.sqrt(self.head_dim)
+        for layer, kv in zip(self.model.layers, self.kv):
+            a = layer.attn
+            q, k, v = a.qkv_proj(layer.attn_norm(x)).view(-1, 3 * self.heads, self.head_dim).split(self.heads, dim=1)
+            q = K.paged_append(q, k, v, a.rope_cos, a.rope_sin, kv, self.table, self.lens, cu)
+            o = K.paged_attention(q, kv, self.table, self.lens, cu, scale=scale)
+            x = x + a.out_proj(o.flatten(1))
+            if layer.fuse:
+                x = layer.ffn.fused_decode_residual(x, layer.ffn_norm.weight, layer.ffn_norm.eps)
+            else:
+                x = x + layer._ffn(layer.ffn_norm(x)[None])[0]
+        return x
+
+    @torch.no_grad()
+    def logits(self, x: torch.Tensor) -> torch.Tensor:
+        return self.model.lm_head(self.model.final_norm(x))
+
+    @torch.no_grad()
+    def prompt(self, prompts: Sequence[torch.Tensor], room: int = 0) -> torch.Tensor:
+        """Starts the slots with these prompts (1-D token ids, at least one token
+        each) and pages for `room` tokens more; logits [prompts, vocab] behind
+        their last tokens."""
+        n = [int(p.numel()) for p in prompts]
+        if not n or min(n) < 1 or len(n) > self.slots:
+            raise ValueError(f"prompt: 1 to {self.slots} prompts of at least one token")
+        empty = [0] * (self.slots - len(n))
+        self.release()
+        self.reserve([t + room for t in n] + empty)
+        self.lens.copy_(torch.tensor(n + empty, dtype=torch.int32))
+        cu = torch.tensor([0, *n, *empty], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(self.lens.device)
+        x = self.forward(torch.cat([p.reshape(-1) for p in prompts]).to(self.tokens.device), cu)
+        return self.logits(x.index_select(0, cu[1:len(n) + 1].long() - 1))
+
+    @torch.no_grad()
+    def step(self, u: torch.Tensor, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
+        """One token more of each live slot: self.tokens go in, are replaced by
+        the drawn ones (K.sample_tokens with the uniform numbers u [slots]) and
+        returned.  Slots out of use keep theirs."""
+        self.lens.add_(self.live)
+        logits = self.logits(self.forward(self.tokens))
+        drawn = K.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+        self.tokens.copy_(torch.where(self.live > 0, drawn, self.tokens))
+        return self.tokens
+
+    @torch.no_grad()
+    def generate(self, prompts: Sequence[torch.Tensor], length: int, *, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0,
+                 generator: torch.Generator | None = None, graph: bool = True) -> torch.Tensor:
+        """`length` tokens behind each prompt, int64 [prompts, length].  Settings
+        are numbers, or tensors [slots] (K.sample_tokens); temperature 0 is
+        greedy.  graph: the step is captured once and replayed."""
+        if length < 1:
+            raise ValueError("generate: at least one token")
+        n, dev = len(prompts), self.lens.device
+        u = torch.rand(length, self.slots, generator=generator, device=dev)
+        settings = (temperature, top_k, top_p, min_p)
+        first = self.prompt(prompts, room=length - 1)
+        of = [s[:n] if isinstance(s, torch.Tensor) else s for s in settings]
+        self.tokens[:n] = K.sample_tokens(first, u[0, :n], *of)
+        out = torch.empty(n, length, dtype=torch.int64, device=dev)
+        out[:, 0] = self.tokens[:n]
+        now, step = torch.empty_like(u[0]), None
+        if graph and length > 2:
+            step = self._capture(now, settings)
+        for i in range(1, length):
+            now.copy_(u[i])
+            if step is None:
+                self.step(now, *settings)
+            else:
+                step.replay()
+            out[:, i] = self.tokens[:n]
+        return out
+
+    def _capture(self, u: torch.Tensor, settings) -> torch.cuda.CUDAGraph:
+        """The step as a HIP graph.  The warm-up runs change nothing: with no
+        live slot and lengths of 0 no key is stored and no token replaced."""
+        self.model.freeze_for_compile()
+        lens, live = self.lens.clone(), self.live.clone()
+        self.lens.zero_()
+        self.live.zero_()
+        side = torch.cuda.Stream(device=u.device)
+        side.wait_stream(torch.cuda.current_stream(u.device))
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                self.step(u, *settings)
+        torch.cuda.current_stream(u.device).wait_stream(side)
+        torch.cuda.synchronize(u.device)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            self.step(u, *settings)
+        self.lens.copy_(lens)
+        self.live.copy_(live)
+        return graph
