@@ -759,7 +759,7 @@ int64_t moc_paged_attention_workspace_size(int64_t tokens, int64_t seqs, int rag
                                            int64_t kv_heads, int64_t head_dim, int64_t page, int64_t width);
 
 /* out = softmax(scale q K^T) V of each row of q over the positions up to its own;
- * q head h reads kv head h / (q_heads / kv_heads).  Scores, softmax and sums in
+ * q head h reads kv head h / (q_heads / kv_heads).  page * width: at most 2^30.  Scores, softmax and sums in
  * f32; probabilities go to the second product as bf16.  A row that sees no
  * position is 0; one that sees a position without a page is NaN. */
 int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_lh, int64_t tokens, int64_t q_heads,

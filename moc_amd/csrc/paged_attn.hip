@@ -46,6 +46,10 @@ struct PagedAttnArgs {
   int chunk, splits;
   float* part_o;    // [tiles][kv_heads][16 rows][splits][D]
   float2* part_ml;  // [tiles][kv_heads][16 rows][splits]: largest score, sum
+  uint32_t wide_chunk;  // paged_wide_kernel's
+  int wide_splits;
+  float* wide_o;                // [units][kv_heads][128 rows][splits][D]
+  float2* wide_ml;
 };
 
 // Two codes (bytes 2 H, 2 H + 1 of w) as bf16.
@@ -463,190 +467,184 @@ __global__ __launch_bounds__(kPaThreads) void paged_join_kernel(PagedAttnArgs a)
 // ------------------------------------------------------------- many rows
 // Sequences with more than 16 rows a key head (prompts, chunks of them, groups of
 // several drafted tokens): v_mfma_f32_32x32x16_bf16 in the same orientation, 32
-// rows a wave.  The cache's tiles of 64 positions go to LDS as codes, straight from
-// memory (16 positions of a page are 16 D bytes in a row), one step ahead; every
-// wave makes bf16 of them for itself, which halves the LDS bytes of a bf16 tile.
-// 16-byte chunk c of row r lies in slot c ^ chunk_swz(r): the b128 reads of K, a
-// row a lane, then meet all banks, and V's rows are read whole.
-//
-// KVS of the four waves share 32 rows and take every KVS'th tile (their sums join
-// through LDS): 128 / KVS rows a workgroup.  Bound by VALU work beside the MFMAs:
-// per 64 positions and 32 rows 32 MFMAs of 32 clocks, about 330 VALU instructions
-// and 32 exponentials.
+// rows a wave, 128 a workgroup over the same tiles of 64 positions.  Every thread
+// takes its part of the next tile's codes into registers while this one is worked
+// on, and stores them to LDS as bf16: a conversion for all waves, where each wave
+// converting for itself took 128 instructions a tile and as many permutations to
+// transpose V (4 x 1024 new rows over 4096, 16 heads of 128: 279 us, now 236).  V
+// is read transposed (ds_read_b64_tr_b16) under the order of positions that the
+// scores leave in a lane (attn.hip).  16-byte chunk c of a row of 64 tile positions
+// lies in slot c ^ row_swz(row).  Bound by VALU work and LDS reads beside the
+// MFMAs: per 64 positions and 32 rows 32 MFMAs of 32 clocks, 32 KB of LDS, 32
+// exponentials and about 170 instructions: 709 TFLOP/s for 16 x 1024 rows.
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 
+// The transposing reads meet four rows in a row at four neighbouring chunks, K's
+// reads eight rows at one chunk: both fall on different banks.
 template <int D>
-__device__ __forceinline__ int chunk_swz(int r) {
-  return D == 64 ? (r >> 2) & 3 : D == 128 ? r & 7 : r & 15;
+__device__ __forceinline__ int row_swz(int r) {
+  return D == 64 ? 4 * ((r >> 1) & 1) + ((r >> 2) & 3) : 4 * (r & 3) + ((r >> 2) & 3);
 }
 
-// 16 bytes per lane from base + off to LDS bytes m0 + 16 lane.  Counted by hand
-// (vmcnt): the compiler knows nothing of it.
-__device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint32_t m0) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %2"
-      :
-      : "s"(m0), "v"(off), "s"(base)
-      : "memory");
-}
+constexpr int kPaWide = 32 * kPaWaves;  // rows a workgroup
 
-template <int D, bool INT8, int KVS>
-__global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kernel(PagedAttnArgs a) {
-  constexpr int kGroups = kPaWaves / KVS;       // of 32 rows
-  constexpr int kRows = 32 * kGroups;
-  constexpr int kPos = kPaTile * KVS;           // positions a step
-  constexpr int kLd = D / 64;                   // 16-byte loads per lane of 16 positions
-  constexpr int kQ = D / 32, kV = D / 32;       // chunks of K per lane; dimensions of V per lane
-  __shared__ __attribute__((aligned(1024))) uint8_t tile[2][2][kPos * D];  // [step & 1][K, V]
-  __shared__ uint32_t nan_at[2][kPos / 32];  // positions whose V holds a NaN code
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 31, h = lane >> 5, part = wave / kGroups;
-  const int head = blockIdx.x % a.kv_heads, lp = a.log_page, page = 1 << lp, group = a.group;
-  const SeqSpan sp = uniform(find_unit(a.s, blockIdx.x / a.kv_heads, [group, few = a.few](int n, int64_t) {
-    return n * group > few ? (n * group + kRows - 1) / kRows : 0;
+__device__ __forceinline__ SeqSpan find_wide(const PagedAttnArgs& a, int unit) {
+  return uniform(find_unit(a.s, unit, [group = a.group, few = a.few](int n, int64_t) {
+    return n * group > few ? (n * group + kPaWide - 1) / kPaWide : 0;
   }));
+}
+
+template <int D, bool INT8>
+__global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kernel(PagedAttnArgs a) {
+  constexpr int kLd = D / 64;                 // 16-byte loads per lane of 16 positions
+  constexpr int kQ = D / 16, kV = D / 32;     // k steps of the scores, blocks of 32 dimensions
+  constexpr int kBytes = kPaTile * D * 2;
+  constexpr int kBufs = D <= 128 ? 2 : 1;     // two tiles of LDS: one barrier a tile
+  __shared__ __attribute__((aligned(1024))) char lds[kBufs][2][kBytes];
+  __shared__ uint32_t nan_at[kBufs][2];  // positions whose V holds a NaN code
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const int head = blockIdx.x % a.kv_heads, lp = a.log_page, group = a.group;
+  const SeqSpan sp = find_wide(a, blockIdx.x / a.kv_heads);
   if (sp.seq < 0) return;
   // the last rows, which see most, first
-  const int unit = (sp.n * group + kRows - 1) / kRows - 1 - sp.unit;
-  const int r0 = unit * kRows + (wave % kGroups) * 32, r = r0 + col, token = r / group, sub = r - token * group;
+  const int unit = (sp.n * group + kPaWide - 1) / kPaWide - 1 - sp.unit;
+  const int r0 = unit * kPaWide + wave * 32, r = r0 + col, token = r / group, sub = r - token * group;
   const bool live = token < sp.n;
   const int64_t room = static_cast<int64_t>(a.s.width) << lp, before = sp.len - sp.n;
-  const int64_t lim = live ? before + 1 + token : 0;
-  const bool lost = lim > room;
-  auto seen = [&](int row) { return min(max(before + 1 + min(row, sp.n * group - 1) / group, int64_t(0)), room); };
-  const int64_t most = seen(unit * kRows + kRows - 1);     // by any row of the workgroup
-  const int64_t mine = r0 < sp.n * group ? seen(r0 + 31) : 0;  // of the wave
-  const int64_t whole = r0 < sp.n * group ? seen(r0) : 0;      // by each row of the wave
+  const bool lost = live && before + 1 + token > room;
+  // a position, of less than 2^31, plus a tile's or a page group's offset: 32 bits
+  auto seen = [&](int row) {
+    return static_cast<uint32_t>(min(max(before + 1 + min(row, sp.n * group - 1) / group, int64_t(0)), room));
+  };
+  const uint32_t lim = live ? seen(r) : 0;
+  const uint32_t from = blockIdx.y * a.wide_chunk;  // a multiple of a tile
+  const uint32_t most = min(seen(unit * kPaWide + kPaWide - 1), from + a.wide_chunk);  // by any row of the workgroup
+  const uint32_t mine = r0 < sp.n * group ? seen(r0 + 31) : 0;  // of the wave
+  const uint32_t whole = r0 < sp.n * group ? seen(r0) : 0;      // by each row of the wave
+  const uint32_t first = seen(unit * kPaWide);                   // by each row of the workgroup
 
-  bf16x8_t qf[kQ][2];
+  bf16x8_t qf[kQ];
 #pragma unroll
-  for (int i = 0; i < kQ; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint4 t = make_uint4(0, 0, 0, 0);
-      if (live)
-        t = *reinterpret_cast<const uint4*>(a.q + (sp.row0 + token) * a.q_ld + (head * group + sub) * a.q_lh +
-                                            (2 * i + h) * 16 + j * 8);
-      qf[i][j] = __builtin_bit_cast(bf16x8_t, t);
-    }
-  float m = -INFINITY, l = 0.f, v_unit = 0.f;
+  for (int i = 0; i < kQ; ++i) {
+    uint4 t = make_uint4(0, 0, 0, 0);
+    if (live)
+      t = *reinterpret_cast<const uint4*>(a.q + (sp.row0 + token) * a.q_ld + (head * group + sub) * a.q_lh + 16 * i + 8 * h);
+    qf[i] = __builtin_bit_cast(bf16x8_t, t);
+  }
+  float m = -INFINITY, l = 0.f, v_unit = 0.f, unit_inv = 0.f;
   f32x16_t acc[kV];
 #pragma unroll
   for (int j = 0; j < kV; ++j) acc[j] = f32x16_t{};
   const int32_t* table = a.s.table + sp.seq * a.s.ld_table;
 
-  // staging: wave w takes the 16-position groups w, w + 4, ..: kLd loads of the
-  // whole wave each, lane l's chunk of row (1024 j + 16 l) / D of the group
-  uint32_t src[kLd];
+  // wave w stages positions 16 w .. of a tile: 16 D bytes in a row of the cache, load
+  // j of lane l is chunk 16 l % D / 16 of row (1024 j + 16 l) / D of them
+  Groups pg;  // lane l: positions 16 l .. of 1024 that begin at from or a multiple later
+  auto group_at = [&](uint32_t t0) { return t0 + 16 * lane < most ? int64_t(t0 + 16 * lane) : int64_t(-1); };
+  uint4 kr[kLd], vr[kLd];
+  auto load_tile = [&](uint32_t t0) {
+    if (t0 + 16 * wave >= most) return;  // nobody sees what the registers hold
+    const int64_t byte = pg.byte_of(static_cast<int>((t0 - from) % 1024) / 16 + wave);
 #pragma unroll
-  for (int j = 0; j < kLd; ++j) {
-    const int row = (1024 * j + 16 * lane) / D, c = 16 * lane % D / 16;
-    src[j] = row * D + 16 * (c ^ chunk_swz<D>(row));
-  }
-  const uint32_t lds0 = static_cast<uint32_t>(
-      (uintptr_t)((__attribute__((address_space(3))) const char*)(const void*)&tile[0][0][0]));
-  Groups pg;  // lane l: positions 16 l .. of 1024
-  auto group_at = [&](int64_t t0) { return t0 + 16 * lane < most ? t0 + 16 * lane : int64_t(-1); };
-  auto load_tile = [&](int64_t t0, int buf) {
-#pragma unroll
-    for (int i = 0; i < KVS; ++i) {
-      const int at = wave + kPaWaves * i;
-      if (t0 + 16 * at >= most) continue;  // what LDS holds there is not seen
-      const int64_t byte = pg.byte_of(static_cast<int>(t0 % 1024) / 16 + at);
-      const uint32_t dst = lds0 + (2 * buf * kPos + 16 * at) * D;
-#pragma unroll
-      for (int j = 0; j < kLd; ++j) to_lds16(a.kc + byte, src[j], dst + 1024 * j);
-#pragma unroll
-      for (int j = 0; j < kLd; ++j) to_lds16(a.vc + byte, src[j], dst + kPos * D + 1024 * j);
+    for (int j = 0; j < kLd; ++j) {
+      kr[j] = *reinterpret_cast<const uint4*>(a.kc + byte + 1024 * j + 16 * lane);
+      vr[j] = *reinterpret_cast<const uint4*>(a.vc + byte + 1024 * j + 16 * lane);
     }
   };
-
-  // LDS bytes of a tile that this lane reads
-  uint32_t k_at[kQ], v_at[8];
 #pragma unroll
-  for (int i = 0; i < kQ; ++i) k_at[i] = col * D + 16 * ((2 * i + h) ^ chunk_swz<D>(col));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = 4 * h + (i & 3) + 8 * (i >> 2);
-    v_at[i] = row * D + 16 * ((col * kV / 16) ^ chunk_swz<D>(row)) + col * kV % 16;
+  for (int j = 0; j < kLd; ++j) kr[j] = vr[j] = make_uint4(0, 0, 0, 0);
+  if (from < most) {
+    pg.ask(a, table, group_at(from));
+    pg.take(a, group_at(from), head, D);
+    pg.ask(a, table, group_at(from + 1024));
+    load_tile(from);
   }
+  // LDS bytes that this lane reads: of K the row col (+ 32), k step i at k_at ^ 32 i;
+  // of V by transposing reads the rows vrow and vrow + 8 (+ 16 g), block j of 32
+  // dimensions at v_lo, v_hi ^ 64 j
+  const uint32_t k_at = col * (D * 2) + 16 * (h ^ row_swz<D>(col));
+  const int vi = lane & 15, vrow = 4 * (lane >> 5) + (vi >> 2), vch = 2 * ((lane >> 4) & 1) + ((vi >> 1) & 1);
+  const uint32_t v_lo = vrow * (D * 2) + 16 * (vch ^ row_swz<D>(vrow)) + 8 * (vi & 1);
+  const uint32_t v_hi = (vrow + 8) * (D * 2) + 16 * (vch ^ row_swz<D>(vrow + 8)) + 8 * (vi & 1);
 
-  float ksc[4], vsc[4];
-  auto scales = [&](int64_t t0) {
-    const int l = (static_cast<int>(t0 % 1024) + part * kPaTile) / 16;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      ksc[g] = pg.ks_of(l + g);
-      vsc[g] = pg.vs_of(l + g);
-    }
-  };
-  if (most > 0) {
-    pg.ask(a, table, group_at(0));
-    pg.take(a, group_at(0), head, D);
-    pg.ask(a, table, group_at(1024));
-    load_tile(0, 0);
-  }
   int buf = 0;
-  for (int64_t t0 = 0; t0 < most; t0 += kPos, buf ^= 1) {
-    const bool edge_step = !INT8 && t0 + kPos > seen(unit * kRows);  // some row does not see all of it
-    scales(t0);
-    if (edge_step && tid < kPos / 32) nan_at[buf][tid] = 0;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (edge_step) {
-      // 0 times a NaN code would reach rows that do not see it
+  for (uint32_t t0 = from; t0 < most; t0 += kPaTile, buf ^= kBufs - 1) {
+    const bool edge_step = !INT8 && t0 + kPaTile > first;  // some row does not see all of it
+    float ksc[4], vsc[4];
+    {
+      const int g0 = static_cast<int>((t0 - from) % 1024) / 16;
 #pragma unroll
-      for (int i = 0; i < KVS; ++i)
-#pragma unroll
-        for (int j = 0; j < kLd; ++j) {
-          const int row = 16 * (wave + kPaWaves * i) + (1024 * j + 16 * lane) / D;
-          uint4* q = reinterpret_cast<uint4*>(&tile[buf][1][16 * (wave + kPaWaves * i) * D + 1024 * j + 16 * lane]);
-          const uint4 v = *q;
-          if (has_nan_code(v.x) || has_nan_code(v.y) || has_nan_code(v.z) || has_nan_code(v.w)) {
-            if (t0 + row < most) atomicOr(&nan_at[buf][row >> 5], 1u << (row & 31));
-            *q = make_uint4(0, 0, 0, 0);
-          }
-        }
-      __syncthreads();
-    }
-    if (t0 + kPos < most) {
-      if ((t0 + kPos) % 1024 == 0) {
-        pg.take(a, group_at(t0 + kPos), head, D);
-        pg.ask(a, table, group_at(t0 + kPos + 1024));
+      for (int g = 0; g < 4; ++g) {
+        ksc[g] = pg.ks_of(g0 + g);
+        vsc[g] = pg.vs_of(g0 + g);
       }
-      load_tile(t0 + kPos, buf ^ 1);
     }
-    const int64_t t1 = t0 + part * kPaTile;
-    if (t1 >= mine) continue;
-    const uint8_t* kt = &tile[buf][0][part * kPaTile * D];
-    const uint8_t* vt = &tile[buf][1][part * kPaTile * D];
+    if (kBufs == 1) __syncthreads();  // the tile before is read
+    if (edge_step) {
+      if (tid < 2) nan_at[buf][tid] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kLd; ++j)
+        // 0 times a NaN code would reach rows that do not see it
+        if (has_nan_code(vr[j].x) || has_nan_code(vr[j].y) || has_nan_code(vr[j].z) || has_nan_code(vr[j].w)) {
+          const int row = 16 * wave + (1024 * j + 16 * lane) / D;
+          if (t0 + row < most) atomicOr(&nan_at[buf][row >> 5], 1u << (row & 31));
+          vr[j] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    char* kt = lds[buf][0];
+    char* vt = lds[buf][1];
+#pragma unroll
+    for (int j = 0; j < kLd; ++j) {
+      const int row = 16 * wave + (1024 * j + 16 * lane) / D, c = 2 * (16 * lane % D / 16);
+      const uint4 k = kr[j], v = vr[j];
+      const int lo = row * (D * 2) + 16 * (c ^ row_swz<D>(row)), hi = row * (D * 2) + 16 * ((c + 1) ^ row_swz<D>(row));
+      *reinterpret_cast<bf16x8_t*>(kt + lo) = eight_bf16<INT8>(k.x, k.y);
+      *reinterpret_cast<bf16x8_t*>(kt + hi) = eight_bf16<INT8>(k.z, k.w);
+      *reinterpret_cast<bf16x8_t*>(vt + lo) = eight_bf16<INT8>(v.x, v.y);
+      *reinterpret_cast<bf16x8_t*>(vt + hi) = eight_bf16<INT8>(v.z, v.w);
+    }
+    if (t0 + kPaTile < most) {
+      if ((t0 + kPaTile - from) % 1024 == 0) {
+        pg.take(a, group_at(t0 + kPaTile), head, D);
+        pg.ask(a, table, group_at(t0 + kPaTile + 1024));
+      }
+      load_tile(t0 + kPaTile);
+    }
+    __syncthreads();
+    if (t0 >= mine) continue;
     f32x16_t s[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[b] = f32x16_t{};
+    for (int b = 0; b < 2; ++b) s[b] = f32x16_t{};
 #pragma unroll
-      for (int i = 0; i < kQ; ++i) {
-        const uint4 t = *reinterpret_cast<const uint4*>(kt + 32 * b * D + k_at[i]);
-        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_bf16<INT8>(t.x, t.y), qf[i][0], s[b], 0, 0, 0);
-        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight_bf16<INT8>(t.z, t.w), qf[i][1], s[b], 0, 0, 0);
+    for (int i = 0; i < kQ; ++i)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const bf16x8_t k = *reinterpret_cast<const bf16x8_t*>(kt + (k_at ^ (32u * i)) + b * (32 * D * 2));
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[i], s[b], 0, 0, 0);
       }
-    }
     // x[i]: position 32 (i >> 4) + 8 ((i >> 2) & 3) + 4 h + (i & 3), group i >> 3
     float x[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) x[i] = s[i >> 4][i & 15];
+    bool usual = true;  // scales above 0: the largest score is the largest product
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      if (!(ksc[g] > 0.f)) {  // the largest score is the largest product only for scales above 0
+    for (int g = 0; g < 4; ++g) usual = usual && ksc[g] > 0.f;
+    if (!usual) {
+      asm volatile("");  // a branch, not 32 selects in every tile
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
         const float sign = ksc[g] < 0.f ? -1.f : 1.f;
         ksc[g] = ksc[g] == 0.f ? 1e-30f : fabsf(ksc[g]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[8 * g + i] *= sign;
       }
-    if (t1 + kPaTile > whole) {
-      uint32_t nans[2] = {edge_step ? nan_at[buf][2 * part] : 0u, edge_step ? nan_at[buf][2 * part + 1] : 0u};
+    }
+    if (t0 + kPaTile > whole) {
+      uint32_t nans[2] = {edge_step ? nan_at[buf][0] : 0u, edge_step ? nan_at[buf][1] : 0u};
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         if (!(fabsf(vsc[g]) <= 3.4028234e38f) || !(ksc[g] <= 3.4028234e38f)) {
@@ -657,11 +655,10 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
       for (int i = 0; i < 32; ++i) {
         const int at = 8 * ((i >> 2) & 3) + 4 * h + (i & 3);
         if ((nans[i >> 4] >> at) & 1) x[i] = __uint_as_float(0x7FC00000u);
-        if (t1 + 32 * (i >> 4) + at >= lim) x[i] = -INFINITY;
+        if (t0 + 32 * (i >> 4) + at >= lim) x[i] = -INFINITY;
       }
     } else if (edge_step) {
-      const uint32_t nans[2] = {nan_at[buf][2 * part], nan_at[buf][2 * part + 1]};
-      if (nans[0] | nans[1]) l = __uint_as_float(0x7FC00000u);  // every row of the wave sees it
+      if (nan_at[buf][0] | nan_at[buf][1]) l = __uint_as_float(0x7FC00000u);  // every row of the wave sees it
     }
     float mt = -INFINITY;
 #pragma unroll
@@ -692,11 +689,14 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
       }
     // V's scale goes onto the probabilities, relative to the first one: pages of
     // one size of values share theirs
-    if (v_unit == 0.f) v_unit = vsc[0] > 0.f && vsc[0] <= 3.4028234e38f ? vsc[0] : 1.f;
+    if (v_unit == 0.f) {
+      v_unit = vsc[0] >= 1e-30f && vsc[0] <= 1e30f ? vsc[0] : 1.f;
+      unit_inv = 1.0f / v_unit;
+    }
     if (vsc[0] != v_unit || vsc[1] != v_unit || vsc[2] != v_unit || vsc[3] != v_unit) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const float f = vsc[g] / v_unit;
+        const float f = vsc[g] * unit_inv;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[8 * g + i] *= f;
       }
@@ -709,75 +709,83 @@ __global__ __launch_bounds__(kPaThreads, D == 256 ? 1 : 2) void paged_wide_kerne
         pb[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(
                                                  (cvt_f32x2_t){x[8 * g + 2 * i], x[8 * g + 2 * i + 1]}, cvt_bf16x2_t));
       const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, make_uint4(pb[0], pb[1], pb[2], pb[3]));
-      // positions 16 g + 4 h + {0 .. 3, 8 .. 11}, kV neighbouring dimensions
-      constexpr int kW = kV >= 4 ? kV / 4 : 1;
-      uint32_t v[8][kW];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint8_t* src = vt + 16 * g * D + v_at[i];
-        if constexpr (kV == 2) {
-          v[i][0] = *reinterpret_cast<const uint16_t*>(src);
-        } else if constexpr (kV == 4) {
-          v[i][0] = *reinterpret_cast<const uint32_t*>(src);
-        } else {
-          const uint2 t = *reinterpret_cast<const uint2*>(src);
-          v[i][0] = t.x;
-          v[i][1] = t.y;
-        }
+      for (int j = 0; j < kV; ++j) {
+        const char* const lo = vt + (v_lo ^ (64u * j)) + 16 * g * (D * 2);
+        const char* const hi = vt + (v_hi ^ (64u * j)) + 16 * g * (D * 2);
+        const i16x4_t v[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)lo),
+                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)hi)};
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), pf, acc[j], 0, 0, 0);
       }
-#pragma unroll
-      for (int w = 0; w < kW; ++w)
-#pragma unroll
-        for (int jj = 0; jj < (kV == 2 ? 1 : 2); ++jj) {
-          uint32_t z[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) z[i] = jj ? two_bf16<INT8, true>(v[i][w]) : two_bf16<INT8, false>(v[i][w]);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t sel = e ? 0x07060302u : 0x05040100u;
-            const bf16x8_t vf = __builtin_bit_cast(
-                bf16x8_t, make_uint4(__builtin_amdgcn_perm(z[1], z[0], sel), __builtin_amdgcn_perm(z[3], z[2], sel),
-                                     __builtin_amdgcn_perm(z[5], z[4], sel), __builtin_amdgcn_perm(z[7], z[6], sel)));
-            const int j = 4 * w + 2 * jj + e;
-            acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, acc[j], 0, 0, 0);
-          }
-        }
     }
   }
   l += __shfl_xor(l, 32);
   if (lost) l = __uint_as_float(0x7FC00000u);
-  if constexpr (KVS == 2) {
-    // the second half of the waves hands its sums to the first
-    float* po = reinterpret_cast<float*>(tile) + (wave % kGroups) * 32 * D;
-    __shared__ float2 ml[kGroups][32];
-    __syncthreads();
-    if (part == 1) {
-      if (h == 0) ml[wave % kGroups][col] = make_float2(m, l);
-#pragma unroll
-      for (int j = 0; j < kV; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) po[(j * 16 + i) * 64 + lane] = acc[j][i] * v_unit;
-    }
-    __syncthreads();
-    if (part == 1) return;
-    const float2 o = ml[wave % kGroups][col];
-    const float mn = fmaxf(m, o.x), base = mn == -INFINITY ? 0.f : mn;
-    const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(o.x - base);
-    l = l * f0 + o.y * f1;
+  if (!live) return;
+  if (a.wide_splits > 1) {
+    const int64_t slot = (static_cast<int64_t>(blockIdx.x) * kPaWide + wave * 32 + col) * a.wide_splits + blockIdx.y;
+    if (h == 0) a.wide_ml[slot] = make_float2(m, l);
+    if (m == -INFINITY) return;  // nothing here
+    float* o = a.wide_o + slot * D;
 #pragma unroll
     for (int j = 0; j < kV; ++j)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[j][i] = acc[j][i] * (f0 * v_unit) + po[(j * 16 + i) * 64 + lane] * f1;
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(o + 32 * j + 2 * i + 4 * h) = make_float4(
+            acc[j][i] * v_unit, acc[j][i + 1] * v_unit, acc[j][i + 2] * v_unit, acc[j][i + 3] * v_unit);
+    return;
   }
-  if (!live) return;
-  const float inv = l == 0.f ? 0.f : (KVS == 1 ? v_unit : 1.f) / l;
+  const float inv = l == 0.f ? 0.f : v_unit / l;
   uint16_t* o = a.o + (sp.row0 + token) * a.o_ld + (head * group + sub) * a.o_lh;
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+  for (int j = 0; j < kV; ++j)
 #pragma unroll
-    for (int j = 0; j < kV; j += 2)
-      *reinterpret_cast<uint32_t*>(o + (8 * (i >> 2) + 4 * h + (i & 3)) * kV + j) = __builtin_bit_cast(
-          uint32_t, __builtin_convertvector((cvt_f32x2_t){acc[j][i] * inv, acc[j + 1][i] * inv}, cvt_bf16x2_t));
+    for (int i = 0; i < 16; i += 4) {
+      const cvt_bf16x2_t lo = __builtin_convertvector((cvt_f32x2_t){acc[j][i] * inv, acc[j][i + 1] * inv}, cvt_bf16x2_t);
+      const cvt_bf16x2_t hi = __builtin_convertvector((cvt_f32x2_t){acc[j][i + 2] * inv, acc[j][i + 3] * inv}, cvt_bf16x2_t);
+      *reinterpret_cast<uint2*>(o + 32 * j + 2 * i + 4 * h) =
+          make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+    }
+}
+
+// o of paged_wide_kernel's rows from their chunks: 8 dimensions of a row a thread.
+template <int D>
+__global__ __launch_bounds__(kPaThreads) void paged_wide_join_kernel(PagedAttnArgs a) {
+  constexpr int kLanes = D / 8, kAtOnce = kPaThreads / kLanes;
+  const int group = a.group, c = threadIdx.x % kLanes;
+  const int unit = blockIdx.x / a.kv_heads, head = blockIdx.x - unit * a.kv_heads;
+  const SeqSpan sp = find_wide(a, unit);
+  if (sp.seq < 0) return;
+  const int row = blockIdx.y * kAtOnce + threadIdx.x / kLanes;
+  const int r = ((sp.n * group + kPaWide - 1) / kPaWide - 1 - sp.unit) * kPaWide + row;
+  const int token = r / group, sub = r - token * group;
+  if (token >= sp.n) return;
+  const int64_t slot = (static_cast<int64_t>(blockIdx.x) * kPaWide + row) * a.wide_splits;
+  float m = -INFINITY;
+  for (int i = 0; i < a.wide_splits; ++i) m = fmaxf(m, a.wide_ml[slot + i].x);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float v[8] = {};
+  for (int i = 0; i < a.wide_splits; ++i) {
+    const float2 t = a.wide_ml[slot + i];
+    if (t.x == -INFINITY) {
+      l += t.y;  // 0, or NaN where a chunk lies outside the cache
+      continue;
+    }
+    const float f = __builtin_amdgcn_exp2f(t.x - base);
+    l += t.y * f;
+    const float4* p = reinterpret_cast<const float4*>(a.wide_o + (slot + i) * D + 8 * c);
+    const float4 x = p[0], y = p[1];
+    v[0] += x.x * f; v[1] += x.y * f; v[2] += x.z * f; v[3] += x.w * f;
+    v[4] += y.x * f; v[5] += y.y * f; v[6] += y.z * f; v[7] += y.w * f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((cvt_f32x2_t){v[2 * i] * inv, v[2 * i + 1] * inv}, cvt_bf16x2_t));
+  uint16_t* o = a.o + (sp.row0 + token) * a.o_ld + (head * group + sub) * a.o_lh + 8 * c;
+  *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 }  // namespace
@@ -788,10 +796,14 @@ using namespace moc;
 namespace {
 // paged_attn_kernel's chunks of the positions: enough workgroups for the CUs,
 // whole steps.
+constexpr int64_t kWidePlaces = 4, kWideLeast = 512;  // workgroups a CU, positions
+constexpr int64_t kPaRoom = 1LL << 30;                 // positions of a table: 32-bit arithmetic
 struct Plan {
   int64_t tiles, chunk, splits, few;
+  int64_t units, wide_chunk, wide_splits;
+  int64_t few_floats, wide_floats;  // of partial sums
 };
-Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t kv_heads, int64_t room) {
+Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t kv_heads, int64_t dim, int64_t room) {
   Plan p;
   const int64_t rows = tokens * group;
   p.few = !ragged ? group : rows <= kPaAll ? kPaAll : kPaFew;
@@ -805,15 +817,27 @@ Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t k
   const int64_t per = std::max<int64_t>(1, (steps + want - 1) / want);
   p.chunk = per * step;
   p.splits = (steps + per - 1) / per;
+  p.few_floats = p.splits > 1 ? p.tiles * kv_heads * 16 * p.splits * dim : 0;
+  // paged_wide_kernel: sequences of different lengths leave CUs idle at the end
+  // unless there are about 4 workgroups a CU.  With at least 1, 4, 8 of them: 352,
+  // 238, 264 us (512 rows over 32768, 16 heads), 203, 184, 174 and 0, 12, 18 for the
+  // join (2900 rows of 4 sequences of up to 5120), 879, 872, 869 (16 x 1024 over 4096)
+  p.units = ragged && p.few == kPaFew ? rows / kPaWide + std::min(seqs, tokens) : 0;
+  const int64_t places = std::max<int64_t>(1, kWidePlaces * cu_count() / std::max<int64_t>(1, p.units * kv_heads));
+  const int64_t wide_per = (room / places + kPaTile - 1) / kPaTile * kPaTile;
+  p.wide_chunk = std::max<int64_t>(kWideLeast, wide_per);
+  p.wide_splits = std::max<int64_t>(1, (room + p.wide_chunk - 1) / p.wide_chunk);
+  p.wide_floats = p.units > 0 && p.wide_splits > 1 ? p.units * kv_heads * kPaWide * p.wide_splits * dim : 0;
   return p;
 }
 }  // namespace
 
 extern "C" int64_t moc_paged_attention_workspace_size(int64_t tokens, int64_t seqs, int ragged, int64_t q_heads,
                                                       int64_t kv_heads, int64_t head_dim, int64_t page, int64_t width) {
-  if (tokens <= 0 || seqs <= 0 || kv_heads <= 0 || q_heads <= 0) return 0;
-  const Plan p = plan_of(tokens, seqs, ragged != 0, q_heads / kv_heads, kv_heads, page * width);
-  return p.splits > 1 ? p.tiles * kv_heads * 16 * p.splits * (head_dim * 4 + 8) : 0;
+  if (tokens <= 0 || seqs <= 0 || kv_heads <= 0 || q_heads <= 0 || head_dim <= 0) return 0;
+  if (page <= 0 || width < 0 || width > kPaRoom / page) return 0;  // refused
+  const Plan p = plan_of(tokens, seqs, ragged != 0, q_heads / kv_heads, kv_heads, head_dim, page * width);
+  return (p.few_floats + p.wide_floats) / head_dim * (head_dim * 4 + 8);
 }
 
 extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_lh, int64_t tokens, int64_t q_heads,
@@ -832,6 +856,7 @@ extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_l
                   pages >= 0 && tokens < (1 << 24) && seqs < (1 << 24) && kv_heads <= 65535 && q_heads <= 65536 &&
                   pages < (1LL << 31) && width < (1LL << 31),
               "moc_paged_attention_bf16: bad shape");
+  MOC_REQUIRE(page * width <= kPaRoom, "moc_paged_attention_bf16: tables of at most 2^30 positions");
   MOC_REQUIRE(cu != nullptr || tokens == seqs, "moc_paged_attention_bf16: one token a sequence without cu");
   if (tokens == 0 || seqs == 0) return MOC_OK;
   MOC_REQUIRE(pages >= 1, "moc_paged_attention_bf16: the cache has no pages");
@@ -841,7 +866,7 @@ extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_l
                   (q_ld | q_lh | o_ld | o_lh) % 8 == 0,
               "moc_paged_attention_bf16: rows must be 16-byte aligned");
   const int64_t group = q_heads / kv_heads;
-  const Plan p = plan_of(tokens, seqs, cu != nullptr, group, kv_heads, page * width);
+  const Plan p = plan_of(tokens, seqs, cu != nullptr, group, kv_heads, head_dim, page * width);
   const int64_t need = moc_paged_attention_workspace_size(tokens, seqs, cu != nullptr, q_heads, kv_heads, head_dim, page,
                                                           width);
   MOC_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
@@ -861,28 +886,25 @@ extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_l
   a.kv_heads = static_cast<int>(kv_heads);
   a.group = static_cast<int>(group);
   a.c2 = scale * 1.4426950408889634f;
-  a.chunk = static_cast<int>(std::min<int64_t>(p.chunk, 1 << 30));
+  a.chunk = static_cast<int>(p.chunk);
   a.splits = static_cast<int>(p.splits);
   a.few = static_cast<int>(p.few);
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + p.tiles * kv_heads * 16 * p.splits * head_dim);
+  a.wide_o = a.part_o + p.few_floats;
+  a.part_ml = reinterpret_cast<float2*>(a.wide_o + p.wide_floats);
+  a.wide_ml = a.part_ml + p.few_floats / head_dim;
+  a.wide_chunk = static_cast<uint32_t>(p.wide_chunk);
+  a.wide_splits = static_cast<int>(p.wide_splits);
   hipStream_t st = as_stream(stream);
   int rc = MOC_OK;
-  if (cu != nullptr && p.few == kPaFew) {
-    // 64 rows a workgroup where 128 would leave CUs without one
-    const bool half = tokens * group / 128 * kv_heads < 2 * cu_count();
-    const int64_t units = tokens * group / (half ? 64 : 128) + std::min(seqs, tokens);
-    MOC_REQUIRE(units * kv_heads < (1LL << 31), "moc_paged_attention_bf16: too many rows for one call");
-    const dim3 grid(static_cast<unsigned>(units * kv_heads));
-#define MOC_PW(D)                                                                                  \
-  do {                                                                                             \
-    if (code == MOC_I8) {                                                                          \
-      if (half) paged_wide_kernel<D, true, 2><<<grid, kPaThreads, 0, st>>>(a);                     \
-      else paged_wide_kernel<D, true, 1><<<grid, kPaThreads, 0, st>>>(a);                          \
-    } else {                                                                                       \
-      if (half) paged_wide_kernel<D, false, 2><<<grid, kPaThreads, 0, st>>>(a);                    \
-      else paged_wide_kernel<D, false, 1><<<grid, kPaThreads, 0, st>>>(a);                         \
-    }                                                                                              \
+  if (p.units > 0) {
+    MOC_REQUIRE(p.units * kv_heads < (1LL << 31) && p.wide_splits <= 65535,
+                "moc_paged_attention_bf16: too many rows for one call");
+    const dim3 grid(static_cast<unsigned>(p.units * kv_heads), static_cast<unsigned>(p.wide_splits));
+#define MOC_PW(D)                                                                  \
+  do {                                                                             \
+    if (code == MOC_I8) paged_wide_kernel<D, true><<<grid, kPaThreads, 0, st>>>(a); \
+    else paged_wide_kernel<D, false><<<grid, kPaThreads, 0, st>>>(a);              \
   } while (0)
     if (head_dim == 64) MOC_PW(64);
     else if (head_dim == 128) MOC_PW(128);
@@ -890,6 +912,14 @@ extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_l
 #undef MOC_PW
     rc = check_launch("paged_wide_kernel");
     if (rc != MOC_OK) return rc;
+    if (p.wide_splits > 1) {
+      const dim3 jg(static_cast<unsigned>(p.units * kv_heads), static_cast<unsigned>(kPaWide * head_dim / 8 / kPaThreads));
+      if (head_dim == 64) paged_wide_join_kernel<64><<<jg, kPaThreads, 0, st>>>(a);
+      else if (head_dim == 128) paged_wide_join_kernel<128><<<jg, kPaThreads, 0, st>>>(a);
+      else paged_wide_join_kernel<256><<<jg, kPaThreads, 0, st>>>(a);
+      rc = check_launch("paged_wide_join_kernel");
+      if (rc != MOC_OK) return rc;
+    }
   }
   if (p.tiles == 0) return rc;
   const dim3 grid(static_cast<unsigned>(p.tiles), static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.splits));

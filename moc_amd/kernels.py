@@ -1326,7 +1326,7 @@ def paged_attention(q, kv: PagedKV, table, lens, cu=None, *, scale: float | None
     A row that sees nothing (lens 0: a slot of the batch not in use) is 0, one
     that sees a position without a page NaN; rows behind cu[-1] are left alone.
     The table's width bounds the work that is split over the length: pass the
-    columns in use."""
+    columns in use (at most 2^30 positions)."""
     dev = N.one_device(q, *kv, table, lens, cu, out)
     if not N.is_current(dev):
         with torch.cuda.device(dev):

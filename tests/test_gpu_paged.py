@@ -120,6 +120,42 @@ def test_attention_prompts(kind, new, before, q_heads, kv_heads, dim, page):
     _close(o[rows], ref[rows], size[rows])
 
 
+@pytest.mark.parametrize("kind,dim,page", [(E4, 64, 16), (I8, 128, 64), (E4, 128, 256), (E4, 256, 32)])
+def test_attention_prompts_behind_a_long_cache(kind, dim, page):
+    """Many rows of few sequences, split over the length: chunks that all, some or
+    no rows see, a table wider than the sequences, a position without a page and a
+    NaN code in one chunk, a length behind the table."""
+    new, before = [300, 40, 1, 0, 130], [5000, 700, 3000, 0, 0]
+    table, lens, cu, pool = _batch(new, before, page, seed=4, width=-(-5600 // page))
+    kv = _cache(pool, 2, page, dim, kind, 4)
+    q = (1.5 * torch.randn(sum(new), 4, dim, generator=_gen(5))).to(BF).cuda()
+    ends = [0, 1, 127, 128, 200, 299, 300, 339, 340, 341, 342, 468, 470]
+
+    def check(what):
+        o = K.paged_attention(q, kv, table, lens, cu)
+        ref, size = R.attention(q, kv, table, lens, cu, dim ** -0.5, set(ends))
+        _close(o[ends], ref[ends], size[ends], what)
+        return o
+
+    clean = check("whole")
+    hole = int(table[0, 4000 // page])
+    table[0, 4000 // page] = pool
+    o = check("no page")
+    assert torch.isnan(o[:300]).all() and torch.equal(o[300:], clean[300:])
+    table[0, 4000 // page] = hole
+    if kind == E4:
+        at = int(table[0, 5100 // page])
+        kept = _bits(kv.v)[at].clone()
+        _bits(kv.v)[at, :, 5100 % page, 3] = 0x7F
+        o = K.paged_attention(q, kv, table, lens, cu)
+        assert torch.equal(o[:100], clean[:100]) and torch.equal(o[300:], clean[300:])
+        assert torch.isnan(o[100:300]).flatten(1).any(1).all()
+        _bits(kv.v)[at] = kept
+    lens[4] = 130 + table.shape[1] * page  # all its rows are behind the table
+    o = check("behind the table")
+    assert torch.isnan(o[341:]).all() and torch.equal(o[:341], clean[:341])
+
+
 @pytest.mark.parametrize("n", [4, 12, 60, 200])
 def test_attention_codes_that_later_rows_see(n):
     """NaN codes and scales, a page out of range: the rows before them are as

@@ -169,7 +169,8 @@ def test_c_entries_refuse(bad):
 def test_c_entries_refuse_their_own():
     for bad in (dict(table_dtype=2), dict(cos=None), dict(k_ld=12), dict(v=None), dict(angles=-1)):
         assert _c_append(**bad) == N.MOC_ERR_INVALID
-    for bad in (dict(heads=5), dict(heads=0), dict(pages=0), dict(width=4000)):  # the last: no workspace
+    for bad in (dict(heads=5), dict(heads=0), dict(pages=0), dict(width=(1 << 26) + 1),
+                dict(width=4000)):  # the last: no workspace
         assert _c_attention(**bad) == N.MOC_ERR_INVALID, bad
     for bad in (dict(dtype=2), dict(vocab=0), dict(vocab=(1 << 18) + 1), dict(rows=-1), dict(ld=-1), dict(x=None), dict(u=None),
                 dict(out=None)):
