@@ -28,7 +28,7 @@ namespace {
 constexpr int kPaWaves = 4;
 constexpr int kPaThreads = 64 * kPaWaves;
 constexpr int kPaTile = 64;  // positions per wave and step
-constexpr int kPaMaxSplits = 1024;
+constexpr int64_t kPaMaxSplits = 1024;
 constexpr int kPaFew = 16;   // rows of a sequence and key head up to which paged_attn_kernel takes it,
 constexpr int kPaAll = 256;  // rows of a ragged batch up to which it takes all: 2.5 us for a launch without work
 
@@ -126,18 +126,25 @@ __global__ __launch_bounds__(kPaThreads, D == 64 ? 3 : D == 128 ? 2 : 1) void pa
   __shared__ float2 ml[kPaWaves][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, h = lane >> 4;
-  const int head = blockIdx.y, lp = a.log_page, page = 1 << lp;
+  const int lp = a.log_page, page = 1 << lp;
+  // Workgroups go round the 8 XCDs: a tile's heads and chunks are neighbours, so that
+  // all read one long sequence (16 sequences of 16 heads, one of 65536 and the others
+  // of 2048 positions: with tiles as neighbours 384 us, so 87), and a short one's only
+  // chunk is a different neighbour in each tile
+  const uint32_t splits = a.splits, around = blockIdx.x / a.kv_heads, tile = around / splits;
+  const int head = blockIdx.x - around * a.kv_heads;
+  const uint32_t chunk = (around - tile * splits + tile) % splits;
   // the row tile: rows [unit 16, unit 16 + 16) of a sequence's n group
   SeqSpan sp;
   const int group = a.group;
   if (a.s.cu == nullptr) {
-    const int tiles = (group + 15) / 16;
-    sp.seq = sp.row0 = blockIdx.x / tiles;
-    sp.unit = blockIdx.x - sp.seq * tiles;
+    const int each = (group + 15) / 16;
+    sp.seq = sp.row0 = tile / each;
+    sp.unit = tile - sp.seq * each;
     sp.n = 1;
     sp.len = a.s.lens[sp.seq];
   } else {
-    sp = find_unit(a.s, blockIdx.x, [group, few = a.few](int n, int64_t) {
+    sp = find_unit(a.s, tile, [group, few = a.few](int n, int64_t) {
       return n * group <= few ? (n * group + 15) / 16 : 0;
     });
     if (sp.seq < 0) return;
@@ -152,7 +159,7 @@ __global__ __launch_bounds__(kPaThreads, D == 64 ? 3 : D == 128 ? 2 : 1) void pa
   const int64_t most = min(max(sp.len - sp.n + 1 + last, int64_t(0)), room);
   const bool lost = sees > room;  // positions without a page: NaN
   const int64_t lim = sees;
-  const int64_t from = static_cast<int64_t>(blockIdx.z) * a.chunk, to = min(most, from + a.chunk);
+  const int64_t from = static_cast<int64_t>(chunk) * a.chunk, to = min(most, from + a.chunk);
 
   bf16x8_t qf[kLoads][2];
 #pragma unroll
@@ -382,7 +389,7 @@ __global__ __launch_bounds__(kPaThreads, D == 64 ? 3 : D == 128 ? 2 : 1) void pa
           __builtin_bit_cast(uint32_t, __builtin_convertvector((cvt_f32x2_t){out[i] * inv, out[i + 1] * inv}, cvt_bf16x2_t));
     return;
   }
-  const int64_t slot = ((static_cast<int64_t>(blockIdx.x) * a.kv_heads + head) * 16 + row) * a.splits + blockIdx.z;
+  const int64_t slot = ((static_cast<int64_t>(tile) * a.kv_heads + head) * 16 + row) * a.splits + chunk;
   if ((tid & 15) == 0) a.part_ml[slot] = make_float2(mm, ll);
   if (mm == -INFINITY) return;  // nothing in this chunk
   float* po = a.part_o + slot * D + d0;
@@ -794,8 +801,8 @@ __global__ __launch_bounds__(kPaThreads) void paged_wide_join_kernel(PagedAttnAr
 using namespace moc;
 
 namespace {
-// paged_attn_kernel's chunks of the positions: enough workgroups for the CUs,
-// whole steps.
+// The positions' chunks of both kernels.
+constexpr int64_t kPaLongest = 8192;  // positions
 constexpr int64_t kWidePlaces = 4, kWideLeast = 512;  // workgroups a CU, positions
 constexpr int64_t kPaRoom = 1LL << 30;                 // positions of a table: 32-bit arithmetic
 struct Plan {
@@ -810,11 +817,23 @@ Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t k
   p.tiles = !ragged ? seqs * ((group + 15) / 16)
             : p.few == kPaAll ? rows / 16 + std::min(seqs, tokens)
             : group <= kPaFew ? std::min(seqs, tokens) : 0;
-  const int64_t step = kPaTile * kPaWaves;
-  const int64_t want =
-      std::min<int64_t>(kPaMaxSplits, std::max<int64_t>(1, 4LL * cu_count() / std::max<int64_t>(1, p.tiles * kv_heads)));
+  // paged_attn_kernel, whole steps: one workgroup a CU keeps more loads in flight than
+  // several that begin and join, and without chunks there is no second launch.  Row
+  // tiles x key heads, 32 heads of 128 over 4096 positions, us with a workgroup a CU
+  // and with four: 64 19.7, 20.2; 160 27.9, 35.5; 256 43.4, 46.8; past that, where the
+  // second round of CUs is nearly empty, 272 66.4, 54.8; 384 82.9, 78.9; and where two
+  // a CU are nearly full, 448 87.2, 94.6.  A sequence far longer than the others is the
+  // end of the call, so chunks are of about 8192 positions at most (one of 65536 among
+  // 16: whole 383 us, 16384 126, 8192 87, 4096 85; 64 of 8192: 191, with 4096 203).
+  // The tiles are counted as if the rows were spread evenly: the grid's bound is more
+  // than most calls have.
+  const int64_t step = kPaTile * kPaWaves, cus = cu_count(), with_rows = std::min(seqs, tokens);
+  const int64_t tiles = kv_heads * (p.few == kPaAll ? with_rows * ((rows + 16 * with_rows - 1) / (16 * with_rows)) : p.tiles);
   const int64_t steps = std::max<int64_t>(1, (room + step - 1) / step);
-  const int64_t per = std::max<int64_t>(1, (steps + want - 1) / want);
+  int64_t want = std::max<int64_t>(tiles > 0 ? cus / tiles : 1, (room + kPaLongest / 2) / kPaLongest);
+  if (tiles * want > cus && 4 * tiles * want < 7 * cus) want = 4 * cus / tiles;
+  want = std::min(std::max<int64_t>(want, 1), kPaMaxSplits);
+  const int64_t per = (steps + want - 1) / want;
   p.chunk = per * step;
   p.splits = (steps + per - 1) / per;
   p.few_floats = p.splits > 1 ? p.tiles * kv_heads * 16 * p.splits * dim : 0;
@@ -823,7 +842,7 @@ Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t k
   // 238, 264 us (512 rows over 32768, 16 heads), 203, 184, 174 and 0, 12, 18 for the
   // join (2900 rows of 4 sequences of up to 5120), 879, 872, 869 (16 x 1024 over 4096)
   p.units = ragged && p.few == kPaFew ? rows / kPaWide + std::min(seqs, tokens) : 0;
-  const int64_t places = std::max<int64_t>(1, kWidePlaces * cu_count() / std::max<int64_t>(1, p.units * kv_heads));
+  const int64_t places = std::max<int64_t>(1, kWidePlaces * cus / std::max<int64_t>(1, p.units * kv_heads));
   const int64_t wide_per = (room / places + kPaTile - 1) / kPaTile * kPaTile;
   p.wide_chunk = std::max<int64_t>(kWideLeast, wide_per);
   p.wide_splits = std::max<int64_t>(1, (room + p.wide_chunk - 1) / p.wide_chunk);
@@ -922,7 +941,8 @@ extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_l
     }
   }
   if (p.tiles == 0) return rc;
-  const dim3 grid(static_cast<unsigned>(p.tiles), static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.splits));
+  MOC_REQUIRE(p.tiles * kv_heads * p.splits < (1LL << 31), "moc_paged_attention_bf16: too many rows for one call");
+  const dim3 grid(static_cast<unsigned>(p.tiles * kv_heads * p.splits));
 #define MOC_PA(D)                                                                  \
   do {                                                                             \
     if (code == MOC_I8) paged_attn_kernel<D, true><<<grid, kPaThreads, 0, st>>>(a); \
