@@ -55,7 +55,8 @@ class BatchDecoder:
         self.lens.zero_()
 
     def _upload(self) -> None:
-        rows = [h + [0] * (self.table.shape[1] - len(h)) for h in self._held]
+        # -1: no page; a token there is not stored and its logits are NaN
+        rows = [h + [-1] * (self.table.shape[1] - len(h)) for h in self._held]
         self.table.copy_(torch.tensor(rows, dtype=torch.int32))
         self.live.copy_(torch.tensor(self._live, dtype=torch.int32))
 
@@ -115,11 +116,12 @@ class BatchDecoder:
     def step(self, u: torch.Tensor, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
         """One token more of each live slot: self.tokens go in, are replaced by
         the drawn ones (K.sample_tokens with the uniform numbers u [slots]) and
-        returned.  Slots out of use keep theirs."""
+        returned.  Slots out of use keep theirs.  A slot whose pages are full
+        (reserve) or whose logits are NaN gets token 0."""
         self.lens.add_(self.live)
         logits = self.logits(self.forward(self.tokens))
         drawn = K.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
-        self.tokens.copy_(torch.where(self.live > 0, drawn, self.tokens))
+        self.tokens.copy_(torch.where(self.live > 0, drawn.clamp_min(0), self.tokens))
         return self.tokens
 
     @torch.no_grad()
@@ -135,7 +137,7 @@ class BatchDecoder:
         settings = (temperature, top_k, top_p, min_p)
         first = self.prompt(prompts, room=length - 1)
         of = [s[:n] if isinstance(s, torch.Tensor) else s for s in settings]
-        self.tokens[:n] = K.sample_tokens(first, u[0, :n], *of)
+        self.tokens[:n] = K.sample_tokens(first, u[0, :n], *of).clamp_min(0)
         out = torch.empty(n, length, dtype=torch.int64, device=dev)
         out[:, 0] = self.tokens[:n]
         now, step = torch.empty_like(u[0]), None
@@ -157,16 +159,17 @@ class BatchDecoder:
         lens, live = self.lens.clone(), self.live.clone()
         self.lens.zero_()
         self.live.zero_()
-        side = torch.cuda.Stream(device=u.device)
-        side.wait_stream(torch.cuda.current_stream(u.device))
-        with torch.cuda.stream(side):
-            for _ in range(2):
+        with torch.cuda.device(u.device):
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                for _ in range(2):
+                    self.step(u, *settings)
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
                 self.step(u, *settings)
-        torch.cuda.current_stream(u.device).wait_stream(side)
-        torch.cuda.synchronize(u.device)
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
-            self.step(u, *settings)
         self.lens.copy_(lens)
         self.live.copy_(live)
         return graph

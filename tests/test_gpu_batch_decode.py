@@ -103,6 +103,31 @@ def test_slots_do_not_touch_each_other():
         assert int((a[0] == b).int().cumprod(0).sum()) >= 1
 
 
+def test_a_slot_without_room_writes_nowhere():
+    """Steps past the reserved pages: no page changes, the next slot's included."""
+    d = BatchDecoder(_model("global_moc"), 3, page=16)
+    d.prompt(_prompts([16, 16]))
+    before = [[t.view(torch.uint8).clone() if t.dtype == E4 else t.clone() for t in kv] for kv in d.kv]
+    u = torch.zeros(3, device="cuda")
+    for _ in range(2):
+        assert d.step(u).tolist() == [0, 0, 0]
+    for kv, was in zip(d.kv, before):
+        for t, w in zip(kv, was):
+            assert torch.equal(t.view(torch.uint8) if t.dtype == E4 else t, w)
+    d.reserve([40, 16, 0])  # room again: the first goes on
+    d.lens.copy_(torch.tensor([16, 16, 0], dtype=torch.int32))
+    d.lens.add_(d.live)
+    x = d.logits(d.forward(d.tokens))
+    assert torch.isfinite(x[0]).all() and torch.isnan(x[1]).any()
+
+
+def test_logits_of_nan_give_a_word_of_the_vocabulary():
+    m = _model("dense")
+    m.lm_head.weight.data.fill_(float("nan"))
+    out = BatchDecoder(m, 2, page=16).generate(_prompts([5, 9]), 4)
+    assert out.shape == (2, 4) and int(out.min()) >= 0 and int(out.max()) < 500
+
+
 def test_refusals():
     m = _model("dense")
     d = BatchDecoder(m, 2, page=16, pages=5)
