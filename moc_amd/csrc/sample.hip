@@ -32,7 +32,8 @@
 // row is read again for each pass (128 KB of 32000 words from L2 at 64 B a clock:
 // under a microsecond), blocks whose largest value is below the cut are not.  Bound
 // by the 64-bit arithmetic of the weights, 20 instructions a word, and for few
-// words by the chain of passes and barriers.
+// words by the chain of passes and barriers.  256 rows of 128256 f32 words 106 us (25
+// to read them once), 16 of 32000 bf16 words with top-p 27, one with top-k 50 12.3.
 #include <type_traits>
 
 #include "abi.h"

@@ -1287,7 +1287,7 @@ def paged_append(q, k, v, cos, sin, kv: PagedKV, table, lens, cu=None, *, out=No
     table [seqs, width] (int32): the page that holds each sequence's positions
     page * i ..; lens [seqs]: its tokens, the new ones counted; cu [seqs + 1]: its
     rows of q (ascending), None for one token each.  A page that the call writes
-    to belongs to one sequence.  Scales are powers of two and grow with a page's
+    to stands in the table once.  Scales are powers of two and grow with a page's
     largest value, its older codes are then encoded again
     (moc_paged_append_bf16).  Tokens without a place are not stored; rows behind
     cu[-1] are left alone.  out: where the rotated q goes (may be q)."""
