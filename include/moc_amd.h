@@ -783,6 +783,14 @@ int moc_sample_tokens(int dtype, const void* logits, int64_t rows, int64_t vocab
                       const float* top_p, float top_p1, const float* min_p, float min_p1, int64_t* out,
                       void* stream);
 
+/* The same with a workspace (NULL: without), with which few rows of 49152
+ * words up are spread over several workgroups; its size (0: not needed).  No zeroing. */
+int64_t moc_sample_tokens_workspace_size(int64_t rows, int64_t vocab);
+int moc_sample_tokens_ws(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t ld, const float* u,
+                         const float* temperature, float temperature1, const int32_t* top_k, int top_k1,
+                         const float* top_p, float top_p1, const float* min_p, float min_p1, int64_t* out,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

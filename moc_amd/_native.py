@@ -177,6 +177,9 @@ SIGNATURES: dict[str, tuple] = {
                                         _vp, _i64, _vp]),
     "moc_sample_tokens": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _int, _vp,
                                  ctypes.c_float, _vp, ctypes.c_float, _vp, _vp]),
+    "moc_sample_tokens_workspace_size": (_i64, [_i64, _i64]),
+    "moc_sample_tokens_ws": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _int, _vp,
+                                    ctypes.c_float, _vp, ctypes.c_float, _vp, _vp, _i64, _vp]),
 }
 
 _LIB = None

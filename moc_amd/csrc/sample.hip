@@ -34,6 +34,8 @@
 // by the 64-bit arithmetic of the weights, 20 instructions a word, and for few
 // words by the chain of passes and barriers.  256 rows of 128256 f32 words 106 us (25
 // to read them once), 16 of 32000 bf16 words with top-p 27, one with top-k 50 12.3.
+// Few long rows are spread over several workgroups (below).
+#include <algorithm>
 #include <type_traits>
 
 #include "abi.h"
@@ -61,6 +63,18 @@ struct SampleArgs {
   float temp1, top_p1, min_p1;
   int top_k1;
   int64_t* out;
+  char* ws;  // SampleWs of each row
+};
+
+// What the workgroups of a row hand on.
+struct SampleWs {
+  uint64_t hist[kSmBins];        // top-p's weights by bin
+  uint64_t sums[kSmBlocks / 4];  // kept weight of each group of four blocks, without top-p's bin
+  uint64_t w[kSmList];           // the words of top-p's bin
+  float x[kSmList];
+  int id[kSmList];
+  float high[kSmBlocks], odd[kSmBlocks];  // of a block: its largest value; 1: it holds NaN or infinity
+  int n, unused[3];                       // words of top-p's bin
 };
 
 struct SampleLds {
@@ -285,7 +299,239 @@ struct Row {
   }
 };
 
+// The settings of a row, and whether its weights are summed by several workgroups:
+// with top-k the words that count are few, without temperature there is one.
+struct Settings {
+  float T, p, min_p;
+  int k;
+  __device__ __forceinline__ Settings(const SampleArgs& a, int64_t row)
+      : T(a.temp ? a.temp[row] : a.temp1), p(a.top_p ? a.top_p[row] : a.top_p1),
+        min_p(a.min_p ? a.min_p[row] : a.min_p1), k(a.top_k ? a.top_k[row] : a.top_k1) {}
+  __device__ __forceinline__ bool best_alone() const { return !(T > 0.f) || k == 1 || p <= 0.f; }
+  __device__ __forceinline__ bool shared(int vocab) const { return !best_alone() && !(k > 0 && k < vocab); }
+  __device__ __forceinline__ double least() const {
+    return min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+  }
+};
+
+__device__ __forceinline__ Scale scale_of(float top, double c) {
+  return Scale{top, c, static_cast<float>(fmin(c * kSmBinsPerOctave, 3e38))};
+}
+// Words from here on have weight.
+__device__ __forceinline__ float reach_of(float top, double c) {
+  return fmaxf(static_cast<float>(static_cast<double>(top) - 47.0 / c), -3.4028234663852886e38f);
+}
+// No word behind a bin is as large.
+__device__ __forceinline__ float floor_of_bin(float top, double c, float reach, int bin) {
+  return fmaxf(reach, static_cast<float>(static_cast<double>(top) - (bin + 2) / (c * kSmBinsPerOctave)));
+}
+// Words below have less than min-p.
+__device__ __forceinline__ float need_of(float top, double c, float floor, double least) {
+  return least > 0.0 ? fmaxf(floor, static_cast<float>(static_cast<double>(top) + (log2(least) - 0.01) / c)) : floor;
+}
+
+// ------------------------------------------------- several workgroups a row
+// For few long rows: the passes over the whole row by workgroups of four waves, each
+// wave groups of four blocks: the blocks' largest values, top-p's histogram, the
+// groups' kept weights; sample_kernel takes what they left instead of its own passes.
+constexpr int kSmPart = 256;
+
 template <bool BF16>
+__global__ __launch_bounds__(kSmPart) void sample_high_kernel(SampleArgs a) {
+  constexpr int kPer = BF16 ? 8 : 4;
+  const int64_t row = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int groups = (a.vocab + 256 * kPer - 1) / (256 * kPer), stride = 4 * gridDim.x;
+  SampleWs& ws = reinterpret_cast<SampleWs*>(a.ws)[row];
+  const Row<BF16> words{static_cast<const uint16_t*>(a.x) + row * a.ld, static_cast<const float*>(a.x) + row * a.ld,
+                        a.vocab, a.wide};
+  for (int i = blockIdx.x * kSmPart + tid; i < kSmBins; i += gridDim.x * kSmPart) ws.hist[i] = 0;
+  if (blockIdx.x == 0 && tid == 0) ws.n = 0;
+  for (int g = 4 * blockIdx.x + wave; g < groups; g += stride) {
+    uint4 raw[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[j] = words.load(4 * g + j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x[kPer], m = -INFINITY;
+      words.template words<true>(raw[j], x);
+      bool odd = false;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        odd |= !(x[e] < INFINITY);
+        m = fmaxf(m, x[e]);
+      }
+      m = fminf(wave_max_f32(m), 3.4028234663852886e38f);
+      const bool any_odd = any_lane(odd);
+      if (lane == 0) {
+        ws.high[4 * g + j] = m;
+        ws.odd[4 * g + j] = any_odd ? 1.f : 0.f;
+      }
+    }
+  }
+}
+
+// The largest value of a row and whether it is plain, for all threads.
+__device__ __forceinline__ float best_of(const SampleWs& ws, int blocks, float (&lds)[2][kSmPart / 64], bool& plain) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float top = -INFINITY, odd = 0.f;
+  for (int b = tid; b < blocks; b += kSmPart) {
+    top = fmaxf(top, ws.high[b]);
+    odd = fmaxf(odd, ws.odd[b]);
+  }
+  top = wave_max_f32(top);
+  odd = wave_max_f32(odd);
+  if (lane == 0) {
+    lds[0][wave] = top;
+    lds[1][wave] = odd;
+  }
+  __syncthreads();
+  plain = fmaxf(fmaxf(lds[1][0], lds[1][1]), fmaxf(lds[1][2], lds[1][3])) == 0.f;
+  return fmaxf(fmaxf(lds[0][0], lds[0][1]), fmaxf(lds[0][2], lds[0][3]));
+}
+
+// f(block, first id, words of this lane) over the blocks of this workgroup's groups
+// that have a value of at least `floor`, then done(group) for each group.
+template <bool PLAIN, bool BF16, typename F, typename G>
+__device__ __forceinline__ void part_of_row(const Row<BF16>& words, const SampleWs& ws, int groups, float floor, F f, G done) {
+  for (int g = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); g < groups; g += 4 * gridDim.x) {
+    const float4 high = reinterpret_cast<const float4*>(ws.high)[g];
+    const bool in[4] = {high.x >= floor, high.y >= floor, high.z >= floor, high.w >= floor};
+    uint4 raw[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (in[j]) raw[j] = words.load(4 * g + j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!in[j]) continue;
+      float x[Row<BF16>::kPer];
+      words.template words<PLAIN>(raw[j], x);
+      f(words.first(4 * g + j), x);
+    }
+    done(g);
+  }
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kSmPart) void sample_bins_kernel(SampleArgs a) {
+  constexpr int kPer = BF16 ? 8 : 4;
+  __shared__ uint64_t hist[kSmBins];
+  __shared__ float best[2][kSmPart / 64];
+  const int64_t row = blockIdx.y;
+  const int tid = threadIdx.x;
+  const Settings set(a, row);
+  if (!set.shared(a.vocab) || !(set.p < 1.f)) return;
+  const int groups = (a.vocab + 256 * kPer - 1) / (256 * kPer);
+  SampleWs& ws = reinterpret_cast<SampleWs*>(a.ws)[row];
+  for (int i = tid; i < kSmBins; i += kSmPart) hist[i] = 0;
+  bool plain;
+  const float top = best_of(ws, 4 * groups, best, plain);
+  if (top == -INFINITY) return;
+  const Row<BF16> words{static_cast<const uint16_t*>(a.x) + row * a.ld, static_cast<const float*>(a.x) + row * a.ld,
+                        a.vocab, a.wide};
+  const double c = 1.4426950408889634074 / static_cast<double>(set.T);
+  const Scale sc = scale_of(top, c);
+  auto add = [&](int, const float(&x)[kPer]) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int b = sc.bin(x[e]);
+      if (b < kSmBins) atomicAdd(reinterpret_cast<unsigned long long*>(&hist[b]), sc.weight(x[e]));
+    }
+  };
+  if (plain) part_of_row<true>(words, ws, groups, reach_of(top, c), add, [](int) {});
+  else part_of_row<false>(words, ws, groups, reach_of(top, c), add, [](int) {});
+  __syncthreads();
+  for (int i = tid; i < kSmBins; i += kSmPart)
+    if (hist[i] != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&ws.hist[i]), hist[i]);
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kSmPart) void sample_groups_kernel(SampleArgs a) {
+  constexpr int kPer = BF16 ? 8 : 4, kOwn = kSmBins / kSmPart;
+  __shared__ float best[2][kSmPart / 64];
+  __shared__ uint64_t waves[kSmPart / 64];
+  __shared__ int reached;
+  const int64_t row = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Settings set(a, row);
+  if (!set.shared(a.vocab)) return;
+  const int groups = (a.vocab + 256 * kPer - 1) / (256 * kPer);
+  SampleWs& ws = reinterpret_cast<SampleWs*>(a.ws)[row];
+  bool plain;
+  const float top = best_of(ws, 4 * groups, best, plain);
+  if (top == -INFINITY) return;
+  int border = kSmBins;
+  if (set.p < 1.f) {  // the bin that sample_kernel's find_bin finds
+    uint64_t v[kOwn], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+      v[j] = ws.hist[kOwn * tid + j];
+      sum += v[j];
+    }
+    const uint64_t upto = wave_upto64(sum);
+    if (lane == 63) waves[wave] = upto;
+    if (tid == 0) reached = kSmBins;
+    __syncthreads();
+    uint64_t before = upto - sum, total = 0;
+#pragma unroll
+    for (int w = 0; w < kSmPart / 64; ++w) {
+      if (w < wave) before += waves[w];
+      total += waves[w];
+    }
+    const double share = static_cast<double>(set.p) * static_cast<double>(total);
+    if (static_cast<double>(before) < share && static_cast<double>(before + sum) >= share) {
+      int at = kSmBins;
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) {
+        before += v[j];
+        if (at == kSmBins && static_cast<double>(before) >= share) at = kOwn * tid + j;
+      }
+      reached = at;
+    }
+    __syncthreads();
+    border = reached;
+  }
+  const Row<BF16> words{static_cast<const uint16_t*>(a.x) + row * a.ld, static_cast<const float*>(a.x) + row * a.ld,
+                        a.vocab, a.wide};
+  const double c = 1.4426950408889634074 / static_cast<double>(set.T), least = set.least();
+  const Scale sc = scale_of(top, c);
+  const float reach = reach_of(top, c), need = need_of(top, c, reach, least);
+  const bool part = border < kSmBins;
+  double sum = 0.0;
+  auto add = [&](int i, const float(&x)[kPer]) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (part) {
+        const int bin = sc.bin(x[e]);
+        if (bin > border) continue;
+        const double w = sc.weight_f64(x[e]);
+        sum += bin < border && w >= least ? w : 0.0;
+        if (bin == border) {
+          const int at = atomicAdd(&ws.n, 1);
+          if (at < kSmList) {
+            ws.x[at] = x[e];
+            ws.id[at] = i + e;
+            ws.w[at] = units(w);
+          }
+        }
+      } else if (x[e] >= need) {
+        const double w = sc.weight_f64(x[e]);
+        sum += w >= least ? w : 0.0;
+      }
+    }
+  };
+  auto done = [&](int group) {
+    const uint64_t all = wave_sum64(units(sum));
+    if (lane == 0) ws.sums[group] = all;
+    sum = 0.0;
+  };
+  const float floor = part ? floor_of_bin(top, c, reach, border) : need;
+  if (plain) part_of_row<true>(words, ws, groups, floor, add, done);
+  else part_of_row<false>(words, ws, groups, floor, add, done);
+}
+
+// One workgroup a row.  SPLIT: after the three kernels before.
+template <bool BF16, bool SPLIT>
 __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
   constexpr int kPer = BF16 ? 8 : 4;
   __shared__ SampleLds s;
@@ -294,10 +540,11 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
   const int blocks = (a.vocab + 64 * kPer - 1) / (64 * kPer);
   const Row<BF16> words{static_cast<const uint16_t*>(a.x) + row * a.ld, static_cast<const float*>(a.x) + row * a.ld,
                         a.vocab, a.wide};
-  const float T = a.temp ? a.temp[row] : a.temp1;
-  const int k = a.top_k ? a.top_k[row] : a.top_k1;
-  const float p = a.top_p ? a.top_p[row] : a.top_p1, min_p = a.min_p ? a.min_p[row] : a.min_p1;
-  const float u = a.u[row];
+  const Settings set(a, row);
+  const float T = set.T, p = set.p, u = a.u[row];
+  const int k = set.k;
+  const SampleWs* const ws = SPLIT ? reinterpret_cast<const SampleWs*>(a.ws) + row : nullptr;
+  const bool shared = SPLIT && set.shared(a.vocab);
   int turn = 0;
   auto before64 = [&](uint64_t v, uint64_t& total) { return block_before64(v, s.wave, turn, total); };
 
@@ -305,16 +552,23 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
   const int own = 4 * (blocks / (4 * kSmWaves)) + min(max(blocks % (4 * kSmWaves) - 4 * wave, 0), 4);
   float high = -INFINITY;
   bool odd = false;
-  words.template each<true>(own >= 64 ? ~0ull : (1ull << own) - 1, wave, [&](int, int, const float(&x)[kPer], int bit) {
-    float m = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      odd |= !(x[e] < INFINITY);
-      m = fmaxf(m, x[e]);
+  if constexpr (SPLIT) {
+    if (lane < own) {
+      high = ws->high[block_of(lane, wave)];
+      odd = ws->odd[block_of(lane, wave)] != 0.f;
     }
-    m = fminf(wave_max_f32(m), 3.4028234663852886e38f);
-    high = lane == bit ? m : high;
-  });
+  } else {
+    words.template each<true>(own >= 64 ? ~0ull : (1ull << own) - 1, wave, [&](int, int, const float(&x)[kPer], int bit) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        odd |= !(x[e] < INFINITY);
+        m = fmaxf(m, x[e]);
+      }
+      m = fminf(wave_max_f32(m), 3.4028234663852886e38f);
+      high = lane == bit ? m : high;
+    });
+  }
   float top = wave_max_f32(high);
   const bool any_odd = any_lane(odd);
   if (lane == 0) s.odd[wave] = any_odd ? 1.f : 0.f;
@@ -335,7 +589,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
     if (plain) words.template each<true>(__ballot(high >= floor), wave, f, done);
     else words.each(__ballot(high >= floor), wave, f, done);
   };
-  if (!(T > 0.f) || k == 1 || p <= 0.f) {  // the best alone: its lowest id
+  if (set.best_alone()) {  // its lowest id
     int at = a.vocab;
     pass(top, [&](int, int i, const float(&x)[kPer], int) {
 #pragma unroll
@@ -348,10 +602,9 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
     return;
   }
   const double c = 1.4426950408889634074 / static_cast<double>(T);
-  const Scale sc{top, c, static_cast<float>(fmin(c * kSmBinsPerOctave, 3e38))};
-  // words from here on have weight
-  const float reach = fmaxf(static_cast<float>(static_cast<double>(top) - 47.0 / c), -3.4028234663852886e38f);
-  const double least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+  const Scale sc = scale_of(top, c);
+  const float reach = reach_of(top, c);
+  const double least = set.least();
   float cut_x = -INFINITY, floor = reach;
   int cut_id = a.vocab;
   auto kept = [&](float x, int id) { return x > cut_x || (x == cut_x && id <= cut_id); };
@@ -412,10 +665,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
     if (cut_x == -INFINITY) add_weights_of(std::true_type());
     else add_weights_of(std::false_type());
   };
-  // No word behind a bin is as large.
-  auto bin_floor = [&](int bin) {
-    return fmaxf(reach, static_cast<float>(static_cast<double>(top) - (bin + 2) / (c * kSmBinsPerOctave)));
-  };
+  auto bin_floor = [&](int bin) { return floor_of_bin(top, c, reach, bin); };
 
   // The last word that a rule keeps: the one whose amount before it is the last
   // below the rule's.  After find_bin.
@@ -619,15 +869,17 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
       __syncthreads();
     }
   }
-  const bool by_share = p < 1.f && find_bin(std::true_type(), 0, share, add_weights);
+  const bool by_share = p < 1.f && find_bin(std::true_type(), 0, share, [&] {
+    if (!shared) return add_weights();
+    for (int i = tid; i < kSmBins; i += kSmThreads) s.hist[i] = ws->hist[i];
+  });
   const int border = by_share ? s.bin : kSmBins;
   const uint64_t above = by_share ? s.above : 0;
   if (tid < kSmBlocks / 4) s.sums[tid] = 0;
   __syncthreads();
 
   // kept weight of each group of blocks, those of top-p's bin in the list for now
-  float need = floor;
-  if (least > 0.0) need = fmaxf(need, static_cast<float>(static_cast<double>(top) + (log2(least) - 0.01) / c));
+  float need = need_of(top, c, floor, least);
   auto by_groups = [&](auto part, auto simple) {  // simple: no top-k, no min-p
     constexpr bool SIMPLE = decltype(simple)::value;
     double sum = 0.0;
@@ -660,8 +912,18 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
     });
   };
   const bool simple = cut_x == -INFINITY && least == 0.0;
+  if (shared) {
+    if (tid < (blocks + 3) / 4) s.sums[tid] = ws->sums[tid];
+    if (by_share && tid < min(ws->n, kSmList)) {
+      s.x[tid] = ws->x[tid];
+      s.id[tid] = ws->id[tid];
+      s.w[tid] = ws->w[tid];
+    }
+    if (by_share && tid == 0) s.n = ws->n;
+  }
   if (by_share) {
-    if (simple) by_groups(std::true_type(), std::true_type());
+    if (shared) {
+    } else if (simple) by_groups(std::true_type(), std::true_type());
     else by_groups(std::true_type(), std::false_type());
     __syncthreads();
     const int n = s.n;
@@ -678,6 +940,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
       need = fmaxf(need, floor);
       by_groups(std::false_type(), std::false_type());
     }
+  } else if (shared) {
   } else if (simple) {
     by_groups(std::false_type(), std::true_type());
   } else {
@@ -732,20 +995,67 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SampleArgs a) {
 
 using namespace moc;
 
-extern "C" int moc_sample_tokens(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t ld, const float* u,
-                                 const float* temperature, float temperature1, const int32_t* top_k, int top_k1,
-                                 const float* top_p, float top_p1, const float* min_p, float min_p1, int64_t* out,
-                                 void* stream) {
+namespace {
+// Three launches more pay where a pass of one workgroup takes longer and CUs are idle.
+// f32 rows with top-p 0.95, us split and by one workgroup a row: 1 x 32000 28, 27; 1 x
+// 50257 27, 36; 1 x 128256 30, 78; 16 x 128256 42, 81; 64 x 128256 66, 88; 128 x 128256
+// 92, 93; 256 x 128256 138, 99.  With top-k 50, 1 x 32000 17, 14; 1 x 128256 18, 22.
+constexpr int64_t kSmSplitVocab = 49152;
+
+bool sample_splits(int64_t rows, int64_t vocab) { return vocab >= kSmSplitVocab && rows <= cu_count() / 4; }
+
+template <bool BF16>
+int launch_sample(const SampleArgs& a, int64_t rows, hipStream_t st) {
+  if (a.ws == nullptr) {
+    sample_kernel<BF16, false><<<static_cast<unsigned>(rows), kSmThreads, 0, st>>>(a);
+    return check_launch("sample_kernel");
+  }
+  // four workgroups a CU, each wave at least one group
+  const int64_t per = BF16 ? 8 : 4, groups = (a.vocab + 256 * per - 1) / (256 * per);
+  const int64_t parts = std::max<int64_t>(1, std::min((groups + 3) / 4, (4 * cu_count() + rows - 1) / rows));
+  const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(rows));
+  sample_high_kernel<BF16><<<grid, kSmPart, 0, st>>>(a);
+  int rc = check_launch("sample_high_kernel");
+  if (rc != MOC_OK) return rc;
+  sample_bins_kernel<BF16><<<grid, kSmPart, 0, st>>>(a);
+  rc = check_launch("sample_bins_kernel");
+  if (rc != MOC_OK) return rc;
+  sample_groups_kernel<BF16><<<grid, kSmPart, 0, st>>>(a);
+  rc = check_launch("sample_groups_kernel");
+  if (rc != MOC_OK) return rc;
+  sample_kernel<BF16, true><<<static_cast<unsigned>(rows), kSmThreads, 0, st>>>(a);
+  return check_launch("sample_kernel");
+}
+}  // namespace
+
+extern "C" int64_t moc_sample_tokens_workspace_size(int64_t rows, int64_t vocab) {
+  return rows > 0 && vocab > 0 && vocab <= kSmMaxVocab && sample_splits(rows, vocab)
+             ? rows * static_cast<int64_t>(sizeof(SampleWs)) : 0;
+}
+
+extern "C" int moc_sample_tokens_ws(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t ld, const float* u,
+                                    const float* temperature, float temperature1, const int32_t* top_k, int top_k1,
+                                    const float* top_p, float top_p1, const float* min_p, float min_p1, int64_t* out,
+                                    void* workspace, int64_t workspace_bytes, void* stream) {
   MOC_REQUIRE(dtype == MOC_BF16 || dtype == MOC_F32, "moc_sample_tokens: logits must be bf16 or f32");
   MOC_REQUIRE(rows >= 0 && vocab >= 1 && vocab <= kSmMaxVocab && ld >= 0 && rows < (1LL << 31),
               "moc_sample_tokens: 1 to %lld words a row", (long long)kSmMaxVocab);
   if (rows == 0) return MOC_OK;
   MOC_REQUIRE(logits && u && out, "moc_sample_tokens: null pointer");
+  const int64_t need = moc_sample_tokens_workspace_size(rows, vocab);
+  MOC_REQUIRE(workspace == nullptr || (aligned16(workspace) && workspace_bytes >= need),
+              "moc_sample_tokens: workspace of %lld bytes required", (long long)need);
   const bool wide = aligned16(logits) && (rows == 1 || ld % (dtype == MOC_BF16 ? 8 : 4) == 0);
   const SampleArgs a{logits, ld, static_cast<int>(vocab), wide, u, temperature, top_p, min_p, top_k,
-                     temperature1, top_p1, min_p1, top_k1, out};
-  const dim3 grid(static_cast<unsigned>(rows));
-  if (dtype == MOC_BF16) sample_kernel<true><<<grid, kSmThreads, 0, as_stream(stream)>>>(a);
-  else sample_kernel<false><<<grid, kSmThreads, 0, as_stream(stream)>>>(a);
-  return check_launch("sample_kernel");
+                     temperature1, top_p1, min_p1, top_k1, out, need > 0 ? static_cast<char*>(workspace) : nullptr};
+  return dtype == MOC_BF16 ? launch_sample<true>(a, rows, as_stream(stream))
+                           : launch_sample<false>(a, rows, as_stream(stream));
+}
+
+extern "C" int moc_sample_tokens(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t ld, const float* u,
+                                 const float* temperature, float temperature1, const int32_t* top_k, int top_k1,
+                                 const float* top_p, float top_p1, const float* min_p, float min_p1, int64_t* out,
+                                 void* stream) {
+  return moc_sample_tokens_ws(dtype, logits, rows, vocab, ld, u, temperature, temperature1, top_k, top_k1, top_p, top_p1,
+                              min_p, min_p1, out, nullptr, 0, stream);
 }

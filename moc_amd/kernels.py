@@ -1383,6 +1383,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> 
     pp, p1 = _per_row("top_p", top_p, rows, f32)
     mp, m1 = _per_row("min_p", min_p, rows, f32)
     out = torch.empty_like(u, dtype=torch.int64)
-    N.call("moc_sample_tokens", N.dtype_code(x.dtype), x.data_ptr(), rows, vocab, ld, u.data_ptr(), tp, t1, kp,
-           max(min(int(k1), vocab), 0), pp, p1, mp, m1, out.data_ptr(), N.stream_on(dev))
+    nbytes = N.query("moc_sample_tokens_workspace_size", rows, vocab)
+    ws = _empty((nbytes,), torch.uint8, x.device) if nbytes else None
+    N.call("moc_sample_tokens_ws", N.dtype_code(x.dtype), x.data_ptr(), rows, vocab, ld, u.data_ptr(), tp, t1, kp,
+           max(min(int(k1), vocab), 0), pp, p1, mp, m1, out.data_ptr(), N.ptr(ws), nbytes, N.stream_on(dev))
     return out

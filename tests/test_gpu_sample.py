@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 import torch
 
+from moc_amd import _native as N
 from moc_amd import kernels as K
 
 import paged_reference as R
@@ -166,3 +167,72 @@ def test_graph_replays(rows):
         for r in range(0, rows, 13):
             id_, near = R.sample(x[r].cpu().numpy(), float(u[r]), float(t[r]), int(k[r]), float(p[r]), 0.0)
             assert int(out[r]) == id_ or near < 1e-9
+
+
+# ---------------------------------------- rows spread over several workgroups
+def _alone(x, u, temperature, top_k, top_p, min_p):
+    """The form of one workgroup a row, which takes no workspace."""
+    out = torch.empty(x.shape[0], dtype=torch.int64, device="cuda")
+    N.call("moc_sample_tokens", N.dtype_code(x.dtype), x.data_ptr(), *x.shape, x.stride(0), u.data_ptr(),
+           temperature.data_ptr(), 0.0, top_k.data_ptr(), 0, top_p.data_ptr(), 0.0, min_p.data_ptr(), 0.0, out.data_ptr(),
+           torch.cuda.current_stream().cuda_stream)
+    return out
+
+
+@pytest.mark.parametrize("settings", SETTINGS, ids=lambda d: "-".join("%s%g" % i for i in d.items()) or "plain")
+@pytest.mark.parametrize("dtype,vocab", [(F32, 65536), (BF, 128256), (F32, 70001), (BF, 100001)])
+def test_long_rows_against_the_definition(settings, dtype, vocab):
+    _check(_logits(4, vocab, dtype, vocab + 1), _u(4, 5), **settings)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("rows,vocab", [(1, 262144), (7, 49152), (33, 65537), (64, 50257), (300, 66000)])
+def test_long_rows_equal_one_workgroup(dtype, rows, vocab):
+    """Bit for bit, over mixed settings and rows of every kind: equal words, NaN and
+    infinities, all masked, one word alone, a few words over a masked row."""
+    x = _logits(rows, vocab, dtype, rows)
+    kinds = torch.arange(rows) % 8
+    for r in range(rows):
+        kind = int(kinds[r]) if rows > 1 else 0
+        if kind == 1:
+            x[r] = 1.5
+        elif kind == 2:
+            x[r, ::97] = math.nan
+            x[r, 5::1009] = math.inf
+        elif kind == 3:
+            x[r] = -math.inf
+        elif kind == 4:
+            x[r] = torch.finfo(dtype).min
+            x[r, [3, vocab // 2, vocab - 1]] = 2.0
+        elif kind == 5:
+            x[r] = (x[r] * 2).round() / 2
+        elif kind == 6:
+            x[r, 1:] = -math.inf
+    g = torch.Generator().manual_seed(rows)
+    u = torch.rand(rows, generator=g).cuda()
+    pick = lambda values, dt: torch.tensor(values, dtype=dt)[torch.randint(len(values), (rows,), generator=g)].cuda()  # noqa: E731
+    for _ in range(6):
+        s = (pick([1.0, 0.6, 1.7, 0.0, 30.0], F32), pick([0, 0, 0, 3, 700], torch.int32), pick([1.0, 0.95, 0.5, 1e-6, 0.9999], F32),
+             pick([0.0, 0.0, 0.02, 1.0], F32))
+        assert torch.equal(K.sample_tokens(x, u, *s), _alone(x, u, *s))
+
+
+def test_long_rows_strided_and_replayed():
+    """Rows off the 16-byte grid; a captured call follows its inputs, with its own
+    workspace, beside an eager one."""
+    wide = _logits(3, 70003, F32, 9)
+    x = wide[:, 1:70000]
+    u = torch.tensor([0.1, 0.5, 0.9], device="cuda")
+    full = lambda v, dt=F32: torch.full((3,), v, dtype=dt, device="cuda")  # noqa: E731
+    s = (full(1.0), full(0, torch.int32), full(0.9), full(0.0))
+    K.sample_tokens(x, u, *s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = K.sample_tokens(x, u, *s)
+    for i in range(4):
+        wide.copy_(_logits(3, 70003, F32, 20 + i))
+        u.copy_(torch.tensor(_u(3, i), device="cuda"))
+        graph.replay()
+        eager = K.sample_tokens(x, u, *s)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and torch.equal(eager, _alone(x, u, *s)), i

@@ -178,6 +178,17 @@ def test_c_entries_refuse_their_own():
         assert N.last_error().startswith("moc_sample_tokens")
 
 
+def test_sampling_workspace():
+    lib = N.load()
+    assert lib.moc_sample_tokens_workspace_size(4, 32000) == 0 == lib.moc_sample_tokens_workspace_size(0, 128256)
+    need = lib.moc_sample_tokens_workspace_size(2, 128256)
+    assert need > 0 and need == 2 * lib.moc_sample_tokens_workspace_size(1, 128256)
+    for ws, size in ((P, need - 1), (ctypes.c_void_p((1 << 20) + 8), need)):
+        assert lib.moc_sample_tokens_ws(N.MOC_F32, P, 2, 128256, 128256, P, None, 1.0, None, 0, None, 1.0, None, 0.0, P, ws,
+                                        size, None) == N.MOC_ERR_INVALID
+        assert "workspace of %d bytes" % need in N.last_error()
+
+
 def test_c_entries_take_nothing():
     assert _c_append(tokens=0, seqs=0, q=None, k=None, v=None, table=None, lens=None, out=None) == N.MOC_OK
     assert _c_attention(tokens=0, seqs=0, q=None, table=None, lens=None, out=None) == N.MOC_OK
