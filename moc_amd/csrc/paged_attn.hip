@@ -30,7 +30,13 @@ constexpr int kPaWaves = 4;
 constexpr int kPaThreads = 64 * kPaWaves;
 constexpr int kPaTile = 64;  // positions per wave and step
 constexpr int64_t kPaMaxSplits = 1024;
-constexpr int kPaFew = 16;   // rows of a sequence and key head up to which paged_attn_kernel takes it,
+// Rows of a sequence and key head up to which paged_attn_kernel takes it, reading the
+// cache once for 16 of them (the tiles of a head run side by side, L2 serves the rest),
+// where paged_wide_kernel's four waves read it once for 128 of which most are missing:
+// 48 sequences of 8192, 8 key heads of 128: 32 rows 183, 263 us; 48 255, 275; 64 285,
+// 277; of 16384, 4 of 64: 153, 228 and 163, 228; of 32768, one of 256: 399, 522 and
+// 479, 421.
+constexpr int kPaFew = 48;
 constexpr int kPaAll = 256;  // rows of a ragged batch up to which it takes all: 2.5 us for a launch without work
 
 struct PagedAttnArgs {
@@ -473,8 +479,8 @@ __global__ __launch_bounds__(kPaThreads) void paged_join_kernel(PagedAttnArgs a)
 }
 
 // ------------------------------------------------------------- many rows
-// Sequences with more than 16 rows a key head (prompts, chunks of them, groups of
-// several drafted tokens): v_mfma_f32_32x32x16_bf16 in the same orientation, 32
+// Sequences with more than 48 rows a key head (prompts, chunks of them, groups of
+// many drafted tokens): v_mfma_f32_32x32x16_bf16 in the same orientation, 32
 // rows a wave, 128 a workgroup over the same tiles of 64 positions.  Every thread
 // takes its part of the next tile's codes into registers while this one is worked
 // on, and stores them to LDS as bf16: a conversion for all waves, where each wave
@@ -819,11 +825,11 @@ struct Plan {
 };
 Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t kv_heads, int64_t dim, int64_t room) {
   Plan p;
-  const int64_t rows = tokens * group;
+  const int64_t rows = tokens * group, with_rows = std::min(seqs, tokens);
   p.few = !ragged ? group : rows <= kPaAll ? kPaAll : kPaFew;
   p.tiles = !ragged ? seqs * ((group + 15) / 16)
-            : p.few == kPaAll ? rows / 16 + std::min(seqs, tokens)
-            : group <= kPaFew ? std::min(seqs, tokens) : 0;
+            : p.few == kPaAll ? rows / 16 + with_rows
+            : group <= kPaFew ? std::min(rows / 16 + with_rows, with_rows * (kPaFew / 16)) : 0;
   // paged_attn_kernel, whole steps: one workgroup a CU keeps more loads in flight than
   // several that begin and join, and without chunks there is no second launch.  Row
   // tiles x key heads, 32 heads of 128 over 4096 positions, us with a workgroup a CU
@@ -834,8 +840,9 @@ Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t k
   // 16: whole 383 us, 16384 126, 8192 87, 4096 85; 64 of 8192: 191, with 4096 203).
   // The tiles are counted as if the rows were spread evenly: the grid's bound is more
   // than most calls have.
-  const int64_t step = kPaTile * kPaWaves, cus = cu_count(), with_rows = std::min(seqs, tokens);
-  const int64_t tiles = kv_heads * (p.few == kPaAll ? with_rows * ((rows + 16 * with_rows - 1) / (16 * with_rows)) : p.tiles);
+  const int64_t step = kPaTile * kPaWaves, cus = cu_count();
+  const int64_t tiles =
+      kv_heads * (ragged ? std::min(p.tiles, with_rows * ((rows + 16 * with_rows - 1) / (16 * with_rows))) : p.tiles);
   const int64_t steps = std::max<int64_t>(1, (room + step - 1) / step);
   int64_t want = std::max<int64_t>(tiles > 0 ? cus / tiles : 1, (room + kPaLongest / 2) / kPaLongest);
   if (tiles * want > cus && 4 * tiles * want < 7 * cus) want = 4 * cus / tiles;
@@ -848,7 +855,7 @@ Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t k
   // unless there are about 4 workgroups a CU.  With at least 1, 4, 8 of them: 352,
   // 238, 264 us (512 rows over 32768, 16 heads), 203, 184, 174 and 0, 12, 18 for the
   // join (2900 rows of 4 sequences of up to 5120), 879, 872, 869 (16 x 1024 over 4096)
-  p.units = ragged && p.few == kPaFew ? rows / kPaWide + std::min(seqs, tokens) : 0;
+  p.units = ragged && p.few == kPaFew ? rows / kPaWide + with_rows : 0;
   const int64_t places = std::max<int64_t>(1, kWidePlaces * cus / std::max<int64_t>(1, p.units * kv_heads));
   const int64_t wide_per = (room / places + kPaTile - 1) / kPaTile * kPaTile;
   p.wide_chunk = std::max<int64_t>(kWideLeast, wide_per);
