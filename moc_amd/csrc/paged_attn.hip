@@ -816,7 +816,7 @@ using namespace moc;
 namespace {
 // The positions' chunks of both kernels.
 constexpr int64_t kPaLongest = 8192;  // positions
-constexpr int64_t kWidePlaces = 4, kWideLeast = 512;  // workgroups a CU, positions
+constexpr int64_t kWidePlaces = 2, kWideLeast = 512;  // workgroups a CU, positions
 constexpr int64_t kPaRoom = 1LL << 30;                 // positions of a table: 32-bit arithmetic
 struct Plan {
   int64_t tiles, chunk, splits, few;
@@ -851,12 +851,13 @@ Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t k
   p.chunk = per * step;
   p.splits = (steps + per - 1) / per;
   p.few_floats = p.splits > 1 ? p.tiles * kv_heads * 16 * p.splits * dim : 0;
-  // paged_wide_kernel: sequences of different lengths leave CUs idle at the end
-  // unless there are about 4 workgroups a CU.  With at least 1, 4, 8 of them: 352,
-  // 238, 264 us (512 rows over 32768, 16 heads), 203, 184, 174 and 0, 12, 18 for the
-  // join (2900 rows of 4 sequences of up to 5120), 879, 872, 869 (16 x 1024 over 4096)
+  // paged_wide_kernel: two workgroups a CU, counted as if the rows were spread evenly;
+  // more are more to join.  With 1, 2, 4 of them a CU at most: 352, 211, 222 us (512
+  // rows over 32768, 16 heads), 203, 189, 193 (2900 rows of 4 sequences of up to 5120),
+  // 92 and 103 with 2 and 4 (16 sequences of 8192, 64 rows of 8 heads).
   p.units = ragged && p.few == kPaFew ? rows / kPaWide + with_rows : 0;
-  const int64_t places = std::max<int64_t>(1, kWidePlaces * cus / std::max<int64_t>(1, p.units * kv_heads));
+  const int64_t units = kv_heads * with_rows * ((rows + kPaWide * with_rows - 1) / (kPaWide * with_rows));
+  const int64_t places = std::max<int64_t>(1, kWidePlaces * cus / units);
   const int64_t wide_per = (room / places + kPaTile - 1) / kPaTile * kPaTile;
   p.wide_chunk = std::max<int64_t>(kWideLeast, wide_per);
   p.wide_splits = std::max<int64_t>(1, (room + p.wide_chunk - 1) / p.wide_chunk);
