@@ -61,7 +61,9 @@ class BatchDecoder:
         self.live.copy_(torch.tensor(self._live, dtype=torch.int32))
 
     def reserve(self, tokens: Sequence[int]) -> None:
-        """Pages for tokens[slot] tokens of each slot (0: out of use)."""
+        """Pages for tokens[slot] tokens of each slot.  0: out of use; the slot
+        keeps its pages, its length and its token, and goes on when a later call
+        names it again."""
         if len(tokens) != self.slots:
             raise ValueError(f"reserve: {self.slots} slots, got {len(tokens)}")
         if max(tokens) > self.model.cfg.max_seq:
@@ -75,16 +77,19 @@ class BatchDecoder:
         self._upload()
 
     @torch.no_grad()
-    def forward(self, tokens: torch.Tensor, cu: torch.Tensor | None = None) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, cu: torch.Tensor | None = None,
+                lens: torch.Tensor | None = None) -> torch.Tensor:
         """Hidden states [tokens, hidden] of new tokens whose sequences' lengths
-        (self.lens, these counted) are set; cu as in K.paged_append."""
+        (self.lens or the ones given, these tokens counted) are set; cu as in
+        K.paged_append."""
         x = self.model.embed(tokens)
+        lens = self.lens if lens is None else lens
         scale = 1.0 / math.sqrt(self.head_dim)
         for layer, kv in zip(self.model.layers, self.kv):
             a = layer.attn
             q, k, v = a.qkv_proj(layer.attn_norm(x)).view(-1, 3 * self.heads, self.head_dim).split(self.heads, dim=1)
-            q = K.paged_append(q, k, v, a.rope_cos, a.rope_sin, kv, self.table, self.lens, cu)
-            o = K.paged_attention(q, kv, self.table, self.lens, cu, scale=scale)
+            q = K.paged_append(q, k, v, a.rope_cos, a.rope_sin, kv, self.table, lens, cu)
+            o = K.paged_attention(q, kv, self.table, lens, cu, scale=scale)
             x = x + a.out_proj(o.flatten(1))
             if layer.fuse:
                 x = layer.ffn.fused_decode_residual(x, layer.ffn_norm.weight, layer.ffn_norm.eps)
@@ -119,7 +124,8 @@ class BatchDecoder:
         returned.  Slots out of use keep theirs.  A slot whose pages are full
         (reserve) or whose logits are NaN gets token 0."""
         self.lens.add_(self.live)
-        logits = self.logits(self.forward(self.tokens))
+        # a slot out of use has its token still to store: of no length, it stores nothing
+        logits = self.logits(self.forward(self.tokens, lens=self.lens * self.live))
         drawn = K.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
         self.tokens.copy_(torch.where(self.live > 0, drawn.clamp_min(0), self.tokens))
         return self.tokens

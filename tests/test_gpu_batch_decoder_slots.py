@@ -1,0 +1,73 @@
+"""BatchDecoder's slots on the device: sequences that wait against the same ones
+that do not, bit for bit (a step is the same kernels over the same rows)."""
+import pytest
+import torch
+
+from moc_amd.inference.batch_decode import BatchDecoder
+from moc_amd.inference.decode_model import DecodeConfig, DecoderModel
+
+pytestmark = pytest.mark.gpu
+BF, E4, I8 = torch.bfloat16, torch.float8_e4m3fn, torch.int8
+PAGE = 16
+
+
+def _model(row, seed=5):
+    cfg = DecodeConfig(hidden=256, intermediate=704, heads=4, layers=2, vocab=500, k=128, max_seq=96)
+    m = DecoderModel(row, cfg).to("cuda", BF).init_weights(seed)
+    m.embed.weight.data.mul_(50)
+    return m
+
+
+def _prompts(lengths, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, 500, (n,), generator=g).cuda() for n in lengths]
+
+
+def _begin(m, prompts, room, slots=3, codes=E4):
+    """A decoder with stale pages, its prompts run and the first tokens drawn."""
+    d = BatchDecoder(m, slots, page=PAGE, codes=codes)
+    for i, kv in enumerate(d.kv):
+        for t in (kv.k, kv.v):
+            t.view(torch.uint8).copy_(torch.randint(0, 120, t.shape, generator=torch.Generator().manual_seed(i)))
+        kv.k_scale.fill_(0.25)
+        kv.v_scale.fill_(0.5)
+    d.tokens[:len(prompts)] = d.prompt(prompts, room=room).argmax(-1)
+    return d
+
+
+def _pages(d, slot, n):
+    """Codes of a slot's first n positions and their pages' scales, all layers."""
+    ids = d.table[slot, :-(-n // PAGE)].long()
+    out = []
+    for kv in d.kv:
+        for t in (kv.k, kv.v):
+            out.append(t.view(torch.uint8)[ids].transpose(1, 2).flatten(0, 1)[:n])
+        out += [kv.k_scale[ids], kv.v_scale[ids]]
+    return out
+
+
+def _same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def _steps(d, n, u=0.4):
+    u = torch.full((d.slots,), u, device="cuda")
+    return torch.stack([d.step(u, 0.8, 40).clone() for _ in range(n)])
+
+
+@pytest.mark.parametrize("row", ["dense", "global_moc", "moc_2_8"])
+@pytest.mark.parametrize("codes", [E4, I8])
+def test_a_slot_out_of_use_is_left_alone(row, codes):
+    m, prompts = _model(row), _prompts([17, 15, 30])
+    whole = _begin(m, prompts, 12, codes=codes)
+    want = _steps(whole, 9)
+    d = _begin(m, prompts, 12, codes=codes)
+    _steps(d, 2)
+    before, pending = _pages(d, 0, 19), int(d.tokens[0])
+    d.reserve([0, 27, 42])
+    assert (_steps(d, 3)[:, 0] == pending).all() and d.lens.tolist() == [19, 20, 35]
+    assert _same(_pages(d, 0, 19), before)
+    d.reserve([29, 27, 42])
+    rest = _steps(d, 7)
+    assert torch.equal(rest[:, 0], want[2:, 0]) and torch.equal(rest[:4, 1:], want[5:, 1:])
+    assert _same(_pages(d, 0, 26), _pages(whole, 0, 26))
