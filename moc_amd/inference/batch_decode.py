@@ -43,6 +43,7 @@ class BatchDecoder:
         zeros = lambda *s, dtype=torch.int32: torch.zeros(*s, dtype=dtype, device=w.device)  # noqa: E731
         self.table, self.lens = zeros(slots, width), zeros(slots)
         self.live = zeros(slots)                       # 1: the slot takes a token a step
+        self.room = zeros(slots)                       # positions that it has a place and an angle for
         self.tokens = zeros(slots, dtype=torch.int64)  # the last token of each
         self.release()
 
@@ -59,6 +60,8 @@ class BatchDecoder:
         rows = [h + [-1] * (self.table.shape[1] - len(h)) for h in self._held]
         self.table.copy_(torch.tensor(rows, dtype=torch.int32))
         self.live.copy_(torch.tensor(self._live, dtype=torch.int32))
+        room = [min(len(h) * self.page, self.model.cfg.max_seq) for h in self._held]
+        self.room.copy_(torch.tensor(room, dtype=torch.int32))
 
     def reserve(self, tokens: Sequence[int]) -> None:
         """Pages for tokens[slot] tokens of each slot.  0: out of use; the slot
@@ -121,13 +124,15 @@ class BatchDecoder:
     def step(self, u: torch.Tensor, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
         """One token more of each live slot: self.tokens go in, are replaced by
         the drawn ones (K.sample_tokens with the uniform numbers u [slots]) and
-        returned.  Slots out of use keep theirs.  A slot whose pages are full
-        (reserve) or whose logits are NaN gets token 0."""
-        self.lens.add_(self.live)
-        # a slot out of use has its token still to store: of no length, it stores nothing
-        logits = self.logits(self.forward(self.tokens, lens=self.lens * self.live))
+        returned.  Slots out of use keep theirs.  So does one whose pages are full,
+        which goes on once reserve gives it room.  One whose logits are NaN gets
+        token 0."""
+        takes = self.live * (self.lens < self.room)  # 1: it has a place for its token
+        self.lens.add_(takes)
+        # a slot that takes none has its token still to store: of no length, it stores nothing
+        logits = self.logits(self.forward(self.tokens, lens=self.lens * takes))
         drawn = K.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
-        self.tokens.copy_(torch.where(self.live > 0, drawn.clamp_min(0), self.tokens))
+        self.tokens.copy_(torch.where(takes > 0, drawn.clamp_min(0), self.tokens))
         return self.tokens
 
     @torch.no_grad()

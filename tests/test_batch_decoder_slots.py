@@ -111,3 +111,27 @@ def test_a_slot_out_of_use_is_left_alone(decoder):
     rest = torch.stack(_steps(d, 7))
     assert torch.equal(rest[:, 0], want[2:, 0]) and torch.equal(rest[:4, 1:], want[5:, 1:])
     assert torch.equal(_cached(d, 0), _cached(whole, 0))
+
+
+def test_a_full_slot_waits_for_room(decoder):
+    """Steps past the pages that it holds leave its length and its pending token;
+    with room again it goes on as if it had had it from the start."""
+    whole = _begin(decoder(2), [16, 3], room=9)
+    want = torch.stack(_steps(whole, 8))
+    d = _begin(decoder(2), [16, 3], room=0)
+    pending = d.tokens.clone()
+    first = torch.stack(_steps(d, 3))
+    assert d.lens.tolist() == [16, 6] and (first[:, 0] == pending[0]).all()
+    assert torch.equal(first[:, 1], want[:3, 1])
+    d.reserve([40, 40])
+    rest = torch.stack(_steps(d, 8))
+    assert d.lens.tolist() == [24, 14]
+    assert torch.equal(rest[:, 0], want[:, 0]) and torch.equal(rest[:5, 1], want[3:, 1])
+    assert torch.equal(_cached(d, 0), _cached(whole, 0))
+
+
+def test_a_slot_stops_at_the_models_last_position(decoder):
+    """72 positions in pages of 16: the last page has places that no angle has."""
+    d = _begin(decoder(1), [70], room=2)
+    _steps(d, 4)
+    assert d.lens.tolist() == [72]

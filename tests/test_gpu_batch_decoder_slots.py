@@ -71,3 +71,42 @@ def test_a_slot_out_of_use_is_left_alone(row, codes):
     rest = _steps(d, 7)
     assert torch.equal(rest[:, 0], want[2:, 0]) and torch.equal(rest[:4, 1:], want[5:, 1:])
     assert _same(_pages(d, 0, 26), _pages(whole, 0, 26))
+
+
+@pytest.mark.parametrize("row", ["dense", "global_moc"])
+@pytest.mark.parametrize("codes", [E4, I8])
+def test_a_full_slot_waits_for_room(row, codes):
+    """Its length and its pending token stay until reserve() gives it places; the
+    next tokens are those of a sequence that had them from the start."""
+    m, prompts = _model(row), _prompts([16, 3, 40])
+    whole = _begin(m, prompts, 9, codes=codes)
+    want = _steps(whole, 8)
+    d = _begin(m, prompts, 0, codes=codes)
+    pending = int(d.tokens[0])
+    first = _steps(d, 3)
+    assert d.lens.tolist() == [16, 6, 43] and (first[:, 0] == pending).all()
+    assert torch.equal(first[:, 1:], want[:3, 1:])
+    d.reserve([40, 40, 56])
+    rest = _steps(d, 8)
+    assert d.lens.tolist() == [24, 14, 51]
+    assert torch.equal(rest[:, 0], want[:, 0]) and torch.equal(rest[:5, 1:], want[3:, 1:])
+    assert _same(_pages(d, 0, 24), _pages(whole, 0, 24))
+
+
+def test_a_captured_step_follows_reserve():
+    """One graph over slots that run, fill up, pause and go on, against eager steps."""
+    m, prompts = _model("global_moc"), _prompts([14, 20])
+    d, eager = (_begin(m, prompts, 0, slots=3) for _ in range(2))
+    u = torch.full((3,), 0.4, device="cuda")
+    graph = d._capture(u, (0.8, 40, 1.0, 0.0))
+    assert d.lens.tolist() == [14, 20, 0]
+    for i, wanted in enumerate([None, [14, 20, 0], [30, 0, 0], [30, 40, 0], [0, 40, 0], [60, 60, 0]]):
+        if wanted is not None:
+            for x in (d, eager):
+                x.reserve(wanted)
+        for _ in range(4):
+            graph.replay()
+            eager.step(u, 0.8, 40)
+            torch.cuda.synchronize()
+            assert torch.equal(d.tokens, eager.tokens) and torch.equal(d.lens, eager.lens), i
+    assert all(_same(_pages(d, b, int(d.lens[b])), _pages(eager, b, int(d.lens[b]))) for b in range(2))
