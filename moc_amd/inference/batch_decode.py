@@ -165,8 +165,9 @@ class BatchDecoder:
 
     def _capture(self, u: torch.Tensor, settings) -> torch.cuda.CUDAGraph:
         """The step as a HIP graph.  The warm-up runs change nothing: with no
-        live slot and lengths of 0 no key is stored and no token replaced."""
-        self.model.freeze_for_compile()
+        live slot and lengths of 0 no key is stored and no token replaced.  They
+        bring what the FFNs derive from their weights up to date, so that the
+        capture makes none of it and the model need not be frozen."""
         lens, live = self.lens.clone(), self.live.clone()
         self.lens.zero_()
         self.live.zero_()

@@ -110,3 +110,20 @@ def test_a_captured_step_follows_reserve():
             torch.cuda.synchronize()
             assert torch.equal(d.tokens, eager.tokens) and torch.equal(d.lens, eager.lens), i
     assert all(_same(_pages(d, b, int(d.lens[b])), _pages(eager, b, int(d.lens[b]))) for b in range(2))
+
+
+@pytest.mark.parametrize("row", ["global_moc", "moc_2_8"])
+@pytest.mark.parametrize("graph", [True, False])
+def test_generate_follows_the_weights(row, graph):
+    """Weights changed in place between two calls: the tokens of a model that was
+    made with them, also after a call with a graph, and the model's own forward."""
+    m, other = _model(row), _model(row, 6)
+    prompts = _prompts([9, 20, 5])
+    want = BatchDecoder(other, 3, page=PAGE).generate(prompts, 8, graph=False)
+    assert not torch.equal(BatchDecoder(m, 3, page=PAGE).generate(prompts, 8), want)
+    m.load_state_dict(other.state_dict())
+    assert torch.equal(*(BatchDecoder(x, 3, page=PAGE).prompt(prompts) for x in (m, other)))
+    assert torch.equal(BatchDecoder(m, 3, page=PAGE).generate(prompts, 8, graph=graph), want)
+    x = torch.randn(3, 256, generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    with torch.no_grad():
+        assert torch.equal(m.layers[0]._ffn(x[None]), other.layers[0]._ffn(x[None]))
