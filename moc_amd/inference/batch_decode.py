@@ -171,17 +171,19 @@ class BatchDecoder:
         lens, live = self.lens.clone(), self.live.clone()
         self.lens.zero_()
         self.live.zero_()
-        with torch.cuda.device(u.device):
-            side = torch.cuda.Stream()
-            side.wait_stream(torch.cuda.current_stream())
-            with torch.cuda.stream(side):
-                for _ in range(2):
+        try:
+            with torch.cuda.device(u.device):
+                side = torch.cuda.Stream()
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    for _ in range(2):
+                        self.step(u, *settings)
+                torch.cuda.current_stream().wait_stream(side)
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
                     self.step(u, *settings)
-            torch.cuda.current_stream().wait_stream(side)
-            torch.cuda.synchronize()
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                self.step(u, *settings)
-        self.lens.copy_(lens)
-        self.live.copy_(live)
+        finally:
+            self.lens.copy_(lens)
+            self.live.copy_(live)
         return graph

@@ -135,3 +135,20 @@ def test_a_slot_stops_at_the_models_last_position(decoder):
     d = _begin(decoder(1), [70], room=2)
     _steps(d, 4)
     assert d.lens.tolist() == [72]
+
+
+def test_a_capture_that_fails_changes_nothing(decoder, monkeypatch):
+    """The sequences go on after it, as if it had not been tried."""
+    whole = _begin(decoder(2), [5, 9], room=5)
+    want = torch.stack(_steps(whole, 4))
+    d = _begin(decoder(2), [5, 9], room=5)
+
+    def fails(*a):
+        raise RuntimeError("no capture")
+
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "device", fails)
+        with pytest.raises(RuntimeError, match="no capture"):
+            d._capture(torch.zeros(2), (0.0, 0, 1.0, 0.0))
+    assert d.lens.tolist() == [5, 9] and d.live.tolist() == [1, 1]
+    assert torch.equal(torch.stack(_steps(d, 4)), want)
