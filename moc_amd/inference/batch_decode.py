@@ -175,10 +175,12 @@ class BatchDecoder:
             with torch.cuda.device(u.device):
                 side = torch.cuda.Stream()
                 side.wait_stream(torch.cuda.current_stream())
-                with torch.cuda.stream(side):
-                    for _ in range(2):
-                        self.step(u, *settings)
-                torch.cuda.current_stream().wait_stream(side)
+                try:
+                    with torch.cuda.stream(side):
+                        for _ in range(2):
+                            self.step(u, *settings)
+                finally:
+                    torch.cuda.current_stream().wait_stream(side)
                 torch.cuda.synchronize()
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph):
