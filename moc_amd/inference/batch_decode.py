@@ -63,17 +63,22 @@ class BatchDecoder:
         room = [min(len(h) * self.page, self.model.cfg.max_seq) for h in self._held]
         self.room.copy_(torch.tensor(room, dtype=torch.int32))
 
+    def _more(self, what: str, tokens: Sequence[int], held: Sequence[list[int]], free: int) -> list[int]:
+        """Pages that the slots want beside the ones they hold, if there are so many."""
+        if max(tokens) > self.model.cfg.max_seq:
+            raise ValueError(f"{what}: {max(tokens)} tokens, the model has {self.model.cfg.max_seq} positions")
+        more = [max(-(-n // self.page) - len(h), 0) for n, h in zip(tokens, held)]
+        if sum(more) > free:
+            raise ValueError(f"{what}: {sum(more)} pages wanted, {free} are free")
+        return more
+
     def reserve(self, tokens: Sequence[int]) -> None:
         """Pages for tokens[slot] tokens of each slot.  0: out of use; the slot
         keeps its pages, its length and its token, and goes on when a later call
         names it again."""
         if len(tokens) != self.slots:
             raise ValueError(f"reserve: {self.slots} slots, got {len(tokens)}")
-        if max(tokens) > self.model.cfg.max_seq:
-            raise ValueError(f"reserve: {max(tokens)} tokens, the model has {self.model.cfg.max_seq} positions")
-        more = [max(-(-n // self.page) - len(h), 0) for n, h in zip(tokens, self._held)]
-        if sum(more) > len(self._free):
-            raise ValueError(f"reserve: {sum(more)} pages wanted, {len(self._free)} are free")
+        more = self._more("reserve", tokens, self._held, len(self._free))
         for held, m in zip(self._held, more):
             held.extend(self._free.pop() for _ in range(m))
         self._live = [n > 0 for n in tokens]
@@ -108,13 +113,17 @@ class BatchDecoder:
     def prompt(self, prompts: Sequence[torch.Tensor], room: int = 0) -> torch.Tensor:
         """Starts the slots with these prompts (1-D token ids, at least one token
         each) and pages for `room` tokens more; logits [prompts, vocab] behind
-        their last tokens."""
+        their last tokens.  Refused prompts leave the slots as they were."""
         n = [int(p.numel()) for p in prompts]
         if not n or min(n) < 1 or len(n) > self.slots:
             raise ValueError(f"prompt: 1 to {self.slots} prompts of at least one token")
+        if room < 0:
+            raise ValueError(f"prompt: room for {room} tokens")
         empty = [0] * (self.slots - len(n))
+        wanted = [t + room for t in n] + empty
+        self._more("prompt", wanted, [[]] * self.slots, self.pages)
         self.release()
-        self.reserve([t + room for t in n] + empty)
+        self.reserve(wanted)
         self.lens.copy_(torch.tensor(n + empty, dtype=torch.int32))
         cu = torch.tensor([0, *n, *empty], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(self.lens.device)
         x = self.forward(torch.cat([p.reshape(-1) for p in prompts]).to(self.tokens.device), cu)

@@ -152,3 +152,16 @@ def test_a_capture_that_fails_changes_nothing(decoder, monkeypatch):
             d._capture(torch.zeros(2), (0.0, 0, 1.0, 0.0))
     assert d.lens.tolist() == [5, 9] and d.live.tolist() == [1, 1]
     assert torch.equal(torch.stack(_steps(d, 4)), want)
+
+
+def test_a_refused_prompt_leaves_the_running_slots(decoder):
+    """Too long, too many pages, none, room below 0: the sequences go on."""
+    whole = _begin(decoder(2, pages=5), [5, 9], room=5)
+    want = torch.stack(_steps(whole, 4))
+    d = _begin(decoder(2, pages=5), [5, 9], room=5)
+    for prompts, room in ((_prompts([70]), 3), (_prompts([40, 40]), 0), ([], 0), (_prompts([4, 4]), -1),
+                          (_prompts([4, 0]), 0)):
+        with pytest.raises(ValueError):
+            d.prompt(prompts, room=room)
+    assert torch.equal(torch.stack(_steps(d, 4)), want)
+    assert d.prompt(_prompts([40, 40 - PAGE]), room=0).shape == (2, VOCAB)  # all pages
