@@ -1251,15 +1251,22 @@ def _paged_operands(what: str, kv: PagedKV, table, lens, cu, tokens: int):
     return code, shape, seqs, wide[1]
 
 
+def _strides(t: torch.Tensor):
+    """Strides of [tokens, heads, dim], 0 for tokens or heads where there is one:
+    torch leaves any stride there."""
+    n, h, _ = t.shape
+    s = t.stride()
+    return s[0] if n > 1 else 0, s[1] if h > 1 else 0, s[2]
+
+
 def _head_rows(t: torch.Tensor):
     """([tokens, heads, dim] whose rows the kernels can read: unit stride inside,
     16-byte aligned, a copy where they are not; strides; address)."""
-    s, p = t.stride(), t.data_ptr()
-    if s[2] == 1 and not ((s[0] | s[1]) & 7 or p & 15):
-        return t, s, p
-    t = t.contiguous()
-    if t.data_ptr() & 15:
-        t = t.clone()
+    p = t.data_ptr()
+    for s in (t.stride(), _strides(t)):
+        if s[2] == 1 and not ((s[0] | s[1]) & 7 or p & 15):
+            return t, s, p
+    t = t.clone(memory_format=torch.contiguous_format)
     return t, t.stride(), t.data_ptr()
 
 
@@ -1272,7 +1279,7 @@ def _rows_out(what: str, out, like: torch.Tensor):
     t, h, d = like.shape
     if out.shape != like.shape or out.dtype != like.dtype:
         raise ValueError(f"{what}: out must be bf16 {tuple(like.shape)}")
-    s, p = out.stride(), out.data_ptr()
+    s, p = _strides(out), out.data_ptr()
     if s[2] != 1 or (s[0] | s[1]) & 7 or p & 15 or (h > 1 and s[1] < d) or (t > 1 and s[0] < (h - 1) * s[1] + d):
         raise ValueError(f"{what}: out needs 16-byte aligned rows that do not overlap")
     return out, s, p
