@@ -1262,10 +1262,12 @@ def _strides(t: torch.Tensor):
 def _head_rows(t: torch.Tensor):
     """([tokens, heads, dim] whose rows the kernels can read: unit stride inside,
     16-byte aligned, a copy where they are not; strides; address)."""
-    p = t.data_ptr()
-    for s in (t.stride(), _strides(t)):
-        if s[2] == 1 and not ((s[0] | s[1]) & 7 or p & 15):
-            return t, s, p
+    s, p = t.stride(), t.data_ptr()
+    if s[2] == 1 and not ((s[0] | s[1]) & 7 or p & 15):
+        return t, s, p
+    s = _strides(t)
+    if s[2] == 1 and not ((s[0] | s[1]) & 7 or p & 15):
+        return t, s, p
     t = t.clone(memory_format=torch.contiguous_format)
     return t, t.stride(), t.data_ptr()
 
