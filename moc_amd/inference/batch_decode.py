@@ -45,6 +45,8 @@ class BatchDecoder:
         self.live = zeros(slots)                       # 1: the slot takes a token a step
         self.room = zeros(slots)                       # positions that it has a place and an angle for
         self.tokens = zeros(slots, dtype=torch.int64)  # the last token of each
+        # what the last step drew for each: the id; -1: its logits are NaN; -2: it took none
+        self.drawn = zeros(slots, dtype=torch.int64)
         self.release()
 
     def release(self) -> None:
@@ -54,6 +56,7 @@ class BatchDecoder:
         self._live = [False] * self.slots
         self._upload()
         self.lens.zero_()
+        self.drawn.fill_(-2)
 
     def _upload(self) -> None:
         # -1: no page; a token there is not stored and its logits are NaN
@@ -135,12 +138,13 @@ class BatchDecoder:
         the drawn ones (K.sample_tokens with the uniform numbers u [slots]) and
         returned.  Slots out of use keep theirs.  So does one whose pages are full,
         which goes on once reserve gives it room.  One whose logits are NaN gets
-        token 0."""
+        token 0.  self.drawn tells these from a drawn token."""
         takes = self.live * (self.lens < self.room)  # 1: it has a place for its token
         self.lens.add_(takes)
         # a slot that takes none has its token still to store: of no length, it stores nothing
         logits = self.logits(self.forward(self.tokens, lens=self.lens * takes))
         drawn = K.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+        self.drawn.copy_(drawn).masked_fill_(takes == 0, -2)
         self.tokens.copy_(torch.where(takes > 0, drawn.clamp_min(0), self.tokens))
         return self.tokens
 
@@ -149,7 +153,8 @@ class BatchDecoder:
                  generator: torch.Generator | None = None, graph: bool = True) -> torch.Tensor:
         """`length` tokens behind each prompt, int64 [prompts, length].  Settings
         are numbers, or tensors [slots] (K.sample_tokens); temperature 0 is
-        greedy.  graph: the step is captured once and replayed."""
+        greedy.  graph: the step is captured once and replayed.  A sequence whose
+        logits are NaN goes on with token 0 (self.drawn: of the last token)."""
         if length < 1:
             raise ValueError("generate: at least one token")
         n, dev = len(prompts), self.lens.device
@@ -157,7 +162,8 @@ class BatchDecoder:
         settings = (temperature, top_k, top_p, min_p)
         first = self.prompt(prompts, room=length - 1)
         of = [s[:n] if isinstance(s, torch.Tensor) else s for s in settings]
-        self.tokens[:n] = K.sample_tokens(first, u[0, :n], *of).clamp_min(0)
+        self.drawn[:n] = K.sample_tokens(first, u[0, :n], *of)
+        self.tokens[:n] = self.drawn[:n].clamp_min(0)
         out = torch.empty(n, length, dtype=torch.int64, device=dev)
         out[:, 0] = self.tokens[:n]
         now, step = torch.empty_like(u[0]), None

@@ -165,3 +165,19 @@ def test_a_refused_prompt_leaves_the_running_slots(decoder):
             d.prompt(prompts, room=room)
     assert torch.equal(torch.stack(_steps(d, 4)), want)
     assert d.prompt(_prompts([40, 40 - PAGE]), room=0).shape == (2, VOCAB)  # all pages
+
+
+def test_what_was_drawn_is_told_from_what_was_not(decoder):
+    """drawn: the id; -1 behind logits of NaN, whose slot gets token 0; -2 where no
+    step was taken, whose slot keeps its token."""
+    d = _begin(decoder(4), [16, 5, 9], room=0)
+    assert d.drawn.tolist() == [-2] * 4
+    d.tokens[2] = VOCAB - 1
+    d.model.embed.weight.data[VOCAB - 1] = math.nan
+    d.reserve([16, 8, 12, 0])
+    before = d.tokens.clone()
+    after = d.step(torch.zeros(4))
+    assert d.drawn.tolist() == [-2, int(after[1]), -1, -2]
+    assert after[0] == before[0] and after[2] == 0 and after[3] == before[3]
+    d.prompt(_prompts([3]))
+    assert d.drawn.tolist() == [-2] * 4

@@ -109,6 +109,7 @@ def test_a_captured_step_follows_reserve():
             eager.step(u, 0.8, 40)
             torch.cuda.synchronize()
             assert torch.equal(d.tokens, eager.tokens) and torch.equal(d.lens, eager.lens), i
+            assert torch.equal(d.drawn, eager.drawn), i
     assert all(_same(_pages(d, b, int(d.lens[b])), _pages(eager, b, int(d.lens[b]))) for b in range(2))
 
 
@@ -137,3 +138,13 @@ def test_a_capture_that_fails_changes_nothing():
         d._capture(torch.zeros(3, device="cuda"), (0.8, 40, torch.ones(2, device="cuda"), 0.0))
     assert d.lens.tolist() == [9, 20, 0] and d.live.tolist() == [1, 1, 0]
     assert torch.equal(_steps(d, 4), _steps(whole, 4))
+
+
+def test_generate_tells_logits_of_nan():
+    m = _model("dense")
+    d = BatchDecoder(m, 2, page=PAGE)
+    assert torch.equal(d.generate(_prompts([5, 9]), 4)[:, -1], d.drawn)
+    m.lm_head.weight.data.fill_(float("nan"))
+    for length in (1, 2, 4):
+        d.generate(_prompts([5]), length)
+        assert d.drawn.tolist() == [-1, -2]
