@@ -148,3 +148,35 @@ def test_generate_tells_logits_of_nan():
     for length in (1, 2, 4):
         d.generate(_prompts([5]), length)
         assert d.drawn.tolist() == [-1, -2]
+
+
+@pytest.mark.parametrize("row", ["dense", "global_moc", "moc_2_8"])
+@pytest.mark.parametrize("codes", [E4, I8])
+def test_a_slot_sees_its_own_sequence_alone(row, codes):
+    """Another slot's prompt and tokens changed, of the same length, so that every
+    product keeps its shape: the others' logits, of the prompts and of each step,
+    are the same bits, and its own are not."""
+    m, lengths = _model(row), [20, 33, 8]
+    base, other = _prompts(lengths), _prompts(lengths, 9)
+    fed = torch.randint(0, 500, (2, 20, 3), generator=torch.Generator().manual_seed(4)).cuda()
+
+    def logits(changed):
+        prompts = [(other if b == changed else base)[b] for b in range(3)]
+        d = BatchDecoder(m, 3, page=PAGE, codes=codes)
+        out = [d.prompt(prompts, room=20)]
+        for i in range(20):  # over ends of pages
+            d.tokens.copy_(fed[0, i])
+            if changed is not None:
+                d.tokens[changed] = fed[1, i, changed]
+            d.lens.add_(d.live)
+            out.append(d.logits(d.forward(d.tokens)))
+        return torch.stack(out)
+
+    want = logits(None)
+    for b in range(3):
+        got = logits(b)
+        for c in range(3):
+            if c == b:
+                assert not (got[:, c] == want[:, c]).all(-1).any()
+            else:
+                assert torch.equal(got[:, c], want[:, c]), (b, c)
