@@ -47,6 +47,7 @@ class BatchDecoder:
         self.tokens = zeros(slots, dtype=torch.int64)  # the last token of each
         # what the last step drew for each: the id; -1: its logits are NaN; -2: it took none
         self.drawn = zeros(slots, dtype=torch.int64)
+        self._none = torch.full_like(self.drawn, -2)
         self.release()
 
     def release(self) -> None:
@@ -56,7 +57,7 @@ class BatchDecoder:
         self._live = [False] * self.slots
         self._upload()
         self.lens.zero_()
-        self.drawn.fill_(-2)
+        self.drawn.copy_(self._none)
 
     def _upload(self) -> None:
         # -1: no page; a token there is not stored and its logits are NaN
@@ -139,13 +140,13 @@ class BatchDecoder:
         returned.  Slots out of use keep theirs.  So does one whose pages are full,
         which goes on once reserve gives it room.  One whose logits are NaN gets
         token 0.  self.drawn tells these from a drawn token."""
-        takes = self.live * (self.lens < self.room)  # 1: it has a place for its token
+        takes = self.lens < self.room * self.live  # it has a place for its token
         self.lens.add_(takes)
         # a slot that takes none has its token still to store: of no length, it stores nothing
         logits = self.logits(self.forward(self.tokens, lens=self.lens * takes))
         drawn = K.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
-        self.drawn.copy_(drawn).masked_fill_(takes == 0, -2)
-        self.tokens.copy_(torch.where(takes > 0, drawn.clamp_min(0), self.tokens))
+        torch.where(takes, drawn, self._none, out=self.drawn)
+        torch.where(takes, drawn.clamp_min(0), self.tokens, out=self.tokens)
         return self.tokens
 
     @torch.no_grad()
@@ -183,7 +184,7 @@ class BatchDecoder:
         live slot and lengths of 0 no key is stored and no token replaced.  They
         bring what the FFNs derive from their weights up to date, so that the
         capture makes none of it and the model need not be frozen."""
-        lens, live = self.lens.clone(), self.live.clone()
+        lens, live, drawn = self.lens.clone(), self.live.clone(), self.drawn.clone()
         self.lens.zero_()
         self.live.zero_()
         try:
@@ -203,4 +204,5 @@ class BatchDecoder:
         finally:
             self.lens.copy_(lens)
             self.live.copy_(live)
+            self.drawn.copy_(drawn)
         return graph

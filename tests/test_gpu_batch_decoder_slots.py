@@ -134,9 +134,13 @@ def test_a_capture_that_fails_changes_nothing():
     """Settings that a step refuses, behind its forward's launches."""
     m, prompts = _model("global_moc"), _prompts([9, 20])
     whole, d = (_begin(m, prompts, 5) for _ in range(2))
+    d.drawn.copy_(d.tokens)
     with pytest.raises(ValueError, match="top_p"):
         d._capture(torch.zeros(3, device="cuda"), (0.8, 40, torch.ones(2, device="cuda"), 0.0))
     assert d.lens.tolist() == [9, 20, 0] and d.live.tolist() == [1, 1, 0]
+    assert torch.equal(d.drawn, d.tokens)
+    d._capture(torch.zeros(3, device="cuda"), (0.8, 40, 1.0, 0.0))
+    assert d.lens.tolist() == [9, 20, 0] and torch.equal(d.drawn, d.tokens)
     assert torch.equal(_steps(d, 4), _steps(whole, 4))
 
 
