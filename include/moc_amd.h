@@ -738,11 +738,12 @@ int moc_sparse28_down_bf16(const void* ap, int64_t ld_ap, const uint32_t* meta, 
 
 /* RoPE on q and k (interleaved pairs, cos and sin [angles, head_dim / 2] in
  * table_dtype) and the new k and v into the cache.  q_out = rotated q as bf16 (may
- * be q).  A block (one page's places of one head) gets the least power of two s
- * with |x| <= 448 s (e4m3) or 127 s (int8), at least 2^-100, for what it held and
- * gets; a call that writes a page's first place begins it anew; where the scale
- * grows, older codes are encoded again.  Codes are rounded to nearest even; values
- * that are not finite do not count for s and become NaN (e4m3), the ends or 0 (int8).
+ * be q, and shares no memory with k or v).  A block (one page's places of one head)
+ * gets the least power of two s with |x| <= 448 s (e4m3) or 127 s (int8), at least
+ * 2^-100, for what it held and gets; a call that writes a page's first place begins
+ * it anew; where the scale grows, older codes are encoded again.  Codes are rounded
+ * to nearest even; values that are not finite do not count for s and become NaN
+ * (e4m3), the ends or 0 (int8).
  * A token without a place (position negative, behind the table or the angles, page
  * number out of range) is not stored; its q_out is 0 before position 0, NaN behind
  * the table or the angles.  A page that a call writes to stands in the tables once. */

@@ -15,9 +15,12 @@
 //
 // One wave takes one block (or one query head) of the tokens that one page gets
 // in this call: its scale needs them all, and no workgroup has to meet.
-// Bound by HBM traffic for prompts (9 of up to 1000 tokens, 32 heads of 64: 128 MB
-// in 30 us, where a copy of the 113 MB needed takes 22), by the chain length ->
-// page -> scale -> store for single tokens (64 of them, 8 key heads: 4.3 us).
+// Bound for prompts by HBM traffic and by arithmetic beside it (9 of up to 1000
+// tokens, 32 heads of 64: 132 MB in 30 us, where a copy of the 113 MB needed takes
+// 22; VALU instructions issue in 45 % of the clocks: each head turns its own angles
+// to f32, a key's or value's wave reads its rows, and turns a key's, once for the
+// largest value and once for the codes), by the chain length -> page -> scale ->
+// store for single tokens (64 of them, 8 key heads: 4.4 us).
 #include "abi.h"
 #include "paged.h"
 

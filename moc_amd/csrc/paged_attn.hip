@@ -8,10 +8,14 @@
 // row (l & 15), its softmax factors are per-lane values, and the four positions
 // that a 16-position tile of S^T leaves in a lane (4 (l >> 4) + r) are, two
 // tiles together, the eight k of the second product's operand: P never moves
-// between lanes.  V's operand needs the same positions for one dimension: a
+// between lanes.  P is rounded to bf16 for that product, V's type there: an error of
+// at most 2^-8 of each probability, of either sign, where the output's own rounding
+// to bf16 is 2^-8 of the result (together 0.0023 of the output's size against 64
+// bits, 0.0017 with P in f32).  P in two bf16 parts would double that product's
+// instructions.  The sum below the fraction is of P before the rounding.  V's operand needs the same positions for one dimension: a
 // lane reads D / 16 neighbouring dimensions of each of its eight positions and
 // transposes them in registers (v_perm).  Codes become bf16 exactly; the page's
-// scales go onto the scores and the probabilities in f32.
+// scales go onto the scores and the probabilities in f32, V's before P is rounded.
 //
 // The cache is read once for a tile, straight into registers; one workgroup
 // takes a chunk of the positions, a wave 64 at a time, and the waves join
@@ -481,7 +485,8 @@ __global__ __launch_bounds__(kPaThreads) void paged_join_kernel(PagedAttnArgs a)
 // ------------------------------------------------------------- many rows
 // Sequences with more than 48 rows a key head (prompts, chunks of them, groups of
 // many drafted tokens): v_mfma_f32_32x32x16_bf16 in the same orientation, 32
-// rows a wave, 128 a workgroup over the same tiles of 64 positions.  Every thread
+// rows a wave, 128 a workgroup over the same tiles of 64 positions, P in bf16 for the
+// same reason.  Every thread
 // takes its part of the next tile's codes into registers while this one is worked
 // on, and stores them to LDS as bf16: a conversion for all waves, where each wave
 // converting for itself took 128 instructions a tile and as many permutations to
@@ -490,8 +495,10 @@ __global__ __launch_bounds__(kPaThreads) void paged_join_kernel(PagedAttnArgs a)
 // scores leave in a lane (attn.hip).  16-byte chunk c of a row of 64 tile positions
 // lies in slot c ^ row_swz(row).  Bound by VALU work and LDS reads beside the
 // MFMAs: per 64 positions and 32 rows 32 MFMAs of 32 clocks, 32 KB of LDS, 32
-// exponentials and about 170 instructions: 722 TFLOP/s for 16 x 1024 rows, 585 for 4
-// sequences of different lengths (171 us for 100 GFLOP).  The wave
+// exponentials and about 170 instructions: 722 TFLOP/s for 16 x 1024 rows.  585 for 4
+// sequences of different lengths (171 us for 100 GFLOP): their 480 workgroups are one
+// round of 25 to 80 tiles each, since chunks go by the table's width and not by a
+// unit's own length, and the CUs work 72 % of the time.  The wave
 // in its products goes first, the other's softmax fills the gaps (381 us for 4 x 4096
 // rows, 409 with equal priorities).
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -836,7 +843,10 @@ Plan plan_of(int64_t tokens, int64_t seqs, bool ragged, int64_t group, int64_t k
   // tiles x key heads, 32 heads of 128 over 4096 positions, us with a workgroup a CU
   // and with four: 64 19.7, 20.2; 160 27.9, 35.5; 256 43.4, 46.8; past that, where the
   // second round of CUs is nearly empty, 272 66.4, 54.8; 384 82.9, 78.9; and where two
-  // a CU are nearly full, 448 87.2, 94.6.  A sequence far longer than the others is the
+  // a CU are nearly full, 448 87.2, 94.6.  Tables of less than 4096 positions stay whole
+  // there (want is 0): 272 tiles of 1024 positions 20.3 us, with four a CU 21.9, of 512
+  // 13.2, 16.3, and of heads of 64 up to 4032 35.7, 36.3; of 128 from 2048 on the split
+  // would gain, 40.5, 36.1, and 384 tiles 44.1, 44.3.  A sequence far longer than the others is the
   // end of the call, so chunks are of about 8192 positions at most (one of 65536 among
   // 16: whole 383 us, 16384 126, 8192 87, 4096 85; 64 of 8192: 191, with 4096 203).
   // The tiles are counted as if the rows were spread evenly: the grid's bound is more

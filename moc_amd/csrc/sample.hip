@@ -11,9 +11,12 @@
 // is off by 1e-7 of the row's weight and one draw in a few hundred over 32000
 // words would give the neighbour.  So w = 2^y with y in 64 bits, 2^f by a
 // polynomial of the eighth degree (the least largest relative error on |f| <= 1/2
-// with value 1 at 0: 8.1e-13), held in units of 2^-44.  Sums of these are sums of
-// integers (2^18 words: less than 2^62) and have no order, so histograms by
-// atomics give the same bits each time.  A table of 2^(i/64) takes three
+// with value 1 at 0: 8.14e-13), held in units of 2^-44.  Sums of these are sums of
+// integers (2^18 words: at most 2^62) and have no order, so histograms by atomics
+// give the same bits each time.  A weight is off by 8.2e-13 of itself and half a
+// unit (2^-45 of the best's, below which it is 0), a sum by at most 8.2e-13 of it
+// and 2^-45 for each word (2^18 words: 2^-27): the id is that of exact arithmetic
+// unless one of its borders, the draw's, top-p's or min-p's, lies as near as that.  A table of 2^(i/64) takes three
 // multiplications fewer and an LDS read, which the histogram's atomics leave no
 // time for.
 //
@@ -30,10 +33,15 @@
 // One workgroup a row: the largest value of each block (16 bytes a lane of a wave),
 // the rules, the weights by blocks, the block and then the lane of the draw.  The
 // row is read again for each pass (128 KB of 32000 words from L2 at 64 B a clock:
-// under a microsecond), blocks whose largest value is below the cut are not.  Bound
-// by the 64-bit arithmetic of the weights, 20 instructions a word, and for few
-// words by the chain of passes and barriers.  256 rows of 128256 f32 words 106 us (25
-// to read them once), 16 of 32000 bf16 words with top-p 27, one with top-k 50 12.3.
+// under a microsecond), blocks whose largest value is below the cut are not.  A row
+// that no top-k shortens is bound by the 64-bit arithmetic of its weights, 20
+// instructions a word: of 128256 words with top-p 0.95 alone, 78 us, VALU
+// instructions issue in two thirds of its CU's clocks, waits for loads, atomics and
+// barriers take the rest.  A call of many rows is bound by such rows, a CU each: of
+// 256 with settings of their own (106 us; 25 to read them once) the CUs work 40 % of
+// the time and issue VALU instructions in 18 % of the clocks, 256 equal ones 99 us,
+// 89 % and 50 %.  Few words are bound by the chain of passes and barriers: 16 rows
+// of 32000 bf16 words with top-p 27 us, one with top-k 50 12.3.
 // Few long rows are spread over several workgroups (below).
 #include <algorithm>
 #include <type_traits>

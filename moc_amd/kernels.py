@@ -1299,7 +1299,8 @@ def paged_append(q, k, v, cos, sin, kv: PagedKV, table, lens, cu=None, *, out=No
     to stands in the table once.  Scales are powers of two and grow with a page's
     largest value, its older codes are then encoded again
     (moc_paged_append_bf16).  Tokens without a place are not stored; rows behind
-    cu[-1] are left alone.  out: where the rotated q goes (may be q)."""
+    cu[-1] are left alone.  out: where the rotated q goes (may be q, and shares no
+    memory with k or v)."""
     dev = N.one_device(q, k, v, cos, sin, *kv, table, lens, cu, out)
     if not N.is_current(dev):
         with torch.cuda.device(dev):
@@ -1374,8 +1375,10 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> 
     id; top_k <= 0, top_p >= 1 and min_p <= 0 are off.  In this order: the first
     top_k ids (by logit, then the lower id), of those the fewest that hold top_p of
     their weight, of those the ones with min_p of the best's weight; the draw walks
-    what is left by ascending id.  Weights are held in 64 bits, so the id is that
-    of exact arithmetic.  NaN logits are never drawn; a row with nothing to draw
+    what is left by ascending id.  Weights are held in 64 bits: the id is that of
+    exact arithmetic unless one of its borders lies within 8.2e-13 of the weight
+    that counts, plus 2^-45 of the best's for each word (a word lighter than that
+    has none).  NaN logits are never drawn; a row with nothing to draw
     gives -1 (moc_sample_tokens)."""
     settings = (temperature, top_k, top_p, min_p)
     dev = N.one_device(logits, u, *[t for t in settings if isinstance(t, torch.Tensor)])
