@@ -115,9 +115,10 @@ class BatchDecoder:
 
     @torch.no_grad()
     def prompt(self, prompts: Sequence[torch.Tensor], room: int = 0) -> torch.Tensor:
-        """Starts the slots with these prompts (1-D token ids, at least one token
-        each) and pages for `room` tokens more; logits [prompts, vocab] behind
-        their last tokens.  Refused prompts leave the slots as they were."""
+        """Starts the first slots with these prompts (1-D token ids, at least one
+        token each) and pages for `room` tokens more; logits [prompts, vocab] behind
+        their last tokens, from which the caller draws self.tokens.  What ran before
+        ends in every slot, unless the prompts are refused."""
         n = [int(p.numel()) for p in prompts]
         if not n or min(n) < 1 or len(n) > self.slots:
             raise ValueError(f"prompt: 1 to {self.slots} prompts of at least one token")
