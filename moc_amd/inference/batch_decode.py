@@ -142,10 +142,11 @@ class BatchDecoder:
         which goes on once reserve gives it room.  One whose logits are NaN gets
         token 0.  self.drawn tells these from a drawn token."""
         takes = self.lens < self.room * self.live  # it has a place for its token
-        self.lens.add_(takes)
+        lens = self.lens + takes
         # a slot that takes none has its token still to store: of no length, it stores nothing
-        logits = self.logits(self.forward(self.tokens, lens=self.lens * takes))
+        logits = self.logits(self.forward(self.tokens, lens=lens * takes))
         drawn = K.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+        self.lens.copy_(lens)  # only now: a step that is refused is none
         torch.where(takes, drawn, self._none, out=self.drawn)
         torch.where(takes, drawn.clamp_min(0), self.tokens, out=self.tokens)
         return self.tokens

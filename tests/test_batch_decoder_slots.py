@@ -181,3 +181,24 @@ def test_what_was_drawn_is_told_from_what_was_not(decoder):
     assert after[0] == before[0] and after[2] == 0 and after[3] == before[3]
     d.prompt(_prompts([3]))
     assert d.drawn.tolist() == [-2] * 4
+
+
+def test_a_refused_step_is_no_step(decoder, monkeypatch):
+    """Settings that the draw refuses: the next step stores the same tokens at the
+    same positions."""
+    whole = _begin(decoder(2), [5, 15], room=6)
+    want = torch.stack(_steps(whole, 5))
+    d = _begin(decoder(2), [5, 15], room=6)
+    _steps(d, 1)
+
+    def refuses(*a):
+        raise ValueError("settings")
+
+    for _ in range(2):
+        with monkeypatch.context() as m:
+            m.setattr(K, "sample_tokens", refuses)
+            with pytest.raises(ValueError, match="settings"):
+                d.step(torch.zeros(2))
+        assert d.lens.tolist() == [6, 16]
+    assert torch.equal(torch.stack(_steps(d, 4)), want[1:])
+    assert all(torch.equal(_cached(d, b), _cached(whole, b)) for b in range(2))
