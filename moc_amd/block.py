@@ -209,6 +209,40 @@ class _AttentionHalf(torch.autograd.Function):
         return dx, dn, dq, do, None, None, None, None
 
 
+def final_norm(h, norm, norm_type) -> torch.Tensor:
+    """norm(h) for an operator that takes hidden rows: one row kernel each way where
+    the norm is a plain one in the stream's dtype (an f32 stream under autocast: as
+    bf16, what a product makes of it), the module itself elsewhere."""
+    dt = stream_dtype(h)
+    w = getattr(norm, "weight", None)
+    if dt is None or type(norm) is not norm_type or not bare(norm) or not plain(h, w) or h.dim() != 3 or \
+            h.numel() < 1 or h.shape[-1] % 8 or h.shape[-1] > 4096 or w.shape != (h.shape[-1],) or \
+            not all(t.dtype == dt and t.is_contiguous() and t.device == h.device and t.data_ptr() % 16 == 0
+                    for t in (h, w)):
+        return norm(h)
+    return _FinalNorm.apply(h, w, float(norm.eps))
+
+
+class _FinalNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, norm_w, eps):
+        h2 = h.reshape(-1, h.shape[-1])
+        xn, rstd = K.rmsnorm_rows_f32(h2, norm_w, eps) if h.dtype == F32 else K.rmsnorm_rows(h2, norm_w, eps)
+        ctx.save_for_backward(h, norm_w, rstd)
+        ctx.eps = eps
+        return K.unaliased(xn.contiguous(), h.shape)
+
+    @staticmethod
+    def backward(ctx, g):
+        h, norm_w, rstd = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            return (*graph_grads(lambda x, w: rms_norm_f32(x.float(), w, ctx.eps), (h, norm_w),
+                                 ctx.needs_input_grad[:2], g), None)
+        h2, g2 = h.reshape(-1, h.shape[-1]), g.to(BF16).contiguous().reshape(-1, h.shape[-1])
+        dh, dw = (K.rmsnorm_backward_f32 if h.dtype == F32 else K.rmsnorm_backward)(h2, norm_w, rstd, g2)
+        return dh.reshape(h.shape), dw, None
+
+
 def lm_head_ok(h, norm, norm_type, head, weight) -> bool:
     """True if lm_head takes the model's last step, weight @ norm(h): plain
     modules (head: the nn.Linear that holds weight, or None for a tied one) in

@@ -1,0 +1,614 @@
+// Losses over a vocabulary (gfx950): cross entropy against labels and the
+// divergence from a teacher's top logits, of logits that the caller holds or
+// of hidden rows through the head's weight, with their gradients.
+//
+// Row r has words i with shares q_i (sum 1; a label is one word of share 1), a
+// weight w_r and logits z; with the temperature T and p = softmax(z / T)
+//   l_r = T^2 sum_i q_i (ln q_i - ln p_i),  loss = sum_r w_r l_r / n
+//   d loss / d z_j = T w_r / n (p_j - sum_{i: word i = j} q_i)
+// where n is the sum of the weights (mean) or 1 (sum).  A row of weight 0, one
+// whose label is the ignored one and one without words count for nothing, what
+// is in them included: their gradient is 0 and n leaves them out.
+//
+// Logits are kept in units of log2(e) / T behind the first load, so an
+// exponential is one v_exp_f32.  Sums over rows are in 64 bits and in a fixed
+// order.
+#include "abi.h"
+#include "common.h"
+
+namespace moc {
+namespace {
+
+constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr int kMaxWords = 1024;
+constexpr int32_t kNoWord = 0x7FFFFFFF;  // behind the words of a row
+constexpr int32_t kUnknown = -2;         // a label outside the vocabulary
+
+// What the losses read of the targets, in one buffer (targets_layout).
+struct Targets {
+  double* total;    // sum of the weights (1 for a sum of losses)
+  float* factor;    // upstream gradient / total
+  float* weight;    // [rows], 0: the row counts for nothing
+  float* entropy;   // [rows] sum of q ln q (teacher only)
+  int32_t* ids;     // [rows][words] ascending, kNoWord behind the last
+  float* share;     // [rows][words] (teacher only); a word's second entry: -1
+};
+
+int64_t align256(int64_t n) { return (n + 255) & ~255LL; }
+
+// words = 0: labels.
+int64_t targets_layout(int64_t rows, int64_t words, char* base, Targets* t) {
+  int64_t at = 256;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += align256(bytes);
+    return base + here;
+  };
+  char* weight = take(rows * 4);
+  char* ids = take(rows * (words > 0 ? words : 1) * 4);
+  char* entropy = words > 0 ? take(rows * 4) : nullptr;
+  char* share = words > 0 ? take(rows * words * 4) : nullptr;
+  if (t != nullptr) {
+    t->total = reinterpret_cast<double*>(base);
+    t->factor = reinterpret_cast<float*>(base + 8);
+    t->weight = reinterpret_cast<float*>(weight);
+    t->ids = reinterpret_cast<int32_t*>(ids);
+    t->entropy = reinterpret_cast<float*>(entropy);
+    t->share = reinterpret_cast<float*>(share);
+  }
+  return at;
+}
+
+// Sum or maximum over a workgroup of up to 1024 threads, in wave order.
+template <bool MAX>
+__device__ __forceinline__ float block_reduce(float v, float* red) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  if (MAX) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  } else {
+    v = wave_sum(v);
+  }
+  __syncthreads();
+  if (lane == 0) red[wave] = v;
+  __syncthreads();
+  float t = red[0];
+  for (int w = 1; w < waves; ++w) t = MAX ? fmaxf(t, red[w]) : t + red[w];
+  return t;
+}
+
+__device__ __forceinline__ double block_sum64(double v, double* red) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if (lane == 0) red[wave] = v;
+  __syncthreads();
+  double t = red[0];
+  for (int w = 1; w < waves; ++w) t += red[w];
+  return t;
+}
+
+// ------------------------------------------------------------------ targets
+__global__ __launch_bounds__(256) void label_targets_kernel(const int64_t* __restrict__ labels, int64_t rows,
+                                                            int64_t vocab, int64_t ignore,
+                                                            const float* __restrict__ row_weight, Targets t) {
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (r >= rows) return;
+  const int64_t label = labels[r];
+  t.weight[r] = label == ignore ? 0.f : row_weight != nullptr ? row_weight[r] : 1.f;
+  t.ids[r] = label == ignore ? kNoWord : label >= 0 && label < vocab ? static_cast<int32_t>(label) : kUnknown;
+}
+
+// One workgroup a row.  Words sorted by rank (ties by place); entries of the
+// same word become one with the sum of their shares.
+template <typename ID, bool TOP_F32>
+__global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restrict__ ids, int64_t ids_ld,
+                                                              const void* __restrict__ top, int64_t top_ld, int words,
+                                                              int64_t vocab, float heat,
+                                                              const float* __restrict__ row_weight, Targets t) {
+  __shared__ int32_t id[kMaxWords], sorted_id[kMaxWords];
+  __shared__ float q[kMaxWords], sorted_q[kMaxWords];
+  __shared__ float red[4];
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x;
+  float mx = -INFINITY, any = 0.f;
+  bool bad = false;
+  for (int k = tid; k < words; k += 256) {
+    const int64_t word = static_cast<int64_t>(ids[r * ids_ld + k]);
+    const float x = (TOP_F32 ? static_cast<const float*>(top)[r * top_ld + k]
+                             : bf16_to_f32(static_cast<const uint16_t*>(top)[r * top_ld + k])) / heat;
+    const bool there = word >= 0 && word < vocab && x != -INFINITY;
+    id[k] = there ? static_cast<int32_t>(word) : kNoWord;
+    q[k] = there ? x : -INFINITY;
+    if (there) {
+      any = 1.f;
+      mx = fmaxf(mx, x);
+      bad |= !(x < INFINITY);
+    }
+  }
+  any = block_reduce<true>(any, red);
+  if (any == 0.f) {  // uniform: no words
+    for (int k = tid; k < words; k += 256) {
+      t.ids[r * words + k] = kNoWord;
+      t.share[r * words + k] = -1.f;
+    }
+    if (tid == 0) {
+      t.weight[r] = 0.f;
+      t.entropy[r] = 0.f;
+    }
+    return;
+  }
+  mx = block_reduce<true>(bad ? INFINITY : mx, red);
+  float sum = 0.f;
+  for (int k = tid; k < words; k += 256) {
+    const float e = id[k] == kNoWord ? 0.f : exp2f((q[k] - mx) * kLog2E);
+    sum += e;
+    q[k] = e;
+  }
+  sum = block_reduce<false>(sum, red);  // its barriers publish id and q
+  for (int k = tid; k < words; k += 256) {
+    const int32_t mine = id[k];
+    int rank = 0;
+    for (int j = 0; j < words; ++j) rank += id[j] < mine || (id[j] == mine && j < k);
+    sorted_id[rank] = mine;
+    sorted_q[rank] = q[k] / sum;
+  }
+  __syncthreads();
+  float h = 0.f;
+  for (int k = tid; k < words; k += 256) {
+    const int32_t mine = sorted_id[k];
+    float share = -1.f;
+    if (mine != kNoWord && (k == 0 || sorted_id[k - 1] != mine)) {
+      share = sorted_q[k];
+      for (int j = k + 1; j < words && sorted_id[j] == mine; ++j) share += sorted_q[j];
+      h += share > 0.f || share != share ? share * logf(share) : 0.f;
+    }
+    t.ids[r * words + k] = mine;
+    t.share[r * words + k] = share;
+  }
+  h = block_reduce<false>(h, red);
+  if (tid == 0) {
+    t.weight[r] = row_weight != nullptr ? row_weight[r] : 1.f;
+    t.entropy[r] = h;
+  }
+}
+
+// total = sum of the weights or 1, factor = grad / total.  One workgroup.
+__global__ __launch_bounds__(1024) void target_total_kernel(int64_t rows, int mean, const float* __restrict__ grad,
+                                                            Targets t) {
+  __shared__ double red[16];
+  double s = 0;
+  if (mean)
+    for (int64_t r = threadIdx.x; r < rows; r += 1024) s += t.weight[r];
+  s = mean ? block_sum64(s, red) : 1.0;
+  if (threadIdx.x == 0) {
+    *t.total = s;
+    *t.factor = static_cast<float>((grad != nullptr ? static_cast<double>(*grad) : 1.0) / s);
+  }
+}
+
+// loss = sum of the rows' weighted losses / total.  One workgroup.
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const float* __restrict__ row_loss, int64_t rows,
+                                                        const double* __restrict__ total, float* __restrict__ loss) {
+  __shared__ double red[16];
+  double s = 0;
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) s += row_loss[r];
+  s = block_sum64(s, red);
+  if (threadIdx.x == 0) *loss = static_cast<float>(s / *total);
+}
+
+// ------------------------------------------------------------------- logits
+template <typename T> struct Elem;
+template <> struct Elem<uint16_t> {
+  static constexpr int kPer = 8;  // elements of a 16-byte chunk
+  static __device__ __forceinline__ float get(const uint4& v, int e) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    return __uint_as_float((e & 1) ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
+  }
+  static __device__ __forceinline__ float one(uint16_t x) { return bf16_to_f32(x); }
+  static __device__ __forceinline__ uint16_t of(float f) { return bf16_rne(f); }
+};
+template <> struct Elem<float> {
+  static constexpr int kPer = 4;
+  static __device__ __forceinline__ float get(const uint4& v, int e) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    return __uint_as_float(w[e]);
+  }
+  static __device__ __forceinline__ float one(float x) { return x; }
+  static __device__ __forceinline__ float of(float f) { return f; }
+};
+
+// One workgroup a row: maximum, sum, loss, then the gradient (dx may be x).
+template <typename IN, typename OUT>
+__global__ __launch_bounds__(512) void logits_loss_kernel(const IN* x, int64_t ld, int vocab, Targets t, int words,
+                                                          float heat, float* __restrict__ row_loss, OUT* dx,
+                                                          int64_t ldd) {
+  __shared__ float red[8], at_word[kMaxWords];
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x;
+  const float w = t.weight[r];
+  const IN* row = x + r * ld;
+  OUT* out = dx + r * ldd;
+  if (w == 0.f) {  // uniform
+    if (dx != nullptr)
+      for (int j = tid; j < vocab; j += 512) out[j] = Elem<OUT>::of(0.f);
+    if (tid == 0) row_loss[r] = 0.f;
+    return;
+  }
+  const float unit = kLog2E / heat;
+  float mx = -INFINITY;
+  for (int j = tid; j < vocab; j += 512) mx = fmaxf(mx, Elem<IN>::one(row[j]) * unit);
+  mx = block_reduce<true>(mx, red);
+  float sum = 0.f;
+  for (int j = tid; j < vocab; j += 512) sum += exp2f(Elem<IN>::one(row[j]) * unit - mx);
+  sum = block_reduce<false>(sum, red);
+  const float lse = mx + log2f(sum);
+  const int n = words > 0 ? words : 1;
+  const int32_t* ids = t.ids + r * n;
+  float cross = 0.f;
+  bool unknown = false;
+  for (int k = tid; k < n; k += 512) {
+    const int32_t id = ids[k];
+    unknown |= id == kUnknown;
+    const float share = words > 0 ? t.share[r * n + k] : 1.f;
+    if (id < 0 || id == kNoWord || share == -1.f) continue;
+    const float l = Elem<IN>::one(row[id]) * unit - lse;  // log2 p
+    at_word[k] = l;
+    if (share != 0.f) cross -= share * l;
+  }
+  cross = block_reduce<false>(unknown ? NAN : cross, red);
+  const float loss = heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f));
+  if (tid == 0) row_loss[r] = w * loss;
+  if (dx == nullptr) return;
+  const float c = cross == cross ? heat * w * *t.factor : NAN;
+  for (int j = tid; j < vocab; j += 512) out[j] = Elem<OUT>::of(c * exp2f(Elem<IN>::one(row[j]) * unit - lse));
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stored before the words' own
+  __syncthreads();
+  for (int k = tid; k < n; k += 512) {
+    const int32_t id = ids[k];
+    const float share = words > 0 ? t.share[r * n + k] : 1.f;
+    if (id < 0 || id == kNoWord || share == -1.f) continue;
+    out[id] = Elem<OUT>::of(c * (exp2f(at_word[k]) - share));
+  }
+}
+
+// Rows that count, zeros for the others: what is in those reaches no product.
+template <typename T>
+__global__ __launch_bounds__(256) void counted_rows_kernel(const T* __restrict__ h, int64_t ldh, int hidden,
+                                                           const float* __restrict__ weight, T* __restrict__ out,
+                                                           int64_t ldo) {
+  const int64_t r = blockIdx.x;
+  const bool counts = weight[r] != 0.f;
+  for (int j = threadIdx.x; j < hidden; j += 256) out[r * ldo + j] = counts ? h[r * ldh + j] : T(0);
+}
+
+// a += b over n values; out (may be null): the sum as bf16 or f32.
+template <typename OUT>
+__global__ __launch_bounds__(256) void add_f32_kernel(float* a, const float* __restrict__ b, int64_t n, OUT* out) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) {
+    const float s = a[i] + b[i];
+    if (out != nullptr) out[i] = Elem<OUT>::of(s);
+    else a[i] = s;
+  }
+}
+
+// out[i][j] = a_i b_j, the product over one row or one word (the engine takes no
+// operand of one element's pitch).  Columns blockIdx.x, rows blockIdx.y and on.
+template <typename T, typename OUT>
+__global__ __launch_bounds__(256) void outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b,
+                                                    int64_t m, int64_t n, OUT* __restrict__ out) {
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (j >= n) return;
+  const float bj = Elem<T>::one(b[j]);
+  for (int64_t i = blockIdx.y; i < m; i += gridDim.y) out[i * n + j] = Elem<OUT>::of(Elem<T>::one(a[i * lda]) * bj);
+}
+
+// p *= *g in place; leaves at once where *g is 1.
+template <typename T>
+__global__ __launch_bounds__(256) void scale_kernel(T* __restrict__ p, int64_t n, const float* __restrict__ g) {
+  const float f = *g;
+  if (f == 1.f) return;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step)
+    p[i] = Elem<T>::of(Elem<T>::one(p[i]) * f);
+}
+
+unsigned blocks_of(int64_t n) {
+  const int64_t b = (n + 255) / 256;
+  return static_cast<unsigned>(b < 1 ? 1 : b > 4096 ? 4096 : b);
+}
+
+// ------------------------------------------------------------------- pieces
+// Logits exist for a piece of the rows at a time, within about this many bytes.
+constexpr int64_t kPieceBytes = 1LL << 30;
+
+struct Pieces {
+  int64_t rows, count;     // rows of a piece, pieces
+  int64_t ldz;             // row pitch of a piece's logits
+  int64_t z, d, x, acc, part, bytes;  // offsets in the workspace
+  int64_t ldx;
+};
+
+Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, bool grads) {
+  Pieces p{};
+  const bool f32 = dtype == MOC_F32;
+  p.ldz = (vocab + 63) & ~63LL;
+  const int64_t each = p.ldz * (grads && !f32 ? 6 : 4);
+  int64_t n = kPieceBytes / each / 256 * 256;
+  if (n < 256) n = 256;
+  if (n > rows) n = rows < 1 ? 1 : rows;
+  p.rows = n;
+  p.count = rows < 1 ? 0 : (rows + n - 1) / n;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  p.z = take(n * p.ldz * 4);
+  p.d = grads && !f32 ? take(n * p.ldz * 2) : p.z;
+  p.ldx = (hidden + 63) & ~63LL;
+  p.x = grads ? take(rows * p.ldx * (f32 ? 4 : 2)) : 0;
+  if (grads && p.count > 1) {
+    p.acc = take(vocab * hidden * 4);
+    p.part = take(vocab * hidden * 4);
+  }
+  p.bytes = at;
+  return p;
+}
+
+int logits_rows(bool in_f32, bool out_f32, const void* x, int64_t rows, int64_t vocab, int64_t ld, const Targets& t,
+                int64_t words, float heat, float* row_loss, void* dx, int64_t ldd, hipStream_t st) {
+  if (rows == 0) return MOC_OK;
+  const dim3 grid(static_cast<unsigned>(rows));
+  const int v = static_cast<int>(vocab), k = static_cast<int>(words);
+  if (in_f32 && out_f32)
+    logits_loss_kernel<float, float><<<grid, 512, 0, st>>>(static_cast<const float*>(x), ld, v, t, k, heat, row_loss,
+                                                           static_cast<float*>(dx), ldd);
+  else if (in_f32)
+    logits_loss_kernel<float, uint16_t><<<grid, 512, 0, st>>>(static_cast<const float*>(x), ld, v, t, k, heat,
+                                                              row_loss, static_cast<uint16_t*>(dx), ldd);
+  else
+    logits_loss_kernel<uint16_t, uint16_t><<<grid, 512, 0, st>>>(static_cast<const uint16_t*>(x), ld, v, t, k, heat,
+                                                                 row_loss, static_cast<uint16_t*>(dx), ldd);
+  return check_launch("logits_loss_kernel");
+}
+
+// C [M, N] = A B over K = 1, as moc_gemm_ws of these strides would.
+int outer(int dtype, int64_t m, int64_t n, const void* a, int64_t lda, const void* b, void* c, int c_dtype,
+          hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>((n + 255) / 256), static_cast<unsigned>(m < 8192 ? m : 8192));
+  if (dtype == MOC_F32)
+    outer_kernel<float, float><<<grid, 256, 0, st>>>(static_cast<const float*>(a), lda, static_cast<const float*>(b), m,
+                                                     n, static_cast<float*>(c));
+  else if (c_dtype == MOC_F32)
+    outer_kernel<uint16_t, float><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(a), lda,
+                                                        static_cast<const uint16_t*>(b), m, n, static_cast<float*>(c));
+  else
+    outer_kernel<uint16_t, uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(a), lda,
+                                                           static_cast<const uint16_t*>(b), m, n,
+                                                           static_cast<uint16_t*>(c));
+  return check_launch("outer_kernel");
+}
+
+bool sizes_ok(int64_t rows, int64_t vocab, int64_t words) {
+  return rows >= 0 && rows <= (1LL << 24) && vocab >= 1 && vocab <= (1LL << 24) && words >= 0 && words <= kMaxWords;
+}
+
+}  // namespace
+}  // namespace moc
+
+using namespace moc;
+
+#define MOC_SIZES(name)                                                                                          \
+  MOC_REQUIRE(sizes_ok(rows, vocab, words), "%s: up to 2^24 rows, a vocabulary of up to 2^24 words, up to %d of " \
+                                            "them a row", name, kMaxWords)
+
+extern "C" int64_t moc_loss_targets_size(int64_t rows, int64_t words) {
+  if (!sizes_ok(rows, 1, words)) return 0;
+  return targets_layout(rows, words, nullptr, nullptr);
+}
+
+extern "C" int moc_label_targets(const int64_t* labels, int64_t rows, int64_t vocab, int64_t ignore_index,
+                                 const float* row_weight, int mean, const float* grad, void* targets, void* stream) {
+  const int64_t words = 0;
+  MOC_SIZES("moc_label_targets");
+  MOC_REQUIRE((labels != nullptr || rows == 0) && targets != nullptr && aligned16(targets),
+              "moc_label_targets: null operand or unaligned targets");
+  hipStream_t st = as_stream(stream);
+  Targets t;
+  targets_layout(rows, 0, static_cast<char*>(targets), &t);
+  if (rows > 0) {
+    label_targets_kernel<<<static_cast<unsigned>((rows + 255) / 256), 256, 0, st>>>(labels, rows, vocab, ignore_index,
+                                                                                    row_weight, t);
+    const int rc = check_launch("label_targets_kernel");
+    if (rc != MOC_OK) return rc;
+  }
+  target_total_kernel<<<1, 1024, 0, st>>>(rows, mean, grad, t);
+  return check_launch("target_total_kernel");
+}
+
+extern "C" int moc_teacher_targets(const void* ids, int ids_dtype, int64_t ids_ld, const void* top, int top_dtype,
+                                   int64_t top_ld, int64_t rows, int64_t words, int64_t vocab, float temperature,
+                                   const float* row_weight, int mean, const float* grad, void* targets,
+                                   void* stream) {
+  MOC_SIZES("moc_teacher_targets");
+  MOC_REQUIRE(words >= 1, "moc_teacher_targets: a word a row at least");
+  MOC_REQUIRE((ids_dtype == MOC_I32 || ids_dtype == MOC_I64) && (top_dtype == MOC_BF16 || top_dtype == MOC_F32),
+              "moc_teacher_targets: ids are int32 or int64, the teacher's logits bf16 or f32");
+  MOC_REQUIRE(temperature > 0.f && temperature < INFINITY, "moc_teacher_targets: the temperature must be above 0");
+  MOC_REQUIRE(rows == 0 || (ids != nullptr && top != nullptr && (rows == 1 || (ids_ld >= words && top_ld >= words))),
+              "moc_teacher_targets: null operand or rows that overlap");
+  MOC_REQUIRE(targets != nullptr && aligned16(targets), "moc_teacher_targets: null or unaligned targets");
+  hipStream_t st = as_stream(stream);
+  Targets t;
+  targets_layout(rows, words, static_cast<char*>(targets), &t);
+  if (rows > 0) {
+    const dim3 grid(static_cast<unsigned>(rows));
+    const int k = static_cast<int>(words);
+#define MOC_TEACHER(ID, F)                                                                                          \
+  teacher_targets_kernel<ID, F><<<grid, 256, 0, st>>>(static_cast<const ID*>(ids), ids_ld, top, top_ld, k, vocab, \
+                                                      temperature, row_weight, t)
+    if (ids_dtype == MOC_I32 && top_dtype == MOC_F32) MOC_TEACHER(int32_t, true);
+    else if (ids_dtype == MOC_I32) MOC_TEACHER(int32_t, false);
+    else if (top_dtype == MOC_F32) MOC_TEACHER(int64_t, true);
+    else MOC_TEACHER(int64_t, false);
+#undef MOC_TEACHER
+    const int rc = check_launch("teacher_targets_kernel");
+    if (rc != MOC_OK) return rc;
+  }
+  target_total_kernel<<<1, 1024, 0, st>>>(rows, mean, grad, t);
+  return check_launch("target_total_kernel");
+}
+
+extern "C" int moc_logits_loss(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t ld, void* targets,
+                               int64_t words, float temperature, float* row_loss, float* loss, void* dlogits,
+                               int64_t ldd, void* stream) {
+  MOC_SIZES("moc_logits_loss");
+  MOC_REQUIRE(dtype == MOC_BF16 || dtype == MOC_F32, "moc_logits_loss: logits are bf16 or f32");
+  MOC_REQUIRE(temperature > 0.f && temperature < INFINITY, "moc_logits_loss: the temperature must be above 0");
+  MOC_REQUIRE(targets != nullptr && (rows == 0 || (logits != nullptr && row_loss != nullptr)),
+              "moc_logits_loss: null operand");
+  MOC_REQUIRE(rows <= 1 || (ld >= vocab && (dlogits == nullptr || ldd >= vocab)), "moc_logits_loss: rows that overlap");
+  hipStream_t st = as_stream(stream);
+  Targets t;
+  targets_layout(rows, words, static_cast<char*>(targets), &t);
+  const bool f32 = dtype == MOC_F32;
+  int rc = logits_rows(f32, f32, logits, rows, vocab, ld, t, words, temperature, row_loss, dlogits, ldd, st);
+  if (rc != MOC_OK || loss == nullptr) return rc;
+  loss_sum_kernel<<<1, 1024, 0, st>>>(row_loss, rows, t.total, loss);
+  return check_launch("loss_sum_kernel");
+}
+
+extern "C" int64_t moc_linear_loss_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int grads) {
+  if (!sizes_ok(rows, vocab, 0) || hidden < 1) return 0;
+  return pieces_of(dtype, rows, hidden, vocab, grads != 0).bytes;
+}
+
+extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab,
+                                                       int grads) {
+  if (!sizes_ok(rows, vocab, 0) || hidden < 1) return 0;
+  const Pieces p = pieces_of(dtype, rows, hidden, vocab, grads != 0);
+  int64_t most = 0;
+  for (int64_t i = 0; i < p.count; i += p.count > 1 ? p.count - 1 : 1) {  // the first piece and the last
+    const int64_t n = i + 1 < p.count ? p.rows : rows - i * p.rows;
+    int64_t b = moc_gemm_workspace_size(dtype, n, vocab, hidden, 0);
+    if (b > most) most = b;
+    if (!grads) continue;
+    b = moc_gemm_workspace_size(dtype, n, hidden, vocab, 0);
+    if (b > most) most = b;
+    b = moc_gemm_workspace_size(dtype, vocab, hidden, n, 0);
+    if (b > most) most = b;
+  }
+  return most;
+}
+
+extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w,
+                               int64_t vocab, int64_t ldw, void* targets, int64_t words, float temperature,
+                               float* row_loss, float* loss, void* dh, int dh_dtype, void* dw, int dw_dtype,
+                               void* workspace, int64_t workspace_bytes, void* gemm_ws, int64_t gemm_ws_bytes,
+                               void* stream) {
+  MOC_SIZES("moc_linear_loss");
+  MOC_REQUIRE(dtype == MOC_BF16 || dtype == MOC_F32, "moc_linear_loss: operands are bf16 or f32");
+  const bool f32 = dtype == MOC_F32;
+  const int es = f32 ? 4 : 2;
+  MOC_REQUIRE(hidden >= 1 && hidden <= (1 << 20), "moc_linear_loss: hidden size of 1 to 2^20");
+  MOC_REQUIRE(temperature > 0.f && temperature < INFINITY, "moc_linear_loss: the temperature must be above 0");
+  MOC_REQUIRE(targets != nullptr && w != nullptr && (rows == 0 || (h != nullptr && row_loss != nullptr)),
+              "moc_linear_loss: null operand");
+  MOC_REQUIRE(aligned16(h) && aligned16(w) && ldh * es % 16 == 0 && ldw * es % 16 == 0 && ldh >= hidden &&
+                  ldw >= hidden,
+              "moc_linear_loss: operands need 16-byte aligned rows");
+  MOC_REQUIRE(f32 || vocab * ldw * 2 < (1LL << 31) - 1024, "moc_linear_loss: a bf16 weight of up to 2 GiB");
+  MOC_REQUIRE((dh == nullptr || (dh_dtype == MOC_F32 || (dh_dtype == MOC_BF16 && !f32))) &&
+                  (dw == nullptr || (dw_dtype == MOC_F32 || (dw_dtype == MOC_BF16 && !f32))),
+              "moc_linear_loss: gradients are f32, or bf16 of bf16 operands");
+  const bool grads = dh != nullptr || dw != nullptr;
+  const Pieces p = pieces_of(dtype, rows, hidden, vocab, grads);
+  MOC_REQUIRE(workspace_bytes >= p.bytes && (workspace != nullptr || p.bytes == 0) && aligned16(workspace),
+              "moc_linear_loss: workspace of %lld bytes needed", (long long)p.bytes);
+  MOC_REQUIRE(f32 || p.rows * p.ldx * 2 < (1LL << 31) - 1024, "moc_linear_loss: hidden rows of a piece up to 2 GiB");
+  hipStream_t st = as_stream(stream);
+  Targets t;
+  targets_layout(rows, words, static_cast<char*>(targets), &t);
+  char* ws = static_cast<char*>(workspace);
+  const int64_t n_words = words > 0 ? words : 1;
+  int rc;
+  if (grads && rows > 0) {
+    const dim3 grid(static_cast<unsigned>(rows));
+    if (f32)
+      counted_rows_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(h), ldh, (int)hidden, t.weight,
+                                                       reinterpret_cast<float*>(ws + p.x), p.ldx);
+    else
+      counted_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(h), ldh, (int)hidden, t.weight,
+                                                          reinterpret_cast<uint16_t*>(ws + p.x), p.ldx);
+    if ((rc = check_launch("counted_rows_kernel")) != MOC_OK) return rc;
+  }
+  const char* x = grads ? ws + p.x : static_cast<const char*>(h);
+  const int64_t ldx = grads ? p.ldx : ldh;
+  for (int64_t i = 0; i < p.count; ++i) {
+    const int64_t r0 = i * p.rows, n = rows - r0 < p.rows ? rows - r0 : p.rows;
+    const char* xi = x + r0 * ldx * es;
+    rc = moc_gemm_ws(dtype, n, vocab, hidden, xi, ldx, 1, w, 1, ldw, 0, nullptr, 0, 0, nullptr, 0, 0, ws + p.z, p.ldz,
+                     MOC_F32, gemm_ws, gemm_ws_bytes, stream);
+    if (rc != MOC_OK) return rc;
+    Targets ti = t;
+    ti.weight += r0;
+    ti.ids += r0 * n_words;
+    if (words > 0) {
+      ti.entropy += r0;
+      ti.share += r0 * words;
+    }
+    rc = logits_rows(true, f32, ws + p.z, n, vocab, p.ldz, ti, words, temperature, row_loss + r0,
+                     grads ? ws + p.d : nullptr, p.ldz, st);
+    if (rc != MOC_OK) return rc;
+    if (dh != nullptr) {
+      char* to = static_cast<char*>(dh) + r0 * hidden * (dh_dtype == MOC_F32 ? 4 : 2);
+      rc = vocab == 1 ? outer(dtype, n, hidden, ws + p.d, p.ldz, w, to, dh_dtype, st)
+                      : moc_gemm_ws(dtype, n, hidden, vocab, ws + p.d, p.ldz, 1, w, ldw, 1, 0, nullptr, 0, 0, nullptr, 0,
+                                    0, to, hidden, dh_dtype, gemm_ws, gemm_ws_bytes, stream);
+      if (rc != MOC_OK) return rc;
+    }
+    if (dw != nullptr) {
+      const bool one = p.count == 1;
+      char* to = one ? static_cast<char*>(dw) : ws + (i == 0 ? p.acc : p.part);
+      const int to_dtype = one ? dw_dtype : MOC_F32;
+      rc = n == 1 ? outer(dtype, vocab, hidden, ws + p.d, 1, xi, to, to_dtype, st)
+                  : moc_gemm_ws(dtype, vocab, hidden, n, ws + p.d, 1, p.ldz, xi, ldx, 1, 0, nullptr, 0, 0, nullptr, 0, 0,
+                                to, hidden, to_dtype, gemm_ws, gemm_ws_bytes, stream);
+      if (rc != MOC_OK) return rc;
+      if (i > 0) {
+        float* acc = reinterpret_cast<float*>(ws + p.acc);
+        const float* part = reinterpret_cast<const float*>(ws + p.part);
+        const int64_t size = vocab * hidden;
+        void* out = i + 1 == p.count ? dw : nullptr;
+        if (dw_dtype == MOC_F32)
+          add_f32_kernel<float><<<blocks_of(size), 256, 0, st>>>(acc, part, size, static_cast<float*>(out));
+        else
+          add_f32_kernel<uint16_t><<<blocks_of(size), 256, 0, st>>>(acc, part, size, static_cast<uint16_t*>(out));
+        if ((rc = check_launch("add_f32_kernel")) != MOC_OK) return rc;
+      }
+    }
+  }
+  if (rows == 0 && dw != nullptr) {
+    rc = moc_fill_zero(dw, vocab * hidden * (dw_dtype == MOC_F32 ? 4 : 2), stream);
+    if (rc != MOC_OK) return rc;
+  }
+  if (loss == nullptr) return MOC_OK;
+  loss_sum_kernel<<<1, 1024, 0, st>>>(row_loss, rows, t.total, loss);
+  return check_launch("loss_sum_kernel");
+}
+
+extern "C" int moc_scale_inplace(int dtype, void* p, int64_t n, const float* factor, void* stream) {
+  MOC_REQUIRE(dtype == MOC_BF16 || dtype == MOC_F32, "moc_scale_inplace: bf16 or f32");
+  MOC_REQUIRE(n >= 0 && (n == 0 || p != nullptr) && factor != nullptr, "moc_scale_inplace: null operand");
+  if (n == 0) return MOC_OK;
+  hipStream_t st = as_stream(stream);
+  if (dtype == MOC_F32)
+    scale_kernel<float><<<blocks_of(n), 256, 0, st>>>(static_cast<float*>(p), n, factor);
+  else
+    scale_kernel<uint16_t><<<blocks_of(n), 256, 0, st>>>(static_cast<uint16_t*>(p), n, factor);
+  return check_launch("scale_kernel");
+}

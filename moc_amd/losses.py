@@ -1,0 +1,374 @@
+"""Losses over a vocabulary: cross entropy against labels and the divergence from
+a teacher's top logits (moc_amd/csrc/vocab_loss.hip).
+
+    linear_cross_entropy(hidden, weight, labels)            the head's product and
+    linear_distillation(hidden, weight, ids, top)           the loss as one operator
+    distillation_loss(logits, ids, top)                     of logits already there
+
+The first two never hold the logits of all rows: they exist for a piece of the rows
+at a time (at most 1 GiB), and the gradients of hidden rows and weight are computed
+in the forward pass, while the piece is there, so that a backward has nothing left to
+do but the upstream factor.  A second backward of the same graph, and a backward
+captured into a HIP graph without its forward, compute them again; reduction="none"
+computes them in the backward, by the upstream gradient of each row.
+
+Row r has a weight w_r (row_weight, 1 without), words with shares q (a label: one of
+share 1) and logits z; with the temperature T, p = softmax(z / T),
+
+    l_r = T^2 sum_i q_i (ln q_i - ln p_i)        (labels, T = 1: -ln p_label)
+
+"mean" is sum w_r l_r / sum w_r, "sum" the sum and "none" w_r l_r for each row.  A row
+of weight 0, one whose label is ignore_index and one without words count for nothing,
+NaN in their hidden rows or logits included: they have loss and gradient 0 and are left
+out of the mean, which is NaN where no row is left.  A label outside the vocabulary
+gives NaN, as do NaN logits in rows that count.
+
+Losses are f32.  Operands are bf16 or f32, or either under bf16 autocast, where the
+products are those of bf16 casts and gradients come in the operands' own types.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _native as N
+from . import kernels as K
+from .block import graph_grads, plain
+
+BF16, F32 = torch.bfloat16, torch.float32
+REDUCTIONS = ("mean", "sum", "none")
+
+
+def linear_cross_entropy(hidden, weight, labels, row_weight=None, *, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy of the logits hidden @ weight.T against labels: hidden [..., d],
+    weight [vocab, d], labels [...] (int64), row_weight [...] (f32)."""
+    rows = _rows_of("linear_cross_entropy", hidden, labels, row_weight, reduction)
+    targets = _Labels(labels.reshape(rows).contiguous(), _flat(row_weight, rows), int(ignore_index), reduction)
+    return _linear("linear_cross_entropy", hidden, weight, targets)
+
+
+def linear_distillation(hidden, weight, teacher_ids, teacher_logits, row_weight=None, *, temperature: float = 1.0,
+                        reduction: str = "mean") -> torch.Tensor:
+    """Divergence of softmax(hidden @ weight.T / temperature) from a teacher that is
+    known by its top logits: teacher_ids [..., words] (int32 or int64) and
+    teacher_logits [..., words] (bf16 or f32), up to 1024 words a row in any order; q =
+    softmax(teacher_logits / temperature) over the words given.  An id outside the
+    vocabulary (-1, say) or a logit of -infinity is no word, ids that stand twice in a
+    row add up.  Teacher and row_weight get no gradient."""
+    rows = _rows_of("linear_distillation", hidden, None, row_weight, reduction)
+    targets = _teacher("linear_distillation", hidden, teacher_ids, teacher_logits, row_weight, rows, temperature,
+                       reduction)
+    return _linear("linear_distillation", hidden, weight, targets)
+
+
+def distillation_loss(logits, teacher_ids, teacher_logits, row_weight=None, *, temperature: float = 1.0,
+                      reduction: str = "mean") -> torch.Tensor:
+    """linear_distillation of logits [..., vocab] (bf16 or f32) that are there already."""
+    what = "distillation_loss"
+    rows = _rows_of(what, logits, None, row_weight, reduction)
+    if logits.shape[-1] < 1:
+        raise ValueError(f"{what}: a vocabulary of one word at least")
+    targets = _teacher(what, logits, teacher_ids, teacher_logits, row_weight, rows, temperature, reduction)
+    dev = N.one_device(logits, *targets.tensors())
+    if not N.is_current(dev):
+        with torch.cuda.device(dev):
+            return _LogitsLoss.apply(targets, torch.is_grad_enabled(), logits, *targets.tensors())
+    return _LogitsLoss.apply(targets, torch.is_grad_enabled(), logits, *targets.tensors())
+
+
+# --------------------------------------------------------------------- targets
+def _rows_of(what: str, x, labels, row_weight, reduction: str) -> int:
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"{what}: reduction is one of {REDUCTIONS}, got {reduction!r}")
+    if x.dim() < 1 or x.dtype not in (BF16, F32):
+        raise ValueError(f"{what}: rows of bf16 or f32, got {x.dtype} {tuple(x.shape)}")
+    lead = x.shape[:-1]
+    if labels is not None and (labels.shape != lead or labels.dtype != torch.int64):
+        raise ValueError(f"{what}: labels are int64 {tuple(lead)}, got {labels.dtype} {tuple(labels.shape)}")
+    if row_weight is not None and (row_weight.shape != lead or row_weight.dtype != F32):
+        raise ValueError(f"{what}: row_weight is f32 {tuple(lead)}, got {row_weight.dtype} {tuple(row_weight.shape)}")
+    if row_weight is not None and row_weight.requires_grad:
+        raise ValueError(f"{what}: row_weight has no gradient here")
+    rows = math.prod(lead)
+    if rows > 1 << 24:
+        raise ValueError(f"{what}: up to 2^24 rows, got {rows}")
+    return rows
+
+
+def _flat(t, rows: int):
+    return None if t is None else t.reshape(rows).contiguous()
+
+
+class _Labels:
+    words, heat = 0, 1.0
+
+    def __init__(self, labels, row_weight, ignore: int, reduction: str):
+        self.labels, self.row_weight, self.ignore, self.reduction = labels, row_weight, ignore, reduction
+
+    def tensors(self):
+        return self.labels, None, self.row_weight
+
+    def write(self, saved, row_weight, mean: bool, grad, vocab: int, dev) -> torch.Tensor:
+        labels = saved[0]
+        rows = labels.shape[0]
+        out = torch.empty(N.query("moc_loss_targets_size", rows, 0), dtype=torch.uint8, device=labels.device)
+        N.call("moc_label_targets", labels.data_ptr(), rows, vocab, self.ignore, N.ptr(row_weight), mean,
+               N.ptr(grad), out.data_ptr(), N.stream_on(dev))
+        return out
+
+    def rows_f32(self, saved, z):
+        """Each row's loss by f32 tensor operations, and whether it counts."""
+        labels = saved[0]
+        counts = labels != self.ignore
+        z = torch.where(counts[:, None], z, 0.0)
+        known = counts & (labels >= 0) & (labels < z.shape[1])
+        each = -torch.log_softmax(z, -1).gather(1, torch.where(known, labels, 0)[:, None])[:, 0]
+        return torch.where(known, each, math.nan), counts
+
+
+class _Teacher:
+    def __init__(self, ids, top, row_weight, heat: float, reduction: str):
+        self.ids, self.top, self.row_weight, self.heat, self.reduction = ids, top, row_weight, heat, reduction
+        self.words = ids.shape[1]
+
+    def tensors(self):
+        return self.ids, self.top, self.row_weight
+
+    def write(self, saved, row_weight, mean: bool, grad, vocab: int, dev) -> torch.Tensor:
+        ids, top, _ = saved
+        rows, words = ids.shape
+        out = torch.empty(N.query("moc_loss_targets_size", rows, words), dtype=torch.uint8, device=ids.device)
+        N.call("moc_teacher_targets", ids.data_ptr(), N.idx_code(ids.dtype), ids.stride(0), top.data_ptr(),
+               N.dtype_code(top.dtype), top.stride(0), rows, words, vocab, self.heat, N.ptr(row_weight), mean,
+               N.ptr(grad), out.data_ptr(), N.stream_on(dev))
+        return out
+
+    def rows_f32(self, saved, z):
+        ids, top, _ = saved
+        ids, x = ids.long(), top.float() / self.heat
+        there = (ids >= 0) & (ids < z.shape[1]) & (x != -math.inf)
+        counts = there.any(1)
+        z = torch.where(counts[:, None], z, 0.0)
+        log_q = torch.log_softmax(torch.where(counts[:, None], torch.where(there, x, -math.inf), 0.0), 1)
+        q = torch.where(there, log_q.exp(), 0.0)
+        ids = torch.where(there, ids, 0)
+        # shares of one word added up, each entry weighing its own part of them
+        whole = torch.zeros_like(z).scatter_add(1, ids, q).gather(1, ids)
+        log_p = torch.log_softmax(z / self.heat, -1).gather(1, ids)
+        each = torch.where(q > 0, q * (torch.log(torch.where(q > 0, whole, 1.0)) - log_p), q)
+        return self.heat ** 2 * each.sum(1), counts
+
+
+def _teacher(what: str, x, ids, top, row_weight, rows: int, temperature: float, reduction: str) -> _Teacher:
+    lead = x.shape[:-1]
+    if ids.dim() != x.dim() or ids.shape[:-1] != lead or top.shape != ids.shape:
+        raise ValueError(f"{what}: the teacher's ids and logits are {(*lead, 'words')}, got {tuple(ids.shape)} and "
+                         f"{tuple(top.shape)}")
+    words = ids.shape[-1]
+    if not 1 <= words <= 1024:
+        raise ValueError(f"{what}: 1 to 1024 words of the teacher a row, got {words}")
+    if ids.dtype not in (torch.int32, torch.int64) or top.dtype not in (BF16, F32):
+        raise ValueError(f"{what}: the teacher's ids are int32 or int64 and its logits bf16 or f32, got {ids.dtype} and "
+                         f"{top.dtype}")
+    if top.requires_grad:
+        raise ValueError(f"{what}: the teacher has no gradient here")
+    temperature = float(temperature)
+    if not 0 < temperature < math.inf:
+        raise ValueError(f"{what}: the temperature must be above 0, got {temperature}")
+    return _Teacher(_unit(ids.reshape(rows, words)), _unit(top.reshape(rows, words)), _flat(row_weight, rows),
+                    temperature, reduction)
+
+
+def _unit(t):
+    """Rows that do not overlap, of unit stride."""
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) \
+        else t.contiguous()
+
+
+# -------------------------------------------------------------------- operands
+def _rows16(t) -> torch.Tensor:
+    """t [rows, cols] with 16-byte aligned rows of unit stride, a copy if it has others."""
+    rows, cols = t.shape
+    per = 16 // t.element_size()
+    if (t.stride(1) == 1 or cols == 1) and t.data_ptr() % 16 == 0 and (
+            rows <= 1 or (t.stride(0) % per == 0 and t.stride(0) >= cols)):
+        return t
+    out = K.padded_empty(rows, cols, t.dtype, t.device)
+    return out.copy_(t)
+
+
+def _pitch(t) -> int:
+    per = 16 // t.element_size()
+    return t.stride(0) if t.shape[0] > 1 else K.round_up(t.shape[1], per)
+
+
+def _linear(what: str, hidden, weight, targets) -> torch.Tensor:
+    if weight.dim() != 2 or weight.shape[1] != hidden.shape[-1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"{what}: weight is [vocab, {hidden.shape[-1]}], got {tuple(weight.shape)}")
+    if not plain(hidden, weight):
+        raise ValueError(f"{what}: plain tensors only")
+    product = hidden.dtype
+    if torch.is_autocast_enabled("cuda"):
+        product = torch.get_autocast_dtype("cuda")
+        if product != BF16:
+            raise ValueError(f"{what}: autocast to bf16, got {product}")
+        if weight.dtype not in (BF16, F32):
+            raise ValueError(f"{what}: weight is bf16 or f32, got {weight.dtype}")
+    elif weight.dtype != hidden.dtype:
+        raise ValueError(f"{what}: hidden and weight of one type (or under bf16 autocast), got {hidden.dtype} and "
+                         f"{weight.dtype}")
+    vocab, d = weight.shape
+    if vocab > 1 << 24 or d > 1 << 20:
+        raise ValueError(f"{what}: a vocabulary of up to 2^24 words, a hidden size of up to 2^20")
+    if product == BF16 and vocab * K.row_pitch(d, BF16) * 2 >= K.OPERAND_BYTES:
+        raise ValueError(f"{what}: a bf16 weight of up to 2 GiB")
+    dev = N.one_device(hidden, weight, *targets.tensors())
+    if not N.is_current(dev):
+        with torch.cuda.device(dev):
+            return _LinearLoss.apply(targets, product, torch.is_grad_enabled(), hidden, weight, *targets.tensors())
+    return _LinearLoss.apply(targets, product, torch.is_grad_enabled(), hidden, weight, *targets.tensors())
+
+
+def _linear_pass(targets, saved, row_weight, mean, grad, product, hidden, weight, loss: bool, dh: bool, dw: bool):
+    """(loss | None, the rows' losses, dhidden | None, dweight | None)."""
+    dev = hidden.get_device()
+    vocab, d = weight.shape
+    h = _rows16(hidden.reshape(-1, d).to(product))
+    w = _rows16(weight.to(product))
+    rows, grads = h.shape[0], dh or dw
+    code = N.dtype_code(product)
+    where = hidden.device
+    t = targets.write(saved, row_weight, mean, grad, vocab, dev)
+    each = torch.empty(rows, dtype=F32, device=where)
+    total = torch.empty((), dtype=F32, device=where) if loss else None
+    dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=where) if dh else None
+    dweight = torch.empty((vocab, d), dtype=weight.dtype, device=where) if dw else None
+    nbytes = N.query("moc_linear_loss_workspace_size", code, rows, d, vocab, grads)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
+    ngemm = N.query("moc_linear_loss_gemm_workspace_size", code, rows, d, vocab, grads)
+    gemm_ws = K._gemm_workspace(where, ngemm) if ngemm else None
+    N.call("moc_linear_loss", code, h.data_ptr(), rows, d, _pitch(h), w.data_ptr(), vocab, _pitch(w), t.data_ptr(),
+           targets.words, targets.heat, each.data_ptr(), N.ptr(total), N.ptr(dhidden), N.dtype_code(hidden.dtype),
+           N.ptr(dweight), N.dtype_code(weight.dtype), ws.data_ptr(), nbytes, N.ptr(gemm_ws), ngemm, N.stream_on(dev))
+    return total, each, dhidden, dweight
+
+
+def _reduced_f32(targets, saved, z):
+    """The operator by f32 tensor operations."""
+    each, counts = targets.rows_f32(saved, z)
+    row_weight = saved[2]
+    w = counts.float() if row_weight is None else torch.where(counts, row_weight, 0.0)
+    each = torch.where(w == 0, 0.0, each * w)
+    if targets.reduction == "none":
+        return each
+    return each.sum() / (w.sum() if targets.reduction == "mean" else 1.0)
+
+
+class _Kept:
+    """Gradients computed ahead, handed out once: the tensors go to the caller, scaled
+    in place, so that nothing of them is copied."""
+
+    def __init__(self, grads):
+        self.grads = grads
+        self.captured = torch.cuda.is_current_stream_capturing()
+
+    def take(self, g):
+        """The gradients times g, or None: gone, or those of an eager forward in a
+        captured backward, which a replay would scale again."""
+        grads, self.grads = self.grads, None
+        if grads is None or (torch.cuda.is_current_stream_capturing() and not self.captured):
+            return None
+        for t in grads:
+            if t is not None:
+                N.call("moc_scale_inplace", N.dtype_code(t.dtype), t.data_ptr(), t.numel(), g.data_ptr(), N.stream_of(t))
+        return grads
+
+
+def _row_factors(targets, saved, g):
+    """reduction="none": the rows' weights times their upstream gradients."""
+    g = g.reshape(-1).contiguous()
+    return g if saved[2] is None else g * saved[2]
+
+
+class _LinearLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, targets, product, grad_mode, hidden, weight, *saved):
+        dh, dw = (grad_mode and need for need in ctx.needs_input_grad[3:5])
+        ahead = targets.reduction != "none"
+        total, each, dhidden, dweight = _linear_pass(targets, saved, saved[2], targets.reduction == "mean", None, product,
+                                                     hidden, weight, ahead, ahead and dh, ahead and dw)
+        if dh or dw:
+            ctx.save_for_backward(hidden, weight, *saved)
+            ctx.targets, ctx.product = targets, product
+            ctx.kept = _Kept((dhidden, dweight) if ahead else None)
+        return total if ahead else each.view(hidden.shape[:-1])
+
+    @staticmethod
+    def backward(ctx, g):
+        hidden, weight, *saved = ctx.saved_tensors
+        targets = ctx.targets
+        dh, dw = ctx.needs_input_grad[3:5]
+        rest = (None,) * len(saved)
+        if torch.is_grad_enabled():
+            def stock(h, w):
+                z = (h.to(ctx.product).float() @ w.to(ctx.product).float().t()).reshape(-1, w.shape[0])
+                out = _reduced_f32(targets, saved, z)
+                return out.reshape(g.shape)
+            return (None, None, None, *graph_grads(stock, (hidden, weight), (dh, dw), g), *rest)
+        if targets.reduction == "none":
+            got = _linear_pass(targets, saved, _row_factors(targets, saved, g), False, None, ctx.product, hidden, weight,
+                               False, dh, dw)[2:]
+        else:
+            got = ctx.kept.take(g) or _linear_pass(targets, saved, saved[2], targets.reduction == "mean", g, ctx.product,
+                                                   hidden, weight, False, dh, dw)[2:]
+        return (None, None, None, *got, *rest)
+
+
+def _logits_pass(targets, saved, row_weight, mean, grad, logits, loss: bool, grads: bool):
+    """(loss | None, the rows' losses, dlogits | None)."""
+    dev = logits.get_device()
+    vocab = logits.shape[-1]
+    x = logits.reshape(-1, vocab)
+    if (x.stride(1) != 1 and vocab > 1) or (x.shape[0] > 1 and x.stride(0) < vocab):
+        x = x.contiguous()
+    rows = x.shape[0]
+    t = targets.write(saved, row_weight, mean, grad, vocab, dev)
+    each = torch.empty(rows, dtype=F32, device=x.device)
+    total = torch.empty((), dtype=F32, device=x.device) if loss else None
+    dx = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if grads else None
+    N.call("moc_logits_loss", N.dtype_code(x.dtype), x.data_ptr(), rows, vocab, x.stride(0) if rows > 1 else vocab,
+           t.data_ptr(), targets.words, targets.heat, each.data_ptr(), N.ptr(total), N.ptr(dx), vocab, N.stream_on(dev))
+    return total, each, dx
+
+
+class _LogitsLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, targets, grad_mode, logits, *saved):
+        need = grad_mode and ctx.needs_input_grad[2]
+        ahead = targets.reduction != "none"
+        total, each, dx = _logits_pass(targets, saved, saved[2], targets.reduction == "mean", None, logits, ahead,
+                                       ahead and need)
+        if need:
+            ctx.save_for_backward(logits, *saved)
+            ctx.targets = targets
+            ctx.kept = _Kept((dx,) if ahead else None)
+        return total if ahead else each.view(logits.shape[:-1])
+
+    @staticmethod
+    def backward(ctx, g):
+        logits, *saved = ctx.saved_tensors
+        targets = ctx.targets
+        rest = (None,) * len(saved)
+        if torch.is_grad_enabled():
+            def stock(x):
+                return _reduced_f32(targets, saved, x.float().reshape(-1, x.shape[-1])).reshape(g.shape)
+            return (None, None, *graph_grads(stock, (logits,), (True,), g), *rest)
+        if targets.reduction == "none":
+            dx = _logits_pass(targets, saved, _row_factors(targets, saved, g), False, None, logits, False, True)[2]
+        else:
+            kept = ctx.kept.take(g)
+            dx = kept[0] if kept else _logits_pass(targets, saved, saved[2], targets.reduction == "mean", g, logits,
+                                                   False, True)[2]
+        return (None, None, dx, *rest)

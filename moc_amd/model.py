@@ -13,10 +13,11 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .block import (attention_half, attention_half_ok, bare, lm_head, lm_head_ok, next_token_loss, next_token_loss_ok,
-                    runs_stock, stock_method)
+from .block import (attention_half, attention_half_ok, bare, final_norm, lm_head, lm_head_ok, next_token_loss,
+                    next_token_loss_ok, plain, runs_stock, stock_method, stream_dtype)
 from .config import MoCConfig
 from .ffn import MoCSwiGLUFFN, block_ffn, block_ffn_f32_ok, block_ffn_ok, build_ffn
+from .losses import linear_cross_entropy, linear_distillation
 
 FFN_TYPES = ("dense", "moc", "moc_gcp", "moc_2_8", "moc_post_silu_abs")
 
@@ -139,11 +140,50 @@ class LLaMAModel(nn.Module):
             return self.lm_head(h)
         return torch.matmul(h, self.tok_emb.weight.t())
 
-    def forward(self, input_ids, labels=None):
+    def _hidden(self, input_ids):
         h = self.tok_emb(input_ids)
         for block in self.blocks:
             h = block(h)
-        weight = self.tok_emb.weight if self.lm_head is None else getattr(self.lm_head, "weight", None)
+        return h
+
+    def _head_weight(self):
+        return self.tok_emb.weight if self.lm_head is None else getattr(self.lm_head, "weight", None)
+
+    def _head_is_plain(self, h) -> bool:
+        """The logits are h @ weight.T of tensors that the losses' kernels read."""
+        head, weight = self.lm_head, self._head_weight()
+        return (stream_dtype(h) is not None and runs_stock(self, "_logits") and plain(h, weight) and
+                (head is None or (type(head) is nn.Linear and head.bias is None and bare(head))))
+
+    def loss(self, input_ids, labels, row_weight=None):
+        """forward(input_ids, labels)[1] in f32 without the logits, which exist for a
+        piece of the positions at a time (losses.linear_cross_entropy).  row_weight
+        [batch, seq] (f32): the weight of position t's loss, against label t + 1."""
+        h = self._hidden(input_ids)
+        target = F.pad(labels[:, 1:], (0, 1), value=-100)
+        if self._head_is_plain(h):
+            return linear_cross_entropy(final_norm(h, self.norm, RMSNorm), self._head_weight(), target, row_weight)
+        logits = self._logits(self.norm(h)).float()
+        each = F.cross_entropy(logits.flatten(0, 1), target.flatten(), ignore_index=-100, reduction="none")
+        weight = (target != -100).float().flatten()
+        if row_weight is not None:
+            weight = torch.where(weight > 0, row_weight.flatten(), 0.0)
+        return torch.where(weight == 0, 0.0, each * weight).sum() / weight.sum()
+
+    def distill(self, input_ids, teacher_ids, teacher_logits, row_weight=None, *, temperature: float = 1.0):
+        """The divergence of the model's logits from a teacher's top ones at the same
+        positions, [batch, seq, words] ids and logits (losses.linear_distillation, which
+        describes them and row_weight).  Device tensors in bf16, or f32 under bf16
+        autocast."""
+        h = self._hidden(input_ids)
+        if not self._head_is_plain(h):
+            raise ValueError("distill takes a plain LM head on the device, in bf16 or in f32 under bf16 autocast")
+        return linear_distillation(final_norm(h, self.norm, RMSNorm), self._head_weight(), teacher_ids, teacher_logits,
+                                   row_weight, temperature=temperature)
+
+    def forward(self, input_ids, labels=None):
+        h = self._hidden(input_ids)
+        weight = self._head_weight()
         if self.ffn_type != "dense" and runs_stock(self, "_logits") and \
                 lm_head_ok(h, self.norm, RMSNorm, self.lm_head, weight):
             logits = lm_head(h, self.norm, weight)

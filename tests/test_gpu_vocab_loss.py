@@ -1,0 +1,469 @@
+"""Losses over a vocabulary against 64 bits: linear cross entropy, linear
+distillation, distillation of kept logits, with their gradients.
+
+Tolerances.  A logit is a sum of d products that bf16 or f32 operands give without
+or with one rounding of 2^-24: with S the largest sum of |h||w|, an error of 4 sqrt(d)
+2^-24 S (roundings of either sign) and 2 more units for an f32 product's own.  A
+row's loss differs by twice that and by f32 exponentials, logarithms and a sum over
+the vocabulary, 2^-20 of its terms.  A gradient is a sum over dlogits, which are
+rounded to bf16 (2^-8 of each; from f16 exponentials, 2^-11 more) or f32 (2^-23 with
+the exponential's own) behind a relative error of the logits' errors, and rounded
+itself; |dlogits| |operand| in 64 bits bounds what that comes to.  p's relative error
+counts for p, not for p - q: with c the row's factor, c p <= |dlogits| + c q.  A
+gradient that was computed ahead and rounded to bf16 is rounded once more by an
+upstream factor that is no power of two: (1 + 2^-8)^2 - 1 < 2.01 2^-8.
+"""
+import math
+
+import pytest
+import torch
+
+from moc_amd import losses as L
+
+pytestmark = pytest.mark.gpu
+BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+SIZES = [(1, 8, 1), (1, 64, 500), (3, 100, 1003), (17, 256, 4099), (40, 2048, 8190), (256, 64, 32000), (300, 512, 2050),
+         (1030, 96, 777), (129, 1000, 5000), (5, 1, 9), (2, 24, 1), (1, 7, 2)]
+
+
+def rand(*shape, seed):
+    g = torch.Generator().manual_seed(seed + 7 * math.prod(shape))
+    return torch.randn(*shape, generator=g).cuda()
+
+
+def operands(rows, d, vocab, dtype, seed=0):
+    w = (rand(vocab, d, seed=seed) * (1.5 / math.sqrt(d))).to(dtype)
+    h = (rand(rows, d, seed=seed + 1) + 2 * w[torch.arange(rows, device="cuda") % vocab].float()).to(dtype)
+    return h, w
+
+
+def labels_of(rows, vocab, masked, seed=3):
+    g = torch.Generator().manual_seed(seed + rows)
+    y = torch.randint(0, vocab, (rows,), generator=g)
+    y[torch.rand(rows, generator=g) < masked] = -100
+    return y.cuda()
+
+
+def teacher_of(rows, vocab, words, ragged, seed=5, ids_dtype=torch.int32, top_dtype=F32):
+    g = torch.Generator().manual_seed(seed + rows + words)
+    ids = torch.randint(0, vocab, (rows, words), generator=g)  # the same word twice now and then
+    top = torch.randn(rows, words, generator=g) * 2
+    if ragged:
+        ids[torch.rand(rows, words, generator=g) < 0.3] = -1
+        top[torch.rand(rows, words, generator=g) < 0.1] = -math.inf
+        ids[torch.rand(rows, generator=g) < 0.2] = -1
+        ids[rows // 2, 0], top[rows // 2, 0] = vocab - 1, 0.5
+        ids[rows // 2 - 1, -1] = vocab  # outside
+    return ids.to("cuda", ids_dtype), top.to("cuda", top_dtype)
+
+
+def shares(ids, top, vocab, heat):
+    """The teacher's distribution over the whole vocabulary, rows that have one."""
+    ids, x = ids.long(), top.to(F64) / heat
+    there = (ids >= 0) & (ids < vocab) & (x != -math.inf)
+    some = there.any(1)
+    q = torch.where(there, torch.exp(x - torch.where(there, x, -math.inf).amax(1, keepdim=True).clamp(min=-1e30)), 0.0)
+    q = q / q.sum(1, keepdim=True).clamp(min=1e-300)
+    return torch.zeros(ids.shape[0], vocab, dtype=F64, device="cuda").scatter_add_(1, torch.where(there, ids, 0), q), some
+
+
+def reference(z, q, counts, weight, heat, reduction):
+    """(loss or rows' losses, dloss / dz for an upstream gradient of 1, the rows' factors c)."""
+    log_p = torch.log_softmax(z / heat, -1)
+    each = heat ** 2 * torch.where(q > 0, q * (torch.log(q.clamp(min=1e-300)) - log_p), 0.0).sum(-1)
+    w = torch.where(counts, weight, 0.0)
+    dz = heat * (log_p.exp() - q)
+    n = w.sum() if reduction == "mean" else 1.0
+    each = torch.where(w != 0, each * w, 0.0)
+    dz = torch.where((w != 0)[:, None], dz * (w / n)[:, None], 0.0)
+    return (each if reduction == "none" else each.sum() / n), dz, (heat * w / n).abs()[:, None]
+
+
+def logit_error(h, w):
+    s = (h.abs() @ w.abs().t()).amax().item()
+    return (4 * math.sqrt(h.shape[1]) + 2) * 2.0 ** -24 * s
+
+
+def check(out, want, got, leaves, dz, c, q, z_err, heat, factor, weights):
+    """Loss and gradients (None: not asked for) of the linear losses."""
+    scale = (want.abs() if want.dim() else want.abs() + 1) + weights.abs().max()
+    tol = (2 * z_err * heat + 2.0 ** -20 * math.log(2 * q.shape[1]) * heat ** 2) * scale
+    assert ((out.to(F64) - want).abs() <= tol).all(), ((out.to(F64) - want).abs() / tol).max()
+    h, w = leaves
+    dz, c = dz * factor, c * abs(factor)
+    soft = dz.abs() + c * q
+    for got_, want_, size, i in ((got[0], dz @ w, soft @ w.abs(), 0), (got[1], dz.t() @ h, soft.t() @ h.abs(), 1)):
+        if got_ is None:
+            continue
+        half = got_.dtype == BF
+        rel = (2.0 ** -8 + 2.0 ** -11 if half else 2.0 ** -22) + 4 * z_err / heat
+        terms = dz.shape[1 - i]
+        tol = rel * size + (4 * math.sqrt(terms) + 2) * 2.0 ** -24 * size
+        if got_.dtype == BF:
+            tol = tol * (1 + 2.0 ** -7) + (1 if want.dim() else 2.01) * 2.0 ** -8 * want_.abs() + 1e-38
+        err = (got_.to(F64) - want_).abs()
+        assert (err <= tol).all(), (i, (err / tol).max(), err.max())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,d,vocab", SIZES)
+@pytest.mark.parametrize("masked,weighted,reduction", [(0.0, False, "mean"), (0.4, True, "mean"), (0.9, True, "sum"),
+                                                       (0.3, True, "none")])
+def test_linear_cross_entropy(rows, d, vocab, dtype, masked, weighted, reduction):
+    h, w = operands(rows, d, vocab, dtype)
+    y = labels_of(rows, vocab, masked)
+    y[rows // 2] = vocab - 1
+    weight = rand(rows, seed=9) if weighted else torch.ones(rows, device="cuda")
+    if weighted:
+        weight[rows // 2] = 1.5 + rows  # a mean's divisor away from 0
+        weight[rows // 3 + 1:rows // 3 + 2] = 0
+    counts = y != -100
+    h[~counts | (weight == 0)] = math.nan  # nobody looks at these
+    h.requires_grad_()
+    w.requires_grad_()
+    out = L.linear_cross_entropy(h, w, y, weight if weighted else None, reduction=reduction)
+    assert out.dtype == F32
+    g = rand(rows, seed=11) if reduction == "none" else torch.tensor(0.7, device="cuda")
+    got = torch.autograd.grad(out, (h, w), g)
+    hd, wd = h.detach().to(F64), w.detach().to(F64)
+    hd = torch.where((counts & (weight != 0))[:, None], hd, 0.0)
+    q = torch.zeros(rows, vocab, dtype=F64, device="cuda")
+    q[torch.arange(rows, device="cuda"), y.clamp(min=0)] = 1
+    want, dz, c = reference(hd @ wd.t(), q, counts, weight.to(F64), 1.0, reduction)
+    check(out.detach(), want, got, (hd, wd), dz, c, q, logit_error(hd, wd), 1.0, g.to(F64)[:, None] if reduction == "none"
+          else g.to(F64), weight)
+    assert (got[0][~counts] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,d,vocab", SIZES)
+@pytest.mark.parametrize("words,heat,ragged,reduction", [(1, 1.0, False, "mean"), (7, 2.0, True, "mean"),
+                                                         (64, 0.7, False, "sum"), (300, 1.0, True, "none")])
+def test_linear_distillation(rows, d, vocab, dtype, words, heat, ragged, reduction):
+    h, w = operands(rows, d, vocab, dtype)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    ids, top = teacher_of(rows, vocab, words, ragged, ids_dtype=torch.int64 if words == 7 else torch.int32,
+                          top_dtype=BF if words == 64 else F32)
+    out = L.linear_distillation(h, w, ids, top, temperature=heat, reduction=reduction)
+    g = rand(rows, seed=11) if reduction == "none" else torch.tensor(-1.3, device="cuda")
+    got = torch.autograd.grad(out, (h, w), g)
+    hd, wd = h.detach().to(F64), w.detach().to(F64)
+    q, some = shares(ids, top, vocab, heat)
+    one = torch.ones(rows, dtype=F64, device="cuda")
+    want, dz, c = reference(hd @ wd.t(), q, some, one, heat, reduction)
+    check(out.detach(), want, got, (hd, wd), dz, c, q, logit_error(hd, wd), heat,
+          g.to(F64)[:, None] if reduction == "none" else g.to(F64), one)
+    assert (got[0][~some] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (2, 3), (5, 500), (33, 1003), (7, 32000), (3, 50021), (2, 128256),
+                                        (2, 262147), (600, 4096)])
+@pytest.mark.parametrize("words,heat,ragged,reduction", [(1, 1.0, False, "mean"), (20, 2.0, True, "mean"),
+                                                         (101, 0.7, False, "sum"), (1024, 1.0, True, "none")])
+def test_distillation_loss(rows, vocab, dtype, words, heat, ragged, reduction):
+    x = (3 * rand(rows, vocab, seed=2)).to(dtype)
+    ids, top = teacher_of(rows, vocab, words, ragged)
+    q, some = shares(ids, top, vocab, heat)
+    x[~some] = math.nan
+    x.requires_grad_()
+    out = L.distillation_loss(x, ids, top, temperature=heat, reduction=reduction)
+    g = rand(rows, seed=11) if reduction == "none" else torch.tensor(0.7, device="cuda")
+    got = torch.autograd.grad(out, x, g)[0]
+    z = torch.where(some[:, None], x.detach().to(F64), 0.0)
+    want, dz, c = reference(z, q, some, torch.ones(rows, dtype=F64, device="cuda"), heat, reduction)
+    top_z = z.abs().max().item() / heat
+    # scaling a logit and subtracting two f32 numbers of its size, on top of 2^-20
+    rel = 2.0 ** -20 + 4 * 2.0 ** -24 * (top_z + 20)
+    tol = rel * heat ** 2 * (want.abs() / heat ** 2 + math.log(2 * vocab) + top_z)
+    assert ((out.detach().to(F64) - want).abs() <= tol).all()
+    factor = g.to(F64)[:, None] if reduction == "none" else g.to(F64)
+    dz = dz * factor
+    # two roundings: the gradient's own and the upstream factor's
+    tol = 8 * rel * (dz.abs() + c * abs(factor) * q) + (2.01 * 2.0 ** -8 if dtype == BF else 2.0 ** -23) * dz.abs() + 1e-38
+    err = (got.to(F64) - dz).abs()
+    assert (err <= tol).all(), (err / tol).max()
+
+
+def test_rows_in_pieces():
+    """More logits than a piece holds: sums over the pieces."""
+    rows, d, vocab = 5300, 64, 128256
+    h, w = operands(rows, d, vocab, BF)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    y = labels_of(rows, vocab, 0.2)
+    out = L.linear_cross_entropy(h, w, y)
+    got = torch.autograd.grad(out, (h, w))
+    hd, wd = h.detach().to(F64), w.detach().to(F64)
+    q = torch.zeros(rows, vocab, dtype=F64, device="cuda")
+    q[torch.arange(rows, device="cuda"), y.clamp(min=0)] = 1
+    one = torch.ones(rows, dtype=F64, device="cuda")
+    want, dz, c = reference(hd @ wd.t(), q, y != -100, one, 1.0, "mean")
+    check(out.detach(), want, got, (hd, wd), dz, c, q, logit_error(hd, wd), 1.0, 1.0, one)
+
+
+def test_nothing_counts():
+    h, w = operands(9, 64, 300, BF)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    for reduction, value in (("sum", 0.0), ("mean", math.nan), ("none", 0.0)):
+        out = L.linear_cross_entropy(h, w, torch.full((9,), -100, device="cuda"), reduction=reduction)
+        assert ((out == value) | (torch.isnan(out) & math.isnan(value))).all()
+        if reduction != "mean":
+            for t in torch.autograd.grad(out.sum(), (h, w)):
+                assert (t == 0).all()
+
+
+def test_unknown_label_is_nan():
+    h, w = operands(6, 64, 300, BF)
+    y = labels_of(6, 300, 0.0)
+    y[2] = 300
+    each = L.linear_cross_entropy(h, w, y, reduction="none")
+    assert torch.isnan(each).tolist() == [i == 2 for i in range(6)]
+    h = h.requires_grad_()
+    g = torch.autograd.grad(L.linear_cross_entropy(h, w, y), h)[0]
+    assert torch.isnan(g).all(1).tolist() == [i == 2 for i in range(6)]
+
+
+@pytest.mark.parametrize("lead", [(2, 5), (3,), (), (2, 2, 3), (0,), (2, 0)])
+def test_leading_shapes_and_no_rows(lead):
+    h, w = operands(max(1, math.prod(lead)), 64, 300, BF)
+    h = h[:math.prod(lead)].reshape(*lead, 64).clone().requires_grad_()
+    w = w.requires_grad_()
+    y = labels_of(math.prod(lead), 300, 0.0).reshape(lead)
+    each = L.linear_cross_entropy(h, w, y, reduction="none")
+    assert each.shape == h.shape[:-1]
+    flat = L.linear_cross_entropy(h.reshape(-1, 64), w, y.reshape(-1), reduction="none")
+    assert torch.equal(each.reshape(-1), flat)
+    total = L.linear_cross_entropy(h, w, y, reduction="sum")
+    dh, dw = torch.autograd.grad(total, (h, w))
+    assert dh.shape == h.shape and dw.shape == w.shape and torch.isfinite(dw).all()
+    if not math.prod(lead):
+        assert total == 0 and (dw == 0).all()
+
+
+def test_strides_and_alignment():
+    """Views with other strides and bases give what contiguous copies give."""
+    base_h, base_w = operands(50, 200, 700, BF)
+    y = labels_of(50, 700, 0.1)
+    pad = lambda t, a: torch.zeros(t.shape[0], t.shape[1] + a, dtype=t.dtype, device="cuda")  # noqa: E731
+    want = None
+    for make in (lambda t: t.clone(), lambda t: pad(t, 3)[:, 1:-2].copy_(t), lambda t: pad(t, 8)[:, :-8].copy_(t),
+                 lambda t: t.t().contiguous().t(), lambda t: torch.repeat_interleave(t, 2, 0)[::2]):
+        h, w = make(base_h).requires_grad_(), make(base_w).requires_grad_()
+        out = L.linear_cross_entropy(h, w, y)
+        got = (out, *torch.autograd.grad(out, (h, w)))
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    ids, top = teacher_of(50, 700, 9, True)
+    x = (3 * rand(50, 700, seed=1)).to(BF)
+    a = L.distillation_loss(x, ids, top)
+    for make in (lambda t: pad(t, 3)[:, 1:-2].copy_(t), lambda t: t.t().contiguous().t()):
+        assert torch.equal(a, L.distillation_loss(make(x), make(ids.float()).int(), make(top)))
+
+
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+def test_second_backward_and_factor(op):
+    """The gradients ahead are handed out once, computed again then."""
+    h, w = operands(70, 128, 900, BF)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    ids, top = teacher_of(70, 900, 5, True)
+    y = labels_of(70, 900, 0.2)
+    if op == "kept":
+        x = (3 * rand(70, 900, seed=1)).to(BF).requires_grad_()
+        leaves, loss = (x,), L.distillation_loss(x, ids, top)
+    else:
+        leaves = (h, w)
+        loss = L.linear_cross_entropy(h, w, y) if op == "entropy" else L.linear_distillation(h, w, ids, top)
+    first = [t.clone() for t in torch.autograd.grad(loss, leaves, retain_graph=True)]
+    again = torch.autograd.grad(loss, leaves, retain_graph=True)
+    third = torch.autograd.grad(loss, leaves, torch.tensor(4.0, device="cuda"))
+    for a, b, c in zip(first, again, third):
+        assert torch.equal(a, b) and torch.equal(a * 4, c)
+
+
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+def test_only_what_is_asked_for(op):
+    h, w = operands(40, 64, 300, BF)
+    ids, top = teacher_of(40, 300, 5, False)
+    y = labels_of(40, 300, 0.2)
+    run = (lambda a, b: L.linear_cross_entropy(a, b, y)) if op == "entropy" else (
+        lambda a, b: L.linear_distillation(a, b, ids, top)) if op == "teacher" else (
+        lambda a, b: L.distillation_loss(a, ids, top))
+    if op == "kept":
+        h = (3 * rand(40, 300, seed=1)).to(BF)
+    plain = run(h, w)
+    assert not plain.requires_grad
+    with torch.no_grad():
+        assert torch.equal(plain, run(h.clone().requires_grad_(), w.clone().requires_grad_()))
+    a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+    both = torch.autograd.grad(run(a, b), (a, b), allow_unused=op == "kept")
+    assert torch.equal(torch.autograd.grad(run(a, w), a)[0], both[0])
+    if op != "kept":
+        assert torch.equal(torch.autograd.grad(run(h, b), b)[0], both[1])
+
+
+@pytest.mark.parametrize("op", ["entropy", "teacher"])
+@pytest.mark.parametrize("types", [(F32, F32), (BF, F32), (F32, BF)])
+def test_autocast(op, types):
+    """Under bf16 autocast: products of bf16 casts, gradients in the operands' types."""
+    h, w = operands(60, 128, 900, F32)
+    h, w = h.to(types[0]).requires_grad_(), w.to(types[1]).requires_grad_()
+    ids, top = teacher_of(60, 900, 5, True)
+    y = labels_of(60, 900, 0.2)
+    hb, wb = (t.detach().to(BF).requires_grad_() for t in (h, w))
+    run = (lambda a, b: L.linear_cross_entropy(a, b, y)) if op == "entropy" else (
+        lambda a, b: L.linear_distillation(a, b, ids, top))
+    with torch.autocast("cuda", dtype=BF):
+        out = run(h, w)
+    plain = run(hb, wb)
+    assert torch.equal(out, plain)
+    for a, b, t in zip(torch.autograd.grad(out, (h, w)), torch.autograd.grad(plain, (hb, wb)), types):
+        assert a.dtype == t and torch.equal(a.to(BF), b)
+
+
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_second_derivative(op, reduction):
+    """A gradient with a graph of its own, against one in 64 bits."""
+    rows, d, vocab, heat = 6, 16, 40, 1.5
+    h, w = operands(rows, d, vocab, F32)
+    ids, top = teacher_of(rows, vocab, 4, False)
+    y = labels_of(rows, vocab, 0.3)
+    y[0] = 3
+    v = [rand(rows, d, seed=21), rand(vocab, d, seed=22)]
+    if op == "kept":
+        leaves = [(2 * rand(rows, vocab, seed=1)).requires_grad_()]
+        v = [rand(rows, vocab, seed=23)]
+        run = lambda x: L.distillation_loss(x, ids, top, temperature=heat, reduction=reduction)  # noqa: E731
+    else:
+        leaves = [h.requires_grad_(), w.requires_grad_()]
+        run = (lambda a, b: L.linear_cross_entropy(a, b, y, reduction=reduction)) if op == "entropy" else (
+            lambda a, b: L.linear_distillation(a, b, ids, top, temperature=heat, reduction=reduction))
+    grads = torch.autograd.grad(run(*leaves).sum(), leaves, create_graph=True)
+    got = torch.autograd.grad(sum((a * b).sum() for a, b in zip(grads, v)), leaves)
+    exact = [t.detach().to(F64).requires_grad_() for t in leaves]
+    z = exact[0] if op == "kept" else exact[0] @ exact[1].t()
+    log_p = torch.log_softmax(z / (1.0 if op == "entropy" else heat), -1)
+    if op == "entropy":
+        on = y != -100
+        each = -log_p[on, y[on]]
+    else:
+        q, _ = shares(ids, top, vocab, heat)
+        each = -heat ** 2 * (q * log_p).sum(1)
+    loss = each.sum() if reduction == "none" else each.mean()
+    grads = torch.autograd.grad(loss, exact, create_graph=True)
+    want = torch.autograd.grad(sum((a * b.to(F64)).sum() for a, b in zip(grads, v)), exact)
+    for a, b in zip(got, want):
+        # f32 sums of some hundred terms of the result's size
+        assert (a.to(F64) - b).abs().max() <= 1e-4 * b.abs().max()
+
+
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+def test_gradient_by_differences(op):
+    """f32 operands: the loss along a direction against the gradient."""
+    rows, d, vocab = 12, 32, 200
+    h, w = operands(rows, d, vocab, F32)
+    ids, top = teacher_of(rows, vocab, 6, True)
+    y = labels_of(rows, vocab, 0.2)
+    y[0] = 3
+    if op == "kept":
+        leaves = [(2 * rand(rows, vocab, seed=1)).requires_grad_()]
+        run = lambda x: L.distillation_loss(x, ids, top, temperature=2.0, reduction="sum")  # noqa: E731
+    else:
+        leaves = [h.requires_grad_(), w.requires_grad_()]
+        run = (lambda a, b: L.linear_cross_entropy(a, b, y, reduction="sum")) if op == "entropy" else (
+            lambda a, b: L.linear_distillation(a, b, ids, top, temperature=2.0, reduction="sum"))
+    grads = torch.autograd.grad(run(*leaves), leaves)
+    way = [rand(*t.shape, seed=31) for t in leaves]
+    slope = sum((a.to(F64) * b.to(F64)).sum() for a, b in zip(grads, way)).item()
+    step = 2.0 ** -7
+    with torch.no_grad():
+        up, down = (run(*[t + s * b for t, b in zip(leaves, way)]).to(F64).item() for s in (step, -step))
+    # the third derivative along the way (step^2 of the slope's size times its
+    # logits' cube, below 8^3 / 6 each) and f32 losses over 2 step
+    size = abs(up) + 1
+    assert abs((up - down) / (2 * step) - slope) <= step ** 2 * 90 * size + 2.0 ** -20 * size / step
+
+
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+def test_captured_pass(op):
+    """Forward and backward in one HIP graph, replayed on changed inputs."""
+    h, w = operands(130, 128, 2000, BF)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    ids, top = teacher_of(130, 2000, 8, True)
+    y = labels_of(130, 2000, 0.2)
+    x = (3 * rand(130, 2000, seed=1)).to(BF).requires_grad_()
+    factor = torch.tensor(0.7, device="cuda")
+    leaves = (x,) if op == "kept" else (h, w)
+
+    def step():
+        loss = L.linear_cross_entropy(h, w, y) if op == "entropy" else (
+            L.linear_distillation(h, w, ids, top, temperature=2.0) if op == "teacher" else
+            L.distillation_loss(x, ids, top, temperature=2.0))
+        return (loss.detach(), *torch.autograd.grad(loss, leaves, factor))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            for t in leaves:
+                t.copy_((t.float() * (0.9 + 0.1 * i)).to(BF))
+            y.copy_(labels_of(130, 2000, 0.3, seed=i))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+def test_captured_backward_of_an_eager_forward():
+    """Each replay of a captured backward gives the same gradients."""
+    w = operands(30, 64, 500, BF)[1]
+    y = labels_of(30, 500, 0.1)
+    factor = torch.tensor(0.5, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        h = operands(30, 64, 500, BF)[0].requires_grad_()
+        want = torch.autograd.grad(L.linear_cross_entropy(h, w, y), h, factor)[0]
+        loss = L.linear_cross_entropy(h, w, y)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = torch.autograd.grad(loss, h, factor)[0]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        # 0.5 scales without rounding
+        assert torch.equal(got, want)
+
+
+def test_other_stream():
+    h, w = operands(300, 256, 3000, BF)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    y = labels_of(300, 3000, 0.2)
+    want = L.linear_cross_entropy(h, w, y)
+    want = (want, *torch.autograd.grad(want, (h, w)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = L.linear_cross_entropy(h, w, y)
+        got = (out, *torch.autograd.grad(out, (h, w)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals_on_the_device():
+    h, w = operands(6, 64, 300, F32)
+    y = labels_of(6, 300, 0.0)
+    with torch.autocast("cuda", dtype=torch.float16), pytest.raises(ValueError, match="bf16"):
+        L.linear_cross_entropy(h, w, y)
+    with pytest.raises(ValueError, match="device"):
+        L.linear_cross_entropy(h, w, y.cpu())
+    with pytest.raises(ValueError, match="one type"):
+        L.linear_cross_entropy(h, w.to(BF), y)
