@@ -277,7 +277,7 @@ int moc_next_token_loss_backward(const void* logits, int64_t ld, int64_t batch, 
  * ids_ld and top_ld apart; q = softmax(top / T) over a row's entries; one outside
  * the vocabulary or of -infinity is none, entries of one word add up.
  * row_weight [rows], grad (a scalar, on the device): NULL is 1. */
-int64_t moc_loss_targets_size(int64_t rows, int64_t words);
+int64_t moc_loss_targets_size(int64_t rows, int64_t words, int64_t vocab);
 int moc_label_targets(const int64_t* labels, int64_t rows, int64_t vocab, int64_t ignore_index,
                       const float* row_weight, int mean, const float* grad, void* targets, void* stream);
 int moc_teacher_targets(const void* ids, int ids_dtype, int64_t ids_ld, const void* top, int top_dtype,
@@ -294,7 +294,8 @@ int moc_logits_loss(int dtype, const void* logits, int64_t rows, int64_t vocab, 
  * rows), which exist for a piece of the rows at a time: dh [rows, hidden] and dw
  * [vocab, hidden], contiguous, either NULL (both: the loss alone).  A bf16 weight of
  * up to 2 GiB.  gemm_ws: as moc_gemm_ws uses it. */
-int64_t moc_linear_loss_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int grads);
+int64_t moc_linear_loss_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t words,
+                                       int grads);
 int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int grads);
 int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w,
                     int64_t vocab, int64_t ldw, void* targets, int64_t words, float temperature, float* row_loss,

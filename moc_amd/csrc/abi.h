@@ -46,6 +46,18 @@ int launch_gate_up_2of8(const void* x, int64_t nb, int64_t hidden, const void* w
                         int64_t inter, int64_t* idx, uint16_t* sz, hipStream_t st, uint16_t* ap = nullptr,
                         int64_t ld_ap = 0, uint32_t* meta = nullptr, int64_t meta_rows = 0);
 
+// Logits h w^T (bf16, 16-byte aligned rows) of a loss over the vocabulary, not
+// stored (gemm.hip): per row and slab of 64 words the maximum of x = unit logit and
+// the sum of exp2(x - it) (stat [rows][ceil(vocab / 64)]); exp2(x - it + 15) as f16
+// (kept, rows a multiple of 64 apart; null: no); the logits of the words ids
+// [rows][words] (ascending) in z, first [rows][ceil(vocab / 256)]: how many of a
+// row's lie left of each tile of 256 words (null for one word).  1: operands too
+// large for its 32-bit offsets (nothing launched).
+constexpr int kLossTile = 256, kLossSlab = 64;
+int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab,
+                     int64_t ldw, float unit, const int32_t* ids, const uint16_t* first, int64_t words, float* z,
+                     float2* stat, void* kept, int64_t ld_kept, hipStream_t st);
+
 // out = x + y over n values (a multiple of 8), x and out f32, y bf16
 // (rmsnorm.hip).
 int add_f32_bf16(const float* x, const void* y, float* out, int64_t n, hipStream_t st);

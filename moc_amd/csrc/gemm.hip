@@ -167,6 +167,18 @@ struct GemmArgs {
   int grp_nk, grp_M, grp_N, grp_tiles_m, grp_tiles_n, grp_ksplit, grp_kper;
   void* grp_C;
   int64_t grp_ldc, grp_ws_stride;
+  // Logits of a loss (gemm_pp_kernel<..., LOSS = true>): C is not stored, but per
+  // row and slab of 64 columns the maximum m of x = unit C and the sum of exp2(x - m)
+  // (ls_stat [M][ls_slabs]), the exponentials as f16 (C, rows ldc apart, null: not
+  // kept) and C itself in f32 at the columns named by ls_ids [M][ls_words]
+  // (ascending; ls_z of the same shape; ls_first [M][tiles_n]: how many of a row's
+  // lie left of the tile, null for one a row).
+  float2* ls_stat;
+  int ls_slabs, ls_words;
+  float ls_unit;
+  const int32_t* ls_ids;
+  const uint16_t* ls_first;
+  float* ls_z;
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const Operand& o) {
@@ -908,6 +920,94 @@ __device__ __forceinline__ void gu28_epilogue(const GemmArgs& g, char* lds, cons
   }
 }
 
+// ---------------------------------------------------------- loss epilogue
+// The wave's MI x 32 rows of 64 logits while they are in f32: a lane holds 32 of
+// one row's (columns 32j + 8q + 4(l >> 5) + r), lane l ^ 32 the other 32, so a
+// slab's maximum and sum are 31 operations in the lane and one exchange.  What is
+// kept for the gradient is exp2(x - m + 15) as f16: 11 bits, where bf16 would add an
+// error as large as the gradient's own rounding; 2^15 moves f16's range so that
+// values down to 2^-29 of the slab's largest keep all of them and none below 2^-40
+// counts.  Measured at 4096 x 32000 x 2048: see launch_loss_gemm.
+template <int MI>
+__device__ __forceinline__ void loss_epilogue(const GemmArgs& g, char* lds, f32x16_t (&acc)[MI][2], int row0,
+                                              int col0, int tn, int wm, int wn, int wave, int lane) {
+  constexpr int kPitch = 64 * 2 + 16;
+  char* reg = lds + wave * (32 * kPitch);
+  const int slab0 = col0 + wn, half = lane >> 5;
+  const bool edge = slab0 + 64 > g.N;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int row = row0 + wm + 32 * i + (lane & 31);
+    const bool live = row < g.M;
+    if (g.ls_words > 0) {
+      const int32_t* ids = g.ls_ids + static_cast<int64_t>(row) * g.ls_words;
+      float* z = g.ls_z + static_cast<int64_t>(row) * g.ls_words;
+      int k = live && g.ls_first != nullptr ? g.ls_first[static_cast<int64_t>(row) * g.tiles_n + tn] : 0;
+      while (true) {
+        const int c = (live && k < g.ls_words ? ids[k] : 0x7FFFFFFF) - slab0;
+        if (!__any(c < 64 && c > -256)) break;  // words of the tile's slabs to the left come first
+        if (c >= 0 && c < 64 && ((c >> 2) & 1) == half) {
+          const int at = ((c >> 5) << 4) + ((c >> 3) << 2 & 12) + (c & 3);
+          float v = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v = at == e ? acc[i][e >> 4][e & 15] : v;
+          z[k] = v;
+        }
+        ++k;
+      }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float x = acc[i][j][r] * g.ls_unit;
+        if (edge && slab0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3) >= g.N) x = -INFINITY;
+        acc[i][j][r] = x;
+        m = fmaxf(m, x);
+      }
+    m = fmaxf(m, __shfl_xor(m, 32));
+    const float ref = m == -INFINITY ? 0.f : m - 15.f;
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float e = __builtin_amdgcn_exp2f(acc[i][j][r] - ref);
+        acc[i][j][r] = e;
+        s += e;
+      }
+    s += __shfl_xor(s, 32);
+    if (live && half == 0 && slab0 < g.N)
+      g.ls_stat[static_cast<int64_t>(row) * g.ls_slabs + (slab0 >> 6)] = make_float2(m, s * 0x1p-15f);
+    if (g.C == nullptr) continue;
+    char* rowp = reg + (lane & 31) * kPitch;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16_t& a = acc[i][j];
+        typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+        const uint32_t lo = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector((f32x2_t){a[4 * q], a[4 * q + 1]}, f16x2_t));
+        const uint32_t hi = __builtin_bit_cast(
+            uint32_t, __builtin_convertvector((f32x2_t){a[4 * q + 2], a[4 * q + 3]}, f16x2_t));
+        *reinterpret_cast<uint2*>(rowp + (32 * j + 8 * q + 4 * half) * 2) = make_uint2(lo, hi);
+      }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int e = it * 64 + lane, r = e >> 3, seg = e & 7;
+      const uint4 v = *reinterpret_cast<const uint4*>(reg + r * kPitch + seg * 16);
+      const int grow = row0 + wm + 32 * i + r, gcol = slab0 + seg * 8;
+      // rows end at a multiple of 64 columns: a segment that straddles N is stored whole
+      if (grow < g.M && gcol < g.N)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.C) + static_cast<int64_t>(grow) * g.ldc + gcol) = v;
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+  }
+}
+
 // SPLIT: split-K launch (f32 partial tiles into the workspace slices).
 // GU: MoC 2:8 gate/up launch (see GemmArgs::gu_idx).
 // SP: A is 2:4-packed (see GemmArgs::sp_meta) and each 32-channel step of a
@@ -917,8 +1017,9 @@ __device__ __forceinline__ void gu28_epilogue(const GemmArgs& g, char* lds, cons
 // positions, both in the A stage; B and everything else are unchanged.  The
 // sparse operand is the MFMA's first, so the accumulators come out in the
 // MFMA's orientation and leave through store_tile_t.
+// LOSS: the epilogue of a loss over the columns (see GemmArgs::ls_stat).
 template <bool A_KC, bool B_KC, bool OUT_F32, bool DUAL, bool SPLIT, bool GU = false, bool SP = false,
-          bool SHORT = false>
+          bool SHORT = false, bool LOSS = false>
 __global__ __launch_bounds__(kPpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void gemm_pp_kernel(GemmArgs g) {
   static_assert(!SHORT || (A_KC && !GU && !SP), "128-row tiles: K-contiguous A, plain products");
@@ -1235,7 +1336,9 @@ void gemm_pp_kernel(GemmArgs g) {
     compute();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
-  if constexpr (GU) {
+  if constexpr (LOSS) {
+    loss_epilogue<MI>(g, lds, acc, row0, col0, tn, wm, wn, wave, lane);
+  } else if constexpr (GU) {
     gu28_epilogue(g, lds, acc, row0, col0, wm, wn, tid, lane);
   } else if constexpr (SPLIT) {
     GemmArgs gs = g;
@@ -2140,6 +2243,44 @@ PairSplitPlan plan_split_pair(int64_t M1, int64_t N1, int nk1, int64_t M2, int64
 }
 
 }  // namespace
+
+// Logits h w^T of a loss (see GemmArgs::ls_stat and abi.h).  128-row tiles where
+// 256-row ones would leave half of the CUs idle.
+int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab,
+                     int64_t ldw, float unit, const int32_t* ids, const uint16_t* first, int64_t words, float* z,
+                     float2* stat, void* kept, int64_t ld_kept, hipStream_t st) {
+  GemmArgs a{};
+  const bool ok = make_operand(h, ldh, true, rows, hidden, a.a[0]) && make_operand(w, ldw, true, vocab, hidden, a.b[0]);
+  auto no_wrap = [](const Operand& o) {
+    return static_cast<int64_t>(o.bytes) + 512 * o.ld + 4096 < (1LL << 32) && 512 * o.ld < (1LL << 31);
+  };
+  if (!ok || !no_wrap(a.a[0]) || !no_wrap(a.b[0])) return 1;
+  a.a[1] = a.a[0];
+  a.b[1] = a.b[0];
+  a.nk[0] = static_cast<int>((hidden + kBK - 1) / kBK);
+  a.M = static_cast<int>(rows);
+  a.N = static_cast<int>(vocab);
+  a.C = kept;
+  a.ldc = ld_kept;
+  a.tiles_m = static_cast<int>((rows + kBM - 1) / kBM);
+  a.tiles_n = static_cast<int>((vocab + kBN - 1) / kBN);
+  const bool short_m = 2LL * a.tiles_m * a.tiles_n <= cu_count();
+  if (short_m) a.tiles_m = static_cast<int>((rows + 127) / 128);
+  if (static_cast<int64_t>(a.tiles_m) * a.tiles_n >= (1LL << 31)) return 1;
+  a.pp = 1;
+  a.ksplit = 1;
+  a.ls_stat = stat;
+  a.ls_slabs = static_cast<int>((vocab + 63) / 64);
+  a.ls_words = static_cast<int>(words);
+  a.ls_unit = unit;
+  a.ls_ids = ids;
+  a.ls_first = first;
+  a.ls_z = z;
+  const dim3 grid(static_cast<unsigned>(a.tiles_m * a.tiles_n)), block(kPpThreads);
+  if (short_m) gemm_pp_kernel<true, true, false, false, false, false, false, true, true><<<grid, block, 0, st>>>(a);
+  else gemm_pp_kernel<true, true, false, false, false, false, false, false, true><<<grid, block, 0, st>>>(a);
+  return check_launch("gemm_pp_kernel (loss)");
+}
 
 // MoC 2:8 gate/up projection + top-2-of-8 on the 512-thread GEMM kernel
 // (256 tokens x 128 channels of gate and of up per workgroup).  Returns 1

@@ -32,12 +32,15 @@ struct Targets {
   float* entropy;   // [rows] sum of q ln q (teacher only)
   int32_t* ids;     // [rows][words] ascending, kNoWord behind the last
   float* share;     // [rows][words] (teacher only); a word's second entry: -1
+  uint16_t* first;  // [rows][tiles of kLossTile words] (teacher only) words left of the tile
 };
+
+int64_t tiles_of(int64_t vocab) { return (vocab + kLossTile - 1) / kLossTile; }
 
 int64_t align256(int64_t n) { return (n + 255) & ~255LL; }
 
 // words = 0: labels.
-int64_t targets_layout(int64_t rows, int64_t words, char* base, Targets* t) {
+int64_t targets_layout(int64_t rows, int64_t words, int64_t vocab, char* base, Targets* t) {
   int64_t at = 256;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -48,6 +51,7 @@ int64_t targets_layout(int64_t rows, int64_t words, char* base, Targets* t) {
   char* ids = take(rows * (words > 0 ? words : 1) * 4);
   char* entropy = words > 0 ? take(rows * 4) : nullptr;
   char* share = words > 0 ? take(rows * words * 4) : nullptr;
+  char* first = words > 0 ? take(rows * tiles_of(vocab) * 2) : nullptr;
   if (t != nullptr) {
     t->total = reinterpret_cast<double*>(base);
     t->factor = reinterpret_cast<float*>(base + 8);
@@ -55,6 +59,7 @@ int64_t targets_layout(int64_t rows, int64_t words, char* base, Targets* t) {
     t->ids = reinterpret_cast<int32_t*>(ids);
     t->entropy = reinterpret_cast<float*>(entropy);
     t->share = reinterpret_cast<float*>(share);
+    t->first = reinterpret_cast<uint16_t*>(first);
   }
   return at;
 }
@@ -106,7 +111,8 @@ template <typename ID, bool TOP_F32>
 __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restrict__ ids, int64_t ids_ld,
                                                               const void* __restrict__ top, int64_t top_ld, int words,
                                                               int64_t vocab, float heat,
-                                                              const float* __restrict__ row_weight, Targets t) {
+                                                              const float* __restrict__ row_weight, Targets t,
+                                                              int tiles) {
   __shared__ int32_t id[kMaxWords], sorted_id[kMaxWords];
   __shared__ float q[kMaxWords], sorted_q[kMaxWords];
   __shared__ float red[4];
@@ -133,6 +139,7 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restri
       t.ids[r * words + k] = kNoWord;
       t.share[r * words + k] = -1.f;
     }
+    for (int n = tid; n < tiles; n += 256) t.first[r * tiles + n] = 0;
     if (tid == 0) {
       t.weight[r] = 0.f;
       t.entropy[r] = 0.f;
@@ -166,6 +173,15 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restri
     }
     t.ids[r * words + k] = mine;
     t.share[r * words + k] = share;
+  }
+  for (int n = tid; n < tiles; n += 256) {
+    int lo = 0, hi = words;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (sorted_id[mid] < n * kLossTile) lo = mid + 1;
+      else hi = mid;
+    }
+    t.first[r * tiles + n] = static_cast<uint16_t>(lo);
   }
   h = block_reduce<false>(h, red);
   if (tid == 0) {
@@ -273,6 +289,124 @@ __global__ __launch_bounds__(512) void logits_loss_kernel(const IN* x, int64_t l
   }
 }
 
+// ------------------------------------------------- logits that were not stored
+// log2 of a row's sum of exponentials from its slabs' maxima and sums.
+template <bool WAVE>
+__device__ __forceinline__ float slabs_lse(const float2* __restrict__ stat, int slabs, float* red) {
+  const int first = WAVE ? threadIdx.x & 63 : threadIdx.x, step = WAVE ? 64 : blockDim.x;
+  float m = -INFINITY, s = 0.f;
+  for (int i = first; i < slabs; i += step) {
+    const float2 v = stat[i];
+    const float n = fmaxf(m, v.x), ref = n == -INFINITY ? 0.f : n;
+    s = s * __builtin_amdgcn_exp2f(m - ref) + v.y * __builtin_amdgcn_exp2f(v.x - ref);
+    m = n;
+  }
+  float all = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
+  if (!WAVE) all = block_reduce<true>(all, red);
+  s *= m == -INFINITY ? (s == s ? 0.f : s) : __builtin_amdgcn_exp2f(m - all);
+  s = WAVE ? wave_sum(s) : block_reduce<false>(s, red);
+  return all + log2f(s);
+}
+
+// A row's cross entropy sum q (-log2 p) over the words this thread takes, of log2 p
+// of each word, which goes to at_word (may be null); NaN for an unknown label.
+__device__ __forceinline__ float cross_of(const Targets& t, int64_t r, int words, const float* __restrict__ z,
+                                          float unit, float lse, float* at_word, int first, int step) {
+  const int n = words > 0 ? words : 1;
+  float cross = 0.f;
+  for (int k = first; k < n; k += step) {
+    const int32_t id = t.ids[r * n + k];
+    if (id == kUnknown) cross = NAN;
+    const float share = words > 0 ? t.share[r * n + k] : 1.f;
+    if (id < 0 || id == kNoWord || share == -1.f) continue;
+    const float l = z[r * n + k] * unit - lse;
+    if (at_word != nullptr) at_word[k] = l;
+    if (share != 0.f) cross -= share * l;
+  }
+  return cross;
+}
+
+// Losses alone: one wave a row.
+__global__ __launch_bounds__(256) void slabs_loss_kernel(const float2* __restrict__ stat, int slabs, int64_t rows,
+                                                         Targets t, int words, float heat,
+                                                         const float* __restrict__ z, float* __restrict__ row_loss) {
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (r >= rows) return;
+  const float w = t.weight[r];
+  if (w == 0.f) {
+    if (lane == 0) row_loss[r] = 0.f;
+    return;
+  }
+  const float lse = slabs_lse<true>(stat + r * slabs, slabs, nullptr);
+  const float cross = wave_sum(cross_of(t, r, words, z, kLog2E / heat, lse, nullptr, lane, 64));
+  if (lane == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
+}
+
+// One workgroup a row: its loss, and its f16 exponentials into bf16 gradients of
+// the logits, in place: e exp2(m - lse) of a slab's reference m is p.
+__global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld, int vocab,
+                                                         const float2* __restrict__ stat, int slabs, Targets t,
+                                                         int words, float heat, const float* __restrict__ z,
+                                                         float* __restrict__ row_loss) {
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+  __shared__ float red[4], at_word[kMaxWords];
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x;
+  const float w = t.weight[r];
+  uint4* row = reinterpret_cast<uint4*>(e + r * ld);
+  const int chunks = (vocab + 7) / 8;
+  if (w == 0.f) {  // uniform
+    for (int c = tid; c < chunks; c += 256) row[c] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) row_loss[r] = 0.f;
+    return;
+  }
+  const float2* st = stat + r * slabs;
+  const float lse = slabs_lse<false>(st, slabs, red);
+  const float cross = block_reduce<false>(cross_of(t, r, words, z, kLog2E / heat, lse, at_word, tid, 256), red);
+  if (tid == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
+  const float c = cross == cross ? heat * w * *t.factor : NAN;
+  constexpr int kAhead = 4;
+  for (int c0 = tid; c0 < chunks; c0 += 256 * kAhead) {
+    uint4 v[kAhead];
+    float m[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = min(c0 + 256 * i, chunks - 1);
+      v[i] = row[at];
+      m[i] = st[at / (kLossSlab / 8)].x;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = c0 + 256 * i;
+      if (at >= chunks) break;
+      const float f = c * __builtin_amdgcn_exp2f(m[i] - lse - 15.f);
+      const uint32_t in[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      uint32_t out[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, in[q]);
+        out[q] = __builtin_bit_cast(uint32_t,
+                                    __builtin_convertvector((cvt_f32x2_t){static_cast<float>(h.x) * f,
+                                                                          static_cast<float>(h.y) * f},
+                                                            cvt_bf16x2_t));
+      }
+      row[at] = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stored before the words' own
+  __syncthreads();
+  const int n = words > 0 ? words : 1;
+  for (int k = tid; k < n; k += 256) {
+    const int32_t id = t.ids[r * n + k];
+    const float share = words > 0 ? t.share[r * n + k] : 1.f;
+    if (id < 0 || id == kNoWord || share == -1.f) continue;
+    e[r * ld + id] = bf16_rne(c * (__builtin_amdgcn_exp2f(at_word[k]) - share));
+  }
+}
+
 // Rows that count, zeros for the others: what is in those reaches no product.
 template <typename T>
 __global__ __launch_bounds__(256) void counted_rows_kernel(const T* __restrict__ h, int64_t ldh, int hidden,
@@ -325,17 +459,22 @@ unsigned blocks_of(int64_t n) {
 constexpr int64_t kPieceBytes = 1LL << 30;
 
 struct Pieces {
+  bool fused;              // logits inside the product (launch_loss_gemm), not stored
   int64_t rows, count;     // rows of a piece, pieces
   int64_t ldz;             // row pitch of a piece's logits
-  int64_t z, d, x, acc, part, bytes;  // offsets in the workspace
+  int64_t slabs;
+  int64_t z, d, x, acc, part, stat, at_words, bytes;  // offsets in the workspace
   int64_t ldx;
 };
 
-Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, bool grads) {
+Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t words, bool grads) {
   Pieces p{};
   const bool f32 = dtype == MOC_F32;
+  p.fused = !f32;
   p.ldz = (vocab + 63) & ~63LL;
-  const int64_t each = p.ldz * (grads && !f32 ? 6 : 4);
+  p.slabs = (vocab + kLossSlab - 1) / kLossSlab;
+  const int64_t n_words = words > 0 ? words : 1;
+  const int64_t each = p.fused ? (grads ? p.ldz * 2 : p.slabs * 8) : p.ldz * (grads && !f32 ? 6 : 4);
   int64_t n = kPieceBytes / each / 256 * 256;
   if (n < 256) n = 256;
   if (n > rows) n = rows < 1 ? 1 : rows;
@@ -347,8 +486,14 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, bool gr
     at += align256(bytes);
     return here;
   };
-  p.z = take(n * p.ldz * 4);
-  p.d = grads && !f32 ? take(n * p.ldz * 2) : p.z;
+  if (p.fused) {
+    p.stat = take(n * p.slabs * 8);
+    p.at_words = take(n * n_words * 4);
+    p.d = grads ? take(n * p.ldz * 2) : 0;
+  } else {
+    p.z = take(n * p.ldz * 4);
+    p.d = grads && !f32 ? take(n * p.ldz * 2) : p.z;
+  }
   p.ldx = (hidden + 63) & ~63LL;
   p.x = grads ? take(rows * p.ldx * (f32 ? 4 : 2)) : 0;
   if (grads && p.count > 1) {
@@ -406,9 +551,9 @@ using namespace moc;
   MOC_REQUIRE(sizes_ok(rows, vocab, words), "%s: up to 2^24 rows, a vocabulary of up to 2^24 words, up to %d of " \
                                             "them a row", name, kMaxWords)
 
-extern "C" int64_t moc_loss_targets_size(int64_t rows, int64_t words) {
-  if (!sizes_ok(rows, 1, words)) return 0;
-  return targets_layout(rows, words, nullptr, nullptr);
+extern "C" int64_t moc_loss_targets_size(int64_t rows, int64_t words, int64_t vocab) {
+  if (!sizes_ok(rows, vocab, words)) return 0;
+  return targets_layout(rows, words, vocab, nullptr, nullptr);
 }
 
 extern "C" int moc_label_targets(const int64_t* labels, int64_t rows, int64_t vocab, int64_t ignore_index,
@@ -419,7 +564,7 @@ extern "C" int moc_label_targets(const int64_t* labels, int64_t rows, int64_t vo
               "moc_label_targets: null operand or unaligned targets");
   hipStream_t st = as_stream(stream);
   Targets t;
-  targets_layout(rows, 0, static_cast<char*>(targets), &t);
+  targets_layout(rows, 0, vocab, static_cast<char*>(targets), &t);
   if (rows > 0) {
     label_targets_kernel<<<static_cast<unsigned>((rows + 255) / 256), 256, 0, st>>>(labels, rows, vocab, ignore_index,
                                                                                     row_weight, t);
@@ -444,13 +589,13 @@ extern "C" int moc_teacher_targets(const void* ids, int ids_dtype, int64_t ids_l
   MOC_REQUIRE(targets != nullptr && aligned16(targets), "moc_teacher_targets: null or unaligned targets");
   hipStream_t st = as_stream(stream);
   Targets t;
-  targets_layout(rows, words, static_cast<char*>(targets), &t);
+  targets_layout(rows, words, vocab, static_cast<char*>(targets), &t);
   if (rows > 0) {
     const dim3 grid(static_cast<unsigned>(rows));
     const int k = static_cast<int>(words);
 #define MOC_TEACHER(ID, F)                                                                                          \
   teacher_targets_kernel<ID, F><<<grid, 256, 0, st>>>(static_cast<const ID*>(ids), ids_ld, top, top_ld, k, vocab, \
-                                                      temperature, row_weight, t)
+                                                      temperature, row_weight, t, (int)tiles_of(vocab))
     if (ids_dtype == MOC_I32 && top_dtype == MOC_F32) MOC_TEACHER(int32_t, true);
     else if (ids_dtype == MOC_I32) MOC_TEACHER(int32_t, false);
     else if (top_dtype == MOC_F32) MOC_TEACHER(int64_t, true);
@@ -474,7 +619,7 @@ extern "C" int moc_logits_loss(int dtype, const void* logits, int64_t rows, int6
   MOC_REQUIRE(rows <= 1 || (ld >= vocab && (dlogits == nullptr || ldd >= vocab)), "moc_logits_loss: rows that overlap");
   hipStream_t st = as_stream(stream);
   Targets t;
-  targets_layout(rows, words, static_cast<char*>(targets), &t);
+  targets_layout(rows, words, vocab, static_cast<char*>(targets), &t);
   const bool f32 = dtype == MOC_F32;
   int rc = logits_rows(f32, f32, logits, rows, vocab, ld, t, words, temperature, row_loss, dlogits, ldd, st);
   if (rc != MOC_OK || loss == nullptr) return rc;
@@ -482,19 +627,20 @@ extern "C" int moc_logits_loss(int dtype, const void* logits, int64_t rows, int6
   return check_launch("loss_sum_kernel");
 }
 
-extern "C" int64_t moc_linear_loss_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int grads) {
-  if (!sizes_ok(rows, vocab, 0) || hidden < 1) return 0;
-  return pieces_of(dtype, rows, hidden, vocab, grads != 0).bytes;
+extern "C" int64_t moc_linear_loss_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab,
+                                                  int64_t words, int grads) {
+  if (!sizes_ok(rows, vocab, words) || hidden < 1) return 0;
+  return pieces_of(dtype, rows, hidden, vocab, words, grads != 0).bytes;
 }
 
 extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab,
                                                        int grads) {
   if (!sizes_ok(rows, vocab, 0) || hidden < 1) return 0;
-  const Pieces p = pieces_of(dtype, rows, hidden, vocab, grads != 0);
+  const Pieces p = pieces_of(dtype, rows, hidden, vocab, 0, grads != 0);
   int64_t most = 0;
   for (int64_t i = 0; i < p.count; i += p.count > 1 ? p.count - 1 : 1) {  // the first piece and the last
     const int64_t n = i + 1 < p.count ? p.rows : rows - i * p.rows;
-    int64_t b = moc_gemm_workspace_size(dtype, n, vocab, hidden, 0);
+    int64_t b = p.fused ? 0 : moc_gemm_workspace_size(dtype, n, vocab, hidden, 0);
     if (b > most) most = b;
     if (!grads) continue;
     b = moc_gemm_workspace_size(dtype, n, hidden, vocab, 0);
@@ -526,13 +672,13 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
                   (dw == nullptr || (dw_dtype == MOC_F32 || (dw_dtype == MOC_BF16 && !f32))),
               "moc_linear_loss: gradients are f32, or bf16 of bf16 operands");
   const bool grads = dh != nullptr || dw != nullptr;
-  const Pieces p = pieces_of(dtype, rows, hidden, vocab, grads);
+  const Pieces p = pieces_of(dtype, rows, hidden, vocab, words, grads);
   MOC_REQUIRE(workspace_bytes >= p.bytes && (workspace != nullptr || p.bytes == 0) && aligned16(workspace),
               "moc_linear_loss: workspace of %lld bytes needed", (long long)p.bytes);
   MOC_REQUIRE(f32 || p.rows * p.ldx * 2 < (1LL << 31) - 1024, "moc_linear_loss: hidden rows of a piece up to 2 GiB");
   hipStream_t st = as_stream(stream);
   Targets t;
-  targets_layout(rows, words, static_cast<char*>(targets), &t);
+  targets_layout(rows, words, vocab, static_cast<char*>(targets), &t);
   char* ws = static_cast<char*>(workspace);
   const int64_t n_words = words > 0 ? words : 1;
   int rc;
@@ -551,18 +697,36 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
   for (int64_t i = 0; i < p.count; ++i) {
     const int64_t r0 = i * p.rows, n = rows - r0 < p.rows ? rows - r0 : p.rows;
     const char* xi = x + r0 * ldx * es;
-    rc = moc_gemm_ws(dtype, n, vocab, hidden, xi, ldx, 1, w, 1, ldw, 0, nullptr, 0, 0, nullptr, 0, 0, ws + p.z, p.ldz,
-                     MOC_F32, gemm_ws, gemm_ws_bytes, stream);
-    if (rc != MOC_OK) return rc;
     Targets ti = t;
     ti.weight += r0;
     ti.ids += r0 * n_words;
     if (words > 0) {
       ti.entropy += r0;
       ti.share += r0 * words;
+      ti.first += r0 * tiles_of(vocab);
     }
-    rc = logits_rows(true, f32, ws + p.z, n, vocab, p.ldz, ti, words, temperature, row_loss + r0,
-                     grads ? ws + p.d : nullptr, p.ldz, st);
+    if (p.fused) {
+      float2* stat = reinterpret_cast<float2*>(ws + p.stat);
+      float* z = reinterpret_cast<float*>(ws + p.at_words);
+      rc = launch_loss_gemm(xi, n, hidden, ldx, w, vocab, ldw, kLog2E / temperature, ti.ids,
+                            words > 0 ? ti.first : nullptr, n_words, z, stat, grads ? ws + p.d : nullptr, p.ldz, st);
+      MOC_REQUIRE(rc <= 0, "moc_linear_loss: operands of up to 2 GiB");
+      if (rc != MOC_OK) return rc;
+      if (grads)
+        slabs_grad_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(
+            reinterpret_cast<uint16_t*>(ws + p.d), p.ldz, (int)vocab, stat, (int)p.slabs, ti, (int)words, temperature, z,
+            row_loss + r0);
+      else
+        slabs_loss_kernel<<<static_cast<unsigned>((n + 3) / 4), 256, 0, st>>>(stat, (int)p.slabs, n, ti, (int)words,
+                                                                              temperature, z, row_loss + r0);
+      rc = check_launch("slabs_grad_kernel");
+    } else {
+      rc = moc_gemm_ws(dtype, n, vocab, hidden, xi, ldx, 1, w, 1, ldw, 0, nullptr, 0, 0, nullptr, 0, 0, ws + p.z, p.ldz,
+                       MOC_F32, gemm_ws, gemm_ws_bytes, stream);
+      if (rc != MOC_OK) return rc;
+      rc = logits_rows(true, f32, ws + p.z, n, vocab, p.ldz, ti, words, temperature, row_loss + r0,
+                       grads ? ws + p.d : nullptr, p.ldz, st);
+    }
     if (rc != MOC_OK) return rc;
     if (dh != nullptr) {
       char* to = static_cast<char*>(dh) + r0 * hidden * (dh_dtype == MOC_F32 ? 4 : 2);

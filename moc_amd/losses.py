@@ -113,7 +113,7 @@ class _Labels:
     def write(self, saved, row_weight, mean: bool, grad, vocab: int, dev) -> torch.Tensor:
         labels = saved[0]
         rows = labels.shape[0]
-        out = torch.empty(N.query("moc_loss_targets_size", rows, 0), dtype=torch.uint8, device=labels.device)
+        out = torch.empty(N.query("moc_loss_targets_size", rows, 0, vocab), dtype=torch.uint8, device=labels.device)
         N.call("moc_label_targets", labels.data_ptr(), rows, vocab, self.ignore, N.ptr(row_weight), mean,
                N.ptr(grad), out.data_ptr(), N.stream_on(dev))
         return out
@@ -139,7 +139,7 @@ class _Teacher:
     def write(self, saved, row_weight, mean: bool, grad, vocab: int, dev) -> torch.Tensor:
         ids, top, _ = saved
         rows, words = ids.shape
-        out = torch.empty(N.query("moc_loss_targets_size", rows, words), dtype=torch.uint8, device=ids.device)
+        out = torch.empty(N.query("moc_loss_targets_size", rows, words, vocab), dtype=torch.uint8, device=ids.device)
         N.call("moc_teacher_targets", ids.data_ptr(), N.idx_code(ids.dtype), ids.stride(0), top.data_ptr(),
                N.dtype_code(top.dtype), top.stride(0), rows, words, vocab, self.heat, N.ptr(row_weight), mean,
                N.ptr(grad), out.data_ptr(), N.stream_on(dev))
@@ -245,7 +245,7 @@ def _linear_pass(targets, saved, row_weight, mean, grad, product, hidden, weight
     total = torch.empty((), dtype=F32, device=where) if loss else None
     dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=where) if dh else None
     dweight = torch.empty((vocab, d), dtype=weight.dtype, device=where) if dw else None
-    nbytes = N.query("moc_linear_loss_workspace_size", code, rows, d, vocab, grads)
+    nbytes = N.query("moc_linear_loss_workspace_size", code, rows, d, vocab, targets.words, grads)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
     ngemm = N.query("moc_linear_loss_gemm_workspace_size", code, rows, d, vocab, grads)
     gemm_ws = K._gemm_workspace(where, ngemm) if ngemm else None
