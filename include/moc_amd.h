@@ -302,8 +302,9 @@ int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t hidden, int6
                     float* loss, void* dh, int dh_dtype, void* dw, int dw_dtype, void* workspace,
                     int64_t workspace_bytes, void* gemm_ws, int64_t gemm_ws_bytes, void* stream);
 
-/* p *= *factor (a device scalar) over n values, nothing where it is 1. */
-int moc_scale_inplace(int dtype, void* p, int64_t n, const float* factor, void* stream);
+/* p0 and p1 *= *factor (a device scalar) over n0 and n1 values, nothing where it is 1. */
+int moc_scale_inplace(int dtype0, void* p0, int64_t n0, int dtype1, void* p1, int64_t n1, const float* factor,
+                      void* stream);
 
 /* The attention half of a decoder block, h = x + out_proj(attention(RoPE(
  * qkv_proj(RMSNorm(x))))) (moc/model.py:31-64,83-84), one call per pass, bit for

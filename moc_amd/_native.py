@@ -93,7 +93,7 @@ SIGNATURES: dict[str, tuple] = {
     "moc_linear_loss_gemm_workspace_size": (_i64, [_int, _i64, _i64, _i64, _int]),
     "moc_linear_loss": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, ctypes.c_float, _vp, _vp,
                                _vp, _int, _vp, _int, _vp, _i64, _vp, _i64, _vp]),
-    "moc_scale_inplace": (_int, [_int, _vp, _i64, _vp, _vp]),
+    "moc_scale_inplace": (_int, [_int, _vp, _i64, _int, _vp, _i64, _vp, _vp]),
     "moc_attention_half_saved_size": (_i64, [_i64, _i64, _i64, _i64, _int]),
     "moc_attention_half_scratch_size": (_i64, [_i64, _i64, _i64, _i64, _int]),
     "moc_attention_half_workspace_size": (_i64, [_i64, _i64]),

@@ -95,14 +95,104 @@ __device__ __forceinline__ double block_sum64(double v, double* red) {
 }
 
 // ------------------------------------------------------------------ targets
+// Weight of a label's row.
+__device__ __forceinline__ float label_weight(int64_t label, int64_t ignore, const float* row_weight, int64_t r) {
+  return label == ignore ? 0.f : row_weight != nullptr ? row_weight[r] : 1.f;
+}
+
+__device__ __forceinline__ void put_total(const Targets& t, double s, int mean, const float* grad) {
+  if (!mean) s = 1.0;
+  *t.total = s;
+  *t.factor = static_cast<float>((grad != nullptr ? static_cast<double>(*grad) : 1.0) / s);
+}
+
+// Workgroup 0 sums the weights beside the others, which write the rows' targets.
 __global__ __launch_bounds__(256) void label_targets_kernel(const int64_t* __restrict__ labels, int64_t rows,
                                                             int64_t vocab, int64_t ignore,
-                                                            const float* __restrict__ row_weight, Targets t) {
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+                                                            const float* __restrict__ row_weight, int mean,
+                                                            const float* __restrict__ grad, Targets t) {
+  if (blockIdx.x == 0) {
+    __shared__ double red[4];
+    double s = 0;
+    if (mean) {
+#pragma unroll 8
+      for (int64_t r = threadIdx.x; r < rows; r += 256) s += label_weight(labels[r], ignore, row_weight, r);
+    }
+    s = block_sum64(s, red);
+    if (threadIdx.x == 0) put_total(t, s, mean, grad);
+    return;
+  }
+  const int64_t r = (static_cast<int64_t>(blockIdx.x) - 1) * 256 + threadIdx.x;
   if (r >= rows) return;
   const int64_t label = labels[r];
-  t.weight[r] = label == ignore ? 0.f : row_weight != nullptr ? row_weight[r] : 1.f;
+  t.weight[r] = label_weight(label, ignore, row_weight, r);
   t.ids[r] = label == ignore ? kNoWord : label >= 0 && label < vocab ? static_cast<int32_t>(label) : kUnknown;
+}
+
+// One wave a row of up to 64 words, a lane a word; as the kernel below.
+template <typename ID, bool TOP_F32>
+__global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict__ ids, int64_t ids_ld,
+                                                           const void* __restrict__ top, int64_t top_ld, int64_t rows,
+                                                           int words, int64_t vocab, float heat,
+                                                           const float* __restrict__ row_weight, Targets t,
+                                                           int tiles) {
+  __shared__ int32_t sorted[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+  if (r >= rows) return;
+  int32_t id = kNoWord;
+  float x = -INFINITY;
+  if (lane < words) {
+    const int64_t word = static_cast<int64_t>(ids[r * ids_ld + lane]);
+    x = (TOP_F32 ? static_cast<const float*>(top)[r * top_ld + lane]
+                 : bf16_to_f32(static_cast<const uint16_t*>(top)[r * top_ld + lane])) / heat;
+    if (word >= 0 && word < vocab && x != -INFINITY) id = static_cast<int32_t>(word);
+    else x = -INFINITY;
+  }
+  const bool some = __any(id != kNoWord);
+  float mx = x;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+  float q = id == kNoWord ? 0.f : exp2f((x - mx) * kLog2E);
+  q = q / wave_sum(q);
+  int rank = 0;
+  for (int j = 0; j < words; ++j) {
+    const int32_t other = __builtin_amdgcn_readlane(id, j);
+    rank += other < id || (other == id && j < lane);
+  }
+  if (lane >= words) rank = lane;
+  id = __builtin_amdgcn_ds_permute(rank * 4, id);
+  q = __int_as_float(__builtin_amdgcn_ds_permute(rank * 4, __float_as_int(q)));
+  // a word's first entry gets the shares of the others, which follow it
+  const int32_t before = __shfl_up(id, 1);
+  const bool head = id != kNoWord && (lane == 0 || before != id);
+  float share = q;
+  for (int o = 1; o < words; ++o) {
+    const bool same = __shfl_down(id, o) == id && id != kNoWord && lane + o < 64;
+    const float other = __shfl_down(q, o);
+    if (!__any(same)) break;
+    if (same) share += other;
+  }
+  const float h = wave_sum(head && (share > 0.f || share != share) ? share * logf(share) : 0.f);
+  if (lane < words) {
+    t.ids[r * words + lane] = id;
+    t.share[r * words + lane] = head ? share : -1.f;
+  }
+  if (lane == 0) {
+    t.weight[r] = !some ? 0.f : row_weight != nullptr ? row_weight[r] : 1.f;
+    t.entropy[r] = some ? h : 0.f;
+  }
+  sorted[wave][lane] = id;
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own row
+  __builtin_amdgcn_wave_barrier();
+  for (int n = lane; n < tiles; n += 64) {
+    int lo = 0;
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1)
+      if (sorted[wave][lo + step - 1] < n * kLossTile) lo += step;
+    lo += sorted[wave][lo] < n * kLossTile;
+    t.first[r * tiles + n] = static_cast<uint16_t>(lo);
+  }
 }
 
 // One workgroup a row.  Words sorted by rank (ties by place); entries of the
@@ -195,13 +285,12 @@ __global__ __launch_bounds__(1024) void target_total_kernel(int64_t rows, int me
                                                             Targets t) {
   __shared__ double red[16];
   double s = 0;
-  if (mean)
+  if (mean) {
+#pragma unroll 8
     for (int64_t r = threadIdx.x; r < rows; r += 1024) s += t.weight[r];
-  s = mean ? block_sum64(s, red) : 1.0;
-  if (threadIdx.x == 0) {
-    *t.total = s;
-    *t.factor = static_cast<float>((grad != nullptr ? static_cast<double>(*grad) : 1.0) / s);
   }
+  s = block_sum64(s, red);
+  if (threadIdx.x == 0) put_total(t, s, mean, grad);
 }
 
 // loss = sum of the rows' weighted losses / total.  One workgroup.
@@ -209,6 +298,7 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const float* __restrict_
                                                         const double* __restrict__ total, float* __restrict__ loss) {
   __shared__ double red[16];
   double s = 0;
+#pragma unroll 8
   for (int64_t r = threadIdx.x; r < rows; r += 1024) s += row_loss[r];
   s = block_sum64(s, red);
   if (threadIdx.x == 0) *loss = static_cast<float>(s / *total);
@@ -235,57 +325,150 @@ template <> struct Elem<float> {
   static __device__ __forceinline__ float of(float f) { return f; }
 };
 
-// One workgroup a row: maximum, sum, loss, then the gradient (dx may be x).
-template <typename IN, typename OUT>
-__global__ __launch_bounds__(512) void logits_loss_kernel(const IN* x, int64_t ld, int vocab, Targets t, int words,
-                                                          float heat, float* __restrict__ row_loss, OUT* dx,
-                                                          int64_t ldd) {
-  __shared__ float red[8], at_word[kMaxWords];
+// 16 bytes of a row that starts at any element.
+typedef uint32_t chunk_t __attribute__((ext_vector_type(4)));
+typedef chunk_t loose2_t __attribute__((aligned(2)));
+typedef chunk_t loose4_t __attribute__((aligned(4)));
+__device__ __forceinline__ uint4 load_chunk(const uint16_t* p) {
+  const chunk_t v = *reinterpret_cast<const loose2_t*>(p);
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ uint4 load_chunk(const float* p) {
+  const chunk_t v = *reinterpret_cast<const loose4_t*>(p);
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+// Elements p[0 .. per of the input chunk) = c exp2(unit x - lse).
+__device__ __forceinline__ void store_grad(uint16_t* p, const float (&v)[8]) {
+  chunk_t o;
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    o[q] = __builtin_bit_cast(uint32_t, __builtin_convertvector((cvt_f32x2_t){v[2 * q], v[2 * q + 1]}, cvt_bf16x2_t));
+  *reinterpret_cast<loose2_t*>(p) = o;
+}
+__device__ __forceinline__ void store_grad(float* p, const float (&v)[4]) {
+  chunk_t o;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) o[q] = __float_as_uint(v[q]);
+  *reinterpret_cast<loose4_t*>(p) = o;
+}
+
+// One workgroup a row: maximum, sum, loss, gradient (dx may be x).  NC > 0: the row
+// stays in registers, NC chunks of 16 bytes a thread, all loads in flight before the
+// first is used; NC = 0: it is read twice, the second time from the caches.
+template <typename T, int NC, int TH>
+__global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld, int vocab, Targets t, int words,
+                                                         float heat, float* __restrict__ row_loss, T* dx, int64_t ldd) {
+  constexpr int kPer = Elem<T>::kPer, kAhead = 4;
+  __shared__ float red[TH / 64], at_word[kMaxWords];
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x;
   const float w = t.weight[r];
-  const IN* row = x + r * ld;
-  OUT* out = dx + r * ldd;
-  if (w == 0.f) {  // uniform
-    if (dx != nullptr)
-      for (int j = tid; j < vocab; j += 512) out[j] = Elem<OUT>::of(0.f);
+  const T* row = x + r * ld;
+  T* out = dx + r * ldd;
+  const int full = vocab / kPer, rest = vocab % kPer;  // whole chunks, elements behind them
+  if (w == 0.f) {                                      // uniform
+    if (dx != nullptr) {
+      const float zero[kPer] = {};
+      for (int c = tid; c < full; c += TH) store_grad(out + c * kPer, zero);
+      if (tid < rest) out[full * kPer + tid] = Elem<T>::of(0.f);
+    }
     if (tid == 0) row_loss[r] = 0.f;
     return;
   }
   const float unit = kLog2E / heat;
-  float mx = -INFINITY;
-  for (int j = tid; j < vocab; j += 512) mx = fmaxf(mx, Elem<IN>::one(row[j]) * unit);
-  mx = block_reduce<true>(mx, red);
-  float sum = 0.f;
-  for (int j = tid; j < vocab; j += 512) sum += exp2f(Elem<IN>::one(row[j]) * unit - mx);
-  sum = block_reduce<false>(sum, red);
+  const float last = tid < rest ? Elem<T>::one(row[full * kPer + tid]) : -INFINITY;
+  uint4 v[NC > 0 ? NC : 1];
+  float mx = last, sum = 0.f;
+  if constexpr (NC > 0) {
+    if (full > 0) {
+      // behind the end a thread reads the last chunk again, which leaves the maximum
+      // and is not summed
+#pragma unroll
+      for (int i = 0; i < NC; ++i) v[i] = load_chunk(row + min(tid + TH * i, full - 1) * kPer);
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) mx = fmaxf(mx, Elem<T>::get(v[i], e));
+    }
+    mx = block_reduce<true>(mx, red) * unit;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (tid + TH * i < full)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) sum += __builtin_amdgcn_exp2f(fmaf(Elem<T>::get(v[i], e), unit, -mx));
+    if (tid < rest) sum += __builtin_amdgcn_exp2f(fmaf(last, unit, -mx));
+    sum = block_reduce<false>(sum, red);
+  } else {
+    mx = tid < rest ? last * unit : -INFINITY;
+    sum = tid < rest ? (last == last && mx != INFINITY ? 1.f : NAN) : 0.f;
+    if (tid < rest && mx == -INFINITY) sum = 0.f;
+    for (int c0 = tid; c0 < full; c0 += TH * kAhead) {
+      uint4 a[kAhead];
+      float m = mx;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) a[i] = load_chunk(row + min(c0 + TH * i, full - 1) * kPer);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) m = fmaxf(m, Elem<T>::get(a[i], e) * unit);
+      const float ref = m == -INFINITY ? 0.f : m;
+      sum *= mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - ref);  // nothing summed yet, or NaN
+      mx = m;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (c0 + TH * i < full)
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) sum += __builtin_amdgcn_exp2f(fmaf(Elem<T>::get(a[i], e), unit, -ref));
+    }
+    const float all = block_reduce<true>(mx, red);
+    sum *= mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - all);
+    sum = block_reduce<false>(sum, red);
+    mx = all;
+  }
   const float lse = mx + log2f(sum);
   const int n = words > 0 ? words : 1;
-  const int32_t* ids = t.ids + r * n;
   float cross = 0.f;
-  bool unknown = false;
-  for (int k = tid; k < n; k += 512) {
-    const int32_t id = ids[k];
-    unknown |= id == kUnknown;
+  for (int k = tid; k < n; k += TH) {
+    const int32_t id = t.ids[r * n + k];
+    if (id == kUnknown) cross = NAN;
     const float share = words > 0 ? t.share[r * n + k] : 1.f;
     if (id < 0 || id == kNoWord || share == -1.f) continue;
-    const float l = Elem<IN>::one(row[id]) * unit - lse;  // log2 p
+    const float l = fmaf(Elem<T>::one(row[id]), unit, -lse);  // log2 p
     at_word[k] = l;
     if (share != 0.f) cross -= share * l;
   }
-  cross = block_reduce<false>(unknown ? NAN : cross, red);
-  const float loss = heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f));
-  if (tid == 0) row_loss[r] = w * loss;
+  cross = block_reduce<false>(cross, red);
+  if (tid == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
   if (dx == nullptr) return;
   const float c = cross == cross ? heat * w * *t.factor : NAN;
-  for (int j = tid; j < vocab; j += 512) out[j] = Elem<OUT>::of(c * exp2f(Elem<IN>::one(row[j]) * unit - lse));
+  auto grad = [&](const uint4& a, int at) {
+    float o[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] = c * __builtin_amdgcn_exp2f(fmaf(Elem<T>::get(a, e), unit, -lse));
+    store_grad(out + at * kPer, o);
+  };
+  if constexpr (NC > 0) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (tid + TH * i < full) grad(v[i], tid + TH * i);
+  } else {
+    for (int c0 = tid; c0 < full; c0 += TH * kAhead) {
+      uint4 a[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) a[i] = load_chunk(row + min(c0 + TH * i, full - 1) * kPer);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (c0 + TH * i < full) grad(a[i], c0 + TH * i);
+    }
+  }
+  if (tid < rest) out[full * kPer + tid] = Elem<T>::of(c * __builtin_amdgcn_exp2f(fmaf(last, unit, -lse)));
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stored before the words' own
   __syncthreads();
-  for (int k = tid; k < n; k += 512) {
-    const int32_t id = ids[k];
+  for (int k = tid; k < n; k += TH) {
+    const int32_t id = t.ids[r * n + k];
     const float share = words > 0 ? t.share[r * n + k] : 1.f;
     if (id < 0 || id == kNoWord || share == -1.f) continue;
-    out[id] = Elem<OUT>::of(c * (exp2f(at_word[k]) - share));
+    out[id] = Elem<T>::of(c * (__builtin_amdgcn_exp2f(at_word[k]) - share));
   }
 }
 
@@ -439,19 +622,35 @@ __global__ __launch_bounds__(256) void outer_kernel(const T* __restrict__ a, int
   for (int64_t i = blockIdx.y; i < m; i += gridDim.y) out[i * n + j] = Elem<OUT>::of(Elem<T>::one(a[i * lda]) * bj);
 }
 
-// p *= *g in place; leaves at once where *g is 1.
+// p *= *g in place over whole 16-byte chunks and what is behind them.
 template <typename T>
-__global__ __launch_bounds__(256) void scale_kernel(T* __restrict__ p, int64_t n, const float* __restrict__ g) {
+__device__ __forceinline__ void scale_values(T* __restrict__ p, int64_t n, float f) {
+  constexpr int kPer = Elem<T>::kPer;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256, first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  for (int64_t i = first; i < n / kPer; i += step) {
+    const uint4 v = load_chunk(p + i * kPer);
+    float o[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] = Elem<T>::get(v, e) * f;
+    store_grad(p + i * kPer, o);
+  }
+  if (first < n % kPer) p[n / kPer * kPer + first] = Elem<T>::of(Elem<T>::one(p[n / kPer * kPer + first]) * f);
+}
+
+// Two tensors times *g; leaves at once where *g is 1.
+__global__ __launch_bounds__(256) void scale_kernel(int f32_0, void* p0, int64_t n0, int f32_1, void* p1, int64_t n1,
+                                                    const float* __restrict__ g) {
   const float f = *g;
   if (f == 1.f) return;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step)
-    p[i] = Elem<T>::of(Elem<T>::one(p[i]) * f);
+  if (f32_0) scale_values(static_cast<float*>(p0), n0, f);
+  else scale_values(static_cast<uint16_t*>(p0), n0, f);
+  if (f32_1) scale_values(static_cast<float*>(p1), n1, f);
+  else scale_values(static_cast<uint16_t*>(p1), n1, f);
 }
 
 unsigned blocks_of(int64_t n) {
   const int64_t b = (n + 255) / 256;
-  return static_cast<unsigned>(b < 1 ? 1 : b > 4096 ? 4096 : b);
+  return static_cast<unsigned>(b < 1 ? 1 : b > 2048 ? 2048 : b);
 }
 
 // ------------------------------------------------------------------- pieces
@@ -474,7 +673,7 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   p.ldz = (vocab + 63) & ~63LL;
   p.slabs = (vocab + kLossSlab - 1) / kLossSlab;
   const int64_t n_words = words > 0 ? words : 1;
-  const int64_t each = p.fused ? (grads ? p.ldz * 2 : p.slabs * 8) : p.ldz * (grads && !f32 ? 6 : 4);
+  const int64_t each = !p.fused ? p.ldz * 4 : grads ? p.ldz * 2 : p.slabs * 8;
   int64_t n = kPieceBytes / each / 256 * 256;
   if (n < 256) n = 256;
   if (n > rows) n = rows < 1 ? 1 : rows;
@@ -492,7 +691,7 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
     p.d = grads ? take(n * p.ldz * 2) : 0;
   } else {
     p.z = take(n * p.ldz * 4);
-    p.d = grads && !f32 ? take(n * p.ldz * 2) : p.z;
+    p.d = p.z;  // in place
   }
   p.ldx = (hidden + 63) & ~63LL;
   p.x = grads ? take(rows * p.ldx * (f32 ? 4 : 2)) : 0;
@@ -504,20 +703,31 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   return p;
 }
 
-int logits_rows(bool in_f32, bool out_f32, const void* x, int64_t rows, int64_t vocab, int64_t ld, const Targets& t,
-                int64_t words, float heat, float* row_loss, void* dx, int64_t ldd, hipStream_t st) {
-  if (rows == 0) return MOC_OK;
+template <typename T>
+void launch_logits(const T* x, int64_t rows, int vocab, int64_t ld, const Targets& t, int words, float heat,
+                   float* row_loss, T* dx, int64_t ldd, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(rows));
+  const int chunks = vocab / Elem<T>::kPer;
+#define MOC_LOGITS(NC, TH) \
+  logits_loss_kernel<T, NC, TH><<<grid, TH, 0, st>>>(x, ld, vocab, t, words, heat, row_loss, dx, ldd)
+  if (chunks <= 4 * 256) MOC_LOGITS(4, 256);
+  else if (chunks <= 4 * 512) MOC_LOGITS(4, 512);
+  else if (chunks <= 8 * 512) MOC_LOGITS(8, 512);
+  else if (chunks <= 8 * 1024) MOC_LOGITS(8, 1024);
+  else if (chunks <= 16 * 1024) MOC_LOGITS(16, 1024);
+  else MOC_LOGITS(0, 1024);
+#undef MOC_LOGITS
+}
+
+int logits_rows(bool f32, const void* x, int64_t rows, int64_t vocab, int64_t ld, const Targets& t, int64_t words,
+                float heat, float* row_loss, void* dx, int64_t ldd, hipStream_t st) {
+  if (rows == 0) return MOC_OK;
   const int v = static_cast<int>(vocab), k = static_cast<int>(words);
-  if (in_f32 && out_f32)
-    logits_loss_kernel<float, float><<<grid, 512, 0, st>>>(static_cast<const float*>(x), ld, v, t, k, heat, row_loss,
-                                                           static_cast<float*>(dx), ldd);
-  else if (in_f32)
-    logits_loss_kernel<float, uint16_t><<<grid, 512, 0, st>>>(static_cast<const float*>(x), ld, v, t, k, heat,
-                                                              row_loss, static_cast<uint16_t*>(dx), ldd);
+  if (f32)
+    launch_logits(static_cast<const float*>(x), rows, v, ld, t, k, heat, row_loss, static_cast<float*>(dx), ldd, st);
   else
-    logits_loss_kernel<uint16_t, uint16_t><<<grid, 512, 0, st>>>(static_cast<const uint16_t*>(x), ld, v, t, k, heat,
-                                                                 row_loss, static_cast<uint16_t*>(dx), ldd);
+    launch_logits(static_cast<const uint16_t*>(x), rows, v, ld, t, k, heat, row_loss, static_cast<uint16_t*>(dx), ldd,
+                  st);
   return check_launch("logits_loss_kernel");
 }
 
@@ -565,14 +775,9 @@ extern "C" int moc_label_targets(const int64_t* labels, int64_t rows, int64_t vo
   hipStream_t st = as_stream(stream);
   Targets t;
   targets_layout(rows, 0, vocab, static_cast<char*>(targets), &t);
-  if (rows > 0) {
-    label_targets_kernel<<<static_cast<unsigned>((rows + 255) / 256), 256, 0, st>>>(labels, rows, vocab, ignore_index,
-                                                                                    row_weight, t);
-    const int rc = check_launch("label_targets_kernel");
-    if (rc != MOC_OK) return rc;
-  }
-  target_total_kernel<<<1, 1024, 0, st>>>(rows, mean, grad, t);
-  return check_launch("target_total_kernel");
+  label_targets_kernel<<<static_cast<unsigned>(1 + (rows + 255) / 256), 256, 0, st>>>(labels, rows, vocab, ignore_index,
+                                                                                      row_weight, mean, grad, t);
+  return check_launch("label_targets_kernel");
 }
 
 extern "C" int moc_teacher_targets(const void* ids, int ids_dtype, int64_t ids_ld, const void* top, int top_dtype,
@@ -591,11 +796,12 @@ extern "C" int moc_teacher_targets(const void* ids, int ids_dtype, int64_t ids_l
   Targets t;
   targets_layout(rows, words, vocab, static_cast<char*>(targets), &t);
   if (rows > 0) {
-    const dim3 grid(static_cast<unsigned>(rows));
-    const int k = static_cast<int>(words);
-#define MOC_TEACHER(ID, F)                                                                                          \
-  teacher_targets_kernel<ID, F><<<grid, 256, 0, st>>>(static_cast<const ID*>(ids), ids_ld, top, top_ld, k, vocab, \
-                                                      temperature, row_weight, t, (int)tiles_of(vocab))
+    const int k = static_cast<int>(words), tiles = static_cast<int>(tiles_of(vocab));
+#define MOC_TEACHER(ID, F)                                                                                            \
+  (k <= 64 ? teacher_wave_kernel<ID, F><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(                        \
+                 static_cast<const ID*>(ids), ids_ld, top, top_ld, rows, k, vocab, temperature, row_weight, t, tiles) \
+           : teacher_targets_kernel<ID, F><<<static_cast<unsigned>(rows), 256, 0, st>>>(                               \
+                 static_cast<const ID*>(ids), ids_ld, top, top_ld, k, vocab, temperature, row_weight, t, tiles))
     if (ids_dtype == MOC_I32 && top_dtype == MOC_F32) MOC_TEACHER(int32_t, true);
     else if (ids_dtype == MOC_I32) MOC_TEACHER(int32_t, false);
     else if (top_dtype == MOC_F32) MOC_TEACHER(int64_t, true);
@@ -621,7 +827,7 @@ extern "C" int moc_logits_loss(int dtype, const void* logits, int64_t rows, int6
   Targets t;
   targets_layout(rows, words, vocab, static_cast<char*>(targets), &t);
   const bool f32 = dtype == MOC_F32;
-  int rc = logits_rows(f32, f32, logits, rows, vocab, ld, t, words, temperature, row_loss, dlogits, ldd, st);
+  int rc = logits_rows(f32, logits, rows, vocab, ld, t, words, temperature, row_loss, dlogits, ldd, st);
   if (rc != MOC_OK || loss == nullptr) return rc;
   loss_sum_kernel<<<1, 1024, 0, st>>>(row_loss, rows, t.total, loss);
   return check_launch("loss_sum_kernel");
@@ -724,7 +930,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       rc = moc_gemm_ws(dtype, n, vocab, hidden, xi, ldx, 1, w, 1, ldw, 0, nullptr, 0, 0, nullptr, 0, 0, ws + p.z, p.ldz,
                        MOC_F32, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
-      rc = logits_rows(true, f32, ws + p.z, n, vocab, p.ldz, ti, words, temperature, row_loss + r0,
+      rc = logits_rows(true, ws + p.z, n, vocab, p.ldz, ti, words, temperature, row_loss + r0,
                        grads ? ws + p.d : nullptr, p.ldz, st);
     }
     if (rc != MOC_OK) return rc;
@@ -765,14 +971,14 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
   return check_launch("loss_sum_kernel");
 }
 
-extern "C" int moc_scale_inplace(int dtype, void* p, int64_t n, const float* factor, void* stream) {
-  MOC_REQUIRE(dtype == MOC_BF16 || dtype == MOC_F32, "moc_scale_inplace: bf16 or f32");
-  MOC_REQUIRE(n >= 0 && (n == 0 || p != nullptr) && factor != nullptr, "moc_scale_inplace: null operand");
-  if (n == 0) return MOC_OK;
-  hipStream_t st = as_stream(stream);
-  if (dtype == MOC_F32)
-    scale_kernel<float><<<blocks_of(n), 256, 0, st>>>(static_cast<float*>(p), n, factor);
-  else
-    scale_kernel<uint16_t><<<blocks_of(n), 256, 0, st>>>(static_cast<uint16_t*>(p), n, factor);
+extern "C" int moc_scale_inplace(int dtype0, void* p0, int64_t n0, int dtype1, void* p1, int64_t n1,
+                                 const float* factor, void* stream) {
+  MOC_REQUIRE((dtype0 == MOC_BF16 || dtype0 == MOC_F32) && (dtype1 == MOC_BF16 || dtype1 == MOC_F32),
+              "moc_scale_inplace: bf16 or f32");
+  MOC_REQUIRE(n0 >= 0 && n1 >= 0 && (n0 == 0 || p0 != nullptr) && (n1 == 0 || p1 != nullptr) && factor != nullptr,
+              "moc_scale_inplace: null operand");
+  if (n0 + n1 == 0) return MOC_OK;
+  scale_kernel<<<blocks_of((n0 > n1 ? n0 : n1) / 8), 256, 0, as_stream(stream)>>>(dtype0 == MOC_F32, p0, n0,
+                                                                                dtype1 == MOC_F32, p1, n1, factor);
   return check_launch("scale_kernel");
 }

@@ -280,9 +280,10 @@ class _Kept:
         grads, self.grads = self.grads, None
         if grads is None or (torch.cuda.is_current_stream_capturing() and not self.captured):
             return None
-        for t in grads:
-            if t is not None:
-                N.call("moc_scale_inplace", N.dtype_code(t.dtype), t.data_ptr(), t.numel(), g.data_ptr(), N.stream_of(t))
+        given = [t for t in grads if t is not None]
+        a, b = given[0], given[-1]
+        N.call("moc_scale_inplace", N.dtype_code(a.dtype), a.data_ptr(), a.numel(), N.dtype_code(b.dtype), b.data_ptr(),
+               b.numel() if len(given) > 1 else 0, g.data_ptr(), N.stream_of(a))
         return grads
 
 

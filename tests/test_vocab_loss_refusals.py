@@ -92,9 +92,10 @@ def test_entry_points_refuse():
         ("moc_linear_loss", (0, p, 3, 0, 8, p, 10, 8, p, 0, 1.0, p, p, None, 0, None, 0, p, 1 << 40, None, 0, None)),
         ("moc_linear_loss", (0, p, 3, 128, 128, p, 1 << 23, 128, p, 0, 1.0, p, p, None, 0, None, 0, p, 1 << 40, None, 0,
                              None)),
-        ("moc_scale_inplace", (5, p, 8, p, None)),
-        ("moc_scale_inplace", (0, None, 8, p, None)),
-        ("moc_scale_inplace", (0, p, 8, None, None)),
+        ("moc_scale_inplace", (5, p, 8, 0, None, 0, p, None)),
+        ("moc_scale_inplace", (0, None, 8, 0, None, 0, p, None)),
+        ("moc_scale_inplace", (0, p, 8, 0, None, 8, p, None)),
+        ("moc_scale_inplace", (0, p, 8, 0, None, 0, None, None)),
     ]
     for name, args in bad:
         assert getattr(lib, name)(*args) == N.MOC_ERR_INVALID, (name, args)
