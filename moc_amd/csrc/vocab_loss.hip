@@ -473,23 +473,139 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
 }
 
 // ------------------------------------------------- logits that were not stored
-// log2 of a row's sum of exponentials from its slabs' maxima and sums.
-template <bool WAVE>
+// Up to 16 rows, losses alone: the weight is read once, straight into the operand
+// registers of v_mfma_f32_16x16x32_bf16 (a wave 16 words, a workgroup a slab of 64),
+// 16 loads ahead; the rows stand in LDS in fragment order.  Bound by the weight's
+// bytes: few_us below.
+constexpr int kFewRows = 16, kFewAhead = 16, kFewHidden = 4096;
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+__global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restrict__ h, int64_t ldh, int rows,
+                                                       const uint16_t* __restrict__ w, int64_t ldw, int vocab,
+                                                       int hidden, float unit, const int32_t* __restrict__ ids,
+                                                       const uint16_t* __restrict__ first, int words,
+                                                       float* __restrict__ z, float2* __restrict__ stat, int slabs) {
+  extern __shared__ uint4 frag[];  // [steps][64], then the waves' maxima and sums
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int steps = (hidden + 31) / 32, tiles = (vocab + kLossTile - 1) / kLossTile;
+  float2* part = reinterpret_cast<float2*>(frag + steps * 64);  // [2][4][16]
+  const int row = lane & 15, quad = lane >> 4;
+  const bool ragged = hidden % 32 != 0 && 32 * (steps - 1) + 8 * quad >= hidden;  // its last chunk lies behind
+  auto load = [&](uint4 (&a)[kFewAhead], const uint16_t* src, int s0) {
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int s = min(s0 + i, steps - 1);
+      a[i] = *reinterpret_cast<const uint4*>(src + 32 * (ragged && s == steps - 1 ? 0 : s));
+    }
+  };
+  auto word_of = [&](int slab) {
+    return w + static_cast<int64_t>(min(slab * kLossSlab + wave * 16 + row, vocab - 1)) * ldw + 8 * quad;
+  };
+  uint4 a[kFewAhead], b[kFewAhead];
+  int slab = blockIdx.x;
+  load(a, word_of(slab), 0);
+  for (int i = tid; i < steps * 64; i += 256) {
+    const int n = i & 15, k = i / 64 * 32 + 8 * (i % 64 / 16);
+    frag[i] = n < rows && k < hidden ? *reinterpret_cast<const uint4*>(h + n * ldh + k) : make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
+  for (int turn = 0; slab < slabs; slab += gridDim.x, turn ^= 1) {
+    const uint16_t* src = word_of(slab);
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    auto products = [&](uint4 (&v)[kFewAhead], int s0) {
+#pragma unroll
+      for (int i = 0; i < kFewAhead; ++i) {
+        if (s0 + i >= steps) break;
+        uint4 x = v[i];
+        if (ragged && s0 + i == steps - 1) x = make_uint4(0, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x),
+                                                      __builtin_bit_cast(bf16x8_t, frag[(s0 + i) * 64 + lane]), acc, 0,
+                                                      0, 0);
+      }
+    };
+    for (int s0 = 0; s0 < steps; s0 += 2 * kFewAhead) {
+      if (s0 + kFewAhead < steps) load(b, src, s0 + kFewAhead);
+      products(a, s0);
+      if (s0 + 2 * kFewAhead < steps) load(a, src, s0 + 2 * kFewAhead);
+      else if (slab + static_cast<int>(gridDim.x) < slabs) load(a, word_of(slab + gridDim.x), 0);
+      products(b, s0 + kFewAhead);
+    }
+    // lane: row, words slab * 64 + wave * 16 + 4 quad + e
+    const int c0 = wave * 16 + 4 * quad;
+    if (row < rows) {
+      int k = first != nullptr ? first[row * tiles + slab / (kLossTile / kLossSlab)] : 0;
+      for (; k < words; ++k) {
+        const int c = ids[row * words + k] - slab * kLossSlab - c0;
+        if (c >= 4) break;
+        if (c >= 0 && c < 4) z[row * words + k] = c == 0 ? acc[0] : c == 1 ? acc[1] : c == 2 ? acc[2] : acc[3];
+      }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[e] = slab * kLossSlab + c0 + e < vocab ? acc[e] * unit : -INFINITY;
+      m = fmaxf(m, acc[e]);
+    }
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(acc[e] - ref);
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if (lane < 16) part[(turn * 4 + wave) * 16 + row] = make_float2(m, s);
+    __syncthreads();
+    if (tid < rows) {
+      float all = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) all = fmaxf(all, part[(turn * 4 + i) * 16 + tid].x);
+      const float r = all == -INFINITY ? 0.f : all;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = part[(turn * 4 + i) * 16 + tid];
+        sum += v.y * __builtin_amdgcn_exp2f(v.x - r);
+      }
+      stat[static_cast<int64_t>(tid) * slabs + slab] = make_float2(all, sum);
+    }
+  }
+}
+
+int launch_few(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab, int64_t ldw,
+               float unit, const Targets& t, int64_t words, float* z, float2* stat, int64_t slabs, hipStream_t st) {
+  const int steps = static_cast<int>((hidden + 31) / 32);
+  const int lds = steps * 1024 + 2 * 4 * 16 * 8;
+  const int64_t resident = static_cast<int64_t>(cu_count()) * (160 * 1024 / lds < 8 ? 160 * 1024 / lds : 8);
+  const unsigned grid = static_cast<unsigned>(slabs < resident ? slabs : resident);
+  few_rows_kernel<<<grid, 256, lds, st>>>(static_cast<const uint16_t*>(h), ldh, (int)rows,
+                                          static_cast<const uint16_t*>(w), ldw, (int)vocab, (int)hidden, unit, t.ids,
+                                          words > 0 ? t.first : nullptr, (int)(words > 0 ? words : 1), z, stat,
+                                          (int)slabs);
+  return check_launch("few_rows_kernel");
+}
+
+// log2 of a row's sum of exponentials from its slabs' maxima and sums; 256 threads,
+// a slab's loads in flight with its seven followers'.
 __device__ __forceinline__ float slabs_lse(const float2* __restrict__ stat, int slabs, float* red) {
-  const int first = WAVE ? threadIdx.x & 63 : threadIdx.x, step = WAVE ? 64 : blockDim.x;
   float m = -INFINITY, s = 0.f;
-  for (int i = first; i < slabs; i += step) {
-    const float2 v = stat[i];
-    const float n = fmaxf(m, v.x), ref = n == -INFINITY ? 0.f : n;
-    s = s * __builtin_amdgcn_exp2f(m - ref) + v.y * __builtin_amdgcn_exp2f(v.x - ref);
+  for (int i0 = threadIdx.x; i0 < slabs; i0 += 256 * 8) {
+    float2 v[8];
+    float n = m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = i0 + 256 * i < slabs ? stat[i0 + 256 * i] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n = fmaxf(n, v[i].x);
+    const float ref = n == -INFINITY ? 0.f : n;
+    s *= m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - ref);  // nothing summed yet, or NaN
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += v[i].y * __builtin_amdgcn_exp2f(v[i].x - ref);
     m = n;
   }
-  float all = m;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
-  if (!WAVE) all = block_reduce<true>(all, red);
-  s *= m == -INFINITY ? (s == s ? 0.f : s) : __builtin_amdgcn_exp2f(m - all);
-  s = WAVE ? wave_sum(s) : block_reduce<false>(s, red);
+  const float all = block_reduce<true>(m, red);
+  s *= m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - all);
+  s = block_reduce<false>(s, red);
   return all + log2f(s);
 }
 
@@ -511,21 +627,20 @@ __device__ __forceinline__ float cross_of(const Targets& t, int64_t r, int words
   return cross;
 }
 
-// Losses alone: one wave a row.
-__global__ __launch_bounds__(256) void slabs_loss_kernel(const float2* __restrict__ stat, int slabs, int64_t rows,
-                                                         Targets t, int words, float heat,
-                                                         const float* __restrict__ z, float* __restrict__ row_loss) {
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (r >= rows) return;
+// Losses alone: one workgroup a row.
+__global__ __launch_bounds__(256) void slabs_loss_kernel(const float2* __restrict__ stat, int slabs, Targets t,
+                                                         int words, float heat, const float* __restrict__ z,
+                                                         float* __restrict__ row_loss) {
+  __shared__ float red[4];
+  const int64_t r = blockIdx.x;
   const float w = t.weight[r];
-  if (w == 0.f) {
-    if (lane == 0) row_loss[r] = 0.f;
+  if (w == 0.f) {  // uniform
+    if (threadIdx.x == 0) row_loss[r] = 0.f;
     return;
   }
-  const float lse = slabs_lse<true>(stat + r * slabs, slabs, nullptr);
-  const float cross = wave_sum(cross_of(t, r, words, z, kLog2E / heat, lse, nullptr, lane, 64));
-  if (lane == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
+  const float lse = slabs_lse(stat + r * slabs, slabs, red);
+  const float cross = block_reduce<false>(cross_of(t, r, words, z, kLog2E / heat, lse, nullptr, threadIdx.x, 256), red);
+  if (threadIdx.x == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
 }
 
 // One workgroup a row: its loss, and its f16 exponentials into bf16 gradients of
@@ -547,7 +662,7 @@ __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld
     return;
   }
   const float2* st = stat + r * slabs;
-  const float lse = slabs_lse<false>(st, slabs, red);
+  const float lse = slabs_lse(st, slabs, red);
   const float cross = block_reduce<false>(cross_of(t, r, words, z, kLog2E / heat, lse, at_word, tid, 256), red);
   if (tid == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
   const float c = cross == cross ? heat * w * *t.factor : NAN;
@@ -914,7 +1029,9 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     if (p.fused) {
       float2* stat = reinterpret_cast<float2*>(ws + p.stat);
       float* z = reinterpret_cast<float*>(ws + p.at_words);
-      rc = launch_loss_gemm(xi, n, hidden, ldx, w, vocab, ldw, kLog2E / temperature, ti.ids,
+      const bool few = !grads && n <= kFewRows && hidden % 8 == 0 && hidden <= kFewHidden;
+      rc = few ? launch_few(xi, n, hidden, ldx, w, vocab, ldw, kLog2E / temperature, ti, words, z, stat, p.slabs, st)
+               : launch_loss_gemm(xi, n, hidden, ldx, w, vocab, ldw, kLog2E / temperature, ti.ids,
                             words > 0 ? ti.first : nullptr, n_words, z, stat, grads ? ws + p.d : nullptr, p.ldz, st);
       MOC_REQUIRE(rc <= 0, "moc_linear_loss: operands of up to 2 GiB");
       if (rc != MOC_OK) return rc;
@@ -923,8 +1040,8 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
             reinterpret_cast<uint16_t*>(ws + p.d), p.ldz, (int)vocab, stat, (int)p.slabs, ti, (int)words, temperature, z,
             row_loss + r0);
       else
-        slabs_loss_kernel<<<static_cast<unsigned>((n + 3) / 4), 256, 0, st>>>(stat, (int)p.slabs, n, ti, (int)words,
-                                                                              temperature, z, row_loss + r0);
+        slabs_loss_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(stat, (int)p.slabs, ti, (int)words, temperature, z,
+                                                                    row_loss + r0);
       rc = check_launch("slabs_grad_kernel");
     } else {
       rc = moc_gemm_ws(dtype, n, vocab, hidden, xi, ldx, 1, w, 1, ldw, 0, nullptr, 0, 0, nullptr, 0, 0, ws + p.z, p.ldz,

@@ -189,11 +189,13 @@ def _unit(t):
 
 # -------------------------------------------------------------------- operands
 def _rows16(t) -> torch.Tensor:
-    """t [rows, cols] with 16-byte aligned rows of unit stride, a copy if it has others."""
+    """t [rows, cols] with 16-byte aligned rows of unit stride, whose storage holds all
+    of the last one's pitch (the kernels read whole chunks); a copy of any other."""
     rows, cols = t.shape
     per = 16 // t.element_size()
-    if (t.stride(1) == 1 or cols == 1) and t.data_ptr() % 16 == 0 and (
-            rows <= 1 or (t.stride(0) % per == 0 and t.stride(0) >= cols)):
+    pitch = _pitch(t)
+    if (t.stride(1) == 1 or cols == 1) and t.data_ptr() % 16 == 0 and pitch % per == 0 and pitch >= cols and (
+            (t.storage_offset() + rows * pitch) * t.element_size() <= t.untyped_storage().nbytes()):
         return t
     out = K.padded_empty(rows, cols, t.dtype, t.device)
     return out.copy_(t)

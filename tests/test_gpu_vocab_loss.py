@@ -157,6 +157,35 @@ def test_linear_distillation(rows, d, vocab, dtype, words, heat, ragged, reducti
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [1, 3, 16, 17, 129])
+@pytest.mark.parametrize("d,vocab", [(8, 1), (40, 63), (104, 64), (64, 65), (256, 1003), (1000, 4099), (2048, 32000),
+                                     (4096, 5000), (4104, 700), (520, 128256)])
+def test_losses_alone(rows, d, vocab, dtype):
+    """Without gradients: rows' losses and their mean, labels and a teacher's words."""
+    h, w = operands(rows, d, vocab, dtype)
+    y = labels_of(rows, vocab, 0.3)
+    y[rows // 2] = vocab - 1
+    ids, top = teacher_of(rows, vocab, 70 if rows == 3 else 9, True)
+    hd, wd = h.to(F64), w.to(F64)
+    z, z_err = hd @ wd.t(), logit_error(hd, wd)
+    h[y == -100] = math.nan
+    label = torch.zeros(rows, vocab, dtype=F64, device="cuda")
+    label[torch.arange(rows, device="cuda"), y.clamp(min=0)] = 1
+    weight = rand(rows, seed=9).abs() + 0.1
+    want, _, _ = reference(z, label, y != -100, weight.to(F64), 1.0, "none")
+    out = L.linear_cross_entropy(h, w, y, weight, reduction="none")
+    check(out, want, (None, None), (hd, wd), z, z, label, z_err, 1.0, 1.0, weight)
+    mean = L.linear_cross_entropy(h, w, y, weight)
+    check(mean, want.sum() / torch.where(y != -100, weight.to(F64), 0.0).sum(), (None, None), (hd, wd), z, z, label, z_err,
+          1.0, 1.0, weight)
+    h = torch.where((y == -100)[:, None], hd.to(dtype), h)
+    q, some = shares(ids, top, vocab, 1.5)
+    want, _, _ = reference(z, q, some, weight.to(F64), 1.5, "none")
+    check(L.linear_distillation(h, w, ids, top, weight, temperature=1.5, reduction="none"), want, (None, None), (hd, wd), z,
+          z, q, z_err, 1.5, 1.0, weight)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (2, 3), (5, 500), (33, 1003), (7, 32000), (3, 50021), (2, 128256),
                                         (2, 262147), (600, 4096)])
 @pytest.mark.parametrize("words,heat,ragged,reduction", [(1, 1.0, False, "mean"), (20, 2.0, True, "mean"),
