@@ -354,8 +354,9 @@ __device__ __forceinline__ void store_grad(float* p, const float (&v)[4]) {
 
 // One workgroup a row: maximum, sum, loss, gradient (dx may be x).  NC > 0: the row
 // stays in registers, NC chunks of 16 bytes a thread, all loads in flight before the
-// first is used; NC = 0: it is read twice, the second time from the caches.
-template <typename T, int NC, int TH>
+// first is used, and LC more in LDS; NC = 0: it is read twice, the second time from
+// the caches.
+template <typename T, int NC, int TH, int LC = 0>
 __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld, int vocab, Targets t, int words,
                                                          float heat, float* __restrict__ row_loss, T* dx, int64_t ldd) {
   constexpr int kPer = Elem<T>::kPer, kAhead = 4;
@@ -378,11 +379,20 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
   const float unit = kLog2E / heat;
   const float last = tid < rest ? Elem<T>::one(row[full * kPer + tid]) : -INFINITY;
   uint4 v[NC > 0 ? NC : 1];
+  __shared__ uint4 more[LC > 0 ? LC * TH : 1];  // chunks NC .. NC + LC of each thread, read by it alone
   float mx = last, sum = 0.f;
   if constexpr (NC > 0) {
     if (full > 0) {
       // behind the end a thread reads the last chunk again, which leaves the maximum
       // and is not summed
+#pragma unroll
+      for (int i = 0; i < LC; ++i) v[i] = load_chunk(row + min(tid + TH * (NC + i), full - 1) * kPer);
+#pragma unroll
+      for (int i = 0; i < LC; ++i) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) mx = fmaxf(mx, Elem<T>::get(v[i], e));
+        more[i * TH + tid] = v[i];
+      }
 #pragma unroll
       for (int i = 0; i < NC; ++i) v[i] = load_chunk(row + min(tid + TH * i, full - 1) * kPer);
 #pragma unroll
@@ -391,6 +401,13 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
         for (int e = 0; e < kPer; ++e) mx = fmaxf(mx, Elem<T>::get(v[i], e));
     }
     mx = block_reduce<true>(mx, red) * unit;
+#pragma unroll
+    for (int i = 0; i < LC; ++i)
+      if (tid + TH * (NC + i) < full) {
+        const uint4 a = more[i * TH + tid];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) sum += __builtin_amdgcn_exp2f(fmaf(Elem<T>::get(a, e), unit, -mx));
+      }
 #pragma unroll
     for (int i = 0; i < NC; ++i)
       if (tid + TH * i < full)
@@ -451,6 +468,9 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
 #pragma unroll
     for (int i = 0; i < NC; ++i)
       if (tid + TH * i < full) grad(v[i], tid + TH * i);
+#pragma unroll
+    for (int i = 0; i < LC; ++i)
+      if (tid + TH * (NC + i) < full) grad(more[i * TH + tid], tid + TH * (NC + i));
   } else {
     for (int c0 = tid; c0 < full; c0 += TH * kAhead) {
       uint4 a[kAhead];
@@ -818,18 +838,21 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   return p;
 }
 
+constexpr int moc_th(int th, int = 0) { return th; }
+
 template <typename T>
 void launch_logits(const T* x, int64_t rows, int vocab, int64_t ld, const Targets& t, int words, float heat,
                    float* row_loss, T* dx, int64_t ldd, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(rows));
   const int chunks = vocab / Elem<T>::kPer;
-#define MOC_LOGITS(NC, TH) \
-  logits_loss_kernel<T, NC, TH><<<grid, TH, 0, st>>>(x, ld, vocab, t, words, heat, row_loss, dx, ldd)
+#define MOC_LOGITS(NC, ...) \
+  logits_loss_kernel<T, NC, __VA_ARGS__><<<grid, moc_th(__VA_ARGS__), 0, st>>>(x, ld, vocab, t, words, heat, row_loss, dx, ldd)
   if (chunks <= 4 * 256) MOC_LOGITS(4, 256);
   else if (chunks <= 4 * 512) MOC_LOGITS(4, 512);
   else if (chunks <= 8 * 512) MOC_LOGITS(8, 512);
   else if (chunks <= 8 * 1024) MOC_LOGITS(8, 1024);
   else if (chunks <= 16 * 1024) MOC_LOGITS(16, 1024);
+  else if (chunks <= 32 * 1024) MOC_LOGITS(24, 1024, 8);
   else MOC_LOGITS(0, 1024);
 #undef MOC_LOGITS
 }
