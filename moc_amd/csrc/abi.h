@@ -50,13 +50,19 @@ int launch_gate_up_2of8(const void* x, int64_t nb, int64_t hidden, const void* w
 // stored (gemm.hip): per row and slab of 64 words the maximum of x = unit logit and
 // the sum of exp2(x - it) (stat [rows][ceil(vocab / 64)]); exp2(x - it + 15) as f16
 // (kept, rows a multiple of 64 apart; null: no); the logits of the words ids
-// [rows][words] (ascending) in z, first [rows][ceil(vocab / 256)]: how many of a
-// row's lie left of each tile of 256 words (null for one word).  1: operands too
-// large for its 32-bit offsets (nothing launched).
-constexpr int kLossTile = 256, kLossSlab = 64;
+// [rows][words] (ascending) in z, first [slabs + 1][ld_first]: how many of a row's
+// lie left of each slab (null for one word).  1: operands too large for its 32-bit
+// offsets (nothing launched).
+constexpr int kLossSlab = 64;
 int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab,
-                     int64_t ldw, float unit, const int32_t* ids, const uint16_t* first, int64_t words, float* z,
-                     float2* stat, void* kept, int64_t ld_kept, hipStream_t st);
+                     int64_t ldw, float unit, const int32_t* ids, const uint16_t* first, int64_t ld_first,
+                     int64_t words, float* z, float2* stat, void* kept, int64_t ld_kept, hipStream_t st);
+
+// C [M, N] = A [M, K] B [K, N] (bf16, K-contiguous A, N-contiguous B) over a long K
+// (gemm.hip); workspace as moc_gemm_ws uses it.
+int64_t gemm_long_k_workspace(int64_t M, int64_t N, int64_t K);
+int gemm_long_k(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
+                int64_t ldc, int c_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 // out = x + y over n values (a multiple of 8), x and out f32, y bf16
 // (rmsnorm.hip).

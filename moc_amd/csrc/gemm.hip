@@ -171,13 +171,14 @@ struct GemmArgs {
   // row and slab of 64 columns the maximum m of x = unit C and the sum of exp2(x - m)
   // (ls_stat [M][ls_slabs]), the exponentials as f16 (C, rows ldc apart, null: not
   // kept) and C itself in f32 at the columns named by ls_ids [M][ls_words]
-  // (ascending; ls_z of the same shape; ls_first [M][tiles_n]: how many of a row's
-  // lie left of the tile, null for one a row).
+  // (ascending; ls_z of the same shape; ls_first [ls_slabs + 1][ls_ld_first]: how many
+  // of a row's lie left of each slab, null for one a row).
   float2* ls_stat;
   int ls_slabs, ls_words;
   float ls_unit;
   const int32_t* ls_ids;
   const uint16_t* ls_first;
+  int64_t ls_ld_first;
   float* ls_z;
 };
 
@@ -921,6 +922,10 @@ __device__ __forceinline__ void gu28_epilogue(const GemmArgs& g, char* lds, cons
 }
 
 // ---------------------------------------------------------- loss epilogue
+// LDS from here on is the epilogue's: the slots before it take the first halves of
+// the workgroup's next tile meanwhile (sequence numbers 0 to 2).
+constexpr int kLossStage = 3 * kSlotBytes;
+static_assert(kLossStage + 8 * 32 * (64 * 2 + 16) <= kRingBytes, "LOSS: staging behind three slots");
 // The wave's MI x 32 rows of 64 logits while they are in f32: a lane holds 32 of
 // one row's (columns 32j + 8q + 4(l >> 5) + r), lane l ^ 32 the other 32, so a
 // slab's maximum and sum are 31 operations in the lane and one exchange.  What is
@@ -930,54 +935,80 @@ __device__ __forceinline__ void gu28_epilogue(const GemmArgs& g, char* lds, cons
 // counts.  Measured at 4096 x 32000 x 2048: see launch_loss_gemm.
 template <int MI>
 __device__ __forceinline__ void loss_epilogue(const GemmArgs& g, char* lds, f32x16_t (&acc)[MI][2], int row0,
-                                              int col0, int tn, int wm, int wn, int wave, int lane) {
+                                              int col0, int wm, int wn, int wave, int lane) {
   constexpr int kPitch = 64 * 2 + 16;
-  char* reg = lds + wave * (32 * kPitch);
+  char* reg = lds + kLossStage + wave * (32 * kPitch);
   const int slab0 = col0 + wn, half = lane >> 5;
   const bool edge = slab0 + 64 > g.N;
+  // which of its words each row has in the slab, all rows' loads together
+  int next[MI], last[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int row = row0 + wm + 32 * i + (lane & 31);
+    next[i] = last[i] = 0;
+    if (row < g.M && slab0 < g.N) {
+      if (g.ls_first != nullptr) {
+        const uint16_t* first = g.ls_first + static_cast<int64_t>(slab0 >> 6) * g.ls_ld_first + row;
+        next[i] = first[0];
+        last[i] = first[g.ls_ld_first];
+      } else {  // one word a row
+        last[i] = g.ls_ids[row] >> 6 == slab0 >> 6;
+      }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int row = row0 + wm + 32 * i + (lane & 31);
     const bool live = row < g.M;
-    if (g.ls_words > 0) {
-      const int32_t* ids = g.ls_ids + static_cast<int64_t>(row) * g.ls_words;
-      float* z = g.ls_z + static_cast<int64_t>(row) * g.ls_words;
-      int k = live && g.ls_first != nullptr ? g.ls_first[static_cast<int64_t>(row) * g.tiles_n + tn] : 0;
-      while (true) {
-        const int c = (live && k < g.ls_words ? ids[k] : 0x7FFFFFFF) - slab0;
-        if (!__any(c < 64 && c > -256)) break;  // words of the tile's slabs to the left come first
-        if (c >= 0 && c < 64 && ((c >> 2) & 1) == half) {
-          const int at = ((c >> 5) << 4) + ((c >> 3) << 2 & 12) + (c & 3);
-          float v = 0.f;
+    // logits of the row's words among the lane's 32: the register by the bits of its number
+    float* z = g.ls_z + static_cast<int64_t>(row) * g.ls_words;
+    auto put = [&](int c, int k) {
+      float v[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v = at == e ? acc[i][e >> 4][e & 15] : v;
-          z[k] = v;
-        }
-        ++k;
+      for (int e = 0; e < 16; ++e) {
+        const float lo = acc[i][0][e], hi = acc[i][1][e];
+        v[e] = c & 32 ? hi : lo;
       }
+#pragma unroll
+      for (int n = 8; n > 0; n >>= 1)  // columns 16, 8, 2 and 1 apart
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+          const float lo = v[e], hi = v[e + n];
+          v[e] = c & (n > 2 ? 2 * n : n) ? hi : lo;
+        }
+      z[k] = v[0];
+    };
+    for (int k = next[i]; __any(k < last[i]); ++k) {
+      const int c = k < last[i] ? g.ls_ids[static_cast<int64_t>(row) * g.ls_words + k] - slab0 : -1;
+      if (c >= 0 && ((c >> 2) & 1) == half) put(c, k);
+    }
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (slab0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3) >= g.N) acc[i][j][r] = -INFINITY;
     }
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float x = acc[i][j][r] * g.ls_unit;
-        if (edge && slab0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3) >= g.N) x = -INFINITY;
-        acc[i][j][r] = x;
-        m = fmaxf(m, x);
-      }
-    m = fmaxf(m, __shfl_xor(m, 32));
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+    m = fmaxf(m, __shfl_xor(m, 32)) * g.ls_unit;
     const float ref = m == -INFINITY ? 0.f : m - 15.f;
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float e = __builtin_amdgcn_exp2f(acc[i][j][r] - ref);
+        const float e = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], g.ls_unit, -ref));
         acc[i][j][r] = e;
         s += e;
       }
     s += __shfl_xor(s, 32);
+    // the next tile's first halves have landed before this one's stores are issued:
+    // its main loop waits for no store right away
+    if (i == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (live && half == 0 && slab0 < g.N)
       g.ls_stat[static_cast<int64_t>(row) * g.ls_slabs + (slab0 >> 6)] = make_float2(m, s * 0x1p-15f);
     if (g.C == nullptr) continue;
@@ -1066,7 +1097,7 @@ void gemm_pp_kernel(GemmArgs g) {
   }
   int tm, tn;
   tile_coords(tbid, g.tiles_m, g.tiles_n, tm, tn);
-  if (!GU && !DUAL && !SPLIT && g.ncat_tn > 0 && tn >= g.ncat_tn) {
+  if (!GU && !DUAL && !SPLIT && !LOSS && g.ncat_tn > 0 && tn >= g.ncat_tn) {
     tn -= g.ncat_tn;
     g.b[0] = g.b[1];
     g.C = g.C2;
@@ -1074,8 +1105,8 @@ void gemm_pp_kernel(GemmArgs g) {
     g.ldc = g.ldc2;
     g.vec_store = g.vec_store2;
   }
-  const int row0 = tm * (SHORT ? 128 : kBM);
-  const int col0 = GU ? tn * 128 : tn * kBN;  // GU: channel base of the gate and up halves
+  int row0 = tm * (SHORT ? 128 : kBM);
+  int col0 = GU ? tn * 128 : tn * kBN;  // GU: channel base of the gate and up halves
   const int wm = (sw >> 1) * (SHORT ? 64 : 128);
   const int wn = (sw & 1) * 128 + grp * 64;
   const uint32_t lds0 = lds_addr(lds);
@@ -1098,12 +1129,15 @@ void gemm_pp_kernel(GemmArgs g) {
   fb_map.init(kSlotB, wn - hb * 128, lane);
 
   f32x16_t acc[MI][2];
+  auto clear = [&]() {
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  };
+  clear();
 
   bf16x8_t fa[4][MI], fb[4][2];  // [k16 step][block]  (SP: fa[32-channel step][block])
   uint32_t fm[4];               // SP: positions of the stored A values, per block
@@ -1295,10 +1329,42 @@ void gemm_pp_kernel(GemmArgs g) {
   // out a load's latency in the phase that issued it.  Slot reuse: H0(t + 1)
   // takes the slot of H1(t - 1) and H1(t + 2) that of H0(t - 1), both last
   // read in phase 2t - 1.
+  // LOSS: a workgroup's tiles are bid, bid + gridDim, ...; the first halves of the next
+  // one are requested behind the last phase, before the epilogue, and a group's
+  // waits (vmcnt(0) there) leave them landed.
+  auto tile_first = [&]() {
+    if (grp == 0) {
+      load_half(kt0, 0);
+      load_half(kt0, 1);
+    } else if (kt0 + 1 < nk) {
+      load_half(kt0 + 1, 1);
+    }
+  };
+  tile_first();
+  [[maybe_unused]] auto lane_again = []() {
+    int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  [[maybe_unused]] int at_row0 = row0, at_col0 = col0;
+  [[maybe_unused]] bool more = false;
+  [[maybe_unused]] auto tile_next = [&]() {
+    at_row0 = row0;
+    at_col0 = col0;
+    tbid += static_cast<int>(gridDim.x);
+    more = tbid < g.tiles_m * g.tiles_n;
+    if (!more) return;
+    tile_coords(tbid, g.tiles_m, g.tiles_n, tm, tn);
+    row0 = tm * (SHORT ? 128 : kBM);
+    col0 = tn * kBN;
+    const int l = lane_again();  // nothing of this is kept in registers over the tiles
+    ma0.init(g.a[0], row0, sw, l);
+    mb0.init(g.b[0], col0, sw, l);
+    tile_first();
+  };
+  if (grp == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+next_tile:
   if (grp == 0) {
-    load_half(kt0, 0);
-    load_half(kt0, 1);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     fix_half(kt0, 0);
     fix_half(kt0, 1);
     phase_end();
@@ -1313,8 +1379,8 @@ void gemm_pp_kernel(GemmArgs g) {
       }
       phase_end();  // phase 2t+1 -> 2t+2
     }
+    if constexpr (LOSS) tile_next();
   } else {
-    if (kt0 + 1 < nk) load_half(kt0 + 1, 1);
     phase_end();
     for (int t = kt0; t < nk; ++t) {
       if (t > kt0) compute();
@@ -1334,10 +1400,20 @@ void gemm_pp_kernel(GemmArgs g) {
       phase_end();  // phase 2t+1 -> 2t+2
     }
     compute();
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (LOSS) tile_next();
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   if constexpr (LOSS) {
-    loss_epilogue<MI>(g, lds, acc, row0, col0, tn, wm, wn, wave, lane);
+    loss_epilogue<MI>(g, lds, acc, at_row0, at_col0, wm, wn, wave, lane_again());
+    if (more) {
+      clear();
+      // group 1 starts without a product: its fragments' old values are not kept
+#pragma unroll
+      for (int e = 0; e < 4 * MI; ++e) asm volatile("" : "=v"(fa[e / MI][e % MI]));
+      asm volatile("" : "=v"(fb[0][0]), "=v"(fb[0][1]), "=v"(fb[1][0]), "=v"(fb[1][1]), "=v"(fb[2][0]), "=v"(fb[2][1]),
+                   "=v"(fb[3][0]), "=v"(fb[3][1]));
+      goto next_tile;
+    }
   } else if constexpr (GU) {
     gu28_epilogue(g, lds, acc, row0, col0, wm, wn, tid, lane);
   } else if constexpr (SPLIT) {
@@ -1986,13 +2062,16 @@ struct SplitPlan {
   int64_t bytes = 0;
 };
 
-SplitPlan plan_split(int64_t M, int64_t N, int nk) {
+// step > 1: only multiples of it (see gemm_long_k).
+SplitPlan plan_split(int64_t M, int64_t N, int nk, int step = 1) {
   SplitPlan p;
   p.kper = nk;
   const int64_t tiles = ((M + kBM - 1) / kBM) * ((N + kBN - 1) / kBN);
   const int cus = cu_count();
   if (tiles <= 0 || 3 * tiles > cus) return p;
   int ks = static_cast<int>(std::min<int64_t>(cus / tiles, nk / 4));
+  if (step > 1)
+    for (ks -= ks % step; ks > 0 && (nk + ks - 1) / ks * (ks - 1) >= nk;) ks -= step;
   if (ks < 2) return p;
   const int kper = (nk + ks - 1) / ks;
   ks = (nk + kper - 1) / kper;
@@ -2031,7 +2110,9 @@ SplitPlan plan_split(int64_t M, int64_t N, int nk) {
 // small tiles (17 to 12000 rows, 4 to 164 K tiles): within 20 %, 6 % in the
 // mean.  The costs above are up to half high where K is long (1280 x 2605 x
 // 6200: 70 against 54 us) and a third low for the shortest.
-MidPlan plan_mid(int64_t M, int64_t N, int nk, int64_t n2, int64_t ws_bytes) {
+//
+// step > 1: K splits in multiples of it alone (see gemm_long_k).
+MidPlan plan_mid(int64_t M, int64_t N, int nk, int64_t n2, int64_t ws_bytes, int step = 1) {
   struct Tile {
     int bm, bn;
     double t1, t2, t0;  // cost
@@ -2058,6 +2139,7 @@ MidPlan plan_mid(int64_t M, int64_t N, int nk, int64_t n2, int64_t ws_bytes) {
     for (int ks = 1; ks <= ks_max; ++ks) {
       const int kper = (nk + ks - 1) / ks;
       if (kper * (ks - 1) >= nk) continue;  // the last part would be empty
+      if (ks > 1 && ks % step != 0) continue;
       const int64_t bytes = ks > 1 ? kFixCounterBytes + ks * M * ldw * 4 : 0;
       if (bytes > ws_bytes) break;
       const int full = n * ks / (2 * cus), rem = n * ks - full * 2 * cus;
@@ -2170,13 +2252,13 @@ bool short_whole_ok(int64_t M, int64_t N, int nk) {
 //   3604 x 712 x 5544   45.6 (5 parts)      53.6 (128 x 128, in 4)
 //   1280 x 3398 x 5000  60.8 (3 parts)      79.3 (128 x 128, in 2)
 //   1280 x 2605 x 6200  56.2 (4 parts)      52.9 (128 x 128, in 2)
-double wide_us(int64_t M, int64_t N, int nk, bool two, bool a_kc, int64_t ws_bytes) {
+double wide_us(int64_t M, int64_t N, int nk, bool two, bool a_kc, int64_t ws_bytes, int step = 1) {
   if (a_kc && short_whole_ok(M, N, nk)) return 5.8 + 0.74 * nk + (two ? 2 : 0);
   if (a_kc) {
     const FixPlan f = plan_fix_short(M, N, nk);
     if (f.tail > 0 && f.bytes <= ws_bytes) return (11.6 + 0.73 * f.cost) / 0.9;
   }
-  const SplitPlan s = plan_split(M, N, nk);
+  const SplitPlan s = plan_split(M, N, nk, step);
   if (s.ksplit > 1 && s.bytes <= ws_bytes)
     return (9.7 + 1.23 * s.kper + s.ksplit * 2.0 * M * s.ldw * 4 / 6.8e6) / 0.95;
   return HUGE_VAL;
@@ -2247,8 +2329,8 @@ PairSplitPlan plan_split_pair(int64_t M1, int64_t N1, int nk1, int64_t M2, int64
 // Logits h w^T of a loss (see GemmArgs::ls_stat and abi.h).  128-row tiles where
 // 256-row ones would leave half of the CUs idle.
 int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab,
-                     int64_t ldw, float unit, const int32_t* ids, const uint16_t* first, int64_t words, float* z,
-                     float2* stat, void* kept, int64_t ld_kept, hipStream_t st) {
+                     int64_t ldw, float unit, const int32_t* ids, const uint16_t* first, int64_t ld_first,
+                     int64_t words, float* z, float2* stat, void* kept, int64_t ld_kept, hipStream_t st) {
   GemmArgs a{};
   const bool ok = make_operand(h, ldh, true, rows, hidden, a.a[0]) && make_operand(w, ldw, true, vocab, hidden, a.b[0]);
   auto no_wrap = [](const Operand& o) {
@@ -2275,8 +2357,10 @@ int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, c
   a.ls_unit = unit;
   a.ls_ids = ids;
   a.ls_first = first;
+  a.ls_ld_first = ld_first;
   a.ls_z = z;
-  const dim3 grid(static_cast<unsigned>(a.tiles_m * a.tiles_n)), block(kPpThreads);
+  const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
+  const dim3 grid(static_cast<unsigned>(tiles < cu_count() ? tiles : cu_count())), block(kPpThreads);
   if (short_m) gemm_pp_kernel<true, true, false, false, false, false, false, true, true><<<grid, block, 0, st>>>(a);
   else gemm_pp_kernel<true, true, false, false, false, false, false, false, true><<<grid, block, 0, st>>>(a);
   return check_launch("gemm_pp_kernel (loss)");
@@ -2518,7 +2602,8 @@ namespace {
 int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int64_t a_sm, int64_t a_sk,
                  const void* B, int64_t b_sk, int64_t b_sn, int64_t K2, const void* A2, int64_t a2_sm,
                  int64_t a2_sk, const void* B2, int64_t b2_sk, int64_t b2_sn, void* C, int64_t ldc, int c_dtype,
-                 void* workspace, int64_t workspace_bytes, void* stream, const void* res, int64_t ldres) {
+                 void* workspace, int64_t workspace_bytes, void* stream, const void* res, int64_t ldres,
+                 int step = 1) {
   MOC_REQUIRE(dtype == MOC_BF16 || dtype == MOC_F32, "moc_gemm: dtype must be bf16 or f32");
   MOC_REQUIRE(res == nullptr || (dtype == MOC_BF16 && c_dtype == MOC_BF16 && aligned16(res) && ldres % 8 == 0 &&
                                  ldres >= N),
@@ -2658,8 +2743,8 @@ int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int6
   // small tiles (a K split only with a workspace for its partials)
   const int nk_all = a.nk[0] + a.nk[1];
   const int64_t ws_have = workspace != nullptr && aligned16(workspace) ? workspace_bytes : 0;
-  const MidPlan mp = a.pp ? plan_mid(M, N, nk_all, 0, ws_have) : MidPlan();
-  if (mp.bm > 0 && mp.us <= wide_us(M, N, nk_all, a.nk[1] > 0, la == 1, ws_have)) {
+  const MidPlan mp = a.pp ? plan_mid(M, N, nk_all, 0, ws_have, step) : MidPlan();
+  if (mp.bm > 0 && mp.us <= wide_us(M, N, nk_all, a.nk[1] > 0, la == 1, ws_have, step)) {
     GemmArgs run = a;
     run.tiles_m = static_cast<int>((M + mp.bm - 1) / mp.bm);
     run.tiles_n = static_cast<int>((N + mp.bn - 1) / mp.bn);
@@ -2695,7 +2780,7 @@ int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int6
   a.ksplit = 1;
   a.kper = a.nk[0] + a.nk[1];
   a.ws_stride = 0;
-  const SplitPlan sp = short_m ? SplitPlan() : plan_split(M, N, a.nk[0] + a.nk[1]);
+  const SplitPlan sp = short_m ? SplitPlan() : plan_split(M, N, a.nk[0] + a.nk[1], step);
   const bool split = a.pp && sp.ksplit > 1 && workspace != nullptr && workspace_bytes >= sp.bytes &&
                      reinterpret_cast<uintptr_t>(workspace) % 16 == 0;
   GemmArgs run = a;
@@ -2750,6 +2835,27 @@ extern "C" int moc_gemm_ws(int dtype, int64_t M, int64_t N, int64_t K, const voi
   return gemm_ws_impl(dtype, M, N, K, A, a_sm, a_sk, B, b_sk, b_sn, K2, A2, a2_sm, a2_sk, B2, b2_sk, b2_sn, C,
                       ldc, c_dtype, workspace, workspace_bytes, stream, nullptr, 0);
 }
+
+namespace moc {
+
+// C [M, N] = A B, A [M, K] rows of lda, B [K, N] rows of ldb, bf16, K long (a
+// gradient of hidden rows: K is the vocabulary).  As moc_gemm_ws, but K is split in
+// multiples of 8 ways alone: workgroup ids go to the XCDs in turn, so a K range then
+// stays in one XCD's L2, where 9 ways have every XCD read every range (777 x 512 x
+// 32000: TIMES).
+int64_t gemm_long_k_workspace(int64_t M, int64_t N, int64_t K) {
+  const int nk = static_cast<int>((K + kBK - 1) / kBK);
+  return std::max({plan_split(M, N, nk, 8).bytes, plan_fix(M, N, nk).bytes, plan_fix_short(M, N, nk).bytes,
+                   plan_mid(M, N, nk, 0, INT64_MAX, 8).bytes});
+}
+
+int gemm_long_k(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
+                int64_t ldc, int c_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  return gemm_ws_impl(MOC_BF16, M, N, K, A, lda, 1, B, ldb, 1, 0, nullptr, 0, 0, nullptr, 0, 0, C, ldc, c_dtype,
+                      workspace, workspace_bytes, stream, nullptr, 0, 8);
+}
+
+}  // namespace moc
 
 // C = bf16(bf16(A B) + R): moc_gemm_ws for bf16 operands and output with the
 // residual R [M, N] (rows ldres apart) added in the epilogue (the decoder

@@ -32,10 +32,10 @@ struct Targets {
   float* entropy;   // [rows] sum of q ln q (teacher only)
   int32_t* ids;     // [rows][words] ascending, kNoWord behind the last
   float* share;     // [rows][words] (teacher only); a word's second entry: -1
-  uint16_t* first;  // [rows][tiles of kLossTile words] (teacher only) words left of the tile
+  uint16_t* first;  // [slabs + 1][rows] (teacher only) words left of each slab
 };
 
-int64_t tiles_of(int64_t vocab) { return (vocab + kLossTile - 1) / kLossTile; }
+int64_t slabs_of(int64_t vocab) { return (vocab + kLossSlab - 1) / kLossSlab; }
 
 int64_t align256(int64_t n) { return (n + 255) & ~255LL; }
 
@@ -51,7 +51,7 @@ int64_t targets_layout(int64_t rows, int64_t words, int64_t vocab, char* base, T
   char* ids = take(rows * (words > 0 ? words : 1) * 4);
   char* entropy = words > 0 ? take(rows * 4) : nullptr;
   char* share = words > 0 ? take(rows * words * 4) : nullptr;
-  char* first = words > 0 ? take(rows * tiles_of(vocab) * 2) : nullptr;
+  char* first = words > 0 ? take(rows * (slabs_of(vocab) + 1) * 2) : nullptr;
   if (t != nullptr) {
     t->total = reinterpret_cast<double*>(base);
     t->factor = reinterpret_cast<float*>(base + 8);
@@ -134,9 +134,7 @@ template <typename ID, bool TOP_F32>
 __global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict__ ids, int64_t ids_ld,
                                                            const void* __restrict__ top, int64_t top_ld, int64_t rows,
                                                            int words, int64_t vocab, float heat,
-                                                           const float* __restrict__ row_weight, Targets t,
-                                                           int tiles) {
-  __shared__ int32_t sorted[4][64];
+                                                           const float* __restrict__ row_weight, Targets t) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + wave;
   if (r >= rows) return;
@@ -182,17 +180,6 @@ __global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict_
     t.weight[r] = !some ? 0.f : row_weight != nullptr ? row_weight[r] : 1.f;
     t.entropy[r] = some ? h : 0.f;
   }
-  sorted[wave][lane] = id;
-  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own row
-  __builtin_amdgcn_wave_barrier();
-  for (int n = lane; n < tiles; n += 64) {
-    int lo = 0;
-#pragma unroll
-    for (int step = 32; step > 0; step >>= 1)
-      if (sorted[wave][lo + step - 1] < n * kLossTile) lo += step;
-    lo += sorted[wave][lo] < n * kLossTile;
-    t.first[r * tiles + n] = static_cast<uint16_t>(lo);
-  }
 }
 
 // One workgroup a row.  Words sorted by rank (ties by place); entries of the
@@ -201,8 +188,7 @@ template <typename ID, bool TOP_F32>
 __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restrict__ ids, int64_t ids_ld,
                                                               const void* __restrict__ top, int64_t top_ld, int words,
                                                               int64_t vocab, float heat,
-                                                              const float* __restrict__ row_weight, Targets t,
-                                                              int tiles) {
+                                                              const float* __restrict__ row_weight, Targets t) {
   __shared__ int32_t id[kMaxWords], sorted_id[kMaxWords];
   __shared__ float q[kMaxWords], sorted_q[kMaxWords];
   __shared__ float red[4];
@@ -229,7 +215,6 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restri
       t.ids[r * words + k] = kNoWord;
       t.share[r * words + k] = -1.f;
     }
-    for (int n = tid; n < tiles; n += 256) t.first[r * tiles + n] = 0;
     if (tid == 0) {
       t.weight[r] = 0.f;
       t.entropy[r] = 0.f;
@@ -264,19 +249,46 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restri
     t.ids[r * words + k] = mine;
     t.share[r * words + k] = share;
   }
-  for (int n = tid; n < tiles; n += 256) {
-    int lo = 0, hi = words;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (sorted_id[mid] < n * kLossTile) lo = mid + 1;
-      else hi = mid;
-    }
-    t.first[r * tiles + n] = static_cast<uint16_t>(lo);
-  }
   h = block_reduce<false>(h, red);
   if (tid == 0) {
     t.weight[r] = row_weight != nullptr ? row_weight[r] : 1.f;
     t.entropy[r] = h;
+  }
+}
+
+// How many of a row's words lie left of each slab: 64 rows a workgroup, a lane a
+// row, so that the table's lines are written and read whole; each of the 16 waves
+// walks a sixteenth of the slabs along its rows' words, which stand in LDS up to
+// kWordsLds of them (a chain of loads from memory otherwise: 8192 rows of 64 words
+// 22 us, 500 slabs).
+constexpr int kWordsLds = 200;
+
+__global__ __launch_bounds__(1024) void words_left_kernel(const int32_t* __restrict__ ids, int64_t rows, int words,
+                                                          int slabs, uint16_t* __restrict__ first) {
+  extern __shared__ int32_t held[];  // [64][words | 1]
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64, r = r0 + (threadIdx.x & 63);
+  const int32_t* mine = ids + r * words;
+  if (words <= kWordsLds) {
+    const int n = static_cast<int>(rows - r0 < 64 ? rows - r0 : 64) * words;
+    for (int i = threadIdx.x; i < n; i += 1024) held[i / words * (words | 1) + i % words] = ids[r0 * words + i];
+    __syncthreads();
+    mine = held + (threadIdx.x & 63) * (words | 1);
+  }
+  if (r >= rows) return;
+  const int per = (slabs + 16) / 16, n0 = threadIdx.x / 64 * per;
+  int lo = 0, hi = words;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (mine[mid] < n0 * kLossSlab) lo = mid + 1;
+    else hi = mid;
+  }
+  int id = lo < words ? mine[lo] : kNoWord;
+  for (int n = n0; n < n0 + per && n <= slabs; ++n) {
+    while (id < n * kLossSlab) {
+      ++lo;
+      id = lo < words ? mine[lo] : kNoWord;
+    }
+    first[n * rows + r] = static_cast<uint16_t>(lo);
   }
 }
 
@@ -504,11 +516,11 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restrict__ h, int64_t ldh, int rows,
                                                        const uint16_t* __restrict__ w, int64_t ldw, int vocab,
                                                        int hidden, float unit, const int32_t* __restrict__ ids,
-                                                       const uint16_t* __restrict__ first, int words,
+                                                       const uint16_t* __restrict__ first, int64_t ld_first, int words,
                                                        float* __restrict__ z, float2* __restrict__ stat, int slabs) {
   extern __shared__ uint4 frag[];  // [steps][64], then the waves' maxima and sums
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int steps = (hidden + 31) / 32, tiles = (vocab + kLossTile - 1) / kLossTile;
+  const int steps = (hidden + 31) / 32;
   float2* part = reinterpret_cast<float2*>(frag + steps * 64);  // [2][4][16]
   const int row = lane & 15, quad = lane >> 4;
   const bool ragged = hidden % 32 != 0 && 32 * (steps - 1) + 8 * quad >= hidden;  // its last chunk lies behind
@@ -554,7 +566,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
     // lane: row, words slab * 64 + wave * 16 + 4 quad + e
     const int c0 = wave * 16 + 4 * quad;
     if (row < rows) {
-      int k = first != nullptr ? first[row * tiles + slab / (kLossTile / kLossSlab)] : 0;
+      int k = first != nullptr ? first[slab * ld_first + row] : 0;
       for (; k < words; ++k) {
         const int c = ids[row * words + k] - slab * kLossSlab - c0;
         if (c >= 4) break;
@@ -593,15 +605,16 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
 }
 
 int launch_few(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab, int64_t ldw,
-               float unit, const Targets& t, int64_t words, float* z, float2* stat, int64_t slabs, hipStream_t st) {
+               float unit, const Targets& t, int64_t ld_first, int64_t words, float* z, float2* stat, int64_t slabs,
+               hipStream_t st) {
   const int steps = static_cast<int>((hidden + 31) / 32);
   const int lds = steps * 1024 + 2 * 4 * 16 * 8;
   const int64_t resident = static_cast<int64_t>(cu_count()) * (160 * 1024 / lds < 8 ? 160 * 1024 / lds : 8);
   const unsigned grid = static_cast<unsigned>(slabs < resident ? slabs : resident);
   few_rows_kernel<<<grid, 256, lds, st>>>(static_cast<const uint16_t*>(h), ldh, (int)rows,
                                           static_cast<const uint16_t*>(w), ldw, (int)vocab, (int)hidden, unit, t.ids,
-                                          words > 0 ? t.first : nullptr, (int)(words > 0 ? words : 1), z, stat,
-                                          (int)slabs);
+                                          words > 0 ? t.first : nullptr, ld_first, (int)(words > 0 ? words : 1), z,
+                                          stat, (int)slabs);
   return check_launch("few_rows_kernel");
 }
 
@@ -726,13 +739,29 @@ __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld
 }
 
 // Rows that count, zeros for the others: what is in those reaches no product.
+// Rows of 16-byte chunks, whose last one is cut off at the hidden size.
 template <typename T>
-__global__ __launch_bounds__(256) void counted_rows_kernel(const T* __restrict__ h, int64_t ldh, int hidden,
-                                                           const float* __restrict__ weight, T* __restrict__ out,
-                                                           int64_t ldo) {
-  const int64_t r = blockIdx.x;
-  const bool counts = weight[r] != 0.f;
-  for (int j = threadIdx.x; j < hidden; j += 256) out[r * ldo + j] = counts ? h[r * ldh + j] : T(0);
+__global__ __launch_bounds__(256) void counted_rows_kernel(const T* __restrict__ h, int64_t ldh, int64_t rows,
+                                                           int hidden, const float* __restrict__ weight,
+                                                           T* __restrict__ out, int64_t ldo) {
+  constexpr int kPer = Elem<T>::kPer;
+  const int chunks = (hidden + kPer - 1) / kPer;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows * chunks; i += step) {
+    const int64_t r = i / chunks;
+    const int k = static_cast<int>(i - r * chunks) * kPer;
+    T part[kPer] = {};
+    if (weight[r] != 0.f) {
+      if (k + kPer <= hidden) {
+        *reinterpret_cast<uint4*>(out + r * ldo + k) = *reinterpret_cast<const uint4*>(h + r * ldh + k);
+        continue;
+      }
+      for (int e = 0; k + e < hidden; ++e) part[e] = h[r * ldh + k + e];
+    }
+    uint4 v;
+    __builtin_memcpy(&v, part, 16);
+    *reinterpret_cast<uint4*>(out + r * ldo + k) = v;
+  }
 }
 
 // a += b over n values; out (may be null): the sum as bf16 or f32.
@@ -806,7 +835,7 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   const bool f32 = dtype == MOC_F32;
   p.fused = !f32;
   p.ldz = (vocab + 63) & ~63LL;
-  p.slabs = (vocab + kLossSlab - 1) / kLossSlab;
+  p.slabs = slabs_of(vocab);
   const int64_t n_words = words > 0 ? words : 1;
   const int64_t each = !p.fused ? p.ldz * 4 : grads ? p.ldz * 2 : p.slabs * 8;
   int64_t n = kPieceBytes / each / 256 * 256;
@@ -934,12 +963,12 @@ extern "C" int moc_teacher_targets(const void* ids, int ids_dtype, int64_t ids_l
   Targets t;
   targets_layout(rows, words, vocab, static_cast<char*>(targets), &t);
   if (rows > 0) {
-    const int k = static_cast<int>(words), tiles = static_cast<int>(tiles_of(vocab));
+    const int k = static_cast<int>(words);
 #define MOC_TEACHER(ID, F)                                                                                            \
   (k <= 64 ? teacher_wave_kernel<ID, F><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(                        \
-                 static_cast<const ID*>(ids), ids_ld, top, top_ld, rows, k, vocab, temperature, row_weight, t, tiles) \
+                 static_cast<const ID*>(ids), ids_ld, top, top_ld, rows, k, vocab, temperature, row_weight, t) \
            : teacher_targets_kernel<ID, F><<<static_cast<unsigned>(rows), 256, 0, st>>>(                               \
-                 static_cast<const ID*>(ids), ids_ld, top, top_ld, k, vocab, temperature, row_weight, t, tiles))
+                 static_cast<const ID*>(ids), ids_ld, top, top_ld, k, vocab, temperature, row_weight, t))
     if (ids_dtype == MOC_I32 && top_dtype == MOC_F32) MOC_TEACHER(int32_t, true);
     else if (ids_dtype == MOC_I32) MOC_TEACHER(int32_t, false);
     else if (top_dtype == MOC_F32) MOC_TEACHER(int64_t, true);
@@ -987,7 +1016,7 @@ extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, 
     int64_t b = p.fused ? 0 : moc_gemm_workspace_size(dtype, n, vocab, hidden, 0);
     if (b > most) most = b;
     if (!grads) continue;
-    b = moc_gemm_workspace_size(dtype, n, hidden, vocab, 0);
+    b = p.fused ? gemm_long_k_workspace(n, hidden, vocab) : moc_gemm_workspace_size(dtype, n, hidden, vocab, 0);
     if (b > most) most = b;
     b = moc_gemm_workspace_size(dtype, vocab, hidden, n, 0);
     if (b > most) most = b;
@@ -1027,14 +1056,20 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
   const int64_t n_words = words > 0 ? words : 1;
   int rc;
   if (grads && rows > 0) {
-    const dim3 grid(static_cast<unsigned>(rows));
+    const unsigned grid = blocks_of(rows * ((hidden * es + 15) / 16));
     if (f32)
-      counted_rows_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(h), ldh, (int)hidden, t.weight,
+      counted_rows_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(h), ldh, rows, (int)hidden, t.weight,
                                                        reinterpret_cast<float*>(ws + p.x), p.ldx);
     else
-      counted_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(h), ldh, (int)hidden, t.weight,
-                                                          reinterpret_cast<uint16_t*>(ws + p.x), p.ldx);
+      counted_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(h), ldh, rows, (int)hidden,
+                                                          t.weight, reinterpret_cast<uint16_t*>(ws + p.x), p.ldx);
     if ((rc = check_launch("counted_rows_kernel")) != MOC_OK) return rc;
+  }
+  if (p.fused && words > 0 && rows > 0) {
+    words_left_kernel<<<static_cast<unsigned>((rows + 63) / 64), 1024,
+                        words <= kWordsLds ? 64 * (words | 1) * 4 : 0, st>>>(t.ids, rows, (int)words, (int)p.slabs,
+                                                                             t.first);
+    if ((rc = check_launch("words_left_kernel")) != MOC_OK) return rc;
   }
   const char* x = grads ? ws + p.x : static_cast<const char*>(h);
   const int64_t ldx = grads ? p.ldx : ldh;
@@ -1047,15 +1082,15 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     if (words > 0) {
       ti.entropy += r0;
       ti.share += r0 * words;
-      ti.first += r0 * tiles_of(vocab);
+      ti.first += r0;
     }
     if (p.fused) {
       float2* stat = reinterpret_cast<float2*>(ws + p.stat);
       float* z = reinterpret_cast<float*>(ws + p.at_words);
       const bool few = !grads && n <= kFewRows && hidden % 8 == 0 && hidden <= kFewHidden;
-      rc = few ? launch_few(xi, n, hidden, ldx, w, vocab, ldw, kLog2E / temperature, ti, words, z, stat, p.slabs, st)
+      rc = few ? launch_few(xi, n, hidden, ldx, w, vocab, ldw, kLog2E / temperature, ti, rows, words, z, stat, p.slabs, st)
                : launch_loss_gemm(xi, n, hidden, ldx, w, vocab, ldw, kLog2E / temperature, ti.ids,
-                            words > 0 ? ti.first : nullptr, n_words, z, stat, grads ? ws + p.d : nullptr, p.ldz, st);
+                            words > 0 ? ti.first : nullptr, rows, n_words, z, stat, grads ? ws + p.d : nullptr, p.ldz, st);
       MOC_REQUIRE(rc <= 0, "moc_linear_loss: operands of up to 2 GiB");
       if (rc != MOC_OK) return rc;
       if (grads)
@@ -1077,6 +1112,8 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     if (dh != nullptr) {
       char* to = static_cast<char*>(dh) + r0 * hidden * (dh_dtype == MOC_F32 ? 4 : 2);
       rc = vocab == 1 ? outer(dtype, n, hidden, ws + p.d, p.ldz, w, to, dh_dtype, st)
+           : p.fused  ? gemm_long_k(n, hidden, vocab, ws + p.d, p.ldz, w, ldw, to, hidden, dh_dtype, gemm_ws,
+                                    gemm_ws_bytes, stream)
                       : moc_gemm_ws(dtype, n, hidden, vocab, ws + p.d, p.ldz, 1, w, ldw, 1, 0, nullptr, 0, 0, nullptr, 0,
                                     0, to, hidden, dh_dtype, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
