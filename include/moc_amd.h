@@ -269,7 +269,7 @@ int moc_next_token_loss_backward(const void* logits, int64_t ld, int64_t batch, 
  * n the sum of the weights (mean = 1) or 1 (mean = 0).  A row of weight 0, with the
  * ignored label or without words counts for nothing, whatever it holds: its loss
  * and gradients are 0 and n leaves it out (no row left: a mean of NaN).  A label
- * outside the vocabulary gives NaN.  Up to 2^24 rows, 2^24 words, 1024 a row.
+ * outside the vocabulary gives NaN.  Up to 2^24 rows, 2^21 words, 1024 a row.
  *
  * targets: what the losses read of labels or teacher, written by one of the
  * first two calls (moc_loss_targets_size bytes, 16-byte aligned; words = 0 for

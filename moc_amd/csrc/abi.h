@@ -58,11 +58,13 @@ int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, c
                      int64_t ldw, float unit, const int32_t* ids, const uint16_t* first, int64_t ld_first,
                      int64_t words, float* z, float2* stat, void* kept, int64_t ld_kept, hipStream_t st);
 
-// C [M, N] = A [M, K] B [K, N] (bf16, K-contiguous A, N-contiguous B) over a long K
-// (gemm.hip); workspace as moc_gemm_ws uses it.
-int64_t gemm_long_k_workspace(int64_t M, int64_t N, int64_t K);
-int gemm_long_k(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
-                int64_t ldc, int c_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+// C [M, N] = *alpha A B (f16 operands, A with a unit stride along M or K, rows of B
+// ldb apart; C bf16 or f32) (gemm.hip); 16-byte aligned rows, workspace as
+// moc_gemm_ws uses it.
+int64_t gemm_half_workspace(int64_t M, int64_t N, int64_t K);
+int gemm_half(int64_t M, int64_t N, int64_t K, const void* A, int64_t a_sm, int64_t a_sk, const void* B, int64_t ldb,
+              void* C, int64_t ldc, int c_dtype, const float* alpha, void* workspace, int64_t workspace_bytes,
+              void* stream);
 
 // out = x + y over n values (a multiple of 8), x and out f32, y bf16
 // (rmsnorm.hip).

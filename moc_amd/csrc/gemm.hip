@@ -53,6 +53,7 @@ namespace {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x16_t __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void_t;
@@ -180,7 +181,28 @@ struct GemmArgs {
   const uint16_t* ls_first;
   int64_t ls_ld_first;
   float* ls_z;
+  // f16 operands (HALF = true; moc::gemm_half): C = *alpha A B
+  const float* alpha;
 };
+
+// The 16-bit type of a product's operands is the MFMA's business alone.
+template <bool HALF>
+__device__ __forceinline__ f32x16_t mfma16(bf16x8_t a, bf16x8_t b, f32x16_t c) {
+  if constexpr (HALF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                  0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+template <int MI, int NJ>
+__device__ __forceinline__ void scale_tile(f32x16_t (&acc)[MI][NJ], const float* alpha) {
+  const float f = *alpha;
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] *= f;
+}
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const Operand& o) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(o.p), (short)0, o.bytes,
@@ -1050,7 +1072,7 @@ __device__ __forceinline__ void loss_epilogue(const GemmArgs& g, char* lds, f32x
 // MFMA's orientation and leave through store_tile_t.
 // LOSS: the epilogue of a loss over the columns (see GemmArgs::ls_stat).
 template <bool A_KC, bool B_KC, bool OUT_F32, bool DUAL, bool SPLIT, bool GU = false, bool SP = false,
-          bool SHORT = false, bool LOSS = false>
+          bool SHORT = false, bool LOSS = false, bool HALF = false>
 __global__ __launch_bounds__(kPpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void gemm_pp_kernel(GemmArgs g) {
   static_assert(!SHORT || (A_KC && !GU && !SP), "128-row tiles: K-contiguous A, plain products");
@@ -1213,7 +1235,7 @@ void gemm_pp_kernel(GemmArgs g) {
         for (int i = 0; i < MI; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[ks][j], fa[ks][i], acc[i][j], 0, 0, 0);
+            acc[i][j] = mfma16<HALF>(fb[ks][j], fa[ks][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
           }
     }
@@ -1424,6 +1446,7 @@ next_tile:
   } else {
     if (part >= 0 && !fix_arrive<MI>(g, acc, slot, part, tid, reinterpret_cast<int*>(lds + kFlagOffset)))
       return;
+    if constexpr (HALF) scale_tile(acc, g.alpha);
     if constexpr (SP) store_tile_t<OUT_F32, 2>(g, lds, acc, row0, col0, wm, wn, wave, lane);
     else store_tile_w<OUT_F32, 2, MI>(g, lds, acc, row0, col0, wm, wn, wave, lane);
   }
@@ -1511,7 +1534,7 @@ struct MidMap {
   }
 };
 
-template <bool A_KC, bool B_KC, bool OUT_F32, int BM, int BN, int NS>
+template <bool A_KC, bool B_KC, bool OUT_F32, int BM, int BN, int NS, bool HALF = false>
 __global__ __launch_bounds__(kMidThreads) void gemm_mid_kernel(GemmArgs g) {
   constexpr int MI = BM / 64, NJ = BN / 64;         // 32-wide blocks of a wave's tile
   constexpr int kABytes = BM * kBK * 2, kStage = kABytes + BN * kBK * 2;
@@ -1597,11 +1620,12 @@ __global__ __launch_bounds__(kMidThreads) void gemm_mid_kernel(GemmArgs g) {
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+          acc[i][j] = mfma16<HALF>(fb[j], fa[i], acc[i][j]);
     }
   }
   __syncthreads();  // the ring becomes the epilogue's staging
   if (g.ksplit > 1) g.C = static_cast<float*>(g.C) + split * g.ws_stride;
+  else if constexpr (HALF) scale_tile(acc, g.alpha);
   store_tile_w<OUT_F32, NJ, MI>(g, lds, acc, row0, col0, wm, wn, wave, lane);
 }
 
@@ -1612,7 +1636,7 @@ template <bool OUT_F32>
 __device__ __forceinline__ void splitk_reduce_quad(int64_t q, const float* __restrict__ ws, int64_t stride,
                                                    int ksplit, int M, int N, int64_t ldw, void* __restrict__ C,
                                                    int64_t ldc, int vec, const uint16_t* __restrict__ res,
-                                                   int64_t ldres) {
+                                                   int64_t ldres, const float* __restrict__ alpha = nullptr) {
   const int qpr = (N + 3) / 4;
   if (q >= static_cast<int64_t>(M) * qpr) return;
   const int row = static_cast<int>(q / qpr), c = static_cast<int>(q % qpr) * 4;
@@ -1624,6 +1648,10 @@ __device__ __forceinline__ void splitk_reduce_quad(int64_t q, const float* __res
     s.y += v.y;
     s.z += v.z;
     s.w += v.w;
+  }
+  if (alpha != nullptr) {
+    const float f = *alpha;
+    s = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
   }
   float r[4] = {s.x, s.y, s.z, s.w};
   if (!OUT_F32 && res != nullptr) {
@@ -1656,9 +1684,10 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float* __restr
                                                             int ksplit, int M, int N, int64_t ldw,
                                                             void* __restrict__ C, int64_t ldc, int vec,
                                                             const uint16_t* __restrict__ res = nullptr,
-                                                            int64_t ldres = 0) {
+                                                            int64_t ldres = 0,
+                                                            const float* __restrict__ alpha = nullptr) {
   splitk_reduce_quad<OUT_F32>(static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, ws, stride, ksplit, M, N,
-                              ldw, C, ldc, vec, res, ldres);
+                              ldw, C, ldc, vec, res, ldres, alpha);
 }
 
 // The sums of a grouped split-K launch's two products in one launch:
@@ -1938,6 +1967,28 @@ void launch_bf16(const GemmArgs& a, bool out_f32, hipStream_t st, bool short_m =
                                        : static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.ksplit;
   const dim3 grid(static_cast<unsigned>(units)), block(kThreads);
   const bool dual = a.nk[1] > 0;
+  if constexpr (!B_KC) {
+    if (a.alpha != nullptr) {  // f16 operands (gemm_half: one product, 32-bit offsets)
+      const dim3 pblock(kPpThreads);
+      constexpr bool H = true;
+      if constexpr (A_KC) {
+        if (short_m) {
+          if (out_f32)
+            gemm_pp_kernel<A_KC, B_KC, true, false, false, false, false, true, false, H><<<grid, pblock, 0, st>>>(a);
+          else
+            gemm_pp_kernel<A_KC, B_KC, false, false, false, false, false, true, false, H><<<grid, pblock, 0, st>>>(a);
+          return;
+        }
+      }
+      if (a.ksplit > 1)
+        gemm_pp_kernel<A_KC, B_KC, true, false, true, false, false, false, false, H><<<grid, pblock, 0, st>>>(a);
+      else if (out_f32)
+        gemm_pp_kernel<A_KC, B_KC, true, false, false, false, false, false, false, H><<<grid, pblock, 0, st>>>(a);
+      else
+        gemm_pp_kernel<A_KC, B_KC, false, false, false, false, false, false, false, H><<<grid, pblock, 0, st>>>(a);
+      return;
+    }
+  }
   if constexpr (A_KC) {
     if (a.pp && short_m) {  // 128 x 256 tiles, whole or with the two-part fix-up (no split)
       const dim3 pblock(kPpThreads);
@@ -1983,13 +2034,16 @@ struct MidPlan {
   double us = 0;               // predicted time
 };
 
-template <bool A_KC, bool B_KC, bool OUT_F32>
+template <bool A_KC, bool B_KC, bool OUT_F32, bool HALF = false>
 void launch_mid_tile(const GemmArgs& a, const MidPlan& p, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.ksplit)), block(kMidThreads);
-  if (p.bm == 64 && p.bn == 64) gemm_mid_kernel<A_KC, B_KC, OUT_F32, 64, 64, 4><<<grid, block, 0, st>>>(a);
-  else if (p.bm == 64) gemm_mid_kernel<A_KC, B_KC, OUT_F32, 64, 128, 3><<<grid, block, 0, st>>>(a);
-  else if (p.bn == 64) gemm_mid_kernel<A_KC, B_KC, OUT_F32, 128, 64, 3><<<grid, block, 0, st>>>(a);
-  else gemm_mid_kernel<A_KC, B_KC, OUT_F32, 128, 128, 2><<<grid, block, 0, st>>>(a);
+  if constexpr (!B_KC && !HALF) {
+    if (a.alpha != nullptr) return launch_mid_tile<A_KC, B_KC, OUT_F32, true>(a, p, st);  // f16 operands
+  }
+  if (p.bm == 64 && p.bn == 64) gemm_mid_kernel<A_KC, B_KC, OUT_F32, 64, 64, 4, HALF><<<grid, block, 0, st>>>(a);
+  else if (p.bm == 64) gemm_mid_kernel<A_KC, B_KC, OUT_F32, 64, 128, 3, HALF><<<grid, block, 0, st>>>(a);
+  else if (p.bn == 64) gemm_mid_kernel<A_KC, B_KC, OUT_F32, 128, 64, 3, HALF><<<grid, block, 0, st>>>(a);
+  else gemm_mid_kernel<A_KC, B_KC, OUT_F32, 128, 128, 2, HALF><<<grid, block, 0, st>>>(a);
 }
 
 void launch_mid(const GemmArgs& a, const MidPlan& p, bool a_kc, bool b_kc, bool out_f32, hipStream_t st) {
@@ -2062,7 +2116,7 @@ struct SplitPlan {
   int64_t bytes = 0;
 };
 
-// step > 1: only multiples of it (see gemm_long_k).
+// step > 1: only multiples of it (see gemm_half).
 SplitPlan plan_split(int64_t M, int64_t N, int nk, int step = 1) {
   SplitPlan p;
   p.kper = nk;
@@ -2111,7 +2165,7 @@ SplitPlan plan_split(int64_t M, int64_t N, int nk, int step = 1) {
 // mean.  The costs above are up to half high where K is long (1280 x 2605 x
 // 6200: 70 against 54 us) and a third low for the shortest.
 //
-// step > 1: K splits in multiples of it alone (see gemm_long_k).
+// step > 1: K splits in multiples of it alone (see gemm_half).
 MidPlan plan_mid(int64_t M, int64_t N, int nk, int64_t n2, int64_t ws_bytes, int step = 1) {
   struct Tile {
     int bm, bn;
@@ -2598,12 +2652,12 @@ extern "C" int moc_gemm(int dtype, int64_t M, int64_t N, int64_t K, const void* 
 namespace {
 
 // moc_gemm_ws with an optional bf16 residual R added to a bf16 C (res may be
-// null): C = bf16(bf16(A B (+ A2 B2)) + R).
+// null): C = bf16(bf16(A B (+ A2 B2)) + R).  step, alpha: see moc::gemm_half.
 int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int64_t a_sm, int64_t a_sk,
                  const void* B, int64_t b_sk, int64_t b_sn, int64_t K2, const void* A2, int64_t a2_sm,
                  int64_t a2_sk, const void* B2, int64_t b2_sk, int64_t b2_sn, void* C, int64_t ldc, int c_dtype,
                  void* workspace, int64_t workspace_bytes, void* stream, const void* res, int64_t ldres,
-                 int step = 1) {
+                 int step = 1, const float* alpha = nullptr) {
   MOC_REQUIRE(dtype == MOC_BF16 || dtype == MOC_F32, "moc_gemm: dtype must be bf16 or f32");
   MOC_REQUIRE(res == nullptr || (dtype == MOC_BF16 && c_dtype == MOC_BF16 && aligned16(res) && ldres % 8 == 0 &&
                                  ldres >= N),
@@ -2740,6 +2794,8 @@ int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int6
     return static_cast<int64_t>(o.bytes) + 512 * o.ld + 4096 < (1LL << 32) && 512 * o.ld < (1LL << 31);
   };
   a.pp = no_wrap(a.a[0]) && no_wrap(a.b[0]) && no_wrap(a.a[1]) && no_wrap(a.b[1]);
+  a.alpha = alpha;
+  MOC_REQUIRE(alpha == nullptr || (a.pp && lb == 0 && !second), "moc_gemm: f16 operands need 32-bit offsets");
   // small tiles (a K split only with a workspace for its partials)
   const int nk_all = a.nk[0] + a.nk[1];
   const int64_t ws_have = workspace != nullptr && aligned16(workspace) ? workspace_bytes : 0;
@@ -2764,10 +2820,10 @@ int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int6
     const float* parts = static_cast<const float*>(run.C);
     if (of)
       splitk_reduce_kernel<true><<<grid, 256, 0, st>>>(parts, run.ws_stride, mp.ksplit, (int)M, (int)N, mp.ldw, C, ldc,
-                                                       a.vec_store);
+                                                       a.vec_store, nullptr, 0, alpha);
     else
       splitk_reduce_kernel<false><<<grid, 256, 0, st>>>(parts, run.ws_stride, mp.ksplit, (int)M, (int)N, mp.ldw, C,
-                                                        ldc, a.vec_store, a.res, a.ldres);
+                                                        ldc, a.vec_store, a.res, a.ldres, alpha);
     return check_launch("splitk_reduce_kernel");
   }
   const bool short_whole = a.pp && la == 1 && short_whole_ok(M, N, a.nk[0] + a.nk[1]);
@@ -2817,10 +2873,10 @@ int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int6
     const float* parts = static_cast<const float*>(run.C);
     if (of)
       splitk_reduce_kernel<true><<<grid, 256, 0, st>>>(parts, run.ws_stride, sp.ksplit, (int)M, (int)N, sp.ldw,
-                                                       C, ldc, a.vec_store);
+                                                       C, ldc, a.vec_store, nullptr, 0, alpha);
     else
       splitk_reduce_kernel<false><<<grid, 256, 0, st>>>(parts, run.ws_stride, sp.ksplit, (int)M, (int)N, sp.ldw,
-                                                        C, ldc, a.vec_store, a.res, a.ldres);
+                                                        C, ldc, a.vec_store, a.res, a.ldres, alpha);
     return check_launch("splitk_reduce_kernel");
   }
 }
@@ -2838,21 +2894,24 @@ extern "C" int moc_gemm_ws(int dtype, int64_t M, int64_t N, int64_t K, const voi
 
 namespace moc {
 
-// C [M, N] = A B, A [M, K] rows of lda, B [K, N] rows of ldb, bf16, K long (a
-// gradient of hidden rows: K is the vocabulary).  As moc_gemm_ws, but K is split in
-// multiples of 8 ways alone: workgroup ids go to the XCDs in turn, so a K range then
-// stays in one XCD's L2, where 9 ways have every XCD read every range (777 x 512 x
-// 32000: TIMES).
-int64_t gemm_long_k_workspace(int64_t M, int64_t N, int64_t K) {
+// C [M, N] = *alpha A B, A (a_sm, a_sk: one of them 1) and B [K, N] (rows of ldb)
+// in f16, C in bf16 or f32: the gradients of a product whose own gradient needs more
+// than bf16's 8 bits.  As moc_gemm_ws with the f16 MFMA (the same rate), but K is
+// split in multiples of 8 ways alone: workgroup ids go to the XCDs in turn, so a K
+// range then stays in one XCD's L2, where 9 ways have every XCD read every range
+// (777 x 512 x 32000, bf16: 76 us in 9 parts, 36 in 8).
+int64_t gemm_half_workspace(int64_t M, int64_t N, int64_t K) {
   const int nk = static_cast<int>((K + kBK - 1) / kBK);
   return std::max({plan_split(M, N, nk, 8).bytes, plan_fix(M, N, nk).bytes, plan_fix_short(M, N, nk).bytes,
                    plan_mid(M, N, nk, 0, INT64_MAX, 8).bytes});
 }
 
-int gemm_long_k(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
-                int64_t ldc, int c_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
-  return gemm_ws_impl(MOC_BF16, M, N, K, A, lda, 1, B, ldb, 1, 0, nullptr, 0, 0, nullptr, 0, 0, C, ldc, c_dtype,
-                      workspace, workspace_bytes, stream, nullptr, 0, 8);
+int gemm_half(int64_t M, int64_t N, int64_t K, const void* A, int64_t a_sm, int64_t a_sk, const void* B, int64_t ldb,
+              void* C, int64_t ldc, int c_dtype, const float* alpha, void* workspace, int64_t workspace_bytes,
+              void* stream) {
+  MOC_REQUIRE(alpha != nullptr, "gemm_half: null alpha");
+  return gemm_ws_impl(MOC_BF16, M, N, K, A, a_sm, a_sk, B, ldb, 1, 0, nullptr, 0, 0, nullptr, 0, 0, C, ldc, c_dtype,
+                      workspace, workspace_bytes, stream, nullptr, 0, 8, alpha);
 }
 
 }  // namespace moc

@@ -28,6 +28,8 @@ constexpr int32_t kUnknown = -2;         // a label outside the vocabulary
 struct Targets {
   double* total;    // sum of the weights (1 for a sum of losses)
   float* factor;    // upstream gradient / total
+  float* largest;   // a power of two, no weight above it; 0: no row counts
+  float* alpha;     // [2] what the f16 products for dhidden and dweight are times
   float* weight;    // [rows], 0: the row counts for nothing
   float* entropy;   // [rows] sum of q ln q (teacher only)
   int32_t* ids;     // [rows][words] ascending, kNoWord behind the last
@@ -55,6 +57,8 @@ int64_t targets_layout(int64_t rows, int64_t words, int64_t vocab, char* base, T
   if (t != nullptr) {
     t->total = reinterpret_cast<double*>(base);
     t->factor = reinterpret_cast<float*>(base + 8);
+    t->largest = reinterpret_cast<float*>(base + 12);
+    t->alpha = reinterpret_cast<float*>(base + 16);
     t->weight = reinterpret_cast<float*>(weight);
     t->ids = reinterpret_cast<int32_t*>(ids);
     t->entropy = reinterpret_cast<float*>(entropy);
@@ -100,29 +104,41 @@ __device__ __forceinline__ float label_weight(int64_t label, int64_t ignore, con
   return label == ignore ? 0.f : row_weight != nullptr ? row_weight[r] : 1.f;
 }
 
-__device__ __forceinline__ void put_total(const Targets& t, double s, int mean, const float* grad) {
+// The least power of two, a normal number, that x >= 0 is not above.
+__device__ __forceinline__ float power_above(float x) {
+  const uint32_t up = (__float_as_uint(x) + 0x7FFFFFu) >> 23;
+  return __uint_as_float((up < 1 ? 1u : up > 254 ? 254u : up) << 23);
+}
+
+__device__ __forceinline__ void put_total(const Targets& t, double s, float most, int mean, const float* grad) {
   if (!mean) s = 1.0;
   *t.total = s;
   *t.factor = static_cast<float>((grad != nullptr ? static_cast<double>(*grad) : 1.0) / s);
+  *t.largest = most > 0.f ? power_above(most) : 0.f;
 }
 
 // Workgroup 0 sums the weights beside the others, which write the rows' targets.
-__global__ __launch_bounds__(256) void label_targets_kernel(const int64_t* __restrict__ labels, int64_t rows,
+__global__ __launch_bounds__(1024) void label_targets_kernel(const int64_t* __restrict__ labels, int64_t rows,
                                                             int64_t vocab, int64_t ignore,
                                                             const float* __restrict__ row_weight, int mean,
                                                             const float* __restrict__ grad, Targets t) {
   if (blockIdx.x == 0) {
-    __shared__ double red[4];
+    __shared__ double red[16];
+    __shared__ float most[16];
     double s = 0;
-    if (mean) {
+    float m = 0.f;
 #pragma unroll 8
-      for (int64_t r = threadIdx.x; r < rows; r += 256) s += label_weight(labels[r], ignore, row_weight, r);
+    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+      const float w = label_weight(labels[r], ignore, row_weight, r);
+      s += w;
+      m = fmaxf(m, fabsf(w));
     }
     s = block_sum64(s, red);
-    if (threadIdx.x == 0) put_total(t, s, mean, grad);
+    m = block_reduce<true>(m, most);
+    if (threadIdx.x == 0) put_total(t, s, m, mean, grad);
     return;
   }
-  const int64_t r = (static_cast<int64_t>(blockIdx.x) - 1) * 256 + threadIdx.x;
+  const int64_t r = (static_cast<int64_t>(blockIdx.x) - 1) * 1024 + threadIdx.x;
   if (r >= rows) return;
   const int64_t label = labels[r];
   t.weight[r] = label_weight(label, ignore, row_weight, r);
@@ -296,13 +312,17 @@ __global__ __launch_bounds__(1024) void words_left_kernel(const int32_t* __restr
 __global__ __launch_bounds__(1024) void target_total_kernel(int64_t rows, int mean, const float* __restrict__ grad,
                                                             Targets t) {
   __shared__ double red[16];
+  __shared__ float most[16];
   double s = 0;
-  if (mean) {
+  float m = 0.f;
 #pragma unroll 8
-    for (int64_t r = threadIdx.x; r < rows; r += 1024) s += t.weight[r];
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    s += t.weight[r];
+    m = fmaxf(m, fabsf(t.weight[r]));
   }
   s = block_sum64(s, red);
-  if (threadIdx.x == 0) put_total(t, s, mean, grad);
+  m = block_reduce<true>(m, most);
+  if (threadIdx.x == 0) put_total(t, s, m, mean, grad);
 }
 
 // loss = sum of the rows' weighted losses / total.  One workgroup.
@@ -326,6 +346,9 @@ template <> struct Elem<uint16_t> {
   }
   static __device__ __forceinline__ float one(uint16_t x) { return bf16_to_f32(x); }
   static __device__ __forceinline__ uint16_t of(float f) { return bf16_rne(f); }
+};
+template <> struct Elem<_Float16> {
+  static __device__ __forceinline__ float one(_Float16 x) { return static_cast<float>(x); }
 };
 template <> struct Elem<float> {
   static constexpr int kPer = 4;
@@ -676,8 +699,12 @@ __global__ __launch_bounds__(256) void slabs_loss_kernel(const float2* __restric
   if (threadIdx.x == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
 }
 
-// One workgroup a row: its loss, and its f16 exponentials into bf16 gradients of
-// the logits, in place: e exp2(m - lse) of a slab's reference m is p.
+// One workgroup a row: its loss, and its f16 exponentials into gradients of the
+// logits, in place: e exp2(m - lse) of a slab's reference m is p.  The gradients stay
+// in f16, as (w / largest) 2^14 (p - q): a bf16 rounding of them, 2^-8 of each, would
+// add to the products' sums, where the words' parts cancel, more than the sums' own
+// rounding (measured: up to 1.9 times the error of f32 ones); 2^-11 does not show.
+// Down to 2^-28 of the largest they have all 11 bits, below 2^-39 they are 0.
 __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld, int vocab,
                                                          const float2* __restrict__ stat, int slabs, Targets t,
                                                          int words, float heat, const float* __restrict__ z,
@@ -698,7 +725,7 @@ __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld
   const float lse = slabs_lse(st, slabs, red);
   const float cross = block_reduce<false>(cross_of(t, r, words, z, kLog2E / heat, lse, at_word, tid, 256), red);
   if (tid == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
-  const float c = cross == cross ? heat * w * *t.factor : NAN;
+  const float c = cross == cross ? w / *t.largest * 0x1p14f : NAN;
   constexpr int kAhead = 4;
   for (int c0 = tid; c0 < chunks; c0 += 256 * kAhead) {
     uint4 v[kAhead];
@@ -722,7 +749,7 @@ __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld
         out[q] = __builtin_bit_cast(uint32_t,
                                     __builtin_convertvector((cvt_f32x2_t){static_cast<float>(h.x) * f,
                                                                           static_cast<float>(h.y) * f},
-                                                            cvt_bf16x2_t));
+                                                            f16x2_t));
       }
       row[at] = make_uint4(out[0], out[1], out[2], out[3]);
     }
@@ -734,34 +761,140 @@ __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld
     const int32_t id = t.ids[r * n + k];
     const float share = words > 0 ? t.share[r * n + k] : 1.f;
     if (id < 0 || id == kNoWord || share == -1.f) continue;
-    e[r * ld + id] = bf16_rne(c * (__builtin_amdgcn_exp2f(at_word[k]) - share));
+    e[r * ld + id] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(c * (__builtin_amdgcn_exp2f(at_word[k]) - share)));
   }
 }
 
-// Rows that count, zeros for the others: what is in those reaches no product.
+// Rows that count, zeros for the others: what is in those reaches no product (f32).
 // Rows of 16-byte chunks, whose last one is cut off at the hidden size.
-template <typename T>
-__global__ __launch_bounds__(256) void counted_rows_kernel(const T* __restrict__ h, int64_t ldh, int64_t rows,
+__global__ __launch_bounds__(256) void counted_rows_kernel(const float* __restrict__ h, int64_t ldh, int64_t rows,
                                                            int hidden, const float* __restrict__ weight,
-                                                           T* __restrict__ out, int64_t ldo) {
-  constexpr int kPer = Elem<T>::kPer;
-  const int chunks = (hidden + kPer - 1) / kPer;
+                                                           float* __restrict__ out, int64_t ldo) {
+  const int chunks = (hidden + 3) / 4;
   const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows * chunks; i += step) {
     const int64_t r = i / chunks;
-    const int k = static_cast<int>(i - r * chunks) * kPer;
-    T part[kPer] = {};
+    const int k = static_cast<int>(i - r * chunks) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (weight[r] != 0.f) {
-      if (k + kPer <= hidden) {
-        *reinterpret_cast<uint4*>(out + r * ldo + k) = *reinterpret_cast<const uint4*>(h + r * ldh + k);
-        continue;
-      }
-      for (int e = 0; k + e < hidden; ++e) part[e] = h[r * ldh + k + e];
+      v = *reinterpret_cast<const float4*>(h + r * ldh + k);
+      if (k + 1 >= hidden) v.y = 0.f;
+      if (k + 2 >= hidden) v.z = 0.f;
+      if (k + 3 >= hidden) v.w = 0.f;
     }
-    uint4 v;
-    __builtin_memcpy(&v, part, 16);
-    *reinterpret_cast<uint4*>(out + r * ldo + k) = v;
+    *reinterpret_cast<float4*>(out + r * ldo + k) = v;
   }
+}
+
+// ------------------------------------------------------- operands in f16
+// Hidden rows and weight for the products with f16 gradients: bf16 values times a
+// power of two, which f16 holds as they are from 2^-17 up and rounds by at most 2^-25
+// below; rows that do not count become 0.  The power is a guess that suits what
+// networks hold (the largest of the hidden rows in [2^-3, 2^13], of the weight in
+// [2^-7, 2^9]: what is rounded is off by 2^-24 of the largest at most); the largest
+// value is found on the way, and halves_again_kernel redoes a tensor that it does not
+// suit.
+struct Halves {
+  const uint16_t* from;
+  int64_t ld, rows;
+  _Float16* to;  // null: not wanted
+  float guess, least, most;
+};
+
+__device__ __forceinline__ float halves_scale(const Halves& h, uint32_t range) {
+  const float x = __uint_as_float(range);
+  if (range == 0 || !(x < INFINITY) || (x >= h.least && x <= h.most)) return h.guess;
+  const int e = static_cast<int>((__float_as_uint(power_above(x)) >> 23)) - 127;  // x <= 2^e
+  return ldexpf(1.f, 15 - e < 126 ? 15 - e : 126);
+}
+
+// Rows of h by hidden columns into rows of ldo (a multiple of 64, zeros behind the
+// hidden size), a wave a row, four rows' loads in flight; the bits of the largest
+// |value| this lane met.
+__device__ __forceinline__ uint32_t halve_rows(const Halves& h, int hidden, int64_t ldo, const float* weight,
+                                               float scale) {
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+  constexpr int kRows = 4;
+  const int lane = threadIdx.x & 63, chunks = static_cast<int>(ldo / 8);
+  const int64_t waves = static_cast<int64_t>(gridDim.x) * 4;
+  uint32_t most = 0;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r0 < h.rows; r0 += waves * kRows) {
+    for (int c = lane; c < chunks; c += 64) {
+      const int k = 8 * c;
+      uint4 v[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int64_t r = r0 + waves * i;
+        v[i] = k < hidden && r < h.rows && (weight == nullptr || weight[r] != 0.f)
+                   ? *reinterpret_cast<const uint4*>(h.from + r * h.ld + k)
+                   : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int64_t r = r0 + waves * i;
+        if (r >= h.rows) break;
+        const uint32_t in[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          // what a chunk holds behind the hidden size is another tensor's or padding
+          const uint32_t w = in[q] & (k + 2 * q + 1 < hidden ? 0xFFFFFFFFu : k + 2 * q < hidden ? 0xFFFFu : 0u);
+          most = max(most, max(w << 16 & 0x7FFF0000u, w & 0x7FFF0000u));
+          o[q] = __builtin_bit_cast(uint32_t,
+                                    __builtin_convertvector((cvt_f32x2_t){__uint_as_float(w << 16) * scale,
+                                                                          __uint_as_float(w & 0xFFFF0000u) * scale},
+                                                            f16x2_t));
+        }
+        *reinterpret_cast<uint4*>(h.to + r * ldo + k) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+  }
+  return most;
+}
+
+__device__ __forceinline__ uint32_t block_max_bits(uint32_t m, uint32_t* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o)));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return max(max(red[0], red[1]), max(red[2], red[3]));
+}
+
+// most [2][gridDim]: the workgroups' largest values (one word for all of them would
+// have thousands of atomics in a row: 30 us).
+__global__ __launch_bounds__(256) void halves_kernel(Halves hidden_rows, Halves weight_rows, int hidden, int64_t ldo,
+                                                     Targets t, uint32_t* __restrict__ most) {
+  __shared__ uint32_t red[4];
+  uint32_t m = hidden_rows.to != nullptr ? halve_rows(hidden_rows, hidden, ldo, t.weight, hidden_rows.guess) : 0;
+  m = block_max_bits(m, red);
+  if (threadIdx.x == 0) most[blockIdx.x] = m;
+  m = weight_rows.to != nullptr ? halve_rows(weight_rows, hidden, ldo, nullptr, weight_rows.guess) : 0;
+  m = block_max_bits(m, red);
+  if (threadIdx.x == 0) most[gridDim.x + blockIdx.x] = m;
+}
+
+// Redoes a tensor whose largest value the guess did not suit; the products' factors.
+__global__ __launch_bounds__(256) void halves_again_kernel(Halves hidden_rows, Halves weight_rows, int hidden,
+                                                           int64_t ldo, float heat, Targets t,
+                                                           const uint32_t* __restrict__ most, int parts) {
+  __shared__ uint32_t red[4];
+  uint32_t m[2] = {0, 0};
+#pragma unroll 8
+  for (int i = threadIdx.x; i < parts; i += 256) {
+    m[0] = max(m[0], most[i]);
+    m[1] = max(m[1], most[parts + i]);
+  }
+  const float sx = halves_scale(hidden_rows, block_max_bits(m[0], red));
+  const float sw = halves_scale(weight_rows, block_max_bits(m[1], red));
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    // no row counts: gradients of 0, whatever the divisor
+    const float f = *t.largest > 0.f ? heat * *t.factor * *t.largest * 0x1p-14f : 0.f;
+    t.alpha[0] = f / sw;
+    t.alpha[1] = f / sx;
+  }
+  if (hidden_rows.to != nullptr && sx != hidden_rows.guess) halve_rows(hidden_rows, hidden, ldo, t.weight, sx);
+  if (weight_rows.to != nullptr && sw != weight_rows.guess) halve_rows(weight_rows, hidden, ldo, nullptr, sw);
 }
 
 // a += b over n values; out (may be null): the sum as bf16 or f32.
@@ -775,14 +908,15 @@ __global__ __launch_bounds__(256) void add_f32_kernel(float* a, const float* __r
   }
 }
 
-// out[i][j] = a_i b_j, the product over one row or one word (the engine takes no
+// out[i][j] = *alpha a_i b_j (alpha null: 1), the product over one row or one word (the engine takes no
 // operand of one element's pitch).  Columns blockIdx.x, rows blockIdx.y and on.
 template <typename T, typename OUT>
 __global__ __launch_bounds__(256) void outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b,
-                                                    int64_t m, int64_t n, OUT* __restrict__ out) {
+                                                    int64_t m, int64_t n, const float* __restrict__ alpha,
+                                                    OUT* __restrict__ out) {
   const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (j >= n) return;
-  const float bj = Elem<T>::one(b[j]);
+  const float bj = Elem<T>::one(b[j]) * (alpha != nullptr ? *alpha : 1.f);
   for (int64_t i = blockIdx.y; i < m; i += gridDim.y) out[i * n + j] = Elem<OUT>::of(Elem<T>::one(a[i * lda]) * bj);
 }
 
@@ -812,9 +946,11 @@ __global__ __launch_bounds__(256) void scale_kernel(int f32_0, void* p0, int64_t
   else scale_values(static_cast<uint16_t*>(p1), n1, f);
 }
 
+constexpr int kMostBlocks = 2048;  // of a grid that strides over its work
+
 unsigned blocks_of(int64_t n) {
   const int64_t b = (n + 255) / 256;
-  return static_cast<unsigned>(b < 1 ? 1 : b > 2048 ? 2048 : b);
+  return static_cast<unsigned>(b < 1 ? 1 : b > kMostBlocks ? kMostBlocks : b);
 }
 
 // ------------------------------------------------------------------- pieces
@@ -826,7 +962,7 @@ struct Pieces {
   int64_t rows, count;     // rows of a piece, pieces
   int64_t ldz;             // row pitch of a piece's logits
   int64_t slabs;
-  int64_t z, d, x, acc, part, stat, at_words, bytes;  // offsets in the workspace
+  int64_t z, d, x, w, acc, part, stat, at_words, most, bytes;  // offsets in the workspace
   int64_t ldx;
 };
 
@@ -859,6 +995,8 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   }
   p.ldx = (hidden + 63) & ~63LL;
   p.x = grads ? take(rows * p.ldx * (f32 ? 4 : 2)) : 0;
+  p.w = grads && !f32 ? take(vocab * p.ldx * 2) : 0;
+  p.most = grads && !f32 ? take(2 * 4 * kMostBlocks) : 0;
   if (grads && p.count > 1) {
     p.acc = take(vocab * hidden * 4);
     p.part = take(vocab * hidden * 4);
@@ -898,25 +1036,25 @@ int logits_rows(bool f32, const void* x, int64_t rows, int64_t vocab, int64_t ld
   return check_launch("logits_loss_kernel");
 }
 
-// C [M, N] = A B over K = 1, as moc_gemm_ws of these strides would.
-int outer(int dtype, int64_t m, int64_t n, const void* a, int64_t lda, const void* b, void* c, int c_dtype,
-          hipStream_t st) {
+// C [M, N] = *alpha A B over K = 1, as moc_gemm_ws or gemm_half of these strides would.
+int outer(bool f32, int64_t m, int64_t n, const void* a, int64_t lda, const void* b, const float* alpha, void* c,
+          int c_dtype, hipStream_t st) {
+  typedef _Float16 H;
   const dim3 grid(static_cast<unsigned>((n + 255) / 256), static_cast<unsigned>(m < 8192 ? m : 8192));
-  if (dtype == MOC_F32)
+  if (f32)
     outer_kernel<float, float><<<grid, 256, 0, st>>>(static_cast<const float*>(a), lda, static_cast<const float*>(b), m,
-                                                     n, static_cast<float*>(c));
+                                                     n, nullptr, static_cast<float*>(c));
   else if (c_dtype == MOC_F32)
-    outer_kernel<uint16_t, float><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(a), lda,
-                                                        static_cast<const uint16_t*>(b), m, n, static_cast<float*>(c));
+    outer_kernel<H, float><<<grid, 256, 0, st>>>(static_cast<const H*>(a), lda, static_cast<const H*>(b), m, n, alpha,
+                                                 static_cast<float*>(c));
   else
-    outer_kernel<uint16_t, uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(a), lda,
-                                                           static_cast<const uint16_t*>(b), m, n,
-                                                           static_cast<uint16_t*>(c));
+    outer_kernel<H, uint16_t><<<grid, 256, 0, st>>>(static_cast<const H*>(a), lda, static_cast<const H*>(b), m, n, alpha,
+                                                    static_cast<uint16_t*>(c));
   return check_launch("outer_kernel");
 }
 
 bool sizes_ok(int64_t rows, int64_t vocab, int64_t words) {
-  return rows >= 0 && rows <= (1LL << 24) && vocab >= 1 && vocab <= (1LL << 24) && words >= 0 && words <= kMaxWords;
+  return rows >= 0 && rows <= (1LL << 24) && vocab >= 1 && vocab <= (1LL << 21) && words >= 0 && words <= kMaxWords;
 }
 
 }  // namespace
@@ -925,7 +1063,7 @@ bool sizes_ok(int64_t rows, int64_t vocab, int64_t words) {
 using namespace moc;
 
 #define MOC_SIZES(name)                                                                                          \
-  MOC_REQUIRE(sizes_ok(rows, vocab, words), "%s: up to 2^24 rows, a vocabulary of up to 2^24 words, up to %d of " \
+  MOC_REQUIRE(sizes_ok(rows, vocab, words), "%s: up to 2^24 rows, a vocabulary of up to 2^21 words, up to %d of " \
                                             "them a row", name, kMaxWords)
 
 extern "C" int64_t moc_loss_targets_size(int64_t rows, int64_t words, int64_t vocab) {
@@ -942,8 +1080,8 @@ extern "C" int moc_label_targets(const int64_t* labels, int64_t rows, int64_t vo
   hipStream_t st = as_stream(stream);
   Targets t;
   targets_layout(rows, 0, vocab, static_cast<char*>(targets), &t);
-  label_targets_kernel<<<static_cast<unsigned>(1 + (rows + 255) / 256), 256, 0, st>>>(labels, rows, vocab, ignore_index,
-                                                                                      row_weight, mean, grad, t);
+  label_targets_kernel<<<static_cast<unsigned>(1 + (rows + 1023) / 1024), 1024, 0, st>>>(
+      labels, rows, vocab, ignore_index, row_weight, mean, grad, t);
   return check_launch("label_targets_kernel");
 }
 
@@ -1016,9 +1154,9 @@ extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, 
     int64_t b = p.fused ? 0 : moc_gemm_workspace_size(dtype, n, vocab, hidden, 0);
     if (b > most) most = b;
     if (!grads) continue;
-    b = p.fused ? gemm_long_k_workspace(n, hidden, vocab) : moc_gemm_workspace_size(dtype, n, hidden, vocab, 0);
+    b = p.fused ? gemm_half_workspace(n, hidden, vocab) : moc_gemm_workspace_size(dtype, n, hidden, vocab, 0);
     if (b > most) most = b;
-    b = moc_gemm_workspace_size(dtype, vocab, hidden, n, 0);
+    b = p.fused ? gemm_half_workspace(vocab, hidden, n) : moc_gemm_workspace_size(dtype, vocab, hidden, n, 0);
     if (b > most) most = b;
   }
   return most;
@@ -1055,15 +1193,22 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
   char* ws = static_cast<char*>(workspace);
   const int64_t n_words = words > 0 ? words : 1;
   int rc;
-  if (grads && rows > 0) {
-    const unsigned grid = blocks_of(rows * ((hidden * es + 15) / 16));
-    if (f32)
-      counted_rows_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(h), ldh, rows, (int)hidden, t.weight,
-                                                       reinterpret_cast<float*>(ws + p.x), p.ldx);
-    else
-      counted_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(h), ldh, rows, (int)hidden,
-                                                          t.weight, reinterpret_cast<uint16_t*>(ws + p.x), p.ldx);
+  if (grads && rows > 0 && f32) {
+    counted_rows_kernel<<<blocks_of(rows * ((hidden + 3) / 4)), 256, 0, st>>>(
+        static_cast<const float*>(h), ldh, rows, (int)hidden, t.weight, reinterpret_cast<float*>(ws + p.x), p.ldx);
     if ((rc = check_launch("counted_rows_kernel")) != MOC_OK) return rc;
+  } else if (grads && rows > 0) {
+    const Halves hx{static_cast<const uint16_t*>(h), ldh, rows,
+                    dw != nullptr ? reinterpret_cast<_Float16*>(ws + p.x) : nullptr, 0x1p2f, 0x1p-3f, 0x1p13f};
+    const Halves hw{static_cast<const uint16_t*>(w), ldw, vocab,
+                    dh != nullptr ? reinterpret_cast<_Float16*>(ws + p.w) : nullptr, 0x1p6f, 0x1p-7f, 0x1p9f};
+    const unsigned grid = blocks_of((rows > vocab ? rows : vocab) * 16);  // four waves of four rows
+    uint32_t* most = reinterpret_cast<uint32_t*>(ws + p.most);
+    halves_kernel<<<grid, 256, 0, st>>>(hx, hw, (int)hidden, p.ldx, t, most);
+    if ((rc = check_launch("halves_kernel")) != MOC_OK) return rc;
+    halves_again_kernel<<<grid < 512 ? grid : 512, 256, 0, st>>>(hx, hw, (int)hidden, p.ldx, temperature, t, most,
+                                                                 (int)grid);
+    if ((rc = check_launch("halves_again_kernel")) != MOC_OK) return rc;
   }
   if (p.fused && words > 0 && rows > 0) {
     words_left_kernel<<<static_cast<unsigned>((rows + 63) / 64), 1024,
@@ -1071,8 +1216,11 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
                                                                              t.first);
     if ((rc = check_launch("words_left_kernel")) != MOC_OK) return rc;
   }
-  const char* x = grads ? ws + p.x : static_cast<const char*>(h);
-  const int64_t ldx = grads ? p.ldx : ldh;
+  // f32: the rows that count in every product; bf16: in dweight's alone, as nothing is
+  // read of the others' logits
+  const bool copied = grads && f32;
+  const char* x = copied ? ws + p.x : static_cast<const char*>(h);
+  const int64_t ldx = copied ? p.ldx : ldh;
   for (int64_t i = 0; i < p.count; ++i) {
     const int64_t r0 = i * p.rows, n = rows - r0 < p.rows ? rows - r0 : p.rows;
     const char* xi = x + r0 * ldx * es;
@@ -1111,10 +1259,11 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     if (rc != MOC_OK) return rc;
     if (dh != nullptr) {
       char* to = static_cast<char*>(dh) + r0 * hidden * (dh_dtype == MOC_F32 ? 4 : 2);
-      rc = vocab == 1 ? outer(dtype, n, hidden, ws + p.d, p.ldz, w, to, dh_dtype, st)
-           : p.fused  ? gemm_long_k(n, hidden, vocab, ws + p.d, p.ldz, w, ldw, to, hidden, dh_dtype, gemm_ws,
-                                    gemm_ws_bytes, stream)
-                      : moc_gemm_ws(dtype, n, hidden, vocab, ws + p.d, p.ldz, 1, w, ldw, 1, 0, nullptr, 0, 0, nullptr, 0,
+      const char* b = p.fused ? ws + p.w : static_cast<const char*>(w);
+      rc = vocab == 1 ? outer(f32, n, hidden, ws + p.d, p.ldz, b, t.alpha, to, dh_dtype, st)
+           : p.fused  ? gemm_half(n, hidden, vocab, ws + p.d, p.ldz, 1, b, p.ldx, to, hidden, dh_dtype, t.alpha, gemm_ws,
+                                  gemm_ws_bytes, stream)
+                      : moc_gemm_ws(dtype, n, hidden, vocab, ws + p.d, p.ldz, 1, b, ldw, 1, 0, nullptr, 0, 0, nullptr, 0,
                                     0, to, hidden, dh_dtype, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
     }
@@ -1122,9 +1271,12 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       const bool one = p.count == 1;
       char* to = one ? static_cast<char*>(dw) : ws + (i == 0 ? p.acc : p.part);
       const int to_dtype = one ? dw_dtype : MOC_F32;
-      rc = n == 1 ? outer(dtype, vocab, hidden, ws + p.d, 1, xi, to, to_dtype, st)
-                  : moc_gemm_ws(dtype, vocab, hidden, n, ws + p.d, 1, p.ldz, xi, ldx, 1, 0, nullptr, 0, 0, nullptr, 0, 0,
-                                to, hidden, to_dtype, gemm_ws, gemm_ws_bytes, stream);
+      const char* b = ws + p.x + r0 * p.ldx * es;
+      rc = n == 1    ? outer(f32, vocab, hidden, ws + p.d, 1, b, t.alpha + 1, to, to_dtype, st)
+           : p.fused ? gemm_half(vocab, hidden, n, ws + p.d, 1, p.ldz, b, p.ldx, to, hidden, to_dtype, t.alpha + 1,
+                                 gemm_ws, gemm_ws_bytes, stream)
+                     : moc_gemm_ws(dtype, vocab, hidden, n, ws + p.d, 1, p.ldz, b, p.ldx, 1, 0, nullptr, 0, 0, nullptr, 0,
+                                   0, to, hidden, to_dtype, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
       if (i > 0) {
         float* acc = reinterpret_cast<float*>(ws + p.acc);

@@ -68,8 +68,8 @@ def distillation_loss(logits, teacher_ids, teacher_logits, row_weight=None, *, t
     """linear_distillation of logits [..., vocab] (bf16 or f32) that are there already."""
     what = "distillation_loss"
     rows = _rows_of(what, logits, None, row_weight, reduction)
-    if logits.shape[-1] < 1:
-        raise ValueError(f"{what}: a vocabulary of one word at least")
+    if not 1 <= logits.shape[-1] <= 1 << 21:
+        raise ValueError(f"{what}: a vocabulary of 1 to 2^21 words, got {logits.shape[-1]}")
     targets = _teacher(what, logits, teacher_ids, teacher_logits, row_weight, rows, temperature, reduction)
     dev = N.one_device(logits, *targets.tensors())
     if not N.is_current(dev):
@@ -222,8 +222,8 @@ def _linear(what: str, hidden, weight, targets) -> torch.Tensor:
         raise ValueError(f"{what}: hidden and weight of one type (or under bf16 autocast), got {hidden.dtype} and "
                          f"{weight.dtype}")
     vocab, d = weight.shape
-    if vocab > 1 << 24 or d > 1 << 20:
-        raise ValueError(f"{what}: a vocabulary of up to 2^24 words, a hidden size of up to 2^20")
+    if vocab > 1 << 21 or d > 1 << 20:
+        raise ValueError(f"{what}: a vocabulary of up to 2^21 words, a hidden size of up to 2^20")
     if product == BF16 and vocab * K.row_pitch(d, BF16) * 2 >= K.OPERAND_BYTES:
         raise ValueError(f"{what}: a bf16 weight of up to 2 GiB")
     dev = N.one_device(hidden, weight, *targets.tensors())

@@ -6,8 +6,9 @@ or with one rounding of 2^-24: with S the largest sum of |h||w|, an error of 4 s
 2^-24 S (roundings of either sign) and 2 more units for an f32 product's own.  A
 row's loss differs by twice that and by f32 exponentials, logarithms and a sum over
 the vocabulary, 2^-20 of its terms.  A gradient is a sum over dlogits, which are
-rounded to bf16 (2^-8 of each; from f16 exponentials, 2^-11 more) or f32 (2^-23 with
-the exponential's own) behind a relative error of the logits' errors, and rounded
+rounded to f16 twice (2^-11 of each; 2^-39 of the row's factor where it is smallest),
+its other operand by 2^-24 of its largest value, or stay f32 (2^-23 with the
+exponential's own), behind a relative error of the logits' errors, and is rounded
 itself; |dlogits| |operand| in 64 bits bounds what that comes to.  p's relative error
 counts for p, not for p - q: with c the row's factor, c p <= |dlogits| + c q.  A
 gradient that was computed ahead and rounded to bf16 is rounded once more by an
@@ -96,9 +97,13 @@ def check(out, want, got, leaves, dz, c, q, z_err, heat, factor, weights):
         if got_ is None:
             continue
         half = got_.dtype == BF
-        rel = (2.0 ** -8 + 2.0 ** -11 if half else 2.0 ** -22) + 4 * z_err / heat
+        rel = (2.01 * 2.0 ** -11 if half else 2.0 ** -22) + 4 * z_err / heat
         terms = dz.shape[1 - i]
         tol = rel * size + (4 * math.sqrt(terms) + 2) * 2.0 ** -24 * size
+        if half:
+            other = (w if i == 0 else h).abs()
+            tol = tol + 2.0 ** -39 * c.max() * other.sum(0) + 2.0 ** -24 * other.max() * (
+                soft.sum(1)[:, None] if i == 0 else soft.sum(0)[:, None])
         if got_.dtype == BF:
             tol = tol * (1 + 2.0 ** -7) + (1 if want.dim() else 2.01) * 2.0 ** -8 * want_.abs() + 1e-38
         err = (got_.to(F64) - want_).abs()
@@ -212,6 +217,30 @@ def test_distillation_loss(rows, vocab, dtype, words, heat, ragged, reduction):
     tol = 8 * rel * (dz.abs() + c * abs(factor) * q) + (2.01 * 2.0 ** -8 if dtype == BF else 2.0 ** -23) * dz.abs() + 1e-38
     err = (got.to(F64) - dz).abs()
     assert (err <= tol).all(), (err / tol).max()
+
+
+@pytest.mark.parametrize("up", [-60, -14, -5, 9, 40])
+@pytest.mark.parametrize("op", ["entropy", "teacher"])
+def test_operands_of_any_size(up, op):
+    """Hidden rows of another size and a weight that makes up for it; row weights of
+    any size."""
+    h, w = operands(70, 200, 900, BF)
+    h[3, 5] = 100.0
+    h, w = (h.float() * 2.0 ** up).to(BF).requires_grad_(), (w.float() * 2.0 ** -up).to(BF).requires_grad_()
+    ids, top = teacher_of(70, 900, 5, True)
+    y = labels_of(70, 900, 0.2)
+    weight = (rand(70, seed=4).abs() + 0.5) * 2.0 ** (up / 2)
+    out = L.linear_cross_entropy(h, w, y, weight, reduction="sum") if op == "entropy" else (
+        L.linear_distillation(h, w, ids, top, weight, reduction="sum"))
+    got = torch.autograd.grad(out, (h, w))
+    hd, wd = h.detach().to(F64), w.detach().to(F64)
+    if op == "entropy":
+        q, some = torch.zeros(70, 900, dtype=F64, device="cuda"), y != -100
+        q[torch.arange(70, device="cuda"), y.clamp(min=0)] = 1
+    else:
+        q, some = shares(ids, top, 900, 1.0)
+    want, dz, c = reference(hd @ wd.t(), q, some, weight.to(F64), 1.0, "sum")
+    check(out.detach(), want, got, (hd, wd), dz, c, q, logit_error(hd, wd), 1.0, 1.0, weight)
 
 
 def test_rows_in_pieces():

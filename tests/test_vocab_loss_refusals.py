@@ -31,9 +31,8 @@ def teacher():
     (dict(row_weight=torch.ones(2, 3, dtype=torch.float64)), "row_weight"),
     (dict(row_weight=torch.ones(6)), "row_weight"),
     (dict(row_weight=torch.ones(2, 3, requires_grad=True)), "no gradient"),
-    (dict(weight=torch.zeros(1, 8).expand(1 << 25, 8)), "2\\^24"),
-    (dict(hidden=torch.zeros(2, 3, 8, dtype=BF), weight=torch.zeros(1, 8, dtype=BF).expand(1 << 24, 8),), None),
-    (dict(hidden=torch.zeros(2, 3, 128, dtype=BF), weight=torch.zeros(1, 128, dtype=BF).expand(1 << 23, 128)), "2 GiB"),
+    (dict(weight=torch.zeros(1, 8).expand((1 << 21) + 1, 8)), "2\\^21"),
+    (dict(hidden=torch.zeros(2, 3, 512, dtype=BF), weight=torch.zeros(1, 512, dtype=BF).expand(1 << 21, 512)), "2 GiB"),
     (dict(), "device tensors"),
 ])
 def test_cross_entropy(change, says):
@@ -73,6 +72,7 @@ def test_entry_points_refuse():
         ("moc_label_targets", (None, 4, 10, -100, None, 1, None, p, None)),
         ("moc_label_targets", (p, 4, 10, -100, None, 1, None, None, None)),
         ("moc_label_targets", (p, 4, 0, -100, None, 1, None, p, None)),
+        ("moc_label_targets", (p, 4, (1 << 21) + 1, -100, None, 1, None, p, None)),
         ("moc_label_targets", (p, (1 << 24) + 1, 10, -100, None, 1, None, p, None)),
         ("moc_teacher_targets", (p, 1, 4, p, 1, 4, 3, 0, 10, 1.0, None, 1, None, p, None)),
         ("moc_teacher_targets", (p, 1, 4, p, 1, 4, 3, 1025, 10, 1.0, None, 1, None, p, None)),
@@ -90,7 +90,7 @@ def test_entry_points_refuse():
         ("moc_linear_loss", (0, p, 3, 8, 12, p, 10, 8, p, 0, 1.0, p, p, None, 0, None, 0, p, 1 << 40, None, 0, None)),
         ("moc_linear_loss", (1, p, 3, 8, 8, p, 10, 8, p, 0, 1.0, p, p, p, 0, None, 0, p, 1 << 40, None, 0, None)),
         ("moc_linear_loss", (0, p, 3, 0, 8, p, 10, 8, p, 0, 1.0, p, p, None, 0, None, 0, p, 1 << 40, None, 0, None)),
-        ("moc_linear_loss", (0, p, 3, 128, 128, p, 1 << 23, 128, p, 0, 1.0, p, p, None, 0, None, 0, p, 1 << 40, None, 0,
+        ("moc_linear_loss", (0, p, 3, 512, 512, p, 1 << 21, 512, p, 0, 1.0, p, p, None, 0, None, 0, p, 1 << 40, None, 0,
                              None)),
         ("moc_scale_inplace", (5, p, 8, 0, None, 0, p, None)),
         ("moc_scale_inplace", (0, None, 8, 0, None, 0, p, None)),
