@@ -271,34 +271,36 @@ int moc_next_token_loss_backward(const void* logits, int64_t ld, int64_t batch, 
  * and gradients are 0 and n leaves it out (no row left: a mean of NaN).  A label
  * outside the vocabulary gives NaN.  Up to 2^24 rows, 2^21 words, 1024 a row.
  *
- * targets: what the losses read of labels or teacher, written by one of the
- * first two calls (moc_loss_targets_size bytes, 16-byte aligned; words = 0 for
- * labels).  moc_teacher_targets: ids (int32 or int64) and top [rows, words], rows
- * ids_ld and top_ld apart; q = softmax(top / T) over a row's entries; one outside
- * the vocabulary or of -infinity is none, entries of one word add up.
- * row_weight [rows], grad (a scalar, on the device): NULL is 1. */
-int64_t moc_loss_targets_size(int64_t rows, int64_t words, int64_t vocab);
-int moc_label_targets(const int64_t* labels, int64_t rows, int64_t vocab, int64_t ignore_index,
-                      const float* row_weight, int mean, const float* grad, void* targets, void* stream);
-int moc_teacher_targets(const void* ids, int ids_dtype, int64_t ids_ld, const void* top, int top_dtype,
-                        int64_t top_ld, int64_t rows, int64_t words, int64_t vocab, float temperature,
-                        const float* row_weight, int mean, const float* grad, void* targets, void* stream);
-
-/* Of logits [rows, vocab] (rows ld apart): row_loss [rows] = w_r l_r, loss (NULL:
- * none), dlogits = grad dloss / dlogits of the logits' dtype (NULL: none). */
-int moc_logits_loss(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t ld, void* targets,
-                    int64_t words, float temperature, float* row_loss, float* loss, void* dlogits, int64_t ldd,
+ * A teacher: ids (MOC_I32 or MOC_I64) and top (its logits, MOC_BF16 or MOC_F32)
+ * [rows, words], rows ids_ld and top_ld apart; q = softmax(top / T) over a row's
+ * entries; one outside the vocabulary or of -infinity is none, entries of one word add
+ * up.  row_weight [rows], grad (the upstream gradient, a scalar on the device): NULL
+ * is 1.  row_loss [rows] = w_r l_r and loss: NULL where not wanted.  counters:
+ * MOC_GEMM_WS_COUNTER_BYTES of zeros, left zero; the start of a GEMM workspace.
+ *
+ * Of logits [rows, vocab] (rows ld apart): dlogits = grad dloss / dlogits (rows ldd
+ * apart) of the logits' dtype (NULL: none). */
+int64_t moc_logits_loss_workspace_size(int64_t rows, int64_t words);
+int moc_logits_loss(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t ld, const void* ids,
+                    int ids_dtype, int64_t ids_ld, const void* top, int top_dtype, int64_t top_ld, int64_t words,
+                    float temperature, const float* row_weight, int mean, const float* grad, float* row_loss,
+                    float* loss, void* dlogits, int64_t ldd, void* workspace, int64_t workspace_bytes, void* counters,
                     void* stream);
 
 /* The same of the logits h w^T, h [rows, hidden], w [vocab, hidden] (16-byte aligned
- * rows), which exist for a piece of the rows at a time: dh [rows, hidden] and dw
- * [vocab, hidden], contiguous, either NULL (both: the loss alone).  A bf16 weight of
- * up to 2 GiB.  gemm_ws: as moc_gemm_ws uses it. */
+ * rows whose pitch their storage holds to the last one's end), which exist for a piece
+ * of the rows at a time: dh [rows, hidden] and dw [vocab, hidden], contiguous, either
+ * NULL (both: the losses alone).  words = 0: against labels (temperature 1), else
+ * against a teacher.  A bf16 weight of up to 2 GiB.  bf16 operands' gradients are f16
+ * on their way (see vocab_loss.hip).  gemm_ws: as moc_gemm_ws uses it, its counters
+ * too. */
 int64_t moc_linear_loss_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t words,
                                        int grads);
 int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int grads);
 int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w,
-                    int64_t vocab, int64_t ldw, void* targets, int64_t words, float temperature, float* row_loss,
+                    int64_t vocab, int64_t ldw, const int64_t* labels, int64_t ignore_index, const void* ids,
+                    int ids_dtype, int64_t ids_ld, const void* top, int top_dtype, int64_t top_ld, int64_t words,
+                    float temperature, const float* row_weight, int mean, const float* grad, float* row_loss,
                     float* loss, void* dh, int dh_dtype, void* dw, int dw_dtype, void* workspace,
                     int64_t workspace_bytes, void* gemm_ws, int64_t gemm_ws_bytes, void* stream);
 

@@ -84,15 +84,14 @@ SIGNATURES: dict[str, tuple] = {
                                                 _vp, _i64, _vp]),
     "moc_next_token_loss_backward": (_int, [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _int, _vp,
                                             _i64, _vp]),
-    "moc_loss_targets_size": (_i64, [_i64, _i64, _i64]),
-    "moc_label_targets": (_int, [_vp, _i64, _i64, _i64, _vp, _int, _vp, _vp, _vp]),
-    "moc_teacher_targets": (_int, [_vp, _int, _i64, _vp, _int, _i64, _i64, _i64, _i64, ctypes.c_float, _vp, _int,
-                                   _vp, _vp, _vp]),
-    "moc_logits_loss": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _i64, ctypes.c_float, _vp, _vp, _vp, _i64, _vp]),
+    "moc_logits_loss_workspace_size": (_i64, [_i64, _i64]),
+    "moc_logits_loss": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _int, _i64, _vp, _int, _i64, _i64, ctypes.c_float, _vp,
+                               _int, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp]),
     "moc_linear_loss_workspace_size": (_i64, [_int, _i64, _i64, _i64, _i64, _int]),
     "moc_linear_loss_gemm_workspace_size": (_i64, [_int, _i64, _i64, _i64, _int]),
-    "moc_linear_loss": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, ctypes.c_float, _vp, _vp,
-                               _vp, _int, _vp, _int, _vp, _i64, _vp, _i64, _vp]),
+    "moc_linear_loss": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _int, _i64, _vp, _int, _i64,
+                               _i64, ctypes.c_float, _vp, _int, _vp, _vp, _vp, _vp, _int, _vp, _int, _vp, _i64, _vp,
+                               _i64, _vp]),
     "moc_scale_inplace": (_int, [_int, _vp, _i64, _int, _vp, _i64, _vp, _vp]),
     "moc_attention_half_saved_size": (_i64, [_i64, _i64, _i64, _i64, _int]),
     "moc_attention_half_scratch_size": (_i64, [_i64, _i64, _i64, _i64, _int]),

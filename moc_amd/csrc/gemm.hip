@@ -171,15 +171,15 @@ struct GemmArgs {
   // Logits of a loss (gemm_pp_kernel<..., LOSS = true>): C is not stored, but per
   // row and slab of 64 columns the maximum m of x = unit C and the sum of exp2(x - m)
   // (ls_stat [M][ls_slabs]), the exponentials as f16 (C, rows ldc apart, null: not
-  // kept) and C itself in f32 at the columns named by ls_ids [M][ls_words]
-  // (ascending; ls_z of the same shape; ls_first [ls_slabs + 1][ls_ld_first]: how many
+  // kept) and C itself in f32 (ls_z [M][ls_words]) at the columns named by ls_ids
+  // [M][ls_words] (rows ls_ld_ids apart, ascending; others than columns: none; ls_first [ls_slabs + 1][ls_ld_first]: how many
   // of a row's lie left of each slab, null for one a row).
   float2* ls_stat;
   int ls_slabs, ls_words;
   float ls_unit;
   const int32_t* ls_ids;
   const uint16_t* ls_first;
-  int64_t ls_ld_first;
+  int64_t ls_ld_ids, ls_ld_first;
   float* ls_z;
   // f16 operands (HALF = true; moc::gemm_half): C = *alpha A B
   const float* alpha;
@@ -974,7 +974,7 @@ __device__ __forceinline__ void loss_epilogue(const GemmArgs& g, char* lds, f32x
         next[i] = first[0];
         last[i] = first[g.ls_ld_first];
       } else {  // one word a row
-        last[i] = g.ls_ids[row] >> 6 == slab0 >> 6;
+        last[i] = g.ls_ids[row * g.ls_ld_ids] >> 6 == slab0 >> 6;
       }
     }
   }
@@ -1001,7 +1001,7 @@ __device__ __forceinline__ void loss_epilogue(const GemmArgs& g, char* lds, f32x
       z[k] = v[0];
     };
     for (int k = next[i]; __any(k < last[i]); ++k) {
-      const int c = k < last[i] ? g.ls_ids[static_cast<int64_t>(row) * g.ls_words + k] - slab0 : -1;
+      const int c = k < last[i] ? g.ls_ids[row * g.ls_ld_ids + k] - slab0 : -1;
       if (c >= 0 && ((c >> 2) & 1) == half) put(c, k);
     }
     if (edge) {
@@ -2383,8 +2383,8 @@ PairSplitPlan plan_split_pair(int64_t M1, int64_t N1, int nk1, int64_t M2, int64
 // Logits h w^T of a loss (see GemmArgs::ls_stat and abi.h).  128-row tiles where
 // 256-row ones would leave half of the CUs idle.
 int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab,
-                     int64_t ldw, float unit, const int32_t* ids, const uint16_t* first, int64_t ld_first,
-                     int64_t words, float* z, float2* stat, void* kept, int64_t ld_kept, hipStream_t st) {
+                     int64_t ldw, float unit, const int32_t* ids, int64_t ld_ids, const uint16_t* first,
+                     int64_t ld_first, int64_t words, float* z, float2* stat, void* kept, int64_t ld_kept, hipStream_t st) {
   GemmArgs a{};
   const bool ok = make_operand(h, ldh, true, rows, hidden, a.a[0]) && make_operand(w, ldw, true, vocab, hidden, a.b[0]);
   auto no_wrap = [](const Operand& o) {
@@ -2411,6 +2411,7 @@ int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, c
   a.ls_unit = unit;
   a.ls_ids = ids;
   a.ls_first = first;
+  a.ls_ld_ids = ld_ids;
   a.ls_ld_first = ld_first;
   a.ls_z = z;
   const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;

@@ -24,48 +24,101 @@ constexpr int kMaxWords = 1024;
 constexpr int32_t kNoWord = 0x7FFFFFFF;  // behind the words of a row
 constexpr int32_t kUnknown = -2;         // a label outside the vocabulary
 
-// What the losses read of the targets, in one buffer (targets_layout).
+// What the losses read of the targets.  The pointers of a row's data are those of
+// all rows; kernels of a piece of the rows add its first.
 struct Targets {
+  // labels (null: a teacher)
+  const int64_t* labels;
+  int64_t ignore;
+  const float* row_weight;  // null: 1
+  // a teacher
+  float* weight;    // [rows], 0: the row counts for nothing
+  float* entropy;   // [rows] sum of q ln q
+  int32_t* ids;     // [rows][words] ascending, kNoWord behind the last
+  float* share;     // [rows][words]; a word's second entry: -1
+  uint16_t* first;  // [slabs + 1][rows] words left of each slab
+  // over all rows
   double* total;    // sum of the weights (1 for a sum of losses)
   float* factor;    // upstream gradient / total
   float* largest;   // a power of two, no weight above it; 0: no row counts
   float* alpha;     // [2] what the f16 products for dhidden and dweight are times
-  float* weight;    // [rows], 0: the row counts for nothing
-  float* entropy;   // [rows] sum of q ln q (teacher only)
-  int32_t* ids;     // [rows][words] ascending, kNoWord behind the last
-  float* share;     // [rows][words] (teacher only); a word's second entry: -1
-  uint16_t* first;  // [slabs + 1][rows] (teacher only) words left of each slab
 };
+
+__device__ __forceinline__ float weight_of(const Targets& t, int64_t r) {
+  if (t.labels == nullptr) return t.weight[r];
+  return t.labels[r] == t.ignore ? 0.f : t.row_weight != nullptr ? t.row_weight[r] : 1.f;
+}
+
+// Word k of row r, kUnknown for a label outside the vocabulary; its share, -1 for
+// what is no word of its own.
+__device__ __forceinline__ int32_t word_of(const Targets& t, int64_t r, int words, int k, int vocab, float& share) {
+  if (t.labels != nullptr) {
+    const int64_t label = t.labels[r];
+    share = 1.f;
+    return label >= 0 && label < vocab ? static_cast<int32_t>(label) : kUnknown;
+  }
+  const int32_t id = t.ids[r * words + k];
+  share = id == kNoWord ? -1.f : t.share[r * words + k];
+  return id;
+}
 
 int64_t slabs_of(int64_t vocab) { return (vocab + kLossSlab - 1) / kLossSlab; }
 
 int64_t align256(int64_t n) { return (n + 255) & ~255LL; }
 
-// words = 0: labels.
-int64_t targets_layout(int64_t rows, int64_t words, int64_t vocab, char* base, Targets* t) {
-  int64_t at = 256;
-  auto take = [&](int64_t bytes) {
+// A workspace's parts, taken one after another.
+struct Taken {
+  char* base;
+  int64_t at = 0;
+  template <typename T>
+  T* take(int64_t n) {
     const int64_t here = at;
-    at += align256(bytes);
-    return base + here;
-  };
-  char* weight = take(rows * 4);
-  char* ids = take(rows * (words > 0 ? words : 1) * 4);
-  char* entropy = words > 0 ? take(rows * 4) : nullptr;
-  char* share = words > 0 ? take(rows * words * 4) : nullptr;
-  char* first = words > 0 ? take(rows * (slabs_of(vocab) + 1) * 2) : nullptr;
-  if (t != nullptr) {
-    t->total = reinterpret_cast<double*>(base);
-    t->factor = reinterpret_cast<float*>(base + 8);
-    t->largest = reinterpret_cast<float*>(base + 12);
-    t->alpha = reinterpret_cast<float*>(base + 16);
-    t->weight = reinterpret_cast<float*>(weight);
-    t->ids = reinterpret_cast<int32_t*>(ids);
-    t->entropy = reinterpret_cast<float*>(entropy);
-    t->share = reinterpret_cast<float*>(share);
-    t->first = reinterpret_cast<uint16_t*>(first);
+    at += align256(n * static_cast<int64_t>(sizeof(T)));
+    return reinterpret_cast<T*>(base + here);
   }
-  return at;
+};
+
+// table: with the words left of each slab (linear losses).
+void take_targets(Taken& ws, int64_t rows, int64_t words, int64_t slabs, bool table, Targets& t) {
+  t.total = ws.take<double>(32);
+  t.factor = reinterpret_cast<float*>(t.total + 1);
+  t.largest = t.factor + 1;
+  t.alpha = t.factor + 2;
+  if (words > 0) {
+    t.weight = ws.take<float>(rows);
+    t.entropy = ws.take<float>(rows);
+    t.ids = ws.take<int32_t>(rows * words);
+    t.share = ws.take<float>(rows * words);
+    if (table) t.first = ws.take<uint16_t>(rows * (slabs + 1));
+  }
+}
+
+// Arrival counters of a launch, in the zeroed bytes at the start of a GEMM workspace
+// (the products' own count from the front, as many as the CUs) and left zero.
+constexpr int kTeacherCounter = 1022, kLossCounter = 1023;
+static_assert(kLossCounter * 4 < MOC_GEMM_WS_COUNTER_BYTES, "counters");
+// Rows whose losses the last workgroup of their own launch sums up: more have a
+// launch for it, since arrivals at one word take some 4 ns each.
+constexpr int64_t kArriveRows = 2048;
+
+// Values that another workgroup of the same launch reads: through to memory, past the
+// L2 of this XCD.
+__device__ __forceinline__ void put_far(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get_far(const float* p) {
+  return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Counts the workgroup; called by its thread 0, behind its put_far, which has reached
+// memory when the count does.  True for the launch's last, for which get_far has what
+// all of them put.  Nothing waits for another workgroup.
+__device__ __forceinline__ bool arrive(int* counter, int blocks) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  const bool last =
+      __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == blocks - 1;
+  if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return last;
 }
 
 // Sum or maximum over a workgroup of up to 1024 threads, in wave order.
@@ -99,103 +152,131 @@ __device__ __forceinline__ double block_sum64(double v, double* red) {
 }
 
 // ------------------------------------------------------------------ targets
-// Weight of a label's row.
-__device__ __forceinline__ float label_weight(int64_t label, int64_t ignore, const float* row_weight, int64_t r) {
-  return label == ignore ? 0.f : row_weight != nullptr ? row_weight[r] : 1.f;
-}
-
 // The least power of two, a normal number, that x >= 0 is not above.
 __device__ __forceinline__ float power_above(float x) {
   const uint32_t up = (__float_as_uint(x) + 0x7FFFFFu) >> 23;
   return __uint_as_float((up < 1 ? 1u : up > 254 ? 254u : up) << 23);
 }
 
-__device__ __forceinline__ void put_total(const Targets& t, double s, float most, int mean, const float* grad) {
+// Sum and largest of the weights by one workgroup: total (a sum of losses: 1),
+// factor = grad / total, largest.  FAR: of weights from the same launch.
+template <bool FAR>
+__device__ __forceinline__ void put_total(const Targets& t, int64_t rows, int mean, const float* grad, double* red64,
+                                          float* red) {
+  double s = 0;
+  float m = 0.f;
+#pragma unroll 8
+  for (int64_t r = threadIdx.x; r < rows; r += blockDim.x) {
+    const float w = FAR ? get_far(t.weight + r) : weight_of(t, r);
+    s += w;
+    m = fmaxf(m, fabsf(w));
+  }
+  s = block_sum64(s, red64);
+  m = block_reduce<true>(m, red);
+  if (threadIdx.x != 0) return;
   if (!mean) s = 1.0;
   *t.total = s;
   *t.factor = static_cast<float>((grad != nullptr ? static_cast<double>(*grad) : 1.0) / s);
-  *t.largest = most > 0.f ? power_above(most) : 0.f;
+  *t.largest = m > 0.f ? power_above(m) : 0.f;
 }
 
-// Workgroup 0 sums the weights beside the others, which write the rows' targets.
-__global__ __launch_bounds__(1024) void label_targets_kernel(const int64_t* __restrict__ labels, int64_t rows,
-                                                            int64_t vocab, int64_t ignore,
+// A teacher's rows of up to 64 W words, a wave a row, W words a lane: sorted by rank
+// (ties by place), entries of one word made one.  counter (null: not here): the last
+// workgroup sums the weights.
+template <typename ID, bool TOP_F32, int W>
+__global__ __launch_bounds__(1024) void teacher_wave_kernel(const ID* __restrict__ ids, int64_t ids_ld,
+                                                            const void* __restrict__ top, int64_t top_ld, int64_t rows,
+                                                            int words, int vocab, float heat,
                                                             const float* __restrict__ row_weight, int mean,
-                                                            const float* __restrict__ grad, Targets t) {
-  if (blockIdx.x == 0) {
-    __shared__ double red[16];
-    __shared__ float most[16];
-    double s = 0;
-    float m = 0.f;
-#pragma unroll 8
-    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
-      const float w = label_weight(labels[r], ignore, row_weight, r);
-      s += w;
-      m = fmaxf(m, fabsf(w));
-    }
-    s = block_sum64(s, red);
-    m = block_reduce<true>(m, most);
-    if (threadIdx.x == 0) put_total(t, s, m, mean, grad);
-    return;
-  }
-  const int64_t r = (static_cast<int64_t>(blockIdx.x) - 1) * 1024 + threadIdx.x;
-  if (r >= rows) return;
-  const int64_t label = labels[r];
-  t.weight[r] = label_weight(label, ignore, row_weight, r);
-  t.ids[r] = label == ignore ? kNoWord : label >= 0 && label < vocab ? static_cast<int32_t>(label) : kUnknown;
-}
-
-// One wave a row of up to 64 words, a lane a word; as the kernel below.
-template <typename ID, bool TOP_F32>
-__global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict__ ids, int64_t ids_ld,
-                                                           const void* __restrict__ top, int64_t top_ld, int64_t rows,
-                                                           int words, int64_t vocab, float heat,
-                                                           const float* __restrict__ row_weight, Targets t) {
+                                                            const float* __restrict__ grad, Targets t, int* counter) {
+  constexpr int kWide = 64 * W;
+  __shared__ __attribute__((aligned(16))) int32_t id_of[16][kWide];
+  __shared__ int32_t sorted_id[16][kWide];
+  __shared__ float sorted_q[16][kWide];
+  __shared__ double red64[16];
+  __shared__ float red[16];
+  __shared__ int flag;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  if (r >= rows) return;
-  int32_t id = kNoWord;
-  float x = -INFINITY;
-  if (lane < words) {
-    const int64_t word = static_cast<int64_t>(ids[r * ids_ld + lane]);
-    x = (TOP_F32 ? static_cast<const float*>(top)[r * top_ld + lane]
-                 : bf16_to_f32(static_cast<const uint16_t*>(top)[r * top_ld + lane])) / heat;
-    if (word >= 0 && word < vocab && x != -INFINITY) id = static_cast<int32_t>(word);
-    else x = -INFINITY;
-  }
-  const bool some = __any(id != kNoWord);
-  float mx = x;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 16 + wave;
+  if (r < rows) {
+    int32_t id[W];
+    float q[W], mx = -INFINITY;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-  float q = id == kNoWord ? 0.f : exp2f((x - mx) * kLog2E);
-  q = q / wave_sum(q);
-  int rank = 0;
-  for (int j = 0; j < words; ++j) {
-    const int32_t other = __builtin_amdgcn_readlane(id, j);
-    rank += other < id || (other == id && j < lane);
+    for (int i = 0; i < W; ++i) {
+      const int k = lane + 64 * i;
+      id[i] = kNoWord;
+      q[i] = -INFINITY;
+      if (k < words) {
+        const int64_t word = static_cast<int64_t>(ids[r * ids_ld + k]);
+        const float x = (TOP_F32 ? static_cast<const float*>(top)[r * top_ld + k]
+                                 : bf16_to_f32(static_cast<const uint16_t*>(top)[r * top_ld + k])) / heat;
+        if (word >= 0 && word < vocab && x != -INFINITY) {
+          id[i] = static_cast<int32_t>(word);
+          q[i] = x;
+        }
+      }
+      mx = fmaxf(mx, q[i]);
+      id_of[wave][k] = id[i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    float sum = 0.f;
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      some |= id[i] != kNoWord;
+      q[i] = id[i] == kNoWord ? 0.f : exp2f((q[i] - mx) * kLog2E);
+      sum += q[i];
+    }
+    some = __any(some);
+    sum = wave_sum(sum);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own row of LDS
+    __builtin_amdgcn_wave_barrier();
+    int rank[W] = {};
+    for (int j = 0; j < kWide; j += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(&id_of[wave][j]);
+      const int32_t other[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+          rank[i] += other[e] < id[i] || (other[e] == id[i] && j + e < lane + 64 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      sorted_id[wave][rank[i]] = id[i];
+      sorted_q[wave][rank[i]] = q[i] / sum;
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __builtin_amdgcn_wave_barrier();
+    float h = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int k = lane + 64 * i;
+      const int32_t mine = sorted_id[wave][k];
+      float share = -1.f;
+      if (mine != kNoWord && (k == 0 || sorted_id[wave][k - 1] != mine)) {
+        share = sorted_q[wave][k];
+        for (int j = k + 1; j < words && sorted_id[wave][j] == mine; ++j) share += sorted_q[wave][j];
+        h += share > 0.f || share != share ? share * logf(share) : 0.f;
+      }
+      if (k < words) {
+        t.ids[r * words + k] = mine;
+        t.share[r * words + k] = share;
+      }
+    }
+    h = wave_sum(h);
+    if (lane == 0) {
+      put_far(t.weight + r, !some ? 0.f : row_weight != nullptr ? row_weight[r] : 1.f);
+      t.entropy[r] = some ? h : 0.f;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // there before the workgroup is counted
+    }
   }
-  if (lane >= words) rank = lane;
-  id = __builtin_amdgcn_ds_permute(rank * 4, id);
-  q = __int_as_float(__builtin_amdgcn_ds_permute(rank * 4, __float_as_int(q)));
-  // a word's first entry gets the shares of the others, which follow it
-  const int32_t before = __shfl_up(id, 1);
-  const bool head = id != kNoWord && (lane == 0 || before != id);
-  float share = q;
-  for (int o = 1; o < words; ++o) {
-    const bool same = __shfl_down(id, o) == id && id != kNoWord && lane + o < 64;
-    const float other = __shfl_down(q, o);
-    if (!__any(same)) break;
-    if (same) share += other;
-  }
-  const float h = wave_sum(head && (share > 0.f || share != share) ? share * logf(share) : 0.f);
-  if (lane < words) {
-    t.ids[r * words + lane] = id;
-    t.share[r * words + lane] = head ? share : -1.f;
-  }
-  if (lane == 0) {
-    t.weight[r] = !some ? 0.f : row_weight != nullptr ? row_weight[r] : 1.f;
-    t.entropy[r] = some ? h : 0.f;
-  }
+  if (counter == nullptr) return;
+  __syncthreads();  // every wave's row; thread 0's count covers them (put_far by each wave's lane 0)
+  if (threadIdx.x == 0) flag = arrive(counter, gridDim.x);
+  __syncthreads();
+  if (flag) put_total<true>(t, rows, mean, grad, red64, red);
 }
 
 // One workgroup a row.  Words sorted by rank (ties by place); entries of the
@@ -203,7 +284,7 @@ __global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict_
 template <typename ID, bool TOP_F32>
 __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restrict__ ids, int64_t ids_ld,
                                                               const void* __restrict__ top, int64_t top_ld, int words,
-                                                              int64_t vocab, float heat,
+                                                              int vocab, float heat,
                                                               const float* __restrict__ row_weight, Targets t) {
   __shared__ int32_t id[kMaxWords], sorted_id[kMaxWords];
   __shared__ float q[kMaxWords], sorted_q[kMaxWords];
@@ -272,26 +353,24 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restri
   }
 }
 
-// How many of a row's words lie left of each slab: 64 rows a workgroup, a lane a
-// row, so that the table's lines are written and read whole; each of the 16 waves
-// walks a sixteenth of the slabs along its rows' words, which stand in LDS up to
-// kWordsLds of them (a chain of loads from memory otherwise: 8192 rows of 64 words
-// 22 us, 500 slabs).
-constexpr int kWordsLds = 200;
+// How many of a row's words lie left of each slab: 16 rows a workgroup, 16 threads a
+// row that walk a sixteenth of the slabs each along its words (64 rows and 4 threads
+// each: 35 us of 777 rows and 500 slabs), a line's quarter written at a time; the words
+// in LDS up to kWordsLds of them (a chain of loads from memory otherwise).
+constexpr int kWordsLds = 256;
 
-__global__ __launch_bounds__(1024) void words_left_kernel(const int32_t* __restrict__ ids, int64_t rows, int words,
-                                                          int slabs, uint16_t* __restrict__ first) {
-  extern __shared__ int32_t held[];  // [64][words | 1]
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64, r = r0 + (threadIdx.x & 63);
+__device__ __forceinline__ void words_left(const int32_t* __restrict__ ids, int64_t rows, int words, int slabs,
+                                           uint16_t* __restrict__ first, int block, int32_t* held) {
+  const int64_t r0 = static_cast<int64_t>(block) * 16, r = r0 + (threadIdx.x & 15);
   const int32_t* mine = ids + r * words;
   if (words <= kWordsLds) {
-    const int n = static_cast<int>(rows - r0 < 64 ? rows - r0 : 64) * words;
-    for (int i = threadIdx.x; i < n; i += 1024) held[i / words * (words | 1) + i % words] = ids[r0 * words + i];
+    const int n = static_cast<int>(rows - r0 < 16 ? rows - r0 : 16) * words;
+    for (int i = threadIdx.x; i < n; i += 256) held[i / words * (words | 1) + i % words] = ids[r0 * words + i];
     __syncthreads();
-    mine = held + (threadIdx.x & 63) * (words | 1);
+    mine = held + (threadIdx.x & 15) * (words | 1);
   }
   if (r >= rows) return;
-  const int per = (slabs + 16) / 16, n0 = threadIdx.x / 64 * per;
+  const int per = (slabs + 16) / 16, n0 = threadIdx.x / 16 * per;
   int lo = 0, hi = words;
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
@@ -308,32 +387,54 @@ __global__ __launch_bounds__(1024) void words_left_kernel(const int32_t* __restr
   }
 }
 
-// total = sum of the weights or 1, factor = grad / total.  One workgroup.
-__global__ __launch_bounds__(1024) void target_total_kernel(int64_t rows, int mean, const float* __restrict__ grad,
-                                                            Targets t) {
-  __shared__ double red[16];
-  __shared__ float most[16];
-  double s = 0;
-  float m = 0.f;
-#pragma unroll 8
-  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
-    s += t.weight[r];
-    m = fmaxf(m, fabsf(t.weight[r]));
-  }
-  s = block_sum64(s, red);
-  m = block_reduce<true>(m, most);
-  if (threadIdx.x == 0) put_total(t, s, m, mean, grad);
+__global__ __launch_bounds__(256) void words_left_kernel(Targets t, int64_t rows, int words, int slabs) {
+  __shared__ int32_t held[16 * (kWordsLds + 1)];
+  words_left(t.ids, rows, words, slabs, t.first, blockIdx.x, held);
 }
 
-// loss = sum of the rows' weighted losses / total.  One workgroup.
-__global__ __launch_bounds__(1024) void loss_sum_kernel(const float* __restrict__ row_loss, int64_t rows,
-                                                        const double* __restrict__ total, float* __restrict__ loss) {
-  __shared__ double red[16];
-  double s = 0;
+// The sums over the weights where no other launch makes them.
+__global__ __launch_bounds__(1024) void target_total_kernel(int64_t rows, int mean, const float* __restrict__ grad,
+                                                            Targets t) {
+  __shared__ double red64[16];
+  __shared__ float red[16];
+  put_total<false>(t, rows, mean, grad, red64, red);
+}
+
+// What a kernel of the rows' losses leaves: each row's, and from the last workgroup
+// of the launch to count itself the loss of all (loss null: not here).
+struct LossOut {
+  float* row_loss;  // [rows of all]
+  float* loss;
+  int64_t rows;    // of all
+  int mean, known;  // known: total holds the divisor
+  int* counter;
+};
+
+// loss = sum of the rows' weighted losses / sum of their weights (mean) or 1, by one
+// workgroup.  FAR: of rows from the same launch.
+template <bool FAR>
+__device__ __forceinline__ void put_loss(const Targets& t, const LossOut& o, double* red64) {
+  double s = 0, w = 0;
+  const bool weights = o.mean && !o.known;
 #pragma unroll 8
-  for (int64_t r = threadIdx.x; r < rows; r += 1024) s += row_loss[r];
-  s = block_sum64(s, red);
-  if (threadIdx.x == 0) *loss = static_cast<float>(s / *total);
+  for (int64_t r = threadIdx.x; r < o.rows; r += blockDim.x) {
+    s += FAR ? get_far(o.row_loss + r) : o.row_loss[r];
+    if (weights) w += weight_of(t, r);
+  }
+  s = block_sum64(s, red64);
+  if (weights) w = block_sum64(w, red64);
+  if (threadIdx.x == 0) *o.loss = static_cast<float>(!o.mean ? s : s / (o.known ? *t.total : w));
+}
+
+__global__ __launch_bounds__(1024) void loss_sum_kernel(Targets t, LossOut o) {
+  __shared__ double red64[16];
+  put_loss<false>(t, o, red64);
+}
+
+// A row's loss, by thread 0 of its workgroup; true where put_loss is this one's.
+__device__ __forceinline__ bool put_row(const LossOut& o, int64_t r, float loss, int blocks) {
+  put_far(o.row_loss + r, loss);
+  return o.loss != nullptr && arrive(o.counter, blocks);
 }
 
 // ------------------------------------------------------------------- logits
@@ -391,16 +492,16 @@ __device__ __forceinline__ void store_grad(float* p, const float (&v)[4]) {
 // stays in registers, NC chunks of 16 bytes a thread, all loads in flight before the
 // first is used, and LC more in LDS; NC = 0: it is read twice, the second time from
 // the caches.
-template <typename T, int NC, int TH, int LC = 0>
-__global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld, int vocab, Targets t, int words,
-                                                         float heat, float* __restrict__ row_loss, T* dx, int64_t ldd) {
+template <typename T, int NC, int TH, int LC>
+__device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, const Targets& t, int64_t r0, int words,
+                                           float heat, const LossOut& o, int& flag, T* dx, int64_t ldd) {
   constexpr int kPer = Elem<T>::kPer, kAhead = 4;
   __shared__ float red[TH / 64], at_word[kMaxWords];
-  const int64_t r = blockIdx.x;
+  const int64_t r = r0 + blockIdx.x;
   const int tid = threadIdx.x;
-  const float w = t.weight[r];
-  const T* row = x + r * ld;
-  T* out = dx + r * ldd;
+  const float w = weight_of(t, r);
+  const T* row = x + blockIdx.x * ld;
+  T* out = dx + blockIdx.x * ldd;
   const int full = vocab / kPer, rest = vocab % kPer;  // whole chunks, elements behind them
   if (w == 0.f) {                                      // uniform
     if (dx != nullptr) {
@@ -408,7 +509,7 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
       for (int c = tid; c < full; c += TH) store_grad(out + c * kPer, zero);
       if (tid < rest) out[full * kPer + tid] = Elem<T>::of(0.f);
     }
-    if (tid == 0) row_loss[r] = 0.f;
+    if (tid == 0) flag = put_row(o, r, 0.f, gridDim.x);
     return;
   }
   const float unit = kLog2E / heat;
@@ -481,16 +582,18 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
   const int n = words > 0 ? words : 1;
   float cross = 0.f;
   for (int k = tid; k < n; k += TH) {
-    const int32_t id = t.ids[r * n + k];
+    float share;
+    const int32_t id = word_of(t, r, words, k, vocab, share);
     if (id == kUnknown) cross = NAN;
-    const float share = words > 0 ? t.share[r * n + k] : 1.f;
-    if (id < 0 || id == kNoWord || share == -1.f) continue;
+    if (id == kUnknown || share == -1.f) continue;
     const float l = fmaf(Elem<T>::one(row[id]), unit, -lse);  // log2 p
     at_word[k] = l;
     if (share != 0.f) cross -= share * l;
   }
   cross = block_reduce<false>(cross, red);
-  if (tid == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
+  // counted before the gradient is written, which its wait then overlaps
+  if (tid == 0)
+    flag = put_row(o, r, w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f))), gridDim.x);
   if (dx == nullptr) return;
   const float c = cross == cross ? heat * w * *t.factor : NAN;
   auto grad = [&](const uint4& a, int at) {
@@ -520,11 +623,21 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stored before the words' own
   __syncthreads();
   for (int k = tid; k < n; k += TH) {
-    const int32_t id = t.ids[r * n + k];
-    const float share = words > 0 ? t.share[r * n + k] : 1.f;
-    if (id < 0 || id == kNoWord || share == -1.f) continue;
+    float share;
+    const int32_t id = word_of(t, r, words, k, vocab, share);
+    if (id == kUnknown || share == -1.f) continue;
     out[id] = Elem<T>::of(c * (__builtin_amdgcn_exp2f(at_word[k]) - share));
   }
+}
+
+template <typename T, int NC, int TH, int LC = 0>
+__global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld, int vocab, Targets t, int64_t r0,
+                                                         int words, float heat, LossOut o, T* dx, int64_t ldd) {
+  __shared__ double red64[TH / 64];
+  __shared__ int flag;
+  logits_row<T, NC, TH, LC>(x, ld, vocab, t, r0, words, heat, o, flag, dx, ldd);
+  __syncthreads();
+  if (flag) put_loss<true>(t, o, red64);
 }
 
 // ------------------------------------------------- logits that were not stored
@@ -539,7 +652,8 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restrict__ h, int64_t ldh, int rows,
                                                        const uint16_t* __restrict__ w, int64_t ldw, int vocab,
                                                        int hidden, float unit, const int32_t* __restrict__ ids,
-                                                       const uint16_t* __restrict__ first, int64_t ld_first, int words,
+                                                       int64_t ld_ids, const uint16_t* __restrict__ first,
+                                                       int64_t ld_first, int words,
                                                        float* __restrict__ z, float2* __restrict__ stat, int slabs) {
   extern __shared__ uint4 frag[];  // [steps][64], then the waves' maxima and sums
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -591,7 +705,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
     if (row < rows) {
       int k = first != nullptr ? first[slab * ld_first + row] : 0;
       for (; k < words; ++k) {
-        const int c = ids[row * words + k] - slab * kLossSlab - c0;
+        const int c = ids[row * ld_ids + k] - slab * kLossSlab - c0;
         if (c >= 4) break;
         if (c >= 0 && c < 4) z[row * words + k] = c == 0 ? acc[0] : c == 1 ? acc[1] : c == 2 ? acc[2] : acc[3];
       }
@@ -627,20 +741,6 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
   }
 }
 
-int launch_few(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab, int64_t ldw,
-               float unit, const Targets& t, int64_t ld_first, int64_t words, float* z, float2* stat, int64_t slabs,
-               hipStream_t st) {
-  const int steps = static_cast<int>((hidden + 31) / 32);
-  const int lds = steps * 1024 + 2 * 4 * 16 * 8;
-  const int64_t resident = static_cast<int64_t>(cu_count()) * (160 * 1024 / lds < 8 ? 160 * 1024 / lds : 8);
-  const unsigned grid = static_cast<unsigned>(slabs < resident ? slabs : resident);
-  few_rows_kernel<<<grid, 256, lds, st>>>(static_cast<const uint16_t*>(h), ldh, (int)rows,
-                                          static_cast<const uint16_t*>(w), ldw, (int)vocab, (int)hidden, unit, t.ids,
-                                          words > 0 ? t.first : nullptr, ld_first, (int)(words > 0 ? words : 1), z,
-                                          stat, (int)slabs);
-  return check_launch("few_rows_kernel");
-}
-
 // log2 of a row's sum of exponentials from its slabs' maxima and sums; 256 threads,
 // a slab's loads in flight with its seven followers'.
 __device__ __forceinline__ float slabs_lse(const float2* __restrict__ stat, int slabs, float* red) {
@@ -665,125 +765,50 @@ __device__ __forceinline__ float slabs_lse(const float2* __restrict__ stat, int 
   return all + log2f(s);
 }
 
-// A row's cross entropy sum q (-log2 p) over the words this thread takes, of log2 p
-// of each word, which goes to at_word (may be null); NaN for an unknown label.
-__device__ __forceinline__ float cross_of(const Targets& t, int64_t r, int words, const float* __restrict__ z,
-                                          float unit, float lse, float* at_word, int first, int step) {
-  const int n = words > 0 ? words : 1;
+// A row's cross entropy sum q (-log2 p) over the words this thread takes, log2 p of
+// each into at_word (may be null); NaN for an unknown label.  z: its words' logits.
+__device__ __forceinline__ float cross_of(const Targets& t, int64_t r, int words, int vocab,
+                                          const float* __restrict__ z, float unit, float lse, float* at_word) {
   float cross = 0.f;
-  for (int k = first; k < n; k += step) {
-    const int32_t id = t.ids[r * n + k];
+  for (int k = threadIdx.x; k < (words > 0 ? words : 1); k += 256) {
+    float share;
+    const int32_t id = word_of(t, r, words, k, vocab, share);
     if (id == kUnknown) cross = NAN;
-    const float share = words > 0 ? t.share[r * n + k] : 1.f;
-    if (id < 0 || id == kNoWord || share == -1.f) continue;
-    const float l = z[r * n + k] * unit - lse;
+    if (id == kUnknown || share == -1.f) continue;
+    const float l = z[k] * unit - lse;
     if (at_word != nullptr) at_word[k] = l;
     if (share != 0.f) cross -= share * l;
   }
   return cross;
 }
 
+// What a row's logits left (launch_loss_gemm): statistics of its slabs and its words'
+// logits, rows of the piece; r0: the piece's first row.
+struct Slabs {
+  const float2* stat;
+  const float* z;
+  int count, vocab, words;
+  int64_t r0;
+  float heat;
+};
+
 // Losses alone: one workgroup a row.
-__global__ __launch_bounds__(256) void slabs_loss_kernel(const float2* __restrict__ stat, int slabs, Targets t,
-                                                         int words, float heat, const float* __restrict__ z,
-                                                         float* __restrict__ row_loss) {
+__global__ __launch_bounds__(256) void slabs_loss_kernel(Slabs s, Targets t, LossOut o) {
   __shared__ float red[4];
-  const int64_t r = blockIdx.x;
-  const float w = t.weight[r];
-  if (w == 0.f) {  // uniform
-    if (threadIdx.x == 0) row_loss[r] = 0.f;
-    return;
+  __shared__ double red64[4];
+  __shared__ int flag;
+  const int64_t r = s.r0 + blockIdx.x;
+  const float w = weight_of(t, r);
+  float loss = 0.f;
+  if (w != 0.f) {  // uniform
+    const float lse = slabs_lse(s.stat + static_cast<int64_t>(blockIdx.x) * s.count, s.count, red);
+    const float* z = s.z + static_cast<int64_t>(blockIdx.x) * (s.words > 0 ? s.words : 1);
+    const float cross = block_reduce<false>(cross_of(t, r, s.words, s.vocab, z, kLog2E / s.heat, lse, nullptr), red);
+    loss = w * (s.heat * s.heat * (cross * kLn2 + (s.words > 0 ? t.entropy[r] : 0.f)));
   }
-  const float lse = slabs_lse(stat + r * slabs, slabs, red);
-  const float cross = block_reduce<false>(cross_of(t, r, words, z, kLog2E / heat, lse, nullptr, threadIdx.x, 256), red);
-  if (threadIdx.x == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
-}
-
-// One workgroup a row: its loss, and its f16 exponentials into gradients of the
-// logits, in place: e exp2(m - lse) of a slab's reference m is p.  The gradients stay
-// in f16, as (w / largest) 2^14 (p - q): a bf16 rounding of them, 2^-8 of each, would
-// add to the products' sums, where the words' parts cancel, more than the sums' own
-// rounding (measured: up to 1.9 times the error of f32 ones); 2^-11 does not show.
-// Down to 2^-28 of the largest they have all 11 bits, below 2^-39 they are 0.
-__global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld, int vocab,
-                                                         const float2* __restrict__ stat, int slabs, Targets t,
-                                                         int words, float heat, const float* __restrict__ z,
-                                                         float* __restrict__ row_loss) {
-  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-  __shared__ float red[4], at_word[kMaxWords];
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x;
-  const float w = t.weight[r];
-  uint4* row = reinterpret_cast<uint4*>(e + r * ld);
-  const int chunks = (vocab + 7) / 8;
-  if (w == 0.f) {  // uniform
-    for (int c = tid; c < chunks; c += 256) row[c] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) row_loss[r] = 0.f;
-    return;
-  }
-  const float2* st = stat + r * slabs;
-  const float lse = slabs_lse(st, slabs, red);
-  const float cross = block_reduce<false>(cross_of(t, r, words, z, kLog2E / heat, lse, at_word, tid, 256), red);
-  if (tid == 0) row_loss[r] = w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f)));
-  const float c = cross == cross ? w / *t.largest * 0x1p14f : NAN;
-  constexpr int kAhead = 4;
-  for (int c0 = tid; c0 < chunks; c0 += 256 * kAhead) {
-    uint4 v[kAhead];
-    float m[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int at = min(c0 + 256 * i, chunks - 1);
-      v[i] = row[at];
-      m[i] = st[at / (kLossSlab / 8)].x;
-    }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int at = c0 + 256 * i;
-      if (at >= chunks) break;
-      const float f = c * __builtin_amdgcn_exp2f(m[i] - lse - 15.f);
-      const uint32_t in[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-      uint32_t out[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f16x2_t h = __builtin_bit_cast(f16x2_t, in[q]);
-        out[q] = __builtin_bit_cast(uint32_t,
-                                    __builtin_convertvector((cvt_f32x2_t){static_cast<float>(h.x) * f,
-                                                                          static_cast<float>(h.y) * f},
-                                                            f16x2_t));
-      }
-      row[at] = make_uint4(out[0], out[1], out[2], out[3]);
-    }
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stored before the words' own
+  if (threadIdx.x == 0) flag = put_row(o, r, loss, gridDim.x);
   __syncthreads();
-  const int n = words > 0 ? words : 1;
-  for (int k = tid; k < n; k += 256) {
-    const int32_t id = t.ids[r * n + k];
-    const float share = words > 0 ? t.share[r * n + k] : 1.f;
-    if (id < 0 || id == kNoWord || share == -1.f) continue;
-    e[r * ld + id] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(c * (__builtin_amdgcn_exp2f(at_word[k]) - share)));
-  }
-}
-
-// Rows that count, zeros for the others: what is in those reaches no product (f32).
-// Rows of 16-byte chunks, whose last one is cut off at the hidden size.
-__global__ __launch_bounds__(256) void counted_rows_kernel(const float* __restrict__ h, int64_t ldh, int64_t rows,
-                                                           int hidden, const float* __restrict__ weight,
-                                                           float* __restrict__ out, int64_t ldo) {
-  const int chunks = (hidden + 3) / 4;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows * chunks; i += step) {
-    const int64_t r = i / chunks;
-    const int k = static_cast<int>(i - r * chunks) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (weight[r] != 0.f) {
-      v = *reinterpret_cast<const float4*>(h + r * ldh + k);
-      if (k + 1 >= hidden) v.y = 0.f;
-      if (k + 2 >= hidden) v.z = 0.f;
-      if (k + 3 >= hidden) v.w = 0.f;
-    }
-    *reinterpret_cast<float4*>(out + r * ldo + k) = v;
-  }
+  if (flag) put_loss<true>(t, o, red64);
 }
 
 // ------------------------------------------------------- operands in f16
@@ -792,7 +817,7 @@ __global__ __launch_bounds__(256) void counted_rows_kernel(const float* __restri
 // below; rows that do not count become 0.  The power is a guess that suits what
 // networks hold (the largest of the hidden rows in [2^-3, 2^13], of the weight in
 // [2^-7, 2^9]: what is rounded is off by 2^-24 of the largest at most); the largest
-// value is found on the way, and halves_again_kernel redoes a tensor that it does not
+// value is found on the way, and slabs_grad_kernel redoes a tensor that it does not
 // suit.
 struct Halves {
   const uint16_t* from;
@@ -811,21 +836,21 @@ __device__ __forceinline__ float halves_scale(const Halves& h, uint32_t range) {
 // Rows of h by hidden columns into rows of ldo (a multiple of 64, zeros behind the
 // hidden size), a wave a row, four rows' loads in flight; the bits of the largest
 // |value| this lane met.
-__device__ __forceinline__ uint32_t halve_rows(const Halves& h, int hidden, int64_t ldo, const float* weight,
-                                               float scale) {
+__device__ __forceinline__ uint32_t halve_rows(const Halves& h, int hidden, int64_t ldo, const Targets* counts,
+                                               float scale, int block, int blocks) {
   typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
   constexpr int kRows = 4;
   const int lane = threadIdx.x & 63, chunks = static_cast<int>(ldo / 8);
-  const int64_t waves = static_cast<int64_t>(gridDim.x) * 4;
+  const int64_t waves = static_cast<int64_t>(blocks) * 4;
   uint32_t most = 0;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r0 < h.rows; r0 += waves * kRows) {
+  for (int64_t r0 = static_cast<int64_t>(block) * 4 + (threadIdx.x >> 6); r0 < h.rows; r0 += waves * kRows) {
     for (int c = lane; c < chunks; c += 64) {
       const int k = 8 * c;
       uint4 v[kRows];
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         const int64_t r = r0 + waves * i;
-        v[i] = k < hidden && r < h.rows && (weight == nullptr || weight[r] != 0.f)
+        v[i] = k < hidden && r < h.rows && (counts == nullptr || weight_of(*counts, r) != 0.f)
                    ? *reinterpret_cast<const uint4*>(h.from + r * h.ld + k)
                    : make_uint4(0, 0, 0, 0);
       }
@@ -861,40 +886,153 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t m, uint32_t* red) {
   return max(max(red[0], red[1]), max(red[2], red[3]));
 }
 
-// most [2][gridDim]: the workgroups' largest values (one word for all of them would
-// have thousands of atomics in a row: 30 us).
+// most [2][blocks]: the workgroups' largest values (one word for all of them would
+// have as many atomics in a row).  Workgroup 0 sums the rows' weights meanwhile, and
+// those behind it look up a teacher's words, so that neither is a launch of its own.
 __global__ __launch_bounds__(256) void halves_kernel(Halves hidden_rows, Halves weight_rows, int hidden, int64_t ldo,
-                                                     Targets t, uint32_t* __restrict__ most) {
+                                                     Targets t, int64_t rows, int mean,
+                                                     const float* __restrict__ grad, int words, int slabs,
+                                                     uint32_t* __restrict__ most, int blocks) {
+  __shared__ int32_t held[16 * (kWordsLds + 1)];
   __shared__ uint32_t red[4];
-  uint32_t m = hidden_rows.to != nullptr ? halve_rows(hidden_rows, hidden, ldo, t.weight, hidden_rows.guess) : 0;
-  m = block_max_bits(m, red);
-  if (threadIdx.x == 0) most[blockIdx.x] = m;
-  m = weight_rows.to != nullptr ? halve_rows(weight_rows, hidden, ldo, nullptr, weight_rows.guess) : 0;
-  m = block_max_bits(m, red);
-  if (threadIdx.x == 0) most[gridDim.x + blockIdx.x] = m;
+  __shared__ float redf[4];
+  __shared__ double red64[4];
+  const int extra = static_cast<int>(gridDim.x) - blocks, block = static_cast<int>(blockIdx.x) - extra;
+  if (blockIdx.x == 0) {
+    put_total<false>(t, rows, mean, grad, red64, redf);
+  } else if (block < 0) {
+    words_left(t.ids, rows, words, slabs, t.first, blockIdx.x - 1, held);
+  } else {
+    uint32_t m = hidden_rows.to != nullptr ? halve_rows(hidden_rows, hidden, ldo, &t, hidden_rows.guess, block, blocks) : 0;
+    m = block_max_bits(m, red);
+    if (threadIdx.x == 0) most[block] = m;
+    m = weight_rows.to != nullptr ? halve_rows(weight_rows, hidden, ldo, nullptr, weight_rows.guess, block, blocks) : 0;
+    m = block_max_bits(m, red);
+    if (threadIdx.x == 0) most[blocks + block] = m;
+  }
 }
 
-// Redoes a tensor whose largest value the guess did not suit; the products' factors.
-__global__ __launch_bounds__(256) void halves_again_kernel(Halves hidden_rows, Halves weight_rows, int hidden,
-                                                           int64_t ldo, float heat, Targets t,
-                                                           const uint32_t* __restrict__ most, int parts) {
+// One workgroup a row: its loss, and its f16 exponentials into gradients of the
+// logits, in place: e exp2(m - lse) of a slab's reference m is p.  The gradients stay
+// in f16, as (w / largest) 2^14 (p - q): a bf16 rounding of them, 2^-8 of each, would
+// add to the products' sums, where the words' parts cancel, more than the sums' own
+// rounding (measured: up to 1.9 times the error of f32 ones); 2^-11 does not show.
+// Down to 2^-28 of the largest they have all 11 bits, below 2^-39 they are 0.
+__device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Slabs& s, const Targets& t,
+                                               const LossOut& o, int& flag, int64_t at, int rows) {
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+  __shared__ float red[4], at_word[kMaxWords];
+  const int64_t r = s.r0 + at;
+  const int tid = threadIdx.x;
+  const float w = weight_of(t, r);
+  uint16_t* out = e + at * ld;
+  uint4* row = reinterpret_cast<uint4*>(out);
+  const int chunks = (s.vocab + 7) / 8;
+  if (w == 0.f) {  // uniform
+    for (int c = tid; c < chunks; c += 256) row[c] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) flag = put_row(o, r, 0.f, rows);
+    return;
+  }
+  const float2* st = s.stat + at * s.count;
+  const float lse = slabs_lse(st, s.count, red);
+  const float* z = s.z + at * (s.words > 0 ? s.words : 1);
+  const float cross = block_reduce<false>(cross_of(t, r, s.words, s.vocab, z, kLog2E / s.heat, lse, at_word), red);
+  // counted before the gradient is written, which its wait then overlaps
+  if (tid == 0)
+    flag = put_row(o, r, w * (s.heat * s.heat * (cross * kLn2 + (s.words > 0 ? t.entropy[r] : 0.f))), rows);
+  const float c = cross == cross ? w / *t.largest * 0x1p14f : NAN;
+  constexpr int kAhead = 4;
+  for (int c0 = tid; c0 < chunks; c0 += 256 * kAhead) {
+    uint4 v[kAhead];
+    float m[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = min(c0 + 256 * i, chunks - 1);
+      v[i] = row[at];
+      m[i] = st[at / (kLossSlab / 8)].x;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = c0 + 256 * i;
+      if (at >= chunks) break;
+      const float f = c * __builtin_amdgcn_exp2f(m[i] - lse - 15.f);
+      const uint32_t in[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      uint32_t out[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, in[q]);
+        out[q] = __builtin_bit_cast(uint32_t,
+                                    __builtin_convertvector((cvt_f32x2_t){static_cast<float>(h.x) * f,
+                                                                          static_cast<float>(h.y) * f},
+                                                            f16x2_t));
+      }
+      row[at] = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stored before the words' own
+  __syncthreads();
+  for (int k = tid; k < (s.words > 0 ? s.words : 1); k += 256) {
+    float share;
+    const int32_t id = word_of(t, r, s.words, k, s.vocab, share);
+    if (id == kUnknown || share == -1.f) continue;
+    out[id] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(c * (__builtin_amdgcn_exp2f(at_word[k]) - share)));
+  }
+}
+
+// The first piece has kAgainBlocks workgroups more, which look at the f16 operands:
+// those that the guess did not suit are done again, and the products' factors written.
+constexpr int kAgainBlocks = 64;
+
+__global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld, Slabs s, Targets t, LossOut o,
+                                                         Halves hidden_rows, Halves weight_rows, int hidden,
+                                                         int64_t ldo, const uint32_t* __restrict__ most, int parts) {
+  __shared__ double red64[4];
   __shared__ uint32_t red[4];
-  uint32_t m[2] = {0, 0};
-#pragma unroll 8
-  for (int i = threadIdx.x; i < parts; i += 256) {
-    m[0] = max(m[0], most[i]);
-    m[1] = max(m[1], most[parts + i]);
+  __shared__ int flag;
+  const int again = s.r0 == 0 ? kAgainBlocks : 0;
+  if (static_cast<int>(blockIdx.x) < again) {
+    uint32_t m[2] = {0, 0};
+#pragma unroll 4
+    for (int i = threadIdx.x; i < parts; i += 256) {
+      m[0] = max(m[0], most[i]);
+      m[1] = max(m[1], most[parts + i]);
+    }
+    const float sx = halves_scale(hidden_rows, block_max_bits(m[0], red));
+    const float sw = halves_scale(weight_rows, block_max_bits(m[1], red));
+    if (sx != hidden_rows.guess) halve_rows(hidden_rows, hidden, ldo, &t, sx, blockIdx.x, again);
+    if (sw != weight_rows.guess) halve_rows(weight_rows, hidden, ldo, nullptr, sw, blockIdx.x, again);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      // no row counts: gradients of 0, whatever the divisor
+      const float f = *t.largest > 0.f ? s.heat * *t.factor * *t.largest * 0x1p-14f : 0.f;
+      t.alpha[0] = f / sw;
+      t.alpha[1] = f / sx;
+    }
+    return;
   }
-  const float sx = halves_scale(hidden_rows, block_max_bits(m[0], red));
-  const float sw = halves_scale(weight_rows, block_max_bits(m[1], red));
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    // no row counts: gradients of 0, whatever the divisor
-    const float f = *t.largest > 0.f ? heat * *t.factor * *t.largest * 0x1p-14f : 0.f;
-    t.alpha[0] = f / sw;
-    t.alpha[1] = f / sx;
+  slabs_grad_row(e, ld, s, t, o, flag, blockIdx.x - again, gridDim.x - again);
+  __syncthreads();
+  if (flag) put_loss<true>(t, o, red64);
+}
+
+// Rows that count, zeros for the others: what is in those reaches no product (f32).
+// Rows of 16-byte chunks, whose last one is cut off at the hidden size.
+__global__ __launch_bounds__(256) void counted_rows_kernel(const float* __restrict__ h, int64_t ldh, int64_t rows,
+                                                           int hidden, Targets t, float* __restrict__ out,
+                                                           int64_t ldo) {
+  const int chunks = (hidden + 3) / 4;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows * chunks; i += step) {
+    const int64_t r = i / chunks;
+    const int k = static_cast<int>(i - r * chunks) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (weight_of(t, r) != 0.f) {
+      v = *reinterpret_cast<const float4*>(h + r * ldh + k);
+      if (k + 1 >= hidden) v.y = 0.f;
+      if (k + 2 >= hidden) v.z = 0.f;
+      if (k + 3 >= hidden) v.w = 0.f;
+    }
+    *reinterpret_cast<float4*>(out + r * ldo + k) = v;
   }
-  if (hidden_rows.to != nullptr && sx != hidden_rows.guess) halve_rows(hidden_rows, hidden, ldo, t.weight, sx);
-  if (weight_rows.to != nullptr && sw != weight_rows.guess) halve_rows(weight_rows, hidden, ldo, nullptr, sw);
 }
 
 // a += b over n values; out (may be null): the sum as bf16 or f32.
@@ -953,67 +1091,116 @@ unsigned blocks_of(int64_t n) {
   return static_cast<unsigned>(b < 1 ? 1 : b > kMostBlocks ? kMostBlocks : b);
 }
 
-// ------------------------------------------------------------------- pieces
+// --------------------------------------------------------------------- host
 // Logits exist for a piece of the rows at a time, within about this many bytes.
 constexpr int64_t kPieceBytes = 1LL << 30;
+constexpr int kHalvesBlocks = 1024;  // workgroups of halves_kernel that write f16 rows
 
+// A linear loss's pieces and the parts of its workspace.
 struct Pieces {
-  bool fused;              // logits inside the product (launch_loss_gemm), not stored
-  int64_t rows, count;     // rows of a piece, pieces
-  int64_t ldz;             // row pitch of a piece's logits
+  bool fused;           // bf16: logits inside the product (launch_loss_gemm), not stored
+  int64_t rows, count;  // rows of a piece, pieces
+  int64_t ldz, ldx;     // row pitches: a piece's logits, the copies of hidden rows and weight
   int64_t slabs;
-  int64_t z, d, x, w, acc, part, stat, at_words, most, bytes;  // offsets in the workspace
-  int64_t ldx;
+  Targets t;
+  float* row_loss;
+  char *d, *x, *w;  // logits, then their gradients; copies of hidden rows and weight
+  float *acc, *part, *z;
+  uint32_t* most;
+  float2* stat;
+  int64_t bytes;
 };
 
-Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t words, bool grads) {
+Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t words, bool grads, void* base) {
   Pieces p{};
   const bool f32 = dtype == MOC_F32;
+  const int64_t es = f32 ? 4 : 2;
   p.fused = !f32;
   p.ldz = (vocab + 63) & ~63LL;
+  p.ldx = (hidden + 63) & ~63LL;
   p.slabs = slabs_of(vocab);
-  const int64_t n_words = words > 0 ? words : 1;
-  const int64_t each = !p.fused ? p.ldz * 4 : grads ? p.ldz * 2 : p.slabs * 8;
+  const int64_t each = f32 ? p.ldz * 4 : grads ? p.ldz * 2 : p.slabs * 8;
   int64_t n = kPieceBytes / each / 256 * 256;
   if (n < 256) n = 256;
   if (n > rows) n = rows < 1 ? 1 : rows;
   p.rows = n;
   p.count = rows < 1 ? 0 : (rows + n - 1) / n;
-  int64_t at = 0;
-  auto take = [&](int64_t bytes) {
-    const int64_t here = at;
-    at += align256(bytes);
-    return here;
-  };
+  Taken ws{static_cast<char*>(base)};
+  take_targets(ws, rows, words, p.slabs, p.fused, p.t);
+  p.row_loss = ws.take<float>(rows);
   if (p.fused) {
-    p.stat = take(n * p.slabs * 8);
-    p.at_words = take(n * n_words * 4);
-    p.d = grads ? take(n * p.ldz * 2) : 0;
-  } else {
-    p.z = take(n * p.ldz * 4);
-    p.d = p.z;  // in place
+    p.stat = ws.take<float2>(n * p.slabs);
+    p.z = ws.take<float>(n * (words > 0 ? words : 1));
   }
-  p.ldx = (hidden + 63) & ~63LL;
-  p.x = grads ? take(rows * p.ldx * (f32 ? 4 : 2)) : 0;
-  p.w = grads && !f32 ? take(vocab * p.ldx * 2) : 0;
-  p.most = grads && !f32 ? take(2 * 4 * kMostBlocks) : 0;
+  if (f32 || grads) p.d = ws.take<char>(n * p.ldz * es);
+  if (grads) p.x = ws.take<char>(rows * p.ldx * es);
+  if (grads && p.fused) {
+    p.w = ws.take<char>(vocab * p.ldx * 2);
+    p.most = ws.take<uint32_t>(2 * kHalvesBlocks);
+  }
   if (grads && p.count > 1) {
-    p.acc = take(vocab * hidden * 4);
-    p.part = take(vocab * hidden * 4);
+    p.acc = ws.take<float>(vocab * hidden);
+    p.part = ws.take<float>(vocab * hidden);
   }
-  p.bytes = at;
+  p.bytes = ws.at;
   return p;
+}
+
+// A teacher as its caller has it.
+struct Teacher {
+  const void* ids;
+  int ids_dtype;
+  int64_t ids_ld;
+  const void* top;
+  int top_dtype;
+  int64_t top_ld;
+  float heat;
+};
+
+template <typename ID, bool TOP_F32>
+void launch_teacher(const Teacher& a, int64_t rows, int words, int vocab, const float* row_weight, int mean,
+                    const float* grad, const Targets& t, int* counter, hipStream_t st) {
+  const ID* ids = static_cast<const ID*>(a.ids);
+#define MOC_WAVES(W)                                                                                                \
+  teacher_wave_kernel<ID, TOP_F32, W><<<static_cast<unsigned>((rows + 15) / 16), 1024, 0, st>>>(                      \
+      ids, a.ids_ld, a.top, a.top_ld, rows, words, vocab, a.heat, row_weight, mean, grad, t, counter)
+  if (words <= 64) MOC_WAVES(1);
+  else if (words <= 128) MOC_WAVES(2);
+  else if (words <= 256) MOC_WAVES(4);
+  else
+    teacher_targets_kernel<ID, TOP_F32><<<static_cast<unsigned>(rows), 256, 0, st>>>(ids, a.ids_ld, a.top, a.top_ld,
+                                                                                     words, vocab, a.heat, row_weight, t);
+#undef MOC_WAVES
+}
+
+// Words, shares and weights; total: the weights' sums too.
+int run_teacher(const Teacher& a, int64_t rows, int64_t words, int64_t vocab, const float* row_weight, int mean,
+                const float* grad, const Targets& t, bool total, int* counters, hipStream_t st) {
+  if (rows == 0) return MOC_OK;
+  const int k = static_cast<int>(words), v = static_cast<int>(vocab);
+  int* counter = total ? counters + kTeacherCounter : nullptr;
+#define MOC_TEACHER(ID, F) launch_teacher<ID, F>(a, rows, k, v, row_weight, mean, grad, t, counter, st)
+  if (a.ids_dtype == MOC_I32 && a.top_dtype == MOC_F32) MOC_TEACHER(int32_t, true);
+  else if (a.ids_dtype == MOC_I32) MOC_TEACHER(int32_t, false);
+  else if (a.top_dtype == MOC_F32) MOC_TEACHER(int64_t, true);
+  else MOC_TEACHER(int64_t, false);
+#undef MOC_TEACHER
+  const int rc = check_launch("teacher_wave_kernel");
+  if (rc != MOC_OK || !total || words <= 256) return rc;
+  target_total_kernel<<<1, 1024, 0, st>>>(rows, mean, grad, t);
+  return check_launch("target_total_kernel");
 }
 
 constexpr int moc_th(int th, int = 0) { return th; }
 
 template <typename T>
-void launch_logits(const T* x, int64_t rows, int vocab, int64_t ld, const Targets& t, int words, float heat,
-                   float* row_loss, T* dx, int64_t ldd, hipStream_t st) {
+void launch_logits(const T* x, int64_t rows, int vocab, int64_t ld, const Targets& t, int64_t r0, int words, float heat,
+                   const LossOut& o, T* dx, int64_t ldd, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(rows));
   const int chunks = vocab / Elem<T>::kPer;
-#define MOC_LOGITS(NC, ...) \
-  logits_loss_kernel<T, NC, __VA_ARGS__><<<grid, moc_th(__VA_ARGS__), 0, st>>>(x, ld, vocab, t, words, heat, row_loss, dx, ldd)
+#define MOC_LOGITS(NC, ...)                                                                                        \
+  logits_loss_kernel<T, NC, __VA_ARGS__><<<grid, moc_th(__VA_ARGS__), 0, st>>>(x, ld, vocab, t, r0, words, heat, o, dx, \
+                                                                               ldd)
   if (chunks <= 4 * 256) MOC_LOGITS(4, 256);
   else if (chunks <= 4 * 512) MOC_LOGITS(4, 512);
   else if (chunks <= 8 * 512) MOC_LOGITS(8, 512);
@@ -1024,16 +1211,35 @@ void launch_logits(const T* x, int64_t rows, int vocab, int64_t ld, const Target
 #undef MOC_LOGITS
 }
 
-int logits_rows(bool f32, const void* x, int64_t rows, int64_t vocab, int64_t ld, const Targets& t, int64_t words,
-                float heat, float* row_loss, void* dx, int64_t ldd, hipStream_t st) {
-  if (rows == 0) return MOC_OK;
+int logits_rows(bool f32, const void* x, int64_t rows, int64_t vocab, int64_t ld, const Targets& t, int64_t r0,
+                int64_t words, float heat, const LossOut& o, void* dx, int64_t ldd, hipStream_t st) {
   const int v = static_cast<int>(vocab), k = static_cast<int>(words);
   if (f32)
-    launch_logits(static_cast<const float*>(x), rows, v, ld, t, k, heat, row_loss, static_cast<float*>(dx), ldd, st);
+    launch_logits(static_cast<const float*>(x), rows, v, ld, t, r0, k, heat, o, static_cast<float*>(dx), ldd, st);
   else
-    launch_logits(static_cast<const uint16_t*>(x), rows, v, ld, t, k, heat, row_loss, static_cast<uint16_t*>(dx), ldd,
-                  st);
+    launch_logits(static_cast<const uint16_t*>(x), rows, v, ld, t, r0, k, heat, o, static_cast<uint16_t*>(dx), ldd, st);
   return check_launch("logits_loss_kernel");
+}
+
+// The loss where the rows' own launch does not sum it up.
+int sum_loss(const Targets& t, LossOut o, float* loss, hipStream_t st) {
+  o.loss = loss;
+  loss_sum_kernel<<<1, 1024, 0, st>>>(t, o);
+  return check_launch("loss_sum_kernel");
+}
+
+// Logits of up to kFewRows rows, losses alone.
+int launch_few(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab, int64_t ldw,
+               float unit, const int32_t* ids, int64_t ld_ids, const uint16_t* first, int64_t ld_first, int64_t words,
+               float* z, float2* stat, int64_t slabs, hipStream_t st) {
+  const int steps = static_cast<int>((hidden + 31) / 32);
+  const int lds = steps * 1024 + 2 * 4 * 16 * 8;
+  const int64_t resident = static_cast<int64_t>(cu_count()) * (160 * 1024 / lds < 8 ? 160 * 1024 / lds : 8);
+  const unsigned grid = static_cast<unsigned>(slabs < resident ? slabs : resident);
+  few_rows_kernel<<<grid, 256, lds, st>>>(static_cast<const uint16_t*>(h), ldh, (int)rows,
+                                          static_cast<const uint16_t*>(w), ldw, (int)vocab, (int)hidden, unit, ids,
+                                          ld_ids, first, ld_first, (int)words, z, stat, (int)slabs);
+  return check_launch("few_rows_kernel");
 }
 
 // C [M, N] = *alpha A B over K = 1, as moc_gemm_ws or gemm_half of these strides would.
@@ -1057,6 +1263,16 @@ bool sizes_ok(int64_t rows, int64_t vocab, int64_t words) {
   return rows >= 0 && rows <= (1LL << 24) && vocab >= 1 && vocab <= (1LL << 21) && words >= 0 && words <= kMaxWords;
 }
 
+bool temperature_ok(float t) { return t > 0.f && t < INFINITY; }
+
+int teacher_ok(const char* name, const Teacher& a, int64_t rows, int64_t words) {
+  MOC_REQUIRE((a.ids_dtype == MOC_I32 || a.ids_dtype == MOC_I64) && (a.top_dtype == MOC_BF16 || a.top_dtype == MOC_F32),
+              "%s: ids are int32 or int64, the teacher's logits bf16 or f32", name);
+  MOC_REQUIRE(rows == 0 || (a.ids != nullptr && a.top != nullptr && (rows == 1 || (a.ids_ld >= words && a.top_ld >= words))),
+              "%s: a teacher's operand is null or its rows overlap", name);
+  return MOC_OK;
+}
+
 }  // namespace
 }  // namespace moc
 
@@ -1064,106 +1280,79 @@ using namespace moc;
 
 #define MOC_SIZES(name)                                                                                          \
   MOC_REQUIRE(sizes_ok(rows, vocab, words), "%s: up to 2^24 rows, a vocabulary of up to 2^21 words, up to %d of " \
-                                            "them a row", name, kMaxWords)
+                                            "them a row", name, kMaxWords);                                       \
+  MOC_REQUIRE(temperature_ok(temperature), "%s: the temperature must be above 0", name)
 
-extern "C" int64_t moc_loss_targets_size(int64_t rows, int64_t words, int64_t vocab) {
-  if (!sizes_ok(rows, vocab, words)) return 0;
-  return targets_layout(rows, words, vocab, nullptr, nullptr);
+extern "C" int64_t moc_logits_loss_workspace_size(int64_t rows, int64_t words) {
+  if (!sizes_ok(rows, 1, words)) return 0;
+  Taken ws{nullptr};
+  Targets t{};
+  take_targets(ws, rows, words, 0, false, t);
+  ws.take<float>(rows);
+  return ws.at;
 }
 
-extern "C" int moc_label_targets(const int64_t* labels, int64_t rows, int64_t vocab, int64_t ignore_index,
-                                 const float* row_weight, int mean, const float* grad, void* targets, void* stream) {
-  const int64_t words = 0;
-  MOC_SIZES("moc_label_targets");
-  MOC_REQUIRE((labels != nullptr || rows == 0) && targets != nullptr && aligned16(targets),
-              "moc_label_targets: null operand or unaligned targets");
-  hipStream_t st = as_stream(stream);
-  Targets t;
-  targets_layout(rows, 0, vocab, static_cast<char*>(targets), &t);
-  label_targets_kernel<<<static_cast<unsigned>(1 + (rows + 1023) / 1024), 1024, 0, st>>>(
-      labels, rows, vocab, ignore_index, row_weight, mean, grad, t);
-  return check_launch("label_targets_kernel");
-}
-
-extern "C" int moc_teacher_targets(const void* ids, int ids_dtype, int64_t ids_ld, const void* top, int top_dtype,
-                                   int64_t top_ld, int64_t rows, int64_t words, int64_t vocab, float temperature,
-                                   const float* row_weight, int mean, const float* grad, void* targets,
-                                   void* stream) {
-  MOC_SIZES("moc_teacher_targets");
-  MOC_REQUIRE(words >= 1, "moc_teacher_targets: a word a row at least");
-  MOC_REQUIRE((ids_dtype == MOC_I32 || ids_dtype == MOC_I64) && (top_dtype == MOC_BF16 || top_dtype == MOC_F32),
-              "moc_teacher_targets: ids are int32 or int64, the teacher's logits bf16 or f32");
-  MOC_REQUIRE(temperature > 0.f && temperature < INFINITY, "moc_teacher_targets: the temperature must be above 0");
-  MOC_REQUIRE(rows == 0 || (ids != nullptr && top != nullptr && (rows == 1 || (ids_ld >= words && top_ld >= words))),
-              "moc_teacher_targets: null operand or rows that overlap");
-  MOC_REQUIRE(targets != nullptr && aligned16(targets), "moc_teacher_targets: null or unaligned targets");
-  hipStream_t st = as_stream(stream);
-  Targets t;
-  targets_layout(rows, words, vocab, static_cast<char*>(targets), &t);
-  if (rows > 0) {
-    const int k = static_cast<int>(words);
-#define MOC_TEACHER(ID, F)                                                                                            \
-  (k <= 64 ? teacher_wave_kernel<ID, F><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(                        \
-                 static_cast<const ID*>(ids), ids_ld, top, top_ld, rows, k, vocab, temperature, row_weight, t) \
-           : teacher_targets_kernel<ID, F><<<static_cast<unsigned>(rows), 256, 0, st>>>(                               \
-                 static_cast<const ID*>(ids), ids_ld, top, top_ld, k, vocab, temperature, row_weight, t))
-    if (ids_dtype == MOC_I32 && top_dtype == MOC_F32) MOC_TEACHER(int32_t, true);
-    else if (ids_dtype == MOC_I32) MOC_TEACHER(int32_t, false);
-    else if (top_dtype == MOC_F32) MOC_TEACHER(int64_t, true);
-    else MOC_TEACHER(int64_t, false);
-#undef MOC_TEACHER
-    const int rc = check_launch("teacher_targets_kernel");
-    if (rc != MOC_OK) return rc;
-  }
-  target_total_kernel<<<1, 1024, 0, st>>>(rows, mean, grad, t);
-  return check_launch("target_total_kernel");
-}
-
-extern "C" int moc_logits_loss(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t ld, void* targets,
-                               int64_t words, float temperature, float* row_loss, float* loss, void* dlogits,
-                               int64_t ldd, void* stream) {
+extern "C" int moc_logits_loss(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t ld, const void* ids,
+                               int ids_dtype, int64_t ids_ld, const void* top, int top_dtype, int64_t top_ld,
+                               int64_t words, float temperature, const float* row_weight, int mean, const float* grad,
+                               float* row_loss, float* loss, void* dlogits, int64_t ldd, void* workspace,
+                               int64_t workspace_bytes, void* counters, void* stream) {
   MOC_SIZES("moc_logits_loss");
   MOC_REQUIRE(dtype == MOC_BF16 || dtype == MOC_F32, "moc_logits_loss: logits are bf16 or f32");
-  MOC_REQUIRE(temperature > 0.f && temperature < INFINITY, "moc_logits_loss: the temperature must be above 0");
-  MOC_REQUIRE(targets != nullptr && (rows == 0 || (logits != nullptr && row_loss != nullptr)),
-              "moc_logits_loss: null operand");
+  MOC_REQUIRE(words >= 1, "moc_logits_loss: a word a row at least");
+  const Teacher a{ids, ids_dtype, ids_ld, top, top_dtype, top_ld, temperature};
+  int rc = teacher_ok("moc_logits_loss", a, rows, words);
+  if (rc != MOC_OK) return rc;
+  MOC_REQUIRE(rows == 0 || logits != nullptr, "moc_logits_loss: null logits");
   MOC_REQUIRE(rows <= 1 || (ld >= vocab && (dlogits == nullptr || ldd >= vocab)), "moc_logits_loss: rows that overlap");
+  Taken ws{static_cast<char*>(workspace)};
+  Targets t{};
+  take_targets(ws, rows, words, 0, false, t);
+  float* each = ws.take<float>(rows);
+  MOC_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= ws.at && counters != nullptr &&
+                  aligned16(counters),
+              "moc_logits_loss: counters and a workspace of %lld bytes needed", (long long)ws.at);
+  if (row_loss == nullptr) row_loss = each;
   hipStream_t st = as_stream(stream);
-  Targets t;
-  targets_layout(rows, words, vocab, static_cast<char*>(targets), &t);
-  const bool f32 = dtype == MOC_F32;
-  int rc = logits_rows(f32, logits, rows, vocab, ld, t, words, temperature, row_loss, dlogits, ldd, st);
-  if (rc != MOC_OK || loss == nullptr) return rc;
-  loss_sum_kernel<<<1, 1024, 0, st>>>(row_loss, rows, t.total, loss);
-  return check_launch("loss_sum_kernel");
+  int* count = static_cast<int*>(counters);
+  const bool total = dlogits != nullptr && rows > 0;
+  rc = run_teacher(a, rows, words, vocab, row_weight, mean, grad, t, total, count, st);
+  if (rc != MOC_OK) return rc;
+  const bool arrive = rows > 0 && rows <= kArriveRows;
+  const LossOut o{row_loss, arrive ? loss : nullptr, rows, mean, total, count + kLossCounter};
+  if (rows > 0) {
+    rc = logits_rows(dtype == MOC_F32, logits, rows, vocab, ld, t, 0, words, temperature, o, dlogits, ldd, st);
+    if (rc != MOC_OK) return rc;
+  }
+  return loss == nullptr || arrive ? MOC_OK : sum_loss(t, o, loss, st);
 }
 
 extern "C" int64_t moc_linear_loss_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab,
                                                   int64_t words, int grads) {
   if (!sizes_ok(rows, vocab, words) || hidden < 1) return 0;
-  return pieces_of(dtype, rows, hidden, vocab, words, grads != 0).bytes;
+  return pieces_of(dtype, rows, hidden, vocab, words, grads != 0, nullptr).bytes;
 }
 
 extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab,
                                                        int grads) {
-  if (!sizes_ok(rows, vocab, 0) || hidden < 1) return 0;
-  const Pieces p = pieces_of(dtype, rows, hidden, vocab, 0, grads != 0);
-  int64_t most = 0;
+  int64_t most = MOC_GEMM_WS_COUNTER_BYTES;
+  if (!sizes_ok(rows, vocab, 0) || hidden < 1) return most;
+  const Pieces p = pieces_of(dtype, rows, hidden, vocab, 0, grads != 0, nullptr);
+  auto need = [&](int64_t b) { most = b > most ? b : most; };
   for (int64_t i = 0; i < p.count; i += p.count > 1 ? p.count - 1 : 1) {  // the first piece and the last
     const int64_t n = i + 1 < p.count ? p.rows : rows - i * p.rows;
-    int64_t b = p.fused ? 0 : moc_gemm_workspace_size(dtype, n, vocab, hidden, 0);
-    if (b > most) most = b;
+    if (!p.fused) need(moc_gemm_workspace_size(dtype, n, vocab, hidden, 0));
     if (!grads) continue;
-    b = p.fused ? gemm_half_workspace(n, hidden, vocab) : moc_gemm_workspace_size(dtype, n, hidden, vocab, 0);
-    if (b > most) most = b;
-    b = p.fused ? gemm_half_workspace(vocab, hidden, n) : moc_gemm_workspace_size(dtype, vocab, hidden, n, 0);
-    if (b > most) most = b;
+    need(p.fused ? gemm_half_workspace(n, hidden, vocab) : moc_gemm_workspace_size(dtype, n, hidden, vocab, 0));
+    need(p.fused ? gemm_half_workspace(vocab, hidden, n) : moc_gemm_workspace_size(dtype, vocab, hidden, n, 0));
   }
   return most;
 }
 
 extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w,
-                               int64_t vocab, int64_t ldw, void* targets, int64_t words, float temperature,
+                               int64_t vocab, int64_t ldw, const int64_t* labels, int64_t ignore_index, const void* ids,
+                               int ids_dtype, int64_t ids_ld, const void* top, int top_dtype, int64_t top_ld,
+                               int64_t words, float temperature, const float* row_weight, int mean, const float* grad,
                                float* row_loss, float* loss, void* dh, int dh_dtype, void* dw, int dw_dtype,
                                void* workspace, int64_t workspace_bytes, void* gemm_ws, int64_t gemm_ws_bytes,
                                void* stream) {
@@ -1172,9 +1361,13 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
   const bool f32 = dtype == MOC_F32;
   const int es = f32 ? 4 : 2;
   MOC_REQUIRE(hidden >= 1 && hidden <= (1 << 20), "moc_linear_loss: hidden size of 1 to 2^20");
-  MOC_REQUIRE(temperature > 0.f && temperature < INFINITY, "moc_linear_loss: the temperature must be above 0");
-  MOC_REQUIRE(targets != nullptr && w != nullptr && (rows == 0 || (h != nullptr && row_loss != nullptr)),
-              "moc_linear_loss: null operand");
+  MOC_REQUIRE(w != nullptr && (rows == 0 || h != nullptr), "moc_linear_loss: null operand");
+  const Teacher a{ids, ids_dtype, ids_ld, top, top_dtype, top_ld, temperature};
+  int rc = MOC_OK;
+  if (words > 0) rc = teacher_ok("moc_linear_loss", a, rows, words);
+  if (rc != MOC_OK) return rc;
+  MOC_REQUIRE(words > 0 || labels != nullptr || rows == 0, "moc_linear_loss: null labels");
+  MOC_REQUIRE(words > 0 || temperature == 1.f, "moc_linear_loss: labels have the temperature 1");
   MOC_REQUIRE(aligned16(h) && aligned16(w) && ldh * es % 16 == 0 && ldw * es % 16 == 0 && ldh >= hidden &&
                   ldw >= hidden,
               "moc_linear_loss: operands need 16-byte aligned rows");
@@ -1183,110 +1376,120 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
                   (dw == nullptr || (dw_dtype == MOC_F32 || (dw_dtype == MOC_BF16 && !f32))),
               "moc_linear_loss: gradients are f32, or bf16 of bf16 operands");
   const bool grads = dh != nullptr || dw != nullptr;
-  const Pieces p = pieces_of(dtype, rows, hidden, vocab, words, grads);
-  MOC_REQUIRE(workspace_bytes >= p.bytes && (workspace != nullptr || p.bytes == 0) && aligned16(workspace),
-              "moc_linear_loss: workspace of %lld bytes needed", (long long)p.bytes);
-  MOC_REQUIRE(f32 || p.rows * p.ldx * 2 < (1LL << 31) - 1024, "moc_linear_loss: hidden rows of a piece up to 2 GiB");
+  Pieces p = pieces_of(dtype, rows, hidden, vocab, words, grads, workspace);
+  MOC_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= p.bytes && gemm_ws != nullptr &&
+                  gemm_ws_bytes >= MOC_GEMM_WS_COUNTER_BYTES && aligned16(gemm_ws),
+              "moc_linear_loss: workspaces of %lld and at least %d bytes needed", (long long)p.bytes,
+              MOC_GEMM_WS_COUNTER_BYTES);
+  const int64_t ld_most = ldh > p.ldx ? ldh : p.ldx, ldv_most = ldw > p.ldx ? ldw : p.ldx;
+  MOC_REQUIRE(f32 || (p.rows * ld_most * 2 < (1LL << 31) - 1024 && vocab * ldv_most * 2 < (1LL << 31) - 1024),
+              "moc_linear_loss: operands of up to 2 GiB a piece");
   hipStream_t st = as_stream(stream);
-  Targets t;
-  targets_layout(rows, words, vocab, static_cast<char*>(targets), &t);
-  char* ws = static_cast<char*>(workspace);
+  int* count = static_cast<int*>(gemm_ws);
+  Targets& t = p.t;
+  if (words == 0) {
+    t.labels = labels;
+    t.ignore = ignore_index;
+    t.row_weight = row_weight;
+  }
+  if (row_loss == nullptr) row_loss = p.row_loss;
   const int64_t n_words = words > 0 ? words : 1;
-  int rc;
+  if (words > 0) {
+    rc = run_teacher(a, rows, words, vocab, row_weight, mean, grad, t, grads && f32, count, st);
+    if (rc != MOC_OK) return rc;
+  }
+  const bool table = p.fused && words > 0 && rows > 0;
+  const unsigned table_blocks = table ? static_cast<unsigned>((rows + 15) / 16) : 0;
+  if (table && !grads) {
+    words_left_kernel<<<table_blocks, 256, 0, st>>>(t, rows, (int)words, (int)p.slabs);
+    if ((rc = check_launch("words_left_kernel")) != MOC_OK) return rc;
+  }
+  const Halves hx{static_cast<const uint16_t*>(h), ldh, rows, dw != nullptr ? reinterpret_cast<_Float16*>(p.x) : nullptr,
+                  0x1p2f, 0x1p-3f, 0x1p13f};
+  const Halves hw{static_cast<const uint16_t*>(w), ldw, vocab, dh != nullptr ? reinterpret_cast<_Float16*>(p.w) : nullptr,
+                  0x1p6f, 0x1p-7f, 0x1p9f};
+  int halves = 0;
   if (grads && rows > 0 && f32) {
+    if (words == 0) {
+      target_total_kernel<<<1, 1024, 0, st>>>(rows, mean, grad, t);
+      if ((rc = check_launch("target_total_kernel")) != MOC_OK) return rc;
+    }
     counted_rows_kernel<<<blocks_of(rows * ((hidden + 3) / 4)), 256, 0, st>>>(
-        static_cast<const float*>(h), ldh, rows, (int)hidden, t.weight, reinterpret_cast<float*>(ws + p.x), p.ldx);
+        static_cast<const float*>(h), ldh, rows, (int)hidden, t, reinterpret_cast<float*>(p.x), p.ldx);
     if ((rc = check_launch("counted_rows_kernel")) != MOC_OK) return rc;
   } else if (grads && rows > 0) {
-    const Halves hx{static_cast<const uint16_t*>(h), ldh, rows,
-                    dw != nullptr ? reinterpret_cast<_Float16*>(ws + p.x) : nullptr, 0x1p2f, 0x1p-3f, 0x1p13f};
-    const Halves hw{static_cast<const uint16_t*>(w), ldw, vocab,
-                    dh != nullptr ? reinterpret_cast<_Float16*>(ws + p.w) : nullptr, 0x1p6f, 0x1p-7f, 0x1p9f};
-    const unsigned grid = blocks_of((rows > vocab ? rows : vocab) * 16);  // four waves of four rows
-    uint32_t* most = reinterpret_cast<uint32_t*>(ws + p.most);
-    halves_kernel<<<grid, 256, 0, st>>>(hx, hw, (int)hidden, p.ldx, t, most);
+    const int64_t want = ((rows > vocab ? rows : vocab) + 15) / 16;  // four waves of four rows
+    halves = static_cast<int>(want < kHalvesBlocks ? want : kHalvesBlocks);
+    halves_kernel<<<1 + table_blocks + halves, 256, 0, st>>>(hx, hw, (int)hidden, p.ldx, t, rows, mean, grad, (int)words,
+                                                             (int)p.slabs, p.most, halves);
     if ((rc = check_launch("halves_kernel")) != MOC_OK) return rc;
-    halves_again_kernel<<<grid < 512 ? grid : 512, 256, 0, st>>>(hx, hw, (int)hidden, p.ldx, temperature, t, most,
-                                                                 (int)grid);
-    if ((rc = check_launch("halves_again_kernel")) != MOC_OK) return rc;
-  }
-  if (p.fused && words > 0 && rows > 0) {
-    words_left_kernel<<<static_cast<unsigned>((rows + 63) / 64), 1024,
-                        words <= kWordsLds ? 64 * (words | 1) * 4 : 0, st>>>(t.ids, rows, (int)words, (int)p.slabs,
-                                                                             t.first);
-    if ((rc = check_launch("words_left_kernel")) != MOC_OK) return rc;
   }
   // f32: the rows that count in every product; bf16: in dweight's alone, as nothing is
   // read of the others' logits
   const bool copied = grads && f32;
-  const char* x = copied ? ws + p.x : static_cast<const char*>(h);
+  const char* x = copied ? p.x : static_cast<const char*>(h);
   const int64_t ldx = copied ? p.ldx : ldh;
+  // a label is one word, the low half of its int64
+  const int32_t* word_ids = words > 0 ? t.ids : reinterpret_cast<const int32_t*>(labels);
+  const int64_t ld_ids = words > 0 ? words : 2;
+  const bool arrive = p.count == 1 && rows <= kArriveRows;
+  const LossOut o{row_loss, arrive ? loss : nullptr, rows, mean, grads && rows > 0, count + kLossCounter};
   for (int64_t i = 0; i < p.count; ++i) {
     const int64_t r0 = i * p.rows, n = rows - r0 < p.rows ? rows - r0 : p.rows;
     const char* xi = x + r0 * ldx * es;
-    Targets ti = t;
-    ti.weight += r0;
-    ti.ids += r0 * n_words;
-    if (words > 0) {
-      ti.entropy += r0;
-      ti.share += r0 * words;
-      ti.first += r0;
-    }
     if (p.fused) {
-      float2* stat = reinterpret_cast<float2*>(ws + p.stat);
-      float* z = reinterpret_cast<float*>(ws + p.at_words);
-      const bool few = !grads && n <= kFewRows && hidden % 8 == 0 && hidden <= kFewHidden;
-      rc = few ? launch_few(xi, n, hidden, ldx, w, vocab, ldw, kLog2E / temperature, ti, rows, words, z, stat, p.slabs, st)
-               : launch_loss_gemm(xi, n, hidden, ldx, w, vocab, ldw, kLog2E / temperature, ti.ids,
-                            words > 0 ? ti.first : nullptr, rows, n_words, z, stat, grads ? ws + p.d : nullptr, p.ldz, st);
+      const uint16_t* first = words > 0 ? t.first + r0 : nullptr;
+      const float unit = kLog2E / temperature;
+      if (!grads && n <= kFewRows && hidden % 8 == 0 && hidden <= kFewHidden)
+        rc = launch_few(xi, n, hidden, ldx, w, vocab, ldw, unit, word_ids + r0 * ld_ids, ld_ids, first, rows, n_words, p.z,
+                        p.stat, p.slabs, st);
+      else
+        rc = launch_loss_gemm(xi, n, hidden, ldx, w, vocab, ldw, unit, word_ids + r0 * ld_ids, ld_ids, first, rows, n_words,
+                              p.z, p.stat, grads ? p.d : nullptr, p.ldz, st);
       MOC_REQUIRE(rc <= 0, "moc_linear_loss: operands of up to 2 GiB");
       if (rc != MOC_OK) return rc;
+      const Slabs s{p.stat, p.z, (int)p.slabs, (int)vocab, (int)words, r0, temperature};
       if (grads)
-        slabs_grad_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(
-            reinterpret_cast<uint16_t*>(ws + p.d), p.ldz, (int)vocab, stat, (int)p.slabs, ti, (int)words, temperature, z,
-            row_loss + r0);
+        slabs_grad_kernel<<<static_cast<unsigned>(n) + (i == 0 ? kAgainBlocks : 0), 256, 0, st>>>(
+            reinterpret_cast<uint16_t*>(p.d), p.ldz, s, t, o, hx, hw, (int)hidden, p.ldx, p.most, halves);
       else
-        slabs_loss_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(stat, (int)p.slabs, ti, (int)words, temperature, z,
-                                                                    row_loss + r0);
+        slabs_loss_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(s, t, o);
       rc = check_launch("slabs_grad_kernel");
     } else {
-      rc = moc_gemm_ws(dtype, n, vocab, hidden, xi, ldx, 1, w, 1, ldw, 0, nullptr, 0, 0, nullptr, 0, 0, ws + p.z, p.ldz,
+      rc = moc_gemm_ws(dtype, n, vocab, hidden, xi, ldx, 1, w, 1, ldw, 0, nullptr, 0, 0, nullptr, 0, 0, p.d, p.ldz,
                        MOC_F32, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
-      rc = logits_rows(true, ws + p.z, n, vocab, p.ldz, ti, words, temperature, row_loss + r0,
-                       grads ? ws + p.d : nullptr, p.ldz, st);
+      rc = logits_rows(true, p.d, n, vocab, p.ldz, t, r0, words, temperature, o, grads ? p.d : nullptr, p.ldz, st);
     }
     if (rc != MOC_OK) return rc;
     if (dh != nullptr) {
       char* to = static_cast<char*>(dh) + r0 * hidden * (dh_dtype == MOC_F32 ? 4 : 2);
-      const char* b = p.fused ? ws + p.w : static_cast<const char*>(w);
-      rc = vocab == 1 ? outer(f32, n, hidden, ws + p.d, p.ldz, b, t.alpha, to, dh_dtype, st)
-           : p.fused  ? gemm_half(n, hidden, vocab, ws + p.d, p.ldz, 1, b, p.ldx, to, hidden, dh_dtype, t.alpha, gemm_ws,
+      const char* b = p.fused ? p.w : static_cast<const char*>(w);
+      rc = vocab == 1 ? outer(f32, n, hidden, p.d, p.ldz, b, t.alpha, to, dh_dtype, st)
+           : p.fused  ? gemm_half(n, hidden, vocab, p.d, p.ldz, 1, b, p.ldx, to, hidden, dh_dtype, t.alpha, gemm_ws,
                                   gemm_ws_bytes, stream)
-                      : moc_gemm_ws(dtype, n, hidden, vocab, ws + p.d, p.ldz, 1, b, ldw, 1, 0, nullptr, 0, 0, nullptr, 0,
-                                    0, to, hidden, dh_dtype, gemm_ws, gemm_ws_bytes, stream);
+                      : moc_gemm_ws(dtype, n, hidden, vocab, p.d, p.ldz, 1, b, ldw, 1, 0, nullptr, 0, 0, nullptr, 0, 0, to,
+                                    hidden, dh_dtype, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
     }
     if (dw != nullptr) {
       const bool one = p.count == 1;
-      char* to = one ? static_cast<char*>(dw) : ws + (i == 0 ? p.acc : p.part);
+      char* to = one ? static_cast<char*>(dw) : reinterpret_cast<char*>(i == 0 ? p.acc : p.part);
       const int to_dtype = one ? dw_dtype : MOC_F32;
-      const char* b = ws + p.x + r0 * p.ldx * es;
-      rc = n == 1    ? outer(f32, vocab, hidden, ws + p.d, 1, b, t.alpha + 1, to, to_dtype, st)
-           : p.fused ? gemm_half(vocab, hidden, n, ws + p.d, 1, p.ldz, b, p.ldx, to, hidden, to_dtype, t.alpha + 1,
-                                 gemm_ws, gemm_ws_bytes, stream)
-                     : moc_gemm_ws(dtype, vocab, hidden, n, ws + p.d, 1, p.ldz, b, p.ldx, 1, 0, nullptr, 0, 0, nullptr, 0,
-                                   0, to, hidden, to_dtype, gemm_ws, gemm_ws_bytes, stream);
+      const char* b = p.x + r0 * p.ldx * es;
+      rc = n == 1    ? outer(f32, vocab, hidden, p.d, 1, b, t.alpha + 1, to, to_dtype, st)
+           : p.fused ? gemm_half(vocab, hidden, n, p.d, 1, p.ldz, b, p.ldx, to, hidden, to_dtype, t.alpha + 1, gemm_ws,
+                                 gemm_ws_bytes, stream)
+                     : moc_gemm_ws(dtype, vocab, hidden, n, p.d, 1, p.ldz, b, p.ldx, 1, 0, nullptr, 0, 0, nullptr, 0, 0, to,
+                                   hidden, to_dtype, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
       if (i > 0) {
-        float* acc = reinterpret_cast<float*>(ws + p.acc);
-        const float* part = reinterpret_cast<const float*>(ws + p.part);
         const int64_t size = vocab * hidden;
         void* out = i + 1 == p.count ? dw : nullptr;
         if (dw_dtype == MOC_F32)
-          add_f32_kernel<float><<<blocks_of(size), 256, 0, st>>>(acc, part, size, static_cast<float*>(out));
+          add_f32_kernel<float><<<blocks_of(size), 256, 0, st>>>(p.acc, p.part, size, static_cast<float*>(out));
         else
-          add_f32_kernel<uint16_t><<<blocks_of(size), 256, 0, st>>>(acc, part, size, static_cast<uint16_t*>(out));
+          add_f32_kernel<uint16_t><<<blocks_of(size), 256, 0, st>>>(p.acc, p.part, size, static_cast<uint16_t*>(out));
         if ((rc = check_launch("add_f32_kernel")) != MOC_OK) return rc;
       }
     }
@@ -1295,9 +1498,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     rc = moc_fill_zero(dw, vocab * hidden * (dw_dtype == MOC_F32 ? 4 : 2), stream);
     if (rc != MOC_OK) return rc;
   }
-  if (loss == nullptr) return MOC_OK;
-  loss_sum_kernel<<<1, 1024, 0, st>>>(row_loss, rows, t.total, loss);
-  return check_launch("loss_sum_kernel");
+  return loss == nullptr || (rows > 0 && arrive) ? MOC_OK : sum_loss(t, o, loss, st);
 }
 
 extern "C" int moc_scale_inplace(int dtype0, void* p0, int64_t n0, int dtype1, void* p1, int64_t n1,

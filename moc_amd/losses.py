@@ -29,6 +29,7 @@ products are those of bf16 casts and gradients come in the operands' own types.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 
 import torch
 
@@ -38,6 +39,7 @@ from .block import graph_grads, plain
 
 BF16, F32 = torch.bfloat16, torch.float32
 REDUCTIONS = ("mean", "sum", "none")
+COUNTER_BYTES = 4096  # MOC_GEMM_WS_COUNTER_BYTES
 
 
 def linear_cross_entropy(hidden, weight, labels, row_weight=None, *, ignore_index: int = -100,
@@ -110,13 +112,9 @@ class _Labels:
     def tensors(self):
         return self.labels, None, self.row_weight
 
-    def write(self, saved, row_weight, mean: bool, grad, vocab: int, dev) -> torch.Tensor:
-        labels = saved[0]
-        rows = labels.shape[0]
-        out = torch.empty(N.query("moc_loss_targets_size", rows, 0, vocab), dtype=torch.uint8, device=labels.device)
-        N.call("moc_label_targets", labels.data_ptr(), rows, vocab, self.ignore, N.ptr(row_weight), mean,
-               N.ptr(grad), out.data_ptr(), N.stream_on(dev))
-        return out
+    def given(self, saved):
+        """moc_linear_loss's arguments from labels to temperature."""
+        return saved[0].data_ptr(), self.ignore, None, N.MOC_I32, 0, None, N.MOC_F32, 0, 0, 1.0
 
     def rows_f32(self, saved, z):
         """Each row's loss by f32 tensor operations, and whether it counts."""
@@ -136,14 +134,11 @@ class _Teacher:
     def tensors(self):
         return self.ids, self.top, self.row_weight
 
-    def write(self, saved, row_weight, mean: bool, grad, vocab: int, dev) -> torch.Tensor:
+    def given(self, saved):
+        """moc_linear_loss's arguments from labels to temperature."""
         ids, top, _ = saved
-        rows, words = ids.shape
-        out = torch.empty(N.query("moc_loss_targets_size", rows, words, vocab), dtype=torch.uint8, device=ids.device)
-        N.call("moc_teacher_targets", ids.data_ptr(), N.idx_code(ids.dtype), ids.stride(0), top.data_ptr(),
-               N.dtype_code(top.dtype), top.stride(0), rows, words, vocab, self.heat, N.ptr(row_weight), mean,
-               N.ptr(grad), out.data_ptr(), N.stream_on(dev))
-        return out
+        return (None, 0, ids.data_ptr(), N.idx_code(ids.dtype), ids.stride(0), top.data_ptr(), N.dtype_code(top.dtype),
+                top.stride(0), self.words, self.heat)
 
     def rows_f32(self, saved, z):
         ids, top, _ = saved
@@ -233,28 +228,46 @@ def _linear(what: str, hidden, weight, targets) -> torch.Tensor:
     return _LinearLoss.apply(targets, product, torch.is_grad_enabled(), hidden, weight, *targets.tensors())
 
 
-def _linear_pass(targets, saved, row_weight, mean, grad, product, hidden, weight, loss: bool, dh: bool, dw: bool):
-    """(loss | None, the rows' losses, dhidden | None, dweight | None)."""
-    dev = hidden.get_device()
+@lru_cache(maxsize=256)
+def _linear_sizes(code: int, rows: int, d: int, vocab: int, words: int, grads: bool) -> tuple[int, int]:
+    """(workspace, GEMM workspace) bytes of a shape."""
+    return (N.query("moc_linear_loss_workspace_size", code, rows, d, vocab, words, grads),
+            N.query("moc_linear_loss_gemm_workspace_size", code, rows, d, vocab, grads))
+
+
+def _counted_workspace(device, nbytes: int) -> torch.Tensor:
+    """A GEMM workspace, its counters zero: the stream's, or one of the graph's own
+    under capture, since two graphs that were captured on one stream may run beside
+    each other."""
+    if not torch.cuda.is_current_stream_capturing():
+        return K._gemm_workspace(device, nbytes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    N.call("moc_fill_zero", ws.data_ptr(), COUNTER_BYTES, N.stream_of(ws))
+    return ws
+
+
+def _linear_pass(targets, saved, row_weight, mean, grad, product, hidden, weight, each: bool, dh: bool, dw: bool):
+    """(the loss, or with `each` the rows' losses; dhidden | None; dweight | None)."""
+    dev, where = hidden.get_device(), hidden.device
     vocab, d = weight.shape
-    h = _rows16(hidden.reshape(-1, d).to(product))
-    w = _rows16(weight.to(product))
-    rows, grads = h.shape[0], dh or dw
-    code = N.dtype_code(product)
-    where = hidden.device
-    t = targets.write(saved, row_weight, mean, grad, vocab, dev)
-    each = torch.empty(rows, dtype=F32, device=where)
-    total = torch.empty((), dtype=F32, device=where) if loss else None
+    h, w = hidden.reshape(-1, d), weight
+    if h.dtype != product:
+        h = h.to(product)
+    if w.dtype != product:
+        w = w.to(product)
+    h, w = _rows16(h), _rows16(w)
+    rows, code = h.shape[0], N.dtype_code(product)
+    out = torch.empty(rows if each else (), dtype=F32, device=where)
     dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=where) if dh else None
     dweight = torch.empty((vocab, d), dtype=weight.dtype, device=where) if dw else None
-    nbytes = N.query("moc_linear_loss_workspace_size", code, rows, d, vocab, targets.words, grads)
+    nbytes, ngemm = _linear_sizes(code, rows, d, vocab, targets.words, dh or dw)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
-    ngemm = N.query("moc_linear_loss_gemm_workspace_size", code, rows, d, vocab, grads)
-    gemm_ws = K._gemm_workspace(where, ngemm) if ngemm else None
-    N.call("moc_linear_loss", code, h.data_ptr(), rows, d, _pitch(h), w.data_ptr(), vocab, _pitch(w), t.data_ptr(),
-           targets.words, targets.heat, each.data_ptr(), N.ptr(total), N.ptr(dhidden), N.dtype_code(hidden.dtype),
-           N.ptr(dweight), N.dtype_code(weight.dtype), ws.data_ptr(), nbytes, N.ptr(gemm_ws), ngemm, N.stream_on(dev))
-    return total, each, dhidden, dweight
+    gemm_ws = _counted_workspace(where, ngemm)
+    N.call("moc_linear_loss", code, h.data_ptr(), rows, d, _pitch(h), w.data_ptr(), vocab, _pitch(w),
+           *targets.given(saved), N.ptr(row_weight), mean, N.ptr(grad), out.data_ptr() if each else None,
+           None if each else out.data_ptr(), N.ptr(dhidden), N.dtype_code(hidden.dtype), N.ptr(dweight),
+           N.dtype_code(weight.dtype), ws.data_ptr(), nbytes, gemm_ws.data_ptr(), ngemm, N.stream_on(dev))
+    return out, dhidden, dweight
 
 
 def _reduced_f32(targets, saved, z):
@@ -277,8 +290,8 @@ class _Kept:
         self.captured = torch.cuda.is_current_stream_capturing()
 
     def take(self, g):
-        """The gradients times g, or None: gone, or those of an eager forward in a
-        captured backward, which a replay would scale again."""
+        """The gradients times g, or None: there are none, or no more, or those of an
+        eager forward in a captured backward, which a replay would scale again."""
         grads, self.grads = self.grads, None
         if grads is None or (torch.cuda.is_current_stream_capturing() and not self.captured):
             return None
@@ -289,7 +302,7 @@ class _Kept:
         return grads
 
 
-def _row_factors(targets, saved, g):
+def _row_factors(saved, g):
     """reduction="none": the rows' weights times their upstream gradients."""
     g = g.reshape(-1).contiguous()
     return g if saved[2] is None else g * saved[2]
@@ -298,80 +311,85 @@ def _row_factors(targets, saved, g):
 class _LinearLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, targets, product, grad_mode, hidden, weight, *saved):
-        dh, dw = (grad_mode and need for need in ctx.needs_input_grad[3:5])
-        ahead = targets.reduction != "none"
-        total, each, dhidden, dweight = _linear_pass(targets, saved, saved[2], targets.reduction == "mean", None, product,
-                                                     hidden, weight, ahead, ahead and dh, ahead and dw)
+        needs = ctx.needs_input_grad
+        dh, dw = grad_mode and needs[3], grad_mode and needs[4]
+        each = targets.reduction == "none"
+        out, *grads = _linear_pass(targets, saved, saved[2], targets.reduction == "mean", None, product, hidden, weight,
+                                   each, dh and not each, dw and not each)
         if dh or dw:
             ctx.save_for_backward(hidden, weight, *saved)
             ctx.targets, ctx.product = targets, product
-            ctx.kept = _Kept((dhidden, dweight) if ahead else None)
-        return total if ahead else each.view(hidden.shape[:-1])
+            ctx.kept = _Kept(None if each else grads)
+        return out.view(hidden.shape[:-1]) if each else out
 
     @staticmethod
     def backward(ctx, g):
+        rest = None, None, None
+        if not torch.is_grad_enabled() and (kept := ctx.kept.take(g)):
+            return (None, None, None, *kept, *rest)
         hidden, weight, *saved = ctx.saved_tensors
         targets = ctx.targets
         dh, dw = ctx.needs_input_grad[3:5]
-        rest = (None,) * len(saved)
         if torch.is_grad_enabled():
             def stock(h, w):
                 z = (h.to(ctx.product).float() @ w.to(ctx.product).float().t()).reshape(-1, w.shape[0])
-                out = _reduced_f32(targets, saved, z)
-                return out.reshape(g.shape)
+                return _reduced_f32(targets, saved, z).reshape(g.shape)
             return (None, None, None, *graph_grads(stock, (hidden, weight), (dh, dw), g), *rest)
         if targets.reduction == "none":
-            got = _linear_pass(targets, saved, _row_factors(targets, saved, g), False, None, ctx.product, hidden, weight,
-                               False, dh, dw)[2:]
+            got = _linear_pass(targets, saved, _row_factors(saved, g), False, None, ctx.product, hidden, weight, True, dh,
+                               dw)
         else:
-            got = ctx.kept.take(g) or _linear_pass(targets, saved, saved[2], targets.reduction == "mean", g, ctx.product,
-                                                   hidden, weight, False, dh, dw)[2:]
-        return (None, None, None, *got, *rest)
+            got = _linear_pass(targets, saved, saved[2], targets.reduction == "mean", g, ctx.product, hidden, weight, False,
+                               dh, dw)
+        return (None, None, None, *got[1:], *rest)
 
 
-def _logits_pass(targets, saved, row_weight, mean, grad, logits, loss: bool, grads: bool):
-    """(loss | None, the rows' losses, dlogits | None)."""
-    dev = logits.get_device()
+def _logits_pass(targets, saved, row_weight, mean, grad, logits, each: bool, grads: bool):
+    """(the loss, or with `each` the rows' losses; dlogits | None)."""
+    dev, where = logits.get_device(), logits.device
     vocab = logits.shape[-1]
     x = logits.reshape(-1, vocab)
     if (x.stride(1) != 1 and vocab > 1) or (x.shape[0] > 1 and x.stride(0) < vocab):
         x = x.contiguous()
     rows = x.shape[0]
-    t = targets.write(saved, row_weight, mean, grad, vocab, dev)
-    each = torch.empty(rows, dtype=F32, device=x.device)
-    total = torch.empty((), dtype=F32, device=x.device) if loss else None
-    dx = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if grads else None
+    out = torch.empty(rows if each else (), dtype=F32, device=where)
+    dx = torch.empty(logits.shape, dtype=x.dtype, device=where) if grads else None
+    nbytes = N.query("moc_logits_loss_workspace_size", rows, targets.words)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
+    counters = _counted_workspace(where, COUNTER_BYTES)
     N.call("moc_logits_loss", N.dtype_code(x.dtype), x.data_ptr(), rows, vocab, x.stride(0) if rows > 1 else vocab,
-           t.data_ptr(), targets.words, targets.heat, each.data_ptr(), N.ptr(total), N.ptr(dx), vocab, N.stream_on(dev))
-    return total, each, dx
+           *targets.given(saved)[2:], N.ptr(row_weight), mean, N.ptr(grad), out.data_ptr() if each else None,
+           None if each else out.data_ptr(), N.ptr(dx), vocab, ws.data_ptr(), nbytes, counters.data_ptr(),
+           N.stream_on(dev))
+    return out, dx
 
 
 class _LogitsLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, targets, grad_mode, logits, *saved):
         need = grad_mode and ctx.needs_input_grad[2]
-        ahead = targets.reduction != "none"
-        total, each, dx = _logits_pass(targets, saved, saved[2], targets.reduction == "mean", None, logits, ahead,
-                                       ahead and need)
+        each = targets.reduction == "none"
+        out, dx = _logits_pass(targets, saved, saved[2], targets.reduction == "mean", None, logits, each,
+                               need and not each)
         if need:
             ctx.save_for_backward(logits, *saved)
             ctx.targets = targets
-            ctx.kept = _Kept((dx,) if ahead else None)
-        return total if ahead else each.view(logits.shape[:-1])
+            ctx.kept = _Kept(None if each else (dx,))
+        return out.view(logits.shape[:-1]) if each else out
 
     @staticmethod
     def backward(ctx, g):
+        rest = None, None, None
+        if not torch.is_grad_enabled() and (kept := ctx.kept.take(g)):
+            return (None, None, *kept, *rest)
         logits, *saved = ctx.saved_tensors
         targets = ctx.targets
-        rest = (None,) * len(saved)
         if torch.is_grad_enabled():
             def stock(x):
                 return _reduced_f32(targets, saved, x.float().reshape(-1, x.shape[-1])).reshape(g.shape)
             return (None, None, *graph_grads(stock, (logits,), (True,), g), *rest)
         if targets.reduction == "none":
-            dx = _logits_pass(targets, saved, _row_factors(targets, saved, g), False, None, logits, False, True)[2]
+            dx = _logits_pass(targets, saved, _row_factors(saved, g), False, None, logits, True, True)[1]
         else:
-            kept = ctx.kept.take(g)
-            dx = kept[0] if kept else _logits_pass(targets, saved, saved[2], targets.reduction == "mean", g, logits,
-                                                   False, True)[2]
+            dx = _logits_pass(targets, saved, saved[2], targets.reduction == "mean", g, logits, False, True)[1]
         return (None, None, dx, *rest)

@@ -68,30 +68,30 @@ def test_entry_points_refuse():
     """The library's own checks, before any device work: none of these pointers is read."""
     lib = N.load()
     p = ctypes.c_void_p(4096)
+    null, teacher = (None, 1, 0, None, 1, 0), (p, 1, 4, p, 1, 4)  # ids, dtype, ld, top, dtype, ld
+
+    def logits(dtype=0, x=p, rows=3, vocab=10, ld=10, by=teacher, words=4, heat=1.0, ldd=10, ws=p, size=1 << 40,
+               counters=p):
+        return "moc_logits_loss", (dtype, x, rows, vocab, ld, *by, words, heat, None, 1, None, None, p, p, ldd, ws, size,
+                                   counters, None)
+
+    def linear(dtype=0, h=p, rows=3, d=8, ldh=8, w=p, vocab=10, ldw=8, labels=p, by=null, words=0, heat=1.0, dh=p,
+               dh_dtype=0, ws=p, size=1 << 40, gws=p, gsize=1 << 30):
+        return "moc_linear_loss", (dtype, h, rows, d, ldh, w, vocab, ldw, labels, -100, *by, words, heat, None, 1, None,
+                                   None, p, dh, dh_dtype, None, 0, ws, size, gws, gsize, None)
+
     bad = [
-        ("moc_label_targets", (None, 4, 10, -100, None, 1, None, p, None)),
-        ("moc_label_targets", (p, 4, 10, -100, None, 1, None, None, None)),
-        ("moc_label_targets", (p, 4, 0, -100, None, 1, None, p, None)),
-        ("moc_label_targets", (p, 4, (1 << 21) + 1, -100, None, 1, None, p, None)),
-        ("moc_label_targets", (p, (1 << 24) + 1, 10, -100, None, 1, None, p, None)),
-        ("moc_teacher_targets", (p, 1, 4, p, 1, 4, 3, 0, 10, 1.0, None, 1, None, p, None)),
-        ("moc_teacher_targets", (p, 1, 4, p, 1, 4, 3, 1025, 10, 1.0, None, 1, None, p, None)),
-        ("moc_teacher_targets", (p, 0, 4, p, 1, 4, 3, 4, 10, 1.0, None, 1, None, p, None)),
-        ("moc_teacher_targets", (p, 1, 4, p, 2, 4, 3, 4, 10, 1.0, None, 1, None, p, None)),
-        ("moc_teacher_targets", (p, 1, 3, p, 1, 4, 3, 4, 10, 1.0, None, 1, None, p, None)),
-        ("moc_teacher_targets", (p, 1, 4, p, 1, 4, 3, 4, 10, 0.0, None, 1, None, p, None)),
-        ("moc_teacher_targets", (p, 1, 4, p, 1, 4, 3, 4, 10, math.nan, None, 1, None, p, None)),
-        ("moc_logits_loss", (2, p, 3, 10, 10, p, 4, 1.0, p, p, p, 10, None)),
-        ("moc_logits_loss", (0, p, 3, 10, 9, p, 4, 1.0, p, p, p, 10, None)),
-        ("moc_logits_loss", (0, p, 3, 10, 10, p, 4, 1.0, p, p, p, 9, None)),
-        ("moc_logits_loss", (0, None, 3, 10, 10, p, 4, 1.0, p, p, p, 10, None)),
-        ("moc_logits_loss", (0, p, 3, 10, 10, p, 4, -1.0, p, p, p, 10, None)),
-        ("moc_linear_loss", (0, p, 3, 8, 8, p, 10, 8, p, 0, 1.0, p, p, p, 0, p, 0, p, 64, None, 0, None)),  # workspace
-        ("moc_linear_loss", (0, p, 3, 8, 12, p, 10, 8, p, 0, 1.0, p, p, None, 0, None, 0, p, 1 << 40, None, 0, None)),
-        ("moc_linear_loss", (1, p, 3, 8, 8, p, 10, 8, p, 0, 1.0, p, p, p, 0, None, 0, p, 1 << 40, None, 0, None)),
-        ("moc_linear_loss", (0, p, 3, 0, 8, p, 10, 8, p, 0, 1.0, p, p, None, 0, None, 0, p, 1 << 40, None, 0, None)),
-        ("moc_linear_loss", (0, p, 3, 512, 512, p, 1 << 21, 512, p, 0, 1.0, p, p, None, 0, None, 0, p, 1 << 40, None, 0,
-                             None)),
+        logits(dtype=2), logits(x=None), logits(rows=(1 << 24) + 1), logits(vocab=0), logits(vocab=(1 << 21) + 1),
+        logits(ld=9), logits(ldd=9), logits(words=0), logits(words=1025), logits(heat=0.0), logits(heat=math.nan),
+        logits(heat=-1.0), logits(heat=math.inf), logits(by=(p, 0, 4, p, 1, 4)), logits(by=(p, 1, 4, p, 2, 4)),
+        logits(by=(p, 1, 3, p, 1, 4)), logits(by=(p, 1, 4, p, 1, 3)), logits(by=(None, 1, 4, p, 1, 4)),
+        logits(by=(p, 1, 4, None, 1, 4)), logits(ws=None), logits(size=64), logits(counters=None),
+        linear(dtype=2), linear(h=None), linear(w=None), linear(labels=None), linear(d=0), linear(d=(1 << 20) + 1),
+        linear(rows=(1 << 24) + 1), linear(vocab=(1 << 21) + 1), linear(vocab=0), linear(ldh=12), linear(ldw=4),
+        linear(h=ctypes.c_void_p(4100)), linear(heat=2.0), linear(words=4, by=teacher, heat=0.0),
+        linear(words=4, by=(p, 1, 3, p, 1, 4)), linear(words=1025, by=teacher), linear(dtype=1, dh_dtype=0),
+        linear(dh_dtype=5), linear(size=64), linear(ws=None), linear(gws=None), linear(gsize=64),
+        linear(d=512, ldh=512, vocab=1 << 21, ldw=512),
         ("moc_scale_inplace", (5, p, 8, 0, None, 0, p, None)),
         ("moc_scale_inplace", (0, None, 8, 0, None, 0, p, None)),
         ("moc_scale_inplace", (0, p, 8, 0, None, 8, p, None)),
