@@ -1094,6 +1094,7 @@ unsigned blocks_of(int64_t n) {
 // --------------------------------------------------------------------- host
 // Logits exist for a piece of the rows at a time, within about this many bytes.
 constexpr int64_t kPieceBytes = 1LL << 30;
+constexpr int64_t kWidest = 4;
 constexpr int kHalvesBlocks = 1024;  // workgroups of halves_kernel that write f16 rows
 
 // A linear loss's pieces and the parts of its workspace.
@@ -1121,6 +1122,9 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   p.slabs = slabs_of(vocab);
   const int64_t each = f32 ? p.ldz * 4 : grads ? p.ldz * 2 : p.slabs * 8;
   int64_t n = kPieceBytes / each / 256 * 256;
+  // its hidden rows within 32-bit offsets, at up to kWidest times their own pitch
+  const int64_t most = ((1LL << 31) - 4096) / (es * kWidest * p.ldx) / 256 * 256;
+  if (n > most) n = most;
   if (n < 256) n = 256;
   if (n > rows) n = rows < 1 ? 1 : rows;
   p.rows = n;

@@ -70,6 +70,8 @@ def distillation_loss(logits, teacher_ids, teacher_logits, row_weight=None, *, t
     """linear_distillation of logits [..., vocab] (bf16 or f32) that are there already."""
     what = "distillation_loss"
     rows = _rows_of(what, logits, None, row_weight, reduction)
+    if not plain(logits):
+        raise ValueError(f"{what}: plain tensors only")
     if not 1 <= logits.shape[-1] <= 1 << 21:
         raise ValueError(f"{what}: a vocabulary of 1 to 2^21 words, got {logits.shape[-1]}")
     targets = _teacher(what, logits, teacher_ids, teacher_logits, row_weight, rows, temperature, reduction)
@@ -184,12 +186,14 @@ def _unit(t):
 
 # -------------------------------------------------------------------- operands
 def _rows16(t) -> torch.Tensor:
-    """t [rows, cols] with 16-byte aligned rows of unit stride, whose storage holds all
-    of the last one's pitch (the kernels read whole chunks); a copy of any other."""
+    """t [rows, cols] with 16-byte aligned rows of unit stride, at most four times their
+    length apart, whose storage holds all of the last one's pitch (the kernels read
+    whole chunks); a copy of any other."""
     rows, cols = t.shape
     per = 16 // t.element_size()
     pitch = _pitch(t)
-    if (t.stride(1) == 1 or cols == 1) and t.data_ptr() % 16 == 0 and pitch % per == 0 and pitch >= cols and (
+    if (t.stride(1) == 1 or cols == 1) and t.data_ptr() % 16 == 0 and pitch % per == 0 and (
+            cols <= pitch <= 4 * K.round_up(cols, 64)) and (
             (t.storage_offset() + rows * pitch) * t.element_size() <= t.untyped_storage().nbytes()):
         return t
     out = K.padded_empty(rows, cols, t.dtype, t.device)
@@ -235,14 +239,29 @@ def _linear_sizes(code: int, rows: int, d: int, vocab: int, words: int, grads: b
             N.query("moc_linear_loss_gemm_workspace_size", code, rows, d, vocab, grads))
 
 
-def _counted_workspace(device, nbytes: int) -> torch.Tensor:
-    """A GEMM workspace, its counters zero: the stream's, or one of the graph's own
-    under capture, since two graphs that were captured on one stream may run beside
-    each other."""
+_COUNTERS: dict = {}  # (device, stream) -> zeroed bytes that every launch leaves zero
+
+
+def _counters(dev: int, stream: int, where) -> torch.Tensor:
+    """Arrival counters of the stream, or the graph's own under capture, since two
+    graphs that were captured on one stream may run beside each other."""
+    held = _COUNTERS.get((dev, stream))
+    if torch.cuda.is_current_stream_capturing():
+        held = torch.empty(COUNTER_BYTES, dtype=torch.uint8, device=where)
+        N.call("moc_fill_zero", held.data_ptr(), COUNTER_BYTES, stream)
+    elif held is None:
+        held = _COUNTERS[dev, stream] = torch.zeros(COUNTER_BYTES, dtype=torch.uint8, device=where)
+    return held
+
+
+def _gemm_workspace(dev: int, stream: int, where, nbytes: int) -> torch.Tensor:
+    """A GEMM workspace with such counters at its start."""
+    if nbytes <= COUNTER_BYTES:
+        return _counters(dev, stream, where)
     if not torch.cuda.is_current_stream_capturing():
-        return K._gemm_workspace(device, nbytes)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    N.call("moc_fill_zero", ws.data_ptr(), COUNTER_BYTES, N.stream_of(ws))
+        return K._gemm_workspace(where, nbytes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
+    N.call("moc_fill_zero", ws.data_ptr(), COUNTER_BYTES, stream)
     return ws
 
 
@@ -262,11 +281,12 @@ def _linear_pass(targets, saved, row_weight, mean, grad, product, hidden, weight
     dweight = torch.empty((vocab, d), dtype=weight.dtype, device=where) if dw else None
     nbytes, ngemm = _linear_sizes(code, rows, d, vocab, targets.words, dh or dw)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
-    gemm_ws = _counted_workspace(where, ngemm)
+    stream = N.stream_on(dev)
+    gemm_ws = _gemm_workspace(dev, stream, where, ngemm)
     N.call("moc_linear_loss", code, h.data_ptr(), rows, d, _pitch(h), w.data_ptr(), vocab, _pitch(w),
            *targets.given(saved), N.ptr(row_weight), mean, N.ptr(grad), out.data_ptr() if each else None,
            None if each else out.data_ptr(), N.ptr(dhidden), N.dtype_code(hidden.dtype), N.ptr(dweight),
-           N.dtype_code(weight.dtype), ws.data_ptr(), nbytes, gemm_ws.data_ptr(), ngemm, N.stream_on(dev))
+           N.dtype_code(weight.dtype), ws.data_ptr(), nbytes, gemm_ws.data_ptr(), ngemm, stream)
     return out, dhidden, dweight
 
 
@@ -287,18 +307,21 @@ class _Kept:
 
     def __init__(self, grads):
         self.grads = grads
-        self.captured = torch.cuda.is_current_stream_capturing()
+        if grads is not None:
+            given = [t for t in grads if t is not None]
+            a, b = given[0], given[-1]
+            self.scaled = (N.dtype_code(a.dtype), a.data_ptr(), a.numel(), N.dtype_code(b.dtype), b.data_ptr(),
+                           b.numel() if len(given) > 1 else 0)
+            self.device = a.get_device()
+            self.captured = torch.cuda.is_current_stream_capturing()
 
     def take(self, g):
         """The gradients times g, or None: there are none, or no more, or those of an
         eager forward in a captured backward, which a replay would scale again."""
         grads, self.grads = self.grads, None
-        if grads is None or (torch.cuda.is_current_stream_capturing() and not self.captured):
+        if grads is None or (not self.captured and torch.cuda.is_current_stream_capturing()):
             return None
-        given = [t for t in grads if t is not None]
-        a, b = given[0], given[-1]
-        N.call("moc_scale_inplace", N.dtype_code(a.dtype), a.data_ptr(), a.numel(), N.dtype_code(b.dtype), b.data_ptr(),
-               b.numel() if len(given) > 1 else 0, g.data_ptr(), N.stream_of(a))
+        N.call("moc_scale_inplace", *self.scaled, g.data_ptr(), N.stream_on(self.device))
         return grads
 
 
@@ -356,11 +379,12 @@ def _logits_pass(targets, saved, row_weight, mean, grad, logits, each: bool, gra
     dx = torch.empty(logits.shape, dtype=x.dtype, device=where) if grads else None
     nbytes = N.query("moc_logits_loss_workspace_size", rows, targets.words)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
-    counters = _counted_workspace(where, COUNTER_BYTES)
+    stream = N.stream_on(dev)
+    counters = _counters(dev, stream, where)
     N.call("moc_logits_loss", N.dtype_code(x.dtype), x.data_ptr(), rows, vocab, x.stride(0) if rows > 1 else vocab,
            *targets.given(saved)[2:], N.ptr(row_weight), mean, N.ptr(grad), out.data_ptr() if each else None,
            None if each else out.data_ptr(), N.ptr(dx), vocab, ws.data_ptr(), nbytes, counters.data_ptr(),
-           N.stream_on(dev))
+           stream)
     return out, dx
 
 

@@ -143,7 +143,8 @@ def test_linear_cross_entropy(rows, d, vocab, dtype, masked, weighted, reduction
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("rows,d,vocab", SIZES)
 @pytest.mark.parametrize("words,heat,ragged,reduction", [(1, 1.0, False, "mean"), (7, 2.0, True, "mean"),
-                                                         (64, 0.7, False, "sum"), (300, 1.0, True, "none")])
+                                                         (64, 0.7, False, "sum"), (65, 1.0, True, "mean"),
+                                                         (200, 1.0, True, "sum"), (300, 1.0, True, "none")])
 def test_linear_distillation(rows, d, vocab, dtype, words, heat, ragged, reduction):
     h, w = operands(rows, d, vocab, dtype)
     h, w = h.requires_grad_(), w.requires_grad_()
@@ -188,13 +189,22 @@ def test_losses_alone(rows, d, vocab, dtype):
     want, _, _ = reference(z, q, some, weight.to(F64), 1.5, "none")
     check(L.linear_distillation(h, w, ids, top, weight, temperature=1.5, reduction="none"), want, (None, None), (hd, wd), z,
           z, q, z_err, 1.5, 1.0, weight)
+    check(L.linear_distillation(h, w, ids, top, weight, temperature=1.5),
+          want.sum() / torch.where(some, weight.to(F64), 0.0).sum(), (None, None), (hd, wd), z, z, q, z_err, 1.5, 1.0, weight)
+    x = z.to(F32)
+    kept = L.distillation_loss(x, ids, top, weight, temperature=1.5)
+    # the f32 rounding of the logits and the scaling's, twice, on top of the sums'
+    tol = (4 * 2.0 ** -24 * (z.abs().max().item() + 20) + 2.0 ** -20 * math.log(2 * vocab)) * 2.25
+    mean = want.sum() / torch.where(some, weight.to(F64), 0.0).sum()
+    assert abs(kept.item() - mean.item()) <= tol * (abs(mean.item()) + 1)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (2, 3), (5, 500), (33, 1003), (7, 32000), (3, 50021), (2, 128256),
-                                        (2, 262147), (600, 4096)])
+                                        (2, 262147), (2, 270011), (600, 4096), (3000, 77)])
 @pytest.mark.parametrize("words,heat,ragged,reduction", [(1, 1.0, False, "mean"), (20, 2.0, True, "mean"),
-                                                         (101, 0.7, False, "sum"), (1024, 1.0, True, "none")])
+                                                         (101, 0.7, False, "sum"), (256, 1.0, True, "mean"),
+                                                         (257, 1.0, True, "mean"), (1024, 1.0, True, "none")])
 def test_distillation_loss(rows, vocab, dtype, words, heat, ragged, reduction):
     x = (3 * rand(rows, vocab, seed=2)).to(dtype)
     ids, top = teacher_of(rows, vocab, words, ragged)
@@ -316,6 +326,20 @@ def test_strides_and_alignment():
     a = L.distillation_loss(x, ids, top)
     for make in (lambda t: pad(t, 3)[:, 1:-2].copy_(t), lambda t: t.t().contiguous().t()):
         assert torch.equal(a, L.distillation_loss(make(x), make(ids.float()).int(), make(top)))
+
+
+def test_many_rows_without_gradients():
+    """More hidden rows than 32-bit offsets reach: in pieces."""
+    rows, d, vocab = 140000, 4096, 40
+    w = operands(8, d, vocab, BF)[1]
+    h = rand(1000, d, seed=1).to(BF).repeat(rows // 1000, 1)
+    y = labels_of(1000, vocab, 0.2).repeat(rows // 1000)
+    each = L.linear_cross_entropy(h, w, y, reduction="none")
+    assert torch.equal(each[:1000].repeat(rows // 1000), each)
+    assert torch.equal(each[:1000], L.linear_cross_entropy(h[:1000], w, y[:1000], reduction="none"))
+    mean = L.linear_cross_entropy(h, w, y)
+    # the same rows' f32 losses in 64 bits, once
+    assert abs(mean.item() - each[:1000].to(F64).sum().item() / (y[:1000] != -100).sum().item()) <= 2.0 ** -23 * mean.item()
 
 
 @pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
@@ -477,6 +501,45 @@ def test_captured_pass(op):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+def test_two_graphs_at_once(op):
+    """Graphs captured on one stream, replayed beside each other on two."""
+    leaves, graphs, outs = [], [], []
+    ids, top = teacher_of(700, 3000, 8, True)
+    y = labels_of(700, 3000, 0.2)
+
+    def step(h, w, x):
+        if op == "kept":
+            loss = L.distillation_loss(x, ids, top)
+            return (loss.detach(), *torch.autograd.grad(loss, x))
+        loss = L.linear_cross_entropy(h, w, y) if op == "entropy" else L.linear_distillation(h, w, ids, top)
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w)))
+
+    for i in range(2):
+        h, w = operands(700, 256, 3000, BF, seed=10 * i)
+        leaves.append((h.requires_grad_(), w.requires_grad_(), (3 * rand(700, 3000, seed=i)).to(BF).requires_grad_()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*leaves[0])
+    torch.cuda.current_stream().wait_stream(side)
+    for own in leaves:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(step(*own))
+        graphs.append(graph)
+    want = [step(*own) for own in leaves]
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(4):
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for got, exact in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(got, exact))
 
 
 def test_captured_backward_of_an_eager_forward():
