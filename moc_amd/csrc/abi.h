@@ -58,7 +58,7 @@ int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, c
                      int64_t ldw, float unit, const int32_t* ids, int64_t ld_ids, const uint16_t* first,
                      int64_t ld_first, int64_t words, float* z, float2* stat, void* kept, int64_t ld_kept, hipStream_t st);
 
-// C [M, N] = *alpha A B (f16 operands, A with a unit stride along M or K, rows of B
+// C [M, N] = *alpha A B (f16 operands; alpha null: A B, bf16; A with a unit stride along M or K, rows of B
 // ldb apart; C bf16 or f32) (gemm.hip); 16-byte aligned rows, workspace as
 // moc_gemm_ws uses it.
 int64_t gemm_half_workspace(int64_t M, int64_t N, int64_t K);

@@ -447,7 +447,10 @@ __device__ __forceinline__ uint4 add_residual8(uint4 v, const uint16_t* r, int n
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-template <bool OUT_F32, int NJ, int MI = 4>
+// LOOSE: 16-byte segments at any address where C's rows are not 16-byte aligned.
+typedef uint32_t u32x4_loose_t __attribute__((ext_vector_type(4), aligned(2)));
+
+template <bool OUT_F32, int NJ, int MI = 4, bool LOOSE = false>
 __device__ __forceinline__ void store_tile_w(const GemmArgs& g, char* lds, const f32x16_t (&acc)[MI][NJ],
                                              int row0, int col0, int wm, int wn, int wave, int lane) {
   constexpr int kEsz = OUT_F32 ? 4 : 2;
@@ -491,6 +494,8 @@ __device__ __forceinline__ void store_tile_w(const GemmArgs& g, char* lds, const
       char* dst = static_cast<char*>(g.C) + (static_cast<int64_t>(grow) * g.ldc + gcol) * kEsz;
       if (vec && gcol + 16 / kEsz <= g.N) {
         *reinterpret_cast<uint4*>(dst) = v;
+      } else if (LOOSE && gcol + 16 / kEsz <= g.N) {
+        *reinterpret_cast<u32x4_loose_t*>(dst) = (u32x4_loose_t){v.x, v.y, v.z, v.w};
       } else {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         if (OUT_F32) {
@@ -1448,7 +1453,7 @@ next_tile:
       return;
     if constexpr (HALF) scale_tile(acc, g.alpha);
     if constexpr (SP) store_tile_t<OUT_F32, 2>(g, lds, acc, row0, col0, wm, wn, wave, lane);
-    else store_tile_w<OUT_F32, 2, MI>(g, lds, acc, row0, col0, wm, wn, wave, lane);
+    else store_tile_w<OUT_F32, 2, MI, HALF>(g, lds, acc, row0, col0, wm, wn, wave, lane);
   }
 }
 
@@ -1626,7 +1631,7 @@ __global__ __launch_bounds__(kMidThreads) void gemm_mid_kernel(GemmArgs g) {
   __syncthreads();  // the ring becomes the epilogue's staging
   if (g.ksplit > 1) g.C = static_cast<float*>(g.C) + split * g.ws_stride;
   else if constexpr (HALF) scale_tile(acc, g.alpha);
-  store_tile_w<OUT_F32, NJ, MI>(g, lds, acc, row0, col0, wm, wn, wave, lane);
+  store_tile_w<OUT_F32, NJ, MI, HALF>(g, lds, acc, row0, col0, wm, wn, wave, lane);
 }
 
 // Sum of the ksplit f32 partial tiles of a split-K GEMM, in split order (the
@@ -2116,7 +2121,7 @@ struct SplitPlan {
   int64_t bytes = 0;
 };
 
-// step > 1: only multiples of it (see gemm_half).
+// step > 1: splits up to it and multiples of it alone (see gemm_half).
 SplitPlan plan_split(int64_t M, int64_t N, int nk, int step = 1) {
   SplitPlan p;
   p.kper = nk;
@@ -2124,7 +2129,7 @@ SplitPlan plan_split(int64_t M, int64_t N, int nk, int step = 1) {
   const int cus = cu_count();
   if (tiles <= 0 || 3 * tiles > cus) return p;
   int ks = static_cast<int>(std::min<int64_t>(cus / tiles, nk / 4));
-  if (step > 1)
+  if (ks > step && step > 1)
     for (ks -= ks % step; ks > 0 && (nk + ks - 1) / ks * (ks - 1) >= nk;) ks -= step;
   if (ks < 2) return p;
   const int kper = (nk + ks - 1) / ks;
@@ -2165,7 +2170,7 @@ SplitPlan plan_split(int64_t M, int64_t N, int nk, int step = 1) {
 // mean.  The costs above are up to half high where K is long (1280 x 2605 x
 // 6200: 70 against 54 us) and a third low for the shortest.
 //
-// step > 1: K splits in multiples of it alone (see gemm_half).
+// step > 1: K splits up to it and in multiples of it alone (see gemm_half).
 MidPlan plan_mid(int64_t M, int64_t N, int nk, int64_t n2, int64_t ws_bytes, int step = 1) {
   struct Tile {
     int bm, bn;
@@ -2193,7 +2198,7 @@ MidPlan plan_mid(int64_t M, int64_t N, int nk, int64_t n2, int64_t ws_bytes, int
     for (int ks = 1; ks <= ks_max; ++ks) {
       const int kper = (nk + ks - 1) / ks;
       if (kper * (ks - 1) >= nk) continue;  // the last part would be empty
-      if (ks > 1 && ks % step != 0) continue;
+      if (ks > step && ks % step != 0) continue;
       const int64_t bytes = ks > 1 ? kFixCounterBytes + ks * M * ldw * 4 : 0;
       if (bytes > ws_bytes) break;
       const int full = n * ks / (2 * cus), rem = n * ks - full * 2 * cus;
@@ -2896,11 +2901,15 @@ extern "C" int moc_gemm_ws(int dtype, int64_t M, int64_t N, int64_t K, const voi
 namespace moc {
 
 // C [M, N] = *alpha A B, A (a_sm, a_sk: one of them 1) and B [K, N] (rows of ldb)
-// in f16, C in bf16 or f32: the gradients of a product whose own gradient needs more
-// than bf16's 8 bits.  As moc_gemm_ws with the f16 MFMA (the same rate), but K is
-// split in multiples of 8 ways alone: workgroup ids go to the XCDs in turn, so a K
-// range then stays in one XCD's L2, where 9 ways have every XCD read every range
-// (777 x 512 x 32000, bf16: 76 us in 9 parts, 36 in 8).
+// in f16 (alpha null: C = A B of bf16), C in bf16 or f32: the gradients of a product
+// whose own gradient needs more than bf16's 8 bits.  As moc_gemm_ws, f16 at the same
+// rate, but K is
+// split up to 8 ways or in multiples of 8: workgroup ids go to the XCDs in turn, so a
+// K range then stays in one XCD's L2, where 9 ways have every XCD read every range
+// (777 x 512 x 32000, bf16: 76 us in 9 parts, 36 in 8); and rows of C that are not
+// 16-byte aligned are stored in 16-byte pieces all the same, which the memory takes at
+// any address (a gradient of 16921 x 1500 over 44 rows: 54 us with
+// 2-byte stores, 22).
 int64_t gemm_half_workspace(int64_t M, int64_t N, int64_t K) {
   const int nk = static_cast<int>((K + kBK - 1) / kBK);
   return std::max({plan_split(M, N, nk, 8).bytes, plan_fix(M, N, nk).bytes, plan_fix_short(M, N, nk).bytes,
@@ -2910,7 +2919,6 @@ int64_t gemm_half_workspace(int64_t M, int64_t N, int64_t K) {
 int gemm_half(int64_t M, int64_t N, int64_t K, const void* A, int64_t a_sm, int64_t a_sk, const void* B, int64_t ldb,
               void* C, int64_t ldc, int c_dtype, const float* alpha, void* workspace, int64_t workspace_bytes,
               void* stream) {
-  MOC_REQUIRE(alpha != nullptr, "gemm_half: null alpha");
   return gemm_ws_impl(MOC_BF16, M, N, K, A, a_sm, a_sk, B, ldb, 1, 0, nullptr, 0, 0, nullptr, 0, 0, C, ldc, c_dtype,
                       workspace, workspace_bytes, stream, nullptr, 0, 8, alpha);
 }

@@ -181,25 +181,27 @@ __device__ __forceinline__ void put_total(const Targets& t, int64_t rows, int me
 }
 
 // A teacher's rows of up to 64 W words, a wave a row, W words a lane: sorted by rank
-// (ties by place), entries of one word made one.  counter (null: not here): the last
+// (ties by place), entries of one word made one.  Four rows a workgroup: its
+// comparisons keep a SIMD busy (256 words, 807 rows: 47 us with 16).  counter (null: not here): the last
 // workgroup sums the weights.
 template <typename ID, bool TOP_F32, int W>
-__global__ __launch_bounds__(1024) void teacher_wave_kernel(const ID* __restrict__ ids, int64_t ids_ld,
+__global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict__ ids, int64_t ids_ld,
                                                             const void* __restrict__ top, int64_t top_ld, int64_t rows,
                                                             int words, int vocab, float heat,
                                                             const float* __restrict__ row_weight, int mean,
                                                             const float* __restrict__ grad, Targets t, int* counter) {
   constexpr int kWide = 64 * W;
-  __shared__ __attribute__((aligned(16))) int32_t id_of[16][kWide];
-  __shared__ int32_t sorted_id[16][kWide];
-  __shared__ float sorted_q[16][kWide];
-  __shared__ double red64[16];
-  __shared__ float red[16];
+  __shared__ __attribute__((aligned(16))) uint32_t keys[4][kWide];
+  __shared__ int32_t sorted_id[4][kWide];
+  __shared__ float sorted_q[4][kWide];
+  __shared__ double red64[4];
+  __shared__ float red[4];
   __shared__ int flag;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 16 + wave;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + wave;
   if (r < rows) {
     int32_t id[W];
+    uint32_t key[W];  // the word, then its place: no two alike
     float q[W], mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
@@ -216,7 +218,8 @@ __global__ __launch_bounds__(1024) void teacher_wave_kernel(const ID* __restrict
         }
       }
       mx = fmaxf(mx, q[i]);
-      id_of[wave][k] = id[i];
+      key[i] = (id[i] == kNoWord ? 1u << 31 : static_cast<uint32_t>(id[i]) << 10) + k;
+      keys[wave][k] = key[i];
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
@@ -234,13 +237,12 @@ __global__ __launch_bounds__(1024) void teacher_wave_kernel(const ID* __restrict
     __builtin_amdgcn_wave_barrier();
     int rank[W] = {};
     for (int j = 0; j < kWide; j += 4) {
-      const int4 o = *reinterpret_cast<const int4*>(&id_of[wave][j]);
-      const int32_t other[4] = {o.x, o.y, o.z, o.w};
+      const uint4 o = *reinterpret_cast<const uint4*>(&keys[wave][j]);
+      const uint32_t other[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int i = 0; i < W; ++i)
-          rank[i] += other[e] < id[i] || (other[e] == id[i] && j + e < lane + 64 * i);
+        for (int i = 0; i < W; ++i) rank[i] += other[e] < key[i];
     }
 #pragma unroll
     for (int i = 0; i < W; ++i) {
@@ -918,8 +920,12 @@ __global__ __launch_bounds__(256) void halves_kernel(Halves hidden_rows, Halves 
 // add to the products' sums, where the words' parts cancel, more than the sums' own
 // rounding (measured: up to 1.9 times the error of f32 ones); 2^-11 does not show.
 // Down to 2^-28 of the largest they have all 11 bits, below 2^-39 they are 0.
+//
+// TWO (few rows): as two bf16 parts too, rows [0, rows) and [rows, 2 rows) of two, for
+// a product with the weight as it is.
+template <bool TWO>
 __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Slabs& s, const Targets& t,
-                                               const LossOut& o, int& flag, int64_t at, int rows) {
+                                               const LossOut& o, int& flag, int64_t at, int rows, uint16_t* two) {
   typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
   __shared__ float red[4], at_word[kMaxWords];
   const int64_t r = s.r0 + at;
@@ -927,9 +933,14 @@ __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Sl
   const float w = weight_of(t, r);
   uint16_t* out = e + at * ld;
   uint4* row = reinterpret_cast<uint4*>(out);
+  uint16_t* part[2] = {two + at * ld, two + (rows + at) * ld};
   const int chunks = (s.vocab + 7) / 8;
   if (w == 0.f) {  // uniform
-    for (int c = tid; c < chunks; c += 256) row[c] = make_uint4(0, 0, 0, 0);
+    for (int c = tid; c < chunks; c += 256) {
+      row[c] = make_uint4(0, 0, 0, 0);
+      if constexpr (TWO)
+        for (uint16_t* p : part) reinterpret_cast<uint4*>(p)[c] = make_uint4(0, 0, 0, 0);
+    }
     if (tid == 0) flag = put_row(o, r, 0.f, rows);
     return;
   }
@@ -957,16 +968,23 @@ __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Sl
       if (at >= chunks) break;
       const float f = c * __builtin_amdgcn_exp2f(m[i] - lse - 15.f);
       const uint32_t in[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-      uint32_t out[4];
+      uint32_t out[4], high[4], low[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const f16x2_t h = __builtin_bit_cast(f16x2_t, in[q]);
-        out[q] = __builtin_bit_cast(uint32_t,
-                                    __builtin_convertvector((cvt_f32x2_t){static_cast<float>(h.x) * f,
-                                                                          static_cast<float>(h.y) * f},
-                                                            f16x2_t));
+        const cvt_f32x2_t g = {static_cast<float>(h.x) * f, static_cast<float>(h.y) * f};
+        out[q] = __builtin_bit_cast(uint32_t, __builtin_convertvector(g, f16x2_t));
+        if constexpr (TWO) {
+          high[q] = __builtin_bit_cast(uint32_t, __builtin_convertvector(g, cvt_bf16x2_t));
+          const cvt_f32x2_t rest = {g.x - __uint_as_float(high[q] << 16), g.y - __uint_as_float(high[q] & 0xFFFF0000u)};
+          low[q] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, cvt_bf16x2_t));
+        }
       }
       row[at] = make_uint4(out[0], out[1], out[2], out[3]);
+      if constexpr (TWO) {
+        reinterpret_cast<uint4*>(part[0])[at] = make_uint4(high[0], high[1], high[2], high[3]);
+        reinterpret_cast<uint4*>(part[1])[at] = make_uint4(low[0], low[1], low[2], low[3]);
+      }
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stored before the words' own
@@ -975,7 +993,12 @@ __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Sl
     float share;
     const int32_t id = word_of(t, r, s.words, k, s.vocab, share);
     if (id == kUnknown || share == -1.f) continue;
-    out[id] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(c * (__builtin_amdgcn_exp2f(at_word[k]) - share)));
+    const float g = c * (__builtin_amdgcn_exp2f(at_word[k]) - share);
+    out[id] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(g));
+    if constexpr (TWO) {
+      part[0][id] = bf16_rne(g);
+      part[1][id] = bf16_rne(g - bf16_to_f32(part[0][id]));
+    }
   }
 }
 
@@ -983,9 +1006,11 @@ __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Sl
 // those that the guess did not suit are done again, and the products' factors written.
 constexpr int kAgainBlocks = 64;
 
+template <bool TWO>
 __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld, Slabs s, Targets t, LossOut o,
                                                          Halves hidden_rows, Halves weight_rows, int hidden,
-                                                         int64_t ldo, const uint32_t* __restrict__ most, int parts) {
+                                                         int64_t ldo, const uint32_t* __restrict__ most, int parts,
+                                                         uint16_t* two) {
   __shared__ double red64[4];
   __shared__ uint32_t red[4];
   __shared__ int flag;
@@ -1009,7 +1034,7 @@ __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld
     }
     return;
   }
-  slabs_grad_row(e, ld, s, t, o, flag, blockIdx.x - again, gridDim.x - again);
+  slabs_grad_row<TWO>(e, ld, s, t, o, flag, blockIdx.x - again, gridDim.x - again, two);
   __syncthreads();
   if (flag) put_loss<true>(t, o, red64);
 }
@@ -1044,6 +1069,14 @@ __global__ __launch_bounds__(256) void add_f32_kernel(float* a, const float* __r
     if (out != nullptr) out[i] = Elem<OUT>::of(s);
     else a[i] = s;
   }
+}
+
+// The rows of a product with gradients in two parts: out = *alpha (a[r] + a[rows + r]).
+template <typename OUT>
+__global__ __launch_bounds__(256) void two_parts_kernel(const float* __restrict__ a, int64_t n,
+                                                        const float* __restrict__ alpha, OUT* __restrict__ out) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) out[i] = Elem<OUT>::of(*alpha * (a[i] + a[n + i]));
 }
 
 // out[i][j] = *alpha a_i b_j (alpha null: 1), the product over one row or one word (the engine takes no
@@ -1095,6 +1128,9 @@ unsigned blocks_of(int64_t n) {
 // Logits exist for a piece of the rows at a time, within about this many bytes.
 constexpr int64_t kPieceBytes = 1LL << 30;
 constexpr int64_t kWidest = 4;
+// Up to this many rows dhidden comes from gradients in two bf16 parts, twice the rows,
+// with the weight as it is: less than a copy of the weight in f16 takes (TWO).
+constexpr int64_t kTwoRows = 256;
 constexpr int kHalvesBlocks = 1024;  // workgroups of halves_kernel that write f16 rows
 
 // A linear loss's pieces and the parts of its workspace.
@@ -1107,6 +1143,8 @@ struct Pieces {
   float* row_loss;
   char *d, *x, *w;  // logits, then their gradients; copies of hidden rows and weight
   float *acc, *part, *z;
+  char* two;    // up to kTwoRows rows: gradients in two parts,
+  float* both;  // their product
   uint32_t* most;
   float2* stat;
   int64_t bytes;
@@ -1139,7 +1177,12 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   if (f32 || grads) p.d = ws.take<char>(n * p.ldz * es);
   if (grads) p.x = ws.take<char>(rows * p.ldx * es);
   if (grads && p.fused) {
-    p.w = ws.take<char>(vocab * p.ldx * 2);
+    if (rows <= kTwoRows && vocab > 1) {
+      p.two = ws.take<char>(2 * rows * p.ldz * 2);
+      p.both = ws.take<float>(2 * rows * hidden);
+    } else {
+      p.w = ws.take<char>(vocab * p.ldx * 2);
+    }
     p.most = ws.take<uint32_t>(2 * kHalvesBlocks);
   }
   if (grads && p.count > 1) {
@@ -1166,7 +1209,7 @@ void launch_teacher(const Teacher& a, int64_t rows, int words, int vocab, const 
                     const float* grad, const Targets& t, int* counter, hipStream_t st) {
   const ID* ids = static_cast<const ID*>(a.ids);
 #define MOC_WAVES(W)                                                                                                \
-  teacher_wave_kernel<ID, TOP_F32, W><<<static_cast<unsigned>((rows + 15) / 16), 1024, 0, st>>>(                      \
+  teacher_wave_kernel<ID, TOP_F32, W><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(                         \
       ids, a.ids_ld, a.top, a.top_ld, rows, words, vocab, a.heat, row_weight, mean, grad, t, counter)
   if (words <= 64) MOC_WAVES(1);
   else if (words <= 128) MOC_WAVES(2);
@@ -1182,7 +1225,8 @@ int run_teacher(const Teacher& a, int64_t rows, int64_t words, int64_t vocab, co
                 const float* grad, const Targets& t, bool total, int* counters, hipStream_t st) {
   if (rows == 0) return MOC_OK;
   const int k = static_cast<int>(words), v = static_cast<int>(vocab);
-  int* counter = total ? counters + kTeacherCounter : nullptr;
+  const bool arrive = words <= 256 && rows <= 2 * kArriveRows;  // four rows a workgroup
+  int* counter = total && arrive ? counters + kTeacherCounter : nullptr;
 #define MOC_TEACHER(ID, F) launch_teacher<ID, F>(a, rows, k, v, row_weight, mean, grad, t, counter, st)
   if (a.ids_dtype == MOC_I32 && a.top_dtype == MOC_F32) MOC_TEACHER(int32_t, true);
   else if (a.ids_dtype == MOC_I32) MOC_TEACHER(int32_t, false);
@@ -1190,7 +1234,7 @@ int run_teacher(const Teacher& a, int64_t rows, int64_t words, int64_t vocab, co
   else MOC_TEACHER(int64_t, false);
 #undef MOC_TEACHER
   const int rc = check_launch("teacher_wave_kernel");
-  if (rc != MOC_OK || !total || words <= 256) return rc;
+  if (rc != MOC_OK || !total || arrive) return rc;
   target_total_kernel<<<1, 1024, 0, st>>>(rows, mean, grad, t);
   return check_launch("target_total_kernel");
 }
@@ -1347,7 +1391,8 @@ extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, 
     const int64_t n = i + 1 < p.count ? p.rows : rows - i * p.rows;
     if (!p.fused) need(moc_gemm_workspace_size(dtype, n, vocab, hidden, 0));
     if (!grads) continue;
-    need(p.fused ? gemm_half_workspace(n, hidden, vocab) : moc_gemm_workspace_size(dtype, n, hidden, vocab, 0));
+    need(!p.fused ? moc_gemm_workspace_size(dtype, n, hidden, vocab, 0)
+                  : gemm_half_workspace(rows <= kTwoRows ? 2 * n : n, hidden, vocab));
     need(p.fused ? gemm_half_workspace(vocab, hidden, n) : moc_gemm_workspace_size(dtype, vocab, hidden, n, 0));
   }
   return most;
@@ -1410,8 +1455,10 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
   }
   const Halves hx{static_cast<const uint16_t*>(h), ldh, rows, dw != nullptr ? reinterpret_cast<_Float16*>(p.x) : nullptr,
                   0x1p2f, 0x1p-3f, 0x1p13f};
-  const Halves hw{static_cast<const uint16_t*>(w), ldw, vocab, dh != nullptr ? reinterpret_cast<_Float16*>(p.w) : nullptr,
-                  0x1p6f, 0x1p-7f, 0x1p9f};
+  const bool two = grads && p.fused && rows <= kTwoRows && vocab > 1;
+  const bool copy_w = dh != nullptr && !two;
+  const Halves hw{static_cast<const uint16_t*>(w), ldw, vocab, copy_w ? reinterpret_cast<_Float16*>(p.w) : nullptr,
+                  copy_w ? 0x1p6f : 1.f, 0x1p-7f, 0x1p9f};
   int halves = 0;
   if (grads && rows > 0 && f32) {
     if (words == 0) {
@@ -1422,7 +1469,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
         static_cast<const float*>(h), ldh, rows, (int)hidden, t, reinterpret_cast<float*>(p.x), p.ldx);
     if ((rc = check_launch("counted_rows_kernel")) != MOC_OK) return rc;
   } else if (grads && rows > 0) {
-    const int64_t want = ((rows > vocab ? rows : vocab) + 15) / 16;  // four waves of four rows
+    const int64_t most_rows = copy_w && vocab > rows ? vocab : rows, want = (most_rows + 15) / 16;  // four waves of four rows
     halves = static_cast<int>(want < kHalvesBlocks ? want : kHalvesBlocks);
     halves_kernel<<<1 + table_blocks + halves, 256, 0, st>>>(hx, hw, (int)hidden, p.ldx, t, rows, mean, grad, (int)words,
                                                              (int)p.slabs, p.most, halves);
@@ -1453,9 +1500,14 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       MOC_REQUIRE(rc <= 0, "moc_linear_loss: operands of up to 2 GiB");
       if (rc != MOC_OK) return rc;
       const Slabs s{p.stat, p.z, (int)p.slabs, (int)vocab, (int)words, r0, temperature};
-      if (grads)
-        slabs_grad_kernel<<<static_cast<unsigned>(n) + (i == 0 ? kAgainBlocks : 0), 256, 0, st>>>(
-            reinterpret_cast<uint16_t*>(p.d), p.ldz, s, t, o, hx, hw, (int)hidden, p.ldx, p.most, halves);
+      const unsigned blocks = static_cast<unsigned>(n) + (i == 0 ? kAgainBlocks : 0);
+      uint16_t* d = reinterpret_cast<uint16_t*>(p.d);
+      if (two && dh != nullptr)
+        slabs_grad_kernel<true><<<blocks, 256, 0, st>>>(d, p.ldz, s, t, o, hx, hw, (int)hidden, p.ldx, p.most, halves,
+                                                        reinterpret_cast<uint16_t*>(p.two));
+      else if (grads)
+        slabs_grad_kernel<false><<<blocks, 256, 0, st>>>(d, p.ldz, s, t, o, hx, hw, (int)hidden, p.ldx, p.most, halves,
+                                                         nullptr);
       else
         slabs_loss_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(s, t, o);
       rc = check_launch("slabs_grad_kernel");
@@ -1466,7 +1518,18 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       rc = logits_rows(true, p.d, n, vocab, p.ldz, t, r0, words, temperature, o, grads ? p.d : nullptr, p.ldz, st);
     }
     if (rc != MOC_OK) return rc;
-    if (dh != nullptr) {
+    if (dh != nullptr && two) {
+      rc = gemm_half(2 * n, hidden, vocab, p.two, p.ldz, 1, w, ldw, p.both, hidden, MOC_F32, nullptr, gemm_ws,
+                     gemm_ws_bytes, stream);
+      if (rc != MOC_OK) return rc;
+      const int64_t size = n * hidden;
+      const unsigned blocks = static_cast<unsigned>((size + 255) / 256);
+      if (dh_dtype == MOC_F32)
+        two_parts_kernel<float><<<blocks, 256, 0, st>>>(p.both, size, t.alpha, static_cast<float*>(dh));
+      else
+        two_parts_kernel<uint16_t><<<blocks, 256, 0, st>>>(p.both, size, t.alpha, static_cast<uint16_t*>(dh));
+      if ((rc = check_launch("two_parts_kernel")) != MOC_OK) return rc;
+    } else if (dh != nullptr) {
       char* to = static_cast<char*>(dh) + r0 * hidden * (dh_dtype == MOC_F32 ? 4 : 2);
       const char* b = p.fused ? p.w : static_cast<const char*>(w);
       rc = vocab == 1 ? outer(f32, n, hidden, p.d, p.ldz, b, t.alpha, to, dh_dtype, st)

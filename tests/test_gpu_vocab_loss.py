@@ -6,7 +6,8 @@ or with one rounding of 2^-24: with S the largest sum of |h||w|, an error of 4 s
 2^-24 S (roundings of either sign) and 2 more units for an f32 product's own.  A
 row's loss differs by twice that and by f32 exponentials, logarithms and a sum over
 the vocabulary, 2^-20 of its terms.  A gradient is a sum over dlogits, which are
-rounded to f16 twice (2^-11 of each; 2^-39 of the row's factor where it is smallest),
+rounded to f16 twice (2^-11 of each; 2^-39 of the row's factor where it is smallest)
+or to f16 once and two bf16 parts (less),
 its other operand by 2^-24 of its largest value, or stay f32 (2^-23 with the
 exponential's own), behind a relative error of the logits' errors, and is rounded
 itself; |dlogits| |operand| in 64 bits bounds what that comes to.  p's relative error
@@ -24,7 +25,7 @@ from moc_amd import losses as L
 pytestmark = pytest.mark.gpu
 BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
 SIZES = [(1, 8, 1), (1, 64, 500), (3, 100, 1003), (17, 256, 4099), (40, 2048, 8190), (256, 64, 32000), (300, 512, 2050),
-         (1030, 96, 777), (129, 1000, 5000), (5, 1, 9), (2, 24, 1), (1, 7, 2)]
+         (1030, 96, 777), (129, 1000, 5000), (5, 1, 9), (2, 24, 1), (1, 7, 2), (257, 333, 700)]
 
 
 def rand(*shape, seed):
