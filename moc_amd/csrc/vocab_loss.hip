@@ -1128,9 +1128,20 @@ unsigned blocks_of(int64_t n) {
 // Logits exist for a piece of the rows at a time, within about this many bytes.
 constexpr int64_t kPieceBytes = 1LL << 30;
 constexpr int64_t kWidest = 4;
-// Up to this many rows dhidden comes from gradients in two bf16 parts, twice the rows,
-// with the weight as it is: less than a copy of the weight in f16 takes (TWO).
-constexpr int64_t kTwoRows = 256;
+// Few rows: dhidden comes from gradients in two bf16 parts, twice the rows, with the
+// weight as it is (TWO), else from f16 ones and a copy of the weight.  The copy moves 4
+// bytes of each of the weight's values, the parts cost as many products and 16 bytes of
+// each logit again.  GPU time of a step, us, copy / two parts:
+//   32000 words, hidden  256:   64 rows  68 /  69   128  71 /  74   256  79 /  89
+//   32000               1024:   64       99 /  96   128 111 / 111   256 134 / 136
+//   32000               2048:   64      180 / 139   256 251 / 226   384 289 / 288
+//   32000               4096:   64      354 / 280   256 425 / 405   384 497 / 503
+//   100000              1024:   64      296 / 233   192 342 / 320   384 464 / 509
+//   100000              2048:   64      542 / 410   256 657 / 593   512 890 / 923
+bool in_two_parts(int64_t rows, int64_t hidden, int64_t vocab) {
+  return rows * (hidden + 960) <= 420 * hidden && vocab > 1;
+}
+
 constexpr int kHalvesBlocks = 1024;  // workgroups of halves_kernel that write f16 rows
 
 // A linear loss's pieces and the parts of its workspace.
@@ -1143,7 +1154,7 @@ struct Pieces {
   float* row_loss;
   char *d, *x, *w;  // logits, then their gradients; copies of hidden rows and weight
   float *acc, *part, *z;
-  char* two;    // up to kTwoRows rows: gradients in two parts,
+  char* two;    // few rows (in_two_parts): gradients in two parts,
   float* both;  // their product
   uint32_t* most;
   float2* stat;
@@ -1177,7 +1188,7 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   if (f32 || grads) p.d = ws.take<char>(n * p.ldz * es);
   if (grads) p.x = ws.take<char>(rows * p.ldx * es);
   if (grads && p.fused) {
-    if (rows <= kTwoRows && vocab > 1) {
+    if (in_two_parts(rows, hidden, vocab)) {
       p.two = ws.take<char>(2 * rows * p.ldz * 2);
       p.both = ws.take<float>(2 * rows * hidden);
     } else {
@@ -1392,7 +1403,7 @@ extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, 
     if (!p.fused) need(moc_gemm_workspace_size(dtype, n, vocab, hidden, 0));
     if (!grads) continue;
     need(!p.fused ? moc_gemm_workspace_size(dtype, n, hidden, vocab, 0)
-                  : gemm_half_workspace(rows <= kTwoRows ? 2 * n : n, hidden, vocab));
+                  : gemm_half_workspace(in_two_parts(rows, hidden, vocab) ? 2 * n : n, hidden, vocab));
     need(p.fused ? gemm_half_workspace(vocab, hidden, n) : moc_gemm_workspace_size(dtype, vocab, hidden, n, 0));
   }
   return most;
@@ -1455,7 +1466,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
   }
   const Halves hx{static_cast<const uint16_t*>(h), ldh, rows, dw != nullptr ? reinterpret_cast<_Float16*>(p.x) : nullptr,
                   0x1p2f, 0x1p-3f, 0x1p13f};
-  const bool two = grads && p.fused && rows <= kTwoRows && vocab > 1;
+  const bool two = grads && p.fused && in_two_parts(rows, hidden, vocab);
   const bool copy_w = dh != nullptr && !two;
   const Halves hw{static_cast<const uint16_t*>(w), ldw, vocab, copy_w ? reinterpret_cast<_Float16*>(p.w) : nullptr,
                   copy_w ? 0x1p6f : 1.f, 0x1p-7f, 0x1p9f};
