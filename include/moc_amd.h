@@ -304,6 +304,9 @@ int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t hidden, int6
                     float* loss, void* dh, int dh_dtype, void* dw, int dw_dtype, void* workspace,
                     int64_t workspace_bytes, void* gemm_ws, int64_t gemm_ws_bytes, void* stream);
 
+/* A number that names the HIP graph that `stream` is captured into, 0 outside a capture. */
+int64_t moc_capture_id(void* stream);
+
 /* p0 and p1 *= *factor (a device scalar) over n0 and n1 values, nothing where it is 1. */
 int moc_scale_inplace(int dtype0, void* p0, int64_t n0, int dtype1, void* p1, int64_t n1, const float* factor,
                       void* stream);

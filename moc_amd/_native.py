@@ -92,6 +92,7 @@ SIGNATURES: dict[str, tuple] = {
     "moc_linear_loss": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _int, _i64, _vp, _int, _i64,
                                _i64, ctypes.c_float, _vp, _int, _vp, _vp, _vp, _vp, _int, _vp, _int, _vp, _i64, _vp,
                                _i64, _vp]),
+    "moc_capture_id": (_i64, [_vp]),
     "moc_scale_inplace": (_int, [_int, _vp, _i64, _int, _vp, _i64, _vp, _vp]),
     "moc_attention_half_saved_size": (_i64, [_i64, _i64, _i64, _i64, _int]),
     "moc_attention_half_scratch_size": (_i64, [_i64, _i64, _i64, _i64, _int]),

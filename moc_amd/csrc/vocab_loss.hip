@@ -10,8 +10,8 @@
 // whose label is the ignored one and one without words count for nothing, what
 // is in them included: their gradient is 0 and n leaves them out.
 //
-// Logits are kept in units of log2(e) / T behind the first load, so an
-// exponential is one v_exp_f32.  Sums over rows are in 64 bits and in a fixed
+// Logits are in units of log2(e) / T where they meet an exponential, which then is
+// one v_exp_f32.  Sums over rows are in 64 bits and in a fixed
 // order.
 #include "abi.h"
 #include "common.h"
@@ -203,6 +203,7 @@ __global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict_
     int32_t id[W];
     uint32_t key[W];  // the word, then its place: no two alike
     float q[W], mx = -INFINITY;
+    const float unit = kLog2E / heat;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const int k = lane + 64 * i;
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict_
       if (k < words) {
         const int64_t word = static_cast<int64_t>(ids[r * ids_ld + k]);
         const float x = (TOP_F32 ? static_cast<const float*>(top)[r * top_ld + k]
-                                 : bf16_to_f32(static_cast<const uint16_t*>(top)[r * top_ld + k])) / heat;
+                                 : bf16_to_f32(static_cast<const uint16_t*>(top)[r * top_ld + k]));
         if (word >= 0 && word < vocab && x != -INFINITY) {
           id[i] = static_cast<int32_t>(word);
           q[i] = x;
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict_
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       some |= id[i] != kNoWord;
-      q[i] = id[i] == kNoWord ? 0.f : exp2f((q[i] - mx) * kLog2E);
+      q[i] = id[i] == kNoWord ? 0.f : exp2f((q[i] - mx) * unit);
       sum += q[i];
     }
     some = __any(some);
@@ -293,12 +294,13 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restri
   __shared__ float red[4];
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x;
+  const float unit = kLog2E / heat;
   float mx = -INFINITY, any = 0.f;
   bool bad = false;
   for (int k = tid; k < words; k += 256) {
     const int64_t word = static_cast<int64_t>(ids[r * ids_ld + k]);
     const float x = (TOP_F32 ? static_cast<const float*>(top)[r * top_ld + k]
-                             : bf16_to_f32(static_cast<const uint16_t*>(top)[r * top_ld + k])) / heat;
+                             : bf16_to_f32(static_cast<const uint16_t*>(top)[r * top_ld + k]));
     const bool there = word >= 0 && word < vocab && x != -INFINITY;
     id[k] = there ? static_cast<int32_t>(word) : kNoWord;
     q[k] = there ? x : -INFINITY;
@@ -323,7 +325,7 @@ __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restri
   mx = block_reduce<true>(bad ? INFINITY : mx, red);
   float sum = 0.f;
   for (int k = tid; k < words; k += 256) {
-    const float e = id[k] == kNoWord ? 0.f : exp2f((q[k] - mx) * kLog2E);
+    const float e = id[k] == kNoWord ? 0.f : exp2f((q[k] - mx) * unit);
     sum += e;
     q[k] = e;
   }
@@ -538,23 +540,23 @@ __device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, co
 #pragma unroll
         for (int e = 0; e < kPer; ++e) mx = fmaxf(mx, Elem<T>::get(v[i], e));
     }
-    mx = block_reduce<true>(mx, red) * unit;
+    mx = block_reduce<true>(mx, red);
 #pragma unroll
     for (int i = 0; i < LC; ++i)
       if (tid + TH * (NC + i) < full) {
         const uint4 a = more[i * TH + tid];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) sum += __builtin_amdgcn_exp2f(fmaf(Elem<T>::get(a, e), unit, -mx));
+        for (int e = 0; e < kPer; ++e) sum += __builtin_amdgcn_exp2f((Elem<T>::get(a, e) - mx) * unit);
       }
 #pragma unroll
     for (int i = 0; i < NC; ++i)
       if (tid + TH * i < full)
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) sum += __builtin_amdgcn_exp2f(fmaf(Elem<T>::get(v[i], e), unit, -mx));
-    if (tid < rest) sum += __builtin_amdgcn_exp2f(fmaf(last, unit, -mx));
+        for (int e = 0; e < kPer; ++e) sum += __builtin_amdgcn_exp2f((Elem<T>::get(v[i], e) - mx) * unit);
+    if (tid < rest) sum += __builtin_amdgcn_exp2f((last - mx) * unit);
     sum = block_reduce<false>(sum, red);
   } else {
-    mx = tid < rest ? last * unit : -INFINITY;
+    mx = last;
     sum = tid < rest ? (last == last && mx != INFINITY ? 1.f : NAN) : 0.f;
     if (tid < rest && mx == -INFINITY) sum = 0.f;
     for (int c0 = tid; c0 < full; c0 += TH * kAhead) {
@@ -565,22 +567,24 @@ __device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, co
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) m = fmaxf(m, Elem<T>::get(a[i], e) * unit);
+        for (int e = 0; e < kPer; ++e) m = fmaxf(m, Elem<T>::get(a[i], e));
       const float ref = m == -INFINITY ? 0.f : m;
-      sum *= mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - ref);  // nothing summed yet, or NaN
+      sum *= mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mx - ref) * unit);  // nothing summed yet, or NaN
       mx = m;
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
         if (c0 + TH * i < full)
 #pragma unroll
-          for (int e = 0; e < kPer; ++e) sum += __builtin_amdgcn_exp2f(fmaf(Elem<T>::get(a[i], e), unit, -ref));
+          for (int e = 0; e < kPer; ++e) sum += __builtin_amdgcn_exp2f((Elem<T>::get(a[i], e) - ref) * unit);
     }
     const float all = block_reduce<true>(mx, red);
-    sum *= mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - all);
+    sum *= mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mx - all) * unit);
     sum = block_reduce<false>(sum, red);
     mx = all;
   }
-  const float lse = mx + log2f(sum);
+  // log2 p = (z - mx) unit - lsum: the difference first, as z unit of a mask of the
+  // type's lowest value is beyond f32
+  const float lsum = log2f(sum);
   const int n = words > 0 ? words : 1;
   float cross = 0.f;
   for (int k = tid; k < n; k += TH) {
@@ -588,20 +592,20 @@ __device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, co
     const int32_t id = word_of(t, r, words, k, vocab, share);
     if (id == kUnknown) cross = NAN;
     if (id == kUnknown || share == -1.f) continue;
-    const float l = fmaf(Elem<T>::one(row[id]), unit, -lse);  // log2 p
-    at_word[k] = l;
-    if (share != 0.f) cross -= share * l;
+    const float z = Elem<T>::one(row[id]) - mx;
+    at_word[k] = fmaf(z, unit, -lsum);
+    if (share != 0.f) cross += share * (heat * (lsum * kLn2) - z);  // -T ln p
   }
   cross = block_reduce<false>(cross, red);
   // counted before the gradient is written, which its wait then overlaps
   if (tid == 0)
-    flag = put_row(o, r, w * (heat * heat * (cross * kLn2 + (words > 0 ? t.entropy[r] : 0.f))), gridDim.x);
+    flag = put_row(o, r, w * (heat * (cross + (words > 0 ? heat * t.entropy[r] : 0.f))), gridDim.x);
   if (dx == nullptr) return;
   const float c = cross == cross ? heat * w * *t.factor : NAN;
   auto grad = [&](const uint4& a, int at) {
     float o[kPer];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] = c * __builtin_amdgcn_exp2f(fmaf(Elem<T>::get(a, e), unit, -lse));
+    for (int e = 0; e < kPer; ++e) o[e] = c * __builtin_amdgcn_exp2f(fmaf(Elem<T>::get(a, e) - mx, unit, -lsum));
     store_grad(out + at * kPer, o);
   };
   if constexpr (NC > 0) {
@@ -621,7 +625,7 @@ __device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, co
         if (c0 + TH * i < full) grad(a[i], c0 + TH * i);
     }
   }
-  if (tid < rest) out[full * kPer + tid] = Elem<T>::of(c * __builtin_amdgcn_exp2f(fmaf(last, unit, -lse)));
+  if (tid < rest) out[full * kPer + tid] = Elem<T>::of(c * __builtin_amdgcn_exp2f(fmaf(last - mx, unit, -lsum)));
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stored before the words' own
   __syncthreads();
   for (int k = tid; k < n; k += TH) {
@@ -1577,6 +1581,16 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     if (rc != MOC_OK) return rc;
   }
   return loss == nullptr || (rows > 0 && arrive) ? MOC_OK : sum_loss(t, o, loss, st);
+}
+
+extern "C" int64_t moc_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(as_stream(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status == hipStreamCaptureStatusNone ? 0 : static_cast<int64_t>(id) + 1;
 }
 
 extern "C" int moc_scale_inplace(int dtype0, void* p0, int64_t n0, int dtype1, void* p1, int64_t n1,

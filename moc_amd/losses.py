@@ -144,11 +144,14 @@ class _Teacher:
 
     def rows_f32(self, saved, z):
         ids, top, _ = saved
-        ids, x = ids.long(), top.float() / self.heat
+        ids, x = ids.long(), top.float()
         there = (ids >= 0) & (ids < z.shape[1]) & (x != -math.inf)
         counts = there.any(1)
+        # from the largest, as masks of the type's lowest value over a T below 1 are beyond f32
+        x = torch.where(counts[:, None], torch.where(there, x, -math.inf), 0.0)
+        log_q = torch.log_softmax((x - x.amax(1, keepdim=True)) / self.heat, 1)
         z = torch.where(counts[:, None], z, 0.0)
-        log_q = torch.log_softmax(torch.where(counts[:, None], torch.where(there, x, -math.inf), 0.0), 1)
+        z = z - z.detach().amax(1, keepdim=True)
         q = torch.where(there, log_q.exp(), 0.0)
         ids = torch.where(there, ids, 0)
         # shares of one word added up, each entry weighing its own part of them
@@ -185,19 +188,24 @@ def _unit(t):
 
 
 # -------------------------------------------------------------------- operands
-def _rows16(t) -> torch.Tensor:
+def _rows16(t, most: int = 1 << 62) -> torch.Tensor:
     """t [rows, cols] with 16-byte aligned rows of unit stride, at most four times their
-    length apart, whose storage holds all of the last one's pitch (the kernels read
-    whole chunks); a copy of any other."""
+    length apart and bf16 ones within `most` bytes, whose storage holds all of the last
+    one's pitch (the kernels read whole chunks); a copy of any other."""
     rows, cols = t.shape
     per = 16 // t.element_size()
     pitch = _pitch(t)
     if (t.stride(1) == 1 or cols == 1) and t.data_ptr() % 16 == 0 and pitch % per == 0 and (
-            cols <= pitch <= 4 * K.round_up(cols, 64)) and (
+            cols <= pitch <= 4 * K.round_up(cols, 64)) and (t.dtype != BF16 or rows * pitch * 2 < most) and (
             (t.storage_offset() + rows * pitch) * t.element_size() <= t.untyped_storage().nbytes()):
         return t
+    t, ld = K._rows_view(t)
+    if ld < cols:  # rows that overlap
+        t, ld = t.contiguous(), cols
     out = K.padded_empty(rows, cols, t.dtype, t.device)
-    return out.copy_(t)
+    N.call("moc_copy_pad_2d", N.dtype_code(t.dtype), t.data_ptr(), rows, cols, ld, out.data_ptr(), out.stride(0),
+           out.stride(0), N.stream_of(t))
+    return out
 
 
 def _pitch(t) -> int:
@@ -274,7 +282,7 @@ def _linear_pass(targets, saved, row_weight, mean, grad, product, hidden, weight
         h = h.to(product)
     if w.dtype != product:
         w = w.to(product)
-    h, w = _rows16(h), _rows16(w)
+    h, w = _rows16(h), _rows16(w, K.OPERAND_BYTES)
     rows, code = h.shape[0], N.dtype_code(product)
     out = torch.empty(rows if each else (), dtype=F32, device=where)
     dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=where) if dh else None
@@ -301,6 +309,11 @@ def _reduced_f32(targets, saved, z):
     return each.sum() / (w.sum() if targets.reduction == "mean" else 1.0)
 
 
+def _capture(dev: int) -> int:
+    """What names the HIP graph that the current stream is captured into, or 0."""
+    return N.query("moc_capture_id", N.stream_on(dev)) if torch.cuda.is_current_stream_capturing() else 0
+
+
 class _Kept:
     """Gradients computed ahead, handed out once: the tensors go to the caller, scaled
     in place, so that nothing of them is copied."""
@@ -313,13 +326,14 @@ class _Kept:
             self.scaled = (N.dtype_code(a.dtype), a.data_ptr(), a.numel(), N.dtype_code(b.dtype), b.data_ptr(),
                            b.numel() if len(given) > 1 else 0)
             self.device = a.get_device()
-            self.captured = torch.cuda.is_current_stream_capturing()
+            self.capture = _capture(self.device)
 
     def take(self, g):
-        """The gradients times g, or None: there are none, or no more, or those of an
-        eager forward in a captured backward, which a replay would scale again."""
+        """The gradients times g, or None: there are none, or no more, or those of a
+        forward outside the capture of this backward, whose replay would scale them
+        again."""
         grads, self.grads = self.grads, None
-        if grads is None or (not self.captured and torch.cuda.is_current_stream_capturing()):
+        if grads is None or ((now := _capture(self.device)) and now != self.capture):
             return None
         N.call("moc_scale_inplace", *self.scaled, g.data_ptr(), N.stream_on(self.device))
         return grads
@@ -328,7 +342,7 @@ class _Kept:
 def _row_factors(saved, g):
     """reduction="none": the rows' weights times their upstream gradients."""
     g = g.reshape(-1).contiguous()
-    return g if saved[2] is None else g * saved[2]
+    return g if saved[2] is None else torch.where(saved[2] == 0, 0.0, g * saved[2])  # NaN g in rows without weight
 
 
 class _LinearLoss(torch.autograd.Function):

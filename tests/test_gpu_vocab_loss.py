@@ -589,3 +589,125 @@ def test_refusals_on_the_device():
         L.linear_cross_entropy(h, w, y.cpu())
     with pytest.raises(ValueError, match="one type"):
         L.linear_cross_entropy(h, w.to(BF), y)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("vocab", [500, 4099, 50021, 270011])
+@pytest.mark.parametrize("words,heat", [(7, 1.0), (7, 0.5), (300, 2.0)])
+def test_lowest_value_in_masked_places(vocab, dtype, words, heat):
+    """Masks of the type's lowest value, which f32 does not hold in other units: in half
+    of a row's logits, in all of them, in a word's, in some of a teacher's words, in
+    all of them."""
+    low = torch.finfo(dtype).min
+    g = torch.Generator().manual_seed(vocab + words)
+    x = (3 * torch.randn(5, vocab, generator=g)).to(dtype)
+    ids = torch.stack([torch.randperm(vocab, generator=g)[:words] for _ in range(5)])
+    top = torch.randn(5, words, generator=g).to(dtype)
+    masked = torch.rand(vocab, generator=g) < 0.5
+    masked[ids[0]] = False
+    x[0, masked] = low
+    x[1] = low
+    top[2, 0] = top[2].min() - 1
+    x[2, ids[2, 0]] = low
+    top[3, words // 2:] = low
+    top[4] = low
+    x, ids, top = x.cuda().requires_grad_(), ids.cuda(), top.cuda()
+    out = L.distillation_loss(x, ids, top, temperature=heat, reduction="none")
+    got = torch.autograd.grad(out.sum(), x)[0]
+    z = x.detach().to(F64)
+    q = torch.zeros(5, vocab, dtype=F64, device="cuda").scatter_(1, ids, torch.softmax(top.to(F64) / heat, 1))
+    ones = torch.ones(5, dtype=F64, device="cuda")
+    want, dz, c = reference(z, q, ones != 0, ones, heat, "none")
+    top_z = torch.where(z < -1e30, 0.0, z).abs().max().item() / heat
+    rel = 2.0 ** -20 + 4 * 2.0 ** -24 * (top_z + 20)
+    tol = rel * heat ** 2 * (want.abs() / heat ** 2 + math.log(2 * vocab) + top_z)
+    assert ((out.detach().to(F64) - want).abs() <= tol).all()
+    tol = 8 * rel * (dz.abs() + c * q) + (2.0 ** -8 if dtype == BF else 2.0 ** -23) * dz.abs() + 1e-38
+    err = (got.to(F64) - dz).abs()
+    assert (err <= tol).all(), (err / tol).max()
+    again = torch.autograd.grad(L.distillation_loss(x, ids, top, temperature=heat, reduction="none").sum(), x,
+                                create_graph=True)[0]
+    # f32 operations: z / T and their sums round like the operator's
+    assert ((again.to(F64) - dz).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+def test_upstream_nan_in_rows_that_do_not_count(op):
+    """A masked mean's where() sends NaN or infinity to rows of weight 0."""
+    h, w = operands(40, 64, 900, BF)
+    ids, top = teacher_of(40, 900, 5, True)
+    y = labels_of(40, 900, 0.2)
+    weight = rand(40, seed=4).abs() + 0.5
+    weight[::3] = 0
+    x = (3 * rand(40, 900, seed=1)).to(BF)
+    leaves = (x,) if op == "kept" else (h, w)
+    for t in leaves:
+        t.requires_grad_()
+    each = L.linear_cross_entropy(h, w, y, weight, reduction="none") if op == "entropy" else (
+        L.linear_distillation(h, w, ids, top, weight, reduction="none") if op == "teacher" else
+        L.distillation_loss(x, ids, top, weight, reduction="none"))
+    g, dead = rand(40, seed=2), weight == 0
+    want = torch.autograd.grad(each, leaves, torch.where(dead, 0.0, g), retain_graph=True)
+    for value in (math.nan, math.inf):
+        got = torch.autograd.grad(each, leaves, torch.where(dead, value, g), retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("op", ["entropy", "kept"])
+def test_forward_and_backward_in_two_graphs(op):
+    """The backward's graph, replayed twice behind one replay of the forward's, gives
+    the same gradients twice."""
+    h, w = operands(130, 128, 2000, BF)
+    ids, top = teacher_of(130, 2000, 8, True)
+    y = labels_of(130, 2000, 0.2)
+    x = (3 * rand(130, 2000, seed=1)).to(BF)
+    factor = torch.tensor(2.0, device="cuda")
+    leaves = (x,) if op == "kept" else (h, w)
+    for t in leaves:
+        t.requires_grad_()
+
+    def forward():
+        return L.distillation_loss(x, ids, top) if op == "kept" else L.linear_cross_entropy(h, w, y)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(forward(), leaves, factor)
+        torch.cuda.synchronize()
+        first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(first, stream=side):
+            loss = forward()
+        with torch.cuda.graph(second, pool=first.pool(), stream=side):
+            got = torch.autograd.grad(loss, leaves, factor)
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(3):
+        with torch.no_grad():
+            for t in leaves:
+                t.copy_((t.float() * (0.9 + 0.1 * i)).to(BF))
+        want = torch.autograd.grad(forward(), leaves, factor)
+        first.replay()
+        for _ in range(2):
+            second.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+def test_weight_rows_far_apart():
+    """A view whose rows' pitch passes what the products address: a copy of it."""
+    vocab, d = 131100, 2048
+    w = torch.empty(vocab, 4 * d, dtype=BF, device="cuda")[:, :d].copy_(rand(vocab, d, seed=1) / 40)
+    h, y = rand(3, d, seed=2).to(BF), torch.tensor([5, vocab - 1, 70000], device="cuda")
+    assert torch.equal(L.linear_cross_entropy(h, w, y, reduction="none"),
+                       L.linear_cross_entropy(h, w.contiguous(), y, reduction="none"))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rows_that_overlap(dtype):
+    """Expanded rows and windows of one buffer."""
+    base = rand(400, seed=3).to(dtype)
+    w = operands(1, 30, 300, dtype)[1].requires_grad_()
+    y = labels_of(40, 300, 0.1)
+    for h in (base[:30].expand(40, 30), base.as_strided((40, 30), (5, 1), 3), base.as_strided((40, 30), (1, 7))):
+        out, same = L.linear_cross_entropy(h, w, y), L.linear_cross_entropy(h.contiguous(), w, y)
+        assert torch.equal(out, same)
+        assert torch.equal(*(torch.autograd.grad(t, w)[0] for t in (out, same)))
