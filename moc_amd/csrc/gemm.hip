@@ -2385,8 +2385,11 @@ PairSplitPlan plan_split_pair(int64_t M1, int64_t N1, int nk1, int64_t M2, int64
 
 }  // namespace
 
-// Logits h w^T of a loss (see GemmArgs::ls_stat and abi.h).  128-row tiles where
-// 256-row ones would leave half of the CUs idle.
+// Logits h w^T of a loss (see GemmArgs::ls_stat and abi.h).  A 128-row tile takes
+// about four fifths of a 256-row one's time (hidden size, us with 256 / 128 rows:
+// 64 / 128 tiles of 8192 words, 1024: 26 / 20; 128 / 256, 512: 18 / 13; 196 / 196 of
+// 50021 words and 128 rows, 768: 24 / 18), so it is taken where its rounds of the CUs
+// come to less.
 int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab,
                      int64_t ldw, float unit, const int32_t* ids, int64_t ld_ids, const uint16_t* first,
                      int64_t ld_first, int64_t words, float* z, float2* stat, void* kept, int64_t ld_kept, hipStream_t st) {
@@ -2405,8 +2408,10 @@ int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, c
   a.ldc = ld_kept;
   a.tiles_m = static_cast<int>((rows + kBM - 1) / kBM);
   a.tiles_n = static_cast<int>((vocab + kBN - 1) / kBN);
-  const bool short_m = 2LL * a.tiles_m * a.tiles_n <= cu_count();
-  if (short_m) a.tiles_m = static_cast<int>((rows + 127) / 128);
+  const int64_t tiles_128 = (rows + 127) / 128;
+  auto rounds = [&](int64_t m) { return (m * a.tiles_n + cu_count() - 1) / cu_count(); };
+  const bool short_m = 4 * rounds(tiles_128) < 5 * rounds(a.tiles_m);
+  if (short_m) a.tiles_m = static_cast<int>(tiles_128);
   if (static_cast<int64_t>(a.tiles_m) * a.tiles_n >= (1LL << 31)) return 1;
   a.pp = 1;
   a.ksplit = 1;

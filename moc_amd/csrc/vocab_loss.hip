@@ -506,18 +506,24 @@ __device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, co
   const float w = weight_of(t, r);
   const T* row = x + blockIdx.x * ld;
   T* out = dx + blockIdx.x * ldd;
-  const int full = vocab / kPer, rest = vocab % kPer;  // whole chunks, elements behind them
+  // whole chunks, from the first 16-byte boundary on, and the `loose` elements before and
+  // behind them, a thread each
+  const int head = min(vocab, static_cast<int>(-(reinterpret_cast<uintptr_t>(row) / sizeof(T)) & (kPer - 1)));
+  const int full = (vocab - head) / kPer, loose = vocab - full * kPer;
+  const int lone = tid < head ? tid : full * kPer + tid;  // this thread's, tid < loose
+  const T* chunks = row + head;
+  T* out_chunks = out + head;
   if (w == 0.f) {                                      // uniform
     if (dx != nullptr) {
       const float zero[kPer] = {};
-      for (int c = tid; c < full; c += TH) store_grad(out + c * kPer, zero);
-      if (tid < rest) out[full * kPer + tid] = Elem<T>::of(0.f);
+      for (int c = tid; c < full; c += TH) store_grad(out_chunks + c * kPer, zero);
+      if (tid < loose) out[lone] = Elem<T>::of(0.f);
     }
     if (tid == 0) flag = put_row(o, r, 0.f, gridDim.x);
     return;
   }
   const float unit = kLog2E / heat;
-  const float last = tid < rest ? Elem<T>::one(row[full * kPer + tid]) : -INFINITY;
+  const float last = tid < loose ? Elem<T>::one(row[lone]) : -INFINITY;
   uint4 v[NC > 0 ? NC : 1];
   __shared__ uint4 more[LC > 0 ? LC * TH : 1];  // chunks NC .. NC + LC of each thread, read by it alone
   float mx = last, sum = 0.f;
@@ -526,7 +532,7 @@ __device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, co
       // behind the end a thread reads the last chunk again, which leaves the maximum
       // and is not summed
 #pragma unroll
-      for (int i = 0; i < LC; ++i) v[i] = load_chunk(row + min(tid + TH * (NC + i), full - 1) * kPer);
+      for (int i = 0; i < LC; ++i) v[i] = load_chunk(chunks + min(tid + TH * (NC + i), full - 1) * kPer);
 #pragma unroll
       for (int i = 0; i < LC; ++i) {
 #pragma unroll
@@ -534,7 +540,7 @@ __device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, co
         more[i * TH + tid] = v[i];
       }
 #pragma unroll
-      for (int i = 0; i < NC; ++i) v[i] = load_chunk(row + min(tid + TH * i, full - 1) * kPer);
+      for (int i = 0; i < NC; ++i) v[i] = load_chunk(chunks + min(tid + TH * i, full - 1) * kPer);
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
@@ -553,17 +559,17 @@ __device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, co
       if (tid + TH * i < full)
 #pragma unroll
         for (int e = 0; e < kPer; ++e) sum += __builtin_amdgcn_exp2f((Elem<T>::get(v[i], e) - mx) * unit);
-    if (tid < rest) sum += __builtin_amdgcn_exp2f((last - mx) * unit);
+    if (tid < loose) sum += __builtin_amdgcn_exp2f((last - mx) * unit);
     sum = block_reduce<false>(sum, red);
   } else {
     mx = last;
-    sum = tid < rest ? (last == last && mx != INFINITY ? 1.f : NAN) : 0.f;
-    if (tid < rest && mx == -INFINITY) sum = 0.f;
+    sum = tid < loose ? (last == last && mx != INFINITY ? 1.f : NAN) : 0.f;
+    if (tid < loose && mx == -INFINITY) sum = 0.f;
     for (int c0 = tid; c0 < full; c0 += TH * kAhead) {
       uint4 a[kAhead];
       float m = mx;
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) a[i] = load_chunk(row + min(c0 + TH * i, full - 1) * kPer);
+      for (int i = 0; i < kAhead; ++i) a[i] = load_chunk(chunks + min(c0 + TH * i, full - 1) * kPer);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
 #pragma unroll
@@ -606,7 +612,7 @@ __device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, co
     float o[kPer];
 #pragma unroll
     for (int e = 0; e < kPer; ++e) o[e] = c * __builtin_amdgcn_exp2f(fmaf(Elem<T>::get(a, e) - mx, unit, -lsum));
-    store_grad(out + at * kPer, o);
+    store_grad(out_chunks + at * kPer, o);
   };
   if constexpr (NC > 0) {
 #pragma unroll
@@ -619,13 +625,13 @@ __device__ __forceinline__ void logits_row(const T* x, int64_t ld, int vocab, co
     for (int c0 = tid; c0 < full; c0 += TH * kAhead) {
       uint4 a[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) a[i] = load_chunk(row + min(c0 + TH * i, full - 1) * kPer);
+      for (int i = 0; i < kAhead; ++i) a[i] = load_chunk(chunks + min(c0 + TH * i, full - 1) * kPer);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
         if (c0 + TH * i < full) grad(a[i], c0 + TH * i);
     }
   }
-  if (tid < rest) out[full * kPer + tid] = Elem<T>::of(c * __builtin_amdgcn_exp2f(fmaf(last - mx, unit, -lsum)));
+  if (tid < loose) out[lone] = Elem<T>::of(c * __builtin_amdgcn_exp2f(fmaf(last - mx, unit, -lsum)));
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // stored before the words' own
   __syncthreads();
   for (int k = tid; k < n; k += TH) {
