@@ -1262,6 +1262,19 @@ int run_teacher(const Teacher& a, int64_t rows, int64_t words, int64_t vocab, co
 
 constexpr int moc_th(int th, int = 0) { return th; }
 
+// The smallest of these that holds a row, so that few of its loads repeat the last
+// chunk, and two workgroups or more on a CU (up to 128 registers, 80 KB of LDS), since
+// one alone leaves the memory idle while it computes.  us, one / the next:
+//   bf16    8000 words x 8192 rows  (4, 256)      55 / (4, 512)        85
+//          16000       x 8192       (8, 256)     109 / (4, 512)       121
+//          32000       x 8192       (8, 512)     205 / (16, 256)      211, (8, 1024) 334, read twice 317
+//          40000       x 4096       (12, 512)    135 / (8, 512, 8)    148, (8, 1024) 193
+//          50021       x 4096       (8, 512, 8)  176 / (16, 512)      180, (8, 1024) 228
+//          80000       x 2048       (16, 512, 8) 143 / (24, 512, 8)   148, (16, 1024) 181
+//         128256       x 2048       (24, 512, 8) 214 / (16, 1024)     253
+//   f32   128256       x 2048       (24, 1024, 8) 415 / read twice    507
+//         262144       x 1024       read twice by 1024 threads 579 / by 512 625
+// (32000 x 8192 in bf16: 5.1 TB/s, 128256 x 2048 in f32: 5.1).
 template <typename T>
 void launch_logits(const T* x, int64_t rows, int vocab, int64_t ld, const Targets& t, int64_t r0, int words, float heat,
                    const LossOut& o, T* dx, int64_t ldd, hipStream_t st) {
@@ -1271,10 +1284,12 @@ void launch_logits(const T* x, int64_t rows, int vocab, int64_t ld, const Target
   logits_loss_kernel<T, NC, __VA_ARGS__><<<grid, moc_th(__VA_ARGS__), 0, st>>>(x, ld, vocab, t, r0, words, heat, o, dx, \
                                                                                ldd)
   if (chunks <= 4 * 256) MOC_LOGITS(4, 256);
-  else if (chunks <= 4 * 512) MOC_LOGITS(4, 512);
+  else if (chunks <= 8 * 256) MOC_LOGITS(8, 256);
   else if (chunks <= 8 * 512) MOC_LOGITS(8, 512);
-  else if (chunks <= 8 * 1024) MOC_LOGITS(8, 1024);
-  else if (chunks <= 16 * 1024) MOC_LOGITS(16, 1024);
+  else if (chunks <= 12 * 512) MOC_LOGITS(12, 512);
+  else if (chunks <= 16 * 512) MOC_LOGITS(8, 512, 8);
+  else if (chunks <= 24 * 512) MOC_LOGITS(16, 512, 8);
+  else if (chunks <= 32 * 512) MOC_LOGITS(24, 512, 8);
   else if (chunks <= 32 * 1024) MOC_LOGITS(24, 1024, 8);
   else MOC_LOGITS(0, 1024);
 #undef MOC_LOGITS

@@ -711,3 +711,30 @@ def test_rows_that_overlap(dtype):
         out, same = L.linear_cross_entropy(h, w, y), L.linear_cross_entropy(h.contiguous(), w, y)
         assert torch.equal(out, same)
         assert torch.equal(*(torch.autograd.grad(t, w)[0] for t in (out, same)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("vocab", [7001, 12000, 20001, 40003, 80001])
+def test_distillation_loss_of_other_widths(vocab, dtype):
+    """Row widths between those of test_distillation_loss: other shares of a row in
+    registers and LDS."""
+    test_distillation_loss(3, vocab, dtype, 20, 2.0, True, "mean")
+    test_distillation_loss(3, vocab, dtype, 300, 0.7, False, "none")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("vocab", [5, 1003, 50021])
+def test_rows_at_any_offset(vocab, dtype):
+    """Views whose rows start anywhere in a 16-byte chunk give what copies give."""
+    x = (3 * rand(4, vocab, seed=1)).to(dtype)
+    ids, top = teacher_of(4, vocab, 6, False)
+    want = None
+    for ahead in range(9):
+        v = torch.zeros(4, vocab + 11, dtype=dtype, device="cuda")[:, ahead:ahead + vocab].copy_(x).requires_grad_()
+        out = L.distillation_loss(v, ids, top, reduction="none")
+        got = (out.detach(), torch.autograd.grad(out.sum(), v)[0])
+        want = want or got
+        # the sum's order goes by the chunks: 2^-20 of the terms, as everywhere here
+        assert torch.allclose(got[0], want[0], rtol=2.0 ** -20, atol=2.0 ** -20 * math.log(2 * vocab))
+        step = 2.0 ** -7 if dtype == BF else 2.0 ** -20  # one bf16 step where the f32 values differ
+        assert ((got[1] - want[1]).abs().float() <= step * want[1].abs().float() + 2.0 ** -20 * 2).all()
