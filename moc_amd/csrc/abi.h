@@ -47,20 +47,20 @@ int launch_gate_up_2of8(const void* x, int64_t nb, int64_t hidden, const void* w
                         int64_t ld_ap = 0, uint32_t* meta = nullptr, int64_t meta_rows = 0);
 
 // Logits h w^T (bf16, 16-byte aligned rows) of a loss over the vocabulary, not
-// stored (gemm.hip): per row and slab of 64 words the maximum of x = unit logit and
-// the sum of exp2(x - it) (stat [rows][ceil(vocab / 64)]); exp2(x - it + 15) as f16
+// stored (gemm.hip): per row and slab of 64 words the maximum of x = unit logit, rounded
+// up to an integer, and the sum of exp2(x - it) (stat [rows][ceil(vocab / 64)]); exp2(x - it + 15) as f16
 // (kept, rows a multiple of 64 apart; null: no); the logits of the words ids
-// [rows][words] (rows ld_ids apart, ascending) in z [rows][words], first [slabs + 1][ld_first]: how many of a row's
-// lie left of each slab (null for one word).  1: operands too large for its 32-bit
-// offsets (nothing launched).
+// [rows][words] (rows ld_ids apart, ascending) in z [rows][words], first [slabs + 1]
+// [ld_first]: how many of a row's lie left of each slab (null for one word).  1:
+// operands too large for its 32-bit offsets (nothing launched).
 constexpr int kLossSlab = 64;
 int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab,
                      int64_t ldw, float unit, const int32_t* ids, int64_t ld_ids, const uint16_t* first,
                      int64_t ld_first, int64_t words, float* z, float2* stat, void* kept, int64_t ld_kept, hipStream_t st);
 
-// C [M, N] = *alpha A B (f16 operands; alpha null: A B, bf16; A with a unit stride along M or K, rows of B
-// ldb apart; C bf16 or f32) (gemm.hip); 16-byte aligned rows, workspace as
-// moc_gemm_ws uses it.
+// C [M, N] = *alpha A B (f16 operands; alpha null: A B, bf16; A with a unit stride along
+// M or K, rows of B ldb apart; C bf16 or f32) (gemm.hip); 16-byte aligned rows,
+// workspace as moc_gemm_ws uses it.
 int64_t gemm_half_workspace(int64_t M, int64_t N, int64_t K);
 int gemm_half(int64_t M, int64_t N, int64_t K, const void* A, int64_t a_sm, int64_t a_sk, const void* B, int64_t ldb,
               void* C, int64_t ldc, int c_dtype, const float* alpha, void* workspace, int64_t workspace_bytes,

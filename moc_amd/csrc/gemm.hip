@@ -169,11 +169,13 @@ struct GemmArgs {
   void* grp_C;
   int64_t grp_ldc, grp_ws_stride;
   // Logits of a loss (gemm_pp_kernel<..., LOSS = true>): C is not stored, but per
-  // row and slab of 64 columns the maximum m of x = unit C and the sum of exp2(x - m)
+  // row and slab of 64 columns the maximum m of x = unit C, rounded up to an integer
+  // (shifts by it and differences of two are exact), and the sum of exp2(x - m)
   // (ls_stat [M][ls_slabs]), the exponentials as f16 (C, rows ldc apart, null: not
   // kept) and C itself in f32 (ls_z [M][ls_words]) at the columns named by ls_ids
-  // [M][ls_words] (rows ls_ld_ids apart, ascending; others than columns: none; ls_first [ls_slabs + 1][ls_ld_first]: how many
-  // of a row's lie left of each slab, null for one a row).
+  // [M][ls_words] (rows ls_ld_ids apart, ascending; others than columns: none;
+  // ls_first [ls_slabs + 1][ls_ld_first]: how many of a row's lie left of each slab,
+  // null for one a row).
   float2* ls_stat;
   int ls_slabs, ls_words;
   float ls_unit;
@@ -958,8 +960,9 @@ static_assert(kLossStage + 8 * 32 * (64 * 2 + 16) <= kRingBytes, "LOSS: staging 
 // slab's maximum and sum are 31 operations in the lane and one exchange.  What is
 // kept for the gradient is exp2(x - m + 15) as f16: 11 bits, where bf16 would add an
 // error as large as the gradient's own rounding; 2^15 moves f16's range so that
-// values down to 2^-29 of the slab's largest keep all of them and none below 2^-40
-// counts.  Measured at 4096 x 32000 x 2048: see launch_loss_gemm.
+// values down to 2^-28 of the slab's largest keep all of them and none below 2^-39
+// counts.  A tile of 256 x 256 takes 1.3 us a K tile of 64 and 8 more for the
+// statistics, 12 with what is kept.
 template <int MI>
 __device__ __forceinline__ void loss_epilogue(const GemmArgs& g, char* lds, f32x16_t (&acc)[MI][2], int row0,
                                               int col0, int wm, int wn, int wave, int lane) {
@@ -1021,7 +1024,7 @@ __device__ __forceinline__ void loss_epilogue(const GemmArgs& g, char* lds, f32x
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
-    m = fmaxf(m, __shfl_xor(m, 32)) * g.ls_unit;
+    m = ceilf(fmaxf(m, __shfl_xor(m, 32)) * g.ls_unit);
     const float ref = m == -INFINITY ? 0.f : m - 15.f;
     float s = 0.f;
 #pragma unroll
@@ -2389,7 +2392,9 @@ PairSplitPlan plan_split_pair(int64_t M1, int64_t N1, int nk1, int64_t M2, int64
 // about four fifths of a 256-row one's time (hidden size, us with 256 / 128 rows:
 // 64 / 128 tiles of 8192 words, 1024: 26 / 20; 128 / 256, 512: 18 / 13; 196 / 196 of
 // 50021 words and 128 rows, 768: 24 / 18), so it is taken where its rounds of the CUs
-// come to less.
+// come to less.  A workgroup takes several tiles in turn, the next one's first loads in
+// flight during the epilogue: 16384 x 2048 x 32000 1.85 ms with what is kept (1160
+// TFLOP/s), 1.64 without; 4099 x 768 x 50021 0.32 without (980).
 int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab,
                      int64_t ldw, float unit, const int32_t* ids, int64_t ld_ids, const uint16_t* first,
                      int64_t ld_first, int64_t words, float* z, float2* stat, void* kept, int64_t ld_kept, hipStream_t st) {
@@ -2908,12 +2913,12 @@ namespace moc {
 // C [M, N] = *alpha A B, A (a_sm, a_sk: one of them 1) and B [K, N] (rows of ldb)
 // in f16 (alpha null: C = A B of bf16), C in bf16 or f32: the gradients of a product
 // whose own gradient needs more than bf16's 8 bits.  As moc_gemm_ws, f16 at the same
-// rate, but K is
-// split up to 8 ways or in multiples of 8: workgroup ids go to the XCDs in turn, so a
-// K range then stays in one XCD's L2, where 9 ways have every XCD read every range
-// (777 x 512 x 32000, bf16: 76 us in 9 parts, 36 in 8); and rows of C that are not
-// 16-byte aligned are stored in 16-byte pieces all the same, which the memory takes at
-// any address (a gradient of 16921 x 1500 over 44 rows: 54 us with
+// rate (16384 x 2048 x 32000 1.64 ms, 32000 x 2048 x 16384 1.68: 1310 and 1280
+// TFLOP/s), but K is split up to 8 ways or in multiples of 8: workgroup ids go to the
+// XCDs in turn, so a K range then stays in one XCD's L2, where 9 ways have every XCD
+// read every range (777 x 512 x 32000, bf16: 76 us in 9 parts, 36 in 8); and rows of C
+// that are not 16-byte aligned are stored in 16-byte pieces all the same, which the
+// memory takes at any address (a gradient of 16921 x 1500 over 44 rows: 54 us with
 // 2-byte stores, 22).
 int64_t gemm_half_workspace(int64_t M, int64_t N, int64_t K) {
   const int nk = static_cast<int>((K + kBK - 1) / kBK);

@@ -13,6 +13,20 @@
 // Logits are in units of log2(e) / T where they meet an exponential, which then is
 // one v_exp_f32.  Sums over rows are in 64 bits and in a fixed
 // order.
+//
+// A linear loss in bf16, by pieces of the rows (pieces_of), a row with all its words in
+// one piece: with pieces of the words the gradient would need the logits a second time.
+//   1. a teacher's words sorted, shares of one word added up (teacher_wave_kernel)
+//   2. hidden rows and weight in f16 (halves_kernel), where there are gradients
+//   3. the logits' product, of which the maximum and the sum of exponentials of every
+//      64 words are kept, the exponentials as f16 and the targets' logits
+//      (launch_loss_gemm)
+//   4. each row's loss, and the exponentials into gradients of the logits, in place
+//      (slabs_grad_kernel; slabs_loss_kernel without)
+//   5. the products for dhidden and dweight (gemm_half)
+// 16384 x 2048 x 32000: 5.7 ms, the three products 1.85, 1.64 and 1.68 (1160 to 1310
+// TFLOP/s; 6.44e12 FLOP take 4.75 at a large library product's rate), (4) 0.43 at 4.9
+// TB/s, (2) 0.07.
 #include "abi.h"
 #include "common.h"
 
@@ -181,9 +195,10 @@ __device__ __forceinline__ void put_total(const Targets& t, int64_t rows, int me
 }
 
 // A teacher's rows of up to 64 W words, a wave a row, W words a lane: sorted by rank
-// (ties by place), entries of one word made one.  Four rows a workgroup: its
-// comparisons keep a SIMD busy (256 words, 807 rows: 47 us with 16).  counter (null: not here): the last
-// workgroup sums the weights.
+// (ties by place), entries of one word made one.  Bound by words^2 comparisons: four
+// rows a workgroup spread them over the CUs (807 rows of 256 words 12 us, 47 with 16
+// rows a workgroup; 8192 of 64 8.3).  counter (null: not here): the last workgroup sums
+// the weights.
 template <typename ID, bool TOP_F32, int W>
 __global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict__ ids, int64_t ids_ld,
                                                             const void* __restrict__ top, int64_t top_ld, int64_t rows,
@@ -282,8 +297,8 @@ __global__ __launch_bounds__(256) void teacher_wave_kernel(const ID* __restrict_
   if (flag) put_total<true>(t, rows, mean, grad, red64, red);
 }
 
-// One workgroup a row.  Words sorted by rank (ties by place); entries of the
-// same word become one with the sum of their shares.
+// The same for more words, one workgroup a row (256 words, us, 807 / 4096 rows: 16 /
+// 44, by waves 12 / 26).
 template <typename ID, bool TOP_F32>
 __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restrict__ ids, int64_t ids_ld,
                                                               const void* __restrict__ top, int64_t top_ld, int words,
@@ -656,7 +671,9 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
 // Up to 16 rows, losses alone: the weight is read once, straight into the operand
 // registers of v_mfma_f32_16x16x32_bf16 (a wave 16 words, a workgroup a slab of 64),
 // 16 loads ahead; the rows stand in LDS in fragment order.  Bound by the weight's
-// bytes: few_us below.
+// bytes: 32000 x 2048, 1 row 26.3 us, 5.0 TB/s, 16 rows 27.6 (through the tiled
+// product 30.3 and 30.7); 128256 x 1024, 16 rows 49.7, 5.3 TB/s (53.4); 128256 x 4096,
+// 4 rows 204, 5.2 TB/s (226).
 constexpr int kFewRows = 16, kFewAhead = 16, kFewHidden = 4096;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -725,15 +742,15 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
     float m = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      acc[e] = slab * kLossSlab + c0 + e < vocab ? acc[e] * unit : -INFINITY;
+      acc[e] = slab * kLossSlab + c0 + e < vocab ? acc[e] : -INFINITY;
       m = fmaxf(m, acc[e]);
     }
     m = fmaxf(m, __shfl_xor(m, 16));
-    m = fmaxf(m, __shfl_xor(m, 32));
+    m = ceilf(fmaxf(m, __shfl_xor(m, 32)) * unit);  // as in launch_loss_gemm's statistics
     const float ref = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(acc[e] - ref);
+    for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(fmaf(acc[e], unit, -ref));
     s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
     if (lane < 16) part[(turn * 4 + wave) * 16 + row] = make_float2(m, s);
@@ -753,9 +770,15 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
   }
 }
 
-// log2 of a row's sum of exponentials from its slabs' maxima and sums; 256 threads,
-// a slab's loads in flight with its seven followers'.
-__device__ __forceinline__ float slabs_lse(const float2* __restrict__ stat, int slabs, float* red) {
+// A row's sum of exponentials from its slabs' references and sums: the largest
+// reference, and log2 of the sum against it (one number would be rounded at the
+// reference's size, and a small loss with it); 256 threads, a slab's loads in flight
+// with its seven followers'.
+struct Lse {
+  float ref, log2_sum;
+};
+
+__device__ __forceinline__ Lse slabs_lse(const float2* __restrict__ stat, int slabs, float* red) {
   float m = -INFINITY, s = 0.f;
   for (int i0 = threadIdx.x; i0 < slabs; i0 += 256 * 8) {
     float2 v[8];
@@ -774,20 +797,20 @@ __device__ __forceinline__ float slabs_lse(const float2* __restrict__ stat, int 
   const float all = block_reduce<true>(m, red);
   s *= m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - all);
   s = block_reduce<false>(s, red);
-  return all + log2f(s);
+  return {all, log2f(s)};
 }
 
 // A row's cross entropy sum q (-log2 p) over the words this thread takes, log2 p of
 // each into at_word (may be null); NaN for an unknown label.  z: its words' logits.
 __device__ __forceinline__ float cross_of(const Targets& t, int64_t r, int words, int vocab,
-                                          const float* __restrict__ z, float unit, float lse, float* at_word) {
+                                          const float* __restrict__ z, float unit, const Lse& lse, float* at_word) {
   float cross = 0.f;
   for (int k = threadIdx.x; k < (words > 0 ? words : 1); k += 256) {
     float share;
     const int32_t id = word_of(t, r, words, k, vocab, share);
     if (id == kUnknown) cross = NAN;
     if (id == kUnknown || share == -1.f) continue;
-    const float l = z[k] * unit - lse;
+    const float l = fmaf(z[k], unit, -lse.ref) - lse.log2_sum;
     if (at_word != nullptr) at_word[k] = l;
     if (share != 0.f) cross -= share * l;
   }
@@ -804,7 +827,8 @@ struct Slabs {
   float heat;
 };
 
-// Losses alone: one workgroup a row.
+// Losses alone: one workgroup a row, bound by latency (4099 rows of 782 slabs, 26 MB:
+// 11 us).
 __global__ __launch_bounds__(256) void slabs_loss_kernel(Slabs s, Targets t, LossOut o) {
   __shared__ float red[4];
   __shared__ double red64[4];
@@ -813,7 +837,7 @@ __global__ __launch_bounds__(256) void slabs_loss_kernel(Slabs s, Targets t, Los
   const float w = weight_of(t, r);
   float loss = 0.f;
   if (w != 0.f) {  // uniform
-    const float lse = slabs_lse(s.stat + static_cast<int64_t>(blockIdx.x) * s.count, s.count, red);
+    const Lse lse = slabs_lse(s.stat + static_cast<int64_t>(blockIdx.x) * s.count, s.count, red);
     const float* z = s.z + static_cast<int64_t>(blockIdx.x) * (s.words > 0 ? s.words : 1);
     const float cross = block_reduce<false>(cross_of(t, r, s.words, s.vocab, z, kLog2E / s.heat, lse, nullptr), red);
     loss = w * (s.heat * s.heat * (cross * kLn2 + (s.words > 0 ? t.entropy[r] : 0.f)));
@@ -830,7 +854,8 @@ __global__ __launch_bounds__(256) void slabs_loss_kernel(Slabs s, Targets t, Los
 // networks hold (the largest of the hidden rows in [2^-3, 2^13], of the weight in
 // [2^-7, 2^9]: what is rounded is off by 2^-24 of the largest at most); the largest
 // value is found on the way, and slabs_grad_kernel redoes a tensor that it does not
-// suit.
+// suit.  Bound by its bytes: 32000 x 2048 and 16384 rows 69 us, 5.8 TB/s;
+// 128256 x 2048 and 4096 rows 203, 5.3.
 struct Halves {
   const uint16_t* from;
   int64_t ld, rows;
@@ -929,7 +954,10 @@ __global__ __launch_bounds__(256) void halves_kernel(Halves hidden_rows, Halves 
 // in f16, as (w / largest) 2^14 (p - q): a bf16 rounding of them, 2^-8 of each, would
 // add to the products' sums, where the words' parts cancel, more than the sums' own
 // rounding (measured: up to 1.9 times the error of f32 ones); 2^-11 does not show.
-// Down to 2^-28 of the largest they have all 11 bits, below 2^-39 they are 0.
+// Down to 2^-28 of the largest they have all 11 bits, below 2^-39 they are 0, so rows
+// whose weights lie further below the largest get gradients of fewer bits, or none.
+// Bound by its bytes: 16384 x 32000 427 us, 4.9 TB/s; 8192 165, 6.3 with what the caches
+// still hold.
 //
 // TWO (few rows): as two bf16 parts too, rows [0, rows) and [rows, 2 rows) of two, for
 // a product with the weight as it is.
@@ -955,7 +983,7 @@ __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Sl
     return;
   }
   const float2* st = s.stat + at * s.count;
-  const float lse = slabs_lse(st, s.count, red);
+  const Lse lse = slabs_lse(st, s.count, red);
   const float* z = s.z + at * (s.words > 0 ? s.words : 1);
   const float cross = block_reduce<false>(cross_of(t, r, s.words, s.vocab, z, kLog2E / s.heat, lse, at_word), red);
   // counted before the gradient is written, which its wait then overlaps
@@ -976,7 +1004,7 @@ __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Sl
     for (int i = 0; i < kAhead; ++i) {
       const int at = c0 + 256 * i;
       if (at >= chunks) break;
-      const float f = c * __builtin_amdgcn_exp2f(m[i] - lse - 15.f);
+      const float f = c * __builtin_amdgcn_exp2f(m[i] - lse.ref - lse.log2_sum - 15.f);
       const uint32_t in[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
       uint32_t out[4], high[4], low[4];
 #pragma unroll
@@ -1089,8 +1117,9 @@ __global__ __launch_bounds__(256) void two_parts_kernel(const float* __restrict_
   if (i < n) out[i] = Elem<OUT>::of(*alpha * (a[i] + a[n + i]));
 }
 
-// out[i][j] = *alpha a_i b_j (alpha null: 1), the product over one row or one word (the engine takes no
-// operand of one element's pitch).  Columns blockIdx.x, rows blockIdx.y and on.
+// out[i][j] = *alpha a_i b_j (alpha null: 1), the product over one row or one word (the
+// engine takes no operand of one element's pitch).  Columns blockIdx.x, rows blockIdx.y
+// and on.
 template <typename T, typename OUT>
 __global__ __launch_bounds__(256) void outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b,
                                                     int64_t m, int64_t n, const float* __restrict__ alpha,

@@ -24,7 +24,11 @@ out of the mean, which is NaN where no row is left.  A label outside the vocabul
 gives NaN, as do NaN logits in rows that count.
 
 Losses are f32.  Operands are bf16 or f32, or either under bf16 autocast, where the
-products are those of bf16 casts and gradients come in the operands' own types.
+products are those of bf16 casts and gradients come in the operands' own types.  The
+gradients of bf16 products' logits are f16 scaled by the largest row weight: rows
+whose weight is less than 2^-28 of it lose bits, below 2^-39 all of them.  An upstream
+factor that is no power of two rounds bf16 gradients a second time.  A backward with
+create_graph=True takes f32 tensor operations, with the logits of all rows.
 """
 from __future__ import annotations
 

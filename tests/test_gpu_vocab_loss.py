@@ -738,3 +738,25 @@ def test_rows_at_any_offset(vocab, dtype):
         assert torch.allclose(got[0], want[0], rtol=2.0 ** -20, atol=2.0 ** -20 * math.log(2 * vocab))
         step = 2.0 ** -7 if dtype == BF else 2.0 ** -20  # one bf16 step where the f32 values differ
         assert ((got[1] - want[1]).abs().float() <= step * want[1].abs().float() + 2.0 ** -20 * 2).all()
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("up", [0, 64, 4096])
+def test_loss_of_logits_that_all_are_large(rows, up):
+    """What all of a row's logits share leaves no rounding in its loss.  Logits are exact
+    here: up, and -16 to 2 in steps of 1/8."""
+    vocab = 500
+    h, w = torch.zeros(rows, 64, device="cuda"), torch.zeros(vocab, 64, device="cuda")
+    h[:, 0], h[:, 1] = 1, 1 + torch.arange(rows, device="cuda") % 2
+    w[:, 0], w[:, 1] = up, -(torch.arange(vocab, device="cuda") * 37 % 65) / 8
+    w[77, 1] = 1
+    y = torch.full((rows,), 77, device="cuda")
+    h, w = h.to(BF), w.to(BF)
+    want = -torch.log_softmax(h.to(F64) @ w.to(F64).t(), -1)[:, 77]
+    # in units of log2: a logit's distance from the slab's reference, at most 18 log2(e) + 1,
+    # rounded and scaled by a rounded log2(e), twice; sum, exponential and logarithm
+    tol = math.log(2) * (4 * 27 * 2.0 ** -25 + 2.0 ** -21)
+    out = L.linear_cross_entropy(h, w, y, reduction="none").to(F64)
+    assert ((out - want).abs() <= tol).all(), (out - want).abs().max()
+    mean = L.linear_cross_entropy(h.requires_grad_(), w, y)
+    assert abs(mean.item() - want.mean().item()) <= tol + 2.0 ** -24 * want.max().item()
