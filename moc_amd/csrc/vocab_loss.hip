@@ -674,10 +674,12 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
 // bytes: 32000 x 2048, 1 row 26.3 us, 5.0 TB/s, 16 rows 27.6 (through the tiled
 // product 30.3 and 30.7); 128256 x 1024, 16 rows 49.7, 5.3 TB/s (53.4); 128256 x 4096,
 // 4 rows 204, 5.2 TB/s (226).
-constexpr int kFewRows = 16, kFewAhead = 16, kFewHidden = 4096;
+constexpr int kFewRows = 16, kFewAhead = 16, kFewHidden = 4096, kFewSums = 4;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
+// RAGGED: a hidden size that is no multiple of 32 (its masks cost 1.5 us of 28).
+template <bool RAGGED>
 __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restrict__ h, int64_t ldh, int rows,
                                                        const uint16_t* __restrict__ w, int64_t ldw, int vocab,
                                                        int hidden, float unit, const int32_t* __restrict__ ids,
@@ -689,7 +691,15 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
   const int steps = (hidden + 31) / 32;
   float2* part = reinterpret_cast<float2*>(frag + steps * 64);  // [2][4][16]
   const int row = lane & 15, quad = lane >> 4;
-  const bool ragged = hidden % 32 != 0 && 32 * (steps - 1) + 8 * quad >= hidden;  // its last chunk lies behind
+  const bool ragged = RAGGED && 32 * (steps - 1) + 8 * quad >= hidden;  // its last chunk lies behind
+  // what a chunk of 8 at column k holds of the hidden size (behind it is another tensor's
+  // or padding)
+  auto held = [&](uint4 v, int k) {
+    const int n = hidden - k;
+    auto word = [&](uint32_t x, int at) { return at + 1 < n ? x : at < n ? x & 0xFFFFu : 0u; };
+    return make_uint4(word(v.x, 0), word(v.y, 2), word(v.z, 4), word(v.w, 6));
+  };
+  const uint4 end = held(make_uint4(~0u, ~0u, ~0u, ~0u), 32 * (steps - 1) + 8 * quad);
   auto load = [&](uint4 (&a)[kFewAhead], const uint16_t* src, int s0) {
 #pragma unroll
     for (int i = 0; i < kFewAhead; ++i) {
@@ -705,21 +715,24 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
   load(a, word_of(slab), 0);
   for (int i = tid; i < steps * 64; i += 256) {
     const int n = i & 15, k = i / 64 * 32 + 8 * (i % 64 / 16);
-    frag[i] = n < rows && k < hidden ? *reinterpret_cast<const uint4*>(h + n * ldh + k) : make_uint4(0, 0, 0, 0);
+    frag[i] = n < rows && (!RAGGED || k < hidden) ? *reinterpret_cast<const uint4*>(h + n * ldh + k)
+                                                  : make_uint4(0, 0, 0, 0);
+    if constexpr (RAGGED) frag[i] = held(frag[i], k);
   }
   __syncthreads();
   for (int turn = 0; slab < slabs; slab += gridDim.x, turn ^= 1) {
     const uint16_t* src = word_of(slab);
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    f32x4_t sums[kFewSums] = {};  // chains of a quarter of the steps: fewer roundings in a row
     auto products = [&](uint4 (&v)[kFewAhead], int s0) {
 #pragma unroll
       for (int i = 0; i < kFewAhead; ++i) {
         if (s0 + i >= steps) break;
         uint4 x = v[i];
-        if (ragged && s0 + i == steps - 1) x = make_uint4(0, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x),
-                                                      __builtin_bit_cast(bf16x8_t, frag[(s0 + i) * 64 + lane]), acc, 0,
-                                                      0, 0);
+        if (RAGGED && s0 + i == steps - 1) x = make_uint4(x.x & end.x, x.y & end.y, x.z & end.z, x.w & end.w);
+        f32x4_t& to = sums[i % kFewSums];
+        to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x),
+                                                     __builtin_bit_cast(bf16x8_t, frag[(s0 + i) * 64 + lane]), to, 0, 0,
+                                                     0);
       }
     };
     for (int s0 = 0; s0 < steps; s0 += 2 * kFewAhead) {
@@ -729,6 +742,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
       else if (slab + static_cast<int>(gridDim.x) < slabs) load(a, word_of(slab + gridDim.x), 0);
       products(b, s0 + kFewAhead);
     }
+    f32x4_t acc = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     // lane: row, words slab * 64 + wave * 16 + 4 quad + e
     const int c0 = wave * 16 + 4 * quad;
     if (row < rows) {
@@ -1349,9 +1363,10 @@ int launch_few(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const v
   const int lds = steps * 1024 + 2 * 4 * 16 * 8;
   const int64_t resident = static_cast<int64_t>(cu_count()) * (160 * 1024 / lds < 8 ? 160 * 1024 / lds : 8);
   const unsigned grid = static_cast<unsigned>(slabs < resident ? slabs : resident);
-  few_rows_kernel<<<grid, 256, lds, st>>>(static_cast<const uint16_t*>(h), ldh, (int)rows,
-                                          static_cast<const uint16_t*>(w), ldw, (int)vocab, (int)hidden, unit, ids,
-                                          ld_ids, first, ld_first, (int)words, z, stat, (int)slabs);
+  auto kernel = hidden % 32 != 0 ? few_rows_kernel<true> : few_rows_kernel<false>;
+  kernel<<<grid, 256, lds, st>>>(static_cast<const uint16_t*>(h), ldh, (int)rows, static_cast<const uint16_t*>(w), ldw,
+                                 (int)vocab, (int)hidden, unit, ids, ld_ids, first, ld_first, (int)words, z, stat,
+                                 (int)slabs);
   return check_launch("few_rows_kernel");
 }
 
@@ -1556,7 +1571,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     if (p.fused) {
       const uint16_t* first = words > 0 ? t.first + r0 : nullptr;
       const float unit = kLog2E / temperature;
-      if (!grads && n <= kFewRows && hidden % 8 == 0 && hidden <= kFewHidden)
+      if (!grads && n <= kFewRows && hidden <= kFewHidden)
         rc = launch_few(xi, n, hidden, ldx, w, vocab, ldw, unit, word_ids + r0 * ld_ids, ld_ids, first, rows, n_words, p.z,
                         p.stat, p.slabs, st);
       else

@@ -760,3 +760,39 @@ def test_loss_of_logits_that_all_are_large(rows, up):
     assert ((out - want).abs() <= tol).all(), (out - want).abs().max()
     mean = L.linear_cross_entropy(h.requires_grad_(), w, y)
     assert abs(mean.item() - want.mean().item()) <= tol + 2.0 ** -24 * want.max().item()
+
+
+@pytest.mark.parametrize("rows", [1, 7, 16])
+@pytest.mark.parametrize("d", [1, 7, 31, 100, 250, 1500, 4093])
+def test_few_rows_of_any_hidden_size(rows, d):
+    """Losses alone of up to 16 rows; what lies behind a row's end is NaN."""
+    vocab = 1003
+    h, w = operands(rows, d, vocab, BF, seed=d)
+    hd, wd = h.to(F64), w.to(F64)
+    wide = [torch.full((t.shape[0], -(-d // 8) * 8), math.nan, dtype=BF, device="cuda") for t in (h, w)]
+    h, w = (b[:, :d].copy_(t) for b, t in zip(wide, (h, w)))
+    y = labels_of(rows, vocab, 0.2)
+    label = torch.zeros(rows, vocab, dtype=F64, device="cuda")
+    label[torch.arange(rows, device="cuda"), y.clamp(min=0)] = 1
+    z, ones = hd @ wd.t(), torch.ones(rows, device="cuda")
+    want, _, _ = reference(z, label, y != -100, ones.to(F64), 1.0, "none")
+    out = L.linear_cross_entropy(h, w, y, reduction="none")
+    check(out, want, (None, None), (hd, wd), z, z, label, logit_error(hd, wd), 1.0, 1.0, ones)
+    ids, top = teacher_of(rows, vocab, 9, False)
+    q, some = shares(ids, top, vocab, 1.5)
+    want, _, _ = reference(z, q, some, ones.to(F64), 1.5, "none")
+    check(L.linear_distillation(h, w, ids, top, temperature=1.5, reduction="none"), want, (None, None), (hd, wd), z, z, q,
+          logit_error(hd, wd), 1.5, 1.0, ones)
+
+
+@pytest.mark.parametrize("rows,d,vocab", [(5, 100, 700), (20, 250, 700), (300, 1500, 1003), (40, 7, 300)])
+def test_nan_behind_the_rows(rows, d, vocab):
+    """Gradients of views into wider buffers that hold NaN."""
+    h, w = operands(rows, d, vocab, BF)
+    y = labels_of(rows, vocab, 0.2)
+    wide = [torch.full((t.shape[0], -(-d // 8) * 8 + 8), math.nan, dtype=BF, device="cuda") for t in (h, w)]
+    views = [b[:, :d].copy_(t).requires_grad_() for b, t in zip(wide, (h, w))]
+    out, same = L.linear_cross_entropy(*views, y), L.linear_cross_entropy(h.requires_grad_(), w.requires_grad_(), y)
+    assert torch.equal(out, same)
+    for a, b in zip(torch.autograd.grad(out, views), torch.autograd.grad(same, (h, w))):
+        assert torch.equal(a, b)
