@@ -671,9 +671,8 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
 // Up to 16 rows, losses alone: the weight is read once, straight into the operand
 // registers of v_mfma_f32_16x16x32_bf16 (a wave 16 words, a workgroup a slab of 64),
 // 16 loads ahead; the rows stand in LDS in fragment order.  Bound by the weight's
-// bytes: 32000 x 2048, 1 row 26.3 us, 5.0 TB/s, 16 rows 27.6 (through the tiled
-// product 30.3 and 30.7); 128256 x 1024, 16 rows 49.7, 5.3 TB/s (53.4); 128256 x 4096,
-// 4 rows 204, 5.2 TB/s (226).
+// bytes: 32000 x 2048, 1 row 25.2 us, 5.2 TB/s, 16 rows 26.1; 128256 x 1024, 16 rows
+// 45.1, 5.8 TB/s; 128256 x 4096, 4 rows 202, 5.2 TB/s.
 constexpr int kFewRows = 16, kFewAhead = 16, kFewHidden = 4096, kFewSums = 4;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -1355,14 +1354,31 @@ int sum_loss(const Targets& t, LossOut o, float* loss, hipStream_t st) {
   return check_launch("loss_sum_kernel");
 }
 
+int few_lds(int64_t hidden) { return static_cast<int>((hidden + 31) / 32) * 1024 + 2 * 4 * 16 * 8; }
+
+// Whether few_rows_kernel takes a piece without gradients.  Not where its workgroups, two
+// a CU, have two slabs or more while the tiles of the product are all on a CU at once.
+// us, it / the product, of 4 rows and 32000, 50021, 65536 and 128256 words:
+//   hidden  512    8.6 / 12.1   13.8 / 13.1    15.3 / 14.9    25.6 / 25.7
+//          1024   15.2 / 18.1   22.5 / 19.2    26.2 / 23.0    44.3 / 41.7
+//          2048   25.4 / 30.6   41.7 / 31.8    46.3 / 40.9   102.7 / 123.0
+//          4096   57.3 / 56.3   94.2 / 94.7   113.9 / 122.9  199.4 / 172 to 209 (one a CU)
+bool by_few(int64_t rows, int64_t hidden, int64_t vocab) {
+  if (rows > kFewRows || hidden > kFewHidden) return false;
+  const int64_t cus = cu_count();
+  return 2 * few_lds(hidden) > 160 * 1024 || slabs_of(vocab) <= 2 * cus || (vocab + 255) / 256 > cus;
+}
+
 // Logits of up to kFewRows rows, losses alone.
 int launch_few(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab, int64_t ldw,
                float unit, const int32_t* ids, int64_t ld_ids, const uint16_t* first, int64_t ld_first, int64_t words,
                float* z, float2* stat, int64_t slabs, hipStream_t st) {
-  const int steps = static_cast<int>((hidden + 31) / 32);
-  const int lds = steps * 1024 + 2 * 4 * 16 * 8;
-  const int64_t resident = static_cast<int64_t>(cu_count()) * (160 * 1024 / lds < 8 ? 160 * 1024 / lds : 8);
-  const unsigned grid = static_cast<unsigned>(slabs < resident ? slabs : resident);
+  const int lds = few_lds(hidden);
+  // what registers and LDS let a CU have, each as many slabs: 128256 x 4096 203 us, 221
+  // with two a CU in turn; 50021 x 768 20.5, 22.8 with a workgroup a slab
+  const int64_t resident = static_cast<int64_t>(cu_count()) * (2 * lds > 160 * 1024 ? 1 : 2);
+  const int64_t rounds = (slabs + resident - 1) / resident;
+  const unsigned grid = static_cast<unsigned>((slabs + rounds - 1) / rounds);
   auto kernel = hidden % 32 != 0 ? few_rows_kernel<true> : few_rows_kernel<false>;
   kernel<<<grid, 256, lds, st>>>(static_cast<const uint16_t*>(h), ldh, (int)rows, static_cast<const uint16_t*>(w), ldw,
                                  (int)vocab, (int)hidden, unit, ids, ld_ids, first, ld_first, (int)words, z, stat,
@@ -1571,7 +1587,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     if (p.fused) {
       const uint16_t* first = words > 0 ? t.first + r0 : nullptr;
       const float unit = kLog2E / temperature;
-      if (!grads && n <= kFewRows && hidden <= kFewHidden)
+      if (!grads && by_few(n, hidden, vocab))
         rc = launch_few(xi, n, hidden, ldx, w, vocab, ldw, unit, word_ids + r0 * ld_ids, ld_ids, first, rows, n_words, p.z,
                         p.stat, p.slabs, st);
       else

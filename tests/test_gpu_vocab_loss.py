@@ -796,3 +796,17 @@ def test_nan_behind_the_rows(rows, d, vocab):
     assert torch.equal(out, same)
     for a, b in zip(torch.autograd.grad(out, views), torch.autograd.grad(same, (h, w))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,d,vocab", [(2, 64, 40000), (16, 100, 65536), (3, 4096, 40000), (5, 96, 65600)])
+def test_few_rows_of_wide_vocabularies(rows, d, vocab):
+    """Losses alone on both sides of where few rows go through tiles."""
+    h, w = operands(rows, d, vocab, BF)
+    hd, wd = h.to(F64), w.to(F64)
+    y = labels_of(rows, vocab, 0.0)
+    label = torch.zeros(rows, vocab, dtype=F64, device="cuda")
+    label[torch.arange(rows, device="cuda"), y] = 1
+    z, ones = hd @ wd.t(), torch.ones(rows, device="cuda")
+    want, _, _ = reference(z, label, y >= 0, ones.to(F64), 1.0, "none")
+    out = L.linear_cross_entropy(h, w, y, reduction="none")
+    check(out, want, (None, None), (hd, wd), z, z, label, logit_error(hd, wd), 1.0, 1.0, ones)
