@@ -976,7 +976,8 @@ __global__ __launch_bounds__(256) void halves_kernel(Halves hidden_rows, Halves 
 // a product with the weight as it is.
 template <bool TWO>
 __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Slabs& s, const Targets& t,
-                                               const LossOut& o, int& flag, int64_t at, int rows, uint16_t* two) {
+                                               const LossOut& o, int& flag, int64_t at, int rows, int part, int parts,
+                                               uint16_t* two) {
   typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
   __shared__ float red[4], at_word[kMaxWords];
   const int64_t r = s.r0 + at;
@@ -984,35 +985,42 @@ __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Sl
   const float w = weight_of(t, r);
   uint16_t* out = e + at * ld;
   uint4* row = reinterpret_cast<uint4*>(out);
-  uint16_t* part[2] = {two + at * ld, two + (rows + at) * ld};
-  const int chunks = (s.vocab + 7) / 8;
+  uint16_t* pair[2] = {two + at * ld, two + (rows + at) * ld};
+  // this workgroup's part of the row
+  const int all = (s.vocab + 7) / 8, each = (all + parts - 1) / parts, begin = part * each,
+            chunks = all < begin + each ? all : begin + each;
   if (w == 0.f) {  // uniform
-    for (int c = tid; c < chunks; c += 256) {
+    for (int c = begin + tid; c < chunks; c += 256) {
       row[c] = make_uint4(0, 0, 0, 0);
       if constexpr (TWO)
-        for (uint16_t* p : part) reinterpret_cast<uint4*>(p)[c] = make_uint4(0, 0, 0, 0);
+        for (uint16_t* p : pair) reinterpret_cast<uint4*>(p)[c] = make_uint4(0, 0, 0, 0);
     }
-    if (tid == 0) flag = put_row(o, r, 0.f, rows);
+    if (tid == 0) flag = part == 0 && put_row(o, r, 0.f, rows);
     return;
   }
   const float2* st = s.stat + at * s.count;
+  constexpr int kAhead = 4;
+  uint4 v[kAhead];
+  float m[kAhead];
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int c = min(c0 + 256 * i, chunks - 1);
+      v[i] = row[c];
+      m[i] = st[c / (kLossSlab / 8)].x;
+    }
+  };
+  load(begin + tid);  // on their way during the statistics
   const Lse lse = slabs_lse(st, s.count, red);
   const float* z = s.z + at * (s.words > 0 ? s.words : 1);
   const float cross = block_reduce<false>(cross_of(t, r, s.words, s.vocab, z, kLog2E / s.heat, lse, at_word), red);
   // counted before the gradient is written, which its wait then overlaps
   if (tid == 0)
-    flag = put_row(o, r, w * (s.heat * s.heat * (cross * kLn2 + (s.words > 0 ? t.entropy[r] : 0.f))), rows);
+    flag = part == 0 &&
+           put_row(o, r, w * (s.heat * s.heat * (cross * kLn2 + (s.words > 0 ? t.entropy[r] : 0.f))), rows);
   const float c = cross == cross ? w / *t.largest * 0x1p14f : NAN;
-  constexpr int kAhead = 4;
-  for (int c0 = tid; c0 < chunks; c0 += 256 * kAhead) {
-    uint4 v[kAhead];
-    float m[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int at = min(c0 + 256 * i, chunks - 1);
-      v[i] = row[at];
-      m[i] = st[at / (kLossSlab / 8)].x;
-    }
+  for (int c0 = begin + tid; c0 < chunks; c0 += 256 * kAhead) {
+    if (c0 != begin + tid) load(c0);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int at = c0 + 256 * i;
@@ -1033,8 +1041,8 @@ __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Sl
       }
       row[at] = make_uint4(out[0], out[1], out[2], out[3]);
       if constexpr (TWO) {
-        reinterpret_cast<uint4*>(part[0])[at] = make_uint4(high[0], high[1], high[2], high[3]);
-        reinterpret_cast<uint4*>(part[1])[at] = make_uint4(low[0], low[1], low[2], low[3]);
+        reinterpret_cast<uint4*>(pair[0])[at] = make_uint4(high[0], high[1], high[2], high[3]);
+        reinterpret_cast<uint4*>(pair[1])[at] = make_uint4(low[0], low[1], low[2], low[3]);
       }
     }
   }
@@ -1043,12 +1051,12 @@ __device__ __forceinline__ void slabs_grad_row(uint16_t* e, int64_t ld, const Sl
   for (int k = tid; k < (s.words > 0 ? s.words : 1); k += 256) {
     float share;
     const int32_t id = word_of(t, r, s.words, k, s.vocab, share);
-    if (id == kUnknown || share == -1.f) continue;
+    if (id == kUnknown || share == -1.f || id < 8 * begin || id >= 8 * chunks) continue;
     const float g = c * (__builtin_amdgcn_exp2f(at_word[k]) - share);
     out[id] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(g));
     if constexpr (TWO) {
-      part[0][id] = bf16_rne(g);
-      part[1][id] = bf16_rne(g - bf16_to_f32(part[0][id]));
+      pair[0][id] = bf16_rne(g);
+      pair[1][id] = bf16_rne(g - bf16_to_f32(pair[0][id]));
     }
   }
 }
@@ -1060,8 +1068,8 @@ constexpr int kAgainBlocks = 64;
 template <bool TWO>
 __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld, Slabs s, Targets t, LossOut o,
                                                          Halves hidden_rows, Halves weight_rows, int hidden,
-                                                         int64_t ldo, const uint32_t* __restrict__ most, int parts,
-                                                         uint16_t* two) {
+                                                         int64_t ldo, const uint32_t* __restrict__ most, int blocks,
+                                                         int parts, uint16_t* two) {
   __shared__ double red64[4];
   __shared__ uint32_t red[4];
   __shared__ int flag;
@@ -1069,9 +1077,9 @@ __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld
   if (static_cast<int>(blockIdx.x) < again) {
     uint32_t m[2] = {0, 0};
 #pragma unroll 4
-    for (int i = threadIdx.x; i < parts; i += 256) {
+    for (int i = threadIdx.x; i < blocks; i += 256) {
       m[0] = max(m[0], most[i]);
-      m[1] = max(m[1], most[parts + i]);
+      m[1] = max(m[1], most[blocks + i]);
     }
     const float sx = halves_scale(hidden_rows, block_max_bits(m[0], red));
     const float sw = halves_scale(weight_rows, block_max_bits(m[1], red));
@@ -1085,7 +1093,8 @@ __global__ __launch_bounds__(256) void slabs_grad_kernel(uint16_t* e, int64_t ld
     }
     return;
   }
-  slabs_grad_row<TWO>(e, ld, s, t, o, flag, blockIdx.x - again, gridDim.x - again, two);
+  const int i = static_cast<int>(blockIdx.x) - again, rows = (static_cast<int>(gridDim.x) - again) / parts;
+  slabs_grad_row<TWO>(e, ld, s, t, o, flag, i / parts, rows, i % parts, parts, two);
   __syncthreads();
   if (flag) put_loss<true>(t, o, red64);
 }
@@ -1193,6 +1202,12 @@ constexpr int64_t kWidest = 4;
 bool in_two_parts(int64_t rows, int64_t hidden, int64_t vocab) {
   return rows * (hidden + 960) <= 420 * hidden && vocab > 1;
 }
+
+// Workgroups of slabs_grad_kernel a row, each a part of its gradient (and the
+// statistics, again): few rows leave the CUs idle otherwise.  us, 1 / these: 4 x 32000
+// words 10.3 / 7.1, 64 x 128256 23.9 / 15.3, 100 x 32000 12.4 / 10.5; 400 x 128256 and
+// 512 x 32000 take as long in two parts as in one, 2000 x 32000 56 in four, 52 in one.
+int grad_parts(int64_t rows) { return rows > 256 ? 1 : rows < 64 ? 8 : static_cast<int>(512 / rows); }
 
 constexpr int kHalvesBlocks = 1024;  // workgroups of halves_kernel that write f16 rows
 
@@ -1596,14 +1611,15 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       MOC_REQUIRE(rc <= 0, "moc_linear_loss: operands of up to 2 GiB");
       if (rc != MOC_OK) return rc;
       const Slabs s{p.stat, p.z, (int)p.slabs, (int)vocab, (int)words, r0, temperature};
-      const unsigned blocks = static_cast<unsigned>(n) + (i == 0 ? kAgainBlocks : 0);
+      const int parts = grad_parts(n);
+      const unsigned blocks = static_cast<unsigned>(n) * parts + (i == 0 ? kAgainBlocks : 0);
       uint16_t* d = reinterpret_cast<uint16_t*>(p.d);
       if (two && dh != nullptr)
         slabs_grad_kernel<true><<<blocks, 256, 0, st>>>(d, p.ldz, s, t, o, hx, hw, (int)hidden, p.ldx, p.most, halves,
-                                                        reinterpret_cast<uint16_t*>(p.two));
+                                                        parts, reinterpret_cast<uint16_t*>(p.two));
       else if (grads)
         slabs_grad_kernel<false><<<blocks, 256, 0, st>>>(d, p.ldz, s, t, o, hx, hw, (int)hidden, p.ldx, p.most, halves,
-                                                         nullptr);
+                                                         parts, nullptr);
       else
         slabs_loss_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(s, t, o);
       rc = check_launch("slabs_grad_kernel");
