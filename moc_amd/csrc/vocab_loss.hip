@@ -1186,8 +1186,11 @@ unsigned blocks_of(int64_t n) {
 }
 
 // --------------------------------------------------------------------- host
-// Logits exist for a piece of the rows at a time, within about this many bytes.
-constexpr int64_t kPieceBytes = 1LL << 30;
+// Logits, or what is kept of them, exist for a piece of the rows at a time: within a GiB,
+// f16 gradients within what a product's operand may have, since each piece adds its part
+// of dweight in f32 (16384 x 512 x 128256 8.8 ms by 1 GiB, 8.6 by 2; 8192 x 2048 x 128256
+// 12.3, 11.6).
+constexpr int64_t kPieceBytes = 1LL << 30, kGradPieceBytes = (1LL << 31) - 4096;
 constexpr int64_t kWidest = 4;
 // Few rows: dhidden comes from gradients in two bf16 parts, twice the rows, with the
 // weight as it is (TWO), else from f16 ones and a copy of the weight.  The copy moves 4
@@ -1237,7 +1240,7 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   p.ldx = (hidden + 63) & ~63LL;
   p.slabs = slabs_of(vocab);
   const int64_t each = f32 ? p.ldz * 4 : grads ? p.ldz * 2 : p.slabs * 8;
-  int64_t n = kPieceBytes / each / 256 * 256;
+  int64_t n = (p.fused && grads ? kGradPieceBytes : kPieceBytes) / each / 256 * 256;
   // its hidden rows within 32-bit offsets, at up to kWidest times their own pitch
   const int64_t most = ((1LL << 31) - 4096) / (es * kWidest * p.ldx) / 256 * 256;
   if (n > most) n = most;

@@ -6,7 +6,7 @@ a teacher's top logits (moc_amd/csrc/vocab_loss.hip).
     distillation_loss(logits, ids, top)                     of logits already there
 
 The first two never hold the logits of all rows: they exist for a piece of the rows
-at a time (at most 1 GiB), and the gradients of hidden rows and weight are computed
+at a time (at most 2 GiB), and the gradients of hidden rows and weight are computed
 in the forward pass, while the piece is there, so that a backward has nothing left to
 do but the upstream factor.  A second backward of the same graph, and a backward
 captured into a HIP graph without its forward, compute them again; reduction="none"

@@ -810,3 +810,36 @@ def test_few_rows_of_wide_vocabularies(rows, d, vocab):
     want, _, _ = reference(z, label, y >= 0, ones.to(F64), 1.0, "none")
     out = L.linear_cross_entropy(h, w, y, reduction="none")
     check(out, want, (None, None), (hd, wd), z, z, label, logit_error(hd, wd), 1.0, 1.0, ones)
+
+
+@pytest.mark.parametrize("rows,words", [(8193, 0), (8500, 0), (8300, 7)])
+def test_rows_in_more_pieces(rows, words):
+    """A second piece of the rows, of one and of some."""
+    d, vocab = 64, 128256
+    h, w = operands(rows, d, vocab, BF)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    y = labels_of(rows, vocab, 0.2)
+    y[-1] = 5
+    one = torch.ones(rows, dtype=F64, device="cuda")
+    hd, wd = h.detach().to(F64), w.detach().to(F64)
+    if words:
+        ids, top = teacher_of(rows, vocab, words, False)
+        out = L.linear_distillation(h, w, ids, top)
+        q, some = shares(ids, top, vocab, 1.0)
+    else:
+        out = L.linear_cross_entropy(h, w, y)
+        q, some = torch.zeros(rows, vocab, dtype=F64, device="cuda"), y != -100
+        q[torch.arange(rows, device="cuda"), y.clamp(min=0)] = 1
+    got = torch.autograd.grad(out, (h, w))
+    want, dz, c = reference(hd @ wd.t(), q, some, one, 1.0, "mean")
+    check(out.detach(), want, got, (hd, wd), dz, c, q, logit_error(hd, wd), 1.0, 1.0, one)
+
+
+def test_no_piece_passes_the_products_offsets():
+    """Sizes of the workspace go by the pieces: rows and words of any size have one."""
+    from moc_amd import _native as N
+    for vocab in (1, 63, 32000, 65536, 128256, 1 << 21):
+        for rows in (1, 257, 16384, 1 << 17):
+            need = N.query("moc_linear_loss_workspace_size", N.MOC_BF16, rows, 64, vocab, 0, 1)
+            assert 0 < need < (1 << 31) + 2 * vocab * 64 * 4 + vocab * 64 * 2 + rows * 64 * 2 + (
+                (1 << 31) // (vocab * 2) + 256) * (vocab // 64 + 2) * 8 + (1 << 24) + rows * 8
