@@ -292,8 +292,9 @@ int moc_logits_loss(int dtype, const void* logits, int64_t rows, int64_t vocab, 
  * of the rows at a time: dh [rows, hidden] and dw [vocab, hidden], contiguous, either
  * NULL (both: the losses alone).  words = 0: against labels (temperature 1), else
  * against a teacher.  A bf16 weight of up to 2 GiB.  bf16 operands' gradients are f16
- * on their way (see vocab_loss.hip).  gemm_ws: as moc_gemm_ws uses it, its counters
- * too. */
+ * on their way (see vocab_loss.hip).  gemm_ws: as moc_gemm_ws uses it; its counters are
+ * cleared by the call for f32 operands and for gradients, else they are zero before it,
+ * and they are left zero. */
 int64_t moc_linear_loss_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t words,
                                        int grads);
 int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int grads);

@@ -942,13 +942,14 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t m, uint32_t* red) {
 __global__ __launch_bounds__(256) void halves_kernel(Halves hidden_rows, Halves weight_rows, int hidden, int64_t ldo,
                                                      Targets t, int64_t rows, int mean,
                                                      const float* __restrict__ grad, int words, int slabs,
-                                                     uint32_t* __restrict__ most, int blocks) {
+                                                     uint32_t* __restrict__ most, int blocks, int* counters) {
   __shared__ int32_t held[16 * (kWordsLds + 1)];
   __shared__ uint32_t red[4];
   __shared__ float redf[4];
   __shared__ double red64[4];
   const int extra = static_cast<int>(gridDim.x) - blocks, block = static_cast<int>(blockIdx.x) - extra;
   if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < MOC_GEMM_WS_COUNTER_BYTES / 4; i += 256) counters[i] = 0;  // of the products and losses
     put_total<false>(t, rows, mean, grad, red64, redf);
   } else if (block < 0) {
     words_left(t.ids, rows, words, slabs, t.first, blockIdx.x - 1, held);
@@ -1557,6 +1558,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
   }
   if (row_loss == nullptr) row_loss = p.row_loss;
   const int64_t n_words = words > 0 ? words : 1;
+  if (f32 && (rc = moc_fill_zero(count, MOC_GEMM_WS_COUNTER_BYTES, stream)) != MOC_OK) return rc;
   if (words > 0) {
     rc = run_teacher(a, rows, words, vocab, row_weight, mean, grad, t, grads && f32, count, st);
     if (rc != MOC_OK) return rc;
@@ -1586,7 +1588,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     const int64_t most_rows = copy_w && vocab > rows ? vocab : rows, want = (most_rows + 15) / 16;  // four waves of four rows
     halves = static_cast<int>(want < kHalvesBlocks ? want : kHalvesBlocks);
     halves_kernel<<<1 + table_blocks + halves, 256, 0, st>>>(hx, hw, (int)hidden, p.ldx, t, rows, mean, grad, (int)words,
-                                                             (int)p.slabs, p.most, halves);
+                                                             (int)p.slabs, p.most, halves, count);
     if ((rc = check_launch("halves_kernel")) != MOC_OK) return rc;
   }
   // f32: the rows that count in every product; bf16: in dweight's alone, as nothing is

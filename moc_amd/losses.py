@@ -267,14 +267,10 @@ def _counters(dev: int, stream: int, where) -> torch.Tensor:
 
 
 def _gemm_workspace(dev: int, stream: int, where, nbytes: int) -> torch.Tensor:
-    """A GEMM workspace with such counters at its start."""
-    if nbytes <= COUNTER_BYTES:
-        return _counters(dev, stream, where)
-    if not torch.cuda.is_current_stream_capturing():
-        return K._gemm_workspace(where, nbytes)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
-    N.call("moc_fill_zero", ws.data_ptr(), COUNTER_BYTES, stream)
-    return ws
+    """Counters alone, which are zero between two launches, or the call's own workspace:
+    parts of a product wait there for another launch, between which a second thread
+    may put its own on the stream.  The call clears the counters of such a one."""
+    return _counters(dev, stream, where) if nbytes <= COUNTER_BYTES else torch.empty(nbytes, dtype=torch.uint8, device=where)
 
 
 def _linear_pass(targets, saved, row_weight, mean, grad, product, hidden, weight, each: bool, dh: bool, dw: bool):

@@ -843,3 +843,113 @@ def test_no_piece_passes_the_products_offsets():
             need = N.query("moc_linear_loss_workspace_size", N.MOC_BF16, rows, 64, vocab, 0, 1)
             assert 0 < need < (1 << 31) + 2 * vocab * 64 * 4 + vocab * 64 * 2 + rows * 64 * 2 + (
                 (1 << 31) // (vocab * 2) + 256) * (vocab // 64 + 2) * 8 + (1 << 24) + rows * 8
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+def test_two_threads_on_one_stream(op, dtype):
+    """Calls whose launches mix on a stream: products split along K, teachers, sums."""
+    import threading
+
+    rows, d, vocab, turns = (777, 512, 9000, 25) if dtype == BF else (96, 64, 3000, 25)
+    sets = []
+    for i in range(2):
+        h, w = operands(rows, d, vocab, dtype, seed=20 * i)
+        ids, top = teacher_of(rows, vocab, 5 + i, True)
+        x = (3 * rand(rows, vocab, seed=i)).to(dtype)
+        sets.append((h.requires_grad_(), w.requires_grad_(), x.requires_grad_(), labels_of(rows, vocab, 0.2, seed=i), ids,
+                     top))
+
+    def step(h, w, x, y, ids, top):
+        if op == "kept":
+            loss = L.distillation_loss(x, ids, top)
+            return (loss.detach(), *torch.autograd.grad(loss, x))
+        loss = L.linear_cross_entropy(h, w, y) if op == "entropy" else L.linear_distillation(h, w, ids, top)
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w)))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    wrong = [None, None]
+
+    def work(i):
+        wrong[i] = [t for t in range(turns) if not all(torch.equal(a, b) for a, b in zip(step(*sets[i]), want[i]))]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [[], []]
+
+
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+def test_two_streams_at_once(op):
+    sets = []
+    for i in range(2):
+        h, w = operands(700, 256, 9000, BF, seed=20 * i)
+        ids, top = teacher_of(700, 9000, 5 + i, True)
+        x = (3 * rand(700, 9000, seed=i)).to(BF)
+        sets.append((h.requires_grad_(), w.requires_grad_(), x.requires_grad_(), labels_of(700, 9000, 0.2, seed=i), ids, top))
+
+    def step(h, w, x, y, ids, top):
+        if op == "kept":
+            loss = L.distillation_loss(x, ids, top)
+            return (loss.detach(), *torch.autograd.grad(loss, x))
+        loss = L.linear_cross_entropy(h, w, y) if op == "entropy" else L.linear_distillation(h, w, ids, top)
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w)))
+
+    want = [step(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                got.append(step(*s))
+    torch.cuda.synchronize()
+    for i, one in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(one, want[i % 2])), i
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+def test_captured_rows(op, dtype):
+    """reduction="none" with its backward in a graph, and losses alone."""
+    h, w = operands(40, 64, 2000, dtype)
+    ids, top = teacher_of(40, 2000, 8, True)
+    y, g = labels_of(40, 2000, 0.2), rand(40, seed=3)
+    x = (3 * rand(40, 2000, seed=1)).to(dtype)
+    leaves = (x,) if op == "kept" else (h, w)
+    for t in leaves:
+        t.requires_grad_()
+
+    def loss(reduction):
+        return L.linear_cross_entropy(h, w, y, reduction=reduction) if op == "entropy" else (
+            L.linear_distillation(h, w, ids, top, reduction=reduction) if op == "teacher" else
+            L.distillation_loss(x, ids, top, reduction=reduction))
+
+    def step():
+        each = loss("none")
+        with torch.no_grad():
+            alone = loss("mean")
+        return (each.detach(), alone, *torch.autograd.grad(each, leaves, g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            for t in leaves:
+                t.copy_((t.float() * (0.9 + 0.1 * i)).to(dtype))
+            y.copy_(labels_of(40, 2000, 0.3, seed=i))
+            g.copy_(rand(40, seed=5 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), i
