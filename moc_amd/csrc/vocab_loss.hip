@@ -1153,6 +1153,21 @@ __global__ __launch_bounds__(256) void outer_kernel(const T* __restrict__ a, int
   for (int64_t i = blockIdx.y; i < m; i += gridDim.y) out[i * n + j] = Elem<OUT>::of(Elem<T>::one(a[i * lda]) * bj);
 }
 
+// The words behind the last whole four of f32 gradients of logits (the tiled f32
+// products take extents in fours): dh[r] += sum of d[r][j] w[j], j below rest.
+__global__ __launch_bounds__(256) void rest_words_kernel(const float* __restrict__ d, int64_t ldd,
+                                                         const float* __restrict__ w, int64_t ldw, int rest, int64_t rows,
+                                                         int hidden, float* __restrict__ dh) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows * hidden; i += step) {
+    const int64_t r = i / hidden;
+    const int k = static_cast<int>(i - r * hidden);
+    float s = dh[i];
+    for (int j = 0; j < rest; ++j) s = fmaf(d[r * ldd + j], w[j * ldw + k], s);
+    dh[i] = s;
+  }
+}
+
 // p *= *g in place over whole 16-byte chunks and what is behind them.
 template <typename T>
 __device__ __forceinline__ void scale_values(T* __restrict__ p, int64_t n, float f) {
@@ -1193,6 +1208,7 @@ unsigned blocks_of(int64_t n) {
 // 12.3, 11.6).
 constexpr int64_t kPieceBytes = 1LL << 30, kGradPieceBytes = (1LL << 31) - 4096;
 constexpr int64_t kWidest = 4;
+constexpr int64_t kF32Weight = 48LL << 20;
 // Few rows: dhidden comes from gradients in two bf16 parts, twice the rows, with the
 // weight as it is (TWO), else from f16 ones and a copy of the weight.  The copy moves 4
 // bytes of each of the weight's values, the parts cost as many products and 16 bytes of
@@ -1502,13 +1518,14 @@ extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, 
   if (!sizes_ok(rows, vocab, 0) || hidden < 1) return most;
   const Pieces p = pieces_of(dtype, rows, hidden, vocab, 0, grads != 0, nullptr);
   auto need = [&](int64_t b) { most = b > most ? b : most; };
+  const int64_t four = p.fused || vocab <= 4 ? vocab : vocab & ~3LL;
   for (int64_t i = 0; i < p.count; i += p.count > 1 ? p.count - 1 : 1) {  // the first piece and the last
     const int64_t n = i + 1 < p.count ? p.rows : rows - i * p.rows;
     if (!p.fused) need(moc_gemm_workspace_size(dtype, n, vocab, hidden, 0));
     if (!grads) continue;
-    need(!p.fused ? moc_gemm_workspace_size(dtype, n, hidden, vocab, 0)
+    need(!p.fused ? moc_gemm_workspace_size(dtype, n, hidden, four, 0)
                   : gemm_half_workspace(in_two_parts(rows, hidden, vocab) ? 2 * n : n, hidden, vocab));
-    need(p.fused ? gemm_half_workspace(vocab, hidden, n) : moc_gemm_workspace_size(dtype, vocab, hidden, n, 0));
+    need(p.fused ? gemm_half_workspace(vocab, hidden, n) : moc_gemm_workspace_size(dtype, four, hidden, n, 0));
   }
   return most;
 }
@@ -1599,6 +1616,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
   // a label is one word, the low half of its int64
   const int32_t* word_ids = words > 0 ? t.ids : reinterpret_cast<const int32_t*>(labels);
   const int64_t ld_ids = words > 0 ? words : 2;
+  const int64_t four = vocab & ~3LL;  // f32 products: rest_words_kernel
   const bool arrive = p.count == 1 && rows <= kArriveRows;
   const LossOut o{row_loss, arrive ? loss : nullptr, rows, mean, grads && rows > 0, count + kLossCounter};
   for (int64_t i = 0; i < p.count; ++i) {
@@ -1629,8 +1647,13 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
         slabs_loss_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(s, t, o);
       rc = check_launch("slabs_grad_kernel");
     } else {
-      rc = moc_gemm_ws(dtype, n, vocab, hidden, xi, ldx, 1, w, 1, ldw, 0, nullptr, 0, 0, nullptr, 0, 0, p.d, p.ldz,
-                       MOC_F32, gemm_ws, gemm_ws_bytes, stream);
+      // by words whose weights the last-level cache holds beside the logits, since every 64
+      // rows read them again: 1024 x 768 x 50257 795 us, in one product 1557
+      const int64_t fit = kF32Weight / (ldw * 4) / 64 * 64, cols = fit < 1024 ? 1024 : fit;
+      for (int64_t c = 0; c < vocab && rc == MOC_OK; c += cols)
+        rc = moc_gemm_ws(dtype, n, vocab - c < cols ? vocab - c : cols, hidden, xi, ldx, 1,
+                         static_cast<const float*>(w) + c * ldw, 1, ldw, 0, nullptr, 0, 0, nullptr, 0, 0,
+                         reinterpret_cast<float*>(p.d) + c, p.ldz, MOC_F32, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
       rc = logits_rows(true, p.d, n, vocab, p.ldz, t, r0, words, temperature, o, grads ? p.d : nullptr, p.ldz, st);
     }
@@ -1646,6 +1669,15 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       else
         two_parts_kernel<uint16_t><<<blocks, 256, 0, st>>>(p.both, size, t.alpha, static_cast<uint16_t*>(dh));
       if ((rc = check_launch("two_parts_kernel")) != MOC_OK) return rc;
+    } else if (dh != nullptr && f32 && vocab % 4 != 0 && vocab > 4) {
+      float* to = static_cast<float*>(dh) + r0 * hidden;
+      rc = moc_gemm_ws(dtype, n, hidden, four, p.d, p.ldz, 1, w, ldw, 1, 0, nullptr, 0, 0, nullptr, 0, 0, to, hidden, dh_dtype,
+                       gemm_ws, gemm_ws_bytes, stream);
+      if (rc != MOC_OK) return rc;
+      rest_words_kernel<<<blocks_of(n * hidden), 256, 0, st>>>(reinterpret_cast<const float*>(p.d) + four, p.ldz,
+                                                               static_cast<const float*>(w) + four * ldw, ldw,
+                                                               (int)(vocab - four), n, (int)hidden, to);
+      if ((rc = check_launch("rest_words_kernel")) != MOC_OK) return rc;
     } else if (dh != nullptr) {
       char* to = static_cast<char*>(dh) + r0 * hidden * (dh_dtype == MOC_F32 ? 4 : 2);
       const char* b = p.fused ? p.w : static_cast<const char*>(w);
@@ -1661,10 +1693,18 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       char* to = one ? static_cast<char*>(dw) : reinterpret_cast<char*>(i == 0 ? p.acc : p.part);
       const int to_dtype = one ? dw_dtype : MOC_F32;
       const char* b = p.x + r0 * p.ldx * es;
+      // f32: the whole fours, then the words behind them
+      const int64_t cut = f32 && vocab > 4 && n > 1 ? four : vocab;
+      if (cut < vocab) {
+        rc = moc_gemm_ws(dtype, vocab - cut, hidden, n, reinterpret_cast<const float*>(p.d) + cut, 1, p.ldz, b, p.ldx, 1, 0,
+                         nullptr, 0, 0, nullptr, 0, 0, reinterpret_cast<float*>(to) + cut * hidden, hidden, to_dtype, gemm_ws,
+                         gemm_ws_bytes, stream);
+        if (rc != MOC_OK) return rc;
+      }
       rc = n == 1    ? outer(f32, vocab, hidden, p.d, 1, b, t.alpha + 1, to, to_dtype, st)
            : p.fused ? gemm_half(vocab, hidden, n, p.d, 1, p.ldz, b, p.ldx, to, hidden, to_dtype, t.alpha + 1, gemm_ws,
                                  gemm_ws_bytes, stream)
-                     : moc_gemm_ws(dtype, vocab, hidden, n, p.d, 1, p.ldz, b, p.ldx, 1, 0, nullptr, 0, 0, nullptr, 0, 0, to,
+                     : moc_gemm_ws(dtype, cut, hidden, n, p.d, 1, p.ldz, b, p.ldx, 1, 0, nullptr, 0, 0, nullptr, 0, 0, to,
                                    hidden, to_dtype, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
       if (i > 0) {
