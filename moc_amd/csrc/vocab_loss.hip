@@ -1243,6 +1243,7 @@ struct Pieces {
   float *acc, *part, *z;
   char* two;    // few rows (in_two_parts): gradients in two parts,
   float* both;  // their product
+  float* rest;  // f32: rows of dweight behind the whole fours
   uint32_t* most;
   float2* stat;
   int64_t bytes;
@@ -1274,6 +1275,7 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   }
   if (f32 || grads) p.d = ws.take<char>(n * p.ldz * es);
   if (grads) p.x = ws.take<char>(rows * p.ldx * es);
+  if (grads && f32) p.rest = ws.take<float>(4 * hidden);
   if (grads && p.fused) {
     if (in_two_parts(rows, hidden, vocab)) {
       p.two = ws.take<char>(2 * rows * p.ldz * 2);
@@ -1523,6 +1525,7 @@ extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, 
     const int64_t n = i + 1 < p.count ? p.rows : rows - i * p.rows;
     if (!p.fused) need(moc_gemm_workspace_size(dtype, n, vocab, hidden, 0));
     if (!grads) continue;
+    if (four < vocab) need(moc_gemm_workspace_size(dtype, 4, hidden, n, 0));
     need(!p.fused ? moc_gemm_workspace_size(dtype, n, hidden, four, 0)
                   : gemm_half_workspace(in_two_parts(rows, hidden, vocab) ? 2 * n : n, hidden, vocab));
     need(p.fused ? gemm_half_workspace(vocab, hidden, n) : moc_gemm_workspace_size(dtype, four, hidden, n, 0));
@@ -1693,12 +1696,15 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       char* to = one ? static_cast<char*>(dw) : reinterpret_cast<char*>(i == 0 ? p.acc : p.part);
       const int to_dtype = one ? dw_dtype : MOC_F32;
       const char* b = p.x + r0 * p.ldx * es;
-      // f32: the whole fours, then the words behind them
+      // f32: the whole fours, and the words behind them as four of which the first count
+      // (columns of p.d up to a multiple of 64 are there; what they hold stays in its rows)
       const int64_t cut = f32 && vocab > 4 && n > 1 ? four : vocab;
       if (cut < vocab) {
-        rc = moc_gemm_ws(dtype, vocab - cut, hidden, n, reinterpret_cast<const float*>(p.d) + cut, 1, p.ldz, b, p.ldx, 1, 0,
-                         nullptr, 0, 0, nullptr, 0, 0, reinterpret_cast<float*>(to) + cut * hidden, hidden, to_dtype, gemm_ws,
-                         gemm_ws_bytes, stream);
+        rc = moc_gemm_ws(dtype, 4, hidden, n, reinterpret_cast<const float*>(p.d) + cut, 1, p.ldz, b, p.ldx, 1, 0, nullptr, 0,
+                         0, nullptr, 0, 0, p.rest, hidden, MOC_F32, gemm_ws, gemm_ws_bytes, stream);
+        if (rc != MOC_OK) return rc;
+        const int64_t size = (vocab - cut) * hidden;
+        rc = moc_copy_pad_2d(MOC_F32, p.rest, 1, size, size, reinterpret_cast<float*>(to) + cut * hidden, size, size, stream);
         if (rc != MOC_OK) return rc;
       }
       rc = n == 1    ? outer(f32, vocab, hidden, p.d, 1, b, t.alpha + 1, to, to_dtype, st)

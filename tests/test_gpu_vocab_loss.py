@@ -953,3 +953,33 @@ def test_captured_rows(op, dtype):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+@pytest.mark.parametrize("rows,d,vocab", [(3, 1, 7), (20, 30, 1001), (129, 333, 4099), (1, 101, 50), (2, 6, 5), (64, 9, 4),
+                                          (0, 5, 30)])
+@pytest.mark.parametrize("only", ["both", "hidden", "weight", "losses"])
+def test_f32_of_odd_sizes(rows, d, vocab, only):
+    """Hidden sizes and vocabularies that are no multiple of 4, in f32, and leading
+    dimensions; rows that lie apart."""
+    h, w = operands(rows, d, vocab, F32) if rows else (torch.zeros(0, d, device="cuda"), operands(1, d, vocab, F32)[1])
+    h = torch.cat([h, torch.full_like(h, math.nan)], 1)[:, :d].view(1, rows, d)
+    y = labels_of(rows, vocab, 0.2)
+    if rows:
+        y[0] = vocab - 1
+    h.requires_grad_(only in ("both", "hidden"))
+    w.requires_grad_(only in ("both", "weight"))
+    leaves = [t for t in (h, w) if t.requires_grad]
+    out = L.linear_cross_entropy(h, w, y.view(1, rows), reduction="sum")
+    got = iter(torch.autograd.grad(out, leaves) if leaves else ())
+    got = [next(got) if t.requires_grad else None for t in (h, w)]
+    assert got[0] is None or got[0].shape == h.shape
+    if not rows:
+        assert out == 0 and (got[1] is None or (got[1] == 0).all())
+        return
+    hd, wd = h.detach().view(rows, d).to(F64), w.detach().to(F64)
+    q = torch.zeros(rows, vocab, dtype=F64, device="cuda")
+    q[torch.arange(rows, device="cuda"), y.clamp(min=0)] = 1
+    one = torch.ones(rows, dtype=F64, device="cuda")
+    want, dz, c = reference(hd @ wd.t(), q, y != -100, one, 1.0, "sum")
+    got[0] = None if got[0] is None else got[0].view(rows, d)
+    check(out.detach(), want, got, (hd, wd), dz, c, q, logit_error(hd, wd), 1.0, 1.0, one)
