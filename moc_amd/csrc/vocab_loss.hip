@@ -1154,15 +1154,16 @@ __global__ __launch_bounds__(256) void outer_kernel(const T* __restrict__ a, int
 }
 
 // The words behind the last whole four of f32 gradients of logits (the tiled f32
-// products take extents in fours): dh[r] += sum of d[r][j] w[j], j below rest.
+// products take extents in fours): the sum of d[r][j] w[j], j below rest, is added
+// to dh[r] (add) or stored there.
 __global__ __launch_bounds__(256) void rest_words_kernel(const float* __restrict__ d, int64_t ldd,
-                                                         const float* __restrict__ w, int64_t ldw, int rest, int64_t rows,
-                                                         int hidden, float* __restrict__ dh) {
+                                                         const float* __restrict__ w, int64_t ldw, int add, int rest,
+                                                         int64_t rows, int hidden, float* __restrict__ dh) {
   const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows * hidden; i += step) {
     const int64_t r = i / hidden;
     const int k = static_cast<int>(i - r * hidden);
-    float s = dh[i];
+    float s = add ? dh[i] : 0.f;
     for (int j = 0; j < rest; ++j) s = fmaf(d[r * ldd + j], w[j * ldw + k], s);
     dh[i] = s;
   }
@@ -1243,7 +1244,7 @@ struct Pieces {
   float *acc, *part, *z;
   char* two;    // few rows (in_two_parts): gradients in two parts,
   float* both;  // their product
-  float* rest;  // f32: rows of dweight behind the whole fours
+  float* rest;  // f32: rows of dweight behind the whole fours; parts of dhidden
   uint32_t* most;
   float2* stat;
   int64_t bytes;
@@ -1275,7 +1276,7 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   }
   if (f32 || grads) p.d = ws.take<char>(n * p.ldz * es);
   if (grads) p.x = ws.take<char>(rows * p.ldx * es);
-  if (grads && f32) p.rest = ws.take<float>(4 * hidden);
+  if (grads && f32) p.rest = ws.take<float>((n > 4 ? n : 4) * hidden);
   if (grads && p.fused) {
     if (in_two_parts(rows, hidden, vocab)) {
       p.two = ws.take<char>(2 * rows * p.ldz * 2);
@@ -1520,7 +1521,7 @@ extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, 
   if (!sizes_ok(rows, vocab, 0) || hidden < 1) return most;
   const Pieces p = pieces_of(dtype, rows, hidden, vocab, 0, grads != 0, nullptr);
   auto need = [&](int64_t b) { most = b > most ? b : most; };
-  const int64_t four = p.fused || vocab <= 4 ? vocab : vocab & ~3LL;
+  const int64_t four = p.fused ? vocab : vocab & ~3LL;
   for (int64_t i = 0; i < p.count; i += p.count > 1 ? p.count - 1 : 1) {  // the first piece and the last
     const int64_t n = i + 1 < p.count ? p.rows : rows - i * p.rows;
     if (!p.fused) need(moc_gemm_workspace_size(dtype, n, vocab, hidden, 0));
@@ -1672,23 +1673,29 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       else
         two_parts_kernel<uint16_t><<<blocks, 256, 0, st>>>(p.both, size, t.alpha, static_cast<uint16_t*>(dh));
       if ((rc = check_launch("two_parts_kernel")) != MOC_OK) return rc;
-    } else if (dh != nullptr && f32 && vocab % 4 != 0 && vocab > 4) {
+    } else if (dh != nullptr && f32) {
       float* to = static_cast<float*>(dh) + r0 * hidden;
-      rc = moc_gemm_ws(dtype, n, hidden, four, p.d, p.ldz, 1, w, ldw, 1, 0, nullptr, 0, 0, nullptr, 0, 0, to, hidden, dh_dtype,
-                       gemm_ws, gemm_ws_bytes, stream);
-      if (rc != MOC_OK) return rc;
-      rest_words_kernel<<<blocks_of(n * hidden), 256, 0, st>>>(reinterpret_cast<const float*>(p.d) + four, p.ldz,
-                                                               static_cast<const float*>(w) + four * ldw, ldw,
-                                                               (int)(vocab - four), n, (int)hidden, to);
-      if ((rc = check_launch("rest_words_kernel")) != MOC_OK) return rc;
+      const float *d = reinterpret_cast<const float*>(p.d), *wf = static_cast<const float*>(w);
+      // words whose weights the tiled products reach with 32-bit offsets at a time
+      const int64_t reach = ((1LL << 31) - 64) / (ldw * 4) / 4 * 4, step = reach < 4 ? 4 : reach;
+      for (int64_t c = 0; c < four; c += step) {
+        rc = moc_gemm_ws(dtype, n, hidden, four - c < step ? four - c : step, d + c, p.ldz, 1, wf + c * ldw, ldw, 1, 0, nullptr,
+                         0, 0, nullptr, 0, 0, c == 0 ? to : p.rest, hidden, MOC_F32, gemm_ws, gemm_ws_bytes, stream);
+        if (rc != MOC_OK) return rc;
+        if (c == 0) continue;
+        add_f32_kernel<float><<<blocks_of(n * hidden), 256, 0, st>>>(to, p.rest, n * hidden, nullptr);
+        if ((rc = check_launch("add_f32_kernel")) != MOC_OK) return rc;
+      }
+      if (four < vocab) {
+        rest_words_kernel<<<blocks_of(n * hidden), 256, 0, st>>>(d + four, p.ldz, wf + four * ldw, ldw, four > 0,
+                                                                 (int)(vocab - four), n, (int)hidden, to);
+        if ((rc = check_launch("rest_words_kernel")) != MOC_OK) return rc;
+      }
     } else if (dh != nullptr) {
       char* to = static_cast<char*>(dh) + r0 * hidden * (dh_dtype == MOC_F32 ? 4 : 2);
-      const char* b = p.fused ? p.w : static_cast<const char*>(w);
-      rc = vocab == 1 ? outer(f32, n, hidden, p.d, p.ldz, b, t.alpha, to, dh_dtype, st)
-           : p.fused  ? gemm_half(n, hidden, vocab, p.d, p.ldz, 1, b, p.ldx, to, hidden, dh_dtype, t.alpha, gemm_ws,
-                                  gemm_ws_bytes, stream)
-                      : moc_gemm_ws(dtype, n, hidden, vocab, p.d, p.ldz, 1, b, ldw, 1, 0, nullptr, 0, 0, nullptr, 0, 0, to,
-                                    hidden, dh_dtype, gemm_ws, gemm_ws_bytes, stream);
+      rc = vocab == 1 ? outer(false, n, hidden, p.d, p.ldz, p.w, t.alpha, to, dh_dtype, st)
+                      : gemm_half(n, hidden, vocab, p.d, p.ldz, 1, p.w, p.ldx, to, hidden, dh_dtype, t.alpha, gemm_ws,
+                                  gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
     }
     if (dw != nullptr) {
@@ -1698,7 +1705,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       const char* b = p.x + r0 * p.ldx * es;
       // f32: the whole fours, and the words behind them as four of which the first count
       // (columns of p.d up to a multiple of 64 are there; what they hold stays in its rows)
-      const int64_t cut = f32 && vocab > 4 && n > 1 ? four : vocab;
+      const int64_t cut = f32 && n > 1 ? four : vocab;
       if (cut < vocab) {
         rc = moc_gemm_ws(dtype, 4, hidden, n, reinterpret_cast<const float*>(p.d) + cut, 1, p.ldz, b, p.ldx, 1, 0, nullptr, 0,
                          0, nullptr, 0, 0, p.rest, hidden, MOC_F32, gemm_ws, gemm_ws_bytes, stream);

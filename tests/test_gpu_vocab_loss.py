@@ -983,3 +983,26 @@ def test_f32_of_odd_sizes(rows, d, vocab, only):
     want, dz, c = reference(hd @ wd.t(), q, y != -100, one, 1.0, "sum")
     got[0] = None if got[0] is None else got[0].view(rows, d)
     check(out.detach(), want, got, (hd, wd), dz, c, q, logit_error(hd, wd), 1.0, 1.0, one)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 2), (700, 1), (700, 2), (700, 3), (65, 6)])
+def test_f32_of_a_few_words(rows, vocab):
+    test_f32_of_odd_sizes(rows, 40, vocab, "both")
+    test_f32_of_odd_sizes(rows, 64, vocab, "hidden")
+
+
+def test_f32_weight_beyond_32_bit_offsets():
+    """2.4 GB of f32 weight: dhidden from parts of the words."""
+    rows, d, vocab = 9, 4096, 146001
+    h, w = operands(rows, d, vocab, F32)
+    h.requires_grad_()
+    y = torch.tensor([5, vocab - 1, 131071, 131072, -100, 7, 9, 70000, 145999], device="cuda")
+    out = L.linear_cross_entropy(h, w, y, reduction="sum")
+    got = torch.autograd.grad(out, h)[0]
+    hd = h.detach().to(F64)
+    z = torch.cat([hd @ part.to(F64).t() for part in w.split(20000)], 1)
+    q = torch.zeros(rows, vocab, dtype=F64, device="cuda")
+    q[torch.arange(rows, device="cuda"), y.clamp(min=0)] = 1
+    one = torch.ones(rows, dtype=F64, device="cuda")
+    want, dz, c = reference(z, q, y != -100, one, 1.0, "sum")
+    check(out.detach(), want, (got, None), (hd, w.to(F64)), dz, c, q, logit_error(hd, w.to(F64)), 1.0, 1.0, one)
