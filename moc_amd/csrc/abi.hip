@@ -70,27 +70,42 @@ __global__ void copy_pad_2d_kernel(const T* __restrict__ src, int64_t rows, int6
   }
 }
 
-// bf16 copy into 16-byte aligned destination rows (dst_ld a multiple of 8):
-// row blockIdx.y, each thread one 8-element chunk of it, written with one
-// 16-byte store; the source (any alignment) is read element by element,
-// coalesced across the threads of the row.
-__global__ __launch_bounds__(256) void copy_pad_rows16_kernel(const uint16_t* __restrict__ src,
-                                                              int64_t cols, int64_t src_ld,
-                                                              uint16_t* __restrict__ dst,
-                                                              int64_t dst_ld, int64_t dst_cols) {
-  const int64_t r = blockIdx.y;
-  const int64_t c0 = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8;
-  if (c0 >= dst_cols) return;
-  const uint16_t* s = src + r * src_ld;
-  uint16_t v[8];
+// bf16 copy into 16-byte aligned destination rows (dst_ld a multiple of 8): a wave 512
+// columns of a row, four such parts' loads in flight, 8 elements a lane, read at any
+// address and written with one 16-byte store; what straddles the row's end element by
+// element.  Bound by its bytes: 67778 x 1500 80 us, 5.1 TB/s.
+typedef uint32_t loose16_t __attribute__((ext_vector_type(4), aligned(2)));
+
+__global__ __launch_bounds__(256) void copy_pad_rows16_kernel(const uint16_t* __restrict__ src, int64_t parts,
+                                                              int64_t row_parts, int64_t cols, int64_t src_ld,
+                                                              uint16_t* __restrict__ dst, int64_t dst_ld,
+                                                              int64_t dst_cols) {
+  constexpr int kParts = 4;
+  const int64_t waves = static_cast<int64_t>(gridDim.x) * 4;
+  for (int64_t p0 = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); p0 < parts; p0 += waves * kParts) {
+    uint4 o[kParts];
+    uint16_t* to[kParts];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (c0 + j < cols) ? s[c0 + j] : uint16_t(0);
-  uint4 o;
-  o.x = v[0] | (uint32_t(v[1]) << 16);
-  o.y = v[2] | (uint32_t(v[3]) << 16);
-  o.z = v[4] | (uint32_t(v[5]) << 16);
-  o.w = v[6] | (uint32_t(v[7]) << 16);
-  *reinterpret_cast<uint4*>(dst + r * dst_ld + c0) = o;
+    for (int i = 0; i < kParts; ++i) {
+      const int64_t p = p0 + waves * i, r = p / row_parts, c = (p - r * row_parts) * 512 + (threadIdx.x & 63) * 8;
+      o[i] = make_uint4(0, 0, 0, 0);
+      to[i] = p < parts && c < dst_cols ? dst + r * dst_ld + c : nullptr;
+      if (to[i] == nullptr || c >= cols) continue;
+      const uint16_t* s = src + r * src_ld + c;
+      if (c + 8 <= cols) {
+        const loose16_t v = *reinterpret_cast<const loose16_t*>(s);
+        o[i] = make_uint4(v[0], v[1], v[2], v[3]);
+      } else {
+        uint32_t v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? s[j] : 0;
+        o[i] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kParts; ++i)
+      if (to[i] != nullptr) *reinterpret_cast<uint4*>(to[i]) = o[i];
+  }
 }
 
 }  // namespace
@@ -127,11 +142,10 @@ extern "C" int moc_copy_pad_2d(int dtype, const void* src, int64_t rows, int64_t
   if (blocks > 8192) blocks = 8192;
   const dim3 grid(static_cast<unsigned>(blocks)), block(256);
   hipStream_t st = as_stream(stream);
-  if (dtype == MOC_BF16 && dst_ld % 8 == 0 && dst_cols % 8 == 0 && aligned16(dst) && rows <= 65535) {
-    const int64_t chunks = dst_cols / 8;
-    const dim3 g2(static_cast<unsigned>((chunks + 255) / 256), static_cast<unsigned>(rows));
-    copy_pad_rows16_kernel<<<g2, 256, 0, st>>>(static_cast<const uint16_t*>(src), cols, src_ld,
-                                              static_cast<uint16_t*>(dst), dst_ld, dst_cols);
+  if (dtype == MOC_BF16 && dst_ld % 8 == 0 && dst_cols % 8 == 0 && aligned16(dst)) {
+    const int64_t row_parts = (dst_cols + 511) / 512, parts = rows * row_parts, wgs = (parts + 3) / 4;
+    copy_pad_rows16_kernel<<<static_cast<unsigned>(wgs < 8192 ? wgs : 8192), 256, 0, st>>>(
+        static_cast<const uint16_t*>(src), parts, row_parts, cols, src_ld, static_cast<uint16_t*>(dst), dst_ld, dst_cols);
     return check_launch("copy_pad_rows16_kernel");
   }
   if (dtype == MOC_BF16)

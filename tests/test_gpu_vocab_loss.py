@@ -1006,3 +1006,24 @@ def test_f32_weight_beyond_32_bit_offsets():
     one = torch.ones(rows, dtype=F64, device="cuda")
     want, dz, c = reference(z, q, y != -100, one, 1.0, "sum")
     check(out.detach(), want, (got, None), (hd, w.to(F64)), dz, c, q, logit_error(hd, w.to(F64)), 1.0, 1.0, one)
+
+
+@pytest.mark.parametrize("rows,cols,ahead", [(1, 1, 1), (3, 7, 0), (5, 8, 3), (70000, 12, 1), (9, 511, 2), (66, 513, 7),
+                                             (4, 65533, 5), (1000, 1500, 4), (1, 4099, 0)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_padding_copy(rows, cols, ahead, dtype):
+    """Rows at any address into aligned ones: every value, zeros behind them, nothing else."""
+    from moc_amd import _native as N
+    from moc_amd import kernels as K
+    x = rand(rows, cols + ahead, seed=cols).to(dtype)[:, ahead:]
+    pitch = K.row_pitch(cols, dtype)
+    for width in (pitch, K.round_up(cols, 8) + 8):
+        out = torch.full((rows + 1, K.round_up(cols, 8) + 24 + pitch), 7.0, dtype=dtype, device="cuda")
+        out = out[:, :out.shape[1] // 8 * 8]
+        ld = out.stride(0) // 8 * 8
+        if ld != out.stride(0):
+            out = torch.full((rows + 1, ld), 7.0, dtype=dtype, device="cuda")
+        N.call("moc_copy_pad_2d", N.dtype_code(dtype), x.data_ptr(), rows, cols, x.stride(0) if rows > 1 else cols,
+               out.data_ptr(), ld, width, N.stream_of(x))
+        assert torch.equal(out[:rows, :cols], x)
+        assert (out[:rows, cols:width] == 0).all() and (out[:rows, width:] == 7).all() and (out[rows:] == 7).all()
