@@ -58,13 +58,25 @@ int launch_loss_gemm(const void* h, int64_t rows, int64_t hidden, int64_t ldh, c
                      int64_t ldw, float unit, const int32_t* ids, int64_t ld_ids, const uint16_t* first,
                      int64_t ld_first, int64_t words, float* z, float2* stat, void* kept, int64_t ld_kept, hipStream_t st);
 
-// C [M, N] = *alpha A B (f16 operands; alpha null: A B, bf16; A with a unit stride along
-// M or K, rows of B ldb apart; C bf16 or f32) (gemm.hip); 16-byte aligned rows,
-// workspace as moc_gemm_ws uses it.
+// C [M, N] = *alpha A B (f16 operands; A with a unit stride along M or K, rows of B ldb
+// apart; C bf16 or f32) (gemm.hip); 16-byte aligned rows, workspace as moc_gemm_ws uses
+// it.
 int64_t gemm_half_workspace(int64_t M, int64_t N, int64_t K);
 int gemm_half(int64_t M, int64_t N, int64_t K, const void* A, int64_t a_sm, int64_t a_sk, const void* B, int64_t ldb,
               void* C, int64_t ldc, int c_dtype, const float* alpha, void* workspace, int64_t workspace_bytes,
               void* stream);
+
+// C [rows, N] = *alpha (A[0 .. rows) + A[rows .. 2 rows)) B of bf16 operands where K is
+// split, the halves added up with its parts (done); else the product of all 2 rows in f32
+// (both).
+struct HalfPair {
+  void* C;
+  int c_dtype;
+  const float* alpha;
+  bool done;
+};
+int gemm_pair_rows(int64_t rows, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, float* both,
+                   HalfPair& out, void* workspace, int64_t workspace_bytes, void* stream);
 
 // out = x + y over n values (a multiple of 8), x and out f32, y bf16
 // (rmsnorm.hip).

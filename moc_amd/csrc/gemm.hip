@@ -1644,7 +1644,8 @@ template <bool OUT_F32>
 __device__ __forceinline__ void splitk_reduce_quad(int64_t q, const float* __restrict__ ws, int64_t stride,
                                                    int ksplit, int M, int N, int64_t ldw, void* __restrict__ C,
                                                    int64_t ldc, int vec, const uint16_t* __restrict__ res,
-                                                   int64_t ldres, const float* __restrict__ alpha = nullptr) {
+                                                   int64_t ldres, const float* __restrict__ alpha = nullptr,
+                                                   int64_t low = 0) {
   const int qpr = (N + 3) / 4;
   if (q >= static_cast<int64_t>(M) * qpr) return;
   const int row = static_cast<int>(q / qpr), c = static_cast<int>(q % qpr) * 4;
@@ -1656,6 +1657,15 @@ __device__ __forceinline__ void splitk_reduce_quad(int64_t q, const float* __res
     s.y += v.y;
     s.z += v.z;
     s.w += v.w;
+  }
+  if (low != 0) {  // the row's second part, `low` rows on
+    for (int i = 0; i < ksplit; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(p + low * ldw + i * stride);
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
   }
   if (alpha != nullptr) {
     const float f = *alpha;
@@ -1693,9 +1703,10 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float* __restr
                                                             void* __restrict__ C, int64_t ldc, int vec,
                                                             const uint16_t* __restrict__ res = nullptr,
                                                             int64_t ldres = 0,
-                                                            const float* __restrict__ alpha = nullptr) {
+                                                            const float* __restrict__ alpha = nullptr,
+                                                            int64_t low = 0) {
   splitk_reduce_quad<OUT_F32>(static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, ws, stride, ksplit, M, N,
-                              ldw, C, ldc, vec, res, ldres, alpha);
+                              ldw, C, ldc, vec, res, ldres, alpha, low);
 }
 
 // The sums of a grouped split-K launch's two products in one launch:
@@ -2667,13 +2678,28 @@ extern "C" int moc_gemm(int dtype, int64_t M, int64_t N, int64_t K, const void* 
 
 namespace {
 
+// The sum of a K split's parts of both halves of the rows (moc::gemm_pair_rows).
+int reduce_pair(const float* parts, int64_t stride, int ksplit, int64_t rows, int64_t N, int64_t ldw, HalfPair& out,
+                hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>((rows * ((N + 3) / 4) + 255) / 256));
+  const int vec = aligned16(out.C) && N % 4 == 0;
+  out.done = true;
+  if (out.c_dtype == MOC_F32)
+    splitk_reduce_kernel<true><<<grid, 256, 0, st>>>(parts, stride, ksplit, (int)rows, (int)N, ldw, out.C, N, vec, nullptr, 0,
+                                                     out.alpha, rows);
+  else
+    splitk_reduce_kernel<false><<<grid, 256, 0, st>>>(parts, stride, ksplit, (int)rows, (int)N, ldw, out.C, N, vec, nullptr,
+                                                      0, out.alpha, rows);
+  return check_launch("splitk_reduce_kernel");
+}
+
 // moc_gemm_ws with an optional bf16 residual R added to a bf16 C (res may be
 // null): C = bf16(bf16(A B (+ A2 B2)) + R).  step, alpha: see moc::gemm_half.
 int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int64_t a_sm, int64_t a_sk,
                  const void* B, int64_t b_sk, int64_t b_sn, int64_t K2, const void* A2, int64_t a2_sm,
                  int64_t a2_sk, const void* B2, int64_t b2_sk, int64_t b2_sn, void* C, int64_t ldc, int c_dtype,
                  void* workspace, int64_t workspace_bytes, void* stream, const void* res, int64_t ldres,
-                 int step = 1, const float* alpha = nullptr) {
+                 int step = 1, const float* alpha = nullptr, HalfPair* pair = nullptr) {
   MOC_REQUIRE(dtype == MOC_BF16 || dtype == MOC_F32, "moc_gemm: dtype must be bf16 or f32");
   MOC_REQUIRE(res == nullptr || (dtype == MOC_BF16 && c_dtype == MOC_BF16 && aligned16(res) && ldres % 8 == 0 &&
                                  ldres >= N),
@@ -2834,6 +2860,7 @@ int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int6
     if (rc != MOC_OK || mp.ksplit == 1) return rc;
     const dim3 grid(static_cast<unsigned>((M * ((N + 3) / 4) + 255) / 256));
     const float* parts = static_cast<const float*>(run.C);
+    if (pair != nullptr) return reduce_pair(parts, run.ws_stride, mp.ksplit, M / 2, N, mp.ldw, *pair, st);
     if (of)
       splitk_reduce_kernel<true><<<grid, 256, 0, st>>>(parts, run.ws_stride, mp.ksplit, (int)M, (int)N, mp.ldw, C, ldc,
                                                        a.vec_store, nullptr, 0, alpha);
@@ -2887,6 +2914,7 @@ int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int6
     const int64_t quads = M * ((N + 3) / 4);
     const dim3 grid(static_cast<unsigned>((quads + 255) / 256));
     const float* parts = static_cast<const float*>(run.C);
+    if (pair != nullptr) return reduce_pair(parts, run.ws_stride, sp.ksplit, M / 2, N, sp.ldw, *pair, st);
     if (of)
       splitk_reduce_kernel<true><<<grid, 256, 0, st>>>(parts, run.ws_stride, sp.ksplit, (int)M, (int)N, sp.ldw,
                                                        C, ldc, a.vec_store, nullptr, 0, alpha);
@@ -2911,7 +2939,7 @@ extern "C" int moc_gemm_ws(int dtype, int64_t M, int64_t N, int64_t K, const voi
 namespace moc {
 
 // C [M, N] = *alpha A B, A (a_sm, a_sk: one of them 1) and B [K, N] (rows of ldb)
-// in f16 (alpha null: C = A B of bf16), C in bf16 or f32: the gradients of a product
+// in f16, C in bf16 or f32: the gradients of a product
 // whose own gradient needs more than bf16's 8 bits.  As moc_gemm_ws, f16 at the same
 // rate (16384 x 2048 x 32000 1.64 ms, 32000 x 2048 x 16384 1.68: 1310 and 1280
 // TFLOP/s), but K is split up to 8 ways or in multiples of 8: workgroup ids go to the
@@ -2931,6 +2959,13 @@ int gemm_half(int64_t M, int64_t N, int64_t K, const void* A, int64_t a_sm, int6
               void* stream) {
   return gemm_ws_impl(MOC_BF16, M, N, K, A, a_sm, a_sk, B, ldb, 1, 0, nullptr, 0, 0, nullptr, 0, 0, C, ldc, c_dtype,
                       workspace, workspace_bytes, stream, nullptr, 0, 8, alpha);
+}
+
+int gemm_pair_rows(int64_t rows, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb, float* both,
+                   HalfPair& out, void* workspace, int64_t workspace_bytes, void* stream) {
+  out.done = false;
+  return gemm_ws_impl(MOC_BF16, 2 * rows, N, K, A, lda, 1, B, ldb, 1, 0, nullptr, 0, 0, nullptr, 0, 0, both, N, MOC_F32,
+                      workspace, workspace_bytes, stream, nullptr, 0, 8, nullptr, &out);
 }
 
 }  // namespace moc

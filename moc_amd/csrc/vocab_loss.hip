@@ -1132,7 +1132,8 @@ __global__ __launch_bounds__(256) void add_f32_kernel(float* a, const float* __r
   }
 }
 
-// The rows of a product with gradients in two parts: out = *alpha (a[r] + a[rows + r]).
+// The rows of a product with gradients in two parts, where no K split's sum adds them up
+// (gemm_pair_rows): out = *alpha (a[r] + a[rows + r]).
 template <typename OUT>
 __global__ __launch_bounds__(256) void two_parts_kernel(const float* __restrict__ a, int64_t n,
                                                         const float* __restrict__ alpha, OUT* __restrict__ out) {
@@ -1663,14 +1664,14 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     }
     if (rc != MOC_OK) return rc;
     if (dh != nullptr && two) {
-      rc = gemm_half(2 * n, hidden, vocab, p.two, p.ldz, 1, w, ldw, p.both, hidden, MOC_F32, nullptr, gemm_ws,
-                     gemm_ws_bytes, stream);
+      HalfPair sum{dh, dh_dtype, t.alpha, false};
+      rc = gemm_pair_rows(n, hidden, vocab, p.two, p.ldz, w, ldw, p.both, sum, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
       const int64_t size = n * hidden;
       const unsigned blocks = static_cast<unsigned>((size + 255) / 256);
-      if (dh_dtype == MOC_F32)
+      if (!sum.done && dh_dtype == MOC_F32)
         two_parts_kernel<float><<<blocks, 256, 0, st>>>(p.both, size, t.alpha, static_cast<float*>(dh));
-      else
+      else if (!sum.done)
         two_parts_kernel<uint16_t><<<blocks, 256, 0, st>>>(p.both, size, t.alpha, static_cast<uint16_t*>(dh));
       if ((rc = check_launch("two_parts_kernel")) != MOC_OK) return rc;
     } else if (dh != nullptr && f32) {
