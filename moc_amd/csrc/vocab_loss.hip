@@ -668,7 +668,7 @@ __global__ __launch_bounds__(TH) void logits_loss_kernel(const T* x, int64_t ld,
 }
 
 // ------------------------------------------------- logits that were not stored
-// Up to 16 rows, losses alone: the weight is read once, straight into the operand
+// Up to 16 rows: the weight is read once, straight into the operand
 // registers of v_mfma_f32_16x16x32_bf16 (a wave 16 words, a workgroup a slab of 64),
 // 16 loads ahead; the rows stand in LDS in fragment order.  Bound by the weight's
 // bytes: 32000 x 2048, 1 row 25.2 us, 5.2 TB/s, 16 rows 26.1; 128256 x 1024, 16 rows
@@ -677,14 +677,16 @@ constexpr int kFewRows = 16, kFewAhead = 16, kFewHidden = 4096, kFewSums = 4;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-// RAGGED: a hidden size that is no multiple of 32 (its masks cost 1.5 us of 28).
-template <bool RAGGED>
+// RAGGED: a hidden size that is no multiple of 32 (its masks cost 1.5 us of 28).  KEEP:
+// with exponentials as launch_loss_gemm keeps them.
+template <bool RAGGED, bool KEEP>
 __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restrict__ h, int64_t ldh, int rows,
                                                        const uint16_t* __restrict__ w, int64_t ldw, int vocab,
                                                        int hidden, float unit, const int32_t* __restrict__ ids,
                                                        int64_t ld_ids, const uint16_t* __restrict__ first,
                                                        int64_t ld_first, int words,
-                                                       float* __restrict__ z, float2* __restrict__ stat, int slabs) {
+                                                       float* __restrict__ z, float2* __restrict__ stat, int slabs,
+                                                       _Float16* __restrict__ kept, int64_t ld_kept) {
   extern __shared__ uint4 frag[];  // [steps][64], then the waves' maxima and sums
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int steps = (hidden + 31) / 32;
@@ -768,6 +770,17 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
     s += __shfl_xor(s, 32);
     if (lane < 16) part[(turn * 4 + wave) * 16 + row] = make_float2(m, s);
     __syncthreads();
+    if (KEEP && row < rows) {
+      typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+      float all = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) all = fmaxf(all, part[(turn * 4 + i) * 16 + row].x);
+      const float from = all == -INFINITY ? 0.f : all - 15.f;
+      f16x4_t e;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = static_cast<_Float16>(__builtin_amdgcn_exp2f(fmaf(acc[i], unit, -from)));
+      *reinterpret_cast<f16x4_t*>(kept + row * ld_kept + slab * kLossSlab + c0) = e;  // rows of whole slabs
+    }
     if (tid < rows) {
       float all = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -1395,7 +1408,7 @@ int sum_loss(const Targets& t, LossOut o, float* loss, hipStream_t st) {
 
 int few_lds(int64_t hidden) { return static_cast<int>((hidden + 31) / 32) * 1024 + 2 * 4 * 16 * 8; }
 
-// Whether few_rows_kernel takes a piece without gradients.  Not where its workgroups, two
+// Whether few_rows_kernel takes a piece of the rows.  Not where its workgroups, two
 // a CU, have two slabs or more while the tiles of the product are all on a CU at once.
 // us, it / the product, of 4 rows and 32000, 50021, 65536 and 128256 words:
 //   hidden  512    8.6 / 12.1   13.8 / 13.1    15.3 / 14.9    25.6 / 25.7
@@ -1408,20 +1421,22 @@ bool by_few(int64_t rows, int64_t hidden, int64_t vocab) {
   return 2 * few_lds(hidden) > 160 * 1024 || slabs_of(vocab) <= 2 * cus || (vocab + 255) / 256 > cus;
 }
 
-// Logits of up to kFewRows rows, losses alone.
+// Logits of up to kFewRows rows.
 int launch_few(const void* h, int64_t rows, int64_t hidden, int64_t ldh, const void* w, int64_t vocab, int64_t ldw,
                float unit, const int32_t* ids, int64_t ld_ids, const uint16_t* first, int64_t ld_first, int64_t words,
-               float* z, float2* stat, int64_t slabs, hipStream_t st) {
+               float* z, float2* stat, int64_t slabs, void* kept, int64_t ld_kept, hipStream_t st) {
   const int lds = few_lds(hidden);
   // what registers and LDS let a CU have, each as many slabs: 128256 x 4096 203 us, 221
   // with two a CU in turn; 50021 x 768 20.5, 22.8 with a workgroup a slab
   const int64_t resident = static_cast<int64_t>(cu_count()) * (2 * lds > 160 * 1024 ? 1 : 2);
   const int64_t rounds = (slabs + resident - 1) / resident;
   const unsigned grid = static_cast<unsigned>((slabs + rounds - 1) / rounds);
-  auto kernel = hidden % 32 != 0 ? few_rows_kernel<true> : few_rows_kernel<false>;
+  const bool ragged = hidden % 32 != 0;
+  auto kernel = kept != nullptr ? (ragged ? few_rows_kernel<true, true> : few_rows_kernel<false, true>)
+                                : (ragged ? few_rows_kernel<true, false> : few_rows_kernel<false, false>);
   kernel<<<grid, 256, lds, st>>>(static_cast<const uint16_t*>(h), ldh, (int)rows, static_cast<const uint16_t*>(w), ldw,
                                  (int)vocab, (int)hidden, unit, ids, ld_ids, first, ld_first, (int)words, z, stat,
-                                 (int)slabs);
+                                 (int)slabs, static_cast<_Float16*>(kept), ld_kept);
   return check_launch("few_rows_kernel");
 }
 
@@ -1630,9 +1645,9 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     if (p.fused) {
       const uint16_t* first = words > 0 ? t.first + r0 : nullptr;
       const float unit = kLog2E / temperature;
-      if (!grads && by_few(n, hidden, vocab))
+      if (by_few(n, hidden, vocab))
         rc = launch_few(xi, n, hidden, ldx, w, vocab, ldw, unit, word_ids + r0 * ld_ids, ld_ids, first, rows, n_words, p.z,
-                        p.stat, p.slabs, st);
+                        p.stat, p.slabs, grads ? p.d : nullptr, p.ldz, st);
       else
         rc = launch_loss_gemm(xi, n, hidden, ldx, w, vocab, ldw, unit, word_ids + r0 * ld_ids, ld_ids, first, rows, n_words,
                               p.z, p.stat, grads ? p.d : nullptr, p.ldz, st);

@@ -1027,3 +1027,25 @@ def test_padding_copy(rows, cols, ahead, dtype):
                out.data_ptr(), ld, width, N.stream_of(x))
         assert torch.equal(out[:rows, :cols], x)
         assert (out[:rows, cols:width] == 0).all() and (out[:rows, width:] == 7).all() and (out[rows:] == 7).all()
+
+
+@pytest.mark.parametrize("rows", [1, 5, 16])
+@pytest.mark.parametrize("d,vocab", [(64, 1000), (100, 4099), (1500, 777), (2048, 8190), (4093, 1003), (512, 65600)])
+@pytest.mark.parametrize("op", ["entropy", "teacher"])
+def test_gradients_of_few_rows(rows, d, vocab, op):
+    h, w = operands(rows, d, vocab, BF, seed=d)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    one = torch.ones(rows, dtype=F64, device="cuda")
+    hd, wd = h.detach().to(F64), w.detach().to(F64)
+    if op == "teacher":
+        ids, top = teacher_of(rows, vocab, 20, False)
+        q, some = shares(ids, top, vocab, 2.0)
+        out, heat = L.linear_distillation(h, w, ids, top, temperature=2.0), 2.0
+    else:
+        y = labels_of(rows, vocab, 0.0)
+        q, some = torch.zeros(rows, vocab, dtype=F64, device="cuda"), y >= 0
+        q[torch.arange(rows, device="cuda"), y] = 1
+        out, heat = L.linear_cross_entropy(h, w, y), 1.0
+    got = torch.autograd.grad(out, (h, w))
+    want, dz, c = reference(hd @ wd.t(), q, some, one, heat, "mean")
+    check(out.detach(), want, got, (hd, wd), dz, c, q, logit_error(hd, wd), heat, 1.0, one)
