@@ -276,7 +276,9 @@ def _gemm_workspace(dev: int, stream: int, where, nbytes: int) -> torch.Tensor:
     """Counters alone, which are zero between two launches, or the call's own workspace:
     parts of a product wait there for another launch, between which a second thread
     may put its own on the stream.  The call clears the counters of such a one."""
-    return _counters(dev, stream, where) if nbytes <= COUNTER_BYTES else torch.empty(nbytes, dtype=torch.uint8, device=where)
+    if nbytes <= COUNTER_BYTES:
+        return _counters(dev, stream, where)
+    return torch.empty(nbytes, dtype=torch.uint8, device=where)
 
 
 def _linear_pass(targets, saved, row_weight, mean, grad, product, hidden, weight, each: bool, dh: bool, dw: bool):
