@@ -1680,15 +1680,16 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
     }
     if (rc != MOC_OK) return rc;
     if (dh != nullptr && two) {
-      HalfPair sum{dh, dh_dtype, t.alpha, false};
+      void* to = static_cast<char*>(dh) + r0 * hidden * (dh_dtype == MOC_F32 ? 4 : 2);
+      HalfPair sum{to, dh_dtype, t.alpha, false};
       rc = gemm_pair_rows(n, hidden, vocab, p.two, p.ldz, w, ldw, p.both, sum, gemm_ws, gemm_ws_bytes, stream);
       if (rc != MOC_OK) return rc;
       const int64_t size = n * hidden;
       const unsigned blocks = static_cast<unsigned>((size + 255) / 256);
       if (!sum.done && dh_dtype == MOC_F32)
-        two_parts_kernel<float><<<blocks, 256, 0, st>>>(p.both, size, t.alpha, static_cast<float*>(dh));
+        two_parts_kernel<float><<<blocks, 256, 0, st>>>(p.both, size, t.alpha, static_cast<float*>(to));
       else if (!sum.done)
-        two_parts_kernel<uint16_t><<<blocks, 256, 0, st>>>(p.both, size, t.alpha, static_cast<uint16_t*>(dh));
+        two_parts_kernel<uint16_t><<<blocks, 256, 0, st>>>(p.both, size, t.alpha, static_cast<uint16_t*>(to));
       if ((rc = check_launch("two_parts_kernel")) != MOC_OK) return rc;
     } else if (dh != nullptr && f32) {
       float* to = static_cast<float*>(dh) + r0 * hidden;
