@@ -678,6 +678,22 @@ constexpr int kFewRows = 16, kFewAhead = 16, kFewHidden = 4096, kFewSums = 4;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
+// The column of the chunk of 8 that a quarter of the lanes loads in the last step: the
+// row's first where its own lies behind the hidden size, since a row may hold no more
+// than the hidden size up to a multiple of 8.
+constexpr int few_last_column(int hidden, int quad) {
+  const int k = (hidden - 1) / 32 * 32 + 8 * quad;
+  return k < hidden ? k : 0;
+}
+
+constexpr bool few_columns_in_rows() {
+  for (int hidden = 1; hidden <= kFewHidden; ++hidden)
+    for (int quad = 0; quad < 4; ++quad)
+      if (few_last_column(hidden, quad) + 8 > (hidden + 7) / 8 * 8) return false;
+  return true;
+}
+static_assert(few_columns_in_rows(), "a load behind its row");
+
 // RAGGED: a hidden size that is no multiple of 32 (its masks cost 1.5 us of 28).  KEEP:
 // with exponentials as launch_loss_gemm keeps them.
 template <bool RAGGED, bool KEEP>
@@ -693,7 +709,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
   const int steps = (hidden + 31) / 32;
   float2* part = reinterpret_cast<float2*>(frag + steps * 64);  // [2][4][16]
   const int row = lane & 15, quad = lane >> 4;
-  const bool ragged = RAGGED && 32 * (steps - 1) + 8 * quad >= hidden;  // its last chunk lies behind
+  const int last = few_last_column(hidden, quad) - 8 * quad;
   // what a chunk of 8 at column k holds of the hidden size (behind it is another tensor's
   // or padding)
   auto held = [&](uint4 v, int k) {
@@ -706,7 +722,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const uint16_t* __restric
 #pragma unroll
     for (int i = 0; i < kFewAhead; ++i) {
       const int s = min(s0 + i, steps - 1);
-      a[i] = *reinterpret_cast<const uint4*>(src + 32 * (ragged && s == steps - 1 ? 0 : s));
+      a[i] = *reinterpret_cast<const uint4*>(src + (RAGGED && s == steps - 1 ? last : 32 * s));
     }
   };
   auto word_of = [&](int slab) {

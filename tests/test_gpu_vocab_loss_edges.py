@@ -32,3 +32,20 @@ def test_few_rows_in_two_pieces(op):
     check(out.detach(), want, [t[:, cols] for t in got], (hd, wd), dz, c, q, logit_error(hd, wd), 1.0, 1.0, weight)
     for t in got:
         assert not t.index_fill(1, cols, 0).any()
+
+
+@pytest.mark.parametrize("d", [8, 17, 24])
+def test_few_rows_of_a_weight_up_to_its_segments_end(d):
+    """Hidden sizes of less than a step of the operand registers: the last word's row
+    ends the weight's memory."""
+    vocab = 1 << 21
+    h, w = operands(3, d, vocab, BF)
+    y = torch.tensor([vocab - 1, 5, -100], device="cuda")
+    hd, wd = h.to(F64), w.to(F64)
+    z = hd @ wd.t()
+    label = torch.zeros(3, vocab, dtype=F64, device="cuda")
+    label[torch.arange(3, device="cuda"), y.clamp(min=0)] = 1
+    one = torch.ones(3, dtype=F64, device="cuda")
+    want, _, _ = reference(z, label, y != -100, one, 1.0, "none")
+    check(L.linear_cross_entropy(h, w, y, reduction="none"), want, (None, None), (hd, wd), z, z, label, logit_error(hd, wd),
+          1.0, 1.0, one)
