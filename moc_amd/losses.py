@@ -122,14 +122,16 @@ class _Labels:
         """moc_linear_loss's arguments from labels to temperature."""
         return saved[0].data_ptr(), self.ignore, None, N.MOC_I32, 0, None, N.MOC_F32, 0, 0, 1.0
 
-    def rows_f32(self, saved, z):
-        """Each row's loss by f32 tensor operations, and whether it counts."""
-        labels = saved[0]
-        counts = labels != self.ignore
-        z = torch.where(counts[:, None], z, 0.0)
-        known = counts & (labels >= 0) & (labels < z.shape[1])
+    def counts(self, saved, vocab: int):
+        """The rows with a target."""
+        return saved[0] != self.ignore
+
+    def rows_f32(self, saved, on, z):
+        """Each row's loss by f32 tensor operations; finite where it is not `on`."""
+        labels = torch.where(on, saved[0], 0)
+        known = (labels >= 0) & (labels < z.shape[1])
         each = -torch.log_softmax(z, -1).gather(1, torch.where(known, labels, 0)[:, None])[:, 0]
-        return torch.where(known, each, math.nan), counts
+        return each * torch.where(known, 1.0, math.nan)
 
 
 class _Teacher:
@@ -146,23 +148,27 @@ class _Teacher:
         return (None, 0, ids.data_ptr(), N.idx_code(ids.dtype), ids.stride(0), top.data_ptr(), N.dtype_code(top.dtype),
                 top.stride(0), self.words, self.heat)
 
-    def rows_f32(self, saved, z):
+    def counts(self, saved, vocab: int):
+        return self._words(saved, vocab).any(1)
+
+    @staticmethod
+    def _words(saved, vocab: int):
         ids, top, _ = saved
-        ids, x = ids.long(), top.float()
-        there = (ids >= 0) & (ids < z.shape[1]) & (x != -math.inf)
-        counts = there.any(1)
+        return (ids >= 0) & (ids < vocab) & (top != -math.inf)
+
+    def rows_f32(self, saved, on, z):
+        there = self._words(saved, z.shape[1]) & on[:, None]
+        ids, x = torch.where(there, saved[0].long(), 0), saved[1].float()
         # from the largest, as masks of the type's lowest value over a T below 1 are beyond f32
-        x = torch.where(counts[:, None], torch.where(there, x, -math.inf), 0.0)
+        x = torch.where(on[:, None], torch.where(there, x, -math.inf), 0.0)
         log_q = torch.log_softmax((x - x.amax(1, keepdim=True)) / self.heat, 1)
-        z = torch.where(counts[:, None], z, 0.0)
         z = z - z.detach().amax(1, keepdim=True)
         q = torch.where(there, log_q.exp(), 0.0)
-        ids = torch.where(there, ids, 0)
         # shares of one word added up, each entry weighing its own part of them
         whole = torch.zeros_like(z).scatter_add(1, ids, q).gather(1, ids)
         log_p = torch.log_softmax(z / self.heat, -1).gather(1, ids)
         each = torch.where(q > 0, q * (torch.log(torch.where(q > 0, whole, 1.0)) - log_p), q)
-        return self.heat ** 2 * each.sum(1), counts
+        return self.heat ** 2 * each.sum(1)
 
 
 def _teacher(what: str, x, ids, top, row_weight, rows: int, temperature: float, reduction: str) -> _Teacher:
@@ -324,12 +330,17 @@ def _in_fours(targets, saved, row_weight, mean, grad, hidden, h, w, each: bool, 
     return out, *grads
 
 
-def _reduced_f32(targets, saved, z):
-    """The operator by f32 tensor operations."""
-    each, counts = targets.rows_f32(saved, z)
-    row_weight = saved[2]
+def _reduced_f32(targets, saved, rows, weight=None):
+    """The operator by f32 tensor operations: of rows of logits, or of hidden rows with
+    the head's weight.  Rows that do not count are zeros from the start, as a derivative
+    of 0 times their NaN would be NaN."""
+    vocab = rows.shape[1] if weight is None else weight.shape[0]
+    counts, row_weight = targets.counts(saved, vocab), saved[2]
     w = counts.float() if row_weight is None else torch.where(counts, row_weight, 0.0)
-    each = torch.where(w == 0, 0.0, each * w)
+    on = w != 0
+    rows = torch.where(on[:, None], rows, 0.0)
+    each = targets.rows_f32(saved, on, rows if weight is None else rows @ weight.t())
+    each = torch.where(on, each, 0.0) * w  # whatever the upstream gradient of the others
     if targets.reduction == "none":
         return each
     return each.sum() / (w.sum() if targets.reduction == "mean" else 1.0)
@@ -395,8 +406,8 @@ class _LinearLoss(torch.autograd.Function):
         dh, dw = ctx.needs_input_grad[3:5]
         if torch.is_grad_enabled():
             def stock(h, w):
-                z = (h.to(ctx.product).float() @ w.to(ctx.product).float().t()).reshape(-1, w.shape[0])
-                return _reduced_f32(targets, saved, z).reshape(g.shape)
+                h = h.to(ctx.product).float().reshape(-1, h.shape[-1])
+                return _reduced_f32(targets, saved, h, w.to(ctx.product).float()).reshape(g.shape)
             return (None, None, None, *graph_grads(stock, (hidden, weight), (dh, dw), g), *rest)
         if targets.reduction == "none":
             got = _linear_pass(targets, saved, _row_factors(saved, g), False, None, ctx.product, hidden, weight, True, dh,

@@ -1,4 +1,7 @@
-"""Losses over a vocabulary at the ends of what they take."""
+"""Losses over a vocabulary at the ends of what they take, and rows
+that count for nothing where a gradient has a graph of its own."""
+import math
+
 import pytest
 import torch
 
@@ -49,3 +52,60 @@ def test_few_rows_of_a_weight_up_to_its_segments_end(d):
     want, _, _ = reference(z, label, y != -100, one, 1.0, "none")
     check(L.linear_cross_entropy(h, w, y, reduction="none"), want, (None, None), (hd, wd), z, z, label, logit_error(hd, wd),
           1.0, 1.0, one)
+
+
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_rows_that_do_not_count_in_a_graph(op, reduction):
+    """create_graph: ignored rows, rows without words and rows of weight 0 hold NaN,
+    which reaches no gradient, as in the ones that the kernels compute."""
+    rows, d, vocab = 12, 32, 100
+    h, w = operands(rows, d, vocab, F32)
+    ids, top = teacher_of(rows, vocab, 6, False)
+    y = labels_of(rows, vocab, 0.0)
+    x = 2 * rand(rows, vocab, seed=1)
+    weight = rand(rows, seed=4).abs() + 0.5
+    dead = torch.tensor([1, 2, 7], device="cuda")
+    y[1], ids[1] = -100, -1
+    weight[2] = weight[7] = 0
+    top[7, 2] = math.nan
+    h[dead] = math.nan
+    x[dead] = math.nan
+    if op == "kept":
+        leaves = (x,)
+        run = lambda: L.distillation_loss(x, ids, top, weight, reduction=reduction)  # noqa: E731
+    else:
+        leaves = (h, w)
+        run = (lambda: L.linear_cross_entropy(h, w, y, weight, reduction=reduction)) if op == "entropy" else (
+            lambda: L.linear_distillation(h, w, ids, top, weight, reduction=reduction))
+    for t in leaves:
+        t.requires_grad_()
+    g = torch.tensor(0.5, device="cuda")
+    if reduction == "none":
+        g = rand(rows, seed=9).index_fill(0, dead, math.nan)
+    want = torch.autograd.grad(run(), leaves, g)
+    got = torch.autograd.grad(run(), leaves, g, create_graph=True)
+    for a, b in zip(got, want):
+        assert a.requires_grad and torch.isfinite(a).all() and torch.isfinite(b).all()
+        # two f32 computations of sums of up to 100 terms below the largest
+        assert (a - b).abs().max() <= 2 * 100 * 2.0 ** -23 * b.abs().max()
+    assert (got[0][dead] == 0).all()
+    again = torch.autograd.grad(sum((t * t).sum() for t in got), leaves)
+    assert all(torch.isfinite(t).all() for t in again) and (again[0][dead] == 0).all()
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+def test_unknown_label_in_a_graph(weighted):
+    """create_graph: a label outside the vocabulary gives NaN gradients, to its own
+    hidden row alone, and nothing where its row's weight is 0."""
+    h, w = operands(6, 64, 300, F32)
+    y = labels_of(6, 300, 0.0)
+    y[2], y[4] = 300, -5
+    weight = torch.ones(6, device="cuda")
+    weight[4] = 0
+    h.requires_grad_()
+    for graph in (False, True):
+        g = torch.autograd.grad(L.linear_cross_entropy(h, w, y, weight if weighted else None), h, create_graph=graph)[0]
+        # the mean of NaN losses sends finite factors to all rows
+        assert torch.isnan(g).all(1).tolist() == [i == 2 or (i == 4 and not weighted) for i in range(6)]
+        assert torch.isnan(g).any(1).tolist() == torch.isnan(g).all(1).tolist()
