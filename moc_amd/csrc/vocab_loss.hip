@@ -27,6 +27,8 @@
 // 16384 x 2048 x 32000: 5.7 ms, the three products 1.85, 1.64 and 1.68 (1160 to 1310
 // TFLOP/s; 6.44e12 FLOP take 4.75 at a large library product's rate), (4) 0.43 at 4.9
 // TB/s, (2) 0.07.
+#include <algorithm>
+
 #include "abi.h"
 #include "common.h"
 
@@ -303,11 +305,12 @@ template <typename ID, bool TOP_F32>
 __global__ __launch_bounds__(256) void teacher_targets_kernel(const ID* __restrict__ ids, int64_t ids_ld,
                                                               const void* __restrict__ top, int64_t top_ld, int words,
                                                               int vocab, float heat,
-                                                              const float* __restrict__ row_weight, Targets t) {
+                                                              const float* __restrict__ row_weight, Targets t,
+                                                              int64_t r0) {
   __shared__ int32_t id[kMaxWords], sorted_id[kMaxWords];
   __shared__ float q[kMaxWords], sorted_q[kMaxWords];
   __shared__ float red[4];
-  const int64_t r = blockIdx.x;
+  const int64_t r = r0 + blockIdx.x;
   const int tid = threadIdx.x;
   const float unit = kLog2E / heat;
   float mx = -INFINITY, any = 0.f;
@@ -1325,6 +1328,10 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
   return p;
 }
 
+// Rows of a launch with a workgroup a row: a grid has less than 2^32 threads, and one of
+// 1024 a row for the widest rows.
+constexpr int64_t kLaunchRows = 1 << 20;
+
 // A teacher as its caller has it.
 struct Teacher {
   const void* ids;
@@ -1347,8 +1354,9 @@ void launch_teacher(const Teacher& a, int64_t rows, int words, int vocab, const 
   else if (words <= 128) MOC_WAVES(2);
   else if (words <= 256) MOC_WAVES(4);
   else
-    teacher_targets_kernel<ID, TOP_F32><<<static_cast<unsigned>(rows), 256, 0, st>>>(ids, a.ids_ld, a.top, a.top_ld,
-                                                                                     words, vocab, a.heat, row_weight, t);
+    for (int64_t r0 = 0; r0 < rows; r0 += kLaunchRows)
+      teacher_targets_kernel<ID, TOP_F32><<<static_cast<unsigned>(std::min(rows - r0, kLaunchRows)), 256, 0, st>>>(
+          ids, a.ids_ld, a.top, a.top_ld, words, vocab, a.heat, row_weight, t, r0);
 #undef MOC_WAVES
 }
 
@@ -1409,10 +1417,15 @@ void launch_logits(const T* x, int64_t rows, int vocab, int64_t ld, const Target
 int logits_rows(bool f32, const void* x, int64_t rows, int64_t vocab, int64_t ld, const Targets& t, int64_t r0,
                 int64_t words, float heat, const LossOut& o, void* dx, int64_t ldd, hipStream_t st) {
   const int v = static_cast<int>(vocab), k = static_cast<int>(words);
-  if (f32)
-    launch_logits(static_cast<const float*>(x), rows, v, ld, t, r0, k, heat, o, static_cast<float*>(dx), ldd, st);
-  else
-    launch_logits(static_cast<const uint16_t*>(x), rows, v, ld, t, r0, k, heat, o, static_cast<uint16_t*>(dx), ldd, st);
+  for (int64_t i = 0; i < rows; i += kLaunchRows) {
+    const int64_t n = std::min(rows - i, kLaunchRows);
+    auto launch = [&](auto* to) {  // null: no gradients
+      auto* from = static_cast<decltype(to)>(const_cast<void*>(x));
+      launch_logits(from + i * ld, n, v, ld, t, r0 + i, k, heat, o, to == nullptr ? to : to + i * ldd, ldd, st);
+    };
+    if (f32) launch(static_cast<float*>(dx));
+    else launch(static_cast<uint16_t*>(dx));
+  }
   return check_launch("logits_loss_kernel");
 }
 

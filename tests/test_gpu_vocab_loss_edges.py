@@ -109,3 +109,44 @@ def test_unknown_label_in_a_graph(weighted):
         # the mean of NaN losses sends finite factors to all rows
         assert torch.isnan(g).all(1).tolist() == [i == 2 or (i == 4 and not weighted) for i in range(6)]
         assert torch.isnan(g).any(1).tolist() == torch.isnan(g).all(1).tolist()
+
+
+@pytest.mark.parametrize("words", [3, 0])
+def test_2_24_rows(words):
+    """As many rows as are taken, more than one launch has workgroups of 256 threads."""
+    rows, vocab = 1 << 24, 8
+    block = 1 << 12
+    g = torch.Generator().manual_seed(1)
+    if words:
+        x = torch.randn(block, vocab, generator=g).to(BF).cuda().repeat(rows // block, 1).requires_grad_()
+        ids = torch.randint(0, vocab, (block, words), generator=g).int().cuda().repeat(rows // block, 1)
+        top = torch.randn(block, words, generator=g).to(BF).cuda().repeat(rows // block, 1)
+        run = lambda n: L.distillation_loss(x[:n], ids[:n], top[:n], reduction="none")  # noqa: E731
+    else:
+        x = torch.randn(block, vocab, generator=g).cuda().repeat(rows // block, 1).requires_grad_()
+        w = torch.randn(5, vocab, generator=g).cuda()
+        y = torch.randint(0, 5, (block,), generator=g).cuda().repeat(rows // block)
+        run = lambda n: L.linear_cross_entropy(x[:n], w, y[:n], reduction="none")  # noqa: E731
+    each, few = run(rows), run(block)
+    assert torch.equal(each.view(-1, block), few.expand(rows // block, block))
+    up = rand(block, seed=3)
+    got = torch.autograd.grad(each, x, up.repeat(rows // block))[0].view(-1, block, vocab)
+    want = torch.autograd.grad(few, x, up)[0][:block]
+    assert torch.equal(got, want.expand_as(got))
+
+
+@pytest.mark.parametrize("op", ["kept", "linear"])
+def test_many_rows_of_many_words(op):
+    """Rows of more than 256 words of a teacher, in more than one launch."""
+    rows, block, vocab, words = (1 << 20) + 5, 1 << 10, 300, 257
+    ids, top = teacher_of(block, vocab, words, True, top_dtype=BF)
+    full = lambda t: torch.cat([t.repeat(rows // block, 1), t[:rows % block]])  # noqa: E731
+    if op == "kept":
+        x = (2 * rand(block, vocab, seed=1)).to(BF)
+        run = lambda x, ids, top: L.distillation_loss(x, ids, top, reduction="none")  # noqa: E731
+    else:
+        x, w = operands(block, 16, vocab, BF)
+        run = lambda x, ids, top: L.linear_distillation(x, w, ids, top, reduction="none")  # noqa: E731
+    few = run(x, ids, top)
+    each = run(full(x), full(ids), full(top))
+    assert torch.equal(each, full(few[:, None])[:, 0])
