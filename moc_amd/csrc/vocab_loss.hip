@@ -56,7 +56,7 @@ struct Targets {
   // over all rows
   double* total;    // sum of the weights (1 for a sum of losses)
   float* factor;    // upstream gradient / total
-  float* largest;   // a power of two, no weight above it; 0: no row counts
+  float* largest;   // a power of two, no finite weight above it; 0: no row counts
   float* alpha;     // [2] what the f16 products for dhidden and dweight are times
 };
 
@@ -185,7 +185,8 @@ __device__ __forceinline__ void put_total(const Targets& t, int64_t rows, int me
   for (int64_t r = threadIdx.x; r < rows; r += blockDim.x) {
     const float w = FAR ? get_far(t.weight + r) : weight_of(t, r);
     s += w;
-    m = fmaxf(m, fabsf(w));
+    // an infinite weight makes its own row's gradient infinite, not the others' 0
+    m = fmaxf(m, fabsf(w) < INFINITY ? fabsf(w) : 0x1p-126f);
   }
   s = block_sum64(s, red64);
   m = block_reduce<true>(m, red);

@@ -150,3 +150,25 @@ def test_many_rows_of_many_words(op):
     few = run(x, ids, top)
     each = run(full(x), full(ids), full(top))
     assert torch.equal(each, full(few[:, None])[:, 0])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("op", ["entropy", "teacher", "kept"])
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+def test_infinite_factor_of_one_row(op, dtype, value):
+    """An infinite upstream gradient of one row leaves the others' gradients as they are."""
+    h, w = operands(40, 64, 900, dtype)
+    ids, top = teacher_of(40, 900, 5, False)
+    y = labels_of(40, 900, 0.2)
+    x = (3 * rand(40, 900, seed=1)).to(dtype).requires_grad_()
+    h.requires_grad_()
+    y[7] = 3
+    each = L.linear_cross_entropy(h, w, y, reduction="none") if op == "entropy" else (
+        L.linear_distillation(h, w, ids, top, reduction="none") if op == "teacher" else
+        L.distillation_loss(x, ids, top, reduction="none"))
+    g, leaf = rand(40, seed=2), x if op == "kept" else h
+    others = torch.arange(40, device="cuda") != 7
+    want = torch.autograd.grad(each, leaf, torch.where(others, g, 0.0), retain_graph=True)[0]
+    got = torch.autograd.grad(each, leaf, torch.where(others, g, value))[0]
+    assert torch.equal(got[others], want[others])
+    assert not torch.isfinite(got[7]).any()
