@@ -44,6 +44,9 @@ from .block import graph_grads, plain
 BF16, F32 = torch.bfloat16, torch.float32
 REDUCTIONS = ("mean", "sum", "none")
 COUNTER_BYTES = 4096  # MOC_GEMM_WS_COUNTER_BYTES
+# Elements between two rows that the products' 32-bit offsets take: 256 rows, a tile and the
+# fewest of a piece, within 2 GiB.
+MOST_PITCH = 1 << 21
 
 
 def linear_cross_entropy(hidden, weight, labels, row_weight=None, *, ignore_index: int = -100,
@@ -200,13 +203,14 @@ def _unit(t):
 # -------------------------------------------------------------------- operands
 def _rows16(t, most: int = 1 << 62) -> torch.Tensor:
     """t [rows, cols] with 16-byte aligned rows of unit stride, at most four times their
-    length apart and bf16 ones within `most` bytes, whose storage holds all of the last
-    one's pitch (the kernels read whole chunks); a copy of any other."""
+    length and MOST_PITCH apart and bf16 ones within `most` bytes, whose storage holds all
+    of the last one's pitch (the kernels read whole chunks); a copy of any other."""
     rows, cols = t.shape
     per = 16 // t.element_size()
     pitch = _pitch(t)
     if (t.stride(1) == 1 or cols == 1) and t.data_ptr() % 16 == 0 and pitch % per == 0 and (
-            cols <= pitch <= 4 * K.round_up(cols, 64)) and (t.dtype != BF16 or rows * pitch * 2 < most) and (
+            cols <= pitch <= min(4 * K.round_up(cols, 64), MOST_PITCH)) and (
+            t.dtype != BF16 or rows * pitch * 2 < most) and (
             (t.storage_offset() + rows * pitch) * t.element_size() <= t.untyped_storage().nbytes()):
         return t
     out = K.padded_empty(rows, cols, t.dtype, t.device)

@@ -172,3 +172,15 @@ def test_infinite_factor_of_one_row(op, dtype, value):
     got = torch.autograd.grad(each, leaf, torch.where(others, g, value))[0]
     assert torch.equal(got[others], want[others])
     assert not torch.isfinite(got[7]).any()
+
+
+def test_hidden_rows_far_apart():
+    """Views whose rows' pitch passes what the products address: copies of them."""
+    d, vocab = 1 << 20, 66
+    cols = torch.arange(64, device="cuda") * (d // 64)
+    h, w = operands(3, 64, vocab, BF)
+    y = labels_of(3, vocab, 0.0)
+    wide = lambda t, pitch: torch.zeros(t.shape[0], pitch, dtype=BF, device="cuda").index_copy(1, cols, t)[:, :d]  # noqa: E731
+    want = L.linear_cross_entropy(wide(h, d), wide(w, d), y, reduction="none")
+    assert torch.equal(want, L.linear_cross_entropy(wide(h, 4 * d), wide(w, d), y, reduction="none"))
+    assert torch.equal(want, L.linear_cross_entropy(wide(h, d), wide(w, 4 * d), y, reduction="none"))
