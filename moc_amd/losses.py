@@ -77,11 +77,10 @@ def distillation_loss(logits, teacher_ids, teacher_logits, row_weight=None, *, t
     """linear_distillation of logits [..., vocab] (bf16 or f32) that are there already."""
     what = "distillation_loss"
     rows = _rows_of(what, logits, None, row_weight, reduction)
-    if not plain(logits):
-        raise ValueError(f"{what}: plain tensors only")
     if not 1 <= logits.shape[-1] <= 1 << 21:
         raise ValueError(f"{what}: a vocabulary of 1 to 2^21 words, got {logits.shape[-1]}")
     targets = _teacher(what, logits, teacher_ids, teacher_logits, row_weight, rows, temperature, reduction)
+    _refuse_subclasses(what, logits, *targets.tensors())
     dev = N.one_device(logits, *targets.tensors())
     if not N.is_current(dev):
         with torch.cuda.device(dev):
@@ -106,6 +105,11 @@ def _rows_of(what: str, x, labels, row_weight, reduction: str) -> int:
     if rows > 1 << 24:
         raise ValueError(f"{what}: up to 2^24 rows, got {rows}")
     return rows
+
+
+def _refuse_subclasses(what: str, *tensors) -> None:
+    if not plain(*(t for t in tensors if t is not None)):
+        raise ValueError(f"{what}: plain tensors only")
 
 
 def _flat(t, rows: int):
@@ -236,8 +240,7 @@ def _pitch(t) -> int:
 def _linear(what: str, hidden, weight, targets) -> torch.Tensor:
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[-1] or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"{what}: weight is [vocab, {hidden.shape[-1]}], got {tuple(weight.shape)}")
-    if not plain(hidden, weight):
-        raise ValueError(f"{what}: plain tensors only")
+    _refuse_subclasses(what, hidden, weight, *targets.tensors())
     product = hidden.dtype
     if torch.is_autocast_enabled("cuda"):
         product = torch.get_autocast_dtype("cuda")
