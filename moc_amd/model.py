@@ -14,7 +14,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .block import (attention_half, attention_half_ok, bare, final_norm, lm_head, lm_head_ok, next_token_loss,
-                    next_token_loss_ok, plain, runs_stock, stock_method, stream_dtype)
+                    next_token_loss_ok, plain, runs_stock, stock_method)
 from .config import MoCConfig
 from .ffn import MoCSwiGLUFFN, block_ffn, block_ffn_f32_ok, block_ffn_ok, build_ffn
 from .losses import linear_cross_entropy, linear_distillation
@@ -149,21 +149,32 @@ class LLaMAModel(nn.Module):
     def _head_weight(self):
         return self.tok_emb.weight if self.lm_head is None else getattr(self.lm_head, "weight", None)
 
-    def _head_is_plain(self, h) -> bool:
-        """The logits are h @ weight.T of tensors that the losses' kernels read."""
+    def _loss_rows(self, h):
+        """The rows that the logits are made of, norm(h), and whether that is a product with
+        the head's weight of which the losses' kernels read both."""
         head, weight = self.lm_head, self._head_weight()
-        return (stream_dtype(h) is not None and runs_stock(self, "_logits") and plain(h, weight) and
-                (head is None or (type(head) is nn.Linear and head.bias is None and bare(head))))
+        if not (h.is_cuda and runs_stock(self, "_logits") and plain(h, weight) and
+                (head is None or (type(head) is nn.Linear and head.bias is None and bare(head)))):
+            return self.norm(h), False
+        x = final_norm(h, self.norm, RMSNorm)
+        types = {x.dtype, weight.dtype}
+        if torch.is_autocast_enabled("cuda"):
+            taken = torch.get_autocast_dtype("cuda") == torch.bfloat16 and types <= {torch.bfloat16, torch.float32}
+        else:
+            taken = types in ({torch.bfloat16}, {torch.float32})
+        return x, taken and plain(x)
 
     def loss(self, input_ids, labels, row_weight=None):
         """forward(input_ids, labels)[1] in f32 without the logits, which exist for a
-        piece of the positions at a time (losses.linear_cross_entropy).  row_weight
-        [batch, seq] (f32): the weight of position t's loss, against label t + 1."""
-        h = self._hidden(input_ids)
+        piece of the positions at a time (losses.linear_cross_entropy); of all positions
+        off the device, in other types than distill's and where the head is not a plain
+        product.  row_weight [batch, seq] (f32): the weight of position t's loss, against
+        label t + 1."""
+        x, taken = self._loss_rows(self._hidden(input_ids))
         target = F.pad(labels[:, 1:], (0, 1), value=-100)
-        if self._head_is_plain(h):
-            return linear_cross_entropy(final_norm(h, self.norm, RMSNorm), self._head_weight(), target, row_weight)
-        logits = self._logits(self.norm(h)).float()
+        if taken:
+            return linear_cross_entropy(x, self._head_weight(), target, row_weight)
+        logits = self._logits(x).float()
         each = F.cross_entropy(logits.flatten(0, 1), target.flatten(), ignore_index=-100, reduction="none")
         weight = (target != -100).float().flatten()
         if row_weight is not None:
@@ -173,13 +184,12 @@ class LLaMAModel(nn.Module):
     def distill(self, input_ids, teacher_ids, teacher_logits, row_weight=None, *, temperature: float = 1.0):
         """The divergence of the model's logits from a teacher's top ones at the same
         positions, [batch, seq, words] ids and logits (losses.linear_distillation, which
-        describes them and row_weight).  Device tensors in bf16, or f32 under bf16
-        autocast."""
-        h = self._hidden(input_ids)
-        if not self._head_is_plain(h):
-            raise ValueError("distill takes a plain LM head on the device, in bf16 or in f32 under bf16 autocast")
-        return linear_distillation(final_norm(h, self.norm, RMSNorm), self._head_weight(), teacher_ids, teacher_logits,
-                                   row_weight, temperature=temperature)
+        describes them and row_weight).  Device tensors in bf16 or f32, or either under
+        bf16 autocast."""
+        x, taken = self._loss_rows(self._hidden(input_ids))
+        if not taken:
+            raise ValueError("distill takes a plain LM head on the device, in bf16 or f32 or under bf16 autocast")
+        return linear_distillation(x, self._head_weight(), teacher_ids, teacher_logits, row_weight, temperature=temperature)
 
     def forward(self, input_ids, labels=None):
         h = self._hidden(input_ids)
