@@ -353,6 +353,14 @@ def _reduced_f32(targets, saved, rows, weight=None):
     return each.sum() / (w.sum() if targets.reduction == "mean" else 1.0)
 
 
+def cross_entropy_f32(logits, labels, row_weight=None):
+    """linear_cross_entropy's mean of logits that are there already, by f32 tensor
+    operations, on any device."""
+    rows = labels.numel()
+    targets = _Labels(labels.reshape(rows), None if row_weight is None else row_weight.reshape(rows), -100, "mean")
+    return _reduced_f32(targets, targets.tensors(), logits.float().flatten(0, -2))
+
+
 def _capture(dev: int) -> int:
     """What names the HIP graph that the current stream is captured into, or 0."""
     return N.query("moc_capture_id", N.stream_on(dev)) if torch.cuda.is_current_stream_capturing() else 0

@@ -17,7 +17,7 @@ from .block import (attention_half, attention_half_ok, bare, final_norm, lm_head
                     next_token_loss_ok, plain, runs_stock, stock_method)
 from .config import MoCConfig
 from .ffn import MoCSwiGLUFFN, block_ffn, block_ffn_f32_ok, block_ffn_ok, build_ffn
-from .losses import linear_cross_entropy, linear_distillation
+from .losses import cross_entropy_f32, linear_cross_entropy, linear_distillation
 
 FFN_TYPES = ("dense", "moc", "moc_gcp", "moc_2_8", "moc_post_silu_abs")
 
@@ -174,12 +174,7 @@ class LLaMAModel(nn.Module):
         target = F.pad(labels[:, 1:], (0, 1), value=-100)
         if taken:
             return linear_cross_entropy(x, self._head_weight(), target, row_weight)
-        logits = self._logits(x).float()
-        each = F.cross_entropy(logits.flatten(0, 1), target.flatten(), ignore_index=-100, reduction="none")
-        weight = (target != -100).float().flatten()
-        if row_weight is not None:
-            weight = torch.where(weight > 0, row_weight.flatten(), 0.0)
-        return torch.where(weight == 0, 0.0, each * weight).sum() / weight.sum()
+        return cross_entropy_f32(self._logits(x), target, row_weight)
 
     def distill(self, input_ids, teacher_ids, teacher_logits, row_weight=None, *, temperature: float = 1.0):
         """The divergence of the model's logits from a teacher's top ones at the same
