@@ -496,7 +496,7 @@ __device__ __forceinline__ uint4 load_chunk(const float* p) {
   const chunk_t v = *reinterpret_cast<const loose4_t*>(p);
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
-// Elements p[0 .. per of the input chunk) = c exp2(unit x - lse).
+// A chunk's elements as T, to any element's address.
 __device__ __forceinline__ void store_grad(uint16_t* p, const float (&v)[8]) {
   chunk_t o;
 #pragma unroll

@@ -24,11 +24,20 @@ out of the mean, which is NaN where no row is left.  A label outside the vocabul
 gives NaN, as do NaN logits in rows that count.
 
 Losses are f32.  Operands are bf16 or f32, or either under bf16 autocast, where the
-products are those of bf16 casts and gradients come in the operands' own types.  The
-gradients of bf16 products' logits are f16 scaled by the largest row weight: rows
-whose weight is less than 2^-28 of it lose bits, below 2^-39 all of them.  An upstream
-factor that is no power of two rounds bf16 gradients a second time.  A backward with
-create_graph=True takes f32 tensor operations, with the logits of all rows.
+products are those of bf16 casts and gradients come in the operands' own types.  An
+upstream factor that is no power of two rounds bf16 gradients a second time.  A backward
+with create_graph=True takes f32 tensor operations, with the logits of all rows.
+
+Logits of bf16 products may be up to 2^22 temperatures in size.  Their gradients pass
+through f16, with ranges of their own:
+  gradients of logits, w_r / W (p - q) with W the largest finite row weight to a power of
+    two, have all bits down to 2^-28, fewer below and none from 2^-39;
+  hidden rows for dweight and the weight for dhidden are scaled by one power of two a
+    tensor, so that channels far smaller than others are rounded: values below 2^-19 of
+    hidden rows by up to 2^-27, below 2^-23 of a weight by up to 2^-31, or, where a
+    tensor's largest is outside [2^-3, 2^13] and [2^-7, 2^9], values below 2^-32 of it by
+    up to 2^-39 of it.  dweight of a channel of such values, and of a word whose p is as
+    small in every row, has few bits or is 0.  (A few hundred rows: the weight stays bf16.)
 """
 from __future__ import annotations
 

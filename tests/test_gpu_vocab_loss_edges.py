@@ -184,3 +184,38 @@ def test_hidden_rows_far_apart():
     want = L.linear_cross_entropy(wide(h, d), wide(w, d), y, reduction="none")
     assert torch.equal(want, L.linear_cross_entropy(wide(h, 4 * d), wide(w, d), y, reduction="none"))
     assert torch.equal(want, L.linear_cross_entropy(wide(h, d), wide(w, 4 * d), y, reduction="none"))
+
+
+@pytest.mark.parametrize("up", [0, 20, -30])
+@pytest.mark.parametrize("rows", [40, 600])
+def test_small_channels_beside_large_ones(rows, up):
+    """bf16: channels down to 2^-40 of the largest.  The products for the gradients take
+    hidden rows and weight as f16 under one power of two, which holds bf16 values above
+    2^-19 and 2^-23 as they are (above 2^-32 of a largest that is far from 1) and rounds
+    smaller ones by 2^-27 and 2^-31 (2^-39 of it) at most."""
+    d, vocab = 82, 700
+    h, w = operands(rows, d, vocab, BF)
+    size = 2.0 ** -(torch.arange(d, device="cuda") % 41).float()
+    h = (h.float() * size * 2.0 ** up).to(BF).requires_grad_()
+    w = (w.float() * size.flip(0) * 2.0 ** -up).to(BF).requires_grad_()
+    y = labels_of(rows, vocab, 0.2)
+    out = L.linear_cross_entropy(h, w, y, reduction="sum")
+    got = torch.autograd.grad(out, (h, w))
+    hd, wd = h.detach().to(F64), w.detach().to(F64)
+    q = torch.zeros(rows, vocab, dtype=F64, device="cuda")
+    q[torch.arange(rows, device="cuda"), y.clamp(min=0)] = 1
+    one = torch.ones(rows, dtype=F64, device="cuda")
+    want, dz, c = reference(hd @ wd.t(), q, y != -100, one, 1.0, "sum")
+    z_err = logit_error(hd, wd)
+    assert abs(out.item() - want.item()) <= (2 * z_err + 2.0 ** -20 * math.log(2 * vocab)) * rows
+    soft = dz.abs() + c * q
+    rel = 2.01 * 2.0 ** -11 + 4 * z_err
+    for g, exact, terms, other, lost in ((got[0], dz @ wd, soft, wd, 2.0 ** -31), (got[1], dz.t() @ hd, soft.t(), hd, 2.0 ** -27)):
+        if up:
+            lost = 2.0 ** -39 * other.abs().max().item()
+        # dlogits' roundings (2^-39 of the row's factor where they are smallest), f32 sums, the operand's rounding
+        tol = (rel + (4 * math.sqrt(terms.shape[1]) + 2) * 2.0 ** -24) * (terms @ other.abs())
+        tol = tol + 2.0 ** -39 * other.abs().sum(0) + lost * terms.sum(1)[:, None]
+        tol = tol * (1 + 2.0 ** -7) + 2.0 ** -8 * exact.abs() + 1e-38
+        err = (g.to(F64) - exact).abs()
+        assert (err <= tol).all(), (err / tol).max()
