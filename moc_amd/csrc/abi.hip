@@ -6,6 +6,8 @@
 // every buffer, so each entry point can be recorded into a HIP graph.
 #include <stdio.h>
 
+#include <algorithm>
+
 #include "abi.h"
 #include "common.h"
 
@@ -71,40 +73,39 @@ __global__ void copy_pad_2d_kernel(const T* __restrict__ src, int64_t rows, int6
 }
 
 // bf16 copy into 16-byte aligned destination rows (dst_ld a multiple of 8): a wave 512
-// columns of a row, four such parts' loads in flight, 8 elements a lane, read at any
-// address and written with one 16-byte store; what straddles the row's end element by
-// element.  Bound by its bytes: 67778 x 1500 80 us, 5.1 TB/s.
+// columns of a row at a time, 8 elements a lane, read at any address and written with one
+// 16-byte store.  Parts are counted in 32 bits, since a 64-bit division takes longer than
+// the rest of a small copy.  Bound by its bytes: 67778 x 1500 73 us, 5.6 TB/s; small ones
+// by latency: 16 x 5461 2.0 us, 16 x 700 2.0.
+constexpr int64_t kCopyParts = 1 << 30;  // of a launch
 typedef uint32_t loose16_t __attribute__((ext_vector_type(4), aligned(2)));
 
-__global__ __launch_bounds__(256) void copy_pad_rows16_kernel(const uint16_t* __restrict__ src, int64_t parts,
-                                                              int64_t row_parts, int64_t cols, int64_t src_ld,
+__global__ __launch_bounds__(256) void copy_pad_rows16_kernel(const uint16_t* __restrict__ src, uint32_t parts,
+                                                              uint32_t row_parts, int64_t cols, int64_t src_ld,
                                                               uint16_t* __restrict__ dst, int64_t dst_ld,
                                                               int64_t dst_cols) {
-  constexpr int kParts = 4;
-  const int64_t waves = static_cast<int64_t>(gridDim.x) * 4;
-  for (int64_t p0 = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); p0 < parts; p0 += waves * kParts) {
-    uint4 o[kParts];
-    uint16_t* to[kParts];
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      const int64_t p = p0 + waves * i, r = p / row_parts, c = (p - r * row_parts) * 512 + (threadIdx.x & 63) * 8;
-      o[i] = make_uint4(0, 0, 0, 0);
-      to[i] = p < parts && c < dst_cols ? dst + r * dst_ld + c : nullptr;
-      if (to[i] == nullptr || c >= cols) continue;
-      const uint16_t* s = src + r * src_ld + c;
-      if (c + 8 <= cols) {
-        const loose16_t v = *reinterpret_cast<const loose16_t*>(s);
-        o[i] = make_uint4(v[0], v[1], v[2], v[3]);
-      } else {
-        uint32_t v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? s[j] : 0;
-        o[i] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
-      }
+  for (uint32_t p = blockIdx.x * 4 + (threadIdx.x >> 6); p < parts; p += gridDim.x * 4) {
+    const uint32_t r = p / row_parts;
+    const int64_t c = static_cast<int64_t>(p - r * row_parts) * 512 + (threadIdx.x & 63) * 8;
+    if (c >= dst_cols) continue;
+    const uint16_t* row = src + r * src_ld;
+    uint32_t o[4] = {};
+    if (cols >= 8) {
+      // the last 8 of the row where the lane's own straddle its end, its first ones shifted out
+      const int64_t from = c + 8 <= cols ? c : cols - 8;
+      const int out = c - from < 8 ? static_cast<int>(c - from) : 8;
+      const loose16_t v = *reinterpret_cast<const loose16_t*>(row + from);
+      uint64_t lo = v[0] | static_cast<uint64_t>(v[1]) << 32, hi = v[2] | static_cast<uint64_t>(v[3]) << 32;
+      if (out & 8) lo = hi = 0;
+      if (out & 4) lo = hi, hi = 0;
+      if (const int bits = 16 * (out & 3)) lo = lo >> bits | hi << (64 - bits), hi >>= bits;
+      o[0] = static_cast<uint32_t>(lo), o[1] = static_cast<uint32_t>(lo >> 32);
+      o[2] = static_cast<uint32_t>(hi), o[3] = static_cast<uint32_t>(hi >> 32);
+    } else {
+      for (int j = 0; j < 8; ++j)
+        if (c + j < cols) o[j >> 1] |= static_cast<uint32_t>(row[c + j]) << 16 * (j & 1);
     }
-#pragma unroll
-    for (int i = 0; i < kParts; ++i)
-      if (to[i] != nullptr) *reinterpret_cast<uint4*>(to[i]) = o[i];
+    *reinterpret_cast<uint4*>(dst + r * dst_ld + c) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -143,9 +144,15 @@ extern "C" int moc_copy_pad_2d(int dtype, const void* src, int64_t rows, int64_t
   const dim3 grid(static_cast<unsigned>(blocks)), block(256);
   hipStream_t st = as_stream(stream);
   if (dtype == MOC_BF16 && dst_ld % 8 == 0 && dst_cols % 8 == 0 && aligned16(dst)) {
-    const int64_t row_parts = (dst_cols + 511) / 512, parts = rows * row_parts, wgs = (parts + 3) / 4;
-    copy_pad_rows16_kernel<<<static_cast<unsigned>(wgs < 8192 ? wgs : 8192), 256, 0, st>>>(
-        static_cast<const uint16_t*>(src), parts, row_parts, cols, src_ld, static_cast<uint16_t*>(dst), dst_ld, dst_cols);
+    const int64_t row_parts = (dst_cols + 511) / 512, most = std::max<int64_t>(1, kCopyParts / row_parts);
+    MOC_REQUIRE(row_parts <= kCopyParts, "moc_copy_pad_2d: rows too long");
+    for (int64_t r0 = 0; r0 < rows; r0 += most) {
+      const int64_t parts = std::min(rows - r0, most) * row_parts, wgs = (parts + 3) / 4;
+      const unsigned grid16 = static_cast<unsigned>(wgs < 8192 ? wgs : 8192);
+      copy_pad_rows16_kernel<<<grid16, 256, 0, st>>>(
+          static_cast<const uint16_t*>(src) + r0 * src_ld, static_cast<uint32_t>(parts),
+          static_cast<uint32_t>(row_parts), cols, src_ld, static_cast<uint16_t*>(dst) + r0 * dst_ld, dst_ld, dst_cols);
+    }
     return check_launch("copy_pad_rows16_kernel");
   }
   if (dtype == MOC_BF16)
