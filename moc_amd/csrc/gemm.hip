@@ -1362,7 +1362,7 @@ void gemm_pp_kernel(GemmArgs g) {
   // LOSS: a workgroup's tiles are bid, bid + gridDim, ...; the first halves of the next
   // one are requested behind the last phase, before the epilogue, and a group's
   // waits (vmcnt(0) there) leave them landed.
-  auto tile_first = [&]() {
+  [[maybe_unused]] auto tile_first = [&]() {
     if (grp == 0) {
       load_half(kt0, 0);
       load_half(kt0, 1);
@@ -1370,7 +1370,6 @@ void gemm_pp_kernel(GemmArgs g) {
       load_half(kt0 + 1, 1);
     }
   };
-  tile_first();
   [[maybe_unused]] auto lane_again = []() {
     int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
     asm volatile("" : "+v"(l));
@@ -1392,9 +1391,19 @@ void gemm_pp_kernel(GemmArgs g) {
     mb0.init(g.b[0], col0, sw, l);
     tile_first();
   };
-  if (grp == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // the other products' first halves are requested inside the groups' own branches (apart
+  // from them: 0.1 us a launch more)
+  if constexpr (LOSS) {
+    tile_first();
+    if (grp == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
 next_tile:
   if (grp == 0) {
+    if constexpr (!LOSS) {
+      load_half(kt0, 0);
+      load_half(kt0, 1);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
     fix_half(kt0, 0);
     fix_half(kt0, 1);
     phase_end();
@@ -1411,6 +1420,9 @@ next_tile:
     }
     if constexpr (LOSS) tile_next();
   } else {
+    if constexpr (!LOSS) {
+      if (kt0 + 1 < nk) load_half(kt0 + 1, 1);
+    }
     phase_end();
     for (int t = kt0; t < nk; ++t) {
       if (t > kt0) compute();
@@ -1640,7 +1652,10 @@ __global__ __launch_bounds__(kMidThreads) void gemm_mid_kernel(GemmArgs g) {
 // Sum of the ksplit f32 partial tiles of a split-K GEMM, in split order (the
 // result does not depend on timing), converted to the output type.  One
 // thread per four consecutive columns of a row.
-template <bool OUT_F32>
+//
+// SCALED: C = *alpha times the sum, low > 0: with the rows `low` on added to each (of
+// their own, as the branches cost the others' launches 0.1 us).
+template <bool OUT_F32, bool SCALED = false>
 __device__ __forceinline__ void splitk_reduce_quad(int64_t q, const float* __restrict__ ws, int64_t stride,
                                                    int ksplit, int M, int N, int64_t ldw, void* __restrict__ C,
                                                    int64_t ldc, int vec, const uint16_t* __restrict__ res,
@@ -1658,7 +1673,7 @@ __device__ __forceinline__ void splitk_reduce_quad(int64_t q, const float* __res
     s.z += v.z;
     s.w += v.w;
   }
-  if (low != 0) {  // the row's second part, `low` rows on
+  if (SCALED && low != 0) {
     for (int i = 0; i < ksplit; ++i) {
       const float4 v = *reinterpret_cast<const float4*>(p + low * ldw + i * stride);
       s.x += v.x;
@@ -1667,7 +1682,7 @@ __device__ __forceinline__ void splitk_reduce_quad(int64_t q, const float* __res
       s.w += v.w;
     }
   }
-  if (alpha != nullptr) {
+  if constexpr (SCALED) {
     const float f = *alpha;
     s = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
   }
@@ -1697,7 +1712,7 @@ __device__ __forceinline__ void splitk_reduce_quad(int64_t q, const float* __res
   }
 }
 
-template <bool OUT_F32>
+template <bool OUT_F32, bool SCALED = false>
 __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float* __restrict__ ws, int64_t stride,
                                                             int ksplit, int M, int N, int64_t ldw,
                                                             void* __restrict__ C, int64_t ldc, int vec,
@@ -1705,8 +1720,8 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float* __restr
                                                             int64_t ldres = 0,
                                                             const float* __restrict__ alpha = nullptr,
                                                             int64_t low = 0) {
-  splitk_reduce_quad<OUT_F32>(static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, ws, stride, ksplit, M, N,
-                              ldw, C, ldc, vec, res, ldres, alpha, low);
+  splitk_reduce_quad<OUT_F32, SCALED>(static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, ws, stride, ksplit, M, N,
+                                      ldw, C, ldc, vec, res, ldres, alpha, low);
 }
 
 // The sums of a grouped split-K launch's two products in one launch:
@@ -2678,19 +2693,23 @@ extern "C" int moc_gemm(int dtype, int64_t M, int64_t N, int64_t K, const void* 
 
 namespace {
 
-// The sum of a K split's parts of both halves of the rows (moc::gemm_pair_rows).
+// The sum of a K split's parts: C, with alpha times it (moc::gemm_half).
+int reduce_parts(const float* parts, int64_t stride, int ksplit, int64_t M, int64_t N, int64_t ldw, void* C, int64_t ldc,
+                 bool f32, int vec, const uint16_t* res, int64_t ldres, const float* alpha, int64_t low, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>((M * ((N + 3) / 4) + 255) / 256));
+  auto kernel = alpha != nullptr ? (f32 ? splitk_reduce_kernel<true, true> : splitk_reduce_kernel<false, true>)
+                                 : (f32 ? splitk_reduce_kernel<true> : splitk_reduce_kernel<false>);
+  kernel<<<grid, 256, 0, st>>>(parts, stride, ksplit, (int)M, (int)N, ldw, C, ldc, vec, f32 ? nullptr : res, ldres, alpha,
+                               low);
+  return check_launch("splitk_reduce_kernel");
+}
+
+// That of both halves of the rows (moc::gemm_pair_rows).
 int reduce_pair(const float* parts, int64_t stride, int ksplit, int64_t rows, int64_t N, int64_t ldw, HalfPair& out,
                 hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>((rows * ((N + 3) / 4) + 255) / 256));
-  const int vec = aligned16(out.C) && N % 4 == 0;
   out.done = true;
-  if (out.c_dtype == MOC_F32)
-    splitk_reduce_kernel<true><<<grid, 256, 0, st>>>(parts, stride, ksplit, (int)rows, (int)N, ldw, out.C, N, vec, nullptr, 0,
-                                                     out.alpha, rows);
-  else
-    splitk_reduce_kernel<false><<<grid, 256, 0, st>>>(parts, stride, ksplit, (int)rows, (int)N, ldw, out.C, N, vec, nullptr,
-                                                      0, out.alpha, rows);
-  return check_launch("splitk_reduce_kernel");
+  return reduce_parts(parts, stride, ksplit, rows, N, ldw, out.C, N, out.c_dtype == MOC_F32, aligned16(out.C) && N % 4 == 0,
+                      nullptr, 0, out.alpha, rows, st);
 }
 
 // moc_gemm_ws with an optional bf16 residual R added to a bf16 C (res may be
@@ -2858,16 +2877,9 @@ int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int6
     launch_mid(run, mp, la == 1, lb == 1, mp.ksplit > 1 || of, st);
     const int rc = check_launch("gemm_mid_kernel");
     if (rc != MOC_OK || mp.ksplit == 1) return rc;
-    const dim3 grid(static_cast<unsigned>((M * ((N + 3) / 4) + 255) / 256));
     const float* parts = static_cast<const float*>(run.C);
     if (pair != nullptr) return reduce_pair(parts, run.ws_stride, mp.ksplit, M / 2, N, mp.ldw, *pair, st);
-    if (of)
-      splitk_reduce_kernel<true><<<grid, 256, 0, st>>>(parts, run.ws_stride, mp.ksplit, (int)M, (int)N, mp.ldw, C, ldc,
-                                                       a.vec_store, nullptr, 0, alpha);
-    else
-      splitk_reduce_kernel<false><<<grid, 256, 0, st>>>(parts, run.ws_stride, mp.ksplit, (int)M, (int)N, mp.ldw, C,
-                                                        ldc, a.vec_store, a.res, a.ldres, alpha);
-    return check_launch("splitk_reduce_kernel");
+    return reduce_parts(parts, run.ws_stride, mp.ksplit, M, N, mp.ldw, C, ldc, of, a.vec_store, a.res, a.ldres, alpha, 0, st);
   }
   const bool short_whole = a.pp && la == 1 && short_whole_ok(M, N, a.nk[0] + a.nk[1]);
   // 128-row tiles in two K parts instead of a K split (see plan_fix_short)
@@ -2911,17 +2923,9 @@ int gemm_ws_impl(int dtype, int64_t M, int64_t N, int64_t K, const void* A, int6
   {
     const int rc = check_launch("gemm_bf16_kernel");
     if (rc != MOC_OK) return rc;
-    const int64_t quads = M * ((N + 3) / 4);
-    const dim3 grid(static_cast<unsigned>((quads + 255) / 256));
     const float* parts = static_cast<const float*>(run.C);
     if (pair != nullptr) return reduce_pair(parts, run.ws_stride, sp.ksplit, M / 2, N, sp.ldw, *pair, st);
-    if (of)
-      splitk_reduce_kernel<true><<<grid, 256, 0, st>>>(parts, run.ws_stride, sp.ksplit, (int)M, (int)N, sp.ldw,
-                                                       C, ldc, a.vec_store, nullptr, 0, alpha);
-    else
-      splitk_reduce_kernel<false><<<grid, 256, 0, st>>>(parts, run.ws_stride, sp.ksplit, (int)M, (int)N, sp.ldw,
-                                                        C, ldc, a.vec_store, a.res, a.ldres, alpha);
-    return check_launch("splitk_reduce_kernel");
+    return reduce_parts(parts, run.ws_stride, sp.ksplit, M, N, sp.ldw, C, ldc, of, a.vec_store, a.res, a.ldres, alpha, 0, st);
   }
 }
 
