@@ -1245,6 +1245,12 @@ unsigned blocks_of(int64_t n) {
 constexpr int64_t kPieceBytes = 1LL << 30, kGradPieceBytes = (1LL << 31) - 4096;
 constexpr int64_t kWidest = 4;
 constexpr int64_t kF32Weight = 48LL << 20;
+// Bytes of an f32 product's K split: with more of them the parts' own traffic costs more
+// than the split saves, and up to 16 times the result would be held.  us, split / whole:
+//   dweight  4000 x 128 x 4000 rows     4 MB   56 /   94    10000 x 300 x 3000    144 MB   243 /  229
+//           50048 x 768 x 2048       2460 MB 2596 / 1416   128256 x 256 x  500   1051 MB   870 /  354
+//   dhidden  2048 x 768 x 50256 words  13 MB 1411 / 1838     3000 x 300 x 10000    54 MB   203 /  216
+constexpr int64_t kF32Parts = 64LL << 20;
 // Few rows: dhidden comes from gradients in two bf16 parts, twice the rows, with the
 // weight as it is (TWO), else from f16 ones and a copy of the weight.  The copy moves 4
 // bytes of each of the weight's values, the parts cost as many products and 16 bytes of
@@ -1332,6 +1338,20 @@ Pieces pieces_of(int dtype, int64_t rows, int64_t hidden, int64_t vocab, int64_t
 // Rows of a launch with a workgroup a row: a grid has less than 2^32 threads, and one of
 // 1024 a row for the widest rows.
 constexpr int64_t kLaunchRows = 1 << 20;
+
+// Workspace of an f32 product over K (0: it does not split K).
+int64_t f32_room(int64_t M, int64_t N, int64_t K) {
+  const int64_t b = moc_gemm_workspace_size(MOC_F32, M, N, K, 0);
+  return b <= MOC_GEMM_WS_COUNTER_BYTES + kF32Parts ? b : 0;
+}
+
+// Words whose f32 logits are one product: those whose weights the last-level cache holds
+// beside the logits, since every 64 rows read them again: 1024 x 768 x 50257 795 us, in
+// one product 1557.
+int64_t f32_columns(int64_t ldw) {
+  const int64_t fit = kF32Weight / (ldw * 4) / 64 * 64;
+  return fit < 1024 ? 1024 : fit;
+}
 
 // A teacher as its caller has it.
 struct Teacher {
@@ -1571,12 +1591,16 @@ extern "C" int64_t moc_linear_loss_gemm_workspace_size(int dtype, int64_t rows, 
   const int64_t four = p.fused ? vocab : vocab & ~3LL;
   for (int64_t i = 0; i < p.count; i += p.count > 1 ? p.count - 1 : 1) {  // the first piece and the last
     const int64_t n = i + 1 < p.count ? p.rows : rows - i * p.rows;
-    if (!p.fused) need(moc_gemm_workspace_size(dtype, n, vocab, hidden, 0));
+    if (!p.fused) {
+      const int64_t cols = f32_columns((hidden + 3) & ~3LL);
+      need(f32_room(n, vocab < cols ? vocab : cols, hidden));
+      need(f32_room(n, vocab % cols, hidden));
+    }
     if (!grads) continue;
-    if (four < vocab) need(moc_gemm_workspace_size(dtype, 4, hidden, n, 0));
-    need(!p.fused ? moc_gemm_workspace_size(dtype, n, hidden, four, 0)
-                  : gemm_half_workspace(in_two_parts(rows, hidden, vocab) ? 2 * n : n, hidden, vocab));
-    need(p.fused ? gemm_half_workspace(vocab, hidden, n) : moc_gemm_workspace_size(dtype, four, hidden, n, 0));
+    if (four < vocab) need(f32_room(4, hidden, n));
+    need(p.fused ? gemm_half_workspace(in_two_parts(rows, hidden, vocab) ? 2 * n : n, hidden, vocab)
+                 : f32_room(n, hidden, four));
+    need(p.fused ? gemm_half_workspace(vocab, hidden, n) : f32_room(four, hidden, n));
   }
   return most;
 }
@@ -1618,6 +1642,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
               "moc_linear_loss: operands of up to 2 GiB a piece");
   hipStream_t st = as_stream(stream);
   int* count = static_cast<int*>(gemm_ws);
+  auto room = [&](int64_t M, int64_t N, int64_t K) { return std::min(gemm_ws_bytes, f32_room(M, N, K)); };
   Targets& t = p.t;
   if (words == 0) {
     t.labels = labels;
@@ -1698,13 +1723,13 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
         slabs_loss_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(s, t, o);
       rc = check_launch("slabs_grad_kernel");
     } else {
-      // by words whose weights the last-level cache holds beside the logits, since every 64
-      // rows read them again: 1024 x 768 x 50257 795 us, in one product 1557
-      const int64_t fit = kF32Weight / (ldw * 4) / 64 * 64, cols = fit < 1024 ? 1024 : fit;
-      for (int64_t c = 0; c < vocab && rc == MOC_OK; c += cols)
-        rc = moc_gemm_ws(dtype, n, vocab - c < cols ? vocab - c : cols, hidden, xi, ldx, 1,
-                         static_cast<const float*>(w) + c * ldw, 1, ldw, 0, nullptr, 0, 0, nullptr, 0, 0,
-                         reinterpret_cast<float*>(p.d) + c, p.ldz, MOC_F32, gemm_ws, gemm_ws_bytes, stream);
+      const int64_t cols = f32_columns(ldw);
+      for (int64_t c = 0; c < vocab && rc == MOC_OK; c += cols) {
+        const int64_t m = vocab - c < cols ? vocab - c : cols;
+        rc = moc_gemm_ws(dtype, n, m, hidden, xi, ldx, 1, static_cast<const float*>(w) + c * ldw, 1, ldw, 0, nullptr, 0, 0,
+                         nullptr, 0, 0, reinterpret_cast<float*>(p.d) + c, p.ldz, MOC_F32, gemm_ws, room(n, m, hidden),
+                         stream);
+      }
       if (rc != MOC_OK) return rc;
       rc = logits_rows(true, p.d, n, vocab, p.ldz, t, r0, words, temperature, o, grads ? p.d : nullptr, p.ldz, st);
     }
@@ -1727,8 +1752,9 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       // words whose weights the tiled products reach with 32-bit offsets at a time
       const int64_t reach = ((1LL << 31) - 64) / (ldw * 4) / 4 * 4, step = reach < 4 ? 4 : reach;
       for (int64_t c = 0; c < four; c += step) {
-        rc = moc_gemm_ws(dtype, n, hidden, four - c < step ? four - c : step, d + c, p.ldz, 1, wf + c * ldw, ldw, 1, 0, nullptr,
-                         0, 0, nullptr, 0, 0, c == 0 ? to : p.rest, hidden, MOC_F32, gemm_ws, gemm_ws_bytes, stream);
+        const int64_t k = four - c < step ? four - c : step;
+        rc = moc_gemm_ws(dtype, n, hidden, k, d + c, p.ldz, 1, wf + c * ldw, ldw, 1, 0, nullptr, 0, 0, nullptr, 0, 0,
+                         c == 0 ? to : p.rest, hidden, MOC_F32, gemm_ws, room(n, hidden, k), stream);
         if (rc != MOC_OK) return rc;
         if (c == 0) continue;
         add_f32_kernel<float><<<blocks_of(n * hidden), 256, 0, st>>>(to, p.rest, n * hidden, nullptr);
@@ -1756,7 +1782,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
       const int64_t cut = f32 && n > 1 ? four : vocab;
       if (cut < vocab) {
         rc = moc_gemm_ws(dtype, 4, hidden, n, reinterpret_cast<const float*>(p.d) + cut, 1, p.ldz, b, p.ldx, 1, 0, nullptr, 0,
-                         0, nullptr, 0, 0, p.rest, hidden, MOC_F32, gemm_ws, gemm_ws_bytes, stream);
+                         0, nullptr, 0, 0, p.rest, hidden, MOC_F32, gemm_ws, room(4, hidden, n), stream);
         if (rc != MOC_OK) return rc;
         const int64_t size = (vocab - cut) * hidden;
         rc = moc_copy_pad_2d(MOC_F32, p.rest, 1, size, size, reinterpret_cast<float*>(to) + cut * hidden, size, size, stream);
@@ -1766,7 +1792,7 @@ extern "C" int moc_linear_loss(int dtype, const void* h, int64_t rows, int64_t h
            : p.fused ? gemm_half(vocab, hidden, n, p.d, 1, p.ldz, b, p.ldx, to, hidden, to_dtype, t.alpha + 1, gemm_ws,
                                  gemm_ws_bytes, stream)
                      : moc_gemm_ws(dtype, cut, hidden, n, p.d, 1, p.ldz, b, p.ldx, 1, 0, nullptr, 0, 0, nullptr, 0, 0, to,
-                                   hidden, to_dtype, gemm_ws, gemm_ws_bytes, stream);
+                                   hidden, to_dtype, gemm_ws, room(cut, hidden, n), stream);
       if (rc != MOC_OK) return rc;
       if (i > 0) {
         const int64_t size = vocab * hidden;
